@@ -1,0 +1,439 @@
+// Causal attention over a cache held in 4 bits, and the weight that it gives to every cached row, for one
+// head size (-DTS_HEAD_DIM=64, 128 or 256).
+//
+// For the rows r of a tile (query token i, query head of the key head's group) and the keys j that i may see:
+//   s_rj = scale q_r . k_j      o_r = sum_j p_rj v_j      p_rj = exp(s_rj - m_r) / l_r      l_r = sum_j exp(s_rj - m_r) (+ exp(sink - m_r))
+// with the running maximum m and sum l of one pass over the keys, in 32 bits.  The matrix instructions take bfloat16: keys
+// and values in 4 bits are exact in it, and so are queries of that type.  exp(s - m) is given as two of them (16 bits; one has 8,
+// and half, with 11, loses weights below 2^-24 of the largest), float32 queries and their weights as three.
+//
+// Keys stand on the M side of the instruction: S^T[16 keys][8 rows] = K Q^T and O^T[channels][8 rows] += V^T P^T, so
+// that the few rows of a decode step fill an instruction and every code is unpacked once for all of them.
+#include "kv4.cuh"
+
+#ifndef TS_HEAD_DIM
+#error "compile with -DTS_HEAD_DIM=64, 128 or 256"
+#endif
+
+namespace {
+
+constexpr int D = TS_HEAD_DIM;
+using Rec = Kv4Record<D>;
+constexpr int kWarps = 8;
+constexpr int kStages = 4;  // records in flight per warp
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Params {
+  const void* q;
+  const uint8_t* pool;
+  void* out;
+  float* lse;
+  const float* sinks;
+  const int* cu;
+  const int* context;
+  const int* table;
+  float* part;
+  int table_stride, page_blocks, num_pages, tokens, nq, nkv, group, window, splits, row_tiles;
+  float scale;  // times log2 e
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src));
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// The record of block `blk` of a request, given its entry of the block table.
+__device__ __forceinline__ const uint8_t* record(const Params& p, int page, int blk, int head) {
+  return p.pool + (((size_t)min(max(page, 0), p.num_pages - 1) * p.nkv + head) * p.page_blocks + blk % p.page_blocks) * Rec::kBytes;
+}
+
+// O^T[channels][rows] += V^T P^T of one record.  Lane (g, t) owns the channels [g D/8, (g+1) D/8) and reads of them the
+// tokens 2t, 2t+1, 2t+8, 2t+9; p[tile][part]: the transposed weights of tokens 0..7 and 8..15.  Tokens outside
+// [first, last) count as zeros, whatever the record holds there.
+template <int kTiles, int kP>
+__device__ __forceinline__ void add_values(const uint8_t* rec, const uint32_t (&p)[kTiles][kP][2], float (&o)[kTiles][D / 16][4], int g, int t,
+                                           int first, int last) {
+  constexpr int kWords = D / 64;
+  const uint8_t* codes = rec + Rec::kValues + g * (D / 16);
+  const uint8_t* scales = rec + Rec::kValueScales + g * kWords / 2;  // (heads of 64: two lanes share a group)
+  uint32_t w[4][kWords], sc[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int token = 2 * t + (i & 1) + 8 * (i >> 1);
+    const uint8_t* c = codes + token * (D / 2);
+    if constexpr (kWords == 1) w[i][0] = *reinterpret_cast<const uint32_t*>(c);
+    else if constexpr (kWords == 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(c);
+      w[i][0] = v.x, w[i][1] = v.y;
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(c);
+      w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
+    }
+    if constexpr (kWords == 4) sc[i] = *reinterpret_cast<const uint16_t*>(scales + token * (D / 16));
+    else sc[i] = scales[token * (D / 16)];
+    if (token < first || token >= last) sc[i] = 0;
+  }
+#pragma unroll
+  for (int grp = 0; grp < (kWords + 1) / 2; ++grp) {
+    __nv_bfloat162 f[2], c[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) kv4_factors((sc[2 * i] >> (8 * grp)) & 0xffu, (sc[2 * i + 1] >> (8 * grp)) & 0xffu, f[i], c[i]);
+#pragma unroll
+    for (int k = 2 * grp; k < (kWords == 1 ? 1 : 2 * grp + 2); ++k) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // four channels each: 8k + 4 half + 0..3
+        const uint32_t sel = half ? 0x7632u : 0x5410u;
+        const uint32_t x = __byte_perm(w[0][k], w[1][k], sel), y = __byte_perm(w[2][k], w[3][k], sel);
+        const uint32_t a0 = kv4_pair(x << 3, f[0], c[0]), a1 = kv4_pair(x >> 1, f[0], c[0]);
+        const uint32_t a2 = kv4_pair(y << 3, f[1], c[1]), a3 = kv4_pair(y >> 1, f[1], c[1]);
+        const uint32_t b0 = kv4_pair(x >> 5, f[0], c[0]), b1 = kv4_pair(x >> 9, f[0], c[0]);
+        const uint32_t b2 = kv4_pair(y >> 5, f[1], c[1]), b3 = kv4_pair(y >> 9, f[1], c[1]);
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int part = 0; part < kP; ++part) {
+            kv4_mma(o[n][4 * k + 2 * half], a0, a1, a2, a3, p[n][part][0], p[n][part][1]);
+            kv4_mma(o[n][4 * k + 2 * half + 1], b0, b1, b2, b3, p[n][part][0], p[n][part][1]);
+          }
+      }
+    }
+  }
+}
+
+// What a tile of rows of one sequence and key head is, and which rows it holds.
+struct Tile {
+  int b, head, first_row, rows, q_start, q_len, context;
+  // (lengths are kept within the block table and the tensors, so that no wrong number reads beyond them)
+  __device__ __forceinline__ void open(const Params& p, int seq, int key_head) {
+    b = seq, head = key_head;
+    q_start = min(max(p.cu[b], 0), p.tokens);
+    q_len = min(max(p.cu[b + 1], q_start), p.tokens) - q_start;
+    context = min(p.context[b], p.table_stride * p.page_blocks * KV4_BLOCK);
+    rows = q_len * p.group;
+  }
+  __device__ __forceinline__ int position(const Params& p, int row) const { return context - q_len + row / p.group; }  // the last key it sees
+  __device__ __forceinline__ int token(const Params& p, int row) const { return q_start + row / p.group; }
+  template <typename T>
+  __device__ __forceinline__ const T* query(const Params& p, int row) const {
+    return reinterpret_cast<const T*>(p.q) + ((size_t)token(p, row) * p.nq + query_head(p, row)) * D;
+  }
+  __device__ __forceinline__ int query_head(const Params& p, int row) const { return head * p.group + row % p.group; }
+};
+
+// m, l and O of one row tile, over a set of partial ones: factor of partial i is 2^(m_i - M).
+template <typename T>
+__device__ __forceinline__ void write_row(const Params& p, const Tile& tile, int row, int channel, float4 o, float m, float l) {
+  const int head = tile.query_head(p, row);
+  if (p.sinks != nullptr) {
+    const float sink = p.sinks[head] * kLog2e, top = fmaxf(m, sink);
+    if (top != -INFINITY) {
+      const float f = m == -INFINITY ? 0.f : kv4_exp2(m - top);
+      l = l * f + kv4_exp2(sink - top);
+      o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+      m = top;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
+  const size_t at = ((size_t)tile.token(p, row) * p.nq + head) * D + channel;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  } else {
+    __nv_bfloat162 v[2] = {__floats2bfloat162_rn(o.x * inv, o.y * inv), __floats2bfloat162_rn(o.z * inv, o.w * inv)};
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + at) = *reinterpret_cast<const uint2*>(v);
+  }
+  if (p.lse != nullptr && channel == 0) p.lse[(size_t)tile.token(p, row) * p.nq + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+template <typename T, int kTiles, int kQ, int kP>
+__global__ void __launch_bounds__(kWarps * 32) attention_kernel(const Params p) {
+  constexpr int kRows = 8 * kTiles;
+  extern __shared__ __align__(16) uint8_t smem[];
+  ts_pdl_prologue();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  Tile tile;
+  tile.open(p, blockIdx.z, blockIdx.y % p.nkv);
+  tile.first_row = blockIdx.y / p.nkv * kRows;
+  if (tile.first_row >= tile.rows) return;
+  const int last_row = min(tile.first_row + kRows, tile.rows) - 1;
+  const int first_pos = tile.position(p, tile.first_row), last_pos = tile.position(p, last_row);
+  const int key0 = p.window > 0 ? max(0, first_pos - p.window + 1) : 0, key1 = max(last_pos + 1, 0);
+  const int blk0 = key0 / KV4_BLOCK, blocks = max(0, (key1 + KV4_BLOCK - 1) / KV4_BLOCK - blk0);
+  const int per = (blocks + p.splits - 1) / p.splits;
+  const int begin = blk0 + min(blocks, per * (int)blockIdx.x), end = blk0 + min(blocks, per * ((int)blockIdx.x + 1));
+
+  uint32_t qf[kTiles][kQ][D / 16][2];
+  int pos[kTiles][2];  // last visible key of the rows 2t, 2t+1 of a tile of 8 (rows that do not exist: none)
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+    const int row = tile.first_row + 8 * n + g;
+    kv4_query_row<D, kQ>(row < tile.rows ? tile.query<T>(p, row) + t * (D / 4) : nullptr, qf[n]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = tile.first_row + 8 * n + 2 * t + i;
+      pos[n][i] = r < tile.rows ? tile.position(p, r) : -1;
+    }
+  }
+
+  float o[kTiles][D / 16][4], m[kTiles][2], l[kTiles][2];
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n) {
+    m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+  }
+
+  uint8_t* ring = smem + warp * (kStages * Rec::kBytes);
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const int* table = p.table + (size_t)tile.b * p.table_stride;
+  auto fetch = [&](int blk, int stage) {
+    if (blk < end) {
+      const uint8_t* src = record(p, table[blk / p.page_blocks], blk, tile.head);
+      for (int i = lane * 16; i < Rec::kBytes; i += 512) copy16(ring_at + stage * Rec::kBytes + i, src + i);
+    }
+    copy_commit();
+  };
+  const int mine = begin + warp;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) fetch(mine + s * kWarps, s);
+  int stage = 0;
+  for (int blk = mine; blk < end; blk += kWarps) {
+    fetch(blk + (kStages - 1) * kWarps, (stage + kStages - 1) % kStages);
+    copy_wait<kStages - 1>();
+    __syncwarp();
+    const uint8_t* rec = ring + stage * Rec::kBytes;
+    float s[kTiles][4];
+    kv4_scores<D, kTiles, kQ>(rec, rec + Rec::kKeyScales, qf, s, g, t);
+    const int key = blk * KV4_BLOCK;
+    bool grows = false;
+    float top[kTiles][2];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = key + g + 8 * (i >> 1), c = i & 1;
+        s[n][i] *= p.scale;
+        if (at > pos[n][c] || (p.window > 0 && at <= pos[n][c] - p.window)) s[n][i] = -INFINITY;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        top[n][c] = fmaxf(s[n][c], s[n][c + 2]);
+        grows |= top[n][c] > m[n][c] + 8.f;
+      }
+    }
+    // The maximum moves only when a score passes it by 2^8: until then weights up to 256 are as exact as those up to 1.
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x = top[n][c];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          x = fmaxf(x, m[n][c]);
+          const float f = x == -INFINITY ? 1.f : kv4_exp2(m[n][c] - x);
+          m[n][c] = x;
+          l[n][c] *= f;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) o[n][i][c] *= f, o[n][i][c + 2] *= f;
+        }
+    }
+    uint32_t pf[kTiles][kP][2];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = kv4_exp2(s[n][i] - (m[n][i & 1] == -INFINITY ? 0.f : m[n][i & 1]));
+        l[n][i & 1] += w[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t parts[kP];
+        kv4_split<kP>(w[2 * i], w[2 * i + 1], parts);
+#pragma unroll
+        for (int k = 0; k < kP; ++k) pf[n][k][i] = transpose8x8(parts[k]);
+      }
+    }
+    add_values<kTiles, kP>(rec, pf, o, g, t, key0 - key, key1 - key);
+    __syncwarp();
+    stage = (stage + 1) % kStages;
+  }
+  copy_wait<0>();
+  __syncthreads();
+
+  // The warps' parts meet in shared memory.
+  float* so = reinterpret_cast<float*>(smem);              // [warps][rows][D]
+  float* sm = so + kWarps * kRows * D;                      // [warps][rows]
+  float* sl = sm + kWarps * kRows;
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float x = l[n][c];
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      const int row = 8 * n + 2 * t + c;
+      if (g == 0) sm[warp * kRows + row] = m[n][c], sl[warp * kRows + row] = x;
+      float2* dst = reinterpret_cast<float2*>(so + (warp * kRows + row) * D + g * (D / 8));
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) dst[i] = make_float2(o[n][i][c], o[n][i][c + 2]);
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kRows * (D / 4); i += kWarps * 32) {
+    const int r = i / (D / 4), channel = i % (D / 4) * 4, row = tile.first_row + r;
+    if (row >= tile.rows) continue;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * kRows + r]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = sm[w * kRows + r], f = mw == -INFINITY ? 0.f : kv4_exp2(mw - top);
+      if (mw == -INFINITY && sl[w * kRows + r] == 0.f) continue;
+      const float4 v = *reinterpret_cast<const float4*>(so + (w * kRows + r) * D + channel);
+      sum += f * sl[w * kRows + r];
+      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+    }
+    if (p.splits == 1) {
+      write_row<T>(p, tile, row, channel, acc, top, sum);
+    } else {
+      const size_t slot = ((size_t)tile.token(p, row) * p.nq + tile.query_head(p, row)) * p.splits + blockIdx.x;
+      *reinterpret_cast<float4*>(p.part + slot * (D + 4) + 4 + channel) = acc;
+      if (channel == 0) *reinterpret_cast<float2*>(p.part + slot * (D + 4)) = make_float2(top, sum);
+    }
+  }
+}
+
+// The splits of every row, one warp-wide piece of it per thread: the same sums, in the order of the splits.
+template <typename T>
+__global__ void __launch_bounds__(128) merge_kernel(const Params p, int num_seqs, int rows) {
+  ts_pdl_prologue();
+  const int i = blockIdx.x * 128 + threadIdx.x;
+  const int r = i / (D / 4), channel = i % (D / 4) * 4;
+  if (r >= rows) return;
+  const int token = r / p.nq, head = r % p.nq;
+  if (token >= p.cu[num_seqs]) return;
+  const float* part = p.part + (size_t)r * p.splits * (D + 4);
+  float top = -INFINITY, sum = 0.f;
+  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, part[s * (D + 4)]);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(part + s * (D + 4));
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;
+    const float4 v = *reinterpret_cast<const float4*>(part + s * (D + 4) + 4 + channel);
+    const float f = ml.x == -INFINITY ? 0.f : kv4_exp2(ml.x - top);
+    sum += f * ml.y;
+    acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+  }
+  Tile tile;
+  tile.q_start = token, tile.head = head / p.group;
+  write_row<T>(p, tile, head % p.group, channel, acc, top, sum);
+}
+
+// ---------------------------------------------------------------------------
+// weights: w_j += sum over the rows r of exp(s_rj - lse_r).  A warp owns 16 keys of one head and walks the rows that see them.
+
+template <typename T, int kQ>
+__global__ void __launch_bounds__(kWarps * 32) weights_kernel(const Params p, float* sums) {
+  ts_pdl_prologue();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  Tile tile;
+  tile.open(p, blockIdx.z, blockIdx.y);
+  const int blk = blockIdx.x * kWarps + warp, key = blk * KV4_BLOCK, before = tile.context - tile.q_len;
+  if (key >= tile.context) return;
+  const int first_token = max(0, key - before);
+  const int tokens = p.window > 0 ? min(tile.q_len, key + KV4_BLOCK - 1 + p.window - before) : tile.q_len;
+  if (first_token >= tokens) return;
+  const int page = p.table[(size_t)tile.b * p.table_stride + blk / p.page_blocks];
+  const uint8_t* rec = record(p, page, blk, tile.head);
+  float w[2] = {0.f, 0.f};
+  for (int first = first_token * p.group; first < tokens * p.group; first += 8) {
+    uint32_t qf[1][kQ][D / 16][2];
+    kv4_query_row<D, kQ>(first + g < tile.rows ? tile.query<T>(p, first + g) + t * (D / 4) : nullptr, qf[0]);
+    float s[1][4];
+    kv4_scores<D, 1, kQ>(rec, rec + Rec::kKeyScales, qf, s, g, t);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int r = first + 2 * t + c;
+      if (r >= tile.rows) continue;
+      const int pos = tile.position(p, r);
+      const float lse = p.lse[(size_t)tile.token(p, r) * p.nq + tile.query_head(p, r)] * kLog2e;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = key + g + 8 * i;
+        if (at <= pos && (p.window == 0 || at > pos - p.window)) w[i] += kv4_exp2(s[0][c + 2 * i] * p.scale - lse);
+      }
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    w[i] += __shfl_xor_sync(0xffffffffu, w[i], 1);
+    w[i] += __shfl_xor_sync(0xffffffffu, w[i], 2);
+    const int at = key + g + 8 * i;
+    if (t == 0 && at < tile.context) {
+      float* dst = sums + ((size_t)min(max(page, 0), p.num_pages - 1) * p.nkv + tile.head) * p.page_blocks * KV4_BLOCK + at % (p.page_blocks * KV4_BLOCK);
+      *dst += w[i];
+    }
+  }
+}
+
+template <typename T, int kTiles, int kQ, int kP>
+int launch_attention(const Params& p, int num_seqs, int rows, cudaStream_t stream) {
+  constexpr int ring = kWarps * kStages * Rec::kBytes, meet = kWarps * 8 * kTiles * (D + 2) * 4;
+  constexpr int smem = ring > meet ? ring : meet;
+  static bool set = false;
+  if (!set) {
+    cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kTiles, kQ, kP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    set = true;
+  }
+  int status = ts_launch(attention_kernel<T, kTiles, kQ, kP>, dim3(p.splits, p.nkv * p.row_tiles, num_seqs), dim3(kWarps * 32), smem, stream, p);
+  if (status == 0 && p.splits > 1)
+    status = ts_launch(merge_kernel<T>, dim3((rows * (D / 4) + 127) / 128), dim3(128), 0, stream, p, num_seqs, rows);
+  return status;
+}
+
+}  // namespace
+
+// q, out [tokens][nq][D] of `dtype`, lse [tokens][nq] or null, sinks [nq] or null; part: tokens * nq * splits * (D + 4) floats where splits > 1.
+TS_EXPORT int ts_attention_kv4(const void* q, int dtype, const void* pool, void* out, float* lse, const float* sinks, const int* cu, const int* context,
+                               const int* table, int table_stride, int page_blocks, int num_pages, int tokens, int num_seqs, int max_q, int nq, int nkv, float scale,
+                               int window, int splits, float* part, void* stream) {
+  if (tokens < 1 || num_seqs < 1) return 0;
+  Params p = {q, (const uint8_t*)pool, out, lse, sinks, cu, context, table, part, table_stride, page_blocks, num_pages, tokens, nq, nkv, nq / nkv, window, splits, 1, scale * kLog2e};
+  const int rows = max_q * p.group;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (num_seqs > 65535) return TS_ERR_UNSUPPORTED_SIZE;
+  const bool wide = rows > 8 && D <= 128 && dtype == TS_DTYPE_BF16;
+  p.row_tiles = (rows + (wide ? 15 : 7)) / (wide ? 16 : 8);
+  if ((long long)p.row_tiles * nkv > 65535) return TS_ERR_UNSUPPORTED_SIZE;
+  if (dtype == TS_DTYPE_F32) return launch_attention<float, 1, 3, 3>(p, num_seqs, tokens * nq, s);
+#if TS_HEAD_DIM <= 128
+  if (wide) return launch_attention<__nv_bfloat16, 2, 1, 2>(p, num_seqs, tokens * nq, s);
+#endif
+  return launch_attention<__nv_bfloat16, 1, 1, 2>(p, num_seqs, tokens * nq, s);
+}
+
+TS_EXPORT int ts_attention_kv4_weights(const void* q, int dtype, const void* pool, float* lse, float* sums, const int* cu, const int* context,
+                                       const int* table, int table_stride, int page_blocks, int num_pages, int tokens, int num_seqs, int max_context, int nq, int nkv,
+                                       float scale, int window, void* stream) {
+  if (tokens < 1 || num_seqs < 1 || max_context < 1) return 0;
+  if (num_seqs > 65535 || nkv > 65535) return TS_ERR_UNSUPPORTED_SIZE;
+  Params p = {q, (const uint8_t*)pool, nullptr, lse, nullptr, cu, context, table, nullptr, table_stride, page_blocks, num_pages, tokens, nq, nkv, nq / nkv, window, 1, 1, scale * kLog2e};
+  const dim3 grid((max_context + KV4_BLOCK * kWarps - 1) / (KV4_BLOCK * kWarps), nkv, num_seqs);
+  if (dtype == TS_DTYPE_F32) return ts_launch(weights_kernel<float, 3>, grid, dim3(kWarps * 32), 0, (cudaStream_t)stream, p, sums);
+  return ts_launch(weights_kernel<__nv_bfloat16, 1>, grid, dim3(kWarps * 32), 0, (cudaStream_t)stream, p, sums);
+}

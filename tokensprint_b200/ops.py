@@ -2505,6 +2505,237 @@ def attention_prefill_tcgen05(
 
 
 # ---------------------------------------------------------------------------
+# a cache held in 4 bits: rows in and out, attention over it, the weight that cached rows gather, and
+# eviction by that weight
+
+KV4_BLOCK = 16  # tokens of a record, channels that share a scale
+KV4_HEAD_DIMS = (64, 128, 256)
+_SIGNATURES["ts_kv4_store"] = [_c_void_p, _c_void_p, _c_int, _c_ll, _c_ll, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p]
+_SIGNATURES["ts_kv4_load"] = [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p]
+_SIGNATURES["ts_kv4_evict"] = [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p] + [_c_int] * 8 + [_c_void_p]
+_attention_kv4: dict[int, tuple] = {}
+
+
+def kv4_pool_shape(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int) -> tuple[int, int, int, int]:
+    """Shape of the uint8 pool of a 4-bit cache: 9/8 bytes per channel of a cached row (keys and values).
+
+    A record (last dimension) holds 16 tokens of one head: codes of the key rows, their scales, the same of the
+    values.  A value is (code - 8) * scale with a code of 4 bits and, for every 16 channels, a scale of 5 exponent
+    and 3 mantissa bits (the upper bits of a positive half)."""
+    if head_dim not in KV4_HEAD_DIMS:
+        raise KernelError(f"4-bit cache: heads of {KV4_HEAD_DIMS} channels, got {head_dim}")
+    if page_size < KV4_BLOCK or page_size % KV4_BLOCK:
+        raise KernelError(f"4-bit cache: the page size must be a multiple of {KV4_BLOCK}, got {page_size}")
+    return (num_pages, num_kv_heads, page_size // KV4_BLOCK, 18 * head_dim)
+
+
+def _kv4_pool(name: str, pool: torch.Tensor) -> tuple[int, int, int, int]:
+    """(pages, key/value heads, records per page, head size) of a pool."""
+    _cuda_contig(f"{name}: pool", pool, torch.uint8)
+    if pool.dim() != 4 or pool.shape[3] % 18 or pool.shape[3] // 18 not in KV4_HEAD_DIMS or min(pool.shape) < 1:
+        raise KernelError(f"{name}: the pool must be [pages, heads, page size / 16, 18 * head size] with heads of {KV4_HEAD_DIMS}, got {tuple(pool.shape)}")
+    if pool.data_ptr() % 16 or pool.shape[0] * pool.shape[2] * KV4_BLOCK >= 1 << 31:
+        raise KernelError(f"{name}: the pool must start on a 16-byte boundary and hold fewer than 2^31 rows")
+    return pool.shape[0], pool.shape[1], pool.shape[2], pool.shape[3] // 18
+
+
+def _kv4_sums(name: str, sums: torch.Tensor, pool: torch.Tensor) -> None:
+    _cuda_contig(f"{name}: sums", sums, torch.float32)
+    want = (pool.shape[0], pool.shape[1], pool.shape[2] * KV4_BLOCK)
+    if tuple(sums.shape) != want:
+        raise KernelError(f"{name}: sums must be [pages, heads, page size] = {want}, got {tuple(sums.shape)}")
+
+
+def kv4_store(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, slot_mapping: torch.Tensor, sums: Optional[torch.Tensor] = None) -> None:
+    """Rows of keys and values into a 4-bit cache.
+
+    k, v [T, nkv, d] float32 or bfloat16, a row's heads contiguous (rows may be further apart, as in a product's
+    output that also holds the queries); slot_mapping [T] i32: page * page size + place, -1 = skip.  Per 16 channels: scale = max|x| / 7 rounded to
+    the nearest scale (ties to even, at most 8192), code = round(x / scale).  NaN is stored as 0, infinities as the
+    largest value.  `sums` (the pool's weights, see attention_kv4_weights): set to 0 at the stored rows."""
+    flush_gemm_chain()
+    pages, nkv, blocks, d = _kv4_pool("kv4_store", pool)
+    code = _act_code("kv4_store: k", k)
+    _cuda_contig("kv4_store: slot_mapping", slot_mapping, torch.int32)
+    for name, t in (("k", k), ("v", v)):
+        if not t.is_cuda or t.dtype != k.dtype or t.dim() != 3 or tuple(t.shape[1:]) != (nkv, d) or t.shape[0] != k.shape[0]:
+            raise KernelError(f"kv4_store: {name} must be a CUDA tensor [T, {nkv}, {d}] of k's type, got {tuple(t.shape)} {t.dtype}")
+        if t.shape[0] > 0 and ((t.stride(2) != 1 and d > 1) or (t.stride(1) != d and nkv > 1)):
+            raise KernelError(f"kv4_store: {name}'s heads must lie one behind the other, got strides {t.stride()}")
+        if t.shape[0] > 1 and t.stride(0) * t.element_size() % 16 or t.data_ptr() % 16:
+            raise KernelError(f"kv4_store: {name}'s rows must start on 16-byte boundaries")
+    if slot_mapping.numel() < k.shape[0]:
+        raise KernelError("kv4_store: slot_mapping is shorter than the rows")
+    if sums is not None:
+        _kv4_sums("kv4_store", sums, pool)
+    _check("kv4_store", _fn("ts_kv4_store")(
+        k.data_ptr(), v.data_ptr(), code, k.stride(0), v.stride(0), pool.data_ptr(), _ptr(sums), slot_mapping.data_ptr(), k.shape[0], nkv, d, blocks,
+        pages, _stream()))
+
+
+def kv4_load(pool: torch.Tensor, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+    """Rows of a 4-bit cache as values: k, v [N, nkv, d] float32 or bfloat16 (exact in both); slots [N] i32, a slot outside the pool gives zeros."""
+    flush_gemm_chain()
+    pages, nkv, blocks, d = _kv4_pool("kv4_load", pool)
+    code = _act_code("kv4_load: k", k)
+    _cuda_contig("kv4_load: slots", slots, torch.int32)
+    N = slots.numel()
+    for name, t in (("k", k), ("v", v)):
+        _cuda_contig(f"kv4_load: {name}", t, k.dtype)
+        if tuple(t.shape) != (N, nkv, d) or t.data_ptr() % 16:
+            raise KernelError(f"kv4_load: {name} must be [{N}, {nkv}, {d}] on a 16-byte boundary, got {tuple(t.shape)}")
+    _check("kv4_load", _fn("ts_kv4_load")(
+        pool.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), code, N, nkv, d, blocks, pages, _stream()))
+
+
+def _attention_kv4_fns(head_dim: int) -> tuple:
+    fns = _attention_kv4.get(head_dim)
+    if fns is None:
+        lib = _build.load_variant("kv4_attention", {"TS_HEAD_DIM": head_dim})
+        run, weights = lib.ts_attention_kv4, lib.ts_attention_kv4_weights
+        run.argtypes = [_c_void_p, _c_int] + [_c_void_p] * 7 + [_c_int] * 8 + [_c_float, _c_int, _c_int, _c_void_p, _c_void_p]
+        weights.argtypes = [_c_void_p, _c_int] + [_c_void_p] * 6 + [_c_int] * 8 + [_c_float, _c_int, _c_void_p]
+        run.restype = weights.restype = _c_int
+        fns = _attention_kv4[head_dim] = (run, weights)
+    return fns
+
+
+def _check_attention_kv4(name, q, pool, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, d, window) -> tuple:
+    """Checks the arguments that attention over a 4-bit cache and its weights share; returns (pages, records per page, type code)."""
+    pages, pool_heads, blocks, pool_dim = _kv4_pool(name, pool)
+    code = _act_code(f"{name}: q", q)
+    _cuda_contig(f"{name}: q", q)
+    for label, t in (("cu_seqlens_q", cu_seqlens_q), ("context_lens", context_lens), ("block_table", block_table)):
+        _cuda_contig(f"{name}: {label}", t, torch.int32)
+    if (pool_heads, pool_dim) != (nkv, d):
+        raise KernelError(f"{name}: the pool holds {pool_heads} heads of {pool_dim}, the call names {nkv} of {d}")
+    if nkv < 1 or nq % nkv:
+        raise KernelError(f"{name}: {nq} query heads are no multiple of {nkv} key/value heads")
+    if q.dim() < 1 or q.numel() != q.shape[0] * nq * d or q.data_ptr() % 16:
+        raise KernelError(f"{name}: q must be [T, {nq * d}] on a 16-byte boundary, got {tuple(q.shape)}")
+    if block_table.dim() != 2 or block_table.shape[0] < num_seqs or (num_seqs > 0 and block_table.shape[1] < 1):
+        raise KernelError(f"{name}: block_table must be [B, max_blocks]")
+    if cu_seqlens_q.numel() < num_seqs + 1 or context_lens.numel() < num_seqs:
+        raise KernelError(f"{name}: cu_seqlens_q/context_lens are shorter than the batch")
+    if num_seqs < 0 or max_seqlen_q < 0 or max_context < 0 or window < 0:
+        raise KernelError(f"{name}: negative sizes")
+    return pages, blocks, code
+
+
+def attention_kv4_splits(num_seqs: int, num_kv_heads: int, row_tiles: int, max_context: int) -> int:
+    """Over how many CTAs the keys of a (sequence, key head, row tile) are spread."""
+    pairs = max(1, num_seqs * num_kv_heads * row_tiles)
+    return max(1, min(32, 592 // pairs, -(-max_context // 256)))
+
+
+def attention_kv4(
+    q: torch.Tensor,
+    pool: torch.Tensor,
+    out: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    num_seqs: int,
+    max_seqlen_q: int,
+    max_context: int,
+    num_heads: int,
+    num_kv_heads: int,
+    head_dim: int,
+    scale: float,
+    window: int = 0,
+    head_sinks: Optional[torch.Tensor] = None,
+    lse: Optional[torch.Tensor] = None,
+) -> None:
+    """Causal attention over a 4-bit cache, for decoded tokens and for portions of prompts.
+
+    q/out [T,nq*d] float32 or bfloat16; pool: see kv4_pool_shape; cu_seqlens_q [B+1], context_lens [B] i32,
+    block_table [B,max_blocks] i32.  The tokens of a sequence are consecutive and are its cache's last rows: query i of
+    n sees the rows up to context_lens[b] - n + i.  (A row's number in the cache need not be its position: after kv4_evict it is
+    not.)  `max_seqlen_q` and `max_context` bound the lengths.  window > 0: a query sees the last `window` rows only; head_sinks [nq] f32:
+    a score that joins a head's softmax without a value; lse [T,nq] f32: receives the logarithm of every softmax's denominator
+    (-inf for a query that sees nothing; its output is zero)."""
+    flush_gemm_chain()
+    nq, nkv, d = num_heads, num_kv_heads, head_dim
+    pages, blocks, code = _check_attention_kv4("attention_kv4", q, pool, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context,
+                                               nq, nkv, d, window)
+    T = q.shape[0]
+    _cuda_contig("attention_kv4: out", out, q.dtype)
+    if out.numel() != q.numel() or out.data_ptr() % 16:
+        raise KernelError(f"attention_kv4: out must be of q's size on a 16-byte boundary, got {tuple(out.shape)}")
+    for label, t, n in (("head_sinks", head_sinks, nq), ("lse", lse, T * nq)):
+        if t is not None:
+            _cuda_contig(f"attention_kv4: {label}", t, torch.float32)
+            if t.numel() != n:
+                raise KernelError(f"attention_kv4: {label} must have {n} entries, got {t.numel()}")
+    rows = max_seqlen_q * (nq // nkv)
+    splits = attention_kv4_splits(num_seqs, nkv, -(-rows // 8), min(max_context, window + max_seqlen_q) if window else max_context)
+    part = torch.empty(T * nq * splits * (d + 4), device=q.device, dtype=torch.float32) if splits > 1 else None
+    run, _ = _attention_kv4_fns(d)
+    _check("attention_kv4", run(
+        q.data_ptr(), code, pool.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(head_sinks), cu_seqlens_q.data_ptr(), context_lens.data_ptr(),
+        block_table.data_ptr(), block_table.shape[1], blocks, pages, T, num_seqs, max_seqlen_q, nq, nkv, float(scale), int(window), splits, _ptr(part),
+        _stream()))
+
+
+def attention_kv4_weights(
+    q: torch.Tensor,
+    pool: torch.Tensor,
+    lse: torch.Tensor,
+    sums: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    num_seqs: int,
+    max_seqlen_q: int,
+    max_context: int,
+    num_heads: int,
+    num_kv_heads: int,
+    head_dim: int,
+    scale: float,
+    window: int = 0,
+) -> None:
+    """Adds to every cached row the weight that this step's queries gave it: sums[row] += sum over the queries and the
+    query heads of the row's key head of exp(scale q.k - lse).  Arguments as in attention_kv4, `lse` as it wrote it (sinks are in it);
+    sums [pages, nkv, page size] f32.  Every row's sum is formed in one order: equal inputs give equal bits."""
+    flush_gemm_chain()
+    nq, nkv, d = num_heads, num_kv_heads, head_dim
+    pages, blocks, code = _check_attention_kv4("attention_kv4_weights", q, pool, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q,
+                                               max_context, nq, nkv, d, window)
+    _cuda_contig("attention_kv4_weights: lse", lse, torch.float32)
+    if lse.numel() != q.shape[0] * nq:
+        raise KernelError(f"attention_kv4_weights: lse must have {q.shape[0] * nq} entries, got {lse.numel()}")
+    _kv4_sums("attention_kv4_weights", sums, pool)
+    _, run = _attention_kv4_fns(d)
+    _check("attention_kv4_weights", run(
+        q.data_ptr(), code, pool.data_ptr(), lse.data_ptr(), sums.data_ptr(), cu_seqlens_q.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(),
+        block_table.shape[1], blocks, pages, q.shape[0], num_seqs, max_context, nq, nkv, float(scale), int(window), _stream()))
+
+
+def kv4_evict(pool: torch.Tensor, sums: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor, num_seqs: int,
+              max_context: int, budget: int, recent: int, first: int = 0) -> None:
+    """Cuts requests to `budget` cached rows, every key/value head by its own weights.
+
+    A request with more rows than that keeps, per head, the `first` first ones, the `recent` last ones and of the rest those with
+    the largest `sums` (of equals the earlier, NaN before all).  They move to the front of the request's pages in their order, their sums with
+    them; the sums behind become 0.  block_table [B,max_blocks], context_lens [B] i32 (at most max_context); new_lens [B] i32 receives
+    min(length, budget).  Pages behind the new length can be given back."""
+    flush_gemm_chain()
+    pages, nkv, blocks, d = _kv4_pool("kv4_evict", pool)
+    _kv4_sums("kv4_evict", sums, pool)
+    for label, t in (("block_table", block_table), ("context_lens", context_lens), ("new_lens", new_lens)):
+        _cuda_contig(f"kv4_evict: {label}", t, torch.int32)
+    if block_table.dim() != 2 or block_table.shape[0] < num_seqs or context_lens.numel() < num_seqs or new_lens.numel() < num_seqs:
+        raise KernelError("kv4_evict: block_table/context_lens/new_lens are shorter than the batch")
+    if budget < 1 or recent < 0 or first < 0 or first + recent > budget:
+        raise KernelError(f"kv4_evict: a budget of {budget} rows cannot hold the first {first} and the last {recent}")
+    if max_context < 0 or num_seqs < 0:
+        raise KernelError("kv4_evict: negative sizes")
+    _check("kv4_evict", _fn("ts_kv4_evict")(
+        pool.data_ptr(), sums.data_ptr(), block_table.data_ptr(), block_table.shape[1], context_lens.data_ptr(), new_lens.data_ptr(), num_seqs, nkv, d,
+        blocks, pages, int(budget), int(recent), int(first), _stream()))
+
+
+# ---------------------------------------------------------------------------
 # skinny GEMM on tcgen05 tensor cores (decode steps)
 
 GEMM_SKINNY_MAX_ROWS = 128
@@ -2927,7 +3158,7 @@ _TIMED = ("embed_gather", "feed_tokens", "add_rmsnorm", "residual_add", "swiglu"
           "router_topk", "router", "moe_plan", "moe_gate_up", "moe_down", "moe_combine", "branch_norm_add", "stream_add",
           "qk_joint_norm_rope_store", "gla_scan", "gla_norm_gate", "linear_scan", "rows_dot_f32", "mlstm_gate_scan", "mlstm_norm_gate",
           "ssm_conv", "ssm_gate_norm", "scale_rows", "weighted_sum", "rope_table", "qkv_prepare", "gate_rows", "causal_conv", "delta_scan",
-          "channel_decay", "retention_scan",
+          "channel_decay", "retention_scan", "kv4_store", "kv4_load", "attention_kv4", "attention_kv4_weights", "kv4_evict",
           "softcap_rows", "rglru_scan", "rglru_step", "rmsnorm_rows", "library_bmm_float32")
 _plain_functions: dict[str, object] = {}
 _kernel_events: list[tuple[str, "torch.cuda.Event", "torch.cuda.Event"]] = []

@@ -240,6 +240,7 @@ def build_all() -> list[Path]:
     paths += [build_variant("attention_mma", {"TS_HEAD_DIM": d, "TS_ATT_SCORED": 1}) for d in (64, 128)]
     paths.append(build_variant("attention_tcgen05", {"TS_HEAD_DIM": 128, "TS_ATT_SCORED": 1}))
     paths.append(build_variant("attention_tcgen05", {"TS_HEAD_DIM": 128, "TS_ATT_SCORED": 1, "TS_ATT_ROT": 64}))
+    paths += [build_variant("attention_tcgen05", {"TS_HEAD_DIM": 128, "TS_ATT_LSE": 1, "TS_ATT_FMA_PAIRS": 0, "TS_ATT_SCORED": s}) for s in (0, 1)]
     paths += [build_variant("kv4_attention", {"TS_HEAD_DIM": d}) for d in (64, 128, 256)]
     paths.append(build_variant("latent_attention_mma", {"TS_LAT_RANK": 512, "TS_LAT_ROT": 64}))
     return paths

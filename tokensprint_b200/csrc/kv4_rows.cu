@@ -125,6 +125,51 @@ __global__ void __launch_bounds__(128) load_kernel(const uint8_t* pool, const in
   write_group((values ? v : k) + ((size_t)row * nkv * groups + unit) * 16, x);
 }
 
+// The rows that a batch's queries can see, of heads of 128, as bfloat16 pages of 128 rows for the prompt attention, and the block table of those
+// pages: request b has the pages [b * blocks, (b + 1) * blocks); out_lens: its rows, as many as have a place.  A CTA unpacks 64 rows of one head.
+constexpr int kExpandRows = 64, kExpandPage = 128, kExpandDim = 128;
+__global__ void __launch_bounds__(256) expand_kernel(const uint8_t* pool, const int* table, int table_stride, const int* cu, const int* context, uint4* k,
+                                                     uint4* v, int* out_table, int* out_lens, int nkv, int page_blocks, int num_pages, int blocks,
+                                                     int window) {
+  ts_pdl_prologue();
+  constexpr int kGroups = kExpandDim / 16, kUnits = kExpandRows * kGroups * 2 / 256;
+  const int b = blockIdx.z, head = blockIdx.y, first = blockIdx.x * kExpandRows;
+  const int n = min(context[b], min(table_stride * page_blocks * KV4_BLOCK, blocks * kExpandPage));
+  if (head == 0 && threadIdx.x == 0) {
+    if (first % kExpandPage == 0) out_table[b * blocks + first / kExpandPage] = b * blocks + first / kExpandPage;
+    if (first == 0) out_lens[b] = n;
+  }
+  const int queries = cu[b + 1] - cu[b], oldest = window > 0 ? n - queries - window + 1 : 0;  // the first key that some query sees
+  if (first >= n || first + kExpandRows <= oldest || queries <= 0) return;
+  uint2 code[kUnits];
+  uint32_t scale[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const int unit = threadIdx.x + 256 * i, grp = unit % kGroups, values = unit / (kExpandRows * kGroups);
+    const int row = min(first + unit / kGroups % kExpandRows, n - 1), blk = row / KV4_BLOCK;
+    const int page = min(max(table[(size_t)b * table_stride + blk / page_blocks], 0), num_pages - 1);
+    const uint8_t* rec = pool + (((size_t)page * nkv + head) * page_blocks + blk % page_blocks) * (18 * kExpandDim) + values * 9 * kExpandDim;
+    code[i] = *reinterpret_cast<const uint2*>(rec + row % KV4_BLOCK * (kExpandDim / 2) + grp * 8);
+    scale[i] = rec[8 * kExpandDim + row % KV4_BLOCK * kGroups + grp];
+  }
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const int unit = threadIdx.x + 256 * i, grp = unit % kGroups, values = unit / (kExpandRows * kGroups);
+    const int row = first + unit / kGroups % kExpandRows;
+    __nv_bfloat162 f, c;
+    kv4_factors(scale[i], scale[i], f, c);
+    uint4 out[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t x = j ? code[i].y : code[i].x;
+      const uint32_t p0 = kv4_pair(x << 3, f, c), p1 = kv4_pair(x >> 1, f, c), p2 = kv4_pair(x >> 5, f, c), p3 = kv4_pair(x >> 9, f, c);
+      out[j] = make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
+    }
+    uint4* dst = (values ? v : k) + (((size_t)b * blocks * kExpandPage + row) * nkv + head) * (kExpandDim / 8) + grp * 2;
+    if (row < n) dst[0] = out[0], dst[1] = out[1];
+  }
+}
+
 // ---------------------------------------------------------------------------
 // eviction
 
@@ -287,6 +332,15 @@ TS_EXPORT int ts_kv4_load(const void* pool, const int* slots, void* k, void* v, 
     return ts_launch(load_kernel<float>, grid, dim3(128), 0, s, (const uint8_t*)pool, slots, (float*)k, (float*)v, rows, nkv, d, page_blocks, num_slots);
   return ts_launch(load_kernel<__nv_bfloat16>, grid, dim3(128), 0, s, (const uint8_t*)pool, slots, (__nv_bfloat16*)k, (__nv_bfloat16*)v, rows, nkv, d,
                    page_blocks, num_slots);
+}
+
+// k, v: [num_seqs * blocks][128][nkv][128] bfloat16, out_table [num_seqs][blocks]; blocks * 128 rows hold the longest request.
+TS_EXPORT int ts_kv4_expand(const void* pool, const int* table, int table_stride, const int* cu, const int* context, void* k, void* v, int* out_table,
+                            int* out_lens, int num_seqs, int nkv, int page_blocks, int num_pages, int blocks, int window, void* stream) {
+  if (num_seqs < 1 || blocks < 1) return 0;
+  if (num_seqs > 65535 || nkv > 65535) return TS_ERR_UNSUPPORTED_SIZE;
+  return ts_launch(expand_kernel, dim3(blocks * (kExpandPage / kExpandRows), nkv, num_seqs), dim3(256), 0, (cudaStream_t)stream, (const uint8_t*)pool, table,
+                   table_stride, cu, context, (uint4*)k, (uint4*)v, out_table, out_lens, nkv, page_blocks, num_pages, blocks, window);
 }
 
 TS_EXPORT int ts_kv4_evict(void* pool, float* sums, const int* table, int table_stride, const int* context, int* new_lens, int num_seqs, int nkv, int d,

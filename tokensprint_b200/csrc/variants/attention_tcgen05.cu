@@ -68,6 +68,10 @@ constexpr int MAX_TABLE = 1024;                   // block-table entries kept in
 #define TS_ATT_SCORED 0
 #endif
 [[maybe_unused]] constexpr bool SCORED = TS_ATT_SCORED != 0;
+// Builds with TS_ATT_LSE=1 also write the logarithm of every row's softmax denominator.
+#ifndef TS_ATT_LSE
+#define TS_ATT_LSE 0
+#endif
 struct Params {
   __nv_bfloat16* out;     // [T, nq, D]
   const int* cu_q;        // [B + 1]
@@ -84,6 +88,9 @@ struct Params {
   float cap_raw, cap_inv;   // cap / scale and scale / cap: a raw score s becomes cap_raw * tanh(s * cap_inv); cap_raw 0: no cap
   const float* dist_r1;     // [nq] with dist_r2: the scaled score of key j for a query at position i loses r1 * ln(1 + r2 * (i - j)); null: no penalty
   const float* dist_r2;
+#endif
+#if TS_ATT_LSE
+  float* lse;  // [T, nq], or null
 #endif
 #if TS_ATT_ROT
   const float* gates;  // [T, nq] what a finished row is multiplied by, or null
@@ -209,6 +216,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
+#if TS_ATT_LSE
+// The logarithm of a row's denominator, from its maximum in raw score units and the sum relative to it.
+__device__ __forceinline__ float row_lse(const Params& p, float m, float l) {
+  return l > 0.f ? (m * p.scale_log2 + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+#endif
+
 // The sink score, in raw units, of row `r` of a (sequence, KV head) pair's rows (row r belongs to query head hk * G + r % G).
 __device__ __forceinline__ float row_sink_raw(const Params& p, int hk, int G, int r) {
 #if TS_ATT_SCORED
@@ -528,6 +542,9 @@ __global__ void __launch_bounds__(128, 2) attention_tcgen05_kernel(const __grid_
   __syncthreads();
   if (abort_s == 0 && tid < RT && r < rows_total) {
     const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+#if TS_ATT_LSE
+    if (p.lse != nullptr) p.lse[(size_t)(q_begin + r / G) * p.nq + hk * G + r % G] = row_lse(p, m_run, l_run);
+#endif
     __nv_bfloat16* dst = p.out + ((size_t)(q_begin + r / G) * p.nq + hk * G + r % G) * D;
 #pragma unroll
     for (int c = 0; c < D / 8; ++c) {
@@ -1164,6 +1181,9 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
     asm volatile("bar.sync %0, 256;" ::"r"(1 + t) : "memory");
     l_run += sum_s[t][h ^ 1][row];
     float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+#if TS_ATT_LSE
+    if (p.lse != nullptr && good && h == 0 && row < RT && r < rows_total) p.lse[(size_t)(q_begin + r / G) * p.nq + hk * G + r % G] = row_lse(p, m_run, l_run);
+#endif
 #if TS_ATT_ROT
     if (p.gates != nullptr && row_pos >= 0) inv *= p.gates[(size_t)(q_begin + r) * p.nq + hk];
 #endif
@@ -1344,7 +1364,12 @@ TS_EXPORT int ts_attention_prefill_tcgen05_scored(const void* q, const void* kca
                                                   int max_blocks, int page, long long total_slots, int T, int B, int max_q,
                                                   int nq, int nkv, float scale, int window, int chunk, int has_sink, float sink_score,
                                                   float softcap, const float* head_sinks, int mode, int* error, void* stream_,
-                                                  const float* dist_r1, const float* dist_r2) {
+                                                  const float* dist_r1, const float* dist_r2
+#if TS_ATT_LSE
+                                                  ,
+                                                  float* lse
+#endif
+) {
   if (T <= 0 || B <= 0) return 0;
   if (!SCORED && (head_sinks != nullptr || softcap > 0.f || dist_r1 != nullptr)) return TS_ERR_BAD_ARGUMENT;
   if ((dist_r1 == nullptr) != (dist_r2 == nullptr) || (dist_r1 != nullptr && !(scale > 0.f))) return TS_ERR_BAD_ARGUMENT;
@@ -1380,6 +1405,9 @@ TS_EXPORT int ts_attention_prefill_tcgen05_scored(const void* q, const void* kca
   p.num_seqs = B;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.probe = probe_buffer;
+#if TS_ATT_LSE
+  p.lse = lse;
+#endif
   const int G = nq / nkv;
   const int RT = (BM / G) * G;  // rows of a tile that belong to tokens
   const long long rows = (long long)max_q * G;
@@ -1414,6 +1442,7 @@ TS_EXPORT int ts_attention_prefill_tcgen05_scored(const void* q, const void* kca
                    mv, p);
 }
 
+#if !TS_ATT_LSE
 TS_EXPORT int ts_attention_prefill_tcgen05(const void* q, const void* kcache, const void* vcache, void* out,
                                            const int* cu_q, const int* ctx_len, const int* block_table,
                                            int max_blocks, int page, long long total_slots, int T, int B, int max_q,
@@ -1422,4 +1451,5 @@ TS_EXPORT int ts_attention_prefill_tcgen05(const void* q, const void* kcache, co
   return ts_attention_prefill_tcgen05_scored(q, kcache, vcache, out, cu_q, ctx_len, block_table, max_blocks, page, total_slots, T, B, max_q,
                                              nq, nkv, scale, window, chunk, has_sink, sink_score, 0.f, nullptr, mode, error, stream_, nullptr, nullptr);
 }
+#endif  // TS_ATT_LSE
 #endif  // TS_ATT_ROT

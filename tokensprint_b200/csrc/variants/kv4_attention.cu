@@ -390,6 +390,176 @@ __global__ void __launch_bounds__(kWarps * 32) weights_kernel(const Params p, fl
   }
 }
 
+// The same for many rows (portions of prompts).  A CTA owns 128 keys (64 for heads of 256): its warps keep their keys
+// unpacked in registers, kKeyWarps of them side by side, while the query rows pass through shared memory, 64 at a time and
+// twice buffered; kRowWarps warps share a key and take the rows in turns, and add up at the end in one order.
+constexpr int kKeyTiles = D <= 128 ? 2 : 1;  // of 16 keys per warp
+constexpr int kKeyWarps = 4, kRowWarps = 4, kStageRows = 64;
+constexpr int kChunkKeys = kKeyWarps * kKeyTiles * 16, kWeightThreads = kKeyWarps * kRowWarps * 32;
+
+template <int kQ>
+struct WeightsStage {
+  static constexpr int kBytes = kQ * kStageRows * D * 2 + kStageRows * 8;
+};
+
+template <typename T, int kQ>
+__global__ void __launch_bounds__(kWeightThreads, 1) weights_rows_kernel(const Params p, float* sums) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float meet[kRowWarps][kChunkKeys];
+  constexpr int kStage = WeightsStage<kQ>::kBytes, kChunks = D / 8;  // 16-byte pieces of a row
+  ts_pdl_prologue();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const int key_warp = warp % kKeyWarps, row_warp = warp / kKeyWarps;
+  Tile tile;
+  tile.open(p, blockIdx.z, blockIdx.y);
+  const int chunk_key = blockIdx.x * kChunkKeys, before = tile.context - tile.q_len;
+  if (chunk_key >= tile.context) return;
+  const int last_key = min(chunk_key + kChunkKeys, tile.context) - 1;
+  const int first_token = max(0, chunk_key - before);
+  const int tokens = p.window > 0 ? min(tile.q_len, last_key + p.window - before) : tile.q_len;
+  if (first_token >= tokens) return;
+  const int first_row = first_token * p.group, rows = tokens * p.group;
+
+  // this warp's keys: word u = 4w + t of a row holds the channels 8u..8u+7, unpacked as the pairs (0,1) (2,3) (4,5) (6,7)
+  const int key = chunk_key + key_warp * kKeyTiles * 16;
+  uint32_t a[kKeyTiles][D / 32][2][4];
+#pragma unroll
+  for (int m = 0; m < kKeyTiles; ++m) {
+    const int blk = key / KV4_BLOCK + m;
+    const bool there = blk * KV4_BLOCK < tile.context;
+    const uint8_t* rec = record(p, there ? p.table[(size_t)tile.b * p.table_stride + blk / p.page_blocks] : 0, blk, tile.head);
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int w = 0; w < D / 32; ++w) {
+        const int u = 4 * w + t;
+        const uint32_t x = *reinterpret_cast<const uint32_t*>(rec + (g + 8 * r) * (D / 2) + 4 * u);
+        const uint32_t sc = rec[Rec::kKeyScales + (g + 8 * r) * (D / 16) + u / 2];
+        __nv_bfloat162 f, c;
+        kv4_factors(sc, sc, f, c);
+        const uint32_t p0 = kv4_pair(x << 3, f, c), p1 = kv4_pair(x >> 1, f, c), p2 = kv4_pair(x >> 5, f, c), p3 = kv4_pair(x >> 9, f, c);
+        a[m][w][r][0] = __byte_perm(p0, p1, 0x5410), a[m][w][r][1] = __byte_perm(p2, p3, 0x5410);
+        a[m][w][r][2] = __byte_perm(p0, p1, 0x7632), a[m][w][r][3] = __byte_perm(p2, p3, 0x7632);
+      }
+  }
+
+  // A stage: its rows [part][64][D] bfloat16, the 16-byte piece c of row r at c ^ (r & 1) * 4 (eight lanes of a warp's read
+  // then fall on eight different groups of banks), then every row's logarithm and last visible key.
+  const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(smem);
+  auto fetch = [&](int stage, int base) {
+    uint8_t* buf = smem + stage * kStage;
+    for (int i = threadIdx.x; i < kStageRows * kChunks; i += kWeightThreads) {
+      const int r = i / kChunks, c = i % kChunks, at = r * D * 2 + ((c ^ ((r & 1) * 4)) * 16);
+      const bool there = base + r < rows;
+      const T* src = tile.query<T>(p, there ? base + r : first_row) + c * 8;
+      if constexpr (sizeof(T) == 2) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at + stage * kStage + at), "l"(src), "r"(there ? 16 : 0));
+      } else {
+        const float4 lo = reinterpret_cast<const float4*>(src)[0], hi = reinterpret_cast<const float4*>(src)[1];
+        const float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        uint32_t parts[4][kQ];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kv4_split<kQ>(there ? x[2 * j] : 0.f, there ? x[2 * j + 1] : 0.f, parts[j]);
+#pragma unroll
+        for (int k = 0; k < kQ; ++k)
+          *reinterpret_cast<uint4*>(buf + k * kStageRows * D * 2 + at) = make_uint4(parts[0][k], parts[1][k], parts[2][k], parts[3][k]);
+      }
+    }
+    if (threadIdx.x < kStageRows) {
+      const int row = base + threadIdx.x;
+      float lse = INFINITY;  // a row that does not exist gives no weight
+      int pos = -1;
+      if (row < rows) lse = p.lse[(size_t)tile.token(p, row) * p.nq + tile.query_head(p, row)] * kLog2e, pos = tile.position(p, row);
+      reinterpret_cast<float2*>(buf + kQ * kStageRows * D * 2)[threadIdx.x] = make_float2(lse, __int_as_float(pos));
+    }
+    copy_commit();
+  };
+
+  float w[kKeyTiles][2];
+#pragma unroll
+  for (int m = 0; m < kKeyTiles; ++m) w[m][0] = w[m][1] = 0.f;
+  fetch(0, first_row);
+  int stage = 0;
+  for (int base = first_row; base < rows; base += kStageRows, stage ^= 1) {
+    if (base + kStageRows < rows) fetch(stage ^ 1, base + kStageRows);
+    else copy_commit();
+    copy_wait<1>();
+    __syncthreads();
+    const uint8_t* buf = smem + stage * kStage;
+    const float2* info = reinterpret_cast<const float2*>(buf + kQ * kStageRows * D * 2);
+#pragma unroll 1
+    for (int n = row_warp * 8; n < kStageRows && base + n < rows; n += kRowWarps * 8) {
+      float s[kKeyTiles][4];
+#pragma unroll
+      for (int m = 0; m < kKeyTiles; ++m) s[m][0] = s[m][1] = s[m][2] = s[m][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kQ; ++k)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const uint4 q = *reinterpret_cast<const uint4*>(buf + k * kStageRows * D * 2 + (n + g) * D * 2 + (((4 * i + t) ^ ((g & 1) * 4)) * 16));
+#pragma unroll
+          for (int m = 0; m < kKeyTiles; ++m) kv4_mma(s[m], a[m][i][0][0], a[m][i][1][0], a[m][i][0][1], a[m][i][1][1], q.x, q.y);
+#pragma unroll
+          for (int m = 0; m < kKeyTiles; ++m) kv4_mma(s[m], a[m][i][0][2], a[m][i][1][2], a[m][i][0][3], a[m][i][1][3], q.z, q.w);
+        }
+      const float2 r0 = info[n + 2 * t], r1 = info[n + 2 * t + 1];
+      const int p0 = __float_as_int(r0.y), p1 = __float_as_int(r1.y);
+      // (positions grow with the rows)
+      const int low = __float_as_int(info[n].y), high = __float_as_int(info[min(n + 7, rows - 1 - base)].y);
+      const bool all = low >= key + kKeyTiles * 16 - 1 && (p.window == 0 || high - p.window < key);
+#pragma unroll
+      for (int m = 0; m < kKeyTiles; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int at = key + 16 * m + g + 8 * i;
+          const float e0 = kv4_exp2(fmaf(s[m][2 * i], p.scale, -r0.x)), e1 = kv4_exp2(fmaf(s[m][2 * i + 1], p.scale, -r1.x));
+          if (all) {
+            w[m][i] += e0 + e1;
+          } else {
+            if (at <= p0 && (p.window == 0 || at > p0 - p.window)) w[m][i] += e0;
+            if (at <= p1 && (p.window == 0 || at > p1 - p.window)) w[m][i] += e1;
+          }
+        }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int m = 0; m < kKeyTiles; ++m)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[m][i] += __shfl_xor_sync(0xffffffffu, w[m][i], 1);
+      w[m][i] += __shfl_xor_sync(0xffffffffu, w[m][i], 2);
+      if (t == 0) meet[row_warp][(key_warp * kKeyTiles + m) * 16 + g + 8 * i] = w[m][i];
+    }
+  __syncthreads();
+  const int at = chunk_key + threadIdx.x;
+  if (threadIdx.x < kChunkKeys && at < tile.context) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kRowWarps; ++i) sum += meet[i][threadIdx.x];
+    const int page_size = p.page_blocks * KV4_BLOCK, page = p.table[(size_t)tile.b * p.table_stride + at / page_size];
+    sums[((size_t)min(max(page, 0), p.num_pages - 1) * p.nkv + tile.head) * page_size + at % page_size] += sum;
+  }
+}
+
+template <typename T, int kQ>
+int launch_weights(const Params& p, float* sums, int num_seqs, int max_context, int max_q, cudaStream_t stream) {
+  // A key of few rows is read, used and done with (16 rows are two turns of a warp); with more, unpacking it once pays.
+  if (max_q * p.group <= 16) {
+    const dim3 grid((max_context + KV4_BLOCK * kWarps - 1) / (KV4_BLOCK * kWarps), p.nkv, num_seqs);
+    return ts_launch(weights_kernel<T, kQ>, grid, dim3(kWarps * 32), 0, stream, p, sums);
+  }
+  constexpr int smem = 2 * WeightsStage<kQ>::kBytes;
+  static bool set = false;
+  if (!set) {
+    cudaError_t e = cudaFuncSetAttribute(weights_rows_kernel<T, kQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    set = true;
+  }
+  const dim3 grid((max_context + kChunkKeys - 1) / kChunkKeys, p.nkv, num_seqs);
+  return ts_launch(weights_rows_kernel<T, kQ>, grid, dim3(kWeightThreads), smem, stream, p, sums);
+}
+
 template <typename T, int kTiles, int kQ, int kP>
 int launch_attention(const Params& p, int num_seqs, int rows, cudaStream_t stream) {
   constexpr int ring = kWarps * kStages * Rec::kBytes, meet = kWarps * 8 * kTiles * (D + 2) * 4;
@@ -428,12 +598,11 @@ TS_EXPORT int ts_attention_kv4(const void* q, int dtype, const void* pool, void*
 }
 
 TS_EXPORT int ts_attention_kv4_weights(const void* q, int dtype, const void* pool, float* lse, float* sums, const int* cu, const int* context,
-                                       const int* table, int table_stride, int page_blocks, int num_pages, int tokens, int num_seqs, int max_context, int nq, int nkv,
-                                       float scale, int window, void* stream) {
+                                       const int* table, int table_stride, int page_blocks, int num_pages, int tokens, int num_seqs, int max_q, int max_context, int nq,
+                                       int nkv, float scale, int window, void* stream) {
   if (tokens < 1 || num_seqs < 1 || max_context < 1) return 0;
   if (num_seqs > 65535 || nkv > 65535) return TS_ERR_UNSUPPORTED_SIZE;
   Params p = {q, (const uint8_t*)pool, nullptr, lse, nullptr, cu, context, table, nullptr, table_stride, page_blocks, num_pages, tokens, nq, nkv, nq / nkv, window, 1, 1, scale * kLog2e};
-  const dim3 grid((max_context + KV4_BLOCK * kWarps - 1) / (KV4_BLOCK * kWarps), nkv, num_seqs);
-  if (dtype == TS_DTYPE_F32) return ts_launch(weights_kernel<float, 3>, grid, dim3(kWarps * 32), 0, (cudaStream_t)stream, p, sums);
-  return ts_launch(weights_kernel<__nv_bfloat16, 1>, grid, dim3(kWarps * 32), 0, (cudaStream_t)stream, p, sums);
+  if (dtype == TS_DTYPE_F32) return launch_weights<float, 3>(p, sums, num_seqs, max_context, max_q, (cudaStream_t)stream);
+  return launch_weights<__nv_bfloat16, 1>(p, sums, num_seqs, max_context, max_q, (cudaStream_t)stream);
 }

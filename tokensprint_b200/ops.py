@@ -2513,7 +2513,12 @@ KV4_HEAD_DIMS = (64, 128, 256)
 _SIGNATURES["ts_kv4_store"] = [_c_void_p, _c_void_p, _c_int, _c_ll, _c_ll, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p]
 _SIGNATURES["ts_kv4_load"] = [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p]
 _SIGNATURES["ts_kv4_evict"] = [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p] + [_c_int] * 8 + [_c_void_p]
+_SIGNATURES["ts_kv4_expand"] = [_c_void_p, _c_void_p, _c_int] + [_c_void_p] * 6 + [_c_int] * 6 + [_c_void_p]
 _attention_kv4: dict[int, tuple] = {}
+# Portions of prompts with more rows (tokens x query heads of a key head) than this are attended to on tcgen05 tensor cores, over rows unpacked for the step.
+ATTENTION_KV4_DIRECT_ROWS = 64
+ATTENTION_KV4_EXPAND_BYTES = 1 << 30  # most bytes of unpacked rows at a time
+_attention_kv4_tcgen05: dict[bool, object] = {}
 
 
 def kv4_pool_shape(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int) -> tuple[int, int, int, int]:
@@ -2594,7 +2599,7 @@ def _attention_kv4_fns(head_dim: int) -> tuple:
         lib = _build.load_variant("kv4_attention", {"TS_HEAD_DIM": head_dim})
         run, weights = lib.ts_attention_kv4, lib.ts_attention_kv4_weights
         run.argtypes = [_c_void_p, _c_int] + [_c_void_p] * 7 + [_c_int] * 8 + [_c_float, _c_int, _c_int, _c_void_p, _c_void_p]
-        weights.argtypes = [_c_void_p, _c_int] + [_c_void_p] * 6 + [_c_int] * 8 + [_c_float, _c_int, _c_void_p]
+        weights.argtypes = [_c_void_p, _c_int] + [_c_void_p] * 6 + [_c_int] * 9 + [_c_float, _c_int, _c_void_p]
         run.restype = weights.restype = _c_int
         fns = _attention_kv4[head_dim] = (run, weights)
     return fns
@@ -2668,6 +2673,10 @@ def attention_kv4(
             if t.numel() != n:
                 raise KernelError(f"attention_kv4: {label} must have {n} entries, got {t.numel()}")
     rows = max_seqlen_q * (nq // nkv)
+    if rows > ATTENTION_KV4_DIRECT_ROWS and code == DTYPE_CODES[torch.bfloat16] and attention_tcgen05_supported(nq, nkv, d, _KV4_EXPAND_PAGE) and max_context > 0:
+        _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, scale, window,
+                                head_sinks, lse)
+        return
     splits = attention_kv4_splits(num_seqs, nkv, -(-rows // 8), min(max_context, window + max_seqlen_q) if window else max_context)
     part = torch.empty(T * nq * splits * (d + 4), device=q.device, dtype=torch.float32) if splits > 1 else None
     run, _ = _attention_kv4_fns(d)
@@ -2675,6 +2684,44 @@ def attention_kv4(
         q.data_ptr(), code, pool.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(head_sinks), cu_seqlens_q.data_ptr(), context_lens.data_ptr(),
         block_table.data_ptr(), block_table.shape[1], blocks, pages, T, num_seqs, max_seqlen_q, nq, nkv, float(scale), int(window), splits, _ptr(part),
         _stream()))
+
+
+_KV4_EXPAND_PAGE = 128
+
+
+def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, scale, window, head_sinks,
+                            lse) -> None:
+    """Portions of prompts over a 4-bit cache, heads of 128: the visible rows are unpacked into bfloat16 pages (they are exact in it), then the prompt
+    attention runs over those.  Requests are taken in groups whose unpacked rows fit ATTENTION_KV4_EXPAND_BYTES."""
+    global launch_count
+    d, page = ATTENTION_TCGEN05_HEAD_DIM, _KV4_EXPAND_PAGE
+    scored = head_sinks is not None
+    run = _attention_kv4_tcgen05.get(scored)
+    if run is None:
+        # (the denominators are an output here: every weight from the special-function unit, none from the cubic)
+        lib = _build.load_variant("attention_tcgen05", {"TS_HEAD_DIM": d, "TS_ATT_LSE": 1, "TS_ATT_FMA_PAIRS": 0, "TS_ATT_SCORED": int(scored)})
+        run = lib.ts_attention_prefill_tcgen05_scored
+        run.argtypes = _attention_tcgen05_fns()[0].argtypes + [_c_void_p]
+        run.restype = _c_int
+        _attention_kv4_tcgen05[scored] = run
+    blocks = -(-max_context // page)
+    pages, _, pool_blocks, _ = pool.shape
+    per_seq = 2 * blocks * page * nkv * d * 2
+    group = max(1, min(num_seqs, ATTENTION_KV4_EXPAND_BYTES // per_seq))
+    rows = torch.empty((2, group * blocks, page, nkv, d), device=q.device, dtype=torch.bfloat16)
+    table = torch.empty(group * (blocks + 1), device=q.device, dtype=torch.int32)  # and behind it the lengths
+    kept_lens = table[group * blocks :]
+    _, error = _gemm_workspace(q.device)
+    for lo in range(0, num_seqs, group):
+        n = min(group, num_seqs - lo)
+        cu, lens = cu_seqlens_q[lo : lo + n + 1], context_lens[lo : lo + n]
+        _check("kv4_expand", _fn("ts_kv4_expand")(
+            pool.data_ptr(), block_table[lo:].data_ptr(), block_table.shape[1], cu.data_ptr(), lens.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(),
+            table.data_ptr(), kept_lens.data_ptr(), n, nkv, pool_blocks, pages, blocks, int(window), _stream()))
+        _check("attention_kv4", run(
+            q.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), out.data_ptr(), cu.data_ptr(), kept_lens.data_ptr(), table.data_ptr(), blocks, page,
+            group * blocks * page, q.shape[0], n, max_seqlen_q, nq, nkv, float(scale), int(window), 0, 0, 0.0, 0.0, _ptr(head_sinks), 0, error.data_ptr(),
+            _stream(), None, None, _ptr(lse)))
 
 
 def attention_kv4_weights(
@@ -2708,7 +2755,7 @@ def attention_kv4_weights(
     _, run = _attention_kv4_fns(d)
     _check("attention_kv4_weights", run(
         q.data_ptr(), code, pool.data_ptr(), lse.data_ptr(), sums.data_ptr(), cu_seqlens_q.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(),
-        block_table.shape[1], blocks, pages, q.shape[0], num_seqs, max_context, nq, nkv, float(scale), int(window), _stream()))
+        block_table.shape[1], blocks, pages, q.shape[0], num_seqs, max_seqlen_q, max_context, nq, nkv, float(scale), int(window), _stream()))
 
 
 def kv4_evict(pool: torch.Tensor, sums: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor, num_seqs: int,

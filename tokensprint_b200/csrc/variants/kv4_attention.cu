@@ -20,7 +20,9 @@ namespace {
 constexpr int D = TS_HEAD_DIM;
 using Rec = Kv4Record<D>;
 constexpr int kWarps = 8;
-constexpr int kStages = 4;  // records in flight per warp
+constexpr int kStages = 4;       // records of a warp's ring
+constexpr int kMaxTiles = 1024;  // (sequence, row tile) pairs of a launch: a CTA keeps their key ranges in shared memory
+constexpr int kMaxParts = 64;    // most CTAs that share a key range
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
@@ -33,7 +35,8 @@ struct Params {
   const int* context;
   const int* table;
   float* part;
-  int table_stride, page_blocks, num_pages, tokens, nq, nkv, group, window, splits, row_tiles;
+  int* tickets;
+  int table_stride, page_blocks, num_pages, tokens, num_seqs, nq, nkv, group, window, row_tiles, first_tile;
   float scale;  // times log2 e
 };
 
@@ -60,7 +63,7 @@ __device__ __forceinline__ const uint8_t* record(const Params& p, int page, int 
 // O^T[channels][rows] += V^T P^T of one record.  Lane (g, t) owns the channels [g D/8, (g+1) D/8) and reads of them the
 // tokens 2t, 2t+1, 2t+8, 2t+9; p[tile][part]: the transposed weights of tokens 0..7 and 8..15.  Tokens outside
 // [first, last) count as zeros, whatever the record holds there.
-template <int kTiles, int kP>
+template <int kTiles, int kP, bool kEdge>
 __device__ __forceinline__ void add_values(const uint8_t* rec, const uint32_t (&p)[kTiles][kP][2], float (&o)[kTiles][D / 16][4], int g, int t,
                                            int first, int last) {
   constexpr int kWords = D / 64;
@@ -81,7 +84,7 @@ __device__ __forceinline__ void add_values(const uint8_t* rec, const uint32_t (&
     }
     if constexpr (kWords == 4) sc[i] = *reinterpret_cast<const uint16_t*>(scales + token * (D / 16));
     else sc[i] = scales[token * (D / 16)];
-    if (token < first || token >= last) sc[i] = 0;
+    if (kEdge && (token < first || token >= last)) sc[i] = 0;
   }
 #pragma unroll
   for (int grp = 0; grp < (kWords + 1) / 2; ++grp) {
@@ -130,7 +133,7 @@ struct Tile {
   __device__ __forceinline__ int query_head(const Params& p, int row) const { return head * p.group + row % p.group; }
 };
 
-// m, l and O of one row tile, over a set of partial ones: factor of partial i is 2^(m_i - M).
+// A finished row: o over its sum l of 2^(s - m), with the sink's share.
 template <typename T>
 __device__ __forceinline__ void write_row(const Params& p, const Tile& tile, int row, int channel, float4 o, float m, float l) {
   const int head = tile.query_head(p, row);
@@ -154,192 +157,307 @@ __device__ __forceinline__ void write_row(const Params& p, const Tile& tile, int
   if (p.lse != nullptr && channel == 0) p.lse[(size_t)tile.token(p, row) * p.nq + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
+// Parts of one row (maximum, sum, four channels) added to one another.
+struct RowSum {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float pm, float pl, float4 v, float top) {
+    const float f = pm == -INFINITY ? 0.f : kv4_exp2(pm - top);  // (a part that saw nothing holds zeros; NaN stays NaN)
+    l += f * pl;
+    o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+  }
+};
+
+// The key ranges of all (sequence, row tile) pairs, counted in records, one behind the other; every key head has them again.
+// A CTA's share is an equal part of all of them, whatever the lengths are, and may begin and end inside a range.
+struct Shares {
+  int before[kMaxTiles + 1];  // records of one head before the pair
+};
+
 template <typename T, int kTiles, int kQ, int kP>
-__global__ void __launch_bounds__(kWarps * 32) attention_kernel(const Params p) {
+__global__ void __launch_bounds__(kWarps * 32, kTiles == 1 && D <= 128 && sizeof(T) == 2 ? 2 : 1) attention_kernel(const Params p) {
   constexpr int kRows = 8 * kTiles;
   extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ Shares shares;
+  __shared__ int scratch[kWarps + 2];
   ts_pdl_prologue();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  Tile tile;
-  tile.open(p, blockIdx.z, blockIdx.y % p.nkv);
-  tile.first_row = blockIdx.y / p.nkv * kRows;
-  if (tile.first_row >= tile.rows) return;
-  const int last_row = min(tile.first_row + kRows, tile.rows) - 1;
-  const int first_pos = tile.position(p, tile.first_row), last_pos = tile.position(p, last_row);
-  const int key0 = p.window > 0 ? max(0, first_pos - p.window + 1) : 0, key1 = max(last_pos + 1, 0);
-  const int blk0 = key0 / KV4_BLOCK, blocks = max(0, (key1 + KV4_BLOCK - 1) / KV4_BLOCK - blk0);
-  const int per = (blocks + p.splits - 1) / p.splits;
-  const int begin = blk0 + min(blocks, per * (int)blockIdx.x), end = blk0 + min(blocks, per * ((int)blockIdx.x + 1));
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
+  const int pairs = p.num_seqs * p.row_tiles;
 
-  uint32_t qf[kTiles][kQ][D / 16][2];
-  int pos[kTiles][2];  // last visible key of the rows 2t, 2t+1 of a tile of 8 (rows that do not exist: none)
+  auto open = [&](Tile& tile, int pair, int head) {
+    tile.open(p, pair / p.row_tiles, head);
+    tile.first_row = (p.first_tile + pair % p.row_tiles) * kRows;
+  };
+  auto first_record = [&](const Tile& tile) { return p.window > 0 ? max(0, tile.position(p, tile.first_row) - p.window + 1) / KV4_BLOCK : 0; };
+  // ---- the shares: a block-wide sum over the pairs, each thread a few neighbours
+  int most = 0;
+  {
+    const int each = (pairs + kWarps * 32 - 1) / (kWarps * 32);
+    int sum = 0;
+    for (int i = tid * each; i < min(pairs, (tid + 1) * each); ++i) {
+      Tile tile;
+      open(tile, i, 0);
+      int n = 0;
+      if (tile.first_row < tile.rows) {
+        const int key1 = tile.position(p, min(tile.first_row + kRows, tile.rows) - 1) + 1;
+        if (key1 > 0) n = (key1 + KV4_BLOCK - 1) / KV4_BLOCK - first_record(tile);
+      }
+      shares.before[i] = sum;  // completed below
+      sum += n;
+      most = max(most, n);
+    }
+    int x = sum;
 #pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
-    const int row = tile.first_row + 8 * n + g;
-    kv4_query_row<D, kQ>(row < tile.rows ? tile.query<T>(p, row) + t * (D / 4) : nullptr, qf[n]);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = tile.first_row + 8 * n + 2 * t + i;
-      pos[n][i] = r < tile.rows ? tile.position(p, r) : -1;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
+    if (lane == 31) scratch[warp] = x;
+    if (tid == 0) scratch[kWarps] = 0;
+    __syncthreads();
+    if (lane == 0) atomicMax(&scratch[kWarps], most);
+    int start = x - sum;
+    for (int w = 0; w < warp; ++w) start += scratch[w];
+    for (int i = tid * each; i < min(pairs, (tid + 1) * each); ++i) shares.before[i] += start;
+    if (tid == kWarps * 32 - 1) shares.before[pairs] = start + sum;
+    __syncthreads();
+    most = scratch[kWarps];
+  }
+  // rows of pairs without any visible key: zeros
+  for (int i = blockIdx.x; i < pairs; i += gridDim.x) {
+    if (shares.before[i + 1] > shares.before[i]) continue;
+    Tile tile;
+    for (int head = 0; head < p.nkv; ++head) {
+      open(tile, i, head);
+      for (int x = tid; x < kRows * (D / 4); x += kWarps * 32) {
+        const int row = tile.first_row + x / (D / 4);
+        if (row < tile.rows) write_row<T>(p, tile, row, x % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
+      }
     }
   }
-
-  float o[kTiles][D / 16][4], m[kTiles][2], l[kTiles][2];
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n) {
-    m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-  }
-
-  uint8_t* ring = smem + warp * (kStages * Rec::kBytes);
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-  const int* table = p.table + (size_t)tile.b * p.table_stride;
-  auto fetch = [&](int blk, int stage) {
-    if (blk < end) {
-      const uint8_t* src = record(p, table[blk / p.page_blocks], blk, tile.head);
-      for (int i = lane * 16; i < Rec::kBytes; i += 512) copy16(ring_at + stage * Rec::kBytes + i, src + i);
+  const int total = shares.before[pairs] * p.nkv;
+  // at least a record for every warp, and no range over more than kMaxParts CTAs
+  const int share = max(max(kWarps, (total + (int)gridDim.x - 1) / (int)gridDim.x), (most + kMaxParts - 1) / kMaxParts);
+  const int begin = (int)min((long long)share * blockIdx.x, (long long)total), end = min(begin + share, total);
+  if (begin >= end) return;
+  auto pair_of = [&](int step) {
+    int lo = 0, hi = pairs - 1;  // the last pair that begins at or before the step (pairs without keys begin with the next one)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (shares.before[mid] * p.nkv <= step) lo = mid;
+      else hi = mid - 1;
     }
-    copy_commit();
+    return lo;
+  };
+
+  // ---- a warp's records: begin + warp, + kWarps, ...; lane i looks up where the i-th of the next 32 lies, one round ahead
+  auto look_up = [&](int step) -> uint32_t {
+    if (step >= end) return 0u;
+    const int pair = pair_of(step), n = shares.before[pair + 1] - shares.before[pair], at = step - shares.before[pair] * p.nkv;
+    const int head = at / n;
+    Tile tile;
+    open(tile, pair, head);
+    const int blk = first_record(tile) + at % n;
+    const int page = p.table[(size_t)(pair / p.row_tiles) * p.table_stride + blk / p.page_blocks];
+    return ((uint32_t)min(max(page, 0), p.num_pages - 1) * p.nkv + head) * p.page_blocks + blk % p.page_blocks;
   };
   const int mine = begin + warp;
+  uint32_t here = look_up(mine + lane * kWarps), ahead = look_up(mine + (32 + lane) * kWarps);
+  uint8_t* ring = smem + warp * (kStages * Rec::kBytes);
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+  int fetched = 0;  // records asked for
+  auto fetch = [&]() {
+    if (mine + fetched * kWarps < end) {
+      const uint8_t* src = p.pool + (size_t)__shfl_sync(0xffffffffu, here, fetched & 31) * Rec::kBytes + lane * 16;
+      const uint32_t dst = ring_at + (fetched % kStages) * Rec::kBytes;
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) fetch(mine + s * kWarps, s);
-  int stage = 0;
-  for (int blk = mine; blk < end; blk += kWarps) {
-    fetch(blk + (kStages - 1) * kWarps, (stage + kStages - 1) % kStages);
-    copy_wait<kStages - 1>();
-    __syncwarp();
-    const uint8_t* rec = ring + stage * Rec::kBytes;
-    float s[kTiles][4];
-    kv4_scores<D, kTiles, kQ>(rec, rec + Rec::kKeyScales, qf, s, g, t);
-    const int key = blk * KV4_BLOCK;
-    bool grows = false;
-    float top[kTiles][2];
+      for (int i = 0; i < Rec::kBytes / 512; ++i) copy16(dst + i * 512, src + i * 512);
+      if (Rec::kBytes % 512 && lane < Rec::kBytes % 512 / 16) copy16(dst + Rec::kBytes / 512 * 512, src + Rec::kBytes / 512 * 512);
+    }
+    copy_commit();
+    if ((++fetched & 31) == 0) {
+      here = ahead;
+      ahead = look_up(mine + (fetched + 32 + lane) * kWarps);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch();
+
+  int done = 0;  // records worked on
+  for (int seg = begin; seg < end;) {
+    const int pair = pair_of(seg), n_pair = shares.before[pair + 1] - shares.before[pair];
+    const int head = (seg - shares.before[pair] * p.nkv) / n_pair, base = shares.before[pair] * p.nkv + head * n_pair;
+    const int seg_end = min(end, base + n_pair);
+    Tile tile;
+    open(tile, pair, head);
+    const int first_pos = tile.position(p, tile.first_row), last_pos = tile.position(p, min(tile.first_row + kRows, tile.rows) - 1);
+    const int key0 = p.window > 0 ? max(0, first_pos - p.window + 1) : 0, blk0 = key0 / KV4_BLOCK;
+    // keys that every row sees: [all0, all1)
+    const int all0 = p.window > 0 ? last_pos - p.window + 1 : 0, all1 = first_pos + 1;
+
+    uint32_t qf[kTiles][kQ][D / 16][2];
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = key + g + 8 * (i >> 1), c = i & 1;
-        s[n][i] *= p.scale;
-        if (at > pos[n][c] || (p.window > 0 && at <= pos[n][c] - p.window)) s[n][i] = -INFINITY;
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        top[n][c] = fmaxf(s[n][c], s[n][c + 2]);
-        grows |= top[n][c] > m[n][c] + 8.f;
-      }
+      const int row = tile.first_row + 8 * n + g;
+      kv4_query_row<D, kQ>(row < tile.rows ? tile.query<T>(p, row) + t * (D / 4) : nullptr, qf[n]);
     }
-    // The maximum moves only when a score passes it by 2^8: until then weights up to 256 are as exact as those up to 1.
-    if (__any_sync(0xffffffffu, grows)) {
+    float o[kTiles][D / 16][4], m[kTiles][2], l[kTiles][2];
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n)
+    for (int n = 0; n < kTiles; ++n) {
+      m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    }
+
+    for (; mine + done * kWarps < seg_end; ++done) {
+      fetch();
+      copy_wait<kStages - 1>();
+      __syncwarp();
+      const uint8_t* rec = ring + (done % kStages) * Rec::kBytes;
+      float s[kTiles][4];
+      kv4_scores<D, kTiles, kQ>(rec, rec + Rec::kKeyScales, qf, s, g, t);
+      const int key = (blk0 + mine + done * kWarps - base) * KV4_BLOCK;
+      const bool edge = key < all0 || key + KV4_BLOCK > all1;
+      bool grows = false;
+      float top[kTiles][2];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] *= p.scale;
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int r = tile.first_row + 8 * n + 2 * t + c, pos = r < tile.rows ? tile.position(p, r) : -1;
+#pragma unroll
+            for (int i = c; i < 4; i += 2) {
+              const int at = key + g + 4 * (i - c);
+              if (at > pos || (p.window > 0 && at <= pos - p.window)) s[n][i] = -INFINITY;
+            }
+          }
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float x = top[n][c];
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          x = fmaxf(x, m[n][c]);
-          const float f = x == -INFINITY ? 1.f : kv4_exp2(m[n][c] - x);
-          m[n][c] = x;
-          l[n][c] *= f;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) o[n][i][c] *= f, o[n][i][c + 2] *= f;
+          top[n][c] = fmaxf(s[n][c], s[n][c + 2]);
+          grows |= top[n][c] > m[n][c] + 8.f;
         }
-    }
-    uint32_t pf[kTiles][kP][2];
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      float w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = kv4_exp2(s[n][i] - (m[n][i & 1] == -INFINITY ? 0.f : m[n][i & 1]));
-        l[n][i & 1] += w[i];
       }
+      // The maximum moves only when a score passes it by 2^8: until then weights up to 256 are as exact as those up to 1.
+      if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t parts[kP];
-        kv4_split<kP>(w[2 * i], w[2 * i + 1], parts);
+        for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-        for (int k = 0; k < kP; ++k) pf[n][k][i] = transpose8x8(parts[k]);
+          for (int c = 0; c < 2; ++c) {
+            float x = top[n][c];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            x = fmaxf(x, m[n][c]);
+            const float f = x == -INFINITY ? 1.f : kv4_exp2(m[n][c] - x);
+            m[n][c] = x;
+            l[n][c] *= f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) o[n][i][c] *= f, o[n][i][c + 2] *= f;
+          }
+      }
+      uint32_t pf[kTiles][kP][2];
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        float w[4];
+        const float off[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = kv4_exp2(s[n][i] - off[i & 1]);
+          l[n][i & 1] += w[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t parts[kP];
+          kv4_split<kP>(w[2 * i], w[2 * i + 1], parts);
+#pragma unroll
+          for (int k = 0; k < kP; ++k) pf[n][k][i] = transpose8x8(parts[k]);
+        }
+      }
+      if (edge) add_values<kTiles, kP, true>(rec, pf, o, g, t, key0 - key, last_pos + 1 - key);
+      else add_values<kTiles, kP, false>(rec, pf, o, g, t, 0, KV4_BLOCK);
+      __syncwarp();
+    }
+
+    // ---- the warps' parts of the segment meet in shared memory (behind the rings, which are being filled)
+    float* so = reinterpret_cast<float*>(smem + kWarps * kStages * Rec::kBytes);  // [warps][rows][D]
+    float* sm = so + kWarps * kRows * D;                                           // [warps][rows]
+    float* sl = sm + kWarps * kRows;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x = l[n][c];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int row = 8 * n + 2 * t + c;
+        if (g == 0) sm[warp * kRows + row] = m[n][c], sl[warp * kRows + row] = x;
+        float2* dst = reinterpret_cast<float2*>(so + (warp * kRows + row) * D + g * (D / 8));
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) dst[i] = make_float2(o[n][i][c], o[n][i][c + 2]);
+      }
+    __syncthreads();
+    const bool whole = seg == base && seg_end == base + n_pair;
+    // (a CTA holds at most two ranges in part: the one it begins with, in its first place, and the one it ends with)
+    float* part = p.part + ((size_t)blockIdx.x * 2 + (seg > begin ? 1 : 0)) * kRows * (D + 4);
+    for (int i = tid; i < kRows * (D / 4); i += kWarps * 32) {
+      const int r = i / (D / 4), channel = i % (D / 4) * 4, row = tile.first_row + r;
+      if (row >= tile.rows) continue;
+      RowSum sum;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) sum.m = fmaxf(sum.m, sm[w * kRows + r]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)
+        sum.add(sm[w * kRows + r], sl[w * kRows + r], *reinterpret_cast<const float4*>(so + (w * kRows + r) * D + channel), sum.m);
+      if (whole) {
+        write_row<T>(p, tile, row, channel, sum.o, sum.m, sum.l);
+      } else {
+        *reinterpret_cast<float4*>(part + r * (D + 4) + 4 + channel) = sum.o;
+        if (channel == 0) *reinterpret_cast<float2*>(part + r * (D + 4)) = make_float2(sum.m, sum.l);
       }
     }
-    add_values<kTiles, kP>(rec, pf, o, g, t, key0 - key, key1 - key);
-    __syncwarp();
-    stage = (stage + 1) % kStages;
+    if (!whole) {
+      // The CTA that comes last adds the range's parts up, in the order of the CTAs, and leaves its ticket at zero again.
+      __threadfence();
+      __syncthreads();
+      const int c0 = base / share, c1 = (base + n_pair - 1) / share;
+      if (tid == 0) {
+        int* ticket = p.tickets + pair * p.nkv + head;
+        const bool last = atomicAdd(ticket, 1) == c1 - c0;
+        if (last) *ticket = 0;
+        scratch[kWarps + 1] = last;
+        __threadfence();
+      }
+      __syncthreads();
+      if (scratch[kWarps + 1]) {
+        for (int i = tid; i < kRows * (D / 4); i += kWarps * 32) {
+          const int r = i / (D / 4), channel = i % (D / 4) * 4, row = tile.first_row + r;
+          if (row >= tile.rows) continue;
+          const float* from = p.part + ((size_t)c0 * 2 * kRows + r) * (D + 4);
+          const int skip = base > c0 * share ? kRows * (D + 4) : 0;  // the first CTA may have begun with another range
+          constexpr int kStep = 2 * kRows * (D + 4);
+          RowSum sum;
+#pragma unroll 4
+          for (int c = 0; c <= c1 - c0; ++c) sum.m = fmaxf(sum.m, __ldcg(from + (size_t)c * kStep + (c == 0 ? skip : 0)));
+#pragma unroll 4
+          for (int c = 0; c <= c1 - c0; ++c) {
+            const float* x = from + (size_t)c * kStep + (c == 0 ? skip : 0);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(x));
+            sum.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(x + 4 + channel)), sum.m);
+          }
+          write_row<T>(p, tile, row, channel, sum.o, sum.m, sum.l);
+        }
+      }
+    }
+    __syncthreads();
+    seg = seg_end;
   }
   copy_wait<0>();
-  __syncthreads();
-
-  // The warps' parts meet in shared memory.
-  float* so = reinterpret_cast<float*>(smem);              // [warps][rows][D]
-  float* sm = so + kWarps * kRows * D;                      // [warps][rows]
-  float* sl = sm + kWarps * kRows;
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float x = l[n][c];
-      x += __shfl_xor_sync(0xffffffffu, x, 4);
-      x += __shfl_xor_sync(0xffffffffu, x, 8);
-      x += __shfl_xor_sync(0xffffffffu, x, 16);
-      const int row = 8 * n + 2 * t + c;
-      if (g == 0) sm[warp * kRows + row] = m[n][c], sl[warp * kRows + row] = x;
-      float2* dst = reinterpret_cast<float2*>(so + (warp * kRows + row) * D + g * (D / 8));
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) dst[i] = make_float2(o[n][i][c], o[n][i][c + 2]);
-    }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kRows * (D / 4); i += kWarps * 32) {
-    const int r = i / (D / 4), channel = i % (D / 4) * 4, row = tile.first_row + r;
-    if (row >= tile.rows) continue;
-    float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * kRows + r]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float mw = sm[w * kRows + r], f = mw == -INFINITY ? 0.f : kv4_exp2(mw - top);
-      if (mw == -INFINITY && sl[w * kRows + r] == 0.f) continue;
-      const float4 v = *reinterpret_cast<const float4*>(so + (w * kRows + r) * D + channel);
-      sum += f * sl[w * kRows + r];
-      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-    }
-    if (p.splits == 1) {
-      write_row<T>(p, tile, row, channel, acc, top, sum);
-    } else {
-      const size_t slot = ((size_t)tile.token(p, row) * p.nq + tile.query_head(p, row)) * p.splits + blockIdx.x;
-      *reinterpret_cast<float4*>(p.part + slot * (D + 4) + 4 + channel) = acc;
-      if (channel == 0) *reinterpret_cast<float2*>(p.part + slot * (D + 4)) = make_float2(top, sum);
-    }
-  }
-}
-
-// The splits of every row, one warp-wide piece of it per thread: the same sums, in the order of the splits.
-template <typename T>
-__global__ void __launch_bounds__(128) merge_kernel(const Params p, int num_seqs, int rows) {
-  ts_pdl_prologue();
-  const int i = blockIdx.x * 128 + threadIdx.x;
-  const int r = i / (D / 4), channel = i % (D / 4) * 4;
-  if (r >= rows) return;
-  const int token = r / p.nq, head = r % p.nq;
-  if (token >= p.cu[num_seqs]) return;
-  const float* part = p.part + (size_t)r * p.splits * (D + 4);
-  float top = -INFINITY, sum = 0.f;
-  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, part[s * (D + 4)]);
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(part + s * (D + 4));
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;
-    const float4 v = *reinterpret_cast<const float4*>(part + s * (D + 4) + 4 + channel);
-    const float f = ml.x == -INFINITY ? 0.f : kv4_exp2(ml.x - top);
-    sum += f * ml.y;
-    acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-  }
-  Tile tile;
-  tile.q_start = token, tile.head = head / p.group;
-  write_row<T>(p, tile, head % p.group, channel, acc, top, sum);
 }
 
 // ---------------------------------------------------------------------------
@@ -561,40 +679,75 @@ int launch_weights(const Params& p, float* sums, int num_seqs, int max_context, 
 }
 
 template <typename T, int kTiles, int kQ, int kP>
-int launch_attention(const Params& p, int num_seqs, int rows, cudaStream_t stream) {
-  constexpr int ring = kWarps * kStages * Rec::kBytes, meet = kWarps * 8 * kTiles * (D + 2) * 4;
-  constexpr int smem = ring > meet ? ring : meet;
-  static bool set = false;
-  if (!set) {
-    cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kTiles, kQ, kP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return (int)e;
-    set = true;
+struct Attention {
+  static constexpr int kSmem = kWarps * kStages * Rec::kBytes + kWarps * 8 * kTiles * (D + 2) * 4;
+  // CTAs that run at once on the device, or a negative error
+  static int ctas() {
+    static int n = 0;
+    if (n == 0) {
+      int device = 0, sms = 0, per_sm = 0;
+      cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kTiles, kQ, kP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+      if (e == cudaSuccess) e = cudaGetDevice(&device);
+      if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+      if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_kernel<T, kTiles, kQ, kP>, kWarps * 32, kSmem);
+      if (e != cudaSuccess) return -(int)e - 100;
+      n = sms * (per_sm > 0 ? per_sm : 1);
+    }
+    return n;
   }
-  int status = ts_launch(attention_kernel<T, kTiles, kQ, kP>, dim3(p.splits, p.nkv * p.row_tiles, num_seqs), dim3(kWarps * 32), smem, stream, p);
-  if (status == 0 && p.splits > 1)
-    status = ts_launch(merge_kernel<T>, dim3((rows * (D / 4) + 127) / 128), dim3(128), 0, stream, p, num_seqs, rows);
-  return status;
-}
+  static int launch(const Params& p, int grid, cudaStream_t stream) {
+    return ts_launch(attention_kernel<T, kTiles, kQ, kP>, dim3(grid), dim3(kWarps * 32), kSmem, stream, p);
+  }
+};
 
 }  // namespace
 
-// q, out [tokens][nq][D] of `dtype`, lse [tokens][nq] or null, sinks [nq] or null; part: tokens * nq * splits * (D + 4) floats where splits > 1.
-TS_EXPORT int ts_attention_kv4(const void* q, int dtype, const void* pool, void* out, float* lse, const float* sinks, const int* cu, const int* context,
-                               const int* table, int table_stride, int page_blocks, int num_pages, int tokens, int num_seqs, int max_q, int nq, int nkv, float scale,
-                               int window, int splits, float* part, void* stream) {
-  if (tokens < 1 || num_seqs < 1) return 0;
-  Params p = {q, (const uint8_t*)pool, out, lse, sinks, cu, context, table, part, table_stride, page_blocks, num_pages, tokens, nq, nkv, nq / nkv, window, splits, 1, scale * kLog2e};
-  const int rows = max_q * p.group;
-  cudaStream_t s = (cudaStream_t)stream;
-  if (num_seqs > 65535) return TS_ERR_UNSUPPORTED_SIZE;
-  const bool wide = rows > 8 && D <= 128 && dtype == TS_DTYPE_BF16;
-  p.row_tiles = (rows + (wide ? 15 : 7)) / (wide ? 16 : 8);
-  if ((long long)p.row_tiles * nkv > 65535) return TS_ERR_UNSUPPORTED_SIZE;
-  if (dtype == TS_DTYPE_F32) return launch_attention<float, 1, 3, 3>(p, num_seqs, tokens * nq, s);
+// How many rows a tile has, by the type and the rows of a sequence and key head.
+static int tile_rows(int dtype, int rows) { return dtype == TS_DTYPE_BF16 && rows > 8 && D <= 128 ? 16 : 8; }
+
+// CTAs of a launch (at most), for the size of `part`: grid * 2 * tile rows * (D + 4) floats; negative: an error.
+static int grid_of(int dtype, int rows) {
+  if (dtype == TS_DTYPE_F32) return Attention<float, 1, 3, 3>::ctas();
 #if TS_HEAD_DIM <= 128
-  if (wide) return launch_attention<__nv_bfloat16, 2, 1, 2>(p, num_seqs, tokens * nq, s);
+  if (tile_rows(dtype, rows) == 16) return Attention<__nv_bfloat16, 2, 1, 2>::ctas();
 #endif
-  return launch_attention<__nv_bfloat16, 1, 1, 2>(p, num_seqs, tokens * nq, s);
+  return Attention<__nv_bfloat16, 1, 1, 2>::ctas();
+}
+TS_EXPORT long long ts_attention_kv4_part_floats(int dtype, int rows) {
+  const int grid = grid_of(dtype, rows);
+  return grid < 0 ? grid : (long long)grid * 2 * tile_rows(dtype, rows) * (D + 4);
+}
+
+// q, out [tokens][nq][D] of `dtype`, lse [tokens][nq] or null, sinks [nq] or null; part: see above; tickets: `num_tickets` zeros (zeros again
+// afterwards).  Batches of more pairs than a launch or the tickets hold take several launches.
+TS_EXPORT int ts_attention_kv4(const void* q, int dtype, const void* pool, void* out, float* lse, const float* sinks, const int* cu, const int* context,
+                               const int* table, int table_stride, int page_blocks, int num_pages, int tokens, int num_seqs, int max_q, int nq, int nkv,
+                               float scale, int window, float* part, int* tickets, int num_tickets, void* stream) {
+  if (tokens < 1 || num_seqs < 1 || max_q < 1) return 0;
+  if (num_tickets < nkv || (long long)max_q * (nq / nkv) > 0x7fffffffLL - 16) return TS_ERR_UNSUPPORTED_SIZE;
+  const int rows = max_q * (nq / nkv), grid = grid_of(dtype, rows), row_tiles = (rows + tile_rows(dtype, rows) - 1) / tile_rows(dtype, rows);
+  if (grid < 1) return -grid - 100;
+  // pairs of a launch: their key ranges, counted in records over all heads, stay below 2^31
+  const long long records = (long long)table_stride * page_blocks * nkv;
+  long long most = kMaxTiles;
+  if (most > num_tickets / nkv) most = num_tickets / nkv;
+  if (most > 0x7fff0000LL / records) most = 0x7fff0000LL / records;
+  if (most < 1) return TS_ERR_UNSUPPORTED_SIZE;
+  const int tiles = (int)(most < row_tiles ? most : row_tiles), seqs = (int)(most / tiles);
+  for (int b = 0; b < num_seqs; b += seqs)
+    for (int tile = 0; tile < row_tiles; tile += tiles) {
+      Params p = {q, (const uint8_t*)pool, out, lse, sinks, cu + b, context + b, table + (size_t)b * table_stride, part, tickets, table_stride, page_blocks,
+                  num_pages, tokens, num_seqs - b < seqs ? num_seqs - b : seqs, nq, nkv, nq / nkv, window,
+                  row_tiles - tile < tiles ? row_tiles - tile : tiles, tile, scale * kLog2e};
+      int status;
+      if (dtype == TS_DTYPE_F32) status = Attention<float, 1, 3, 3>::launch(p, grid, (cudaStream_t)stream);
+#if TS_HEAD_DIM <= 128
+      else if (tile_rows(dtype, rows) == 16) status = Attention<__nv_bfloat16, 2, 1, 2>::launch(p, grid, (cudaStream_t)stream);
+#endif
+      else status = Attention<__nv_bfloat16, 1, 1, 2>::launch(p, grid, (cudaStream_t)stream);
+      if (status) return status;
+    }
+  return 0;
 }
 
 TS_EXPORT int ts_attention_kv4_weights(const void* q, int dtype, const void* pool, float* lse, float* sums, const int* cu, const int* context,
@@ -602,7 +755,8 @@ TS_EXPORT int ts_attention_kv4_weights(const void* q, int dtype, const void* poo
                                        int nkv, float scale, int window, void* stream) {
   if (tokens < 1 || num_seqs < 1 || max_context < 1) return 0;
   if (num_seqs > 65535 || nkv > 65535) return TS_ERR_UNSUPPORTED_SIZE;
-  Params p = {q, (const uint8_t*)pool, nullptr, lse, nullptr, cu, context, table, nullptr, table_stride, page_blocks, num_pages, tokens, nq, nkv, nq / nkv, window, 1, 1, scale * kLog2e};
+  Params p = {q, (const uint8_t*)pool, nullptr, lse, nullptr, cu, context, table, nullptr, nullptr, table_stride, page_blocks, num_pages, tokens, num_seqs, nq, nkv,
+              nq / nkv, window, 1, 0, scale * kLog2e};
   if (dtype == TS_DTYPE_F32) return launch_weights<float, 3>(p, sums, num_seqs, max_context, max_q, (cudaStream_t)stream);
   return launch_weights<__nv_bfloat16, 1>(p, sums, num_seqs, max_context, max_q, (cudaStream_t)stream);
 }

@@ -2598,10 +2598,12 @@ def _attention_kv4_fns(head_dim: int) -> tuple:
     if fns is None:
         lib = _build.load_variant("kv4_attention", {"TS_HEAD_DIM": head_dim})
         run, weights = lib.ts_attention_kv4, lib.ts_attention_kv4_weights
-        run.argtypes = [_c_void_p, _c_int] + [_c_void_p] * 7 + [_c_int] * 8 + [_c_float, _c_int, _c_int, _c_void_p, _c_void_p]
+        run.argtypes = [_c_void_p, _c_int] + [_c_void_p] * 7 + [_c_int] * 8 + [_c_float, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p]
+        part_floats = lib.ts_attention_kv4_part_floats
+        part_floats.argtypes, part_floats.restype = [_c_int, _c_int], _c_ll
         weights.argtypes = [_c_void_p, _c_int] + [_c_void_p] * 6 + [_c_int] * 9 + [_c_float, _c_int, _c_void_p]
         run.restype = weights.restype = _c_int
-        fns = _attention_kv4[head_dim] = (run, weights)
+        fns = _attention_kv4[head_dim] = (run, weights, part_floats)
     return fns
 
 
@@ -2625,12 +2627,6 @@ def _check_attention_kv4(name, q, pool, cu_seqlens_q, context_lens, block_table,
     if num_seqs < 0 or max_seqlen_q < 0 or max_context < 0 or window < 0:
         raise KernelError(f"{name}: negative sizes")
     return pages, blocks, code
-
-
-def attention_kv4_splits(num_seqs: int, num_kv_heads: int, row_tiles: int, max_context: int) -> int:
-    """Over how many CTAs the keys of a (sequence, key head, row tile) are spread."""
-    pairs = max(1, num_seqs * num_kv_heads * row_tiles)
-    return max(1, min(32, 592 // pairs, -(-max_context // 256)))
 
 
 def attention_kv4(
@@ -2677,13 +2673,15 @@ def attention_kv4(
         _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, scale, window,
                                 head_sinks, lse)
         return
-    splits = attention_kv4_splits(num_seqs, nkv, -(-rows // 8), min(max_context, window + max_seqlen_q) if window else max_context)
-    part = torch.empty(T * nq * splits * (d + 4), device=q.device, dtype=torch.float32) if splits > 1 else None
-    run, _ = _attention_kv4_fns(d)
+    run, _, part_floats = _attention_kv4_fns(d)
+    need = part_floats(code, rows)
+    if need < 0:
+        _check("attention_kv4", -need - 100)
+    part = torch.empty(need, device=q.device, dtype=torch.float32)
     _check("attention_kv4", run(
         q.data_ptr(), code, pool.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(head_sinks), cu_seqlens_q.data_ptr(), context_lens.data_ptr(),
-        block_table.data_ptr(), block_table.shape[1], blocks, pages, T, num_seqs, max_seqlen_q, nq, nkv, float(scale), int(window), splits, _ptr(part),
-        _stream()))
+        block_table.data_ptr(), block_table.shape[1], blocks, pages, T, num_seqs, max_seqlen_q, nq, nkv, float(scale), int(window), part.data_ptr(),
+        _attention_counters(q.device).data_ptr(), _GEMM_MAX_TILES, _stream()))
 
 
 _KV4_EXPAND_PAGE = 128
@@ -2752,7 +2750,7 @@ def attention_kv4_weights(
     if lse.numel() != q.shape[0] * nq:
         raise KernelError(f"attention_kv4_weights: lse must have {q.shape[0] * nq} entries, got {lse.numel()}")
     _kv4_sums("attention_kv4_weights", sums, pool)
-    _, run = _attention_kv4_fns(d)
+    _, run, _ = _attention_kv4_fns(d)
     _check("attention_kv4_weights", run(
         q.data_ptr(), code, pool.data_ptr(), lse.data_ptr(), sums.data_ptr(), cu_seqlens_q.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(),
         block_table.shape[1], blocks, pages, q.shape[0], num_seqs, max_seqlen_q, max_context, nq, nkv, float(scale), int(window), _stream()))

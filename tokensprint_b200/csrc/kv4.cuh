@@ -109,11 +109,11 @@ __device__ __forceinline__ void kv4_query_row(const float* p, uint32_t (&frag)[k
   }
 }
 
-// Keys 16 x D of a record times query rows: S[token][row] of a tile of 8 rows; `codes` and `scales` point at
-// the record's key codes and scales (shared memory).  Lane (g, t) reads rows g and g + 8, a quarter of their channels.
-template <int D, int kTiles, int kParts>
-__device__ __forceinline__ void kv4_scores(const uint8_t* codes, const uint8_t* scales, const uint32_t (&q)[kTiles][kParts][D / 16][2],
-                                           float (&s)[kTiles][4], int g, int t) {
+// Keys 16 x D of a record times query rows: S[token][row] of tiles of 8 rows; `codes` and `scales` point at the record's
+// key codes and scales.  Lane (g, t) reads rows g and g + 8, a quarter of their channels.  `q(tile, part, word)` gives the lane's
+// four registers of a query tile for the word's two k-steps.
+template <int D, int kTiles, int kParts, typename Query>
+__device__ __forceinline__ void kv4_scores(const uint8_t* codes, const uint8_t* scales, Query q, float (&s)[kTiles][4], int g, int t) {
   constexpr int kWords = D / 32;  // of 8 codes, per lane and row
   uint32_t w[2][kWords], sc[2];
 #pragma unroll
@@ -153,8 +153,9 @@ __device__ __forceinline__ void kv4_scores(const uint8_t* codes, const uint8_t* 
       for (int n = 0; n < kTiles; ++n)
 #pragma unroll
         for (int part = 0; part < kParts; ++part) {
-          kv4_mma(s[n], a00, a01, a02, a03, q[n][part][2 * k][0], q[n][part][2 * k][1]);
-          kv4_mma(s[n], a10, a11, a12, a13, q[n][part][2 * k + 1][0], q[n][part][2 * k + 1][1]);
+          const uint4 b = q(n, part, k);
+          kv4_mma(s[n], a00, a01, a02, a03, b.x, b.y);
+          kv4_mma(s[n], a10, a11, a12, a13, b.z, b.w);
         }
     }
   }

@@ -38,91 +38,119 @@ __device__ __forceinline__ void read_group<__nv_bfloat16>(const __nv_bfloat16* p
   }
 }
 
-// Where the codes and the scales of group `grp` of a row lie.
-struct Place {
-  size_t codes, scales;
-};
-__device__ __forceinline__ Place place_of(int slot, int head, int grp, bool values, int nkv, int page_blocks, int d) {
-  const int page_size = page_blocks * KV4_BLOCK, page = slot / page_size, row = slot % page_size;
-  const size_t rec = (((size_t)page * nkv + head) * page_blocks + row / KV4_BLOCK) * (18 * d) + (values ? 9 * d : 0);
-  return {rec + row % KV4_BLOCK * (d / 2) + grp * 8, rec + 8 * d + row % KV4_BLOCK * (d / 16) + grp};
-}
-
-// A thread takes the 16 channels of one group: their largest, the scale, the codes, 8 + 1 bytes out.
+// A thread takes the 16 channels of one group: their largest, the scale, the codes, 8 + 1 bytes out.  `width` threads (32 or 128) go over the
+// groups of a token, keys first: 32 keep their loads apart from one another's and need few threads, 128 wait once when there are few tokens.
 template <typename T>
 __global__ void __launch_bounds__(128) store_kernel(const T* k, const T* v, long long k_stride, long long v_stride, uint8_t* pool, float* sums,
-                                                    const int* slots, int tokens, int nkv, int d, int page_blocks, int num_slots) {
+                                                    const int* slots, int tokens, int nkv, int log_groups, int page_blocks, int num_slots, int width) {
   ts_pdl_prologue();
-  const int groups = d / 16, per_token = 2 * nkv * groups;
-  const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
-  const int token = (int)(i / per_token), rest = (int)(i % per_token);
+  const int groups = 1 << log_groups, d = 16 * groups, units = nkv << log_groups;
+  const int token = blockIdx.x * (128 / width) + threadIdx.x / width;
   if (token >= tokens) return;
   const int slot = slots[token];
   if (slot < 0 || slot >= num_slots) return;
-  const bool values = rest >= nkv * groups;
-  const int unit = rest % (nkv * groups), head = unit / groups, grp = unit % groups;
-  float x[16];
-  read_group<T>((values ? v + token * v_stride : k + token * k_stride) + unit * 16, x);
-  float amax = 0.f;
+  const int page_size = page_blocks * KV4_BLOCK, page = slot / page_size, in_page = slot % page_size, row = in_page % KV4_BLOCK;
+  uint8_t* records = pool + ((size_t)page * nkv * page_blocks + in_page / KV4_BLOCK) * (18 * d);  // head 0's
+  const T *from_k = k + token * k_stride, *from_v = v + token * v_stride;
+  constexpr int kAhead = 4;
+  for (int first = threadIdx.x % width; first < 2 * units; first += kAhead * width) {
+    float x[kAhead][16];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    if (x[j] != x[j]) x[j] = 0.f;
-    amax = fmaxf(amax, fabsf(x[j]));
-  }
-  const uint32_t byte = scale_byte(amax);
-  const float s = byte ? scale_of(byte) : 1.f;  // (a scale of zero: the whole group rounds to zero)
-  uint32_t w[2] = {0u, 0u};
+    for (int a = 0; a < kAhead; ++a) {
+      const int i = first + a * width;
+      if (i < 2 * units) read_group<T>(i < units ? from_k + i * 16 : from_v + (i - units) * 16, x[a]);
+    }
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const int code = byte ? __float2int_rn(fminf(fmaxf(x[j] / s, -7.f), 7.f)) + 8 : 8;
-    w[j / 8] |= (uint32_t)code << (4 * (j % 8));
-  }
-  const Place at = place_of(slot, head, grp, values, nkv, page_blocks, d);
-  *reinterpret_cast<uint2*>(pool + at.codes) = make_uint2(w[0], w[1]);
-  pool[at.scales] = (uint8_t)byte;
-  if (sums != nullptr && !values && grp == 0) {  // a row that comes in has gathered no weight
-    const int page_size = page_blocks * KV4_BLOCK;
-    sums[((size_t)(slot / page_size) * nkv + head) * page_size + slot % page_size] = 0.f;
+    for (int a = 0; a < kAhead; ++a) {
+      const int i = first + a * width;
+      if (i >= 2 * units) break;
+      const int unit = i < units ? i : i - units, head = unit >> log_groups, grp = unit & (groups - 1);
+      float amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (x[a][j] != x[a][j]) x[a][j] = 0.f;
+        amax = fmaxf(amax, fabsf(x[a][j]));
+      }
+      // The code is round(x / s), found without 16 divisions: c is the rounded product with 1/s, which is off by one at most and only where
+      // x / s lies next to a half; r = x - c s is exact enough to tell (one rounding), and a tie goes to the even code.
+      const uint32_t byte = scale_byte(amax);
+      const float s = byte ? scale_of(byte) : 1.f, inv = 1.f / s, half = 0.5f * s;  // (a scale of zero: the whole group rounds to zero)
+      uint32_t w[2] = {0u, 0u};
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        float c = rintf(fminf(fmaxf(x[a][j] * inv, -7.f), 7.f));
+        const float r = fmaf(-c, s, x[a][j]);
+        const bool odd = ((int)c & 1) != 0;
+        if (fabsf(r) > half || (odd && fabsf(r) == half)) c += copysignf(1.f, r);
+        const int code = byte ? (int)fminf(fmaxf(c, -7.f), 7.f) + 8 : 8;
+        w[j / 8] |= (uint32_t)code << (4 * (j % 8));
+      }
+      uint8_t* rec = records + (size_t)head * page_blocks * (18 * d) + (i < units ? 0 : 9 * d);
+      *reinterpret_cast<uint2*>(rec + row * (d / 2) + grp * 8) = make_uint2(w[0], w[1]);
+      rec[8 * d + row * groups + grp] = (uint8_t)byte;
+      if (sums != nullptr && i < units && grp == 0) sums[((size_t)page * nkv + head) * page_size + in_page] = 0.f;  // it has gathered no weight
+    }
   }
 }
 
-__device__ __forceinline__ void write_group(float* p, const float (&x)[16]) {
+// 16 codes and their scale as 16 bfloat16 in order.
+__device__ __forceinline__ void kv4_unpack(uint2 code, uint32_t scale, uint4 (&out)[2]) {
+  __nv_bfloat162 f, c;
+  kv4_factors(scale, scale, f, c);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-}
-__device__ __forceinline__ void write_group(__nv_bfloat16* p, const float (&x)[16]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    __nv_bfloat162 v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = __floats2bfloat162_rn(x[8 * i + 2 * j], x[8 * i + 2 * j + 1]);
-    reinterpret_cast<uint4*>(p)[i] = *reinterpret_cast<const uint4*>(v);
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t x = j ? code.y : code.x;
+    const uint32_t p0 = kv4_pair(x << 3, f, c), p1 = kv4_pair(x >> 1, f, c), p2 = kv4_pair(x >> 5, f, c), p3 = kv4_pair(x >> 9, f, c);
+    out[j] = make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(128) load_kernel(const uint8_t* pool, const int* slots, T* k, T* v, int rows, int nkv, int d, int page_blocks,
-                                                   int num_slots) {
+__global__ void __launch_bounds__(128) load_kernel(const uint8_t* pool, const int* slots, T* k, T* v, int rows, int nkv, int log_groups, int page_blocks,
+                                                   int num_slots, int width) {
   ts_pdl_prologue();
-  const int groups = d / 16, per_row = 2 * nkv * groups;
-  const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
-  const int row = (int)(i / per_row), rest = (int)(i % per_row);
+  const int groups = 1 << log_groups, d = 16 * groups, units = nkv << log_groups;
+  const int row = blockIdx.x * (128 / width) + threadIdx.x / width;
   if (row >= rows) return;
-  const bool values = rest >= nkv * groups;
-  const int unit = rest % (nkv * groups);
   const int slot = slots[row];
-  float x[16];
-  if (slot < 0 || slot >= num_slots) {
+  const bool there = slot >= 0 && slot < num_slots;
+  const int page_size = page_blocks * KV4_BLOCK, page = there ? slot / page_size : 0, in_page = there ? slot % page_size : 0, at = in_page % KV4_BLOCK;
+  const uint8_t* records = pool + ((size_t)page * nkv * page_blocks + in_page / KV4_BLOCK) * (18 * d);
+  T *to_k = k + (size_t)row * units * 16, *to_v = v + (size_t)row * units * 16;
+  constexpr int kAhead = 4;
+  for (int first = threadIdx.x % width; first < 2 * units; first += kAhead * width) {
+    uint2 code[kAhead];
+    uint32_t scale[kAhead];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = 0.f;
-  } else {
-    const Place at = place_of(slot, unit / groups, unit % groups, values, nkv, page_blocks, d);
-    const uint2 c = *reinterpret_cast<const uint2*>(pool + at.codes);
-    const float s = scale_of(pool[at.scales]);
+    for (int a = 0; a < kAhead; ++a) {
+      const int i = first + a * width, unit = i < units ? i : i - units, grp = unit & (groups - 1);
+      code[a] = make_uint2(0u, 0u), scale[a] = 0u;
+      if (there && i < 2 * units) {
+        const uint8_t* rec = records + (size_t)(unit >> log_groups) * page_blocks * (18 * d) + (i < units ? 0 : 9 * d);
+        code[a] = *reinterpret_cast<const uint2*>(rec + at * (d / 2) + grp * 8);
+        scale[a] = rec[8 * d + at * groups + grp];
+      }
+    }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = (float)((int)(((j < 8 ? c.x : c.y) >> (4 * (j % 8))) & 15u) - 8) * s;
+    for (int a = 0; a < kAhead; ++a) {
+      const int i = first + a * width;
+      if (i >= 2 * units) break;
+      T* dst = i < units ? to_k + i * 16 : to_v + (i - units) * 16;
+      if constexpr (sizeof(T) == 2) {
+        uint4 out[2];
+        kv4_unpack(code[a], scale[a], out);
+        reinterpret_cast<uint4*>(dst)[0] = out[0], reinterpret_cast<uint4*>(dst)[1] = out[1];
+      } else {
+        const float s = scale_of(scale[a]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t c = (j < 2 ? code[a].x : code[a].y) >> (16 * (j & 1));
+          reinterpret_cast<float4*>(dst)[j] = make_float4((float)((int)(c & 15u) - 8) * s, (float)((int)(c >> 4 & 15u) - 8) * s,
+                                                          (float)((int)(c >> 8 & 15u) - 8) * s, (float)((int)(c >> 12 & 15u) - 8) * s);
+        }
+      }
+    }
   }
-  write_group((values ? v : k) + ((size_t)row * nkv * groups + unit) * 16, x);
 }
 
 // The rows that a batch's queries can see, of heads of 128, as bfloat16 pages of 128 rows for the prompt attention, and the block table of those
@@ -156,15 +184,8 @@ __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* pool, const 
   for (int i = 0; i < kUnits; ++i) {
     const int unit = threadIdx.x + 256 * i, grp = unit % kGroups, values = unit / (kExpandRows * kGroups);
     const int row = first + unit / kGroups % kExpandRows;
-    __nv_bfloat162 f, c;
-    kv4_factors(scale[i], scale[i], f, c);
     uint4 out[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint32_t x = j ? code[i].y : code[i].x;
-      const uint32_t p0 = kv4_pair(x << 3, f, c), p1 = kv4_pair(x >> 1, f, c), p2 = kv4_pair(x >> 5, f, c), p3 = kv4_pair(x >> 9, f, c);
-      out[j] = make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
-    }
+    kv4_unpack(code[i], scale[i], out);
     uint4* dst = (values ? v : k) + (((size_t)b * blocks * kExpandPage + row) * nkv + head) * (kExpandDim / 8) + grp * 2;
     if (row < n) dst[0] = out[0], dst[1] = out[1];
   }
@@ -173,7 +194,10 @@ __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* pool, const 
 // ---------------------------------------------------------------------------
 // eviction
 
-constexpr int kEvictThreads = 256;
+constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
+constexpr int kDigits = 2048;          // bins of a pass of the radix select: 11, 11 and 10 bits
+constexpr int kKeptKeys = 16384;       // most weights kept in shared memory; of longer requests they are read again for every pass
+constexpr int kMoveRows = 256;         // rows that a CTA moves at a time
 
 // A weight as an unsigned number of the same order; NaN is the largest, both zeros are one.
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -182,7 +206,7 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sums of both halves of `v` over the threads before this one; `total`: over all of them.
+// The sum of `v` over the threads before this one; `total`: over all of them.
 __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* scratch, uint32_t& total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   uint32_t x = v;
@@ -195,7 +219,7 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* scratch, 
   __syncthreads();
   uint32_t before = 0, all = 0;
 #pragma unroll
-  for (int i = 0; i < kEvictThreads / 32; ++i) {
+  for (int i = 0; i < kEvictWarps; ++i) {
     const uint32_t s = scratch[i];
     if (i < warp) before += s;
     all += s;
@@ -205,133 +229,198 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* scratch, 
   return before + x - v;
 }
 
-// One CTA per request and head.  The weights between the first and the recent rows are ranked by a radix select
-// (four passes over 8 bits each, from the top); then the rows are gone through in order, 256 at a time, and the kept
-// ones move forward.  A row never moves backwards, and what a chunk writes lies before everything that later chunks
-// read, so one barrier between a chunk's reads and its writes makes the move safe in place.
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// A cluster of CTAs per request and head.  Every CTA ranks the weights between the first and the recent rows by a radix
+// select (they are few bytes; ranking them once and telling the others would cost more than reading them again), finds for every
+// kept row its new place and writes down the sources of the places it will fill.  Then the kept rows move forward in
+// rounds, kMoveRows places per CTA: all reads of a round, a barrier of the cluster, its writes.  That is safe in place: a row
+// never moves backwards and the order is kept, so what a round writes lies before everything that later rounds read.
+template <int D>
 __global__ void __launch_bounds__(kEvictThreads) evict_kernel(uint8_t* pool, float* sums, const int* table, int table_stride, const int* context,
-                                                              int* new_lens, int nkv, int d, int page_blocks, int num_pages, int budget, int recent,
-                                                              int first) {
-  __shared__ uint32_t hist[256], scratch[kEvictThreads / 32], chosen[2], list[kEvictThreads];
+                                                              int* new_lens, int* order, int nkv, int page_blocks, int num_pages, int budget, int recent,
+                                                              int first, int cluster, int room) {
+  extern __shared__ uint32_t kept_keys[];
+  __shared__ uint32_t hist[kDigits], scratch[kEvictWarps], chosen[2];
   ts_pdl_prologue();
-  const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int rank = blockIdx.x % cluster, head = blockIdx.x / cluster, b = blockIdx.y, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int page_size = page_blocks * KV4_BLOCK;
   const int n = min(context[b], table_stride * page_size);
-  if (head == 0 && tid == 0) new_lens[b] = min(n, budget);
+  if (blockIdx.x == 0 && tid == 0) new_lens[b] = min(n, budget);
   if (n <= budget) return;
   table += (size_t)b * table_stride;
+  order += ((size_t)b * nkv + head) * budget;
   auto page_of = [&](int row) { return min(max(table[row / page_size], 0), num_pages - 1); };
-  auto weight_at = [&](int row) -> float& { return sums[((size_t)page_of(row) * nkv + head) * page_size + row % page_size]; };
+  auto weight_of = [&](int page, int in_page) -> float& { return sums[((size_t)page * nkv + head) * page_size + in_page]; };
 
-  uint32_t threshold = 0, ties = 0;
-  {
-    uint32_t left = budget - first - recent;  // of the rows [first, n - recent), which are more than that
-    if (left == 0) {
-      threshold = 0xffffffffu;  // nothing passes it, and no tie is taken
-    } else {
-      for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kEvictThreads) hist[i] = 0;
-        __syncthreads();
-        for (int i = first + tid; i < n - recent; i += kEvictThreads) {
-          const uint32_t u = order_of(weight_at(i));
-          if (shift == 24 || (u >> (shift + 8)) == (threshold >> (shift + 8))) atomicAdd(&hist[(u >> shift) & 255u], 1u);
-        }
-        __syncthreads();
-        // the bin in which the count from the top reaches what is left: thread i stands for bin 255 - i
-        uint32_t total;
-        const uint32_t mine = hist[255 - tid];
-        const uint32_t above = block_prefix(mine, scratch, total);
-        if (above < left && above + mine >= left) chosen[0] = 255 - tid, chosen[1] = left - above;
-        __syncthreads();
-        threshold |= chosen[0] << shift;
-        left = chosen[1];
-        __syncthreads();
-      }
-      ties = left;
-    }
-  }
-
-  const int row_words = 9 * d / 32;  // of 4 bytes: key codes, key scales, value codes, value scales
-  const int code_words = d / 8, scale_words = d / 64;
-  auto word_at = [&](int row, int w) {
-    uint8_t* rec = pool + (((size_t)page_of(row) * nkv + head) * page_blocks + row % page_size / KV4_BLOCK) * (18 * d);
-    const int r = row % KV4_BLOCK, half = code_words + scale_words;
-    if (w >= half) w -= half, rec += 9 * d;
-    return reinterpret_cast<uint32_t*>(w < code_words ? rec + r * (d / 2) + 4 * w : rec + 8 * d + r * (d / 16) + 4 * (w - code_words));
-  };
-  int out = 0;
-  for (int base = 0; base < n; base += kEvictThreads) {
-    const int row = base + tid;
-    float w = 0.f;
-    uint32_t flag = 0;  // low half: kept for certain, high half: of the threshold's own weight
-    if (row < n) {
-      w = weight_at(row);
-      const uint32_t u = order_of(w);
-      if (row < first || row >= n - recent) flag = 1u;
-      else if (budget > first + recent) flag = u > threshold ? 1u : u == threshold ? 0x10000u : 0u;
-    }
-    uint32_t total;
-    const uint32_t before = block_prefix(flag, scratch, total);
-    const uint32_t ties_before = min(before >> 16, ties);
-    const bool keep = (flag & 1u) || (flag && (before >> 16) < ties);
-    const int place = (int)((before & 0xffffu) + ties_before);
-    const int count = (int)((total & 0xffffu) + min(total >> 16, ties));
-    if (keep) {
-      list[place] = row;
-      weight_at(out + place) = w;
-    }
-    ties -= min(total >> 16, ties);
+  const bool in_smem = n <= room;
+  if (in_smem) {
+    for (int i = tid; i < n; i += kEvictThreads) kept_keys[i] = order_of(weight_of(page_of(i), i % page_size));
     __syncthreads();
-    constexpr int kHold = 12;
-    for (int at = 0; at < count * row_words; at += kEvictThreads * kHold) {
-      uint32_t hold[kHold];
-#pragma unroll
-      for (int i = 0; i < kHold; ++i) {
-        const int x = at + i * kEvictThreads + tid;
-        if (x < count * row_words) hold[i] = *word_at(list[x / row_words], x % row_words);
+  }
+  auto key_of = [&](int i) { return in_smem ? kept_keys[i] : order_of(weight_of(page_of(i), i % page_size)); };
+
+  uint32_t threshold = 0xffffffffu, ties = 0;  // kept: what is above the threshold, and `ties` of what equals it
+  const bool ranked = budget > first + recent;
+  if (ranked) {
+    uint32_t left = budget - first - recent;  // of the rows [first, n - recent), which are more than that
+    threshold = 0;
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      for (int i = tid; i < kDigits; i += kEvictThreads) hist[i] = 0;
+      __syncthreads();
+      for (int i = first + tid; i < n - recent; i += kEvictThreads) {
+        const uint32_t u = key_of(i);
+        if (pass == 0 || ((u ^ threshold) >> (shift + bits)) == 0) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1u)], 1u);
       }
       __syncthreads();
+      // the bin in which the count from the top reaches what is left: thread i stands for four bins from 2047 - 4 i down
+      constexpr int kBins = kDigits / kEvictThreads;
+      uint32_t count[kBins], mine = 0, total;
 #pragma unroll
-      for (int i = 0; i < kHold; ++i) {
-        const int x = at + i * kEvictThreads + tid;
-        if (x < count * row_words) *word_at(out + x / row_words, x % row_words) = hold[i];
+      for (int j = 0; j < kBins; ++j) mine += count[j] = hist[kDigits - 1 - (tid * kBins + j)];
+      uint32_t above = block_prefix(mine, scratch, total);
+      if (above < left && above + mine >= left) {
+#pragma unroll
+        for (int j = 0; j < kBins; ++j) {
+          if (above < left && above + count[j] >= left) chosen[0] = kDigits - 1 - (tid * kBins + j), chosen[1] = left - above;
+          above += count[j];
+        }
+      }
+      __syncthreads();
+      threshold |= chosen[0] << shift;
+      left = chosen[1];
+    }
+    ties = left;
+  }
+
+  // ---- places: a warp goes over a run of rows, 32 at a time, counting first and then numbering
+  auto state_of = [&](int i) -> int {  // 1: kept, 2: of the threshold's own weight
+    if (i >= n) return 0;
+    if (i < first || i >= n - recent) return 1;
+    if (!ranked) return 0;
+    const uint32_t u = key_of(i);
+    return u > threshold ? 1 : u == threshold ? 2 : 0;
+  };
+  const int run = (n + kEvictThreads - 1) / kEvictThreads * 32, row0 = warp * run;
+  int sure = 0, equal = 0;
+  for (int i = row0; i < row0 + run; i += 32) {
+    const int st = state_of(i + lane);
+    sure += __popc(__ballot_sync(0xffffffffu, st == 1)), equal += __popc(__ballot_sync(0xffffffffu, st == 2));
+  }
+  __syncthreads();
+  if (lane == 0) hist[warp] = sure, hist[kEvictWarps + warp] = equal;
+  __syncthreads();
+  int sure_before = 0, equal_before = 0;
+  for (int i = 0; i < warp; ++i) sure_before += hist[i], equal_before += hist[kEvictWarps + i];
+  for (int i = row0; i < row0 + run; i += 32) {
+    const int row = i + lane, st = state_of(row);
+    const uint32_t sures = __ballot_sync(0xffffffffu, st == 1), equals = __ballot_sync(0xffffffffu, st == 2), lower = (1u << lane) - 1u;
+    const int e = equal_before + __popc(equals & lower);
+    const int place = sure_before + __popc(sures & lower) + min(e, (int)ties);
+    if ((st == 1 || (st == 2 && e < (int)ties)) && place / kMoveRows % cluster == rank) order[place] = page_of(row) * page_size + row % page_size;
+    sure_before += __popc(sures), equal_before += __popc(equals);
+  }
+  __syncthreads();
+
+  // ---- the move: pieces of 16 bytes of codes, pieces of kScale bytes of scales, and the weights
+  constexpr int kPieces = D / 16, kCode = kMoveRows * kPieces / kEvictThreads, kScale = D / 16;
+  auto record_at = [&](int page, int in_page) { return pool + (((size_t)page * nkv + head) * page_blocks + in_page / KV4_BLOCK) * (18 * D); };
+  for (int base = 0; base < budget; base += kMoveRows * cluster) {
+    const int place0 = base + rank * kMoveRows, count = min(max(budget - place0, 0), kMoveRows);
+    uint4 code[kCode];
+    uint32_t scale[kScale / 4];
+    float w = 0.f;
+    auto code_at = [&](int page, int in_page, int piece) {
+      const int values = piece / (kPieces / 2), c = piece % (kPieces / 2);
+      return reinterpret_cast<uint4*>(record_at(page, in_page) + values * 9 * D + in_page % KV4_BLOCK * (D / 2) + c * 16);
+    };
+    auto scale_at = [&](int page, int in_page) {
+      return reinterpret_cast<uint32_t*>(record_at(page, in_page) + (tid / kMoveRows) * 9 * D + 8 * D + in_page % KV4_BLOCK * kScale);
+    };
+#pragma unroll
+    for (int i = 0; i < kCode; ++i) {
+      const int x = tid + i * kEvictThreads, r = x / kPieces;
+      if (r < count) {
+        const int slot = order[place0 + r];
+        code[i] = *code_at(slot / page_size, slot % page_size, x % kPieces);
       }
     }
-    out += count;
-    __syncthreads();
+    static_assert(kEvictThreads == 2 * kMoveRows, "a thread for the scales of a row's keys, one for its values'");
+    if (tid % kMoveRows < count) {
+      const int slot = order[place0 + tid % kMoveRows], page = slot / page_size, in_page = slot % page_size;
+#pragma unroll
+      for (int i = 0; i < kScale / 4; ++i) scale[i] = scale_at(page, in_page)[i];
+      if (tid < kMoveRows) w = weight_of(page, in_page);
+    }
+    cluster_meet();
+#pragma unroll
+    for (int i = 0; i < kCode; ++i) {
+      const int x = tid + i * kEvictThreads, r = x / kPieces, place = place0 + r;
+      if (r < count) *code_at(page_of(place), place % page_size, x % kPieces) = code[i];
+    }
+    if (tid % kMoveRows < count) {
+      const int place = place0 + tid % kMoveRows, page = page_of(place);
+#pragma unroll
+      for (int i = 0; i < kScale / 4; ++i) scale_at(page, place % page_size)[i] = scale[i];
+      if (tid < kMoveRows) weight_of(page, place % page_size) = w;
+    }
   }
-  for (int row = out + tid; row < n; row += kEvictThreads) weight_at(row) = 0.f;
+  // (every CTA of the cluster has read all it reads)
+  for (int row = budget + rank * kEvictThreads + tid; row < n; row += kEvictThreads * cluster) weight_of(page_of(row), row % page_size) = 0.f;
+}
+
+template <int D>
+int launch_evict(uint8_t* pool, float* sums, const int* table, int table_stride, const int* context, int* new_lens, int* order, int num_seqs, int nkv,
+                 int page_blocks, int num_pages, int max_context, int budget, int recent, int first, cudaStream_t stream) {
+  static bool set = false;
+  if (!set) {
+    cudaError_t e = cudaFuncSetAttribute(evict_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeptKeys * 4);
+    if (e != cudaSuccess) return (int)e;
+    set = true;
+  }
+  // CTAs per request and head: as many as rounds of one CTA would be, up to 8, while that fills no more than the device takes at once
+  int cluster = 1;
+  while (cluster < 8 && cluster * kMoveRows < budget && (long long)num_seqs * nkv * cluster < 2 * 148) cluster *= 2;
+  const int room = max_context < kKeptKeys ? max_context : kKeptKeys;  // weights that fit the shared memory
+  return ts_launch_cluster(evict_kernel<D>, dim3(nkv * cluster, num_seqs), dim3(kEvictThreads), (size_t)room * 4, stream, cluster, pool, sums, table, table_stride,
+                           context, new_lens, order, nkv, page_blocks, num_pages, budget, recent, first, cluster, room);
 }
 
 }  // namespace
+
+// Threads per token of the row kernels: with few tokens all groups of a token at once (measured at 8 tokens of 8 heads of 128: see the kernels'
+// table in the design notes), with many a warp per token with four groups in flight.
+static int threads_per_token(int tokens) { return tokens < 1024 ? 128 : 32; }
 
 // k, v: rows [tokens] of nkv * d entries, `stride` entries apart; slots [tokens], -1: not stored; sums: null or the pool's weights.
 TS_EXPORT int ts_kv4_store(const void* k, const void* v, int dtype, long long k_stride, long long v_stride, void* pool, float* sums, const int* slots,
                            int tokens, int nkv, int d, int page_blocks, int num_pages, void* stream) {
   if (tokens < 1) return 0;
-  const long long threads = (long long)tokens * 2 * nkv * (d / 16);
-  const dim3 grid((unsigned)((threads + 127) / 128));
-  const int num_slots = num_pages * page_blocks * KV4_BLOCK;
+  const int width = threads_per_token(tokens), log_groups = d == 64 ? 2 : d == 128 ? 3 : 4, num_slots = num_pages * page_blocks * KV4_BLOCK;
+  const dim3 grid((unsigned)((tokens + 128 / width - 1) / (128 / width)));
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == TS_DTYPE_F32)
     return ts_launch(store_kernel<float>, grid, dim3(128), 0, s, (const float*)k, (const float*)v, k_stride, v_stride, (uint8_t*)pool, sums, slots, tokens,
-                     nkv, d, page_blocks, num_slots);
+                     nkv, log_groups, page_blocks, num_slots, width);
   return ts_launch(store_kernel<__nv_bfloat16>, grid, dim3(128), 0, s, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, k_stride, v_stride, (uint8_t*)pool,
-                   sums, slots, tokens, nkv, d, page_blocks, num_slots);
+                   sums, slots, tokens, nkv, log_groups, page_blocks, num_slots, width);
 }
 
 // k, v [rows][nkv][d]; a slot outside the pool gives zeros.
 TS_EXPORT int ts_kv4_load(const void* pool, const int* slots, void* k, void* v, int dtype, int rows, int nkv, int d, int page_blocks, int num_pages,
                           void* stream) {
   if (rows < 1) return 0;
-  const long long threads = (long long)rows * 2 * nkv * (d / 16);
-  const dim3 grid((unsigned)((threads + 127) / 128));
-  const int num_slots = num_pages * page_blocks * KV4_BLOCK;
+  const int width = threads_per_token(rows), log_groups = d == 64 ? 2 : d == 128 ? 3 : 4, num_slots = num_pages * page_blocks * KV4_BLOCK;
+  const dim3 grid((unsigned)((rows + 128 / width - 1) / (128 / width)));
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == TS_DTYPE_F32)
-    return ts_launch(load_kernel<float>, grid, dim3(128), 0, s, (const uint8_t*)pool, slots, (float*)k, (float*)v, rows, nkv, d, page_blocks, num_slots);
-  return ts_launch(load_kernel<__nv_bfloat16>, grid, dim3(128), 0, s, (const uint8_t*)pool, slots, (__nv_bfloat16*)k, (__nv_bfloat16*)v, rows, nkv, d,
-                   page_blocks, num_slots);
+    return ts_launch(load_kernel<float>, grid, dim3(128), 0, s, (const uint8_t*)pool, slots, (float*)k, (float*)v, rows, nkv, log_groups, page_blocks,
+                     num_slots, width);
+  return ts_launch(load_kernel<__nv_bfloat16>, grid, dim3(128), 0, s, (const uint8_t*)pool, slots, (__nv_bfloat16*)k, (__nv_bfloat16*)v, rows, nkv,
+                   log_groups, page_blocks, num_slots, width);
 }
 
 // k, v: [num_seqs * blocks][128][nkv][128] bfloat16, out_table [num_seqs][blocks]; blocks * 128 rows hold the longest request.
@@ -343,11 +432,13 @@ TS_EXPORT int ts_kv4_expand(const void* pool, const int* table, int table_stride
                    table_stride, cu, context, (uint4*)k, (uint4*)v, out_table, out_lens, nkv, page_blocks, num_pages, blocks, window);
 }
 
-TS_EXPORT int ts_kv4_evict(void* pool, float* sums, const int* table, int table_stride, const int* context, int* new_lens, int num_seqs, int nkv, int d,
-                           int page_blocks, int num_pages, int budget, int recent, int first, void* stream) {
+// order: num_seqs * nkv * budget ints of workspace; context[b] <= max_context.
+TS_EXPORT int ts_kv4_evict(void* pool, float* sums, const int* table, int table_stride, const int* context, int* new_lens, int* order, int num_seqs, int nkv,
+                           int d, int page_blocks, int num_pages, int max_context, int budget, int recent, int first, void* stream) {
   if (num_seqs < 1) return 0;
   if (num_seqs > 65535) return TS_ERR_UNSUPPORTED_SIZE;
   if (recent < 0 || first < 0 || budget < 1 || recent + first > budget) return TS_ERR_BAD_ARGUMENT;
-  return ts_launch(evict_kernel, dim3(nkv, num_seqs), dim3(kEvictThreads), 0, (cudaStream_t)stream, (uint8_t*)pool, sums, table, table_stride, context,
-                   new_lens, nkv, d, page_blocks, num_pages, budget, recent, first);
+  auto launch = d == 64 ? launch_evict<64> : d == 128 ? launch_evict<128> : launch_evict<256>;
+  return launch((uint8_t*)pool, sums, table, table_stride, context, new_lens, order, num_seqs, nkv, page_blocks, num_pages, max_context, budget, recent,
+                first, (cudaStream_t)stream);
 }

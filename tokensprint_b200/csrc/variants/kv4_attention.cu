@@ -19,8 +19,24 @@ namespace {
 
 constexpr int D = TS_HEAD_DIM;
 using Rec = Kv4Record<D>;
-constexpr int kWarps = 8;
-constexpr int kStages = 4;       // records of a warp's ring
+#ifndef X_WARPS
+#define X_WARPS 8
+#endif
+#ifndef X_RING
+#define X_RING 2
+#endif
+#ifndef X_CTAS
+#define X_CTAS 3
+#endif
+#ifndef X_REC
+#define X_REC 1
+#endif
+#ifndef X_CTAS2
+#define X_CTAS2 1
+#endif
+constexpr int kWarps = X_WARPS;
+constexpr int kRing = X_RING;         // records of a warp's ring
+constexpr float kLowest = -3.402823466e38f;  // the running maximum before the first key (finite: no difference of it is NaN)
 constexpr int kMaxTiles = 1024;  // (sequence, row tile) pairs of a launch: a CTA keeps their key ranges in shared memory
 constexpr int kMaxParts = 64;    // most CTAs that share a key range
 constexpr float kLog2e = 1.4426950408889634f;
@@ -138,13 +154,10 @@ template <typename T>
 __device__ __forceinline__ void write_row(const Params& p, const Tile& tile, int row, int channel, float4 o, float m, float l) {
   const int head = tile.query_head(p, row);
   if (p.sinks != nullptr) {
-    const float sink = p.sinks[head] * kLog2e, top = fmaxf(m, sink);
-    if (top != -INFINITY) {
-      const float f = m == -INFINITY ? 0.f : kv4_exp2(m - top);
-      l = l * f + kv4_exp2(sink - top);
-      o.x *= f, o.y *= f, o.z *= f, o.w *= f;
-      m = top;
-    }
+    const float sink = fmaxf(p.sinks[head] * kLog2e, kLowest), top = fmaxf(m, sink), f = kv4_exp2(m - top);
+    l = l * f + kv4_exp2(sink - top);
+    o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+    m = top;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
   const size_t at = ((size_t)tile.token(p, row) * p.nq + head) * D + channel;
@@ -159,23 +172,23 @@ __device__ __forceinline__ void write_row(const Params& p, const Tile& tile, int
 
 // Parts of one row (maximum, sum, four channels) added to one another.
 struct RowSum {
-  float m = -INFINITY, l = 0.f;
+  float m = kLowest, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   __device__ __forceinline__ void add(float pm, float pl, float4 v, float top) {
-    const float f = pm == -INFINITY ? 0.f : kv4_exp2(pm - top);  // (a part that saw nothing holds zeros; NaN stays NaN)
+    const float f = kv4_exp2(pm - top);
     l += f * pl;
     o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
   }
 };
 
-// The key ranges of all (sequence, row tile) pairs, counted in records, one behind the other; every key head has them again.
+// The key ranges of all (sequence, row tile) pairs, counted in steps of kRecords records, one behind the other; every key head has them again.
 // A CTA's share is an equal part of all of them, whatever the lengths are, and may begin and end inside a range.
 struct Shares {
-  int before[kMaxTiles + 1];  // records of one head before the pair
+  int before[kMaxTiles + 1];  // steps of one head before the pair
 };
 
-template <typename T, int kTiles, int kQ, int kP>
-__global__ void __launch_bounds__(kWarps * 32, kTiles == 1 && D <= 128 && sizeof(T) == 2 ? 2 : 1) attention_kernel(const Params p) {
+template <typename T, int kTiles, int kQ, int kP, int kRecords>
+__global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : kTiles == 1 ? X_CTAS : X_CTAS2) attention_kernel(const Params p) {
   constexpr int kRows = 8 * kTiles;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Shares shares;
@@ -200,7 +213,7 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 && D <= 128 && sizeof
       int n = 0;
       if (tile.first_row < tile.rows) {
         const int key1 = tile.position(p, min(tile.first_row + kRows, tile.rows) - 1) + 1;
-        if (key1 > 0) n = (key1 + KV4_BLOCK - 1) / KV4_BLOCK - first_record(tile);
+        if (key1 > 0) n = ((key1 + KV4_BLOCK - 1) / KV4_BLOCK - first_record(tile) + kRecords - 1) / kRecords;
       }
       shares.before[i] = sum;  // completed below
       sum += n;
@@ -232,12 +245,12 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 && D <= 128 && sizeof
       open(tile, i, head);
       for (int x = tid; x < kRows * (D / 4); x += kWarps * 32) {
         const int row = tile.first_row + x / (D / 4);
-        if (row < tile.rows) write_row<T>(p, tile, row, x % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
+        if (row < tile.rows) write_row<T>(p, tile, row, x % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f), kLowest, 0.f);
       }
     }
   }
   const int total = shares.before[pairs] * p.nkv;
-  // at least a record for every warp, and no range over more than kMaxParts CTAs
+  // at least a step for every warp, and no range over more than kMaxParts CTAs
   const int share = max(max(kWarps, (total + (int)gridDim.x - 1) / (int)gridDim.x), (most + kMaxParts - 1) / kMaxParts);
   const int begin = (int)min((long long)share * blockIdx.x, (long long)total), end = min(begin + share, total);
   if (begin >= end) return;
@@ -251,40 +264,54 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 && D <= 128 && sizeof
     return lo;
   };
 
-  // ---- a warp's records: begin + warp, + kWarps, ...; lane i looks up where the i-th of the next 32 lies, one round ahead
-  auto look_up = [&](int step) -> uint32_t {
-    if (step >= end) return 0u;
+  // ---- a warp's steps: begin + warp, + kWarps, ...; lane i looks up where the i-th of its next 32 records lies, one round ahead
+  constexpr uint32_t kNone = 0xffffffffu;
+  auto look_up = [&](int record) -> uint32_t {  // counted over the warp's steps
+    const int step = begin + warp + record / kRecords * kWarps;
+    if (step >= end) return kNone;
     const int pair = pair_of(step), n = shares.before[pair + 1] - shares.before[pair], at = step - shares.before[pair] * p.nkv;
     const int head = at / n;
     Tile tile;
     open(tile, pair, head);
-    const int blk = first_record(tile) + at % n;
+    const int blk = first_record(tile) + at % n * kRecords + record % kRecords;
+    if (blk * KV4_BLOCK >= tile.context) return kNone;  // (an odd number of records)
     const int page = p.table[(size_t)(pair / p.row_tiles) * p.table_stride + blk / p.page_blocks];
     return ((uint32_t)min(max(page, 0), p.num_pages - 1) * p.nkv + head) * p.page_blocks + blk % p.page_blocks;
   };
   const int mine = begin + warp;
-  uint32_t here = look_up(mine + lane * kWarps), ahead = look_up(mine + (32 + lane) * kWarps);
-  uint8_t* ring = smem + warp * (kStages * Rec::kBytes);
+  uint32_t here = look_up(lane), ahead = look_up(32 + lane);
+  uint8_t* ring = smem + warp * (kRing * Rec::kBytes);
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+  const uint8_t* pool_at = p.pool + lane * 16;
+  constexpr int kStages = kRing / kRecords;
   int fetched = 0;  // records asked for
   auto fetch = [&]() {
-    if (mine + fetched * kWarps < end) {
-      const uint8_t* src = p.pool + (size_t)__shfl_sync(0xffffffffu, here, fetched & 31) * Rec::kBytes + lane * 16;
-      const uint32_t dst = ring_at + (fetched % kStages) * Rec::kBytes;
 #pragma unroll
-      for (int i = 0; i < Rec::kBytes / 512; ++i) copy16(dst + i * 512, src + i * 512);
-      if (Rec::kBytes % 512 && lane < Rec::kBytes % 512 / 16) copy16(dst + Rec::kBytes / 512 * 512, src + Rec::kBytes / 512 * 512);
+    for (int r = 0; r < kRecords; ++r) {
+      const uint32_t which = __shfl_sync(0xffffffffu, here, (fetched + r) & 31);
+      if (which != kNone) {
+        const uint8_t* src = pool_at + (size_t)which * Rec::kBytes;
+        const uint32_t dst = ring_at + (fetched % kRing + r) * Rec::kBytes;
+#pragma unroll
+        for (int i = 0; i < Rec::kBytes / 512; ++i) copy16(dst + i * 512, src + i * 512);
+        if (Rec::kBytes % 512 && lane < Rec::kBytes % 512 / 16) copy16(dst + Rec::kBytes / 512 * 512, src + Rec::kBytes / 512 * 512);
+      }
     }
     copy_commit();
-    if ((++fetched & 31) == 0) {
+    fetched += kRecords;
+    if ((fetched & 31) == 0) {
       here = ahead;
-      ahead = look_up(mine + (fetched + 32 + lane) * kWarps);
+      ahead = look_up(fetched + 32 + lane);
     }
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch();
 
-  int done = 0;  // records worked on
+  uint4* sq = reinterpret_cast<uint4*>(smem + kWarps * kRing * Rec::kBytes);                  // [tiles][parts][words][lanes]
+  float* so = reinterpret_cast<float*>(sq + kTiles * kQ * D);                                 // [warps][rows][D]
+  float* sm = so + kWarps * kRows * D;                                                        // [warps][rows]
+  float* sl = sm + kWarps * kRows;
+  int done = 0;  // steps worked on
   for (int seg = begin; seg < end;) {
     const int pair = pair_of(seg), n_pair = shares.before[pair + 1] - shares.before[pair];
     const int head = (seg - shares.before[pair] * p.nkv) / n_pair, base = shares.before[pair] * p.nkv + head * n_pair;
@@ -296,16 +323,22 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 && D <= 128 && sizeof
     // keys that every row sees: [all0, all1)
     const int all0 = p.window > 0 ? last_pos - p.window + 1 : 0, all1 = first_pos + 1;
 
-    uint32_t qf[kTiles][kQ][D / 16][2];
+    // the queries as the products' second operand, one copy for all warps
+    if (warp < kTiles) {
+      uint32_t qf[kQ][D / 16][2];
+      const int row = tile.first_row + 8 * warp + g;
+      kv4_query_row<D, kQ>(row < tile.rows ? tile.query<T>(p, row) + t * (D / 4) : nullptr, qf);
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      const int row = tile.first_row + 8 * n + g;
-      kv4_query_row<D, kQ>(row < tile.rows ? tile.query<T>(p, row) + t * (D / 4) : nullptr, qf[n]);
+      for (int k = 0; k < kQ; ++k)
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w)
+          sq[((warp * kQ + k) * (D / 32) + w) * 32 + lane] = make_uint4(qf[k][2 * w][0], qf[k][2 * w][1], qf[k][2 * w + 1][0], qf[k][2 * w + 1][1]);
     }
+    __syncthreads();
     float o[kTiles][D / 16][4], m[kTiles][2], l[kTiles][2];
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
-      m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+      m[n][0] = m[n][1] = kLowest, l[n][0] = l[n][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
@@ -314,31 +347,40 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 && D <= 128 && sizeof
       fetch();
       copy_wait<kStages - 1>();
       __syncwarp();
-      const uint8_t* rec = ring + (done % kStages) * Rec::kBytes;
-      float s[kTiles][4];
-      kv4_scores<D, kTiles, kQ>(rec, rec + Rec::kKeyScales, qf, s, g, t);
-      const int key = (blk0 + mine + done * kWarps - base) * KV4_BLOCK;
-      const bool edge = key < all0 || key + KV4_BLOCK > all1;
+      const uint8_t* rec = ring + (done % kStages) * (kRecords * Rec::kBytes);
+      float s[kRecords][kTiles][4];
+#pragma unroll
+      for (int r = 0; r < kRecords; ++r)
+        kv4_scores<D, kTiles, kQ>(rec + r * Rec::kBytes, rec + r * Rec::kBytes + Rec::kKeyScales,
+                                  [&](int n, int part, int w) { return sq[((n * kQ + part) * (D / 32) + w) * 32 + lane]; }, s[r], g, t);
+      const int key = (blk0 + (mine + done * kWarps - base) * kRecords) * KV4_BLOCK;
+      const bool edge = key < all0 || key + kRecords * KV4_BLOCK > all1;
       bool grows = false;
       float top[kTiles][2];
 #pragma unroll
       for (int n = 0; n < kTiles; ++n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] *= p.scale;
+        for (int r = 0; r < kRecords; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[r][n][i] *= p.scale;
         if (edge) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const int r = tile.first_row + 8 * n + 2 * t + c, pos = r < tile.rows ? tile.position(p, r) : -1;
+            const int row = tile.first_row + 8 * n + 2 * t + c, pos = row < tile.rows ? tile.position(p, row) : -1;
 #pragma unroll
-            for (int i = c; i < 4; i += 2) {
-              const int at = key + g + 4 * (i - c);
-              if (at > pos || (p.window > 0 && at <= pos - p.window)) s[n][i] = -INFINITY;
-            }
+            for (int r = 0; r < kRecords; ++r)
+#pragma unroll
+              for (int i = c; i < 4; i += 2) {
+                const int at = key + r * KV4_BLOCK + g + 4 * (i - c);
+                if (at > pos || (p.window > 0 && at <= pos - p.window)) s[r][n][i] = -INFINITY;
+              }
           }
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          top[n][c] = fmaxf(s[n][c], s[n][c + 2]);
+          top[n][c] = fmaxf(s[0][n][c], s[0][n][c + 2]);
+#pragma unroll
+          for (int r = 1; r < kRecords; ++r) top[n][c] = fmaxf(top[n][c], fmaxf(s[r][n][c], s[r][n][c + 2]));
           grows |= top[n][c] > m[n][c] + 8.f;
         }
       }
@@ -353,40 +395,40 @@ __global__ void __launch_bounds__(kWarps * 32, kTiles == 1 && D <= 128 && sizeof
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
             x = fmaxf(x, m[n][c]);
-            const float f = x == -INFINITY ? 1.f : kv4_exp2(m[n][c] - x);
+            const float f = kv4_exp2(m[n][c] - x);
             m[n][c] = x;
             l[n][c] *= f;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) o[n][i][c] *= f, o[n][i][c + 2] *= f;
           }
       }
-      uint32_t pf[kTiles][kP][2];
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n) {
-        float w[4];
-        const float off[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
+      for (int r = 0; r < kRecords; ++r) {
+        uint32_t pf[kTiles][kP][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[i] = kv4_exp2(s[n][i] - off[i & 1]);
-          l[n][i & 1] += w[i];
+        for (int n = 0; n < kTiles; ++n) {
+          float w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            w[i] = kv4_exp2(s[r][n][i] - m[n][i & 1]);
+            l[n][i & 1] += w[i];
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t parts[kP];
+            kv4_split<kP>(w[2 * i], w[2 * i + 1], parts);
+#pragma unroll
+            for (int k = 0; k < kP; ++k) pf[n][k][i] = transpose8x8(parts[k]);
+          }
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t parts[kP];
-          kv4_split<kP>(w[2 * i], w[2 * i + 1], parts);
-#pragma unroll
-          for (int k = 0; k < kP; ++k) pf[n][k][i] = transpose8x8(parts[k]);
-        }
+        const int from = key + r * KV4_BLOCK;
+        if (edge) add_values<kTiles, kP, true>(rec + r * Rec::kBytes, pf, o, g, t, key0 - from, last_pos + 1 - from);
+        else add_values<kTiles, kP, false>(rec + r * Rec::kBytes, pf, o, g, t, 0, KV4_BLOCK);
       }
-      if (edge) add_values<kTiles, kP, true>(rec, pf, o, g, t, key0 - key, last_pos + 1 - key);
-      else add_values<kTiles, kP, false>(rec, pf, o, g, t, 0, KV4_BLOCK);
       __syncwarp();
     }
 
     // ---- the warps' parts of the segment meet in shared memory (behind the rings, which are being filled)
-    float* so = reinterpret_cast<float*>(smem + kWarps * kStages * Rec::kBytes);  // [warps][rows][D]
-    float* sm = so + kWarps * kRows * D;                                           // [warps][rows]
-    float* sl = sm + kWarps * kRows;
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
@@ -481,7 +523,9 @@ __global__ void __launch_bounds__(kWarps * 32) weights_kernel(const Params p, fl
     uint32_t qf[1][kQ][D / 16][2];
     kv4_query_row<D, kQ>(first + g < tile.rows ? tile.query<T>(p, first + g) + t * (D / 4) : nullptr, qf[0]);
     float s[1][4];
-    kv4_scores<D, 1, kQ>(rec, rec + Rec::kKeyScales, qf, s, g, t);
+    kv4_scores<D, 1, kQ>(rec, rec + Rec::kKeyScales,
+                         [&](int, int part, int i) { return make_uint4(qf[0][part][2 * i][0], qf[0][part][2 * i][1], qf[0][part][2 * i + 1][0], qf[0][part][2 * i + 1][1]); },
+                         s, g, t);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int r = first + 2 * t + c;
@@ -678,40 +722,46 @@ int launch_weights(const Params& p, float* sums, int num_seqs, int max_context, 
   return ts_launch(weights_rows_kernel<T, kQ>, grid, dim3(kWeightThreads), smem, stream, p, sums);
 }
 
-template <typename T, int kTiles, int kQ, int kP>
+template <typename T, int kTiles, int kQ, int kP, int kRecords>
 struct Attention {
-  static constexpr int kSmem = kWarps * kStages * Rec::kBytes + kWarps * 8 * kTiles * (D + 2) * 4;
+  static constexpr int kSmem = kWarps * kRing * Rec::kBytes + kTiles * kQ * D * 16 + kWarps * 8 * kTiles * (D + 2) * 4;
   // CTAs that run at once on the device, or a negative error
   static int ctas() {
     static int n = 0;
     if (n == 0) {
       int device = 0, sms = 0, per_sm = 0;
-      cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kTiles, kQ, kP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+      cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kTiles, kQ, kP, kRecords>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
       if (e == cudaSuccess) e = cudaGetDevice(&device);
       if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-      if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_kernel<T, kTiles, kQ, kP>, kWarps * 32, kSmem);
+      if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_kernel<T, kTiles, kQ, kP, kRecords>, kWarps * 32, kSmem);
       if (e != cudaSuccess) return -(int)e - 100;
       n = sms * (per_sm > 0 ? per_sm : 1);
     }
     return n;
   }
   static int launch(const Params& p, int grid, cudaStream_t stream) {
-    return ts_launch(attention_kernel<T, kTiles, kQ, kP>, dim3(grid), dim3(kWarps * 32), kSmem, stream, p);
+    return ts_launch(attention_kernel<T, kTiles, kQ, kP, kRecords>, dim3(grid), dim3(kWarps * 32), kSmem, stream, p);
   }
 };
 
 }  // namespace
+
+using AttentionFloat = Attention<float, 1, 3, 3, 1>;
+using AttentionFew = Attention<__nv_bfloat16, 1, 1, 2, D <= 128 ? X_REC : 1>;
+#if TS_HEAD_DIM <= 128
+using AttentionMore = Attention<__nv_bfloat16, 2, 1, 2, 1>;
+#endif
 
 // How many rows a tile has, by the type and the rows of a sequence and key head.
 static int tile_rows(int dtype, int rows) { return dtype == TS_DTYPE_BF16 && rows > 8 && D <= 128 ? 16 : 8; }
 
 // CTAs of a launch (at most), for the size of `part`: grid * 2 * tile rows * (D + 4) floats; negative: an error.
 static int grid_of(int dtype, int rows) {
-  if (dtype == TS_DTYPE_F32) return Attention<float, 1, 3, 3>::ctas();
+  if (dtype == TS_DTYPE_F32) return AttentionFloat::ctas();
 #if TS_HEAD_DIM <= 128
-  if (tile_rows(dtype, rows) == 16) return Attention<__nv_bfloat16, 2, 1, 2>::ctas();
+  if (tile_rows(dtype, rows) == 16) return AttentionMore::ctas();
 #endif
-  return Attention<__nv_bfloat16, 1, 1, 2>::ctas();
+  return AttentionFew::ctas();
 }
 TS_EXPORT long long ts_attention_kv4_part_floats(int dtype, int rows) {
   const int grid = grid_of(dtype, rows);
@@ -740,11 +790,11 @@ TS_EXPORT int ts_attention_kv4(const void* q, int dtype, const void* pool, void*
                   num_pages, tokens, num_seqs - b < seqs ? num_seqs - b : seqs, nq, nkv, nq / nkv, window,
                   row_tiles - tile < tiles ? row_tiles - tile : tiles, tile, scale * kLog2e};
       int status;
-      if (dtype == TS_DTYPE_F32) status = Attention<float, 1, 3, 3>::launch(p, grid, (cudaStream_t)stream);
+      if (dtype == TS_DTYPE_F32) status = AttentionFloat::launch(p, grid, (cudaStream_t)stream);
 #if TS_HEAD_DIM <= 128
-      else if (tile_rows(dtype, rows) == 16) status = Attention<__nv_bfloat16, 2, 1, 2>::launch(p, grid, (cudaStream_t)stream);
+      else if (tile_rows(dtype, rows) == 16) status = AttentionMore::launch(p, grid, (cudaStream_t)stream);
 #endif
-      else status = Attention<__nv_bfloat16, 1, 1, 2>::launch(p, grid, (cudaStream_t)stream);
+      else status = AttentionFew::launch(p, grid, (cudaStream_t)stream);
       if (status) return status;
     }
   return 0;

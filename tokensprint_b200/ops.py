@@ -2512,7 +2512,7 @@ KV4_BLOCK = 16  # tokens of a record, channels that share a scale
 KV4_HEAD_DIMS = (64, 128, 256)
 _SIGNATURES["ts_kv4_store"] = [_c_void_p, _c_void_p, _c_int, _c_ll, _c_ll, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p]
 _SIGNATURES["ts_kv4_load"] = [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p]
-_SIGNATURES["ts_kv4_evict"] = [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p] + [_c_int] * 8 + [_c_void_p]
+_SIGNATURES["ts_kv4_evict"] = [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p] + [_c_int] * 9 + [_c_void_p]
 _SIGNATURES["ts_kv4_expand"] = [_c_void_p, _c_void_p, _c_int] + [_c_void_p] * 6 + [_c_int] * 6 + [_c_void_p]
 _attention_kv4: dict[int, tuple] = {}
 # Portions of prompts with more rows (tokens x query heads of a key head) than this are attended to on tcgen05 tensor cores, over rows unpacked for the step.
@@ -2775,9 +2775,10 @@ def kv4_evict(pool: torch.Tensor, sums: torch.Tensor, block_table: torch.Tensor,
         raise KernelError(f"kv4_evict: a budget of {budget} rows cannot hold the first {first} and the last {recent}")
     if max_context < 0 or num_seqs < 0:
         raise KernelError("kv4_evict: negative sizes")
+    order = torch.empty(num_seqs * nkv * budget, device=pool.device, dtype=torch.int32)  # where every kept row comes from
     _check("kv4_evict", _fn("ts_kv4_evict")(
-        pool.data_ptr(), sums.data_ptr(), block_table.data_ptr(), block_table.shape[1], context_lens.data_ptr(), new_lens.data_ptr(), num_seqs, nkv, d,
-        blocks, pages, int(budget), int(recent), int(first), _stream()))
+        pool.data_ptr(), sums.data_ptr(), block_table.data_ptr(), block_table.shape[1], context_lens.data_ptr(), new_lens.data_ptr(), order.data_ptr(),
+        num_seqs, nkv, d, blocks, pages, int(max_context), int(budget), int(recent), int(first), _stream()))
 
 
 # ---------------------------------------------------------------------------

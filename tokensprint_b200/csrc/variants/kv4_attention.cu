@@ -20,16 +20,16 @@ namespace {
 constexpr int D = TS_HEAD_DIM;
 using Rec = Kv4Record<D>;
 #ifndef X_WARPS
-#define X_WARPS 8
+#define X_WARPS 4
 #endif
 #ifndef X_RING
-#define X_RING 2
+#define X_RING 4
 #endif
 #ifndef X_CTAS
-#define X_CTAS 3
+#define X_CTAS 4
 #endif
 #ifndef X_REC
-#define X_REC 1
+#define X_REC 2
 #endif
 #ifndef X_CTAS2
 #define X_CTAS2 1

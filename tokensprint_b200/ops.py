@@ -2519,6 +2519,7 @@ _attention_kv4: dict[int, tuple] = {}
 ATTENTION_KV4_DIRECT_ROWS = 64
 ATTENTION_KV4_EXPAND_BYTES = 1 << 30  # most bytes of unpacked rows at a time
 _attention_kv4_tcgen05: dict[bool, object] = {}
+_attention_kv4_scratches: dict[tuple, tuple[torch.Tensor, torch.Tensor]] = {}
 
 
 def kv4_pool_shape(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int) -> tuple[int, int, int, int]:
@@ -2534,21 +2535,43 @@ def kv4_pool_shape(num_pages: int, page_size: int, num_kv_heads: int, head_dim: 
     return (num_pages, num_kv_heads, page_size // KV4_BLOCK, 18 * head_dim)
 
 
+_KV4_RECORD_DIMS = {18 * d: d for d in KV4_HEAD_DIMS}
+
+
 def _kv4_pool(name: str, pool: torch.Tensor) -> tuple[int, int, int, int]:
-    """(pages, key/value heads, records per page, head size) of a pool."""
+    """(pages, key/value heads, records per page, head size) of a pool.  (These operators run for every layer of a decode step: what
+    their checks ask is asked once, in one expression, and told apart only where it fails.)"""
+    shape = pool.shape
+    if pool.dtype is torch.uint8 and len(shape) == 4 and pool.is_cuda and pool.is_contiguous():
+        pages, heads, blocks, record = shape
+        d = _KV4_RECORD_DIMS.get(record)
+        if d is not None and heads > 0 and 0 < pages * blocks < 1 << 27 and pool.data_ptr() % 16 == 0:
+            return pages, heads, blocks, d
     _cuda_contig(f"{name}: pool", pool, torch.uint8)
-    if pool.dim() != 4 or pool.shape[3] % 18 or pool.shape[3] // 18 not in KV4_HEAD_DIMS or min(pool.shape) < 1:
-        raise KernelError(f"{name}: the pool must be [pages, heads, page size / 16, 18 * head size] with heads of {KV4_HEAD_DIMS}, got {tuple(pool.shape)}")
-    if pool.data_ptr() % 16 or pool.shape[0] * pool.shape[2] * KV4_BLOCK >= 1 << 31:
-        raise KernelError(f"{name}: the pool must start on a 16-byte boundary and hold fewer than 2^31 rows")
-    return pool.shape[0], pool.shape[1], pool.shape[2], pool.shape[3] // 18
+    if len(shape) != 4 or shape[3] not in _KV4_RECORD_DIMS or min(shape) < 1:
+        raise KernelError(f"{name}: the pool must be [pages, heads, page size / 16, 18 * head size] with heads of {KV4_HEAD_DIMS}, got {tuple(shape)}")
+    raise KernelError(f"{name}: the pool must start on a 16-byte boundary and hold fewer than 2^31 rows")
 
 
 def _kv4_sums(name: str, sums: torch.Tensor, pool: torch.Tensor) -> None:
     _cuda_contig(f"{name}: sums", sums, torch.float32)
-    want = (pool.shape[0], pool.shape[1], pool.shape[2] * KV4_BLOCK)
-    if tuple(sums.shape) != want:
-        raise KernelError(f"{name}: sums must be [pages, heads, page size] = {want}, got {tuple(sums.shape)}")
+    pages, heads, blocks, _ = pool.shape
+    if sums.shape != (pages, heads, blocks * KV4_BLOCK):
+        raise KernelError(f"{name}: sums must be [pages, heads, page size] = {(pages, heads, blocks * KV4_BLOCK)}, got {tuple(sums.shape)}")
+
+
+def _kv4_store_refusal(k, v, slot_mapping, nkv, d) -> None:
+    """Says what is wrong with the arguments of kv4_store."""
+    _act_code("kv4_store: k", k)
+    _cuda_contig("kv4_store: slot_mapping", slot_mapping, torch.int32)
+    for name, t in (("k", k), ("v", v)):
+        if not t.is_cuda or t.dtype != k.dtype or t.dim() != 3 or tuple(t.shape[1:]) != (nkv, d) or t.shape[0] != k.shape[0]:
+            raise KernelError(f"kv4_store: {name} must be a CUDA tensor [T, {nkv}, {d}] of k's type, got {tuple(t.shape)} {t.dtype}")
+        if t.shape[0] > 0 and (t.stride(2) != 1 or (t.stride(1) != d and nkv > 1)):
+            raise KernelError(f"kv4_store: {name}'s heads must lie one behind the other, got strides {t.stride()}")
+        if (t.shape[0] > 1 and t.stride(0) * t.element_size() % 16) or t.data_ptr() % 16:
+            raise KernelError(f"kv4_store: {name}'s rows must start on 16-byte boundaries")
+    raise KernelError("kv4_store: slot_mapping is shorter than the rows")
 
 
 def kv4_store(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, slot_mapping: torch.Tensor, sums: Optional[torch.Tensor] = None) -> None:
@@ -2560,37 +2583,39 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, slot_mapping
     largest value.  `sums` (the pool's weights, see attention_kv4_weights): set to 0 at the stored rows."""
     flush_gemm_chain()
     pages, nkv, blocks, d = _kv4_pool("kv4_store", pool)
-    code = _act_code("kv4_store: k", k)
-    _cuda_contig("kv4_store: slot_mapping", slot_mapping, torch.int32)
-    for name, t in (("k", k), ("v", v)):
-        if not t.is_cuda or t.dtype != k.dtype or t.dim() != 3 or tuple(t.shape[1:]) != (nkv, d) or t.shape[0] != k.shape[0]:
-            raise KernelError(f"kv4_store: {name} must be a CUDA tensor [T, {nkv}, {d}] of k's type, got {tuple(t.shape)} {t.dtype}")
-        if t.shape[0] > 0 and ((t.stride(2) != 1 and d > 1) or (t.stride(1) != d and nkv > 1)):
-            raise KernelError(f"kv4_store: {name}'s heads must lie one behind the other, got strides {t.stride()}")
-        if t.shape[0] > 1 and t.stride(0) * t.element_size() % 16 or t.data_ptr() % 16:
-            raise KernelError(f"kv4_store: {name}'s rows must start on 16-byte boundaries")
-    if slot_mapping.numel() < k.shape[0]:
-        raise KernelError("kv4_store: slot_mapping is shorter than the rows")
+    shape, dtype = k.shape, k.dtype
+    code = DTYPE_CODES.get(dtype)
+    T = shape[0] if len(shape) else 0
+    at_k, at_v = k.data_ptr(), v.data_ptr()
+    if (code is None or shape != (T, nkv, d) or v.shape != shape or v.dtype is not dtype or not (k.is_cuda and v.is_cuda)
+            or slot_mapping.dtype is not torch.int32 or not slot_mapping.is_cuda or not slot_mapping.is_contiguous() or slot_mapping.numel() < T):
+        _kv4_store_refusal(k, v, slot_mapping, nkv, d)
+    (k_stride, k_head, k_one), (v_stride, v_head, v_one) = k.stride(), v.stride()
+    if T > 0 and (k_one != 1 or v_one != 1 or (nkv > 1 and (k_head != d or v_head != d)) or (at_k | at_v) % 16
+                  or (T > 1 and (k_stride | v_stride) % (8 if code else 4))):
+        _kv4_store_refusal(k, v, slot_mapping, nkv, d)
     if sums is not None:
         _kv4_sums("kv4_store", sums, pool)
     _check("kv4_store", _fn("ts_kv4_store")(
-        k.data_ptr(), v.data_ptr(), code, k.stride(0), v.stride(0), pool.data_ptr(), _ptr(sums), slot_mapping.data_ptr(), k.shape[0], nkv, d, blocks,
-        pages, _stream()))
+        at_k, at_v, code, k_stride, v_stride, pool.data_ptr(), _ptr(sums), slot_mapping.data_ptr(), T, nkv, d, blocks, pages, _stream()))
 
 
 def kv4_load(pool: torch.Tensor, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
     """Rows of a 4-bit cache as values: k, v [N, nkv, d] float32 or bfloat16 (exact in both); slots [N] i32, a slot outside the pool gives zeros."""
     flush_gemm_chain()
     pages, nkv, blocks, d = _kv4_pool("kv4_load", pool)
-    code = _act_code("kv4_load: k", k)
-    _cuda_contig("kv4_load: slots", slots, torch.int32)
-    N = slots.numel()
-    for name, t in (("k", k), ("v", v)):
-        _cuda_contig(f"kv4_load: {name}", t, k.dtype)
-        if tuple(t.shape) != (N, nkv, d) or t.data_ptr() % 16:
-            raise KernelError(f"kv4_load: {name} must be [{N}, {nkv}, {d}] on a 16-byte boundary, got {tuple(t.shape)}")
-    _check("kv4_load", _fn("ts_kv4_load")(
-        pool.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), code, N, nkv, d, blocks, pages, _stream()))
+    dtype, N = k.dtype, slots.numel()
+    code = DTYPE_CODES.get(dtype)
+    at_k, at_v, want = k.data_ptr(), v.data_ptr(), (N, nkv, d)
+    if (code is None or k.shape != want or v.shape != want or v.dtype is not dtype or slots.dtype is not torch.int32 or (at_k | at_v) % 16
+            or not (k.is_cuda and v.is_cuda and slots.is_cuda and k.is_contiguous() and v.is_contiguous() and slots.is_contiguous())):
+        _act_code("kv4_load: k", k)
+        _cuda_contig("kv4_load: slots", slots, torch.int32)
+        for name, t in (("k", k), ("v", v)):
+            _cuda_contig(f"kv4_load: {name}", t, dtype)
+            if tuple(t.shape) != want or t.data_ptr() % 16:
+                raise KernelError(f"kv4_load: {name} must be [{N}, {nkv}, {d}] on a 16-byte boundary, got {tuple(t.shape)}")
+    _check("kv4_load", _fn("ts_kv4_load")(pool.data_ptr(), slots.data_ptr(), at_k, at_v, code, N, nkv, d, blocks, pages, _stream()))
 
 
 def _attention_kv4_fns(head_dim: int) -> tuple:
@@ -2608,25 +2633,48 @@ def _attention_kv4_fns(head_dim: int) -> tuple:
 
 
 def _check_attention_kv4(name, q, pool, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, d, window) -> tuple:
-    """Checks the arguments that attention over a 4-bit cache and its weights share; returns (pages, records per page, type code)."""
+    """Checks the arguments that attention over a 4-bit cache and its weights share; returns (pages, records per page, type code, T, entries of a
+    sequence in the block table)."""
     pages, pool_heads, blocks, pool_dim = _kv4_pool(name, pool)
-    code = _act_code(f"{name}: q", q)
+    code = DTYPE_CODES.get(q.dtype)
+    T = q.shape[0] if q.dim() else 0
+    table = block_table.shape
+    i32 = torch.int32
+    if (code is not None and pool_heads == nkv and pool_dim == d and nq % nkv == 0 and q.numel() == T * nq * d and q.data_ptr() % 16 == 0
+            and cu_seqlens_q.dtype is i32 and context_lens.dtype is i32 and block_table.dtype is i32 and len(table) == 2 and table[0] >= num_seqs
+            and (table[1] > 0 or num_seqs == 0) and cu_seqlens_q.numel() > num_seqs and context_lens.numel() >= num_seqs
+            and min(num_seqs, max_seqlen_q, max_context, window) >= 0
+            and q.is_cuda and cu_seqlens_q.is_cuda and context_lens.is_cuda and block_table.is_cuda
+            and q.is_contiguous() and cu_seqlens_q.is_contiguous() and context_lens.is_contiguous() and block_table.is_contiguous()):
+        return pages, blocks, code, T, table[1]
+    _act_code(f"{name}: q", q)
     _cuda_contig(f"{name}: q", q)
     for label, t in (("cu_seqlens_q", cu_seqlens_q), ("context_lens", context_lens), ("block_table", block_table)):
-        _cuda_contig(f"{name}: {label}", t, torch.int32)
+        _cuda_contig(f"{name}: {label}", t, i32)
     if (pool_heads, pool_dim) != (nkv, d):
         raise KernelError(f"{name}: the pool holds {pool_heads} heads of {pool_dim}, the call names {nkv} of {d}")
-    if nkv < 1 or nq % nkv:
+    if nq % nkv:
         raise KernelError(f"{name}: {nq} query heads are no multiple of {nkv} key/value heads")
-    if q.dim() < 1 or q.numel() != q.shape[0] * nq * d or q.data_ptr() % 16:
+    if q.numel() != T * nq * d or q.data_ptr() % 16:
         raise KernelError(f"{name}: q must be [T, {nq * d}] on a 16-byte boundary, got {tuple(q.shape)}")
-    if block_table.dim() != 2 or block_table.shape[0] < num_seqs or (num_seqs > 0 and block_table.shape[1] < 1):
+    if len(table) != 2 or table[0] < num_seqs or table[1] < 1:
         raise KernelError(f"{name}: block_table must be [B, max_blocks]")
     if cu_seqlens_q.numel() < num_seqs + 1 or context_lens.numel() < num_seqs:
         raise KernelError(f"{name}: cu_seqlens_q/context_lens are shorter than the batch")
-    if num_seqs < 0 or max_seqlen_q < 0 or max_context < 0 or window < 0:
-        raise KernelError(f"{name}: negative sizes")
-    return pages, blocks, code
+    raise KernelError(f"{name}: negative sizes")
+
+
+def _attention_kv4_scratch(device: torch.device, head_dim: int, code: int, rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per (device, stream): where CTAs that share a key range leave their parts (the size goes by the device and the kernel alone), and the
+    tickets that tell the last of them (zeros between launches)."""
+    key = (device.index or 0, _stream(), head_dim, code, rows > 8)
+    scratch = _attention_kv4_scratches.get(key)
+    if scratch is None:
+        need = _attention_kv4_fns(head_dim)[2](code, rows)
+        if need < 0:
+            _check("attention_kv4", -need - 100)
+        scratch = _attention_kv4_scratches[key] = (torch.empty(need, device=device, dtype=torch.float32), _attention_counters(device))
+    return scratch
 
 
 def attention_kv4(
@@ -2657,31 +2705,27 @@ def attention_kv4(
     (-inf for a query that sees nothing; its output is zero)."""
     flush_gemm_chain()
     nq, nkv, d = num_heads, num_kv_heads, head_dim
-    pages, blocks, code = _check_attention_kv4("attention_kv4", q, pool, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context,
-                                               nq, nkv, d, window)
-    T = q.shape[0]
-    _cuda_contig("attention_kv4: out", out, q.dtype)
-    if out.numel() != q.numel() or out.data_ptr() % 16:
+    pages, blocks, code, T, width = _check_attention_kv4("attention_kv4", q, pool, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q,
+                                                         max_context, nq, nkv, d, window)
+    if out.dtype is not q.dtype or not out.is_cuda or not out.is_contiguous() or out.numel() != q.numel() or out.data_ptr() % 16:
+        _cuda_contig("attention_kv4: out", out, q.dtype)
         raise KernelError(f"attention_kv4: out must be of q's size on a 16-byte boundary, got {tuple(out.shape)}")
-    for label, t, n in (("head_sinks", head_sinks, nq), ("lse", lse, T * nq)):
-        if t is not None:
-            _cuda_contig(f"attention_kv4: {label}", t, torch.float32)
-            if t.numel() != n:
-                raise KernelError(f"attention_kv4: {label} must have {n} entries, got {t.numel()}")
+    if head_sinks is not None or lse is not None:
+        for label, t, n in (("head_sinks", head_sinks, nq), ("lse", lse, T * nq)):
+            if t is not None:
+                _cuda_contig(f"attention_kv4: {label}", t, torch.float32)
+                if t.numel() != n:
+                    raise KernelError(f"attention_kv4: {label} must have {n} entries, got {t.numel()}")
     rows = max_seqlen_q * (nq // nkv)
-    if rows > ATTENTION_KV4_DIRECT_ROWS and code == DTYPE_CODES[torch.bfloat16] and attention_tcgen05_supported(nq, nkv, d, _KV4_EXPAND_PAGE) and max_context > 0:
+    if rows > ATTENTION_KV4_DIRECT_ROWS and code == 1 and attention_tcgen05_supported(nq, nkv, d, _KV4_EXPAND_PAGE) and max_context > 0:
         _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, scale, window,
                                 head_sinks, lse)
         return
-    run, _, part_floats = _attention_kv4_fns(d)
-    need = part_floats(code, rows)
-    if need < 0:
-        _check("attention_kv4", -need - 100)
-    part = torch.empty(need, device=q.device, dtype=torch.float32)
-    _check("attention_kv4", run(
+    part, tickets = _attention_kv4_scratch(q.device, d, code, rows)
+    _check("attention_kv4", _attention_kv4_fns(d)[0](
         q.data_ptr(), code, pool.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(head_sinks), cu_seqlens_q.data_ptr(), context_lens.data_ptr(),
-        block_table.data_ptr(), block_table.shape[1], blocks, pages, T, num_seqs, max_seqlen_q, nq, nkv, float(scale), int(window), part.data_ptr(),
-        _attention_counters(q.device).data_ptr(), _GEMM_MAX_TILES, _stream()))
+        block_table.data_ptr(), width, blocks, pages, T, num_seqs, max_seqlen_q, nq, nkv, scale, window, part.data_ptr(), tickets.data_ptr(),
+        _GEMM_MAX_TILES, _stream()))
 
 
 _KV4_EXPAND_PAGE = 128
@@ -2744,16 +2788,15 @@ def attention_kv4_weights(
     sums [pages, nkv, page size] f32.  Every row's sum is formed in one order: equal inputs give equal bits."""
     flush_gemm_chain()
     nq, nkv, d = num_heads, num_kv_heads, head_dim
-    pages, blocks, code = _check_attention_kv4("attention_kv4_weights", q, pool, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q,
-                                               max_context, nq, nkv, d, window)
+    pages, blocks, code, T, width = _check_attention_kv4("attention_kv4_weights", q, pool, cu_seqlens_q, context_lens, block_table, num_seqs,
+                                                         max_seqlen_q, max_context, nq, nkv, d, window)
     _cuda_contig("attention_kv4_weights: lse", lse, torch.float32)
-    if lse.numel() != q.shape[0] * nq:
-        raise KernelError(f"attention_kv4_weights: lse must have {q.shape[0] * nq} entries, got {lse.numel()}")
+    if lse.numel() != T * nq:
+        raise KernelError(f"attention_kv4_weights: lse must have {T * nq} entries, got {lse.numel()}")
     _kv4_sums("attention_kv4_weights", sums, pool)
-    _, run, _ = _attention_kv4_fns(d)
-    _check("attention_kv4_weights", run(
+    _check("attention_kv4_weights", _attention_kv4_fns(d)[1](
         q.data_ptr(), code, pool.data_ptr(), lse.data_ptr(), sums.data_ptr(), cu_seqlens_q.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(),
-        block_table.shape[1], blocks, pages, q.shape[0], num_seqs, max_seqlen_q, max_context, nq, nkv, float(scale), int(window), _stream()))
+        width, blocks, pages, T, num_seqs, max_seqlen_q, max_context, nq, nkv, scale, window, _stream()))
 
 
 def kv4_evict(pool: torch.Tensor, sums: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor, num_seqs: int,

@@ -38,6 +38,43 @@ __device__ __forceinline__ void read_group<__nv_bfloat16>(const __nv_bfloat16* p
   }
 }
 
+// 16 values to codes (returned in w) and their scale's byte.
+__device__ __forceinline__ uint32_t quantise(const float (&x)[16], uint2& w) {
+  float amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(amax) : "f"(fabsf(x[j])));
+  uint32_t half[2] = {0u, 0u};
+  const float t = amax / 7.f;
+  if (t >= 6.103515625e-05f && t < 8192.f) {
+    // A normal scale: |x / s| stays below 7.5.  The quotient is rounded as a division would: with inv = 1/s rounded, q = x inv, then q + (x - q s) inv,
+    // whose remainder is exact.  Adding 1.5 * 2^23 + 8 rounds it to a whole number, ties to even, and leaves the code in the low bits.
+    const uint32_t byte = scale_byte(amax);
+    const float s = scale_of(byte), inv = 1.f / s;
+#pragma unroll
+    for (int j = 15; j >= 0; --j) {
+      float q = x[j] * inv;
+      q = fmaf(fmaf(-q, s, x[j]), inv, q);
+      half[j / 8] = (half[j / 8] << 4) | (__float_as_uint(q + 12582920.f) & 15u);
+    }
+    w = make_uint2(half[0], half[1]);
+    return byte;
+  }
+  // NaN, infinities, the smallest and the largest scales
+  float y[16];
+  amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    y[j] = x[j] == x[j] ? x[j] : 0.f;
+    amax = fmaxf(amax, fabsf(y[j]));
+  }
+  const uint32_t byte = scale_byte(amax);
+  const float s = byte ? scale_of(byte) : 1.f;  // (a scale of zero: the whole group rounds to zero)
+#pragma unroll
+  for (int j = 15; j >= 0; --j) half[j / 8] = (half[j / 8] << 4) | (byte ? (uint32_t)(__float2int_rn(fminf(fmaxf(y[j] / s, -7.f), 7.f)) + 8) : 8u);
+  w = make_uint2(half[0], half[1]);
+  return byte;
+}
+
 // A thread takes the 16 channels of one group: their largest, the scale, the codes, 8 + 1 bytes out.  `width` threads (32 or 128) go over the
 // groups of a token, keys first: 32 keep their loads apart from one another's and need few threads, 128 wait once when there are few tokens.
 template <typename T>
@@ -65,89 +102,64 @@ __global__ void __launch_bounds__(128) store_kernel(const T* k, const T* v, long
       const int i = first + a * width;
       if (i >= 2 * units) break;
       const int unit = i < units ? i : i - units, head = unit >> log_groups, grp = unit & (groups - 1);
-      float amax = 0.f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (x[a][j] != x[a][j]) x[a][j] = 0.f;
-        amax = fmaxf(amax, fabsf(x[a][j]));
-      }
-      // The code is round(x / s), found without 16 divisions: c is the rounded product with 1/s, which is off by one at most and only where
-      // x / s lies next to a half; r = x - c s is exact enough to tell (one rounding), and a tie goes to the even code.
-      const uint32_t byte = scale_byte(amax);
-      const float s = byte ? scale_of(byte) : 1.f, inv = 1.f / s, half = 0.5f * s;  // (a scale of zero: the whole group rounds to zero)
-      uint32_t w[2] = {0u, 0u};
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        float c = rintf(fminf(fmaxf(x[a][j] * inv, -7.f), 7.f));
-        const float r = fmaf(-c, s, x[a][j]);
-        const bool odd = ((int)c & 1) != 0;
-        if (fabsf(r) > half || (odd && fabsf(r) == half)) c += copysignf(1.f, r);
-        const int code = byte ? (int)fminf(fmaxf(c, -7.f), 7.f) + 8 : 8;
-        w[j / 8] |= (uint32_t)code << (4 * (j % 8));
-      }
+      uint2 w;
+      const uint32_t byte = quantise(x[a], w);
       uint8_t* rec = records + (size_t)head * page_blocks * (18 * d) + (i < units ? 0 : 9 * d);
-      *reinterpret_cast<uint2*>(rec + row * (d / 2) + grp * 8) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(rec + row * (d / 2) + grp * 8) = w;
       rec[8 * d + row * groups + grp] = (uint8_t)byte;
       if (sums != nullptr && i < units && grp == 0) sums[((size_t)page * nkv + head) * page_size + in_page] = 0.f;  // it has gathered no weight
     }
   }
 }
 
-// 16 codes and their scale as 16 bfloat16 in order.
-__device__ __forceinline__ void kv4_unpack(uint2 code, uint32_t scale, uint4 (&out)[2]) {
+// Eight codes as values: bfloat16 in order.
+__device__ __forceinline__ uint4 kv4_unpack(uint32_t x, uint32_t scale) {
   __nv_bfloat162 f, c;
   kv4_factors(scale, scale, f, c);
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const uint32_t x = j ? code.y : code.x;
-    const uint32_t p0 = kv4_pair(x << 3, f, c), p1 = kv4_pair(x >> 1, f, c), p2 = kv4_pair(x >> 5, f, c), p3 = kv4_pair(x >> 9, f, c);
-    out[j] = make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
-  }
+  const uint32_t p0 = kv4_pair(x << 3, f, c), p1 = kv4_pair(x >> 1, f, c), p2 = kv4_pair(x >> 5, f, c), p3 = kv4_pair(x >> 9, f, c);
+  return make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
 }
 
+// A thread takes eight channels: 4 + 1 bytes in, one store of 16 bytes of bfloat16 out, a warp's stores one behind the other.
 template <typename T>
 __global__ void __launch_bounds__(128) load_kernel(const uint8_t* pool, const int* slots, T* k, T* v, int rows, int nkv, int log_groups, int page_blocks,
                                                    int num_slots, int width) {
   ts_pdl_prologue();
-  const int groups = 1 << log_groups, d = 16 * groups, units = nkv << log_groups;
+  const int log_words = log_groups + 1, d = 8 << log_words, units = nkv << log_words;  // units of 8 channels
   const int row = blockIdx.x * (128 / width) + threadIdx.x / width;
   if (row >= rows) return;
   const int slot = slots[row];
   const bool there = slot >= 0 && slot < num_slots;
   const int page_size = page_blocks * KV4_BLOCK, page = there ? slot / page_size : 0, in_page = there ? slot % page_size : 0, at = in_page % KV4_BLOCK;
   const uint8_t* records = pool + ((size_t)page * nkv * page_blocks + in_page / KV4_BLOCK) * (18 * d);
-  T *to_k = k + (size_t)row * units * 16, *to_v = v + (size_t)row * units * 16;
-  constexpr int kAhead = 4;
+  T *to_k = k + (size_t)row * units * 8, *to_v = v + (size_t)row * units * 8;
+  constexpr int kAhead = 8;
   for (int first = threadIdx.x % width; first < 2 * units; first += kAhead * width) {
-    uint2 code[kAhead];
-    uint32_t scale[kAhead];
+    uint32_t code[kAhead], scale[kAhead];
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
-      const int i = first + a * width, unit = i < units ? i : i - units, grp = unit & (groups - 1);
-      code[a] = make_uint2(0u, 0u), scale[a] = 0u;
+      const int i = first + a * width, unit = i < units ? i : i - units, word = unit & ((1 << log_words) - 1);
+      code[a] = scale[a] = 0u;
       if (there && i < 2 * units) {
-        const uint8_t* rec = records + (size_t)(unit >> log_groups) * page_blocks * (18 * d) + (i < units ? 0 : 9 * d);
-        code[a] = *reinterpret_cast<const uint2*>(rec + at * (d / 2) + grp * 8);
-        scale[a] = rec[8 * d + at * groups + grp];
+        const uint8_t* rec = records + (size_t)(unit >> log_words) * page_blocks * (18 * d) + (i < units ? 0 : 9 * d);
+        code[a] = *reinterpret_cast<const uint32_t*>(rec + at * (d / 2) + word * 4);
+        scale[a] = rec[8 * d + at * (d / 16) + word / 2];
       }
     }
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
       const int i = first + a * width;
       if (i >= 2 * units) break;
-      T* dst = i < units ? to_k + i * 16 : to_v + (i - units) * 16;
+      T* dst = i < units ? to_k + i * 8 : to_v + (i - units) * 8;
       if constexpr (sizeof(T) == 2) {
-        uint4 out[2];
-        kv4_unpack(code[a], scale[a], out);
-        reinterpret_cast<uint4*>(dst)[0] = out[0], reinterpret_cast<uint4*>(dst)[1] = out[1];
+        *reinterpret_cast<uint4*>(dst) = kv4_unpack(code[a], scale[a]);
       } else {
         const float s = scale_of(scale[a]);
+        const uint32_t c = code[a];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t c = (j < 2 ? code[a].x : code[a].y) >> (16 * (j & 1));
-          reinterpret_cast<float4*>(dst)[j] = make_float4((float)((int)(c & 15u) - 8) * s, (float)((int)(c >> 4 & 15u) - 8) * s,
-                                                          (float)((int)(c >> 8 & 15u) - 8) * s, (float)((int)(c >> 12 & 15u) - 8) * s);
-        }
+        for (int j = 0; j < 2; ++j)
+          reinterpret_cast<float4*>(dst)[j] = make_float4((float)((int)(c >> (16 * j) & 15u) - 8) * s, (float)((int)(c >> (16 * j + 4) & 15u) - 8) * s,
+                                                          (float)((int)(c >> (16 * j + 8) & 15u) - 8) * s, (float)((int)(c >> (16 * j + 12) & 15u) - 8) * s);
       }
     }
   }
@@ -160,7 +172,7 @@ __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* pool, const 
                                                      uint4* v, int* out_table, int* out_lens, int nkv, int page_blocks, int num_pages, int blocks,
                                                      int window) {
   ts_pdl_prologue();
-  constexpr int kGroups = kExpandDim / 16, kUnits = kExpandRows * kGroups * 2 / 256;
+  constexpr int kWords = kExpandDim / 8, kUnits = kExpandRows * kWords * 2 / 256;
   const int b = blockIdx.z, head = blockIdx.y, first = blockIdx.x * kExpandRows;
   const int n = min(context[b], min(table_stride * page_blocks * KV4_BLOCK, blocks * kExpandPage));
   if (head == 0 && threadIdx.x == 0) {
@@ -169,25 +181,21 @@ __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* pool, const 
   }
   const int queries = cu[b + 1] - cu[b], oldest = window > 0 ? n - queries - window + 1 : 0;  // the first key that some query sees
   if (first >= n || first + kExpandRows <= oldest || queries <= 0) return;
-  uint2 code[kUnits];
-  uint32_t scale[kUnits];
+  uint32_t code[kUnits], scale[kUnits];
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
-    const int unit = threadIdx.x + 256 * i, grp = unit % kGroups, values = unit / (kExpandRows * kGroups);
-    const int row = min(first + unit / kGroups % kExpandRows, n - 1), blk = row / KV4_BLOCK;
+    const int unit = threadIdx.x + 256 * i, word = unit % kWords, values = unit / (kExpandRows * kWords);
+    const int row = min(first + unit / kWords % kExpandRows, n - 1), blk = row / KV4_BLOCK;
     const int page = min(max(table[(size_t)b * table_stride + blk / page_blocks], 0), num_pages - 1);
     const uint8_t* rec = pool + (((size_t)page * nkv + head) * page_blocks + blk % page_blocks) * (18 * kExpandDim) + values * 9 * kExpandDim;
-    code[i] = *reinterpret_cast<const uint2*>(rec + row % KV4_BLOCK * (kExpandDim / 2) + grp * 8);
-    scale[i] = rec[8 * kExpandDim + row % KV4_BLOCK * kGroups + grp];
+    code[i] = *reinterpret_cast<const uint32_t*>(rec + row % KV4_BLOCK * (kExpandDim / 2) + word * 4);
+    scale[i] = rec[8 * kExpandDim + row % KV4_BLOCK * (kExpandDim / 16) + word / 2];
   }
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
-    const int unit = threadIdx.x + 256 * i, grp = unit % kGroups, values = unit / (kExpandRows * kGroups);
-    const int row = first + unit / kGroups % kExpandRows;
-    uint4 out[2];
-    kv4_unpack(code[i], scale[i], out);
-    uint4* dst = (values ? v : k) + (((size_t)b * blocks * kExpandPage + row) * nkv + head) * (kExpandDim / 8) + grp * 2;
-    if (row < n) dst[0] = out[0], dst[1] = out[1];
+    const int unit = threadIdx.x + 256 * i, word = unit % kWords, values = unit / (kExpandRows * kWords);
+    const int row = first + unit / kWords % kExpandRows;
+    if (row < n) (values ? v : k)[(((size_t)b * blocks * kExpandPage + row) * nkv + head) * kWords + word] = kv4_unpack(code[i], scale[i]);
   }
 }
 

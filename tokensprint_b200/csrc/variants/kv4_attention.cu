@@ -184,18 +184,22 @@ struct RowSum {
 // The key ranges of all (sequence, row tile) pairs, counted in steps of kRecords records, one behind the other; every key head has them again.
 // A CTA's share is an equal part of all of them, whatever the lengths are, and may begin and end inside a range.
 struct Shares {
-  int before[kMaxTiles + 1];  // steps of one head before the pair
+  int* before;  // [pairs + 1]: steps of one head before the pair
 };
 
 template <typename T, int kTiles, int kQ, int kP, int kRecords>
 __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : kTiles == 1 ? X_CTAS : X_CTAS2) attention_kernel(const Params p) {
   constexpr int kRows = 8 * kTiles;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ Shares shares;
   __shared__ int scratch[kWarps + 2];
   ts_pdl_prologue();
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   const int pairs = p.num_seqs * p.row_tiles;
+  uint4* sq = reinterpret_cast<uint4*>(smem + kWarps * kRing * Rec::kBytes);  // the queries: [tiles][parts][words][lanes]
+  float* so = reinterpret_cast<float*>(sq + kTiles * kQ * D);                 // the warps' parts: [warps][rows][D]
+  float* sm = so + kWarps * kRows * D;                                        // [warps][rows]
+  float* sl = sm + kWarps * kRows;
+  const Shares shares = {reinterpret_cast<int*>(sl + kWarps * kRows)};
 
   auto open = [&](Tile& tile, int pair, int head) {
     tile.open(p, pair / p.row_tiles, head);
@@ -307,10 +311,6 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch();
 
-  uint4* sq = reinterpret_cast<uint4*>(smem + kWarps * kRing * Rec::kBytes);                  // [tiles][parts][words][lanes]
-  float* so = reinterpret_cast<float*>(sq + kTiles * kQ * D);                                 // [warps][rows][D]
-  float* sm = so + kWarps * kRows * D;                                                        // [warps][rows]
-  float* sl = sm + kWarps * kRows;
   int done = 0;  // steps worked on
   for (int seg = begin; seg < end;) {
     const int pair = pair_of(seg), n_pair = shares.before[pair + 1] - shares.before[pair];
@@ -724,23 +724,26 @@ int launch_weights(const Params& p, float* sums, int num_seqs, int max_context, 
 
 template <typename T, int kTiles, int kQ, int kP, int kRecords>
 struct Attention {
-  static constexpr int kSmem = kWarps * kRing * Rec::kBytes + kTiles * kQ * D * 16 + kWarps * 8 * kTiles * (D + 2) * 4;
-  // CTAs that run at once on the device, or a negative error
+  static constexpr int kSmem = kWarps * kRing * Rec::kBytes + kTiles * kQ * D * 16 + kWarps * 8 * kTiles * (D + 2) * 4;  // and 4 bytes per pair
+  static constexpr int kFewPairs = 256;
+  // CTAs that run at once on the device (with at most kFewPairs pairs), or a negative error
   static int ctas() {
     static int n = 0;
     if (n == 0) {
       int device = 0, sms = 0, per_sm = 0;
-      cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kTiles, kQ, kP, kRecords>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+      cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kTiles, kQ, kP, kRecords>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           kSmem + (kMaxTiles + 1) * 4);
       if (e == cudaSuccess) e = cudaGetDevice(&device);
       if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-      if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_kernel<T, kTiles, kQ, kP, kRecords>, kWarps * 32, kSmem);
+      if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_kernel<T, kTiles, kQ, kP, kRecords>, kWarps * 32,
+                                                                                kSmem + (kFewPairs + 1) * 4);
       if (e != cudaSuccess) return -(int)e - 100;
       n = sms * (per_sm > 0 ? per_sm : 1);
     }
     return n;
   }
   static int launch(const Params& p, int grid, cudaStream_t stream) {
-    return ts_launch(attention_kernel<T, kTiles, kQ, kP, kRecords>, dim3(grid), dim3(kWarps * 32), kSmem, stream, p);
+    return ts_launch(attention_kernel<T, kTiles, kQ, kP, kRecords>, dim3(grid), dim3(kWarps * 32), kSmem + (p.num_seqs * p.row_tiles + 1) * 4, stream, p);
   }
 };
 

@@ -2729,6 +2729,7 @@ def attention_kv4(
 
 
 _KV4_EXPAND_PAGE = 128
+_KV4_MODE = 0
 
 
 def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, scale, window, head_sinks,
@@ -2762,7 +2763,7 @@ def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_tabl
             table.data_ptr(), kept_lens.data_ptr(), n, nkv, pool_blocks, pages, blocks, int(window), _stream()))
         _check("attention_kv4", run(
             q.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), out.data_ptr(), cu.data_ptr(), kept_lens.data_ptr(), table.data_ptr(), blocks, page,
-            group * blocks * page, q.shape[0], n, max_seqlen_q, nq, nkv, float(scale), int(window), 0, 0, 0.0, 0.0, _ptr(head_sinks), 0, error.data_ptr(),
+            group * blocks * page, q.shape[0], n, max_seqlen_q, nq, nkv, float(scale), int(window), 0, 0, 0.0, 0.0, _ptr(head_sinks), _KV4_MODE, error.data_ptr(),
             _stream(), None, None, _ptr(lse)))
 
 

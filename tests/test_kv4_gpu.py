@@ -234,6 +234,13 @@ def test_long_portion_uses_the_same_numbers():
     check_attention([(700, 512), (300, 260)], 4, 2, 128, 64, torch.bfloat16)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, False), (0, True), (300, False), (130, True)])
+def test_few_rows_over_many_keys(window, sinks):
+    """Portions whose keys are cut into runs that are joined afterwards; some requests have fewer runs than others, one has no rows."""
+    check_attention([(1700, 30), (260, 40), (0, 0), (1024, 1), (50, 50)], 4, 1, 128, 16, torch.bfloat16, window=window, sinks=sinks)
+    check_attention([(900, 150)], 5, 1, 128, 16, torch.bfloat16, window=window, sinks=sinks)
+
+
 def test_portions_in_groups(monkeypatch):
     """Requests whose unpacked rows do not fit the workspace at once are taken in groups."""
     monkeypatch.setattr(ops, "ATTENTION_KV4_EXPAND_BYTES", 2 * 128 * 2 * 3 * 128 * 2 * 2)  # two requests of three pages

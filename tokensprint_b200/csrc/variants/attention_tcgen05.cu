@@ -68,7 +68,8 @@ constexpr int MAX_TABLE = 1024;                   // block-table entries kept in
 #define TS_ATT_SCORED 0
 #endif
 [[maybe_unused]] constexpr bool SCORED = TS_ATT_SCORED != 0;
-// Builds with TS_ATT_LSE=1 also write the logarithm of every row's softmax denominator.
+// Builds with TS_ATT_LSE=1 also write the logarithm of every row's softmax denominator, and may cut the keys of a pair of tiles
+// into runs of blocks, a CTA each, whose results a second kernel joins by those logarithms (see "Runs of blocks").
 #ifndef TS_ATT_LSE
 #define TS_ATT_LSE 0
 #endif
@@ -90,7 +91,11 @@ struct Params {
   const float* dist_r2;
 #endif
 #if TS_ATT_LSE
-  float* lse;  // [T, nq], or null
+  float* lse;      // [T, nq], or null
+  int run_blocks;  // > 0: a CTA takes that many key blocks, and leaves a float32 row and its logarithm
+  int runs, tokens;
+  float* run_out;  // [runs, T, nq, D]
+  float* run_lse;  // [runs, T, nq]
 #endif
 #if TS_ATT_ROT
   const float* gates;  // [T, nq] what a finished row is multiplied by, or null
@@ -284,7 +289,7 @@ __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn_major) {
          ((uint32_t)(BM >> 4) << 24);
 }
 
-#if TS_ATT_ROT == 0
+#if TS_ATT_ROT == 0 && !TS_ATT_LSE
 __global__ void __launch_bounds__(128, 2) attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                    const __grid_constant__ CUtensorMap map_k,
                                                                    const __grid_constant__ CUtensorMap map_v,
@@ -542,9 +547,6 @@ __global__ void __launch_bounds__(128, 2) attention_tcgen05_kernel(const __grid_
   __syncthreads();
   if (abort_s == 0 && tid < RT && r < rows_total) {
     const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-#if TS_ATT_LSE
-    if (p.lse != nullptr) p.lse[(size_t)(q_begin + r / G) * p.nq + hk * G + r % G] = row_lse(p, m_run, l_run);
-#endif
     __nv_bfloat16* dst = p.out + ((size_t)(q_begin + r / G) * p.nq + hk * G + r % G) * D;
 #pragma unroll
     for (int c = 0; c < D / 8; ++c) {
@@ -565,7 +567,7 @@ __global__ void __launch_bounds__(128, 2) attention_tcgen05_kernel(const __grid_
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
   }
 }
-#endif  // TS_ATT_ROT == 0
+#endif  // TS_ATT_ROT == 0 && !TS_ATT_LSE
 
 // ---------------------------------------------------------------------------
 // Two tiles per CTA, roles in warps of their own (long prompt portions).
@@ -735,7 +737,12 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // the CTAs with the most keys to walk are launched first (see the other kernel)
-  const int hk = blockIdx.x % p.nkv, b = (blockIdx.x / p.nkv) % p.num_seqs;
+#if TS_ATT_LSE
+  const int cta = blockIdx.x / p.runs, run = blockIdx.x % p.runs;
+#else
+  const int cta = blockIdx.x;
+#endif
+  const int hk = cta % p.nkv, b = (cta / p.nkv) % p.num_seqs;
   const int G = p.nq / p.nkv;
   const int q_begin = p.cu_q[b];
   const int q_len = p.cu_q[b + 1] - q_begin;
@@ -744,7 +751,7 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
   const int rows_total = q_len * G;
   const int RT = (BM / G) * G;  // rows of a tile that belong to tokens (see the other kernel)
   const int seq_pairs = (rows_total + 2 * RT - 1) / (2 * RT);
-  const int pair = seq_pairs - 1 - (int)(blockIdx.x / (p.nkv * p.num_seqs));
+  const int pair = seq_pairs - 1 - cta / (p.nkv * p.num_seqs);
   if (q_len <= 0 || pair < 0) return;
   const int r0 = pair * 2 * RT;
   const int ntiles = rows_total - r0 > RT ? 2 : 1;
@@ -752,11 +759,17 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
   // the last key any row of the pair sees, and how many key blocks the pair walks
   const int first_pos = start_pos + r0 / G;
   const int lo = first_visible_key(p, first_pos);
-  const int kb0 = lo / PBN;
   const int hi = start_pos + (min(r0 + ntiles * RT, rows_total) - 1) / G;
   // Both tiles walk all blocks of the later one (its last block may be fully masked for the
   // earlier tile): the two tiles stay in step.
+#if TS_ATT_LSE
+  const int kb0 = lo / PBN + run * p.run_blocks;
+  const int nblocks = p.run_blocks > 0 ? min(hi / PBN - kb0 + 1, p.run_blocks) : hi / PBN - kb0 + 1;
+  if (run > 0 && nblocks <= 0) return;
+#else
+  const int kb0 = lo / PBN;
   const int nblocks = hi / PBN - kb0 + 1;
+#endif
 #if TS_ATT_ROT == 0
   const int box_rows = min(p.page, PBN);
   const int copies_per_block = PBN / box_rows;
@@ -1002,7 +1015,12 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
     const uint32_t o_addr = lane_addr + 256 + t * 128 + h * 64;  // its half of the row of O
     // l_run: the sum over this thread's keys only; with a sink both threads of a row start from its score
     // and one of them holds its share of the sum
-    float m_run = p.has_sink ? row_sink_raw(p, hk, G, r) : -INFINITY, l_run = (p.has_sink && h == 0) ? 1.f : 0.f;
+#if TS_ATT_LSE
+    const bool sink_here = p.has_sink && run == 0;
+#else
+    const bool sink_here = p.has_sink;
+#endif
+    float m_run = sink_here ? row_sink_raw(p, hk, G, r) : -INFINITY, l_run = (sink_here && h == 0) ? 1.f : 0.f;
     bool ok = true;
 
     for (int blk = 0; blk < nblocks; ++blk) {
@@ -1182,13 +1200,41 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
     l_run += sum_s[t][h ^ 1][row];
     float inv = l_run > 0.f ? 1.f / l_run : 0.f;
 #if TS_ATT_LSE
-    if (p.lse != nullptr && good && h == 0 && row < RT && r < rows_total) p.lse[(size_t)(q_begin + r / G) * p.nq + hk * G + r % G] = row_lse(p, m_run, l_run);
+    if (good && row < RT && r < rows_total) {
+      const size_t at = (size_t)(q_begin + r / G) * p.nq + hk * G + r % G;
+      if (p.run_blocks > 0) {  // a run's row, as it is in 32 bits
+        const size_t of_run = (size_t)run * p.tokens * p.nq + at;
+        if (h == 0) p.run_lse[of_run] = row_lse(p, m_run, l_run);
+      } else if (p.lse != nullptr && h == 0) {
+        p.lse[at] = row_lse(p, m_run, l_run);
+      }
+    }
+    if (good && p.run_blocks > 0) {
+      const size_t of_run = (size_t)run * p.tokens * p.nq + (size_t)(q_begin + r / G) * p.nq + hk * G + r % G;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t v[32];
+        tmem_ld32(o_addr + c * 32, v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (row < RT && r < rows_total) {
+          float4* dst = reinterpret_cast<float4*>(p.run_out + of_run * D + h * 64 + c * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            dst[i] = make_float4(__uint_as_float(v[4 * i]) * inv, __uint_as_float(v[4 * i + 1]) * inv, __uint_as_float(v[4 * i + 2]) * inv,
+                                 __uint_as_float(v[4 * i + 3]) * inv);
+        }
+      }
+    }
+    const bool good_here = good && p.run_blocks == 0;
+#else
+    const bool good_here = good;
 #endif
 #if TS_ATT_ROT
     if (p.gates != nullptr && row_pos >= 0) inv *= p.gates[(size_t)(q_begin + r) * p.nq + hk];
 #endif
     unsigned char* o_tile = smem + P2_OFF_Q + t * PQ_BYTES;
-    if (good) {
+    if (good_here) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       // The tile goes through shared memory (where its Q lay: the tensor core is done with it), so
       // that rows leave as whole 256-byte lines: row `row` at row * 256, its 16-byte piece c at
@@ -1210,7 +1256,7 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
       }
     }
     asm volatile("bar.sync %0, 256;" ::"r"(1 + t) : "memory");
-    if (good) {
+    if (good_here) {
       const int me = h * BM + row;  // 0..255 among the tile's threads
 #pragma unroll 4
       for (int it = 0; it < 8; ++it) {
@@ -1310,6 +1356,39 @@ TS_EXPORT int ts_latent_rebuilt_attention(const void* q, long long ld_q, const v
 
 #else  // paged keys and values
 
+#if TS_ATT_LSE
+// Runs of blocks.  Few rows over many keys leave most of the device without a CTA (64 CTAs of 256 rows walk 16 blocks each in 45 us while 84
+// SMs wait).  So a pair's keys may be cut into runs; the rows of a run are whole softmaxes of their keys, and a row is their
+// average, weighted by 2^(lse - the largest lse).  A warp joins the runs of one (token, head), always in the same order.
+__global__ void __launch_bounds__(256) join_runs_kernel(const Params p) {
+  ts_pdl_prologue();
+  const int b = blockIdx.y, lane = threadIdx.x & 31, index = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int q_begin = p.cu_q[b], q_len = p.cu_q[b + 1] - q_begin, G = p.nq / p.nkv;
+  const int token = index / p.nq, head = index % p.nq;
+  if (token >= q_len) return;
+  // how many runs the row's pair of tiles has (as its CTAs work it out)
+  const int start_pos = p.ctx_len[b] - q_len, rows_total = q_len * G, RT = (BM / G) * G;
+  const int r0 = (token * G + head % G) / (2 * RT) * (2 * RT);
+  const int lo = first_visible_key(p, start_pos + r0 / G), hi = start_pos + (min(r0 + 2 * RT, rows_total) - 1) / G;
+  const int runs = min(max(1, (hi / PBN - lo / PBN + p.run_blocks) / p.run_blocks), p.runs);
+  const size_t at = (size_t)(q_begin + token) * p.nq + head, step = (size_t)p.tokens * p.nq;
+  float top = -INFINITY;
+  for (int i = 0; i < runs; ++i) top = fmaxf(top, p.run_lse[at + i * step]);
+  float sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < runs; ++i) {
+    const float f = top == -INFINITY ? 0.f : fast_exp2((p.run_lse[at + i * step] - top) * 1.4426950408889634f);
+    const float4 v = *reinterpret_cast<const float4*>(p.run_out + (at + i * step) * D + lane * 4);
+    sum += f;
+    o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+  }
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  *reinterpret_cast<uint2*>(p.out + at * D + lane * 4) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  if (lane == 0 && p.lse != nullptr) p.lse[at] = sum > 0.f ? top + logf(sum) : -INFINITY;
+}
+#endif
+
 // q [T, nq, D] as a 4-d tensor {D, G, nkv, T}; boxes of {64, G, 1, 128 / G}: the rows of a box
 // come out ordered (token, head of the group), which is the tile's row order.
 int query_map(const void* ptr, long long T, int nq, int nkv, CUtensorMap* out) {
@@ -1367,7 +1446,7 @@ TS_EXPORT int ts_attention_prefill_tcgen05_scored(const void* q, const void* kca
                                                   const float* dist_r1, const float* dist_r2
 #if TS_ATT_LSE
                                                   ,
-                                                  float* lse
+                                                  float* lse, int runs, int run_blocks, float* run_out, float* run_lse
 #endif
 ) {
   if (T <= 0 || B <= 0) return 0;
@@ -1406,12 +1485,24 @@ TS_EXPORT int ts_attention_prefill_tcgen05_scored(const void* q, const void* kca
   p.scale_log2 = scale * 1.4426950408889634f;
   p.probe = probe_buffer;
 #if TS_ATT_LSE
+  if (runs < 1 || (runs > 1) != (run_blocks > 0)) return TS_ERR_BAD_ARGUMENT;
   p.lse = lse;
+  p.runs = runs;
+  p.run_blocks = run_blocks;
+  p.tokens = T;
+  p.run_out = run_out;
+  p.run_lse = run_lse;
+#else
+  const int runs = 1;
 #endif
   const int G = nq / nkv;
   const int RT = (BM / G) * G;  // rows of a tile that belong to tokens
   const long long rows = (long long)max_q * G;
+#if TS_ATT_LSE
+  const bool pairs = true;  // (one tile of rows in a CTA of two is no slower than the other kernel, which has no runs)
+#else
   const bool pairs = mode == 2 || (mode == 0 && rows > RT);
+#endif
   const int block_keys = pairs ? PBN : BN;  // keys per copy: a whole page, or a block's worth of a larger one
   CUtensorMap mq, mk, mv;
   int st = query_map(q, T, nq, nkv, &mq);
@@ -1428,9 +1519,15 @@ TS_EXPORT int ts_attention_prefill_tcgen05_scored(const void* q, const void* kca
       if (e != cudaSuccess) return (int)e;
       configured = true;
     }
-    return ts_launch(attention_tcgen05_pair_kernel, dim3((unsigned)(((rows + 2 * RT - 1) / (2 * RT)) * nkv * B)), dim3(608), smem,
-                     (cudaStream_t)stream_, mq, mk, mv, p);
+    const int status = ts_launch(attention_tcgen05_pair_kernel, dim3((unsigned)(((rows + 2 * RT - 1) / (2 * RT)) * nkv * B * runs)), dim3(608), smem,
+                                 (cudaStream_t)stream_, mq, mk, mv, p);
+#if TS_ATT_LSE
+    if (status == 0 && runs > 1)
+      return ts_launch(join_runs_kernel, dim3((unsigned)(((long long)max_q * nq + 7) / 8), B), dim3(256), 0, (cudaStream_t)stream_, p);
+#endif
+    return status;
   }
+#if !TS_ATT_LSE
   const size_t smem = SMEM_TILES + 1024;
   static bool configured = false;
   if (!configured) {
@@ -1440,6 +1537,7 @@ TS_EXPORT int ts_attention_prefill_tcgen05_scored(const void* q, const void* kca
   }
   return ts_launch(attention_tcgen05_kernel, dim3((unsigned)(((rows + RT - 1) / RT) * nkv * B)), dim3(128), smem, (cudaStream_t)stream_, mq, mk,
                    mv, p);
+#endif
 }
 
 #if !TS_ATT_LSE

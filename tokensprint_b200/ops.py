@@ -2729,7 +2729,7 @@ def attention_kv4(
 
 
 _KV4_EXPAND_PAGE = 128
-_KV4_MODE = 0
+_KV4_MIN_RUN = 3  # least key blocks of a run
 
 
 def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, scale, window, head_sinks,
@@ -2744,7 +2744,7 @@ def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_tabl
         # (the denominators are an output here: every weight from the special-function unit, none from the cubic)
         lib = _build.load_variant("attention_tcgen05", {"TS_HEAD_DIM": d, "TS_ATT_LSE": 1, "TS_ATT_FMA_PAIRS": 0, "TS_ATT_SCORED": int(scored)})
         run = lib.ts_attention_prefill_tcgen05_scored
-        run.argtypes = _attention_tcgen05_fns()[0].argtypes + [_c_void_p]
+        run.argtypes = _attention_tcgen05_fns()[0].argtypes + [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p]
         run.restype = _c_int
         _attention_kv4_tcgen05[scored] = run
     blocks = -(-max_context // page)
@@ -2754,6 +2754,16 @@ def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_tabl
     rows = torch.empty((2, group * blocks, page, nkv, d), device=q.device, dtype=torch.bfloat16)
     table = torch.empty(group * (blocks + 1), device=q.device, dtype=torch.int32)  # and behind it the lengths
     kept_lens = table[group * blocks :]
+    # Few rows over many keys: the keys of every 256 rows are cut into runs, as many as the device has room for, of at least _KV4_MIN_RUN blocks.
+    T, G = q.shape[0], nq // nkv
+    ctas = -(-max_seqlen_q * G // (2 * (128 // G) * G)) * nkv * group
+    seen = -(-min(max_context, window + max_seqlen_q + page) // page) if window else blocks
+    runs = max(1, min(seen // _KV4_MIN_RUN, _sm_count(q.device) // ctas))
+    run_blocks = -(-seen // runs) if runs > 1 else 0
+    runs = -(-seen // run_blocks) if runs > 1 else 1
+    run_out = torch.empty(runs * T * nq * (d + 1), device=q.device, dtype=torch.float32) if runs > 1 else None
+    run_at = _ptr(run_out)
+    run_lse_at = None if run_out is None else run_at + runs * T * nq * d * 4
     _, error = _gemm_workspace(q.device)
     for lo in range(0, num_seqs, group):
         n = min(group, num_seqs - lo)
@@ -2763,8 +2773,8 @@ def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_tabl
             table.data_ptr(), kept_lens.data_ptr(), n, nkv, pool_blocks, pages, blocks, int(window), _stream()))
         _check("attention_kv4", run(
             q.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), out.data_ptr(), cu.data_ptr(), kept_lens.data_ptr(), table.data_ptr(), blocks, page,
-            group * blocks * page, q.shape[0], n, max_seqlen_q, nq, nkv, float(scale), int(window), 0, 0, 0.0, 0.0, _ptr(head_sinks), _KV4_MODE, error.data_ptr(),
-            _stream(), None, None, _ptr(lse)))
+            group * blocks * page, T, n, max_seqlen_q, nq, nkv, float(scale), int(window), 0, 0, 0.0, 0.0, _ptr(head_sinks), 0, error.data_ptr(),
+            _stream(), None, None, _ptr(lse), runs, run_blocks, run_at, run_lse_at))
 
 
 def attention_kv4_weights(

@@ -48,6 +48,14 @@ __device__ __forceinline__ void kv4_factors(uint32_t a, uint32_t b, __nv_bfloat1
   c = __hmul2(v, __float2bfloat162_rn(-1.2461512460483586e+35f));  // -1.5 * 2^116
 }
 
+// Eight codes with their scale as values: bfloat16 in order.
+__device__ __forceinline__ uint4 kv4_unpack(uint32_t x, uint32_t scale) {
+  __nv_bfloat162 f, c;
+  kv4_factors(scale, scale, f, c);
+  const uint32_t p0 = kv4_pair(x << 3, f, c), p1 = kv4_pair(x >> 1, f, c), p2 = kv4_pair(x >> 5, f, c), p3 = kv4_pair(x >> 9, f, c);
+  return make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
+}
+
 // D (float32) += A (bfloat16, 16 x 16, row major) * B (bfloat16, 16 x 8).
 __device__ __forceinline__ void kv4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(

@@ -112,14 +112,6 @@ __global__ void __launch_bounds__(128) store_kernel(const T* k, const T* v, long
   }
 }
 
-// Eight codes as values: bfloat16 in order.
-__device__ __forceinline__ uint4 kv4_unpack(uint32_t x, uint32_t scale) {
-  __nv_bfloat162 f, c;
-  kv4_factors(scale, scale, f, c);
-  const uint32_t p0 = kv4_pair(x << 3, f, c), p1 = kv4_pair(x >> 1, f, c), p2 = kv4_pair(x >> 5, f, c), p3 = kv4_pair(x >> 9, f, c);
-  return make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
-}
-
 // A thread takes eight channels: 4 + 1 bytes in, one store of 16 bytes of bfloat16 out, a warp's stores one behind the other.
 template <typename T>
 __global__ void __launch_bounds__(128) load_kernel(const uint8_t* pool, const int* slots, T* k, T* v, int rows, int nkv, int log_groups, int page_blocks,

@@ -27,6 +27,7 @@
 // Built with TS_ATT_ROT=64 the file holds another kernel made of the same parts: prompt portions of a
 // latent attention whose keys and values have been rebuilt from the cached rows (see "Rebuilt keys").
 #include "../common.cuh"
+#include "../kv4.cuh"
 #include "kv_tensor_map.cuh"
 
 #if TS_HEAD_DIM != 128
@@ -1356,35 +1357,245 @@ TS_EXPORT int ts_latent_rebuilt_attention(const void* q, long long ld_q, const v
 
 #else  // paged keys and values
 
+#if TS_ATT_LSE && !TS_ATT_SCORED
+// The weight that a step's queries give every row of a 4-bit cache, for portions of prompts: sums[key] += sum over the rows r of
+// exp(scale q_r . k - lse_r).  A CTA owns 128 keys of one head, unpacked once into shared memory as the first operand; tiles of 128 query rows come
+// by TMA as the second, so that S^T[key][row] lies in tensor memory with a key per lane: a thread adds up its own key's weights in a
+// register, nothing is exchanged until the end.  What bounds it is the special-function unit, 16 exponentials a clock for 16,384 of a
+// tile; the products take half as long and run on the other buffer meanwhile.
+constexpr int W_STAGES = 2;
+constexpr uint32_t W_OFF_Q = 2 * BM * 128, W_SMEM = W_OFF_Q + W_STAGES * Q_BYTES, W_TMEM_COLS = 256;
+struct WeightParams {
+  const uint8_t* pool;
+  float* sums;
+  const float* lse;
+  const int *cu, *context, *table;
+  int* error;
+  int table_stride, page_blocks, num_pages, tokens, nq, nkv, window;
+  float scale_log2;
+};
+__global__ void __launch_bounds__(320, 2) kv4_weights_kernel(const __grid_constant__ CUtensorMap map_q, const WeightParams p) {
+  ts_pdl_wait();  // (tensor memory is never held while waiting for another kernel)
+  extern __shared__ unsigned char smem_unaligned[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) uint64_t q_full[W_STAGES], q_empty[W_STAGES], s_full[2], s_empty[2];
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int abort_s;
+  __shared__ __align__(16) float lse_s[2][BM];
+  __shared__ __align__(16) int pos_s[2][BM];
+  __shared__ float half_s[BM];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hk = blockIdx.y, b = blockIdx.z, G = p.nq / p.nkv, page_size = p.page_blocks * KV4_BLOCK;
+  const int q_begin = min(max(p.cu[b], 0), p.tokens), q_len = min(max(p.cu[b + 1], q_begin), p.tokens) - q_begin;
+  const int ctx = min(p.context[b], p.table_stride * page_size), before = ctx - q_len, key0 = blockIdx.x * BM;
+  if (key0 >= ctx) return;
+  const int last_key = min(key0 + BM, ctx) - 1, per_tile = BM / G, RT = per_tile * G;
+  const int first_token = max(0, key0 - before);
+  const int end_token = p.window > 0 ? min(q_len, last_key + p.window - before) : q_len;
+  if (first_token >= end_token) return;
+  const int tile0 = first_token / per_tile, tiles = (end_token - 1) / per_tile - tile0 + 1;
+  const int* table = p.table + (size_t)b * p.table_stride;
+
+  if (tid == 0) {
+    abort_s = 0;
+    for (int i = 0; i < W_STAGES; ++i) mbar_init(smem_u32(&q_full[i]), 1), mbar_init(smem_u32(&q_empty[i]), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_full[i]), 1), mbar_init(smem_u32(&s_empty[i]), 8);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(W_TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid < 256) {
+    // the keys, unpacked: 16 bytes (8 channels) at a time to their places in the swizzled operand; keys that are none as zeros
+#pragma unroll
+    for (int i = 0; i < BM * 16 / 256; ++i) {
+      const int x = tid + 256 * i, row = x >> 4, c = x & 15, key = key0 + row;
+      uint4 out = make_uint4(0u, 0u, 0u, 0u);
+      if (key < ctx) {
+        const int page = min(max(table[key / page_size], 0), p.num_pages - 1), in_page = key % page_size;
+        const uint8_t* rec = p.pool + (((size_t)page * p.nkv + hk) * p.page_blocks + in_page / KV4_BLOCK) * Kv4Record<D>::kBytes;
+        const uint32_t code = *reinterpret_cast<const uint32_t*>(rec + in_page % KV4_BLOCK * (D / 2) + c * 4);
+        const uint32_t scale = rec[Kv4Record<D>::kKeyScales + in_page % KV4_BLOCK * (D / 16) + c / 2];
+        out = kv4_unpack(code, scale);
+      }
+      *reinterpret_cast<uint4*>(smem + (c >> 3) * (BM * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = out;
+    }
+    // rows of the query tiles that no copy fills: zeros
+    for (int i = tid; i < W_STAGES * 2 * (BM - RT) * 8; i += 256) {
+      const int half = i / ((BM - RT) * 8), rest = i % ((BM - RT) * 8);
+      *reinterpret_cast<uint4*>(smem + W_OFF_Q + half * (BM * 128) + (RT + rest / 8) * 128 + (rest % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  ts_pdl_launch_dependents();
+  const uint32_t tmem_base = tmem_base_s, sm = smem_u32(smem);
+  volatile int* abort_flag = &abort_s;
+
+  if (warp == 8) {
+    int issued = 0;
+    for (int j = 0; j < tiles; ++j) {
+      const int st = j % W_STAGES;
+      if (j >= W_STAGES && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&q_empty[st]), (uint32_t)(j / W_STAGES - 1) & 1, abort_flag))) break;
+      if (lane == 0) mbar_expect_tx(smem_u32(&q_full[st]), (uint32_t)(2 * RT * 128));
+      __syncwarp();
+      if (lane < 2)
+        tma_load_4d(sm + W_OFF_Q + st * Q_BYTES + lane * (BM * 128), &map_q, smem_u32(&q_full[st]), lane * 64, 0, hk, q_begin + (tile0 + j) * per_tile);
+      issued = j + 1;
+    }
+    // no copy is in flight when the CTA ends, whatever happened (bounded, on a count of its own)
+    int patience = 0;
+    for (int j = max(0, issued - W_STAGES); j < issued; ++j) mbar_wait(smem_u32(&q_full[j % W_STAGES]), (uint32_t)(j / W_STAGES) & 1, &patience);
+    if (patience != 0) *abort_flag = 1;
+  } else if (warp == 9) {
+    const uint64_t k_desc = desc_k_major(sm), q_desc = desc_k_major(sm + W_OFF_Q);
+    int asked = 0;
+    for (int j = 0; j < tiles; ++j) {
+      const int st = j % W_STAGES, buf = j & 1;
+      bool ok = mbar_wait(smem_u32(&q_full[st]), (uint32_t)(j / W_STAGES) & 1, abort_flag);
+      if (ok && j >= 2) ok = mbar_wait(smem_u32(&s_empty[buf]), (uint32_t)(j / 2 - 1) & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (elect_one()) {
+        const uint64_t qd = q_desc + (uint64_t)((st * Q_BYTES) >> 4);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = ((ks >> 2) * (BM * 128) + (ks & 3) * 32) >> 4;
+          if (ks == 0) umma_bf16_first(tmem_base + buf * BM, k_desc + off, qd + off, idesc(BM, false));
+          else umma_bf16_more(tmem_base + buf * BM, k_desc + off, qd + off, idesc(BM, false));
+        }
+        umma_commit(smem_u32(&q_empty[st]));
+        umma_commit(smem_u32(&s_full[buf]));
+      }
+      __syncwarp();
+      asked = j + 1;
+    }
+    // and no product, nor the arrival that reports one
+    int patience = 0;
+    for (int j = max(0, asked - 2); j < asked; ++j) {
+      mbar_wait(smem_u32(&q_empty[j % W_STAGES]), (uint32_t)(j / W_STAGES) & 1, &patience);
+      mbar_wait(smem_u32(&s_full[j & 1]), (uint32_t)(j / 2) & 1, &patience);
+    }
+    if (patience != 0) *abort_flag = 1;
+  } else {
+    // ---- a thread per key and half of a tile's rows
+    const int quad = warp & 3, h = warp >> 2, row = quad * 32 + lane, key = key0 + row;
+    const uint32_t addr = tmem_base + ((uint32_t)(quad * 32) << 16) + h * 64;
+    auto tell = [&](int j) {  // a tile's rows: their logarithms and last visible keys; rows that are none give no weight
+      if (tid < BM) {
+        const int token = (tile0 + j) * per_tile + tid / G;
+        const bool there = tid < RT && token < q_len;
+        lse_s[j & 1][tid] = there ? p.lse[(size_t)(q_begin + token) * p.nq + hk * G + tid % G] * 1.4426950408889634f : INFINITY;
+        pos_s[j & 1][tid] = there ? before + token : -1;
+      }
+    };
+    tell(0);
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    bool ok = true;
+    for (int j = 0; j < tiles; ++j) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // tile j's rows are told, tile j - 1's have been read
+      if (j + 1 < tiles) tell(j + 1);
+      const int buf = j & 1;
+      if (ok) ok = mbar_wait(smem_u32(&s_full[buf]), (uint32_t)(j / 2) & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const int first = (tile0 + j) * per_tile, last = first + per_tile - 1;  // the tile's tokens
+        const bool all = last < q_len && before + first >= last_key && (p.window == 0 || before + last - p.window < key0);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[32];
+          tmem_ld32(addr + buf * BM + c * 32, v);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          const float4* lse = reinterpret_cast<const float4*>(&lse_s[buf][h * 64 + c * 32]);
+          const int4* pos = reinterpret_cast<const int4*>(&pos_s[buf][h * 64 + c * 32]);
+          if (all) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 l = lse[i];
+              sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
+              sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
+              sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
+              sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
+            }
+          } else {
+            const int oldest = p.window > 0 ? p.window : 0x7fffffff;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 l = lse[i];
+              const int4 q = pos[i];
+              if (key <= q.x && q.x - key < oldest) sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
+              if (key <= q.y && q.y - key < oldest) sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
+              if (key <= q.z && q.z - key < oldest) sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
+              if (key <= q.w && q.w - key < oldest) sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
+            }
+          }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&s_empty[buf]));
+      }
+    }
+    const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    if (h == 1) half_s[row] = total;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (h == 0 && key < ctx && abort_s == 0) {
+      const int page = min(max(table[key / page_size], 0), p.num_pages - 1);
+      p.sums[((size_t)page * p.nkv + hk) * page_size + key % page_size] += total + half_s[row];
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (abort_s != 0 && tid == 0) *p.error = 1;
+  if (warp == 9) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(W_TMEM_COLS) : "memory");
+  }
+}
+#endif
+
 #if TS_ATT_LSE
 // Runs of blocks.  Few rows over many keys leave most of the device without a CTA (64 CTAs of 256 rows walk 16 blocks each in 45 us while 84
 // SMs wait).  So a pair's keys may be cut into runs; the rows of a run are whole softmaxes of their keys, and a row is their
-// average, weighted by 2^(lse - the largest lse).  A warp joins the runs of one (token, head), always in the same order.
+// average, weighted by exp(lse - the largest lse).  Eight lanes join the runs of one (token, head), always in the same order.
 __global__ void __launch_bounds__(256) join_runs_kernel(const Params p) {
   ts_pdl_prologue();
-  const int b = blockIdx.y, lane = threadIdx.x & 31, index = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int q_begin = p.cu_q[b], q_len = p.cu_q[b + 1] - q_begin, G = p.nq / p.nkv;
+  const int b = blockIdx.y, lane = threadIdx.x & 7, index = blockIdx.x * 32 + (threadIdx.x >> 3);
+  const int q_begin = p.cu_q[b], q_len = p.cu_q[b + 1] - q_begin, ctx = p.ctx_len[b], G = p.nq / p.nkv;
   const int token = index / p.nq, head = index % p.nq;
   if (token >= q_len) return;
   // how many runs the row's pair of tiles has (as its CTAs work it out)
-  const int start_pos = p.ctx_len[b] - q_len, rows_total = q_len * G, RT = (BM / G) * G;
+  const int start_pos = ctx - q_len, rows_total = q_len * G, RT = (BM / G) * G;
   const int r0 = (token * G + head % G) / (2 * RT) * (2 * RT);
   const int lo = first_visible_key(p, start_pos + r0 / G), hi = start_pos + (min(r0 + 2 * RT, rows_total) - 1) / G;
   const int runs = min(max(1, (hi / PBN - lo / PBN + p.run_blocks) / p.run_blocks), p.runs);
   const size_t at = (size_t)(q_begin + token) * p.nq + head, step = (size_t)p.tokens * p.nq;
   float top = -INFINITY;
-  for (int i = 0; i < runs; ++i) top = fmaxf(top, p.run_lse[at + i * step]);
-  float sum = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
+  for (int i = 0; i < runs; ++i) top = fmaxf(top, p.run_lse[at + i * step]);
+  float sum = 0.f, o[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] = 0.f;
+#pragma unroll 2
   for (int i = 0; i < runs; ++i) {
     const float f = top == -INFINITY ? 0.f : fast_exp2((p.run_lse[at + i * step] - top) * 1.4426950408889634f);
-    const float4 v = *reinterpret_cast<const float4*>(p.run_out + (at + i * step) * D + lane * 4);
+    const float4* from = reinterpret_cast<const float4*>(p.run_out + (at + i * step) * D) + lane;
     sum += f;
-    o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float4 v = from[8 * c];
+      o[4 * c] += f * v.x, o[4 * c + 1] += f * v.y, o[4 * c + 2] += f * v.z, o[4 * c + 3] += f * v.w;
+    }
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  *reinterpret_cast<uint2*>(p.out + at * D + lane * 4) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<uint2*>(p.out + at * D + lane * 4 + 32 * c) =
+        make_uint2(pack_bf16(o[4 * c] * inv, o[4 * c + 1] * inv), pack_bf16(o[4 * c + 2] * inv, o[4 * c + 3] * inv));
   if (lane == 0 && p.lse != nullptr) p.lse[at] = sum > 0.f ? top + logf(sum) : -INFINITY;
 }
 #endif
@@ -1523,7 +1734,7 @@ TS_EXPORT int ts_attention_prefill_tcgen05_scored(const void* q, const void* kca
                                  (cudaStream_t)stream_, mq, mk, mv, p);
 #if TS_ATT_LSE
     if (status == 0 && runs > 1)
-      return ts_launch(join_runs_kernel, dim3((unsigned)(((long long)max_q * nq + 7) / 8), B), dim3(256), 0, (cudaStream_t)stream_, p);
+      return ts_launch(join_runs_kernel, dim3((unsigned)(((long long)max_q * nq + 31) / 32), B), dim3(256), 0, (cudaStream_t)stream_, p);
 #endif
     return status;
   }
@@ -1540,7 +1751,30 @@ TS_EXPORT int ts_attention_prefill_tcgen05_scored(const void* q, const void* kca
 #endif
 }
 
-#if !TS_ATT_LSE
+#if TS_ATT_LSE
+#if !TS_ATT_SCORED
+// q [T, nq, 128] bf16 and lse [T, nq] of portions of prompts; pool and sums of a 4-bit cache of heads of 128; at most 128 query heads per key head.
+TS_EXPORT int ts_kv4_weights_tcgen05(const void* q, const void* pool, const float* lse, float* sums, const int* cu, const int* context, const int* table,
+                                     int table_stride, int page_blocks, int num_pages, int T, int B, int max_context, int nq, int nkv, float scale, int window,
+                                     int* error, void* stream) {
+  if (T <= 0 || B <= 0 || max_context <= 0) return 0;
+  if (nq % nkv || nq / nkv > BM || (uintptr_t)q % 16 || B > 65535 || nkv > 65535) return TS_ERR_UNSUPPORTED_SIZE;
+  WeightParams p = {(const uint8_t*)pool, sums, lse, cu, context, table, error, table_stride, page_blocks, num_pages, T, nq, nkv, window,
+                    scale * 1.4426950408889634f};
+  CUtensorMap mq;
+  int st = query_map(q, T, nq, nkv, &mq);
+  if (st) return st;
+  const size_t smem = W_SMEM + 1024;
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e = cudaFuncSetAttribute(kv4_weights_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    configured = true;
+  }
+  return ts_launch(kv4_weights_kernel, dim3((max_context + BM - 1) / BM, nkv, B), dim3(320), smem, (cudaStream_t)stream, mq, p);
+}
+#endif
+#else
 TS_EXPORT int ts_attention_prefill_tcgen05(const void* q, const void* kcache, const void* vcache, void* out,
                                            const int* cu_q, const int* ctx_len, const int* block_table,
                                            int max_blocks, int page, long long total_slots, int T, int B, int max_q,

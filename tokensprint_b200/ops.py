@@ -2519,6 +2519,7 @@ _attention_kv4: dict[int, tuple] = {}
 ATTENTION_KV4_DIRECT_ROWS = 64
 ATTENTION_KV4_EXPAND_BYTES = 1 << 30  # most bytes of unpacked rows at a time
 _attention_kv4_tcgen05: dict[bool, object] = {}
+_weights_kv4_tcgen05 = None
 _attention_kv4_scratches: dict[tuple, tuple[torch.Tensor, torch.Tensor]] = {}
 
 
@@ -2732,6 +2733,12 @@ _KV4_EXPAND_PAGE = 128
 _KV4_MIN_RUN = 3  # least key blocks of a run
 
 
+def _kv4_tcgen05_library(scored: bool = False) -> ctypes.CDLL:
+    # (the denominators are an output here: every weight from the special-function unit, none from the cubic)
+    return _build.load_variant("attention_tcgen05", {"TS_HEAD_DIM": ATTENTION_TCGEN05_HEAD_DIM, "TS_ATT_LSE": 1, "TS_ATT_FMA_PAIRS": 0,
+                                                     "TS_ATT_SCORED": int(scored)})
+
+
 def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, scale, window, head_sinks,
                             lse) -> None:
     """Portions of prompts over a 4-bit cache, heads of 128: the visible rows are unpacked into bfloat16 pages (they are exact in it), then the prompt
@@ -2741,9 +2748,7 @@ def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_tabl
     scored = head_sinks is not None
     run = _attention_kv4_tcgen05.get(scored)
     if run is None:
-        # (the denominators are an output here: every weight from the special-function unit, none from the cubic)
-        lib = _build.load_variant("attention_tcgen05", {"TS_HEAD_DIM": d, "TS_ATT_LSE": 1, "TS_ATT_FMA_PAIRS": 0, "TS_ATT_SCORED": int(scored)})
-        run = lib.ts_attention_prefill_tcgen05_scored
+        run = _kv4_tcgen05_library(scored).ts_attention_prefill_tcgen05_scored
         run.argtypes = _attention_tcgen05_fns()[0].argtypes + [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p]
         run.restype = _c_int
         _attention_kv4_tcgen05[scored] = run
@@ -2805,6 +2810,18 @@ def attention_kv4_weights(
     if lse.numel() != T * nq:
         raise KernelError(f"attention_kv4_weights: lse must have {T * nq} entries, got {lse.numel()}")
     _kv4_sums("attention_kv4_weights", sums, pool)
+    if max_seqlen_q * (nq // nkv) > ATTENTION_KV4_DIRECT_ROWS and code == 1 and attention_tcgen05_supported(nq, nkv, d, _KV4_EXPAND_PAGE):
+        global _weights_kv4_tcgen05
+        if _weights_kv4_tcgen05 is None:
+            run = _kv4_tcgen05_library().ts_kv4_weights_tcgen05
+            run.argtypes = [_c_void_p] * 7 + [_c_int] * 8 + [_c_float, _c_int, _c_void_p, _c_void_p]
+            run.restype = _c_int
+            _weights_kv4_tcgen05 = run
+        _, error = _gemm_workspace(q.device)
+        _check("attention_kv4_weights", _weights_kv4_tcgen05(
+            q.data_ptr(), pool.data_ptr(), lse.data_ptr(), sums.data_ptr(), cu_seqlens_q.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(),
+            width, blocks, pages, T, num_seqs, max_context, nq, nkv, scale, window, error.data_ptr(), _stream()))
+        return
     _check("attention_kv4_weights", _attention_kv4_fns(d)[1](
         q.data_ptr(), code, pool.data_ptr(), lse.data_ptr(), sums.data_ptr(), cu_seqlens_q.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(),
         width, blocks, pages, T, num_seqs, max_seqlen_q, max_context, nq, nkv, scale, window, _stream()))

@@ -117,9 +117,39 @@ __device__ __forceinline__ void kv4_query_row(const float* p, uint32_t (&frag)[k
   }
 }
 
-// Keys 16 x D of a record times query rows: S[token][row] of tiles of 8 rows; `codes` and `scales` point at the record's
-// key codes and scales.  Lane (g, t) reads rows g and g + 8, a quarter of their channels.  `q(tile, part, word)` gives the lane's
-// four registers of a query tile for the word's two k-steps.
+// Keys 16 x D of a record times query rows: S[token][row] of tiles of 8 rows.  Lane (g, t) has of the rows g and g + 8 the words of a quarter of
+// their channels and those channels' scale bytes.  `q(tile, part, word)` gives the lane's four registers of a query tile for the word's
+// two k-steps.
+template <int D, int kTiles, int kParts, typename Query>
+__device__ __forceinline__ void kv4_scores_of(const uint32_t (&w)[2][D / 32], const uint32_t (&sc)[2], Query q, float (&s)[kTiles][4]) {
+#pragma unroll
+  for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; i += 2) {  // 16 channels: one group
+    __nv_bfloat162 f[2], c[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) kv4_factors((sc[r] >> (4 * i)) & 0xffu, (sc[r] >> (4 * i)) & 0xffu, f[r], c[r]);
+#pragma unroll
+    for (int k = i; k < i + 2; ++k) {
+      const uint32_t a00 = kv4_pair(w[0][k] << 3, f[0], c[0]), a01 = kv4_pair(w[1][k] << 3, f[1], c[1]);
+      const uint32_t a02 = kv4_pair(w[0][k] >> 1, f[0], c[0]), a03 = kv4_pair(w[1][k] >> 1, f[1], c[1]);
+      const uint32_t a10 = kv4_pair(w[0][k] >> 5, f[0], c[0]), a11 = kv4_pair(w[1][k] >> 5, f[1], c[1]);
+      const uint32_t a12 = kv4_pair(w[0][k] >> 9, f[0], c[0]), a13 = kv4_pair(w[1][k] >> 9, f[1], c[1]);
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          const uint4 b = q(n, part, k);
+          kv4_mma(s[n], a00, a01, a02, a03, b.x, b.y);
+          kv4_mma(s[n], a10, a11, a12, a13, b.z, b.w);
+        }
+    }
+  }
+}
+
+// The same from where the record's key codes and scales lie.
 template <int D, int kTiles, int kParts, typename Query>
 __device__ __forceinline__ void kv4_scores(const uint8_t* codes, const uint8_t* scales, Query q, float (&s)[kTiles][4], int g, int t) {
   constexpr int kWords = D / 32;  // of 8 codes, per lane and row
@@ -142,29 +172,5 @@ __device__ __forceinline__ void kv4_scores(const uint8_t* codes, const uint8_t* 
       else sc[r] = *reinterpret_cast<const uint32_t*>(ps);
     }
   }
-#pragma unroll
-  for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
-#pragma unroll
-  for (int i = 0; i < kWords; i += 2) {  // 16 channels: one group
-    __nv_bfloat162 f[2], c[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) kv4_factors((sc[r] >> (4 * i)) & 0xffu, (sc[r] >> (4 * i)) & 0xffu, f[r], c[r]);
-#pragma unroll
-    for (int k = i; k < i + 2; ++k) {
-      const uint32_t a00 = kv4_pair(w[0][k] << 3, f[0], c[0]), a01 = kv4_pair(w[1][k] << 3, f[1], c[1]);
-      const uint32_t a02 = kv4_pair(w[0][k] >> 1, f[0], c[0]), a03 = kv4_pair(w[1][k] >> 1, f[1], c[1]);
-      const uint32_t a10 = kv4_pair(w[0][k] >> 5, f[0], c[0]), a11 = kv4_pair(w[1][k] >> 5, f[1], c[1]);
-      const uint32_t a12 = kv4_pair(w[0][k] >> 9, f[0], c[0]), a13 = kv4_pair(w[1][k] >> 9, f[1], c[1]);
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-        for (int part = 0; part < kParts; ++part) {
-          const uint4 b = q(n, part, k);
-          kv4_mma(s[n], a00, a01, a02, a03, b.x, b.y);
-          kv4_mma(s[n], a10, a11, a12, a13, b.z, b.w);
-        }
-    }
-  }
+  kv4_scores_of<D, kTiles, kParts>(w, sc, q, s);
 }

@@ -28,6 +28,9 @@ using Rec = Kv4Record<D>;
 #ifndef X_CTAS
 #define X_CTAS 4
 #endif
+#ifndef X_WCTAS
+#define X_WCTAS 1184
+#endif
 #ifndef X_REC
 #define X_REC 2
 #endif
@@ -187,9 +190,12 @@ struct Shares {
   int* before;  // [pairs + 1]: steps of one head before the pair
 };
 
-template <typename T, int kTiles, int kQ, int kP, int kRecords>
+template <typename T, int kTiles, int kQ, int kP, int kRecords, bool kTwice>
 __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : kTiles == 1 ? X_CTAS : X_CTAS2) attention_kernel(const Params p) {
-  constexpr int kRows = 8 * kTiles;
+  // kTwice: a tile of 4 rows, which stand twice among the 8 columns; the first time with the first part of their weights, the second time
+  // with the second, so that one product adds both (of 24 products a record 16 are left).
+  static_assert(!kTwice || (kTiles == 1 && kP == 2), "four rows, two parts");
+  constexpr int kRows = kTwice ? 4 : 8 * kTiles, kParts = kTwice ? 1 : kP, kColumnRows = kTwice ? 4 : 8;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int scratch[kWarps + 2];
   ts_pdl_prologue();
@@ -326,7 +332,7 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
     // the queries as the products' second operand, one copy for all warps
     if (warp < kTiles) {
       uint32_t qf[kQ][D / 16][2];
-      const int row = tile.first_row + 8 * warp + g;
+      const int row = tile.first_row + 8 * warp + (kTwice ? g & 3 : g);
       kv4_query_row<D, kQ>(row < tile.rows ? tile.query<T>(p, row) + t * (D / 4) : nullptr, qf);
 #pragma unroll
       for (int k = 0; k < kQ; ++k)
@@ -366,7 +372,7 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
         if (edge) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const int row = tile.first_row + 8 * n + 2 * t + c, pos = row < tile.rows ? tile.position(p, row) : -1;
+            const int row = tile.first_row + 8 * n + (2 * t + c) % kColumnRows, pos = row < tile.rows ? tile.position(p, row) : -1;
 #pragma unroll
             for (int r = 0; r < kRecords; ++r)
 #pragma unroll
@@ -404,7 +410,7 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
       }
 #pragma unroll
       for (int r = 0; r < kRecords; ++r) {
-        uint32_t pf[kTiles][kP][2];
+        uint32_t pf[kTiles][kParts][2];
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
           float w[4];
@@ -417,13 +423,17 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
           for (int i = 0; i < 2; ++i) {
             uint32_t parts[kP];
             kv4_split<kP>(w[2 * i], w[2 * i + 1], parts);
+            if constexpr (kTwice) {
+              pf[n][0][i] = transpose8x8(t < 2 ? parts[0] : parts[1]);
+            } else {
 #pragma unroll
-            for (int k = 0; k < kP; ++k) pf[n][k][i] = transpose8x8(parts[k]);
+              for (int k = 0; k < kP; ++k) pf[n][k][i] = transpose8x8(parts[k]);
+            }
           }
         }
         const int from = key + r * KV4_BLOCK;
-        if (edge) add_values<kTiles, kP, true>(rec + r * Rec::kBytes, pf, o, g, t, key0 - from, last_pos + 1 - from);
-        else add_values<kTiles, kP, false>(rec + r * Rec::kBytes, pf, o, g, t, 0, KV4_BLOCK);
+        if (edge) add_values<kTiles, kParts, true>(rec + r * Rec::kBytes, pf, o, g, t, key0 - from, last_pos + 1 - from);
+        else add_values<kTiles, kParts, false>(rec + r * Rec::kBytes, pf, o, g, t, 0, KV4_BLOCK);
       }
       __syncwarp();
     }
@@ -437,11 +447,19 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
         x += __shfl_xor_sync(0xffffffffu, x, 4);
         x += __shfl_xor_sync(0xffffffffu, x, 8);
         x += __shfl_xor_sync(0xffffffffu, x, 16);
-        const int row = 8 * n + 2 * t + c;
-        if (g == 0) sm[warp * kRows + row] = m[n][c], sl[warp * kRows + row] = x;
+        const int row = 8 * n + (2 * t + c) % kColumnRows;
+        if (g == 0 && (!kTwice || t < 2)) sm[warp * kRows + row] = m[n][c], sl[warp * kRows + row] = x;
         float2* dst = reinterpret_cast<float2*>(so + (warp * kRows + row) * D + g * (D / 8));
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) dst[i] = make_float2(o[n][i][c], o[n][i][c + 2]);
+        for (int i = 0; i < D / 16; ++i) {
+          float2 v = make_float2(o[n][i][c], o[n][i][c + 2]);
+          if constexpr (kTwice) {  // both parts' sums, half of the lanes' pairs written by each of the two lanes that hold them
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, 2), v.y += __shfl_xor_sync(0xffffffffu, v.y, 2);
+            if ((i & 1) == t >> 1) dst[i] = v;
+          } else {
+            dst[i] = v;
+          }
+        }
       }
     __syncthreads();
     const bool whole = seg == base && seg_end == base + n_pair;
@@ -465,10 +483,10 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
     }
     if (!whole) {
       // The CTA that comes last adds the range's parts up, in the order of the CTAs, and leaves its ticket at zero again.
-      __threadfence();
       __syncthreads();
       const int c0 = base / share, c1 = (base + n_pair - 1) / share;
       if (tid == 0) {
+        __threadfence();  // (the barrier puts the whole CTA's writes before it)
         int* ticket = p.tickets + pair * p.nkv + head;
         const bool last = atomicAdd(ticket, 1) == c1 - c0;
         if (last) *ticket = 0;
@@ -482,15 +500,27 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
           if (row >= tile.rows) continue;
           const float* from = p.part + ((size_t)c0 * 2 * kRows + r) * (D + 4);
           const int skip = base > c0 * share ? kRows * (D + 4) : 0;  // the first CTA may have begun with another range
-          constexpr int kStep = 2 * kRows * (D + 4);
+          constexpr int kStep = 2 * kRows * (D + 4), kAhead = 8;  // parts whose loads are in flight together
           RowSum sum;
-#pragma unroll 4
-          for (int c = 0; c <= c1 - c0; ++c) sum.m = fmaxf(sum.m, __ldcg(from + (size_t)c * kStep + (c == 0 ? skip : 0)));
-#pragma unroll 4
-          for (int c = 0; c <= c1 - c0; ++c) {
-            const float* x = from + (size_t)c * kStep + (c == 0 ? skip : 0);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(x));
-            sum.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(x + 4 + channel)), sum.m);
+          for (int first = 0; first <= c1 - c0; first += kAhead) {
+            float2 ml[kAhead];
+            float4 v[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+              const int c = first + i;
+              const float* x = from + (size_t)c * kStep + (c == 0 ? skip : 0);
+              ml[i] = make_float2(kLowest, 0.f), v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (c <= c1 - c0) ml[i] = __ldcg(reinterpret_cast<const float2*>(x)), v[i] = __ldcg(reinterpret_cast<const float4*>(x + 4 + channel));
+            }
+            float top = sum.m;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) top = fmaxf(top, ml[i].x);
+            RowSum next;
+            next.m = top;
+            next.add(sum.m, sum.l, sum.o, top);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) next.add(ml[i].x, ml[i].y, v[i], top);
+            sum = next;
           }
           write_row<T>(p, tile, row, channel, sum.o, sum.m, sum.l);
         }
@@ -503,52 +533,97 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
 }
 
 // ---------------------------------------------------------------------------
-// weights: w_j += sum over the rows r of exp(s_rj - lse_r).  A warp owns 16 keys of one head and walks the rows that see them.
+// weights: w_j += sum over the rows r of exp(s_rj - lse_r).  A warp owns 16 keys of one head at a time.
 
-template <typename T, int kQ>
+// Few rows (kTiles tiles of 8): the warp goes over records kWarps * gridDim.x apart, the next one's codes on their way while it works on
+// one; a key's sum is complete when its record is done, and is added without being read first (no other warp adds to it).
+template <typename T, int kQ, int kTiles>
 __global__ void __launch_bounds__(kWarps * 32) weights_kernel(const Params p, float* sums) {
   ts_pdl_prologue();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   Tile tile;
   tile.open(p, blockIdx.z, blockIdx.y);
-  const int blk = blockIdx.x * kWarps + warp, key = blk * KV4_BLOCK, before = tile.context - tile.q_len;
-  if (key >= tile.context) return;
-  const int first_token = max(0, key - before);
-  const int tokens = p.window > 0 ? min(tile.q_len, key + KV4_BLOCK - 1 + p.window - before) : tile.q_len;
-  if (first_token >= tokens) return;
-  const int page = p.table[(size_t)tile.b * p.table_stride + blk / p.page_blocks];
-  const uint8_t* rec = record(p, page, blk, tile.head);
-  float w[2] = {0.f, 0.f};
-  for (int first = first_token * p.group; first < tokens * p.group; first += 8) {
-    uint32_t qf[1][kQ][D / 16][2];
-    kv4_query_row<D, kQ>(first + g < tile.rows ? tile.query<T>(p, first + g) + t * (D / 4) : nullptr, qf[0]);
-    float s[1][4];
-    kv4_scores<D, 1, kQ>(rec, rec + Rec::kKeyScales,
-                         [&](int, int part, int i) { return make_uint4(qf[0][part][2 * i][0], qf[0][part][2 * i][1], qf[0][part][2 * i + 1][0], qf[0][part][2 * i + 1][1]); },
-                         s, g, t);
+  tile.first_row = 0;
+  const int before = tile.context - tile.q_len;
+  if (tile.q_len <= 0 || tile.context <= 0) return;
+  const int begin = p.window > 0 ? max(0, before - p.window + 1) / KV4_BLOCK : 0, end = (tile.context + KV4_BLOCK - 1) / KV4_BLOCK;
+  const int step = kWarps * gridDim.x, page_size = p.page_blocks * KV4_BLOCK;
+  const int* table = p.table + (size_t)tile.b * p.table_stride;
+  int blk = begin + blockIdx.x * kWarps + warp;
+  if (blk >= end) return;
+
+  constexpr int kWords = D / 32;
+  struct Codes {
+    uint32_t w[2][kWords], sc[2];
+  };
+  auto load = [&](int page, int at, Codes& c) {
+    const uint8_t* rec = record(p, page, at, tile.head);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int r = first + 2 * t + c;
-      if (r >= tile.rows) continue;
-      const int pos = tile.position(p, r);
-      const float lse = p.lse[(size_t)tile.token(p, r) * p.nq + tile.query_head(p, r)] * kLog2e;
+    for (int r = 0; r < 2; ++r) {
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(rec + (g + 8 * r) * (D / 2) + t * (D / 8));
+      const uint8_t* scale = rec + Rec::kKeyScales + (g + 8 * r) * (D / 16) + t * (D / 64);
+      if constexpr (kWords == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(from);
+        c.w[r][0] = v.x, c.w[r][1] = v.y, c.sc[r] = *scale;
+      } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = key + g + 8 * i;
-        if (at <= pos && (p.window == 0 || at > pos - p.window)) w[i] += kv4_exp2(s[0][c + 2 * i] * p.scale - lse);
+        for (int i = 0; i < kWords; i += 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(from + i);
+          c.w[r][i] = v.x, c.w[r][i + 1] = v.y, c.w[r][i + 2] = v.z, c.w[r][i + 3] = v.w;
+        }
+        if constexpr (kWords == 4) c.sc[r] = *reinterpret_cast<const uint16_t*>(scale);
+        else c.sc[r] = *reinterpret_cast<const uint32_t*>(scale);
       }
     }
-  }
-  __syncwarp();
+  };
+  int page = table[blk / p.page_blocks], next_page = blk + step < end ? table[(blk + step) / p.page_blocks] : 0;
+  Codes codes;
+  load(page, blk, codes);
+  uint32_t qf[kTiles][kQ][D / 16][2];
+  float lse[kTiles][2];
+  int pos[kTiles][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    w[i] += __shfl_xor_sync(0xffffffffu, w[i], 1);
-    w[i] += __shfl_xor_sync(0xffffffffu, w[i], 2);
-    const int at = key + g + 8 * i;
-    if (t == 0 && at < tile.context) {
-      float* dst = sums + ((size_t)min(max(page, 0), p.num_pages - 1) * p.nkv + tile.head) * p.page_blocks * KV4_BLOCK + at % (p.page_blocks * KV4_BLOCK);
-      *dst += w[i];
+  for (int n = 0; n < kTiles; ++n) {
+    const int row = 8 * n + g;
+    kv4_query_row<D, kQ>(row < tile.rows ? tile.query<T>(p, row) + t * (D / 4) : nullptr, qf[n]);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int r = 8 * n + 2 * t + c;
+      lse[n][c] = INFINITY, pos[n][c] = -1;  // a row that does not exist gives no weight
+      if (r < tile.rows) lse[n][c] = p.lse[(size_t)tile.token(p, r) * p.nq + tile.query_head(p, r)] * kLog2e, pos[n][c] = tile.position(p, r);
     }
+  }
+  const int all0 = p.window > 0 ? tile.context - p.window : 0, all1 = before + 1;  // keys that every row sees
+  while (true) {
+    Codes next;
+    const int next_blk = blk + step;
+    if (next_blk < end) load(next_page, next_blk, next);
+    const int page_after = next_blk + step < end ? table[(next_blk + step) / p.page_blocks] : 0;
+    float s[kTiles][4];
+    kv4_scores_of<D, kTiles, kQ>(
+        codes.w, codes.sc,
+        [&](int n, int part, int i) { return make_uint4(qf[n][part][2 * i][0], qf[n][part][2 * i][1], qf[n][part][2 * i + 1][0], qf[n][part][2 * i + 1][1]); }, s);
+    const int key = blk * KV4_BLOCK;
+    float w[2] = {0.f, 0.f};
+    const bool edge = tile.rows < 8 * kTiles || key < all0 || key + KV4_BLOCK > all1;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = i & 1, at = key + g + 8 * (i >> 1);
+        const float e = kv4_exp2(fmaf(s[n][i], p.scale, -lse[n][c]));
+        if (!edge || (at <= pos[n][c] && (p.window == 0 || at > pos[n][c] - p.window))) w[i >> 1] += e;
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[i] += __shfl_xor_sync(0xffffffffu, w[i], 1);
+      w[i] += __shfl_xor_sync(0xffffffffu, w[i], 2);
+    }
+    const int at = key + g + 8 * (t & 1);
+    if (t < 2 && at < tile.context)
+      atomicAdd(sums + ((size_t)min(max(page, 0), p.num_pages - 1) * p.nkv + tile.head) * page_size + at % page_size, t == 0 ? w[0] : w[1]);
+    if (next_blk >= end) break;
+    blk = next_blk, page = next_page, next_page = page_after, codes = next;
   }
 }
 
@@ -706,10 +781,12 @@ __global__ void __launch_bounds__(kWeightThreads, 1) weights_rows_kernel(const P
 
 template <typename T, int kQ>
 int launch_weights(const Params& p, float* sums, int num_seqs, int max_context, int max_q, cudaStream_t stream) {
-  // A key of few rows is read, used and done with (16 rows are two turns of a warp); with more, unpacking it once pays.
+  // Few rows: a record is read, used and done with, by as many warps as run at once; with more, unpacking it once pays.
   if (max_q * p.group <= 16) {
-    const dim3 grid((max_context + KV4_BLOCK * kWarps - 1) / (KV4_BLOCK * kWarps), p.nkv, num_seqs);
-    return ts_launch(weights_kernel<T, kQ>, grid, dim3(kWarps * 32), 0, stream, p, sums);
+    const int most = (max_context + KV4_BLOCK * kWarps - 1) / (KV4_BLOCK * kWarps), want = X_WCTAS / (p.nkv * num_seqs) + 1;
+    const dim3 grid(most < want ? most : want, p.nkv, num_seqs);
+    if (max_q * p.group <= 8) return ts_launch(weights_kernel<T, kQ, 1>, grid, dim3(kWarps * 32), 0, stream, p, sums);
+    return ts_launch(weights_kernel<T, kQ, 2>, grid, dim3(kWarps * 32), 0, stream, p, sums);
   }
   constexpr int smem = 2 * WeightsStage<kQ>::kBytes;
   static bool set = false;
@@ -722,20 +799,21 @@ int launch_weights(const Params& p, float* sums, int num_seqs, int max_context, 
   return ts_launch(weights_rows_kernel<T, kQ>, grid, dim3(kWeightThreads), smem, stream, p, sums);
 }
 
-template <typename T, int kTiles, int kQ, int kP, int kRecords>
+template <typename T, int kTiles, int kQ, int kP, int kRecords, bool kTwice = false>
 struct Attention {
-  static constexpr int kSmem = kWarps * kRing * Rec::kBytes + kTiles * kQ * D * 16 + kWarps * 8 * kTiles * (D + 2) * 4;  // and 4 bytes per pair
+  static constexpr int kRows = kTwice ? 4 : 8 * kTiles;
+  static constexpr int kSmem = kWarps * kRing * Rec::kBytes + kTiles * kQ * D * 16 + kWarps * kRows * (D + 2) * 4;  // and 4 bytes per pair
   static constexpr int kFewPairs = 256;
   // CTAs that run at once on the device (with at most kFewPairs pairs), or a negative error
   static int ctas() {
     static int n = 0;
     if (n == 0) {
       int device = 0, sms = 0, per_sm = 0;
-      cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kTiles, kQ, kP, kRecords>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      cudaError_t e = cudaFuncSetAttribute(attention_kernel<T, kTiles, kQ, kP, kRecords, kTwice>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            kSmem + (kMaxTiles + 1) * 4);
       if (e == cudaSuccess) e = cudaGetDevice(&device);
       if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-      if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_kernel<T, kTiles, kQ, kP, kRecords>, kWarps * 32,
+      if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_kernel<T, kTiles, kQ, kP, kRecords, kTwice>, kWarps * 32,
                                                                                 kSmem + (kFewPairs + 1) * 4);
       if (e != cudaSuccess) return -(int)e - 100;
       n = sms * (per_sm > 0 ? per_sm : 1);
@@ -743,7 +821,7 @@ struct Attention {
     return n;
   }
   static int launch(const Params& p, int grid, cudaStream_t stream) {
-    return ts_launch(attention_kernel<T, kTiles, kQ, kP, kRecords>, dim3(grid), dim3(kWarps * 32), kSmem + (p.num_seqs * p.row_tiles + 1) * 4, stream, p);
+    return ts_launch(attention_kernel<T, kTiles, kQ, kP, kRecords, kTwice>, dim3(grid), dim3(kWarps * 32), kSmem + (p.num_seqs * p.row_tiles + 1) * 4, stream, p);
   }
 };
 
@@ -751,16 +829,18 @@ struct Attention {
 
 using AttentionFloat = Attention<float, 1, 3, 3, 1>;
 using AttentionFew = Attention<__nv_bfloat16, 1, 1, 2, D <= 128 ? X_REC : 1>;
+using AttentionFour = Attention<__nv_bfloat16, 1, 1, 2, D <= 128 ? X_REC : 1, true>;
 #if TS_HEAD_DIM <= 128
 using AttentionMore = Attention<__nv_bfloat16, 2, 1, 2, 1>;
 #endif
 
 // How many rows a tile has, by the type and the rows of a sequence and key head.
-static int tile_rows(int dtype, int rows) { return dtype == TS_DTYPE_BF16 && rows > 8 && D <= 128 ? 16 : 8; }
+static int tile_rows(int dtype, int rows) { return dtype != TS_DTYPE_BF16 ? 8 : rows <= 4 ? 4 : rows > 8 && D <= 128 ? 16 : 8; }
 
 // CTAs of a launch (at most), for the size of `part`: grid * 2 * tile rows * (D + 4) floats; negative: an error.
 static int grid_of(int dtype, int rows) {
   if (dtype == TS_DTYPE_F32) return AttentionFloat::ctas();
+  if (tile_rows(dtype, rows) == 4) return AttentionFour::ctas();
 #if TS_HEAD_DIM <= 128
   if (tile_rows(dtype, rows) == 16) return AttentionMore::ctas();
 #endif
@@ -794,6 +874,7 @@ TS_EXPORT int ts_attention_kv4(const void* q, int dtype, const void* pool, void*
                   row_tiles - tile < tiles ? row_tiles - tile : tiles, tile, scale * kLog2e};
       int status;
       if (dtype == TS_DTYPE_F32) status = AttentionFloat::launch(p, grid, (cudaStream_t)stream);
+      else if (tile_rows(dtype, rows) == 4) status = AttentionFour::launch(p, grid, (cudaStream_t)stream);
 #if TS_HEAD_DIM <= 128
       else if (tile_rows(dtype, rows) == 16) status = AttentionMore::launch(p, grid, (cudaStream_t)stream);
 #endif

@@ -2668,7 +2668,7 @@ def _check_attention_kv4(name, q, pool, cu_seqlens_q, context_lens, block_table,
 def _attention_kv4_scratch(device: torch.device, head_dim: int, code: int, rows: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Per (device, stream): where CTAs that share a key range leave their parts (the size goes by the device and the kernel alone), and the
     tickets that tell the last of them (zeros between launches)."""
-    key = (device.index or 0, _stream(), head_dim, code, rows > 8)
+    key = (device.index or 0, _stream(), head_dim, code, 4 if rows <= 4 else 8 if rows <= 8 else 16)
     scratch = _attention_kv4_scratches.get(key)
     if scratch is None:
         need = _attention_kv4_fns(head_dim)[2](code, rows)

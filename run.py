@@ -11,7 +11,8 @@ folder from the registered config and a seed when none is there), --prompt-ids (
 instead of text; without tokenizer files in the folder this is the only way),
 --dtype, --kvcache-block-size, --num-kvcache-blocks, --max-num-batched-tokens,
 --chunked-prefill, --seed, --overlap-steps (launch a step before the host has read the ids
-of the step before; default True).
+of the step before; default True), --cache-format kv4 (keys and values in 4 bits), --cache-budget ROWS (with it: about
+how many rows a request keeps, by the attention they get) and --cache-recent ROWS (how many of the last ones always stay).
 """
 
 from __future__ import annotations
@@ -51,6 +52,9 @@ def parse_args(argv=None) -> argparse.Namespace:
     p.add_argument("--chunked-prefill", type=_bool, default=False)
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--overlap-steps", type=_bool, default=True)
+    p.add_argument("--cache-format", choices=("model", "kv4"), default="model")
+    p.add_argument("--cache-budget", type=int, default=0)
+    p.add_argument("--cache-recent", type=int, default=64)
     return p.parse_args(argv)
 
 
@@ -98,6 +102,9 @@ def main(args: argparse.Namespace) -> None:
         max_num_batched_tokens=args.max_num_batched_tokens,
         chunked_prefill=args.chunked_prefill,
         overlap_steps=args.overlap_steps,
+        cache_format=args.cache_format,
+        cache_budget=args.cache_budget,
+        cache_recent=args.cache_recent,
     )
     engine = LLMEngine(model=model, config=config, tokenizer=tokenizer)
     sampling_params = SamplingParams(temperature=args.temperature, max_tokens=args.max_tokens, seed=args.seed)

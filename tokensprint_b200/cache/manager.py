@@ -88,7 +88,10 @@ class RequestCache:
     request: Hashable
     slot: int
     tables: list[list[int]]  # per group; -1 where a page was given back (or never held)
-    num_tokens: int = 0  # positions 0..num_tokens-1 have been given a place
+    num_tokens: int = 0  # rows 0..num_tokens-1 have been given a place (the positions, unless rows were given up)
+    # Rows given up so far (see CacheManager.shrink): the token at position p has the row p - dropped.  The methods of the
+    # manager and the steps of the engine name positions.
+    dropped: int = 0
     released: bool = False
     fresh_slot: bool = True  # the slot's state has not been zeroed on the device yet
     first_held: list[int] = field(default_factory=list)  # per group: first table index still held
@@ -144,6 +147,7 @@ class CacheManager:
         self.free_slots.append(rc.slot)
         rc.released = True
         rc.num_tokens = 0
+        rc.dropped = 0
         del self.live[rc.request]
 
     # -- growth ------------------------------------------------------------------
@@ -182,6 +186,7 @@ class CacheManager:
 
     def can_extend(self, rc: RequestCache, start: int, new_len: int) -> bool:
         """Whether `extend` would succeed right now."""
+        start, new_len = start - rc.dropped, new_len - rc.dropped
         if self._fits_as_is(rc, new_len) and start <= new_len:
             return True
         for pool, (drop, take) in zip(self.pools, self._plan(rc, start, new_len)):
@@ -197,6 +202,7 @@ class CacheManager:
         """
         if rc.released:
             raise CacheError(f"request {rc.request!r} was freed")
+        start, new_len = start - rc.dropped, new_len - rc.dropped
         if self._fits_as_is(rc, new_len) and start <= new_len:
             rc.num_tokens = new_len
             return
@@ -218,19 +224,38 @@ class CacheManager:
                 table.extend(pool.take(take, rc.request))
         rc.num_tokens = max(rc.num_tokens, new_len)
 
+    def shrink(self, rc: RequestCache, rows: int) -> None:
+        """A request's rows have been cut to `rows` that stand at the front of its pages (ops.kv4_evict): the pages behind
+        them are given back, and later tokens follow on the rows that stay.  Groups that give pages back by position have no such rows."""
+        if rc.released:
+            raise CacheError(f"request {rc.request!r} was freed")
+        if self._any_window:
+            raise CacheError("rows are given up only where every group keeps all keys")
+        if not 0 < rows <= rc.num_tokens:
+            raise CacheError(f"cannot cut request {rc.request!r} from {rc.num_tokens} rows to {rows}")
+        pages = -(-rows // self.page_size)
+        for g, pool in enumerate(self.pools):
+            gone = rc.tables[g][pages:]
+            if gone:
+                pool.give(list(reversed(gone)), rc.request)
+                del rc.tables[g][pages:]
+        rc.dropped += rc.num_tokens - rows
+        rc.num_tokens = rows
+
     # -- what a step needs ---------------------------------------------------------
 
     def slots_for(self, rc: RequestCache, g: int, start: int, count: int) -> "np.ndarray":
         """Flat cache slots (page * page_size + offset) of positions start..start+count-1."""
         P = self.page_size
+        start -= rc.dropped
         first = start // P
         pages = np.asarray(rc.tables[g][first : (start + count - 1) // P + 1], dtype=np.int64)
-        positions = np.arange(start, start + count, dtype=np.int64)
-        held = pages[positions // P - first]
+        rows = np.arange(start, start + count, dtype=np.int64)
+        held = pages[rows // P - first]
         if held.size and held.min() < 0:
-            pos = int(positions[int(np.argmax(held < 0))])
+            pos = int(rows[int(np.argmax(held < 0))]) + rc.dropped
             raise CacheError(f"request {rc.request!r}: position {pos} lies in a page that was given back")
-        return held * P + positions % P
+        return held * P + rows % P
 
     # -- checks --------------------------------------------------------------------
 

@@ -64,6 +64,15 @@ class Config:
     # on the device), so that the device does not wait for the host between steps.  A request's
     # end is then seen one step later; what that step computed for it is dropped.
     overlap_steps: bool = True
+    # "kv4": keys and values in 4 bits (9/16 of a byte a value), for models whose layers are all plain attention with heads
+    # of 64, 128 or 256 and pages of a multiple of 16.  cache_budget > 0 (with it): a request keeps about that many rows: once it has
+    # `cache_slack` more, every layer and head gives up those that got the least attention, the first `cache_first` and the last
+    # `cache_recent` ones excepted.
+    cache_format: str = "model"
+    cache_budget: int = 0
+    cache_recent: int = 64
+    cache_first: int = 4
+    cache_slack: int = 64
 
     def __post_init__(self) -> None:
         if not os.path.isdir(self.model):
@@ -80,3 +89,7 @@ class Config:
                 f"gpu_memory_utilization must be in (0, 1], got {self.gpu_memory_utilization}"
             )
         self.dtype = canonical_dtype(self.dtype)
+        if self.cache_format not in ("model", "kv4"):
+            raise ValueError(f"cache_format must be 'model' or 'kv4', got {self.cache_format!r}")
+        if self.cache_budget < 0 or (self.cache_budget and self.cache_format != "kv4"):
+            raise ValueError("cache_budget must not be negative, and needs cache_format 'kv4'")

@@ -31,6 +31,12 @@ using Rec = Kv4Record<D>;
 #ifndef X_WCTAS
 #define X_WCTAS 1184
 #endif
+#ifndef X_AHEAD
+#define X_AHEAD 8
+#endif
+#ifndef X_MIN
+#define X_MIN 1
+#endif
 #ifndef X_REC
 #define X_REC 2
 #endif
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
   }
   const int total = shares.before[pairs] * p.nkv;
   // at least a step for every warp, and no range over more than kMaxParts CTAs
-  const int share = max(max(kWarps, (total + (int)gridDim.x - 1) / (int)gridDim.x), (most + kMaxParts - 1) / kMaxParts);
+  const int share = max(max(kWarps * X_MIN, (total + (int)gridDim.x - 1) / (int)gridDim.x), (most + kMaxParts - 1) / kMaxParts);
   const int begin = (int)min((long long)share * blockIdx.x, (long long)total), end = min(begin + share, total);
   if (begin >= end) return;
   auto pair_of = [&](int step) {
@@ -500,7 +506,7 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
           if (row >= tile.rows) continue;
           const float* from = p.part + ((size_t)c0 * 2 * kRows + r) * (D + 4);
           const int skip = base > c0 * share ? kRows * (D + 4) : 0;  // the first CTA may have begun with another range
-          constexpr int kStep = 2 * kRows * (D + 4), kAhead = 8;  // parts whose loads are in flight together
+          constexpr int kStep = 2 * kRows * (D + 4), kAhead = X_AHEAD;  // parts whose loads are in flight together
           RowSum sum;
           for (int first = 0; first <= c1 - c0; first += kAhead) {
             float2 ml[kAhead];

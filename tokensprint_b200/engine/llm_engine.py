@@ -90,6 +90,11 @@ class LLMEngine:
             gpu_memory_utilization=config.gpu_memory_utilization,
             enforce_eager=config.enforce_eager,
             max_model_len=config.max_model_len,
+            cache_format=config.cache_format,
+            cache_budget=config.cache_budget,
+            cache_recent=config.cache_recent,
+            cache_first=config.cache_first,
+            cache_slack=config.cache_slack,
         )
         # (a model whose mixers keep fixed-size state only has no page pool at all)
         config.num_kvcache_blocks = self.model_runner.num_pages[0] if self.model_runner.num_pages else 0

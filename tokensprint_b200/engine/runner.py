@@ -51,7 +51,7 @@ class _DecodeGraph:
     logits: torch.Tensor  # [bucket, vocab] float32, rewritten by every replay
     kernels: int  # kernels of this library inside the graph
     event: Optional["torch.cuda.Event"] = None
-    # per cache group: row of the batch -> (request cache, table entries written, first entry still held)
+    # per cache group: row of the batch -> (request cache, table entries written, first entry still held, rows given up)
     row_marks: list = None
 
 
@@ -105,6 +105,11 @@ class ModelRunner:
         enforce_eager: bool = True,
         max_model_len: int = 4096,
         max_graph_batch: int = 256,
+        cache_format: str = "model",
+        cache_budget: int = 0,
+        cache_recent: int = 64,
+        cache_first: int = 4,
+        cache_slack: int = 64,
     ) -> None:
         if model.device.type != "cuda":
             raise RuntimeError("ModelRunner needs a CUDA device: the engine has no CPU path")
@@ -118,8 +123,26 @@ class ModelRunner:
 
         needs = [p.need for p in model.cache_plan]
         self.groups, self.cache_group = groups_of(needs)
+        # cache_format "kv4": keys and values in 4 bits.  cache_budget > 0 (with it): after a step, a request with more than budget + slack
+        # rows is cut to the budget, per layer and head to the rows that got the most attention.
+        if cache_format not in ("model", "kv4"):
+            raise ValueError(f"cache_format must be 'model' or 'kv4', got {cache_format!r}")
+        self.kv4 = cache_format == "kv4"
+        self.cache_budget, self.cache_recent, self.cache_first, self.cache_slack = cache_budget, cache_recent, cache_first, cache_slack
+        if self.kv4:
+            for run in model.spec.run_order:
+                why = model.blocks[run.layer].mixer.kv4_refusal()
+                if why is not None:
+                    raise ValueError(f"cache_format 'kv4': layer {run.layer}: {why}")
+            if page_size % 16:
+                raise ValueError(f"cache_format 'kv4' needs pages of a multiple of 16 tokens, got {page_size}")
+        if cache_budget:
+            if not self.kv4 or len(self.groups) != 1 or self.groups[0].kind != "full":
+                raise ValueError("a cache budget needs cache_format 'kv4' and layers that keep all keys")
+            if cache_recent < 0 or cache_first < 0 or cache_slack < 0 or cache_budget < max(1, cache_recent + cache_first):
+                raise ValueError(f"a cache budget of {cache_budget} rows cannot hold the first {cache_first} and the last {cache_recent}")
         itemsize = torch.empty((), dtype=model.dtype).element_size()
-        self.page_bytes = [page_bytes(needs, self.cache_group, g, page_size, itemsize) for g in range(len(self.groups))]
+        self.page_bytes = [page_bytes(needs, self.cache_group, g, page_size, itemsize, self.kv4, bool(cache_budget)) for g in range(len(self.groups))]
         self._needs = needs
         self._pinned: list[torch.Tensor] = []
         self._pinned_events: list[Optional[torch.cuda.Event]] = []
@@ -162,7 +185,8 @@ class ModelRunner:
         self.num_pages = list(pages)
         self.cache_manager = CacheManager(self.groups, self.page_size, self.num_pages, self.num_slots)
         self.cache_tensors = CacheTensors.allocate(
-            self._needs, self.cache_group, self.num_pages, self.page_size, self.num_slots, self.device, self.model.dtype)
+            self._needs, self.cache_group, self.num_pages, self.page_size, self.num_slots, self.device, self.model.dtype,
+            kv4=self.kv4, weighed=bool(self.cache_budget))
         used = self.model.run_cache
         self.layer_caches = [
             self.cache_tensors.layer_cache(used[i], run.writes_cache, used[i + 1 :].count(used[i]))
@@ -280,7 +304,7 @@ class ModelRunner:
             singles = B if singles == B else 0
         widths = []
         for g in range(len(self.groups)):
-            widths.append(max(1, max(-(-(e.start + n) // P) for e, n in zip(entries, lens))))
+            widths.append(max(1, max(-(-(e.start + n - e.cache.dropped) // P) for e, n in zip(entries, lens))))
         layout = _Layout(T, B, R, widths)
         pinned, slot_i = self._pinned_buffer(layout.total)
         host = pinned.numpy()[: layout.total]
@@ -293,7 +317,7 @@ class ModelRunner:
         ev = torch.cuda.Event()
         ev.record()
         self._pinned_events[slot_i] = ev
-        step = self._context(dev, layout, max(lens), max(e.start + n for e, n in zip(entries, lens)))
+        step = self._context(dev, layout, max(lens), max(e.start + n - e.cache.dropped for e, n in zip(entries, lens)))
         step.host_seq_starts = [e.start for e in entries]
         step.host_seq_lens = lens
         step.host_state_slots = [e.cache.slot for e in entries]
@@ -333,10 +357,11 @@ class ModelRunner:
             if id(rc) in seen:
                 raise ValueError(f"request {rc.request!r} appears twice in one step")
             seen.add(id(rc))
-            if e.start < 0 or e.start + n > rc.num_tokens:
+            row = e.start - rc.dropped  # the first token's row (its position, unless rows were given up)
+            if row < 0 or row + n > rc.num_tokens:
                 raise ValueError(
                     f"request {rc.request!r}: tokens {e.start}..{e.start + n - 1} have no place in the cache "
-                    f"({rc.num_tokens} positions were given one)")
+                    f"({rc.num_tokens + rc.dropped} positions were given one)")
             if e.feed >= 0:
                 if n != 1:
                     raise ValueError(f"request {rc.request!r}: only a single token can be fed on the device")
@@ -361,7 +386,7 @@ class ModelRunner:
                 pos[t0 : t0 + n] = np.arange(e.start, e.start + n)
                 sidx[t0 : t0 + n] = b
             cu[b + 1] = t0 + n
-            ctx_lens[b] = e.start + n
+            ctx_lens[b] = row + n
             slots[b] = rc.slot
             if row_base is not None:
                 r0 = row_base[b]
@@ -373,10 +398,10 @@ class ModelRunner:
             for g in range(len(self.groups)):
                 table = rc.tables[g]
                 if n == 1:
-                    page = table[e.start // self.page_size]
+                    page = table[row // self.page_size]
                     if page < 0:
                         raise ValueError(f"request {rc.request!r}: position {e.start} lies in a page that was given back")
-                    slot_maps[g][t0] = page * self.page_size + e.start % self.page_size
+                    slot_maps[g][t0] = page * self.page_size + row % self.page_size
                 else:
                     slot_maps[g][t0 : t0 + n] = self.cache_manager.slots_for(rc, g, e.start, n)
                 count = min(len(table), widths[g])
@@ -384,7 +409,7 @@ class ModelRunner:
                 # row holds: the same request in the same row only gets its new entries written
                 # (and the entries a window gave back), not its whole table again.
                 mark = None if row_marks is None else row_marks[g].get(b)
-                if mark is not None and mark[0] is rc and mark[1] <= count and mark[2] <= rc.first_held[g]:
+                if mark is not None and mark[0] is rc and mark[1] <= count and mark[2] <= rc.first_held[g] and mark[3] == rc.dropped:
                     if mark[1] < count:
                         tables[g][b, mark[1] : count] = table[mark[1] : count]
                     if mark[2] < rc.first_held[g]:
@@ -393,7 +418,7 @@ class ModelRunner:
                     tables[g][b, :count] = table[:count]
                     tables[g][b, count:] = -1
                 if row_marks is not None:
-                    row_marks[g][b] = (rc, count, rc.first_held[g])
+                    row_marks[g][b] = (rc, count, rc.first_held[g], rc.dropped)
             if rc.fresh_slot:
                 self.cache_tensors.zero_slot(rc.slot)
                 rc.fresh_slot = False
@@ -545,17 +570,48 @@ class ModelRunner:
         bucket = self._graph_bucket(entries)
         if bucket is not None:
             for e in entries:
-                if e.cache.released or e.start + 1 > e.cache.num_tokens or not (e.feed >= 0 or 0 <= e.tokens[0] < self.vocab_size):
+                if e.cache.released or not 0 <= e.start - e.cache.dropped < e.cache.num_tokens or not (e.feed >= 0 or 0 <= e.tokens[0] < self.vocab_size):
                     raise ValueError(f"request {e.cache.request!r}: bad decode entry")
                 if any(w != 0 for w in e.want):
                     raise ValueError(f"request {e.cache.request!r}: wanted place outside its 1 token")
-            return self._step_graph(bucket, entries, fed_ids)
+            logits = self._step_graph(bucket, entries, fed_ids)
+            self._cut_to_budget(entries)
+            return logits
         step, rows, R = self.build_context(entries, fed_ids)
         with self.model.chain_scope(step.num_tokens):
             hidden, pending = self.model.forward_hidden(step, self.layer_caches)
             if R == 0:
-                return torch.empty((0, self.vocab_size), device=self.device, dtype=torch.float32)
-            return self.model.logits(hidden, pending, rows, R)
+                logits = torch.empty((0, self.vocab_size), device=self.device, dtype=torch.float32)
+            else:
+                logits = self.model.logits(hidden, pending, rows, R)
+        self._cut_to_budget(entries)
+        return logits
+
+    def _cut_to_budget(self, entries: Sequence[StepEntry]) -> None:
+        """Requests of this step that hold more rows than the budget and its slack give up those with the least weight, in every
+        layer (the kernels follow the step's on the stream; the pages are free for whatever comes behind them)."""
+        if not self.cache_budget or self._sizing_step:
+            return
+        over = [e.cache for e in entries
+                if e.cache.num_tokens > self.cache_budget + self.cache_slack and e.start + len(e.tokens) - e.cache.dropped == e.cache.num_tokens]
+        if not over:
+            return
+        from tokensprint_b200 import ops
+
+        width, longest = max(len(rc.tables[0]) for rc in over), max(rc.num_tokens for rc in over)
+        packed = torch.full((len(over), width + 1), -1, dtype=torch.int32).pin_memory()
+        for i, rc in enumerate(over):
+            packed[i, 0] = rc.num_tokens
+            packed[i, 1 : 1 + len(rc.tables[0])] = torch.tensor(rc.tables[0], dtype=torch.int32)
+        dev = packed.to(self.device, non_blocking=True)
+        self.h2d_bytes += packed.numel() * 4
+        lens, table = dev[:, 0].contiguous(), dev[:, 1:].contiguous()
+        new_lens = torch.empty_like(lens)
+        for pool, sums in zip(self.cache_tensors.kv4, self.cache_tensors.sums):
+            if pool is not None:
+                ops.kv4_evict(pool, sums, table, lens, new_lens, len(over), longest, self.cache_budget, self.cache_recent, self.cache_first)
+        for rc in over:
+            self.cache_manager.shrink(rc, self.cache_budget)
 
     # -- cache life cycle (thin wrappers that keep device memory in step) ------------------
 

@@ -201,6 +201,13 @@ class AttentionMixer(Mixer):
             return CacheNeed(kind="chunk", window=self.chunk, kv_heads=self.num_kv_heads, head_dim=self.kernel_dim)
         return CacheNeed(kind="full", kv_heads=self.num_kv_heads, head_dim=self.kernel_dim)
 
+    def kv4_refusal(self) -> Optional[str]:
+        if self.general or self.joint_norm or self.chunk or self.sink is not None:
+            return "attention over a 4-bit cache takes a norm per head, a rotation and a window, and none of the further options"
+        if self.head_dim not in ops.KV4_HEAD_DIMS:
+            return f"a 4-bit cache takes heads of {ops.KV4_HEAD_DIMS}, got {self.head_dim}"
+        return None
+
     def tensor_specs(self) -> list[TensorSpec]:
         H, nq, nkv, d, e = self.hidden_size, self.num_heads, self.num_kv_heads, self.head_dim, self.value_dim
         n = self.names
@@ -258,6 +265,8 @@ class AttentionMixer(Mixer):
         """x: [T, H], or a PreNormed (its missing 1/rms is applied by the q/k/v product).  With
         `fold` the output projection adds its result into fold.hidden itself and the PreNormed of
         the norm that follows is returned instead of the branch output."""
+        if cache.kv4_pool is not None:
+            return self._forward_kv4(x, step, cache, fold)
         if cache.k_pages is None or cache.group < 0:
             raise ops.KernelError("attention: this mixer needs cache pages (none were bound to its run)")
         xt = x if isinstance(x, torch.Tensor) else x.x
@@ -347,6 +356,43 @@ class AttentionMixer(Mixer):
             ops.gate_rows(out, proj[:, g_off:g_off + (nq if self.gate_per_head else nq * e)] if gated else None, y, nq, e, D,
                           per_head=self.gate_per_head)
             out = y
+        return linear(out, self.o_weight, next_weight=step.weight_after)
+
+    def _forward_kv4(self, x, step: StepContext, cache: LayerCache, fold: Optional[ResidualNorm]):
+        """The same over a cache in 4 bits: norm and rotation into plain buffers, the store, attention, and where rows are weighed what this
+        step's queries add to their weights."""
+        xt = x if isinstance(x, torch.Tensor) else x.x
+        T, tables = xt.shape[0], step.groups[cache.group]
+        nq, nkv, d = self.num_heads, self.num_kv_heads, self.head_dim
+        qkv = linear_scaled(x, self.qkv_weight, next_weight=self.o_weight)
+        q = torch.empty((T, nq * d), device=xt.device, dtype=xt.dtype)
+        k, v = (torch.empty((T, nkv, d), device=xt.device, dtype=xt.dtype) for _ in range(2))
+        inv_freq = self.position.rotary_inv_freq() if self.position is not None else None
+        ops.qk_norm_rope_store(qkv, q, k, v, None, step.positions, self.q_norm_weight, self.k_norm_weight, self.qk_norm_eps, inv_freq, nq, nkv, d)
+        if self.position is not None and inv_freq is None:
+            self.position.apply(q.view(T, nq, d), k, step)
+        if cache.writes:
+            ops.kv4_store(k, v, cache.kv4_pool, tables.slot_mapping, cache.kv4_sums)
+        out = torch.empty_like(q)
+        weighed = cache.kv4_sums is not None
+        lse = torch.empty((T, nq), device=xt.device, dtype=torch.float32) if weighed else None
+
+        def attend(first: int, count: int, tokens: int, max_q: int) -> None:
+            sizes = (step.cu_seqlens_q[first : first + count + 1], step.context_lens[first : first + count], tables.block_table[first : first + count],
+                     count, max_q, step.max_context_len, nq, nkv, d, self.scale)
+            kept = None if lse is None else lse[:tokens]
+            ops.attention_kv4(q[:tokens], cache.kv4_pool, out[:tokens], *sizes, window=self.window, lse=kept)
+            if weighed:
+                ops.attention_kv4_weights(q[:tokens], cache.kv4_pool, kept, cache.kv4_sums, *sizes, window=self.window)
+
+        B, singles = step.num_seqs, step.decode_seqs
+        if 0 < singles < B:  # decoded tokens beside portions of prompts: each kind by itself (the single tokens' requests come first)
+            attend(0, singles, singles, 1)
+            attend(singles, B - singles, T, step.max_seqlen_q)
+        else:
+            attend(0, B, T, step.max_seqlen_q)
+        if fold is not None:
+            return linear_into_residual(out, self.o_weight, fold, next_weight=step.weight_after)
         return linear(out, self.o_weight, next_weight=step.weight_after)
 
     # -- attention proper ---------------------------------------------------

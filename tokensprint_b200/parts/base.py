@@ -236,6 +236,10 @@ class LayerCache:
     state: Optional[torch.Tensor] = None  # [slots, *state_shape]
     writes: bool = True  # False: reads a cache that another run filled
     read_later: int = 0  # how many later runs of the step read these pages
+    # A cache in 4 bits has one pool for keys and values instead (ops.kv4_pool_shape), and, where rows are to be given up by
+    # the weight they get, that weight so far: [pages, kv_heads, page] float32
+    kv4_pool: Optional[torch.Tensor] = None
+    kv4_sums: Optional[torch.Tensor] = None
     # [slots, *shape]: what the block around the mixer keeps per request (Block.state_need); always the
     # run's own, also where the run reads another run's pages
     block_state: Optional[torch.Tensor] = None
@@ -320,6 +324,10 @@ class Mixer(Part):
 
     def cache_need(self) -> CacheNeed:
         return CacheNeed()
+
+    def kv4_refusal(self) -> Optional[str]:
+        """Why this mixer cannot keep its cache in 4 bits; None: it can."""
+        return f"{type(self).__name__} has no 4-bit form"
 
     def forward(self, x: torch.Tensor, step: StepContext, cache: LayerCache) -> torch.Tensor:
         raise NotImplementedError

@@ -239,7 +239,7 @@ __device__ __forceinline__ void cluster_meet() {
 // rounds, kMoveRows places per CTA: all reads of a round, a barrier of the cluster, its writes.  That is safe in place: a row
 // never moves backwards and the order is kept, so what a round writes lies before everything that later rounds read.
 template <int D>
-__global__ void __launch_bounds__(kEvictThreads) evict_kernel(uint8_t* pool, float* sums, const int* table, int table_stride, const int* context,
+__global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(uint8_t* pool, float* sums, const int* table, int table_stride, const int* context,
                                                               int* new_lens, int* order, int nkv, int page_blocks, int num_pages, int budget, int recent,
                                                               int first, int cluster, int room) {
   extern __shared__ uint32_t kept_keys[];
@@ -257,7 +257,18 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(uint8_t* pool, flo
 
   const bool in_smem = n <= room;
   if (in_smem) {
-    for (int i = tid; i < n; i += kEvictThreads) kept_keys[i] = order_of(weight_of(page_of(i), i % page_size));
+    constexpr int kAhead = 4;  // loads under way per thread
+    for (int i0 = tid; i0 < n; i0 += kEvictThreads * kAhead) {
+      int page[kAhead];
+      float w[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) page[u] = page_of(min(i0 + u * kEvictThreads, n - 1));
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) w[u] = weight_of(page[u], min(i0 + u * kEvictThreads, n - 1) % page_size);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (i0 + u * kEvictThreads < n) kept_keys[i0 + u * kEvictThreads] = order_of(w[u]);
+    }
     __syncthreads();
   }
   auto key_of = [&](int i) { return in_smem ? kept_keys[i] : order_of(weight_of(page_of(i), i % page_size)); };
@@ -396,8 +407,19 @@ int launch_evict(uint8_t* pool, float* sums, const int* table, int table_stride,
 static int threads_per_token(int tokens) { return tokens < 1024 ? 128 : 32; }
 
 // k, v: rows [tokens] of nkv * d entries, `stride` entries apart; slots [tokens], -1: not stored; sums: null or the pool's weights.
-TS_EXPORT int ts_kv4_store(const void* k, const void* v, int dtype, long long k_stride, long long v_stride, void* pool, float* sums, const int* slots,
-                           int tokens, int nkv, int d, int page_blocks, int num_pages, void* stream) {
+// (These entry points take their arguments as one block of memory: a call from Python converts one argument instead of fourteen, which is a
+// tenth of what a small call costs the host.)
+struct Kv4StoreArgs {
+  const void *k, *v;
+  long long k_stride, v_stride;
+  void* pool;
+  float* sums;
+  const int* slots;
+  void* stream;
+  int dtype, tokens, nkv, d, page_blocks, num_pages;
+};
+TS_EXPORT int ts_kv4_store(const Kv4StoreArgs* args) {
+  const auto [k, v, k_stride, v_stride, pool, sums, slots, stream, dtype, tokens, nkv, d, page_blocks, num_pages] = *args;
   if (tokens < 1) return 0;
   const int width = threads_per_token(tokens), log_groups = d == 64 ? 2 : d == 128 ? 3 : 4, num_slots = num_pages * page_blocks * KV4_BLOCK;
   const dim3 grid((unsigned)((tokens + 128 / width - 1) / (128 / width)));
@@ -410,8 +432,14 @@ TS_EXPORT int ts_kv4_store(const void* k, const void* v, int dtype, long long k_
 }
 
 // k, v [rows][nkv][d]; a slot outside the pool gives zeros.
-TS_EXPORT int ts_kv4_load(const void* pool, const int* slots, void* k, void* v, int dtype, int rows, int nkv, int d, int page_blocks, int num_pages,
-                          void* stream) {
+struct Kv4LoadArgs {
+  const void* pool;
+  const int* slots;
+  void *k, *v, *stream;
+  int dtype, rows, nkv, d, page_blocks, num_pages;
+};
+TS_EXPORT int ts_kv4_load(const Kv4LoadArgs* args) {
+  const auto [pool, slots, k, v, stream, dtype, rows, nkv, d, page_blocks, num_pages] = *args;
   if (rows < 1) return 0;
   const int width = threads_per_token(rows), log_groups = d == 64 ? 2 : d == 128 ? 3 : 4, num_slots = num_pages * page_blocks * KV4_BLOCK;
   const dim3 grid((unsigned)((rows + 128 / width - 1) / (128 / width)));
@@ -433,8 +461,17 @@ TS_EXPORT int ts_kv4_expand(const void* pool, const int* table, int table_stride
 }
 
 // order: num_seqs * nkv * budget ints of workspace; context[b] <= max_context.
-TS_EXPORT int ts_kv4_evict(void* pool, float* sums, const int* table, int table_stride, const int* context, int* new_lens, int* order, int num_seqs, int nkv,
-                           int d, int page_blocks, int num_pages, int max_context, int budget, int recent, int first, void* stream) {
+struct Kv4EvictArgs {
+  void* pool;
+  float* sums;
+  const int *table, *context;
+  int *new_lens, *order;
+  void* stream;
+  int table_stride, num_seqs, nkv, d, page_blocks, num_pages, max_context, budget, recent, first;
+};
+TS_EXPORT int ts_kv4_evict(const Kv4EvictArgs* args) {
+  const auto [pool, sums, table, context, new_lens, order, stream, table_stride, num_seqs, nkv, d, page_blocks, num_pages, max_context, budget, recent,
+              first] = *args;
   if (num_seqs < 1) return 0;
   if (num_seqs > 65535) return TS_ERR_UNSUPPORTED_SIZE;
   if (recent < 0 || first < 0 || budget < 1 || recent + first > budget) return TS_ERR_BAD_ARGUMENT;

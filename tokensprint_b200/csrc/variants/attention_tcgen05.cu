@@ -624,6 +624,7 @@ constexpr float RESCALE_THRESHOLD = 8.f;
 #ifndef TS_ATT_FMA_PAIRS
 #define TS_ATT_FMA_PAIRS 1
 #endif
+[[maybe_unused]] constexpr int MAX_RANKED = 256;  // pairs of tiles that are put in order (see there)
 constexpr int FMA_PAIRS = REBUILT ? 0 : TS_ATT_FMA_PAIRS;
 
 // two float32 in one 64-bit register, and the packed arithmetic on them
@@ -738,13 +739,34 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // the CTAs with the most keys to walk are launched first (see the other kernel)
+  const int G = p.nq / p.nkv;
 #if TS_ATT_LSE
   const int cta = blockIdx.x / p.runs, run = blockIdx.x % p.runs;
+  // Sequences of different lengths: the pairs of tiles of all of them in the order of their key blocks, the most first (place i of the order goes to
+  // the nkv CTAs from i * nkv on).  Every thread ranks one pair.
+  __shared__ int blocks_s[MAX_RANKED], ranked_s;
+  const int places = (int)(gridDim.x / (p.runs * p.nkv));
+  int place = cta / p.nkv;
+  if (p.num_seqs > 1 && places <= MAX_RANKED) {
+    if (tid < places) {
+      const int i = tid % p.num_seqs, n = p.cu_q[i + 1] - p.cu_q[i], rows = n * G, step = 2 * (BM / G) * G;
+      const int first = ((rows + step - 1) / step - 1 - tid / p.num_seqs) * step, start = p.ctx_len[i] - n;
+      blocks_s[tid] = n <= 0 || first < 0 ? -1 : (start + (min(first + step, rows) - 1) / G) / PBN - first_visible_key(p, start + first / G) / PBN;
+    }
+    __syncthreads();
+    if (tid < places) {
+      const int mine = blocks_s[tid];
+      int rank = 0;
+      for (int i = 0; i < places; ++i) rank += blocks_s[i] > mine || (blocks_s[i] == mine && i < tid);
+      if (rank == place) ranked_s = tid;
+    }
+    __syncthreads();
+    place = ranked_s;
+  }
 #else
-  const int cta = blockIdx.x;
+  const int cta = blockIdx.x, place = cta / p.nkv;
 #endif
-  const int hk = cta % p.nkv, b = (cta / p.nkv) % p.num_seqs;
-  const int G = p.nq / p.nkv;
+  const int hk = cta % p.nkv, b = place % p.num_seqs;
   const int q_begin = p.cu_q[b];
   const int q_len = p.cu_q[b + 1] - q_begin;
   const int ctx = p.ctx_len[b];
@@ -752,7 +774,7 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
   const int rows_total = q_len * G;
   const int RT = (BM / G) * G;  // rows of a tile that belong to tokens (see the other kernel)
   const int seq_pairs = (rows_total + 2 * RT - 1) / (2 * RT);
-  const int pair = seq_pairs - 1 - cta / (p.nkv * p.num_seqs);
+  const int pair = seq_pairs - 1 - place / p.num_seqs;
   if (q_len <= 0 || pair < 0) return;
   const int r0 = pair * 2 * RT;
   const int ntiles = rows_total - r0 > RT ? 2 : 1;

@@ -41,7 +41,7 @@ using Rec = Kv4Record<D>;
 #define X_REC 2
 #endif
 #ifndef X_CTAS2
-#define X_CTAS2 1
+#define X_CTAS2 3
 #endif
 constexpr int kWarps = X_WARPS;
 constexpr int kRing = X_RING;         // records of a warp's ring
@@ -859,9 +859,21 @@ TS_EXPORT long long ts_attention_kv4_part_floats(int dtype, int rows) {
 
 // q, out [tokens][nq][D] of `dtype`, lse [tokens][nq] or null, sinks [nq] or null; part: see above; tickets: `num_tickets` zeros (zeros again
 // afterwards).  Batches of more pairs than a launch or the tickets hold take several launches.
-TS_EXPORT int ts_attention_kv4(const void* q, int dtype, const void* pool, void* out, float* lse, const float* sinks, const int* cu, const int* context,
-                               const int* table, int table_stride, int page_blocks, int num_pages, int tokens, int num_seqs, int max_q, int nq, int nkv,
-                               float scale, int window, float* part, int* tickets, int num_tickets, void* stream) {
+struct Kv4AttentionArgs {
+  const void *q, *pool;
+  void* out;
+  float* lse;
+  const float* sinks;
+  const int *cu, *context, *table;
+  float* part;
+  int* tickets;
+  void* stream;
+  int dtype, table_stride, page_blocks, num_pages, tokens, num_seqs, max_q, nq, nkv, window, num_tickets;
+  float scale;
+};
+TS_EXPORT int ts_attention_kv4(const Kv4AttentionArgs* args) {
+  const auto [q, pool, out, lse, sinks, cu, context, table, part, tickets, stream, dtype, table_stride, page_blocks, num_pages, tokens, num_seqs, max_q, nq,
+              nkv, window, num_tickets, scale] = *args;
   if (tokens < 1 || num_seqs < 1 || max_q < 1) return 0;
   if (num_tickets < nkv || (long long)max_q * (nq / nkv) > 0x7fffffffLL - 16) return TS_ERR_UNSUPPORTED_SIZE;
   const int rows = max_q * (nq / nkv), grid = grid_of(dtype, rows), row_tiles = (rows + tile_rows(dtype, rows) - 1) / tile_rows(dtype, rows);
@@ -890,9 +902,17 @@ TS_EXPORT int ts_attention_kv4(const void* q, int dtype, const void* pool, void*
   return 0;
 }
 
-TS_EXPORT int ts_attention_kv4_weights(const void* q, int dtype, const void* pool, float* lse, float* sums, const int* cu, const int* context,
-                                       const int* table, int table_stride, int page_blocks, int num_pages, int tokens, int num_seqs, int max_q, int max_context, int nq,
-                                       int nkv, float scale, int window, void* stream) {
+struct Kv4WeightsArgs {
+  const void *q, *pool;
+  float *lse, *sums;
+  const int *cu, *context, *table;
+  void* stream;
+  int dtype, table_stride, page_blocks, num_pages, tokens, num_seqs, max_q, max_context, nq, nkv, window;
+  float scale;
+};
+TS_EXPORT int ts_attention_kv4_weights(const Kv4WeightsArgs* args) {
+  const auto [q, pool, lse, sums, cu, context, table, stream, dtype, table_stride, page_blocks, num_pages, tokens, num_seqs, max_q, max_context, nq, nkv,
+              window, scale] = *args;
   if (tokens < 1 || num_seqs < 1 || max_context < 1) return 0;
   if (num_seqs > 65535 || nkv > 65535) return TS_ERR_UNSUPPORTED_SIZE;
   Params p = {q, (const uint8_t*)pool, nullptr, lse, nullptr, cu, context, table, nullptr, nullptr, table_stride, page_blocks, num_pages, tokens, num_seqs, nq, nkv,

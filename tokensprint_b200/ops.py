@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os as _os
+import struct as _struct
 from typing import Optional
 
 import torch
@@ -2510,9 +2511,14 @@ def attention_prefill_tcgen05(
 
 KV4_BLOCK = 16  # tokens of a record, channels that share a scale
 KV4_HEAD_DIMS = (64, 128, 256)
-_SIGNATURES["ts_kv4_store"] = [_c_void_p, _c_void_p, _c_int, _c_ll, _c_ll, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p]
-_SIGNATURES["ts_kv4_load"] = [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p]
-_SIGNATURES["ts_kv4_evict"] = [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p] + [_c_int] * 9 + [_c_void_p]
+# Entry points that take one block of arguments, laid out as the C structs beside them.
+for _name in ("ts_kv4_store", "ts_kv4_load", "ts_kv4_evict"):
+    _SIGNATURES[_name] = [ctypes.c_char_p]
+_KV4_STORE_ARGS = _struct.Struct("@PPqqPPPP6i").pack
+_KV4_LOAD_ARGS = _struct.Struct("@PPPPP6i").pack
+_KV4_EVICT_ARGS = _struct.Struct("@PPPPPPP10i").pack
+_KV4_ATTENTION_ARGS = _struct.Struct("@11P11if").pack
+_KV4_WEIGHTS_ARGS = _struct.Struct("@8P11if").pack
 _SIGNATURES["ts_kv4_expand"] = [_c_void_p, _c_void_p, _c_int] + [_c_void_p] * 6 + [_c_int] * 6 + [_c_void_p]
 _attention_kv4: dict[int, tuple] = {}
 # Portions of prompts with more rows (tokens x query heads of a key head) than this are attended to on tcgen05 tensor cores, over rows unpacked for the step.
@@ -2520,7 +2526,7 @@ ATTENTION_KV4_DIRECT_ROWS = 64
 ATTENTION_KV4_EXPAND_BYTES = 1 << 30  # most bytes of unpacked rows at a time
 _attention_kv4_tcgen05: dict[bool, object] = {}
 _weights_kv4_tcgen05 = None
-_attention_kv4_scratches: dict[tuple, tuple[torch.Tensor, torch.Tensor]] = {}
+_attention_kv4_scratches: dict[tuple, tuple] = {}
 
 
 def kv4_pool_shape(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int) -> tuple[int, int, int, int]:
@@ -2597,8 +2603,9 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, slot_mapping
         _kv4_store_refusal(k, v, slot_mapping, nkv, d)
     if sums is not None:
         _kv4_sums("kv4_store", sums, pool)
-    _check("kv4_store", _fn("ts_kv4_store")(
-        at_k, at_v, code, k_stride, v_stride, pool.data_ptr(), _ptr(sums), slot_mapping.data_ptr(), T, nkv, d, blocks, pages, _stream()))
+    _check("kv4_store", _fn("ts_kv4_store")(_KV4_STORE_ARGS(
+        at_k, at_v, k_stride, v_stride, pool.data_ptr(), 0 if sums is None else sums.data_ptr(), slot_mapping.data_ptr(), _stream(), code, T, nkv, d,
+        blocks, pages)))
 
 
 def kv4_load(pool: torch.Tensor, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -2616,7 +2623,7 @@ def kv4_load(pool: torch.Tensor, slots: torch.Tensor, k: torch.Tensor, v: torch.
             _cuda_contig(f"kv4_load: {name}", t, dtype)
             if tuple(t.shape) != want or t.data_ptr() % 16:
                 raise KernelError(f"kv4_load: {name} must be [{N}, {nkv}, {d}] on a 16-byte boundary, got {tuple(t.shape)}")
-    _check("kv4_load", _fn("ts_kv4_load")(pool.data_ptr(), slots.data_ptr(), at_k, at_v, code, N, nkv, d, blocks, pages, _stream()))
+    _check("kv4_load", _fn("ts_kv4_load")(_KV4_LOAD_ARGS(pool.data_ptr(), slots.data_ptr(), at_k, at_v, _stream(), code, N, nkv, d, blocks, pages)))
 
 
 def _attention_kv4_fns(head_dim: int) -> tuple:
@@ -2624,10 +2631,9 @@ def _attention_kv4_fns(head_dim: int) -> tuple:
     if fns is None:
         lib = _build.load_variant("kv4_attention", {"TS_HEAD_DIM": head_dim})
         run, weights = lib.ts_attention_kv4, lib.ts_attention_kv4_weights
-        run.argtypes = [_c_void_p, _c_int] + [_c_void_p] * 7 + [_c_int] * 8 + [_c_float, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p]
+        run.argtypes = weights.argtypes = [ctypes.c_char_p]
         part_floats = lib.ts_attention_kv4_part_floats
         part_floats.argtypes, part_floats.restype = [_c_int, _c_int], _c_ll
-        weights.argtypes = [_c_void_p, _c_int] + [_c_void_p] * 6 + [_c_int] * 9 + [_c_float, _c_int, _c_void_p]
         run.restype = weights.restype = _c_int
         fns = _attention_kv4[head_dim] = (run, weights, part_floats)
     return fns
@@ -2665,16 +2671,17 @@ def _check_attention_kv4(name, q, pool, cu_seqlens_q, context_lens, block_table,
     raise KernelError(f"{name}: negative sizes")
 
 
-def _attention_kv4_scratch(device: torch.device, head_dim: int, code: int, rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+def _attention_kv4_scratch(device: torch.device, head_dim: int, code: int, rows: int) -> tuple[int, int, torch.Tensor, torch.Tensor]:
     """Per (device, stream): where CTAs that share a key range leave their parts (the size goes by the device and the kernel alone), and the
-    tickets that tell the last of them (zeros between launches)."""
-    key = (device.index or 0, _stream(), head_dim, code, 4 if rows <= 4 else 8 if rows <= 8 else 16)
+    tickets that tell the last of them (zeros between launches): their addresses, and the tensors."""
+    key = (device.index, _stream(), head_dim, code, 4 if rows <= 4 else 8 if rows <= 8 else 16)
     scratch = _attention_kv4_scratches.get(key)
     if scratch is None:
         need = _attention_kv4_fns(head_dim)[2](code, rows)
         if need < 0:
             _check("attention_kv4", -need - 100)
-        scratch = _attention_kv4_scratches[key] = (torch.empty(need, device=device, dtype=torch.float32), _attention_counters(device))
+        part, tickets = torch.empty(need, device=device, dtype=torch.float32), _attention_counters(device)
+        scratch = _attention_kv4_scratches[key] = (part.data_ptr(), tickets.data_ptr(), part, tickets)
     return scratch
 
 
@@ -2722,11 +2729,11 @@ def attention_kv4(
         _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, scale, window,
                                 head_sinks, lse)
         return
-    part, tickets = _attention_kv4_scratch(q.device, d, code, rows)
-    _check("attention_kv4", _attention_kv4_fns(d)[0](
-        q.data_ptr(), code, pool.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(head_sinks), cu_seqlens_q.data_ptr(), context_lens.data_ptr(),
-        block_table.data_ptr(), width, blocks, pages, T, num_seqs, max_seqlen_q, nq, nkv, scale, window, part.data_ptr(), tickets.data_ptr(),
-        _GEMM_MAX_TILES, _stream()))
+    part, tickets, _, _ = _attention_kv4_scratch(q.device, d, code, rows)
+    _check("attention_kv4", _attention_kv4_fns(d)[0](_KV4_ATTENTION_ARGS(
+        q.data_ptr(), pool.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if head_sinks is None else head_sinks.data_ptr(),
+        cu_seqlens_q.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(), part, tickets, _stream(), code, width, blocks, pages, T, num_seqs,
+        max_seqlen_q, nq, nkv, window, _GEMM_MAX_TILES, scale)))
 
 
 _KV4_EXPAND_PAGE = 128
@@ -2822,9 +2829,9 @@ def attention_kv4_weights(
             q.data_ptr(), pool.data_ptr(), lse.data_ptr(), sums.data_ptr(), cu_seqlens_q.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(),
             width, blocks, pages, T, num_seqs, max_context, nq, nkv, scale, window, error.data_ptr(), _stream()))
         return
-    _check("attention_kv4_weights", _attention_kv4_fns(d)[1](
-        q.data_ptr(), code, pool.data_ptr(), lse.data_ptr(), sums.data_ptr(), cu_seqlens_q.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(),
-        width, blocks, pages, T, num_seqs, max_seqlen_q, max_context, nq, nkv, scale, window, _stream()))
+    _check("attention_kv4_weights", _attention_kv4_fns(d)[1](_KV4_WEIGHTS_ARGS(
+        q.data_ptr(), pool.data_ptr(), lse.data_ptr(), sums.data_ptr(), cu_seqlens_q.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(),
+        _stream(), code, width, blocks, pages, T, num_seqs, max_seqlen_q, max_context, nq, nkv, window, scale)))
 
 
 def kv4_evict(pool: torch.Tensor, sums: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor, num_seqs: int,
@@ -2847,9 +2854,9 @@ def kv4_evict(pool: torch.Tensor, sums: torch.Tensor, block_table: torch.Tensor,
     if max_context < 0 or num_seqs < 0:
         raise KernelError("kv4_evict: negative sizes")
     order = torch.empty(num_seqs * nkv * budget, device=pool.device, dtype=torch.int32)  # where every kept row comes from
-    _check("kv4_evict", _fn("ts_kv4_evict")(
-        pool.data_ptr(), sums.data_ptr(), block_table.data_ptr(), block_table.shape[1], context_lens.data_ptr(), new_lens.data_ptr(), order.data_ptr(),
-        num_seqs, nkv, d, blocks, pages, int(max_context), int(budget), int(recent), int(first), _stream()))
+    _check("kv4_evict", _fn("ts_kv4_evict")(_KV4_EVICT_ARGS(
+        pool.data_ptr(), sums.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(), new_lens.data_ptr(), order.data_ptr(), _stream(),
+        block_table.shape[1], num_seqs, nkv, d, blocks, pages, max_context, budget, recent, first)))
 
 
 # ---------------------------------------------------------------------------

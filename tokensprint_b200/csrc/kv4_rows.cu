@@ -75,10 +75,11 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[16], uint2& w) {
   return byte;
 }
 
-// A thread takes the 16 channels of one group: their largest, the scale, the codes, 8 + 1 bytes out.  `width` threads (32 or 128) go over the
-// groups of a token, keys first: 32 keep their loads apart from one another's and need few threads, 128 wait once when there are few tokens.
+// A thread takes the 16 channels of one group at a time: their largest, the scale, the codes, 8 + 1 bytes out; `width` threads (32 or 128) go over
+// the groups of a token, keys first.  With many tokens it is the number of warps that hides the loads (16,384 tokens of 8 heads of 128:
+// 21.7 us with a group at a time and 46 registers, 38.6 with four in flight and 125; 105 MB).
 template <typename T>
-__global__ void __launch_bounds__(128) store_kernel(const T* k, const T* v, long long k_stride, long long v_stride, uint8_t* pool, float* sums,
+__global__ void __launch_bounds__(128, 10) store_kernel(const T* k, const T* v, long long k_stride, long long v_stride, uint8_t* pool, float* sums,
                                                     const int* slots, int tokens, int nkv, int log_groups, int page_blocks, int num_slots, int width) {
   ts_pdl_prologue();
   const int groups = 1 << log_groups, d = 16 * groups, units = nkv << log_groups;
@@ -89,26 +90,16 @@ __global__ void __launch_bounds__(128) store_kernel(const T* k, const T* v, long
   const int page_size = page_blocks * KV4_BLOCK, page = slot / page_size, in_page = slot % page_size, row = in_page % KV4_BLOCK;
   uint8_t* records = pool + ((size_t)page * nkv * page_blocks + in_page / KV4_BLOCK) * (18 * d);  // head 0's
   const T *from_k = k + token * k_stride, *from_v = v + token * v_stride;
-  constexpr int kAhead = 4;
-  for (int first = threadIdx.x % width; first < 2 * units; first += kAhead * width) {
-    float x[kAhead][16];
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int i = first + a * width;
-      if (i < 2 * units) read_group<T>(i < units ? from_k + i * 16 : from_v + (i - units) * 16, x[a]);
-    }
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int i = first + a * width;
-      if (i >= 2 * units) break;
-      const int unit = i < units ? i : i - units, head = unit >> log_groups, grp = unit & (groups - 1);
-      uint2 w;
-      const uint32_t byte = quantise(x[a], w);
-      uint8_t* rec = records + (size_t)head * page_blocks * (18 * d) + (i < units ? 0 : 9 * d);
-      *reinterpret_cast<uint2*>(rec + row * (d / 2) + grp * 8) = w;
-      rec[8 * d + row * groups + grp] = (uint8_t)byte;
-      if (sums != nullptr && i < units && grp == 0) sums[((size_t)page * nkv + head) * page_size + in_page] = 0.f;  // it has gathered no weight
-    }
+  for (int i = threadIdx.x % width; i < 2 * units; i += width) {
+    float x[16];
+    read_group<T>(i < units ? from_k + i * 16 : from_v + (i - units) * 16, x);
+    const int unit = i < units ? i : i - units, head = unit >> log_groups, grp = unit & (groups - 1);
+    uint2 w;
+    const uint32_t byte = quantise(x, w);
+    uint8_t* rec = records + (size_t)head * page_blocks * (18 * d) + (i < units ? 0 : 9 * d);
+    *reinterpret_cast<uint2*>(rec + row * (d / 2) + grp * 8) = w;
+    rec[8 * d + row * groups + grp] = (uint8_t)byte;
+    if (sums != nullptr && i < units && grp == 0) sums[((size_t)page * nkv + head) * page_size + in_page] = 0.f;  // it has gathered no weight
   }
 }
 
@@ -232,18 +223,28 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* scratch, 
 __device__ __forceinline__ void cluster_meet() {
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
+// Four words at `p` of this CTA's shared memory, as the CTA `rank` of the cluster has them.
+__device__ __forceinline__ uint4 peer_words(const uint32_t* p, int rank) {
+  uint32_t at = (uint32_t)__cvta_generic_to_shared(p);
+  uint4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(at) : "r"(rank));
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
 
-// A cluster of CTAs per request and head.  Every CTA ranks the weights between the first and the recent rows by a radix
-// select (they are few bytes; ranking them once and telling the others would cost more than reading them again), finds for every
-// kept row its new place and writes down the sources of the places it will fill.  Then the kept rows move forward in
-// rounds, kMoveRows places per CTA: all reads of a round, a barrier of the cluster, its writes.  That is safe in place: a row
-// never moves backwards and the order is kept, so what a round writes lies before everything that later rounds read.
+// A cluster of CTAs per request and head, every CTA with an equal run of its rows.  The weights between the first and the recent rows are ranked by
+// a radix select whose counts the CTAs add up from one another's shared memory; every kept row gets its new place, and its source is written
+// down there.  Then the kept rows move forward in rounds, kMoveRows places per CTA: all reads of a round, a barrier of the cluster, its writes.
+// That is safe in place: a row never moves backwards and the order is kept, so what a round writes lies before everything that later
+// rounds read.  (Every CTA ranking all rows by itself took 35 us of 72 for 128 pairs of 8,190 rows.)
 template <int D>
 __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(uint8_t* pool, float* sums, const int* table, int table_stride, const int* context,
-                                                              int* new_lens, int* order, int nkv, int page_blocks, int num_pages, int budget, int recent,
-                                                              int first, int cluster, int room) {
+                                                                 int* new_lens, int* order, int nkv, int page_blocks, int num_pages, int budget, int recent,
+                                                                 int first, int cluster, int room) {
   extern __shared__ uint32_t kept_keys[];
-  __shared__ uint32_t hist[kDigits], scratch[kEvictWarps], chosen[2];
+  __shared__ __align__(16) uint32_t hist[3][kDigits], totals[4];
+  __shared__ uint32_t scratch[kEvictWarps], chosen[2], warp_counts[2 * kEvictWarps], source[kMoveRows], target[kMoveRows];
+  __shared__ uint8_t source_row[kMoveRows];
   ts_pdl_prologue();
   const int rank = blockIdx.x % cluster, head = blockIdx.x / cluster, b = blockIdx.y, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int page_size = page_blocks * KV4_BLOCK;
@@ -253,25 +254,29 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(uint8_t* pool, 
   table += (size_t)b * table_stride;
   order += ((size_t)b * nkv + head) * budget;
   auto page_of = [&](int row) { return min(max(table[row / page_size], 0), num_pages - 1); };
-  auto weight_of = [&](int page, int in_page) -> float& { return sums[((size_t)page * nkv + head) * page_size + in_page]; };
+  // a row's record among the pool's (its weight then has the place 16 * record + row % 16)
+  auto record_of = [&](int row) { return ((uint32_t)page_of(row) * nkv + head) * page_blocks + row % page_size / KV4_BLOCK; };
+  auto weight_of = [&](uint32_t record, int row) -> float& { return sums[(size_t)record * KV4_BLOCK + row % KV4_BLOCK]; };
 
-  const bool in_smem = n <= room;
+  const int run = ((n + cluster - 1) / cluster + 31) / 32 * 32, row_lo = min(n, rank * run), row_hi = min(n, row_lo + run);
+  const bool in_smem = run <= room;
+  for (int i = tid; i < 3 * kDigits; i += kEvictThreads) hist[0][i] = 0;
   if (in_smem) {
     constexpr int kAhead = 4;  // loads under way per thread
-    for (int i0 = tid; i0 < n; i0 += kEvictThreads * kAhead) {
-      int page[kAhead];
+    for (int i0 = row_lo + tid; i0 < row_hi; i0 += kEvictThreads * kAhead) {
+      uint32_t record[kAhead];
       float w[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) page[u] = page_of(min(i0 + u * kEvictThreads, n - 1));
+      for (int u = 0; u < kAhead; ++u) record[u] = record_of(min(i0 + u * kEvictThreads, row_hi - 1));
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) w[u] = weight_of(page[u], min(i0 + u * kEvictThreads, n - 1) % page_size);
+      for (int u = 0; u < kAhead; ++u) w[u] = weight_of(record[u], min(i0 + u * kEvictThreads, row_hi - 1));
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        if (i0 + u * kEvictThreads < n) kept_keys[i0 + u * kEvictThreads] = order_of(w[u]);
+        if (i0 + u * kEvictThreads < row_hi) kept_keys[i0 + u * kEvictThreads - row_lo] = order_of(w[u]);
     }
-    __syncthreads();
   }
-  auto key_of = [&](int i) { return in_smem ? kept_keys[i] : order_of(weight_of(page_of(i), i % page_size)); };
+  __syncthreads();
+  auto key_of = [&](int i) { return in_smem ? kept_keys[i - row_lo] : order_of(weight_of(record_of(i), i)); };
 
   uint32_t threshold = 0xffffffffu, ties = 0;  // kept: what is above the threshold, and `ties` of what equals it
   const bool ranked = budget > first + recent;
@@ -280,18 +285,20 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(uint8_t* pool, 
     threshold = 0;
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-      for (int i = tid; i < kDigits; i += kEvictThreads) hist[i] = 0;
-      __syncthreads();
-      for (int i = first + tid; i < n - recent; i += kEvictThreads) {
+      for (int i = max(first, row_lo) + tid; i < min(n - recent, row_hi); i += kEvictThreads) {
         const uint32_t u = key_of(i);
-        if (pass == 0 || ((u ^ threshold) >> (shift + bits)) == 0) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1u)], 1u);
+        if (pass == 0 || ((u ^ threshold) >> (shift + bits)) == 0) atomicAdd(&hist[pass][(u >> shift) & ((1u << bits) - 1u)], 1u);
       }
-      __syncthreads();
+      cluster_meet();
       // the bin in which the count from the top reaches what is left: thread i stands for four bins from 2047 - 4 i down
       constexpr int kBins = kDigits / kEvictThreads;
-      uint32_t count[kBins], mine = 0, total;
-#pragma unroll
-      for (int j = 0; j < kBins; ++j) mine += count[j] = hist[kDigits - 1 - (tid * kBins + j)];
+      static_assert(kBins == 4, "a thread reads its bins at once");
+      uint32_t count[kBins] = {0u, 0u, 0u, 0u}, total;
+      for (int r = 0; r < cluster; ++r) {
+        const uint4 c = peer_words(&hist[pass][kDigits - kBins * (tid + 1)], r);
+        count[0] += c.w, count[1] += c.z, count[2] += c.y, count[3] += c.x;
+      }
+      const uint32_t mine = count[0] + count[1] + count[2] + count[3];
       uint32_t above = block_prefix(mine, scratch, total);
       if (above < left && above + mine >= left) {
 #pragma unroll
@@ -309,78 +316,88 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(uint8_t* pool, 
 
   // ---- places: a warp goes over a run of rows, 32 at a time, counting first and then numbering
   auto state_of = [&](int i) -> int {  // 1: kept, 2: of the threshold's own weight
-    if (i >= n) return 0;
+    if (i >= row_hi) return 0;
     if (i < first || i >= n - recent) return 1;
     if (!ranked) return 0;
     const uint32_t u = key_of(i);
     return u > threshold ? 1 : u == threshold ? 2 : 0;
   };
-  const int run = (n + kEvictThreads - 1) / kEvictThreads * 32, row0 = warp * run;
+  const int warp_run = (run + kEvictThreads - 1) / kEvictThreads * 32, row0 = row_lo + warp * warp_run, row1 = min(row_hi, row0 + warp_run);
   int sure = 0, equal = 0;
-  for (int i = row0; i < row0 + run; i += 32) {
+  for (int i = row0; i < row1; i += 32) {
     const int st = state_of(i + lane);
     sure += __popc(__ballot_sync(0xffffffffu, st == 1)), equal += __popc(__ballot_sync(0xffffffffu, st == 2));
   }
+  if (lane == 0) warp_counts[warp] = sure, warp_counts[kEvictWarps + warp] = equal;
   __syncthreads();
-  if (lane == 0) hist[warp] = sure, hist[kEvictWarps + warp] = equal;
-  __syncthreads();
+  if (tid == 0) {
+    uint32_t a = 0, e = 0;
+    for (int i = 0; i < kEvictWarps; ++i) a += warp_counts[i], e += warp_counts[kEvictWarps + i];
+    totals[0] = a, totals[1] = e;
+  }
+  cluster_meet();
   int sure_before = 0, equal_before = 0;
-  for (int i = 0; i < warp; ++i) sure_before += hist[i], equal_before += hist[kEvictWarps + i];
-  for (int i = row0; i < row0 + run; i += 32) {
+  for (int r = 0; r < rank; ++r) {
+    const uint4 t = peer_words(totals, r);
+    sure_before += t.x, equal_before += t.y;
+  }
+  for (int i = 0; i < warp; ++i) sure_before += warp_counts[i], equal_before += warp_counts[kEvictWarps + i];
+  for (int i = row0; i < row1; i += 32) {
     const int row = i + lane, st = state_of(row);
     const uint32_t sures = __ballot_sync(0xffffffffu, st == 1), equals = __ballot_sync(0xffffffffu, st == 2), lower = (1u << lane) - 1u;
     const int e = equal_before + __popc(equals & lower);
     const int place = sure_before + __popc(sures & lower) + min(e, (int)ties);
-    if ((st == 1 || (st == 2 && e < (int)ties)) && place / kMoveRows % cluster == rank) order[place] = page_of(row) * page_size + row % page_size;
+    if (st == 1 || (st == 2 && e < (int)ties)) __stcg(order + place, row);
     sure_before += __popc(sures), equal_before += __popc(equals);
   }
-  __syncthreads();
+  cluster_meet();
 
   // ---- the move: pieces of 16 bytes of codes, pieces of kScale bytes of scales, and the weights
   constexpr int kPieces = D / 16, kCode = kMoveRows * kPieces / kEvictThreads, kScale = D / 16;
-  auto record_at = [&](int page, int in_page) { return pool + (((size_t)page * nkv + head) * page_blocks + in_page / KV4_BLOCK) * (18 * D); };
+  static_assert(kEvictThreads == 2 * kMoveRows, "a thread for the scales of a row's keys, one for its values'");
+  const int mine = tid % kMoveRows, half = tid / kMoveRows * (9 * D);
+  int coming = rank * kMoveRows + mine < budget ? __ldcg(order + rank * kMoveRows + mine) : 0;  // the source of this thread's place
   for (int base = 0; base < budget; base += kMoveRows * cluster) {
     const int place0 = base + rank * kMoveRows, count = min(max(budget - place0, 0), kMoveRows);
+    if (tid < count) {
+      source[tid] = record_of(coming), source_row[tid] = coming % KV4_BLOCK;
+      target[tid] = record_of(place0 + tid);
+    }
+    __syncthreads();
+    const int next = place0 + kMoveRows * cluster + mine;
+    if (next < budget) coming = __ldcg(order + next);
+    auto code_at = [&](uint32_t record, int row, int piece) {
+      return reinterpret_cast<uint4*>(pool + (size_t)record * (18 * D) + piece / (kPieces / 2) * (9 * D) + row * (D / 2) + piece % (kPieces / 2) * 16);
+    };
+    auto scale_at = [&](uint32_t record, int row) { return reinterpret_cast<uint32_t*>(pool + (size_t)record * (18 * D) + half + 8 * D + row * kScale); };
     uint4 code[kCode];
     uint32_t scale[kScale / 4];
     float w = 0.f;
-    auto code_at = [&](int page, int in_page, int piece) {
-      const int values = piece / (kPieces / 2), c = piece % (kPieces / 2);
-      return reinterpret_cast<uint4*>(record_at(page, in_page) + values * 9 * D + in_page % KV4_BLOCK * (D / 2) + c * 16);
-    };
-    auto scale_at = [&](int page, int in_page) {
-      return reinterpret_cast<uint32_t*>(record_at(page, in_page) + (tid / kMoveRows) * 9 * D + 8 * D + in_page % KV4_BLOCK * kScale);
-    };
 #pragma unroll
     for (int i = 0; i < kCode; ++i) {
       const int x = tid + i * kEvictThreads, r = x / kPieces;
-      if (r < count) {
-        const int slot = order[place0 + r];
-        code[i] = *code_at(slot / page_size, slot % page_size, x % kPieces);
-      }
+      if (r < count) code[i] = *code_at(source[r], source_row[r], x % kPieces);
     }
-    static_assert(kEvictThreads == 2 * kMoveRows, "a thread for the scales of a row's keys, one for its values'");
-    if (tid % kMoveRows < count) {
-      const int slot = order[place0 + tid % kMoveRows], page = slot / page_size, in_page = slot % page_size;
+    if (mine < count) {
 #pragma unroll
-      for (int i = 0; i < kScale / 4; ++i) scale[i] = scale_at(page, in_page)[i];
-      if (tid < kMoveRows) w = weight_of(page, in_page);
+      for (int i = 0; i < kScale / 4; ++i) scale[i] = scale_at(source[mine], source_row[mine])[i];
+      if (half == 0) w = weight_of(source[mine], source_row[mine]);
     }
     cluster_meet();
 #pragma unroll
     for (int i = 0; i < kCode; ++i) {
-      const int x = tid + i * kEvictThreads, r = x / kPieces, place = place0 + r;
-      if (r < count) *code_at(page_of(place), place % page_size, x % kPieces) = code[i];
+      const int x = tid + i * kEvictThreads, r = x / kPieces;
+      if (r < count) *code_at(target[r], (place0 + r) % KV4_BLOCK, x % kPieces) = code[i];
     }
-    if (tid % kMoveRows < count) {
-      const int place = place0 + tid % kMoveRows, page = page_of(place);
+    if (mine < count) {
 #pragma unroll
-      for (int i = 0; i < kScale / 4; ++i) scale_at(page, place % page_size)[i] = scale[i];
-      if (tid < kMoveRows) weight_of(page, place % page_size) = w;
+      for (int i = 0; i < kScale / 4; ++i) scale_at(target[mine], (place0 + mine) % KV4_BLOCK)[i] = scale[i];
+      if (half == 0) weight_of(target[mine], place0 + mine) = w;
     }
+    __syncthreads();
   }
   // (every CTA of the cluster has read all it reads)
-  for (int row = budget + rank * kEvictThreads + tid; row < n; row += kEvictThreads * cluster) weight_of(page_of(row), row % page_size) = 0.f;
+  for (int row = budget + rank * kEvictThreads + tid; row < n; row += kEvictThreads * cluster) weight_of(record_of(row), row) = 0.f;
 }
 
 template <int D>
@@ -395,7 +412,7 @@ int launch_evict(uint8_t* pool, float* sums, const int* table, int table_stride,
   // CTAs per request and head: as many as rounds of one CTA would be, up to 8, while that fills no more than the device takes at once
   int cluster = 1;
   while (cluster < 8 && cluster * kMoveRows < budget && (long long)num_seqs * nkv * cluster < 2 * 148) cluster *= 2;
-  const int room = max_context < kKeptKeys ? max_context : kKeptKeys;  // weights that fit the shared memory
+  const int run = ((max_context + cluster - 1) / cluster + 31) / 32 * 32, room = run < kKeptKeys ? run : kKeptKeys;  // weights in shared memory
   return ts_launch_cluster(evict_kernel<D>, dim3(nkv * cluster, num_seqs), dim3(kEvictThreads), (size_t)room * 4, stream, cluster, pool, sums, table, table_stride,
                            context, new_lens, order, nkv, page_blocks, num_pages, budget, recent, first, cluster, room);
 }

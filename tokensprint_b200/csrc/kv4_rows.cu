@@ -409,9 +409,12 @@ int launch_evict(uint8_t* pool, float* sums, const int* table, int table_stride,
     if (e != cudaSuccess) return (int)e;
     set = true;
   }
-  // CTAs per request and head: as many as rounds of one CTA would be, up to 8, while that fills no more than the device takes at once
+  // CTAs per request and head: no more than there are rounds' worth of rows, four where there are few pairs of a request and a head, and eight only
+  // where there are very few, for clusters of eight find places late (us with 1 / 2 / 4 / 8: 8 pairs of 40,000 rows 384 / 203 / 79 / 48, 32 of
+  // 4,200 51 / 31 / 28 / 44, 64 of 8,190 62 / 46 / 39 / 77, 128 of 8,190 75 / 55 / 41 / 91).
+  const long long pairs = (long long)num_seqs * nkv;
   int cluster = 1;
-  while (cluster < 8 && cluster * kMoveRows < budget && (long long)num_seqs * nkv * cluster < 2 * 148) cluster *= 2;
+  while (cluster < (pairs <= 16 ? 8 : 4) && cluster * kMoveRows < budget && pairs * cluster < 2 * 148) cluster *= 2;
   const int run = ((max_context + cluster - 1) / cluster + 31) / 32 * 32, room = run < kKeptKeys ? run : kKeptKeys;  // weights in shared memory
   return ts_launch_cluster(evict_kernel<D>, dim3(nkv * cluster, num_seqs), dim3(kEvictThreads), (size_t)room * 4, stream, cluster, pool, sums, table, table_stride,
                            context, new_lens, order, nkv, page_blocks, num_pages, budget, recent, first, cluster, room);

@@ -19,32 +19,8 @@ namespace {
 
 constexpr int D = TS_HEAD_DIM;
 using Rec = Kv4Record<D>;
-#ifndef X_WARPS
-#define X_WARPS 4
-#endif
-#ifndef X_RING
-#define X_RING 4
-#endif
-#ifndef X_CTAS
-#define X_CTAS 4
-#endif
-#ifndef X_WCTAS
-#define X_WCTAS 1184
-#endif
-#ifndef X_AHEAD
-#define X_AHEAD 8
-#endif
-#ifndef X_MIN
-#define X_MIN 1
-#endif
-#ifndef X_REC
-#define X_REC 2
-#endif
-#ifndef X_CTAS2
-#define X_CTAS2 3
-#endif
-constexpr int kWarps = X_WARPS;
-constexpr int kRing = X_RING;         // records of a warp's ring
+constexpr int kWarps = 4;
+constexpr int kRing = 4;  // records of a warp's ring
 constexpr float kLowest = -3.402823466e38f;  // the running maximum before the first key (finite: no difference of it is NaN)
 constexpr int kMaxTiles = 1024;  // (sequence, row tile) pairs of a launch: a CTA keeps their key ranges in shared memory
 constexpr int kMaxParts = 64;    // most CTAs that share a key range
@@ -197,7 +173,7 @@ struct Shares {
 };
 
 template <typename T, int kTiles, int kQ, int kP, int kRecords, bool kTwice>
-__global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : kTiles == 1 ? X_CTAS : X_CTAS2) attention_kernel(const Params p) {
+__global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : kTiles == 1 ? 4 : 3) attention_kernel(const Params p) {
   // kTwice: a tile of 4 rows, which stand twice among the 8 columns; the first time with the first part of their weights, the second time
   // with the second, so that one product adds both (of 24 products a record 16 are left).
   static_assert(!kTwice || (kTiles == 1 && kP == 2), "four rows, two parts");
@@ -267,7 +243,7 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
   }
   const int total = shares.before[pairs] * p.nkv;
   // at least a step for every warp, and no range over more than kMaxParts CTAs
-  const int share = max(max(kWarps * X_MIN, (total + (int)gridDim.x - 1) / (int)gridDim.x), (most + kMaxParts - 1) / kMaxParts);
+  const int share = max(max(kWarps, (total + (int)gridDim.x - 1) / (int)gridDim.x), (most + kMaxParts - 1) / kMaxParts);
   const int begin = (int)min((long long)share * blockIdx.x, (long long)total), end = min(begin + share, total);
   if (begin >= end) return;
   auto pair_of = [&](int step) {
@@ -506,7 +482,7 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
           if (row >= tile.rows) continue;
           const float* from = p.part + ((size_t)c0 * 2 * kRows + r) * (D + 4);
           const int skip = base > c0 * share ? kRows * (D + 4) : 0;  // the first CTA may have begun with another range
-          constexpr int kStep = 2 * kRows * (D + 4), kAhead = X_AHEAD;  // parts whose loads are in flight together
+          constexpr int kStep = 2 * kRows * (D + 4), kAhead = 8;  // parts whose loads are in flight together
           RowSum sum;
           for (int first = 0; first <= c1 - c0; first += kAhead) {
             float2 ml[kAhead];
@@ -789,7 +765,7 @@ template <typename T, int kQ>
 int launch_weights(const Params& p, float* sums, int num_seqs, int max_context, int max_q, cudaStream_t stream) {
   // Few rows: a record is read, used and done with, by as many warps as run at once; with more, unpacking it once pays.
   if (max_q * p.group <= 16) {
-    const int most = (max_context + KV4_BLOCK * kWarps - 1) / (KV4_BLOCK * kWarps), want = X_WCTAS / (p.nkv * num_seqs) + 1;
+    const int most = (max_context + KV4_BLOCK * kWarps - 1) / (KV4_BLOCK * kWarps), want = 8 * 148 / (p.nkv * num_seqs) + 1;
     const dim3 grid(most < want ? most : want, p.nkv, num_seqs);
     if (max_q * p.group <= 8) return ts_launch(weights_kernel<T, kQ, 1>, grid, dim3(kWarps * 32), 0, stream, p, sums);
     return ts_launch(weights_kernel<T, kQ, 2>, grid, dim3(kWarps * 32), 0, stream, p, sums);
@@ -834,8 +810,8 @@ struct Attention {
 }  // namespace
 
 using AttentionFloat = Attention<float, 1, 3, 3, 1>;
-using AttentionFew = Attention<__nv_bfloat16, 1, 1, 2, D <= 128 ? X_REC : 1>;
-using AttentionFour = Attention<__nv_bfloat16, 1, 1, 2, D <= 128 ? X_REC : 1, true>;
+using AttentionFew = Attention<__nv_bfloat16, 1, 1, 2, D <= 128 ? 2 : 1>;
+using AttentionFour = Attention<__nv_bfloat16, 1, 1, 2, D <= 128 ? 2 : 1, true>;
 #if TS_HEAD_DIM <= 128
 using AttentionMore = Attention<__nv_bfloat16, 2, 1, 2, 1>;
 #endif

@@ -247,6 +247,26 @@ def test_portions_in_groups(monkeypatch):
     check_attention([(300, 40), (129, 128), (17, 17), (384, 70), (200, 1)], 4, 2, 128, 16, torch.bfloat16, sinks=True)
 
 
+@pytest.mark.parametrize("lens", [[(130, 130)], [(700, 512)], [(900, 40), (200, 200)]])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_portions_without_denominators(lens, sinks):
+    """Where nobody asks for the denominators a lone prompt runs on the build that takes a quarter of its exponentials from a cubic
+    (relative error below 8e-5 < 2^-13): weights off by 2^-8 + 2^-13 at most."""
+    nq, nkv, d, page = 4, 1, 128, 16
+    gen = torch.Generator().manual_seed(17)
+    pool, table, keys, values = filled(lens, nkv, d, page, gen)
+    T = sum(t for _, t in lens)
+    q = torch.randn((T, nq, d), generator=gen).to(torch.bfloat16).to(DEV)
+    sink = torch.randn(nq, generator=gen).to(DEV) if sinks else None
+    cu, context = batch(lens)
+    out = torch.empty((T, nq * d), dtype=torch.bfloat16, device=DEV)
+    ops.attention_kv4(q.flatten(1), pool, out, cu, context, table, len(lens), max(t for _, t in lens), max(n for n, _ in lens), nq, nkv, d, d**-0.5,
+                      head_sinks=sink)
+    want, _, _, spread, reach = plain.attention(q.double(), keys, values, lens, 0, sink.double() if sinks else None, d**-0.5)
+    bound = (2.0**-8 + 2.0**-13 + 2.0**-17 * (reach[..., None] + 1)) * spread + 2.0**-8 * want.abs()
+    assert ((out.double().view(T, nq, d) - want).abs() <= bound).all()
+
+
 def test_offsets_beyond_32_bits():
     """Pages whose records lie more than 4 GB into the pool."""
     page, nkv, d = 64, 2, 128
@@ -421,7 +441,7 @@ def test_refusals():
 
     call()
     for changed in ({"a0": q.half()}, {"a0": q[:, :-1]}, {"a1": pool.float()}, {"a2": q.bfloat16()}, {"a3": cu.long()}, {"a3": cu[:1]}, {"a5": table[0]},
-                    {"a6": 2}, {"a9": 3}, {"a10": 4}, {"a11": 64}, {"window": -1}, {"head_sinks": torch.zeros(3, device=DEV)},
+                    {"a6": 2}, {"a9": 3}, {"a10": 4}, {"a11": 64}, {"a12": 0.0}, {"a12": -1.0}, {"window": -1}, {"head_sinks": torch.zeros(3, device=DEV)},
                     {"lse": torch.zeros((1, 4), device=DEV, dtype=torch.float64)}, {"a2": q.clone().expand(2, -1)}):
         with pytest.raises(ops.KernelError):
             call(**changed)

@@ -2521,7 +2521,9 @@ _KV4_ATTENTION_ARGS = _struct.Struct("@11P11if").pack
 _KV4_WEIGHTS_ARGS = _struct.Struct("@8P11if").pack
 _SIGNATURES["ts_kv4_expand"] = [_c_void_p, _c_void_p, _c_int] + [_c_void_p] * 6 + [_c_int] * 6 + [_c_void_p]
 _attention_kv4: dict[int, tuple] = {}
-# Portions of prompts with more rows (tokens x query heads of a key head) than this are attended to on tcgen05 tensor cores, over rows unpacked for the step.
+# Portions of prompts with more rows (tokens x query heads of a key head) than this are attended to on tcgen05 tensor cores, over rows unpacked for
+# the step; up to it by the kernel of decoded tokens, which unpacks every code once for 16 rows (us, 16 requests of 8,000 rows with 48 / 64 / 96 rows:
+# 177 / 231 / 336 against 243 / 243 / 244; one of 2,000 rows: 24 / 21 / 25 against 23 / 23 / 25).
 ATTENTION_KV4_DIRECT_ROWS = 64
 ATTENTION_KV4_EXPAND_BYTES = 1 << 30  # most bytes of unpacked rows at a time
 _attention_kv4_tcgen05: dict[bool, object] = {}
@@ -2639,7 +2641,7 @@ def _attention_kv4_fns(head_dim: int) -> tuple:
     return fns
 
 
-def _check_attention_kv4(name, q, pool, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, d, window) -> tuple:
+def _check_attention_kv4(name, q, pool, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, d, window, scale) -> tuple:
     """Checks the arguments that attention over a 4-bit cache and its weights share; returns (pages, records per page, type code, T, entries of a
     sequence in the block table)."""
     pages, pool_heads, blocks, pool_dim = _kv4_pool(name, pool)
@@ -2650,7 +2652,7 @@ def _check_attention_kv4(name, q, pool, cu_seqlens_q, context_lens, block_table,
     if (code is not None and pool_heads == nkv and pool_dim == d and nq % nkv == 0 and q.numel() == T * nq * d and q.data_ptr() % 16 == 0
             and cu_seqlens_q.dtype is i32 and context_lens.dtype is i32 and block_table.dtype is i32 and len(table) == 2 and table[0] >= num_seqs
             and (table[1] > 0 or num_seqs == 0) and cu_seqlens_q.numel() > num_seqs and context_lens.numel() >= num_seqs
-            and min(num_seqs, max_seqlen_q, max_context, window) >= 0
+            and min(num_seqs, max_seqlen_q, max_context, window) >= 0 and scale > 0
             and q.is_cuda and cu_seqlens_q.is_cuda and context_lens.is_cuda and block_table.is_cuda
             and q.is_contiguous() and cu_seqlens_q.is_contiguous() and context_lens.is_contiguous() and block_table.is_contiguous()):
         return pages, blocks, code, T, table[1]
@@ -2668,7 +2670,7 @@ def _check_attention_kv4(name, q, pool, cu_seqlens_q, context_lens, block_table,
         raise KernelError(f"{name}: block_table must be [B, max_blocks]")
     if cu_seqlens_q.numel() < num_seqs + 1 or context_lens.numel() < num_seqs:
         raise KernelError(f"{name}: cu_seqlens_q/context_lens are shorter than the batch")
-    raise KernelError(f"{name}: negative sizes")
+    raise KernelError(f"{name}: sizes must not be negative, and the scale must be positive")
 
 
 def _attention_kv4_scratch(device: torch.device, head_dim: int, code: int, rows: int) -> tuple[int, int, torch.Tensor, torch.Tensor]:
@@ -2714,7 +2716,7 @@ def attention_kv4(
     flush_gemm_chain()
     nq, nkv, d = num_heads, num_kv_heads, head_dim
     pages, blocks, code, T, width = _check_attention_kv4("attention_kv4", q, pool, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q,
-                                                         max_context, nq, nkv, d, window)
+                                                         max_context, nq, nkv, d, window, scale)
     if out.dtype is not q.dtype or not out.is_cuda or not out.is_contiguous() or out.numel() != q.numel() or out.data_ptr() % 16:
         _cuda_contig("attention_kv4: out", out, q.dtype)
         raise KernelError(f"attention_kv4: out must be of q's size on a 16-byte boundary, got {tuple(out.shape)}")
@@ -2750,15 +2752,8 @@ def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_tabl
                             lse) -> None:
     """Portions of prompts over a 4-bit cache, heads of 128: the visible rows are unpacked into bfloat16 pages (they are exact in it), then the prompt
     attention runs over those.  Requests are taken in groups whose unpacked rows fit ATTENTION_KV4_EXPAND_BYTES."""
-    global launch_count
     d, page = ATTENTION_TCGEN05_HEAD_DIM, _KV4_EXPAND_PAGE
     scored = head_sinks is not None
-    run = _attention_kv4_tcgen05.get(scored)
-    if run is None:
-        run = _kv4_tcgen05_library(scored).ts_attention_prefill_tcgen05_scored
-        run.argtypes = _attention_tcgen05_fns()[0].argtypes + [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p]
-        run.restype = _c_int
-        _attention_kv4_tcgen05[scored] = run
     blocks = -(-max_context // page)
     pages, _, pool_blocks, _ = pool.shape
     per_seq = 2 * blocks * page * nkv * d * 2
@@ -2773,9 +2768,20 @@ def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_tabl
     runs = max(1, min(seen // _KV4_MIN_RUN, _sm_count(q.device) // ctas))
     run_blocks = -(-seen // runs) if runs > 1 else 0
     runs = -(-seen // run_blocks) if runs > 1 else 1
-    run_out = torch.empty(runs * T * nq * (d + 1), device=q.device, dtype=torch.float32) if runs > 1 else None
-    run_at = _ptr(run_out)
-    run_lse_at = None if run_out is None else run_at + runs * T * nq * d * 4
+    if lse is None and runs == 1 and num_seqs == 1:
+        # neither denominators nor runs, and no sequences to put in order: the build that has none of it, with a quarter of its exponentials
+        # off the special-function unit (a prompt of 2,048: 77 us against 80)
+        run, more = _attention_tcgen05_fns(scored)[0], ()
+    else:
+        run = _attention_kv4_tcgen05.get(scored)
+        if run is None:
+            run = _kv4_tcgen05_library(scored).ts_attention_prefill_tcgen05_scored
+            run.argtypes = _attention_tcgen05_fns()[0].argtypes + [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p]
+            run.restype = _c_int
+            _attention_kv4_tcgen05[scored] = run
+        run_out = torch.empty(runs * T * nq * (d + 1), device=q.device, dtype=torch.float32) if runs > 1 else None
+        run_at = _ptr(run_out)
+        more = (_ptr(lse), runs, run_blocks, run_at, None if run_out is None else run_at + runs * T * nq * d * 4)
     _, error = _gemm_workspace(q.device)
     for lo in range(0, num_seqs, group):
         n = min(group, num_seqs - lo)
@@ -2786,7 +2792,7 @@ def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_tabl
         _check("attention_kv4", run(
             q.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), out.data_ptr(), cu.data_ptr(), kept_lens.data_ptr(), table.data_ptr(), blocks, page,
             group * blocks * page, T, n, max_seqlen_q, nq, nkv, float(scale), int(window), 0, 0, 0.0, 0.0, _ptr(head_sinks), 0, error.data_ptr(),
-            _stream(), None, None, _ptr(lse), runs, run_blocks, run_at, run_lse_at))
+            _stream(), None, None, *more))
 
 
 def attention_kv4_weights(
@@ -2812,7 +2818,7 @@ def attention_kv4_weights(
     flush_gemm_chain()
     nq, nkv, d = num_heads, num_kv_heads, head_dim
     pages, blocks, code, T, width = _check_attention_kv4("attention_kv4_weights", q, pool, cu_seqlens_q, context_lens, block_table, num_seqs,
-                                                         max_seqlen_q, max_context, nq, nkv, d, window)
+                                                         max_seqlen_q, max_context, nq, nkv, d, window, scale)
     _cuda_contig("attention_kv4_weights: lse", lse, torch.float32)
     if lse.numel() != T * nq:
         raise KernelError(f"attention_kv4_weights: lse must have {T * nq} entries, got {lse.numel()}")

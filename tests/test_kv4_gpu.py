@@ -250,8 +250,8 @@ def test_portions_in_groups(monkeypatch):
 @pytest.mark.parametrize("lens", [[(130, 130)], [(700, 512)], [(900, 40), (200, 200)]])
 @pytest.mark.parametrize("sinks", [False, True])
 def test_portions_without_denominators(lens, sinks):
-    """Where nobody asks for the denominators a lone prompt runs on the build that takes a quarter of its exponentials from a cubic
-    (relative error below 8e-5 < 2^-13): weights off by 2^-8 + 2^-13 at most."""
+    """Nobody asks for the denominators; the first rows see one key, whose zeros stay zeros whatever the masked keys hold.  (2^-13: room
+    for exponentials from a cubic, which is not used here.)"""
     nq, nkv, d, page = 4, 1, 128, 16
     gen = torch.Generator().manual_seed(17)
     pool, table, keys, values = filled(lens, nkv, d, page, gen)

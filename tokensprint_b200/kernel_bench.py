@@ -1,7 +1,7 @@
 """Times the engine's kernels one at a time, at the layer sizes of a named preset and over a
 range of batch sizes and context lengths, and prints each one's share of its roofline.
 
-    python -m tokensprint_b200.kernel_bench [--preset qwen3-8b] [--only decode,prompt,gemm,small,layer,latent,experts]
+    python -m tokensprint_b200.kernel_bench [--preset qwen3-8b] [--only decode,prompt,gemm,small,layer,latent,experts,kv4]
 
 Every kernel runs after a read of a buffer larger than the L2 cache, so it reads its operands
 from device memory as it does inside a model step, and is timed on the device inside a CUDA graph,
@@ -379,8 +379,60 @@ def routed_experts(cfg, timer, pk, rows, device):
                 rows.append((name, f"T={T} top={top} of {E}", us, tf / (us * 1e-6), "TFLOP/s", tf / (us * 1e-6) / pk["bf16_tflops"]))
 
 
+def kv4_cache(cfg, timer, pk, rows, device):
+    """The cache in 4 bits: rows in and out, attention over it, the weights of its rows, eviction."""
+    nq, nkv, d, page = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, 16
+    row = nkv * d * 9 / 8  # bytes of a cached row, keys and values
+
+    def add(name, case, us, gb):
+        rows.append((name, case, us, gb / (us * 1e-6), "GB/s", gb / (us * 1e-6) / pk["hbm_gbs"]))
+
+    def filled(B, ctx):
+        blocks = -(-ctx // page)
+        pool = torch.zeros(ops.kv4_pool_shape(B * blocks, page, nkv, d), dtype=torch.uint8, device=device)
+        k, v = (torch.randn(B * blocks * page, nkv, d, device=device).bfloat16() for _ in range(2))
+        ops.kv4_store(k, v, pool, torch.arange(B * blocks * page, dtype=torch.int32, device=device))
+        table = torch.arange(B * blocks, device=device).int().view(B, blocks)
+        sums = torch.rand(B * blocks, nkv, page, device=device)
+        return pool, table, sums, torch.full((B,), ctx, dtype=torch.int32, device=device)
+
+    for T in (8, 8192):
+        pool = torch.zeros(ops.kv4_pool_shape(-(-T // page), page, nkv, d), dtype=torch.uint8, device=device)
+        k, v = (torch.randn(T, nkv, d, device=device).bfloat16() for _ in range(2))
+        slots = torch.randperm(T, device=device).int()
+        add("4-bit store", f"T={T}", timer(lambda: ops.kv4_store(k, v, pool, slots)), T * (row + 4 * nkv * d) / 1e9)
+        add("4-bit load", f"T={T}", timer(lambda: ops.kv4_load(pool, slots, k, v)), T * (row + 4 * nkv * d) / 1e9)
+    for B, ctx in ((1, 1024), (8, 1024), (32, 4096), (4, 32768)):
+        pool, table, sums, lens = filled(B, ctx)
+        q = torch.randn(B, nq * d, device=device).bfloat16()
+        out, lse = torch.empty_like(q), torch.empty(B, nq, device=device)
+        cu = torch.arange(B + 1, dtype=torch.int32, device=device)
+        sizes = (cu, lens, table, B, 1, ctx, nq, nkv, d, d**-0.5)
+        add("4-bit decode attention", f"B={B} ctx={ctx}", timer(lambda: ops.attention_kv4(q, pool, out, *sizes)), B * (ctx * row + 4 * nq * d) / 1e9)
+        ops.attention_kv4(q, pool, out, *sizes, lse=lse)
+        add("weights of 4-bit rows", f"B={B} ctx={ctx}", timer(lambda: ops.attention_kv4_weights(q, pool, lse, sums, *sizes)),
+            B * ctx * (row / 2 + 8 * nkv) / 1e9)
+        new = torch.empty_like(lens)
+        half = ctx // 2
+        add("eviction to half", f"B={B} ctx={ctx}", timer(lambda: ops.kv4_evict(pool, sums, table, lens, new, B, ctx, half, 64, 4)),
+            B * (8 * nkv * ctx + 2 * half * row) / 1e9)
+    for T, ctx in ((512, 2048), (2048, 2048), (8192, 8192)):
+        pool, table, sums, lens = filled(1, ctx)
+        q = torch.randn(T, nq * d, device=device).bfloat16()
+        out, lse = torch.empty_like(q), torch.empty(T, nq, device=device)
+        cu = torch.tensor([0, T], dtype=torch.int32, device=device)
+        sizes = (cu, lens, table, 1, T, ctx, nq, nkv, d, d**-0.5)
+        tf = 4 * nq * d * (T * (ctx - T) + T * (T + 1) / 2) / 1e12
+        us = timer(lambda: ops.attention_kv4(q, pool, out, *sizes))
+        rows.append(("4-bit prompt attention", f"T={T} ctx={ctx}", us, tf / (us * 1e-6), "TFLOP/s", tf / (us * 1e-6) / pk["bf16_tflops"]))
+        ops.attention_kv4(q, pool, out, *sizes, lse=lse)
+        us = timer(lambda: ops.attention_kv4_weights(q, pool, lse, sums, *sizes))
+        rows.append(("weights of 4-bit rows", f"T={T} ctx={ctx}", us, tf / 2 / (us * 1e-6), "TFLOP/s", tf / 2 / (us * 1e-6) / pk["bf16_tflops"]))
+    ops.check_device_errors()
+
+
 GROUPS = {"decode": decode_attention, "prompt": prompt_attention, "gemm": skinny_gemm, "small": small_kernels, "layer": layer_products,
-          "latent": latent_attention, "experts": routed_experts}
+          "latent": latent_attention, "experts": routed_experts, "kv4": kv4_cache}
 
 
 def main(argv=None) -> int:

@@ -2743,7 +2743,8 @@ _KV4_MIN_RUN = 3  # least key blocks of a run
 
 
 def _kv4_tcgen05_library(scored: bool = False) -> ctypes.CDLL:
-    # (the denominators are an output here: every weight from the special-function unit, none from the cubic)
+    # (every weight from the special-function unit: the cubic's 8e-5 is too much for denominators that are an output, and it gives masked keys 2^-120,
+    # not nothing; a prompt of 2,048 pays 80 us for 78)
     return _build.load_variant("attention_tcgen05", {"TS_HEAD_DIM": ATTENTION_TCGEN05_HEAD_DIM, "TS_ATT_LSE": 1, "TS_ATT_FMA_PAIRS": 0,
                                                      "TS_ATT_SCORED": int(scored)})
 
@@ -2768,20 +2769,15 @@ def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_tabl
     runs = max(1, min(seen // _KV4_MIN_RUN, _sm_count(q.device) // ctas))
     run_blocks = -(-seen // runs) if runs > 1 else 0
     runs = -(-seen // run_blocks) if runs > 1 else 1
-    if lse is None and runs == 1 and num_seqs == 1:
-        # neither denominators nor runs, and no sequences to put in order: the build that has none of it, with a quarter of its exponentials
-        # off the special-function unit (a prompt of 2,048: 77 us against 80)
-        run, more = _attention_tcgen05_fns(scored)[0], ()
-    else:
-        run = _attention_kv4_tcgen05.get(scored)
-        if run is None:
-            run = _kv4_tcgen05_library(scored).ts_attention_prefill_tcgen05_scored
-            run.argtypes = _attention_tcgen05_fns()[0].argtypes + [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p]
-            run.restype = _c_int
-            _attention_kv4_tcgen05[scored] = run
-        run_out = torch.empty(runs * T * nq * (d + 1), device=q.device, dtype=torch.float32) if runs > 1 else None
-        run_at = _ptr(run_out)
-        more = (_ptr(lse), runs, run_blocks, run_at, None if run_out is None else run_at + runs * T * nq * d * 4)
+    run = _attention_kv4_tcgen05.get(scored)
+    if run is None:
+        run = _kv4_tcgen05_library(scored).ts_attention_prefill_tcgen05_scored
+        run.argtypes = _attention_tcgen05_fns()[0].argtypes + [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p]
+        run.restype = _c_int
+        _attention_kv4_tcgen05[scored] = run
+    run_out = torch.empty(runs * T * nq * (d + 1), device=q.device, dtype=torch.float32) if runs > 1 else None
+    run_at = _ptr(run_out)
+    more = (_ptr(lse), runs, run_blocks, run_at, None if run_out is None else run_at + runs * T * nq * d * 4)
     _, error = _gemm_workspace(q.device)
     for lo in range(0, num_seqs, group):
         n = min(group, num_seqs - lo)

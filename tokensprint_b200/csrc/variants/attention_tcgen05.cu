@@ -1385,7 +1385,9 @@ TS_EXPORT int ts_latent_rebuilt_attention(const void* q, long long ld_q, const v
 // by TMA as the second, so that S^T[key][row] lies in tensor memory with a key per lane: a thread adds up its own key's weights in a
 // register, nothing is exchanged until the end.  What bounds it is the special-function unit, 16 exponentials a clock for 16,384 of a
 // tile; the products take half as long and run on the other buffer meanwhile.
-constexpr int W_STAGES = 2;
+constexpr int W_STAGES = 2, W_SLICES = 4;  // W_SLICES: warps that share a quarter of the keys, each with as many of a tile's rows
+constexpr int W_ADDERS = 4 * W_SLICES, W_COLUMNS = BM / W_SLICES;
+static_assert(W_COLUMNS == 32, "one load of tensor memory");
 constexpr uint32_t W_OFF_Q = 2 * BM * 128, W_SMEM = W_OFF_Q + W_STAGES * Q_BYTES, W_TMEM_COLS = 256;
 struct WeightParams {
   const uint8_t* pool;
@@ -1396,7 +1398,7 @@ struct WeightParams {
   int table_stride, page_blocks, num_pages, tokens, nq, nkv, window;
   float scale_log2;
 };
-__global__ void __launch_bounds__(320, 2) kv4_weights_kernel(const __grid_constant__ CUtensorMap map_q, const WeightParams p) {
+__global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(const __grid_constant__ CUtensorMap map_q, const WeightParams p) {
   ts_pdl_wait();  // (tensor memory is never held while waiting for another kernel)
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
@@ -1405,7 +1407,7 @@ __global__ void __launch_bounds__(320, 2) kv4_weights_kernel(const __grid_consta
   __shared__ int abort_s;
   __shared__ __align__(16) float lse_s[2][BM];
   __shared__ __align__(16) int pos_s[2][BM];
-  __shared__ float half_s[BM];
+  __shared__ float slice_s[W_SLICES][BM];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hk = blockIdx.y, b = blockIdx.z, G = p.nq / p.nkv, page_size = p.page_blocks * KV4_BLOCK;
   const int q_begin = min(max(p.cu[b], 0), p.tokens), q_len = min(max(p.cu[b + 1], q_begin), p.tokens) - q_begin;
@@ -1421,19 +1423,20 @@ __global__ void __launch_bounds__(320, 2) kv4_weights_kernel(const __grid_consta
   if (tid == 0) {
     abort_s = 0;
     for (int i = 0; i < W_STAGES; ++i) mbar_init(smem_u32(&q_full[i]), 1), mbar_init(smem_u32(&q_empty[i]), 1);
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_full[i]), 1), mbar_init(smem_u32(&s_empty[i]), 8);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_full[i]), 1), mbar_init(smem_u32(&s_empty[i]), W_ADDERS);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
+  if (warp == W_ADDERS + 1) {
     __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(W_TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (tid < 256) {
+  constexpr int adders = W_ADDERS * 32;
+  if (tid < adders) {
     // the keys, unpacked: 16 bytes (8 channels) at a time to their places in the swizzled operand; keys that are none as zeros
 #pragma unroll
-    for (int i = 0; i < BM * 16 / 256; ++i) {
-      const int x = tid + 256 * i, row = x >> 4, c = x & 15, key = key0 + row;
+    for (int i = 0; i < BM * 16 / adders; ++i) {
+      const int x = tid + adders * i, row = x >> 4, c = x & 15, key = key0 + row;
       uint4 out = make_uint4(0u, 0u, 0u, 0u);
       if (key < ctx) {
         const int page = min(max(table[key / page_size], 0), p.num_pages - 1), in_page = key % page_size;
@@ -1445,7 +1448,7 @@ __global__ void __launch_bounds__(320, 2) kv4_weights_kernel(const __grid_consta
       *reinterpret_cast<uint4*>(smem + (c >> 3) * (BM * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = out;
     }
     // rows of the query tiles that no copy fills: zeros
-    for (int i = tid; i < W_STAGES * 2 * (BM - RT) * 8; i += 256) {
+    for (int i = tid; i < W_STAGES * 2 * (BM - RT) * 8; i += adders) {
       const int half = i / ((BM - RT) * 8), rest = i % ((BM - RT) * 8);
       *reinterpret_cast<uint4*>(smem + W_OFF_Q + half * (BM * 128) + (RT + rest / 8) * 128 + (rest % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
@@ -1458,7 +1461,7 @@ __global__ void __launch_bounds__(320, 2) kv4_weights_kernel(const __grid_consta
   const uint32_t tmem_base = tmem_base_s, sm = smem_u32(smem);
   volatile int* abort_flag = &abort_s;
 
-  if (warp == 8) {
+  if (warp == W_ADDERS) {
     int issued = 0;
     for (int j = 0; j < tiles; ++j) {
       const int st = j % W_STAGES;
@@ -1473,7 +1476,7 @@ __global__ void __launch_bounds__(320, 2) kv4_weights_kernel(const __grid_consta
     int patience = 0;
     for (int j = max(0, issued - W_STAGES); j < issued; ++j) mbar_wait(smem_u32(&q_full[j % W_STAGES]), (uint32_t)(j / W_STAGES) & 1, &patience);
     if (patience != 0) *abort_flag = 1;
-  } else if (warp == 9) {
+  } else if (warp == W_ADDERS + 1) {
     const uint64_t k_desc = desc_k_major(sm), q_desc = desc_k_major(sm + W_OFF_Q);
     int asked = 0;
     for (int j = 0; j < tiles; ++j) {
@@ -1504,9 +1507,9 @@ __global__ void __launch_bounds__(320, 2) kv4_weights_kernel(const __grid_consta
     }
     if (patience != 0) *abort_flag = 1;
   } else {
-    // ---- a thread per key and half of a tile's rows
+    // ---- a thread per key and a slice of a tile's rows
     const int quad = warp & 3, h = warp >> 2, row = quad * 32 + lane, key = key0 + row;
-    const uint32_t addr = tmem_base + ((uint32_t)(quad * 32) << 16) + h * 64;
+    const uint32_t addr = tmem_base + ((uint32_t)(quad * 32) << 16) + h * W_COLUMNS;
     auto tell = [&](int j) {  // a tile's rows: their logarithms and last visible keys; rows that are none give no weight
       if (tid < BM) {
         const int token = (tile0 + j) * per_tile + tid / G;
@@ -1519,7 +1522,7 @@ __global__ void __launch_bounds__(320, 2) kv4_weights_kernel(const __grid_consta
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // tile j's rows are told, tile j - 1's have been read
+      asm volatile("bar.sync 1, %0;" ::"n"(adders) : "memory");  // tile j's rows are told, tile j - 1's have been read
       if (j + 1 < tiles) tell(j + 1);
       const int buf = j & 1;
       if (ok) ok = mbar_wait(smem_u32(&s_full[buf]), (uint32_t)(j / 2) & 1, abort_flag);
@@ -1528,33 +1531,30 @@ __global__ void __launch_bounds__(320, 2) kv4_weights_kernel(const __grid_consta
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const int first = (tile0 + j) * per_tile, last = first + per_tile - 1;  // the tile's tokens
         const bool all = last < q_len && before + first >= last_key && (p.window == 0 || before + last - p.window < key0);
+        uint32_t v[W_COLUMNS];
+        tmem_ld32(addr + buf * BM, v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        const float4* lse = reinterpret_cast<const float4*>(&lse_s[buf][h * W_COLUMNS]);
+        const int4* pos = reinterpret_cast<const int4*>(&pos_s[buf][h * W_COLUMNS]);
+        if (all) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t v[32];
-          tmem_ld32(addr + buf * BM + c * 32, v);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          const float4* lse = reinterpret_cast<const float4*>(&lse_s[buf][h * 64 + c * 32]);
-          const int4* pos = reinterpret_cast<const int4*>(&pos_s[buf][h * 64 + c * 32]);
-          if (all) {
+          for (int i = 0; i < W_COLUMNS / 4; ++i) {
+            const float4 l = lse[i];
+            sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
+            sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
+            sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
+            sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
+          }
+        } else {
+          const int oldest = p.window > 0 ? p.window : 0x7fffffff;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 l = lse[i];
-              sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
-              sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
-              sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
-              sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
-            }
-          } else {
-            const int oldest = p.window > 0 ? p.window : 0x7fffffff;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 l = lse[i];
-              const int4 q = pos[i];
-              if (key <= q.x && q.x - key < oldest) sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
-              if (key <= q.y && q.y - key < oldest) sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
-              if (key <= q.z && q.z - key < oldest) sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
-              if (key <= q.w && q.w - key < oldest) sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
-            }
+          for (int i = 0; i < W_COLUMNS / 4; ++i) {
+            const float4 l = lse[i];
+            const int4 q = pos[i];
+            if (key <= q.x && q.x - key < oldest) sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
+            if (key <= q.y && q.y - key < oldest) sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
+            if (key <= q.z && q.z - key < oldest) sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
+            if (key <= q.w && q.w - key < oldest) sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
           }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1563,17 +1563,17 @@ __global__ void __launch_bounds__(320, 2) kv4_weights_kernel(const __grid_consta
       }
     }
     const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    if (h == 1) half_s[row] = total;
-    asm volatile("bar.sync 1, 256;" ::: "memory");
+    slice_s[h][row] = total;
+    asm volatile("bar.sync 1, %0;" ::"n"(adders) : "memory");
     if (h == 0 && key < ctx && abort_s == 0) {
       const int page = min(max(table[key / page_size], 0), p.num_pages - 1);
-      p.sums[((size_t)page * p.nkv + hk) * page_size + key % page_size] += total + half_s[row];
+      p.sums[((size_t)page * p.nkv + hk) * page_size + key % page_size] += (slice_s[0][row] + slice_s[1][row]) + (slice_s[2][row] + slice_s[3][row]);
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (abort_s != 0 && tid == 0) *p.error = 1;
-  if (warp == 9) {
+  if (warp == W_ADDERS + 1) {
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(W_TMEM_COLS) : "memory");
   }
@@ -1793,7 +1793,7 @@ TS_EXPORT int ts_kv4_weights_tcgen05(const void* q, const void* pool, const floa
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
-  return ts_launch(kv4_weights_kernel, dim3((max_context + BM - 1) / BM, nkv, B), dim3(320), smem, (cudaStream_t)stream, mq, p);
+  return ts_launch(kv4_weights_kernel, dim3((max_context + BM - 1) / BM, nkv, B), dim3((W_ADDERS + 2) * 32), smem, (cudaStream_t)stream, mq, p);
 }
 #endif
 #else

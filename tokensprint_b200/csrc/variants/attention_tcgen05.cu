@@ -1385,7 +1385,7 @@ TS_EXPORT int ts_latent_rebuilt_attention(const void* q, long long ld_q, const v
 // by TMA as the second, so that S^T[key][row] lies in tensor memory with a key per lane: a thread adds up its own key's weights in a
 // register, nothing is exchanged until the end.  What bounds it is the special-function unit, 16 exponentials a clock for 16,384 of a
 // tile; the products take half as long and run on the other buffer meanwhile.
-constexpr int W_STAGES = 2, W_SLICES = 4;  // W_SLICES: warps that share a quarter of the keys, each with as many of a tile's rows
+constexpr int W_STAGES = 4, W_SLICES = 4;  // W_SLICES: warps that share a quarter of the keys, each with as many of a tile's rows
 constexpr int W_ADDERS = 4 * W_SLICES, W_COLUMNS = BM / W_SLICES;
 static_assert(W_COLUMNS == 32, "one load of tensor memory");
 constexpr uint32_t W_OFF_Q = 2 * BM * 128, W_SMEM = W_OFF_Q + W_STAGES * Q_BYTES, W_TMEM_COLS = 256;
@@ -1501,29 +1501,37 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
     }
     // and no product, nor the arrival that reports one
     int patience = 0;
-    for (int j = max(0, asked - 2); j < asked; ++j) {
-      mbar_wait(smem_u32(&q_empty[j % W_STAGES]), (uint32_t)(j / W_STAGES) & 1, &patience);
-      mbar_wait(smem_u32(&s_full[j & 1]), (uint32_t)(j / 2) & 1, &patience);
-    }
+    for (int j = max(0, asked - W_STAGES); j < asked; ++j) mbar_wait(smem_u32(&q_empty[j % W_STAGES]), (uint32_t)(j / W_STAGES) & 1, &patience);
+    for (int j = max(0, asked - 2); j < asked; ++j) mbar_wait(smem_u32(&s_full[j & 1]), (uint32_t)(j / 2) & 1, &patience);
     if (patience != 0) *abort_flag = 1;
   } else {
     // ---- a thread per key and a slice of a tile's rows
     const int quad = warp & 3, h = warp >> 2, row = quad * 32 + lane, key = key0 + row;
     const uint32_t addr = tmem_base + ((uint32_t)(quad * 32) << 16) + h * W_COLUMNS;
-    auto tell = [&](int j) {  // a tile's rows: their logarithms and last visible keys; rows that are none give no weight
-      if (tid < BM) {
-        const int token = (tile0 + j) * per_tile + tid / G;
-        const bool there = tid < RT && token < q_len;
-        lse_s[j & 1][tid] = there ? p.lse[(size_t)(q_begin + token) * p.nq + hk * G + tid % G] * 1.4426950408889634f : INFINITY;
-        pos_s[j & 1][tid] = there ? before + token : -1;
-      }
+    // A tile's rows: their logarithms and last visible keys; rows that are none give no weight.  Asked for a tile before they are told, so that nobody
+    // waits for them.
+    float told_lse = INFINITY;
+    int told_pos = -1;
+    auto ask = [&](int j) {
+      const int token = (tile0 + j) * per_tile + tid / G;
+      const bool there = tid < RT && token < q_len && j < tiles;
+      told_lse = there ? p.lse[(size_t)(q_begin + token) * p.nq + hk * G + tid % G] : INFINITY;
+      told_pos = there ? before + token : -1;
     };
-    tell(0);
+    auto tell = [&](int j) { lse_s[j & 1][tid] = told_lse * 1.4426950408889634f, pos_s[j & 1][tid] = told_pos; };
+    if (tid < BM) {
+      ask(0);
+      tell(0);
+      ask(1);
+    }
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
       asm volatile("bar.sync 1, %0;" ::"n"(adders) : "memory");  // tile j's rows are told, tile j - 1's have been read
-      if (j + 1 < tiles) tell(j + 1);
+      if (tid < BM) {
+        tell(j + 1);
+        ask(j + 2);
+      }
       const int buf = j & 1;
       if (ok) ok = mbar_wait(smem_u32(&s_full[buf]), (uint32_t)(j / 2) & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);

@@ -1385,9 +1385,8 @@ TS_EXPORT int ts_latent_rebuilt_attention(const void* q, long long ld_q, const v
 // by TMA as the second, so that S^T[key][row] lies in tensor memory with a key per lane: a thread adds up its own key's weights in a
 // register, nothing is exchanged until the end.  What bounds it is the special-function unit, 16 exponentials a clock for 16,384 of a
 // tile; the products take half as long and run on the other buffer meanwhile.
-constexpr int W_STAGES = 4, W_SLICES = 4;  // W_SLICES: warps that share a quarter of the keys, each with as many of a tile's rows
-constexpr int W_ADDERS = 4 * W_SLICES, W_COLUMNS = BM / W_SLICES;
-static_assert(W_COLUMNS == 32, "one load of tensor memory");
+constexpr int W_STAGES = 4, W_GROUP = 8, W_ADDERS = 2 * W_GROUP;  // warps that add; two groups of them take the tiles in turn
+constexpr int W_COLUMNS = BM / (W_GROUP / 4);                      // a tile's rows that a warp adds up
 constexpr uint32_t W_OFF_Q = 2 * BM * 128, W_SMEM = W_OFF_Q + W_STAGES * Q_BYTES, W_TMEM_COLS = 256;
 struct WeightParams {
   const uint8_t* pool;
@@ -1405,9 +1404,9 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
   __shared__ __align__(8) uint64_t q_full[W_STAGES], q_empty[W_STAGES], s_full[2], s_empty[2];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
-  __shared__ __align__(16) float lse_s[2][BM];
-  __shared__ __align__(16) int pos_s[2][BM];
-  __shared__ float slice_s[W_SLICES][BM];
+  __shared__ __align__(16) float lse_s[2][2][BM];  // [group][its tiles in turn][row]
+  __shared__ __align__(16) int pos_s[2][2][BM];
+  __shared__ float slice_s[W_ADDERS / 4][BM];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hk = blockIdx.y, b = blockIdx.z, G = p.nq / p.nkv, page_size = p.page_blocks * KV4_BLOCK;
   const int q_begin = min(max(p.cu[b], 0), p.tokens), q_len = min(max(p.cu[b + 1], q_begin), p.tokens) - q_begin;
@@ -1423,7 +1422,7 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
   if (tid == 0) {
     abort_s = 0;
     for (int i = 0; i < W_STAGES; ++i) mbar_init(smem_u32(&q_full[i]), 1), mbar_init(smem_u32(&q_empty[i]), 1);
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_full[i]), 1), mbar_init(smem_u32(&s_empty[i]), W_ADDERS);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_full[i]), 1), mbar_init(smem_u32(&s_empty[i]), W_GROUP);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == W_ADDERS + 1) {
@@ -1505,75 +1504,79 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
     for (int j = max(0, asked - 2); j < asked; ++j) mbar_wait(smem_u32(&s_full[j & 1]), (uint32_t)(j / 2) & 1, &patience);
     if (patience != 0) *abort_flag = 1;
   } else {
-    // ---- a thread per key and a slice of a tile's rows
-    const int quad = warp & 3, h = warp >> 2, row = quad * 32 + lane, key = key0 + row;
-    const uint32_t addr = tmem_base + ((uint32_t)(quad * 32) << 16) + h * W_COLUMNS;
+    // ---- a thread per key and a slice of a tile's rows; group g takes the tiles g, g + 2, ...
+    const int quad = warp & 3, h = (warp >> 2) & 1, g = warp / W_GROUP, member = tid % (W_GROUP * 32), row = quad * 32 + lane, key = key0 + row;
+    const uint32_t addr = tmem_base + ((uint32_t)(quad * 32) << 16) + g * BM + h * W_COLUMNS;
     // A tile's rows: their logarithms and last visible keys; rows that are none give no weight.  Asked for a tile before they are told, so that nobody
     // waits for them.
     float told_lse = INFINITY;
     int told_pos = -1;
     auto ask = [&](int j) {
-      const int token = (tile0 + j) * per_tile + tid / G;
-      const bool there = tid < RT && token < q_len && j < tiles;
-      told_lse = there ? p.lse[(size_t)(q_begin + token) * p.nq + hk * G + tid % G] : INFINITY;
+      const int token = (tile0 + j) * per_tile + member / G;
+      const bool there = member < RT && token < q_len && j < tiles;
+      told_lse = there ? p.lse[(size_t)(q_begin + token) * p.nq + hk * G + member % G] : INFINITY;
       told_pos = there ? before + token : -1;
     };
-    auto tell = [&](int j) { lse_s[j & 1][tid] = told_lse * 1.4426950408889634f, pos_s[j & 1][tid] = told_pos; };
-    if (tid < BM) {
-      ask(0);
-      tell(0);
-      ask(1);
+    auto tell = [&](int j) { lse_s[g][(j >> 1) & 1][member] = told_lse * 1.4426950408889634f, pos_s[g][(j >> 1) & 1][member] = told_pos; };
+    if (member < BM) {
+      ask(g);
+      tell(g);
+      ask(g + 2);
     }
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     bool ok = true;
-    for (int j = 0; j < tiles; ++j) {
-      asm volatile("bar.sync 1, %0;" ::"n"(adders) : "memory");  // tile j's rows are told, tile j - 1's have been read
-      if (tid < BM) {
-        tell(j + 1);
-        ask(j + 2);
+    for (int j = g; j < tiles; j += 2) {
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(W_GROUP * 32) : "memory");  // tile j's rows are told, tile j - 2's have been read
+      if (member < BM) {
+        tell(j + 2);
+        ask(j + 4);
       }
-      const int buf = j & 1;
-      if (ok) ok = mbar_wait(smem_u32(&s_full[buf]), (uint32_t)(j / 2) & 1, abort_flag);
+      const int turn = (j >> 1) & 1;
+      if (ok) ok = mbar_wait(smem_u32(&s_full[g]), (uint32_t)turn, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const int first = (tile0 + j) * per_tile, last = first + per_tile - 1;  // the tile's tokens
         const bool all = last < q_len && before + first >= last_key && (p.window == 0 || before + last - p.window < key0);
-        uint32_t v[W_COLUMNS];
-        tmem_ld32(addr + buf * BM, v);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        const float4* lse = reinterpret_cast<const float4*>(&lse_s[buf][h * W_COLUMNS]);
-        const int4* pos = reinterpret_cast<const int4*>(&pos_s[buf][h * W_COLUMNS]);
-        if (all) {
+        const int oldest = p.window > 0 ? p.window : 0x7fffffff;
 #pragma unroll
-          for (int i = 0; i < W_COLUMNS / 4; ++i) {
-            const float4 l = lse[i];
-            sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
-            sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
-            sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
-            sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
+        for (int part = 0; part < W_COLUMNS / 32; ++part) {
+          uint32_t v[32];
+          tmem_ld32(addr + part * 32, v);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          if (part == W_COLUMNS / 32 - 1) {  // the scores are in registers: the next but one product may begin
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&s_empty[g]));
           }
-        } else {
-          const int oldest = p.window > 0 ? p.window : 0x7fffffff;
+          const float4* lse = reinterpret_cast<const float4*>(&lse_s[g][turn][h * W_COLUMNS + part * 32]);
+          const int4* pos = reinterpret_cast<const int4*>(&pos_s[g][turn][h * W_COLUMNS + part * 32]);
+          if (all) {
 #pragma unroll
-          for (int i = 0; i < W_COLUMNS / 4; ++i) {
-            const float4 l = lse[i];
-            const int4 q = pos[i];
-            if (key <= q.x && q.x - key < oldest) sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
-            if (key <= q.y && q.y - key < oldest) sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
-            if (key <= q.z && q.z - key < oldest) sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
-            if (key <= q.w && q.w - key < oldest) sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
+            for (int i = 0; i < 8; ++i) {
+              const float4 l = lse[i];
+              sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
+              sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
+              sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
+              sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 l = lse[i];
+              const int4 q = pos[i];
+              if (key <= q.x && q.x - key < oldest) sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
+              if (key <= q.y && q.y - key < oldest) sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
+              if (key <= q.z && q.z - key < oldest) sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
+              if (key <= q.w && q.w - key < oldest) sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
+            }
           }
         }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&s_empty[buf]));
       }
     }
-    const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    slice_s[h][row] = total;
-    asm volatile("bar.sync 1, %0;" ::"n"(adders) : "memory");
-    if (h == 0 && key < ctx && abort_s == 0) {
+    slice_s[warp >> 2][row] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    asm volatile("bar.sync 3, %0;" ::"n"(adders) : "memory");
+    if (warp < 4 && key < ctx && abort_s == 0) {
       const int page = min(max(table[key / page_size], 0), p.num_pages - 1);
       p.sums[((size_t)page * p.nkv + hk) * page_size + key % page_size] += (slice_s[0][row] + slice_s[1][row]) + (slice_s[2][row] + slice_s[3][row]);
     }

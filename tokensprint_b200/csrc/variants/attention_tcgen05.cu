@@ -1232,20 +1232,35 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
         p.lse[at] = row_lse(p, m_run, l_run);
       }
     }
-    if (good && p.run_blocks > 0) {
-      const size_t of_run = (size_t)run * p.tokens * p.nq + (size_t)(q_begin + r / G) * p.nq + hk * G + r % G;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (p.run_blocks > 0) {
+      // Through shared memory (everything that lay there is done with), so that rows leave as whole lines of 512 bytes: 16-byte piece c of a row at
+      // c ^ row % 32.  (A thread's own row in pieces of 16 bytes, as it has them, took 6.5 us for 256 rows.)
+      unsigned char* run_tile = smem + P2_OFF_Q + t * (BM * D * 4);
+      static_assert(P2_OFF_Q + 2 * BM * D * 4 <= P2_SMEM, "both tiles in 32 bits");
+      if (good) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t v[32];
-        tmem_ld32(o_addr + c * 32, v);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (row < RT && r < rows_total) {
-          float4* dst = reinterpret_cast<float4*>(p.run_out + of_run * D + h * 64 + c * 32);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[32];
+          tmem_ld32(o_addr + c * 32, v);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            dst[i] = make_float4(__uint_as_float(v[4 * i]) * inv, __uint_as_float(v[4 * i + 1]) * inv, __uint_as_float(v[4 * i + 2]) * inv,
-                                 __uint_as_float(v[4 * i + 3]) * inv);
+            *reinterpret_cast<float4*>(run_tile + row * (D * 4) + (((h * 16 + c * 8 + i) ^ (row & 31)) << 4)) =
+                make_float4(__uint_as_float(v[4 * i]) * inv, __uint_as_float(v[4 * i + 1]) * inv, __uint_as_float(v[4 * i + 2]) * inv,
+                            __uint_as_float(v[4 * i + 3]) * inv);
+        }
+      }
+      asm volatile("bar.sync %0, 256;" ::"r"(1 + t) : "memory");
+      if (good) {
+#pragma unroll 4
+        for (int it = 0; it < BM / 8; ++it) {
+          const int rr = it * 8 + (warp & 7), rg = r0 + t * RT + rr;
+          if (rr < RT && rg < rows_total) {
+            const size_t of_run = (size_t)run * p.tokens * p.nq + (size_t)(q_begin + rg / G) * p.nq + hk * G + rg % G;
+            *reinterpret_cast<float4*>(p.run_out + of_run * D + lane * 4) =
+                *reinterpret_cast<const float4*>(run_tile + rr * (D * 4) + ((lane ^ (rr & 31)) << 4));
+          }
         }
       }
     }
@@ -1607,21 +1622,28 @@ __global__ void __launch_bounds__(256) join_runs_kernel(const Params p) {
   const int lo = first_visible_key(p, start_pos + r0 / G), hi = start_pos + (min(r0 + 2 * RT, rows_total) - 1) / G;
   const int runs = min(max(1, (hi / PBN - lo / PBN + p.run_blocks) / p.run_blocks), p.runs);
   const size_t at = (size_t)(q_begin + token) * p.nq + head, step = (size_t)p.tokens * p.nq;
-  float top = -INFINITY;
-#pragma unroll 4
-  for (int i = 0; i < runs; ++i) top = fmaxf(top, p.run_lse[at + i * step]);
-  float sum = 0.f, o[16];
+  float top = -INFINITY, sum = 0.f, o[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) o[i] = 0.f;
-#pragma unroll 2
-  for (int i = 0; i < runs; ++i) {
-    const float f = top == -INFINITY ? 0.f : fast_exp2((p.run_lse[at + i * step] - top) * 1.4426950408889634f);
-    const float4* from = reinterpret_cast<const float4*>(p.run_out + (at + i * step) * D) + lane;
-    sum += f;
+  for (int i0 = 0; i0 < runs; i0 += 2) {  // two at a time, their loads in flight together
+    const bool two = i0 + 1 < runs;
+    float lse[2];
+    float4 v[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const size_t of_run = at + (two ? i0 + i : i0) * step;
+      lse[i] = i == 0 || two ? p.run_lse[of_run] : -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[i][c] = reinterpret_cast<const float4*>(p.run_out + of_run * D)[lane + 8 * c];
+    }
+    const float higher = fmaxf(top, fmaxf(lse[0], lse[1])), base = higher == -INFINITY ? 0.f : higher;
+    const float f0 = fast_exp2((lse[0] - base) * 1.4426950408889634f), f1 = fast_exp2((lse[1] - base) * 1.4426950408889634f);
+    const float keep = fast_exp2((top - base) * 1.4426950408889634f);
+    top = higher, sum = sum * keep + (f0 + f1);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const float4 v = from[8 * c];
-      o[4 * c] += f * v.x, o[4 * c + 1] += f * v.y, o[4 * c + 2] += f * v.z, o[4 * c + 3] += f * v.w;
+      o[4 * c] = o[4 * c] * keep + (f0 * v[0][c].x + f1 * v[1][c].x), o[4 * c + 1] = o[4 * c + 1] * keep + (f0 * v[0][c].y + f1 * v[1][c].y);
+      o[4 * c + 2] = o[4 * c + 2] * keep + (f0 * v[0][c].z + f1 * v[1][c].z), o[4 * c + 3] = o[4 * c + 3] * keep + (f0 * v[0][c].w + f1 * v[1][c].w);
     }
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;

@@ -726,6 +726,9 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
                                                                         int k_rot_column, int q_rot_first,
 #endif
                                                                         const Params p) {
+#if TS_ATT_LSE
+  if (threadIdx.x < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(threadIdx.x == 0 ? &map_q : &map_k) : "memory");
+#endif
   ts_pdl_wait();  // see the other kernel: tensor memory is never held while waiting for another kernel
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
@@ -735,6 +738,9 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
   __shared__ int abort_s;
   __shared__ int table_s[REBUILT ? 1 : MAX_TABLE];  // REBUILT: the row of the sequence's key 0 (may be negative)
   __shared__ int quit_s[2][4][2];   // [tile][quarter of the rows][block parity]: see the softmax warps
+#if TS_ATT_LSE
+  __shared__ int place_s[2][BM];  // [tile][row]: where its result goes, in rows of heads, or -1
+#endif
   __shared__ float sum_s[2][2][BM];  // [tile][half of the keys][row]: what the two threads of a row tell each other (a block's largest score; at the end their sums)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -814,6 +820,13 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+#if TS_ATT_LSE
+    // the queries, before the block table is looked at
+    mbar_expect_tx(smem_u32(&q_full), (uint32_t)(ntiles * 2 * RT * 128));  // per tile two half-head boxes of RT rows
+    for (int t = 0; t < ntiles; ++t)
+      for (int half = 0; half < 2; ++half)
+        tma_load_4d(smem_u32(smem) + P2_OFF_Q + t * PQ_BYTES + half * (BM * 128), &map_q, smem_u32(&q_full), half * 64, 0, hk, q_begin + (r0 + t * RT) / G);
+#endif
   }
 #if TS_ATT_ROT
   if (warp == 16) {
@@ -873,6 +886,7 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
     }
     const int key0_row = table_s[0];
 #else
+#if !TS_ATT_LSE  // (there they are on their way)
     if (lane == 0) {
       mbar_expect_tx(smem_u32(&q_full), (uint32_t)(ntiles * 2 * RT * 128));  // per tile two half-head boxes of RT rows
       for (int t = 0; t < ntiles; ++t)
@@ -880,6 +894,7 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
           tma_load_4d(sm + P2_OFF_Q + t * PQ_BYTES + half * (BM * 128), &map_q, smem_u32(&q_full), half * 64, 0, hk,
                       q_begin + (r0 + t * RT) / G);
     }
+#endif
     const int c = lane >> 1, half = lane & 1;  // this lane's copy within a block, and its half of the head
     const bool copies = c < copies_per_block;
     const uint32_t lane_off = (uint32_t)half * PKV_HALF + (uint32_t)(c * box_rows) * 128u;
@@ -1028,6 +1043,11 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
     const int r = r0 + t * RT + row;
     const int row_pos = (row < RT && r < rows_total) ? start_pos + r / G : -1;
     const int row_lo = row_pos >= 0 ? first_visible_key(p, row_pos) : 0;
+#if TS_ATT_LSE
+    // (worked out once: with the divisions in it, the loop over the rows at the end took 2.9 us)
+    const int place = row < RT && r < rows_total ? (q_begin + r / G) * p.nq + hk * G + r % G : -1;
+    if (h == 0) place_s[t][row] = place;
+#endif
     float dist_a = 0.f, dist_b = 0.f;
     if (has_distance(p) && row_pos >= 0) row_distance(p, hk, G, r, dist_a, dist_b);
     const int tile_first_pos = start_pos + (r0 + t * RT) / G;
@@ -1223,8 +1243,8 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
     l_run += sum_s[t][h ^ 1][row];
     float inv = l_run > 0.f ? 1.f / l_run : 0.f;
 #if TS_ATT_LSE
-    if (good && row < RT && r < rows_total) {
-      const size_t at = (size_t)(q_begin + r / G) * p.nq + hk * G + r % G;
+    if (good && place >= 0) {
+      const size_t at = place;
       if (p.run_blocks > 0) {  // a run's row, as it is in 32 bits
         const size_t of_run = (size_t)run * p.tokens * p.nq + at;
         if (h == 0) p.run_lse[of_run] = row_lse(p, m_run, l_run);
@@ -1255,9 +1275,9 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
       if (good) {
 #pragma unroll 4
         for (int it = 0; it < BM / 8; ++it) {
-          const int rr = it * 8 + (warp & 7), rg = r0 + t * RT + rr;
-          if (rr < RT && rg < rows_total) {
-            const size_t of_run = (size_t)run * p.tokens * p.nq + (size_t)(q_begin + rg / G) * p.nq + hk * G + rg % G;
+          const int rr = it * 8 + (warp & 7), at = place_s[t][rr];
+          if (at >= 0) {
+            const size_t of_run = (size_t)run * p.tokens * p.nq + at;
             *reinterpret_cast<float4*>(p.run_out + of_run * D + lane * 4) =
                 *reinterpret_cast<const float4*>(run_tile + rr * (D * 4) + ((lane ^ (rr & 31)) << 4));
           }
@@ -1300,12 +1320,18 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
       for (int it = 0; it < 8; ++it) {
         const int idx = it * 2 * BM + me;
         const int rr = idx >> 4, piece = idx & 15;
+#if TS_ATT_LSE
+        const int at = place_s[t][rr];
+        if (at >= 0)
+          *reinterpret_cast<uint4*>(p.out + (size_t)at * D + piece * 8) = *reinterpret_cast<const uint4*>(o_tile + rr * 256 + ((piece ^ (rr & 15)) << 4));
+#else
         const int rg = r0 + t * RT + rr;
         if (rr < RT && rg < rows_total) {
           const uint4 chunk = *reinterpret_cast<const uint4*>(o_tile + rr * 256 + ((piece ^ (rr & 15)) << 4));
           __nv_bfloat16* dst = p.out + ((size_t)(q_begin + rg / G) * p.nq + hk * G + rg % G) * D + piece * 8;
           *reinterpret_cast<uint4*>(dst) = chunk;
         }
+#endif
       }
     }
   }

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
   static_assert(!kTwice || (kTiles == 1 && kP == 2), "four rows, two parts");
   constexpr int kRows = kTwice ? 4 : 8 * kTiles, kParts = kTwice ? 1 : kP, kColumnRows = kTwice ? 4 : 8;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int scratch[2 * kWarps + 1];  // the warps' sums, whether this CTA joins a range, the warps' largest
+  __shared__ int scratch[kWarps + 2];
   ts_pdl_prologue();
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   const int pairs = p.num_seqs * p.row_tiles;
@@ -195,11 +195,11 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
   };
   auto first_record = [&](const Tile& tile) { return p.window > 0 ? max(0, tile.position(p, tile.first_row) - p.window + 1) / KV4_BLOCK : 0; };
   // ---- the shares: a block-wide sum over the pairs, each thread a few neighbours
-  int most = 0, empty = 0;
+  int most = 0;
   {
-    const int each = (pairs + kWarps * 32 - 1) / (kWarps * 32), from = tid * each, to = min(pairs, from + each);
+    const int each = (pairs + kWarps * 32 - 1) / (kWarps * 32);
     int sum = 0;
-    for (int i = from; i < to; ++i) {
+    for (int i = tid * each; i < min(pairs, (tid + 1) * each); ++i) {
       Tile tile;
       open(tile, i, 0);
       int n = 0;
@@ -210,29 +210,27 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
       shares.before[i] = sum;  // completed below
       sum += n;
       most = max(most, n);
-      empty |= n == 0;
     }
     int x = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     }
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 31) scratch[warp] = x, scratch[kWarps + 1 + warp] = most;
-    empty = __syncthreads_or(empty);
+    if (lane == 31) scratch[warp] = x;
+    if (tid == 0) scratch[kWarps] = 0;
+    __syncthreads();
+    if (lane == 0) atomicMax(&scratch[kWarps], most);
     int start = x - sum;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      most = max(most, scratch[kWarps + 1 + w]);
-      if (w < warp) start += scratch[w];
-    }
-    for (int i = from; i < to; ++i) shares.before[i] += start;
+    for (int w = 0; w < warp; ++w) start += scratch[w];
+    for (int i = tid * each; i < min(pairs, (tid + 1) * each); ++i) shares.before[i] += start;
     if (tid == kWarps * 32 - 1) shares.before[pairs] = start + sum;
     __syncthreads();
+    most = scratch[kWarps];
   }
   // rows of pairs without any visible key: zeros
-  for (int i = blockIdx.x; empty && i < pairs; i += gridDim.x) {
+  for (int i = blockIdx.x; i < pairs; i += gridDim.x) {
     if (shares.before[i + 1] > shares.before[i]) continue;
     Tile tile;
     for (int head = 0; head < p.nkv; ++head) {
@@ -273,7 +271,7 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
     return ((uint32_t)min(max(page, 0), p.num_pages - 1) * p.nkv + head) * p.page_blocks + blk % p.page_blocks;
   };
   const int mine = begin + warp;
-  uint32_t here = look_up(lane), ahead = kNone;
+  uint32_t here = look_up(lane), ahead = look_up(32 + lane);
   uint8_t* ring = smem + warp * (kRing * Rec::kBytes);
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
   const uint8_t* pool_at = p.pool + lane * 16;
@@ -300,7 +298,6 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch();
-  ahead = look_up(32 + lane);
 
   int done = 0;  // steps worked on
   for (int seg = begin; seg < end;) {
@@ -476,10 +473,10 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
         asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(ticket) : "memory");
         const bool last = before == c1 - c0;
         if (last) *ticket = 0;
-        scratch[kWarps] = last;
+        scratch[kWarps + 1] = last;
       }
       __syncthreads();
-      if (scratch[kWarps]) {
+      if (scratch[kWarps + 1]) {
         for (int i = tid; i < kRows * (D / 4); i += kWarps * 32) {
           const int r = i / (D / 4), channel = i % (D / 4) * 4, row = tile.first_row + r;
           if (row >= tile.rows) continue;

@@ -241,6 +241,15 @@ def test_few_rows_over_many_keys(window, sinks):
     check_attention([(900, 150)], 5, 1, 128, 16, torch.bfloat16, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("tokens,d,dtype", [(20, 128, torch.bfloat16), (50, 128, torch.bfloat16), (12, 128, torch.float32), (33, 64, torch.bfloat16),
+                                            (9, 256, torch.bfloat16)])
+def test_short_portions_over_many_keys(tokens, d, dtype, window):
+    """Many requests with a few tokens each: weights are added up 16 or 32 rows at a time."""
+    lens = [(1300, tokens), (700, 3), (tokens, tokens), (1290, 1), (1033, tokens - 1), (0, 0), (64, 5), (1100, 8)]
+    check_attention(lens, 16, 8, d, 16, dtype, window=window)
+
+
 def test_portions_in_groups(monkeypatch):
     """Requests whose unpacked rows do not fit the workspace at once are taken in groups."""
     monkeypatch.setattr(ops, "ATTENTION_KV4_EXPAND_BYTES", 2 * 128 * 2 * 3 * 128 * 2 * 2)  # two requests of three pages

@@ -520,15 +520,15 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
 // Few rows (kTiles tiles of 8): the warp goes over records kWarps * gridDim.x apart, the next one's codes on their way while it works on
 // one; a key's sum is complete when its record is done, and is added without being read first (no other warp adds to it).
 template <typename T, int kQ, int kTiles>
-__global__ void __launch_bounds__(kWarps * 32) weights_kernel(const Params p, float* sums) {
+__global__ void __launch_bounds__(kWarps * 32) weights_kernel(const Params p, float* sums, int first_row) {
   ts_pdl_prologue();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   Tile tile;
   tile.open(p, blockIdx.z, blockIdx.y);
-  tile.first_row = 0;
-  const int before = tile.context - tile.q_len;
-  if (tile.q_len <= 0 || tile.context <= 0) return;
-  const int begin = p.window > 0 ? max(0, before - p.window + 1) / KV4_BLOCK : 0, end = (tile.context + KV4_BLOCK - 1) / KV4_BLOCK;
+  if (first_row >= tile.rows || tile.context <= 0) return;
+  const int rows = min(8 * kTiles, tile.rows - first_row), first_pos = tile.position(p, first_row), last_pos = tile.position(p, first_row + rows - 1);
+  if (last_pos < 0) return;
+  const int begin = p.window > 0 ? max(0, first_pos - p.window + 1) / KV4_BLOCK : 0, end = last_pos / KV4_BLOCK + 1;
   const int step = kWarps * gridDim.x, page_size = p.page_blocks * KV4_BLOCK;
   const int* table = p.table + (size_t)tile.b * p.table_stride;
   int blk = begin + blockIdx.x * kWarps + warp;
@@ -567,15 +567,18 @@ __global__ void __launch_bounds__(kWarps * 32) weights_kernel(const Params p, fl
 #pragma unroll
   for (int n = 0; n < kTiles; ++n) {
     const int row = 8 * n + g;
-    kv4_query_row<D, kQ>(row < tile.rows ? tile.query<T>(p, row) + t * (D / 4) : nullptr, qf[n]);
+    kv4_query_row<D, kQ>(row < rows ? tile.query<T>(p, first_row + row) + t * (D / 4) : nullptr, qf[n]);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int r = 8 * n + 2 * t + c;
       lse[n][c] = INFINITY, pos[n][c] = -1;  // a row that does not exist gives no weight
-      if (r < tile.rows) lse[n][c] = p.lse[(size_t)tile.token(p, r) * p.nq + tile.query_head(p, r)] * kLog2e, pos[n][c] = tile.position(p, r);
+      if (r < rows) {
+        lse[n][c] = p.lse[(size_t)tile.token(p, first_row + r) * p.nq + tile.query_head(p, first_row + r)] * kLog2e;
+        pos[n][c] = tile.position(p, first_row + r);
+      }
     }
   }
-  const int all0 = p.window > 0 ? tile.context - p.window : 0, all1 = before + 1;  // keys that every row sees
+  const int all0 = p.window > 0 ? last_pos - p.window + 1 : 0, all1 = first_pos + 1;  // keys that every row sees
   while (true) {
     Codes next;
     const int next_blk = blk + step;
@@ -587,7 +590,7 @@ __global__ void __launch_bounds__(kWarps * 32) weights_kernel(const Params p, fl
         [&](int n, int part, int i) { return make_uint4(qf[n][part][2 * i][0], qf[n][part][2 * i][1], qf[n][part][2 * i + 1][0], qf[n][part][2 * i + 1][1]); }, s);
     const int key = blk * KV4_BLOCK;
     float w[2] = {0.f, 0.f};
-    const bool edge = tile.rows < 8 * kTiles || key < all0 || key + KV4_BLOCK > all1;
+    const bool edge = rows < 8 * kTiles || key < all0 || key + KV4_BLOCK > all1;
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
@@ -763,12 +766,23 @@ __global__ void __launch_bounds__(kWeightThreads, 1) weights_rows_kernel(const P
 
 template <typename T, int kQ>
 int launch_weights(const Params& p, float* sums, int num_seqs, int max_context, int max_q, cudaStream_t stream) {
-  // Few rows: a record is read, used and done with, by as many warps as run at once; with more, unpacking it once pays.
-  if (max_q * p.group <= 16) {
+  // Streamed: a record is read, used and done with, by as many warps as run at once, for kPass rows at a time (their registers hold so many queries).
+  // Else keys are unpacked once, 128 of a head to a CTA, which pays where those CTAs are few or the rows many.  us streamed / unpacked once, bfloat16,
+  // 16 requests of 4,096 rows: 24 queries 42 / 136, 64 81 / 154, 128 158 / 205; 2 of 16,384: 24 30 / 72, 64 56 / 80, 128 108 / 104; 1 of 2,048: 24
+  // 10 / 10, 64 17 / 12, 128 33 / 14; float32, 16 of 4,096: 64 180 / 199, 96 266 / 260.  (ops.py has the same rule for where tcgen05 takes over.)
+  constexpr int kPass = kQ == 1 && D <= 128 ? 32 : 16, kStreamed = kQ == 1 ? 128 : 64;
+  const int rows = max_q * p.group, passes = (rows + kPass - 1) / kPass;
+  if (passes == 1 || (rows <= kStreamed && (long long)((max_context + 127) / 128) * p.nkv * num_seqs > 148 * passes)) {
     const int most = (max_context + KV4_BLOCK * kWarps - 1) / (KV4_BLOCK * kWarps), want = 8 * 148 / (p.nkv * num_seqs) + 1;
     const dim3 grid(most < want ? most : want, p.nkv, num_seqs);
-    if (max_q * p.group <= 8) return ts_launch(weights_kernel<T, kQ, 1>, grid, dim3(kWarps * 32), 0, stream, p, sums);
-    return ts_launch(weights_kernel<T, kQ, 2>, grid, dim3(kWarps * 32), 0, stream, p, sums);
+    for (int first = 0; first < rows; first += kPass) {
+      int status;
+      if (rows - first <= 8) status = ts_launch(weights_kernel<T, kQ, 1>, grid, dim3(kWarps * 32), 0, stream, p, sums, first);
+      else if (kPass == 16 || rows - first <= 16) status = ts_launch(weights_kernel<T, kQ, 2>, grid, dim3(kWarps * 32), 0, stream, p, sums, first);
+      else status = ts_launch(weights_kernel<T, kQ, kPass / 8>, grid, dim3(kWarps * 32), 0, stream, p, sums, first);
+      if (status) return status;
+    }
+    return 0;
   }
   constexpr int smem = 2 * WeightsStage<kQ>::kBytes;
   static bool set = false;

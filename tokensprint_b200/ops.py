@@ -2819,7 +2819,10 @@ def attention_kv4_weights(
     if lse.numel() != T * nq:
         raise KernelError(f"attention_kv4_weights: lse must have {T * nq} entries, got {lse.numel()}")
     _kv4_sums("attention_kv4_weights", sums, pool)
-    if max_seqlen_q * (nq // nkv) > ATTENTION_KV4_DIRECT_ROWS and code == 1 and attention_tcgen05_supported(nq, nkv, d, _KV4_EXPAND_PAGE):
+    rows = max_seqlen_q * (nq // nkv)
+    # up to 128 rows of many keys are streamed (the figures stand at the rule in kv4_attention.cu)
+    streamed = rows <= ATTENTION_KV4_DIRECT_ROWS or (rows <= 128 and -(-max_context // 128) * nkv * num_seqs > 148 * -(-rows // 32))
+    if not streamed and code == 1 and attention_tcgen05_supported(nq, nkv, d, _KV4_EXPAND_PAGE):
         global _weights_kv4_tcgen05
         if _weights_kv4_tcgen05 is None:
             run = _kv4_tcgen05_library().ts_kv4_weights_tcgen05

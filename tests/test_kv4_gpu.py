@@ -250,6 +250,23 @@ def test_short_portions_over_many_keys(tokens, d, dtype, window):
     check_attention(lens, 16, 8, d, 16, dtype, window=window)
 
 
+@pytest.mark.parametrize("lens", [[(130, 130)], [(90, 30), (200, 64)], [(50, 50), (100, 37), (64, 1), (9, 4)]])
+@pytest.mark.parametrize("window,sinks", [(0, False), (20, True)])
+@pytest.mark.parametrize("nq,nkv", [(4, 1), (6, 2), (7, 1)])
+def test_small_portions_on_tensor_memory(lens, nq, nkv, window, sinks, monkeypatch):
+    """Portions of so little work that the kernel of decoded tokens takes them by itself, sent through the other one."""
+    monkeypatch.setattr(ops, "_KV4_DIRECT_PIECES", 0)
+    check_attention(lens, nq, nkv, 128, 16, torch.bfloat16, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("lens", [[(n, 1) for n in (600, 3, 1500, 77, 16, 2500, 900)], [(1000, 2)] * 3, [(40, 40), (1, 1), (900, 9)], [(5000, 1)]])
+@pytest.mark.parametrize("nq,nkv,dtype", [(8, 2, torch.bfloat16), (16, 2, torch.bfloat16), (24, 2, torch.bfloat16), (8, 1, torch.float32)])
+def test_shares_of_ranges(lens, nq, nkv, dtype):
+    """Key ranges of one and of many lengths, cut into parts of their own."""
+    check_attention(lens, nq, nkv, 128, 16, dtype)
+    check_attention(lens, nq, nkv, 64, 16, dtype, window=300)
+
+
 def test_portions_in_groups(monkeypatch):
     """Requests whose unpacked rows do not fit the workspace at once are taken in groups."""
     monkeypatch.setattr(ops, "ATTENTION_KV4_EXPAND_BYTES", 2 * 128 * 2 * 3 * 128 * 2 * 2)  # two requests of three pages

@@ -75,9 +75,10 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[16], uint2& w) {
   return byte;
 }
 
-// A thread takes the 16 channels of one group at a time: their largest, the scale, the codes, 8 + 1 bytes out; `width` threads (32 or 128) go over
-// the groups of a token, keys first.  With many tokens it is the number of warps that hides the loads (16,384 tokens of 8 heads of 128:
-// 21.7 us with a group at a time and 46 registers, 38.6 with four in flight and 125; 105 MB).
+// A thread takes the 16 channels of one group at a time: their largest, s = amax / 7 rounded, the codes 8 + x / s rounded, 8 + 1 bytes out; `width`
+// threads (32 or 128) go over the groups of a token, keys first.  One pass, bound by memory: 2 bytes in and 9/16 out per value.  With many tokens
+// it is the number of warps that hides the loads (16,384 tokens of 8 heads of 128: 21.7 us with a group at a time and 46 registers, 38.6 with
+// four in flight and 125; 105 MB).  8,192 tokens: 15.4 us from cold caches, 2.8 TB/s; 8 tokens: 2.4 us, a launch and two trips to memory.
 template <typename T>
 __global__ void __launch_bounds__(128, 10) store_kernel(const T* k, const T* v, long long k_stride, long long v_stride, uint8_t* pool, float* sums,
                                                     const int* slots, int tokens, int nkv, int log_groups, int page_blocks, int num_slots, int width) {
@@ -103,7 +104,8 @@ __global__ void __launch_bounds__(128, 10) store_kernel(const T* k, const T* v, 
   }
 }
 
-// A thread takes eight channels: 4 + 1 bytes in, one store of 16 bytes of bfloat16 out, a warp's stores one behind the other.
+// A thread takes eight channels: 4 + 1 bytes in, one store of 16 bytes of bfloat16 out, a warp's stores one behind the other.  Bound by what
+// it writes: 65,536 rows of 8 heads of 128 (268 MB out) take 58 us, 5.9 TB/s with the codes; 8,192 take 18 us.
 template <typename T>
 __global__ void __launch_bounds__(128) load_kernel(const uint8_t* pool, const int* slots, T* k, T* v, int rows, int nkv, int log_groups, int page_blocks,
                                                    int num_slots, int width) {
@@ -150,6 +152,7 @@ __global__ void __launch_bounds__(128) load_kernel(const uint8_t* pool, const in
 
 // The rows that a batch's queries can see, of heads of 128, as bfloat16 pages of 128 rows for the prompt attention, and the block table of those
 // pages: request b has the pages [b * blocks, (b + 1) * blocks); out_lens: its rows, as many as have a place.  A CTA unpacks 64 rows of one head.
+// 2,048 rows of 8 heads: 6 us (2.4 MB in, 8.4 MB out), most of it the start and two trips to memory; the attention that follows reads them from the L2.
 constexpr int kExpandRows = 64, kExpandPage = 128, kExpandDim = 128;
 __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* pool, const int* table, int table_stride, const int* cu, const int* context, uint4* k,
                                                      uint4* v, int* out_table, int* out_lens, int nkv, int page_blocks, int num_pages, int blocks,
@@ -236,7 +239,9 @@ __device__ __forceinline__ uint4 peer_words(const uint32_t* p, int rank) {
 // a radix select whose counts the CTAs add up from one another's shared memory; every kept row gets its new place, and its source is written
 // down there.  Then the kept rows move forward in rounds, kMoveRows places per CTA: all reads of a round, a barrier of the cluster, its writes.
 // That is safe in place: a row never moves backwards and the order is kept, so what a round writes lies before everything that later
-// rounds read.  (Every CTA ranking all rows by itself took 35 us of 72 for 128 pairs of 8,190 rows.)
+// rounds read.  (Every CTA ranking all rows by itself took 35 us of 72 for 128 pairs of 8,190 rows.)  16 requests of up to 8,190 rows of 8 heads of 128 cut
+// to 4,096: 41 us, where the rows that move (151 MB there and back) would take 23 at the copy rate; the rest is the ranking (three passes over
+// weights in shared memory, each with barriers of the cluster) and rounds that wait for their own reads.  One request: 12 us, all of it such waits.
 template <int D>
 __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(uint8_t* pool, float* sums, const int* table, int table_stride, const int* context,
                                                                  int* new_lens, int* order, int nkv, int page_blocks, int num_pages, int budget, int recent,
@@ -422,8 +427,8 @@ int launch_evict(uint8_t* pool, float* sums, const int* table, int table_stride,
 
 }  // namespace
 
-// Threads per token of the row kernels: with few tokens all groups of a token at once (measured at 8 tokens of 8 heads of 128: see the kernels'
-// table in the design notes), with many a warp per token with four groups in flight.
+// Threads per token of the row kernels: with few tokens all groups of a token at once, with many a warp per token.  us of 128 / 32 threads, rows of 8
+// heads of 128: store of 8 tokens 7 / 10, of 1,024 8 / 10, of 4,096 14 / 12; load of 8 6 / 8, of 1,024 8 / 8, of 4,096 14 / 10.
 static int threads_per_token(int tokens) { return tokens < 1024 ? 128 : 32; }
 
 // k, v: rows [tokens] of nkv * d entries, `stride` entries apart; slots [tokens], -1: not stored; sums: null or the pool's weights.

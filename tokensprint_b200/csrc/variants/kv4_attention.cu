@@ -9,6 +9,13 @@
 //
 // Keys stand on the M side of the instruction: S^T[16 keys][8 rows] = K Q^T and O^T[channels][8 rows] += V^T P^T, so
 // that the few rows of a decode step fill an instruction and every code is unpacked once for all of them.
+//
+// What bounds it: for 4 query rows a key head a record of 16 tokens (2,304 bytes with heads of 128) takes a warp some 400 instructions (the codes
+// of 4,096 values unpacked two at a time: a shift, a mask and an or in one, a multiply-add; 16 products; the softmax), and the pipes that
+// run them (integer 54 % busy, multiply-add 37 %, tensor 20 %) share the issue slots: 3.5 TB/s of cache where the same kernel without the arithmetic
+// reads 5.8.  tcgen05 does not fit: its smallest tile is 128 keys by 8 rows whose operands must lie unpacked in shared memory or tensor memory, so
+// every value would be written and read once more, and unpacking is what the time goes into.  us with 32 query and 8 key heads of 128:
+// 4 requests of up to 60,000 rows 78 (276 MB), 32 of up to 4,096 36 (96 MB), 1 of 517 (16 query heads) 11.4.
 #include "kv4.cuh"
 
 #ifndef TS_HEAD_DIM
@@ -196,10 +203,24 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
   auto first_record = [&](const Tile& tile) { return p.window > 0 ? max(0, tile.position(p, tile.first_row) - p.window + 1) / KV4_BLOCK : 0; };
   // ---- the shares: a block-wide sum over the pairs, each thread a few neighbours
   int most = 0;
+  const int each = (pairs + kWarps * 32 - 1) / (kWarps * 32), my_first = min(pairs, tid * each), my_last = min(pairs, my_first + each);
+  auto sum_before = [&](int sum) {  // of the threads before this one; a barrier stands between what was done ahead of the call and what comes after it
+    int x = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) scratch[warp] = x;
+    __syncthreads();
+    int start = x - sum;
+    for (int w = 0; w < warp; ++w) start += scratch[w];
+    return start;
+  };
   {
-    const int each = (pairs + kWarps * 32 - 1) / (kWarps * 32);
     int sum = 0;
-    for (int i = tid * each; i < min(pairs, (tid + 1) * each); ++i) {
+    if (tid == 0) scratch[kWarps] = 0;
+    for (int i = my_first; i < my_last; ++i) {
       Tile tile;
       open(tile, i, 0);
       int n = 0;
@@ -211,20 +232,11 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
       sum += n;
       most = max(most, n);
     }
-    int x = sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    }
-    if (lane == 31) scratch[warp] = x;
-    if (tid == 0) scratch[kWarps] = 0;
-    __syncthreads();
+    for (int o = 1; o < 32; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const int start = sum_before(sum);
     if (lane == 0) atomicMax(&scratch[kWarps], most);
-    int start = x - sum;
-    for (int w = 0; w < warp; ++w) start += scratch[w];
-    for (int i = tid * each; i < min(pairs, (tid + 1) * each); ++i) shares.before[i] += start;
+    for (int i = my_first; i < my_last; ++i) shares.before[i] += start;
     if (tid == kWarps * 32 - 1) shares.before[pairs] = start + sum;
     __syncthreads();
     most = scratch[kWarps];
@@ -241,9 +253,46 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
       }
     }
   }
-  const int total = shares.before[pairs] * p.nkv;
-  // at least a step for every warp, and no range over more than kMaxParts CTAs
-  const int share = max(max(kWarps, (total + (int)gridDim.x - 1) / (int)gridDim.x), (most + kMaxParts - 1) / kMaxParts);
+  int total = shares.before[pairs] * p.nkv;
+  // At least a step for every warp (of a short range no more than the range), no more parts of a range than pay (one CTA joins them, kRounds times eight
+  // at once: a warp's step costs about as much as the joining of 20 / kRounds parts) and none over more than kMaxParts CTAs.
+  constexpr int kRounds = (kRows * (D / 4) + kWarps * 32 - 1) / (kWarps * 32);
+  const int least = max(max(min(kWarps, most), (int)sqrtf(0.2f * kRounds * most)), (most + kMaxParts - 1) / kMaxParts);
+  int share = max(least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  // Where it costs a warp no more than one step, a CTA has one range only: every range is counted as a whole number of shares.  (A second range in a
+  // CTA costs its queries, its joining and two barriers: us without and with this rule, 32 query and 8 key heads, one request of 517 rows 11.4 / 8.8, of
+  // 2,048 10.2 / 10.4, of 15,000 20.2 / 17.2; its last 4 tokens, 16 rows a key head: 1,900 24.5 / 17.1, 8,192 30 / 26; a prompt of 10 tokens 19.5 / 7.9.)
+  const int spare = (int)gridDim.x - pairs * p.nkv;
+  if (spare > 0 && total > 0) {
+    const int whole = max(least, (total + spare - 1) / spare);
+    if (whole <= share + kWarps) {
+      share = whole;
+      auto parts_of = [&](int n) { return (n + share - 1) / share; };
+      if (total == most * pairs * p.nkv) {  // ranges of one length
+        if (most % share != 0) {
+          const int each_range = parts_of(most) * share;
+          __syncthreads();
+          for (int i = my_first; i < my_last; ++i) shares.before[i] = i * each_range;
+          if (tid == kWarps * 32 - 1) shares.before[pairs] = pairs * each_range;
+          __syncthreads();
+        }
+      } else {
+        const int behind = shares.before[my_last];
+        int sum = 0;
+        for (int i = my_first; i < my_last; ++i) sum += parts_of((i + 1 < my_last ? shares.before[i + 1] : behind) - shares.before[i]) * share;
+        int start = sum_before(sum), from = my_first < my_last ? shares.before[my_first] : 0;
+        for (int i = my_first; i < my_last; ++i) {
+          const int next = i + 1 < my_last ? shares.before[i + 1] : behind;
+          shares.before[i] = start;
+          start += parts_of(next - from) * share;
+          from = next;
+        }
+        if (tid == kWarps * 32 - 1) shares.before[pairs] = start;
+        __syncthreads();
+      }
+      total = shares.before[pairs] * p.nkv;
+    }
+  }
   const int begin = (int)min((long long)share * blockIdx.x, (long long)total), end = min(begin + share, total);
   if (begin >= end) return;
   auto pair_of = [&](int step) {
@@ -518,7 +567,9 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
 // weights: w_j += sum over the rows r of exp(s_rj - lse_r).  A warp owns 16 keys of one head at a time.
 
 // Few rows (kTiles tiles of 8): the warp goes over records kWarps * gridDim.x apart, the next one's codes on their way while it works on
-// one; a key's sum is complete when its record is done, and is added without being read first (no other warp adds to it).
+// one; a key's sum is complete when its record is done, and is added without being read first (no other warp of the launch adds to it, so its
+// value does not depend on any order).  Only the keys' half of a record is read, in words straight to registers: no shared memory, no barrier.
+// Bound like attention_kernel by unpacking; 16 requests of up to 4,096 rows, 4 query rows a key head: 14 us (45 MB with the sums).
 template <typename T, int kQ, int kTiles>
 __global__ void __launch_bounds__(kWarps * 32) weights_kernel(const Params p, float* sums, int first_row) {
   ts_pdl_prologue();

@@ -2523,8 +2523,11 @@ _SIGNATURES["ts_kv4_expand"] = [_c_void_p, _c_void_p, _c_int] + [_c_void_p] * 6 
 _attention_kv4: dict[int, tuple] = {}
 # Portions of prompts with more rows (tokens x query heads of a key head) than this are attended to on tcgen05 tensor cores, over rows unpacked for
 # the step; up to it by the kernel of decoded tokens, which unpacks every code once for 16 rows (us, 16 requests of 8,000 rows with 48 / 64 / 96 rows:
-# 177 / 231 / 336 against 243 / 243 / 244; one of 2,000 rows: 24 / 21 / 25 against 23 / 23 / 25).
+# 177 / 231 / 336 against 243 / 243 / 244).  That kernel also takes prompts of a few records (16 rows of queries x 16 keys count as one piece of work),
+# where the two launches and the start of tcgen05 tiles weigh most: one prompt of 20 / 64 tokens, 80 / 512 pieces: 12 / 14 us against 17 / 20; eight
+# of 32, 1,024 pieces: 20.5 against 19.5; one of 128, 2,048 pieces: 20.5 against 19.5.
 ATTENTION_KV4_DIRECT_ROWS = 64
+_KV4_DIRECT_PIECES = 600
 ATTENTION_KV4_EXPAND_BYTES = 1 << 30  # most bytes of unpacked rows at a time
 _attention_kv4_tcgen05: dict[bool, object] = {}
 _weights_kv4_tcgen05 = None
@@ -2727,7 +2730,8 @@ def attention_kv4(
                 if t.numel() != n:
                     raise KernelError(f"attention_kv4: {label} must have {n} entries, got {t.numel()}")
     rows = max_seqlen_q * (nq // nkv)
-    if rows > ATTENTION_KV4_DIRECT_ROWS and code == 1 and attention_tcgen05_supported(nq, nkv, d, _KV4_EXPAND_PAGE) and max_context > 0:
+    if (rows > ATTENTION_KV4_DIRECT_ROWS and code == 1 and -(-rows // 16) * -(-max_context // KV4_BLOCK) * nkv * num_seqs > _KV4_DIRECT_PIECES
+            and attention_tcgen05_supported(nq, nkv, d, _KV4_EXPAND_PAGE)):
         _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q, max_context, nq, nkv, scale, window,
                                 head_sinks, lse)
         return
@@ -2739,12 +2743,14 @@ def attention_kv4(
 
 
 _KV4_EXPAND_PAGE = 128
-_KV4_MIN_RUN = 3  # least key blocks of a run
+# Least key blocks of a run (us with 1 / 3 / 6 and without runs, 32 query and 8 key heads: 64 tokens over 1,024 rows 28 / 30 / 34 / 34, over 4,096
+# 38 / 36 / 40 / 83; 512 over 2,048 44 / 44 / 44 / 52; 256 over 512 28 / 26 / 26 / 26).
+_KV4_MIN_RUN = 3
 
 
 def _kv4_tcgen05_library(scored: bool = False) -> ctypes.CDLL:
     # (every weight from the special-function unit: the cubic's 8e-5 is too much for denominators that are an output, and it gives masked keys 2^-120,
-    # not nothing; a prompt of 2,048 pays 80 us for 78)
+    # not nothing; a prompt of 2,048 tokens pays 2 us of 80)
     return _build.load_variant("attention_tcgen05", {"TS_HEAD_DIM": ATTENTION_TCGEN05_HEAD_DIM, "TS_ATT_LSE": 1, "TS_ATT_FMA_PAIRS": 0,
                                                      "TS_ATT_SCORED": int(scored)})
 

@@ -1442,6 +1442,7 @@ struct WeightParams {
   float scale_log2;
 };
 __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(const __grid_constant__ CUtensorMap map_q, const WeightParams p) {
+  if (threadIdx.x == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
   ts_pdl_wait();  // (tensor memory is never held while waiting for another kernel)
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
@@ -1463,11 +1464,25 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
   const int tile0 = first_token / per_tile, tiles = (end_token - 1) / per_tile - tile0 + 1;
   const int* table = p.table + (size_t)b * p.table_stride;
 
-  if (tid == 0) {
-    abort_s = 0;
-    for (int i = 0; i < W_STAGES; ++i) mbar_init(smem_u32(&q_full[i]), 1), mbar_init(smem_u32(&q_empty[i]), 1);
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_full[i]), 1), mbar_init(smem_u32(&s_empty[i]), W_GROUP);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  // a tile of queries: two boxes of half a head, asked for by the copying warp
+  auto fetch = [&](int j) {
+    const int st = j % W_STAGES;
+    if (lane == 0) mbar_expect_tx(smem_u32(&q_full[st]), (uint32_t)(2 * RT * 128));
+    __syncwarp();
+    if (lane < 2)
+      tma_load_4d(smem_u32(smem) + W_OFF_Q + st * Q_BYTES + lane * (BM * 128), &map_q, smem_u32(&q_full[st]), lane * 64, 0, hk,
+                  q_begin + (tile0 + j) * per_tile);
+  };
+  if (warp == W_ADDERS) {  // the first tiles come while the keys are unpacked
+    if (lane == 0) {
+      abort_s = 0;
+      for (int i = 0; i < W_STAGES; ++i) mbar_init(smem_u32(&q_full[i]), 1), mbar_init(smem_u32(&q_empty[i]), 1);
+      for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_full[i]), 1), mbar_init(smem_u32(&s_empty[i]), W_GROUP);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncwarp();
+    for (int j = 0; j < min(tiles, W_STAGES); ++j) fetch(j);
   }
   if (warp == W_ADDERS + 1) {
     __syncwarp();
@@ -1505,14 +1520,10 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
   volatile int* abort_flag = &abort_s;
 
   if (warp == W_ADDERS) {
-    int issued = 0;
-    for (int j = 0; j < tiles; ++j) {
-      const int st = j % W_STAGES;
-      if (j >= W_STAGES && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&q_empty[st]), (uint32_t)(j / W_STAGES - 1) & 1, abort_flag))) break;
-      if (lane == 0) mbar_expect_tx(smem_u32(&q_full[st]), (uint32_t)(2 * RT * 128));
-      __syncwarp();
-      if (lane < 2)
-        tma_load_4d(sm + W_OFF_Q + st * Q_BYTES + lane * (BM * 128), &map_q, smem_u32(&q_full[st]), lane * 64, 0, hk, q_begin + (tile0 + j) * per_tile);
+    int issued = min(tiles, W_STAGES);
+    for (int j = W_STAGES; j < tiles; ++j) {
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&q_empty[j % W_STAGES]), (uint32_t)(j / W_STAGES - 1) & 1, abort_flag))) break;
+      fetch(j);
       issued = j + 1;
     }
     // no copy is in flight when the CTA ends, whatever happened (bounded, on a count of its own)

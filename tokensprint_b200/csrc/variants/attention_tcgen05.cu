@@ -1426,214 +1426,287 @@ TS_EXPORT int ts_latent_rebuilt_attention(const void* q, long long ld_q, const v
 // by TMA as the second, so that S^T[key][row] lies in tensor memory with a key per lane: a thread adds up its own key's weights in a
 // register, nothing is exchanged until the end.  What bounds it is the special-function unit, 16 exponentials a clock for 16,384 of a
 // tile; the products take half as long and run on the other buffer meanwhile, and two groups of eight warps take the tiles in turn, so that one's
-// exponentials run while the other waits (a portion of 512 tokens over 2,040 rows, 32 query and 8 key heads: 22 us; with all sixteen warps on a
-// tile 26).  Before the first tile a CTA needs 2.5 us (block table, codes, tensor memory, queries): few tiles over many keys are
-// streamed by the kernel in kv4_attention.cu instead.
+// exponentials run while the other waits (a portion of 512 tokens over 2,048 rows, 32 query and 8 key heads: 22 us; with all sixteen warps on a
+// tile 26).  Before a CTA's first tile 2.5 us pass (block table, codes, tensor memory, queries), so a CTA stays and takes an item of 128 keys after
+// the other: the copying warp works out what they are and asks for their queries ahead, the adding warps have an item's codes in registers when
+// they begin it (16 requests of 4,096 rows with 192 query rows: 119 us, a CTA per item 222).
 constexpr int W_STAGES = 4, W_GROUP = 8, W_ADDERS = 2 * W_GROUP;  // warps that add; two groups of them take the tiles in turn
 constexpr int W_COLUMNS = BM / (W_GROUP / 4);                      // a tile's rows that a warp adds up
 constexpr uint32_t W_OFF_Q = 2 * BM * 128, W_SMEM = W_OFF_Q + W_STAGES * Q_BYTES, W_TMEM_COLS = 256;
+// Places of the ring of items: the copying warp is at most six items ahead of the adding ones (four tiles asked for, two being added up) and writes two further.
+constexpr int W_ITEMS = 16;
 struct WeightParams {
   const uint8_t* pool;
   float* sums;
   const float* lse;
   const int *cu, *context, *table;
   int* error;
-  int table_stride, page_blocks, num_pages, tokens, nq, nkv, window;
+  int table_stride, page_blocks, num_pages, tokens, num_seqs, nq, nkv, chunks, window;  // chunks: of 128 keys of the longest request
   float scale_log2;
+};
+struct WeightItem {
+  int tiles, tile0, key0, ctx, before, q_begin, q_len, head;  // no tiles: the end
+  uint32_t rec[BM / KV4_BLOCK];  // records, counted from the pool's start
 };
 __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(const __grid_constant__ CUtensorMap map_q, const WeightParams p) {
   if (threadIdx.x == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
   ts_pdl_wait();  // (tensor memory is never held while waiting for another kernel)
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t q_full[W_STAGES], q_empty[W_STAGES], s_full[2], s_empty[2];
+  __shared__ __align__(8) uint64_t q_full[W_STAGES], q_empty[W_STAGES], s_full[2], s_empty[2], k_full, item_full[W_ITEMS];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
+  __shared__ WeightItem items[W_ITEMS];
   __shared__ __align__(16) float lse_s[2][2][BM];  // [group][its tiles in turn][row]
   __shared__ __align__(16) int pos_s[2][2][BM];
-  __shared__ float slice_s[W_ADDERS / 4][BM];
+  __shared__ float slice_s[2][W_ADDERS / 4][BM];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int hk = blockIdx.y, b = blockIdx.z, G = p.nq / p.nkv, page_size = p.page_blocks * KV4_BLOCK;
-  const int q_begin = min(max(p.cu[b], 0), p.tokens), q_len = min(max(p.cu[b + 1], q_begin), p.tokens) - q_begin;
-  const int ctx = min(p.context[b], p.table_stride * page_size), before = ctx - q_len, key0 = blockIdx.x * BM;
-  if (key0 >= ctx) return;
-  const int last_key = min(key0 + BM, ctx) - 1, per_tile = BM / G, RT = per_tile * G;
-  const int first_token = max(0, key0 - before);
-  const int end_token = p.window > 0 ? min(q_len, last_key + p.window - before) : q_len;
-  if (first_token >= end_token) return;
-  const int tile0 = first_token / per_tile, tiles = (end_token - 1) / per_tile - tile0 + 1;
-  const int* table = p.table + (size_t)b * p.table_stride;
+  const int G = p.nq / p.nkv, per_tile = BM / G, RT = per_tile * G, page_size = p.page_blocks * KV4_BLOCK;
+  volatile int* abort_flag = &abort_s;
+  constexpr int adders = W_ADDERS * 32;
 
-  // a tile of queries: two boxes of half a head, asked for by the copying warp
-  auto fetch = [&](int j) {
-    const int st = j % W_STAGES;
+  // ---- the copying warp works out this CTA's items, two ahead of the one whose queries it asks for
+  int next_index = blockIdx.x;
+  auto publish = [&](int it) {
+    WeightItem* item = &items[it % W_ITEMS];
+    const int per_seq = p.chunks * p.nkv, all = per_seq * p.num_seqs;
+    int tiles = 0;
+    while (next_index < all) {
+      const int index = next_index, b = index / per_seq, rest = index - b * per_seq, head = rest / p.chunks, key0 = (rest - head * p.chunks) * BM;
+      next_index += gridDim.x;
+      const int q_begin = min(max(p.cu[b], 0), p.tokens), q_len = min(max(p.cu[b + 1], q_begin), p.tokens) - q_begin;
+      const int ctx = min(p.context[b], p.table_stride * page_size), before = ctx - q_len;
+      if (key0 >= ctx) continue;
+      const int last_key = min(key0 + BM, ctx) - 1, first_token = max(0, key0 - before);
+      const int end_token = p.window > 0 ? min(q_len, last_key + p.window - before) : q_len;
+      if (first_token >= end_token) continue;
+      const int tile0 = first_token / per_tile;
+      tiles = (end_token - 1) / per_tile - tile0 + 1;
+      if (lane < BM / KV4_BLOCK) {
+        const int blk = min(key0 / KV4_BLOCK + lane, (ctx - 1) / KV4_BLOCK), page = min(max(p.table[(size_t)b * p.table_stride + blk / p.page_blocks], 0), p.num_pages - 1);
+        item->rec[lane] = ((uint32_t)page * p.nkv + head) * p.page_blocks + blk % p.page_blocks;
+      }
+      if (lane == 0)
+        item->tile0 = tile0, item->key0 = key0, item->ctx = ctx, item->before = before, item->q_begin = q_begin, item->q_len = q_len, item->head = head;
+      break;
+    }
+    if (lane == 0) item->tiles = tiles;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&item_full[it % W_ITEMS]));
+  };
+  // a tile of queries: two boxes of half a head
+  auto fetch = [&](const WeightItem& item, int j, int J) {
+    const int st = J % W_STAGES;
     if (lane == 0) mbar_expect_tx(smem_u32(&q_full[st]), (uint32_t)(2 * RT * 128));
     __syncwarp();
     if (lane < 2)
-      tma_load_4d(smem_u32(smem) + W_OFF_Q + st * Q_BYTES + lane * (BM * 128), &map_q, smem_u32(&q_full[st]), lane * 64, 0, hk,
-                  q_begin + (tile0 + j) * per_tile);
+      tma_load_4d(smem_u32(smem) + W_OFF_Q + st * Q_BYTES + lane * (BM * 128), &map_q, smem_u32(&q_full[st]), lane * 64, 0, item.head,
+                  item.q_begin + (item.tile0 + j) * per_tile);
   };
-  if (warp == W_ADDERS) {  // the first tiles come while the keys are unpacked
+  if (warp == W_ADDERS) {
     if (lane == 0) {
       abort_s = 0;
       for (int i = 0; i < W_STAGES; ++i) mbar_init(smem_u32(&q_full[i]), 1), mbar_init(smem_u32(&q_empty[i]), 1);
       for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_full[i]), 1), mbar_init(smem_u32(&s_empty[i]), W_GROUP);
+      mbar_init(smem_u32(&k_full), W_ADDERS);
+      for (int i = 0; i < W_ITEMS; ++i) mbar_init(smem_u32(&item_full[i]), 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncwarp();
-    for (int j = 0; j < min(tiles, W_STAGES); ++j) fetch(j);
+    publish(0);
+    for (int j = 0; j < min(items[0].tiles, W_STAGES); ++j) fetch(items[0], j, j);
   }
   if (warp == W_ADDERS + 1) {
     __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(W_TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  constexpr int adders = W_ADDERS * 32;
-  if (tid < adders) {
-    // the keys, unpacked: 16 bytes (8 channels) at a time to their places in the swizzled operand; keys that are none as zeros
-#pragma unroll
-    for (int i = 0; i < BM * 16 / adders; ++i) {
-      const int x = tid + adders * i, row = x >> 4, c = x & 15, key = key0 + row;
-      uint4 out = make_uint4(0u, 0u, 0u, 0u);
-      if (key < ctx) {
-        const int page = min(max(table[key / page_size], 0), p.num_pages - 1), in_page = key % page_size;
-        const uint8_t* rec = p.pool + (((size_t)page * p.nkv + hk) * p.page_blocks + in_page / KV4_BLOCK) * Kv4Record<D>::kBytes;
-        const uint32_t code = *reinterpret_cast<const uint32_t*>(rec + in_page % KV4_BLOCK * (D / 2) + c * 4);
-        const uint32_t scale = rec[Kv4Record<D>::kKeyScales + in_page % KV4_BLOCK * (D / 16) + c / 2];
-        out = kv4_unpack(code, scale);
-      }
-      *reinterpret_cast<uint4*>(smem + (c >> 3) * (BM * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = out;
-    }
-    // rows of the query tiles that no copy fills: zeros
-    for (int i = tid; i < W_STAGES * 2 * (BM - RT) * 8; i += adders) {
-      const int half = i / ((BM - RT) * 8), rest = i % ((BM - RT) * 8);
-      *reinterpret_cast<uint4*>(smem + W_OFF_Q + half * (BM * 128) + (RT + rest / 8) * 128 + (rest % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  // rows of the query tiles that no copy fills: zeros
+  for (int i = tid; i < W_STAGES * 2 * (BM - RT) * 8; i += blockDim.x) {
+    const int half = i / ((BM - RT) * 8), rest = i % ((BM - RT) * 8);
+    *reinterpret_cast<uint4*>(smem + W_OFF_Q + half * (BM * 128) + (RT + rest / 8) * 128 + (rest % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
   }
+  if (RT < BM) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   ts_pdl_launch_dependents();
   const uint32_t tmem_base = tmem_base_s, sm = smem_u32(smem);
-  volatile int* abort_flag = &abort_s;
 
   if (warp == W_ADDERS) {
-    int issued = min(tiles, W_STAGES);
-    for (int j = W_STAGES; j < tiles; ++j) {
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&q_empty[j % W_STAGES]), (uint32_t)(j / W_STAGES - 1) & 1, abort_flag))) break;
-      fetch(j);
-      issued = j + 1;
+    int J = min(items[0].tiles, W_STAGES);  // tiles asked for
+    bool ok = true;
+    if (J > 0) publish(1);
+    for (int it = 0, j = J; ok && items[it % W_ITEMS].tiles != 0; ++it, j = 0) {
+      const WeightItem& item = items[it % W_ITEMS];
+      for (; ok && j < item.tiles; ++j) {
+        if (J >= W_STAGES) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_empty[J % W_STAGES]), (uint32_t)(J / W_STAGES - 1) & 1, abort_flag));
+        if (ok) fetch(item, j, J++);
+      }
+      if (ok && items[(it + 1) % W_ITEMS].tiles != 0) publish(it + 2);
     }
     // no copy is in flight when the CTA ends, whatever happened (bounded, on a count of its own)
     int patience = 0;
-    for (int j = max(0, issued - W_STAGES); j < issued; ++j) mbar_wait(smem_u32(&q_full[j % W_STAGES]), (uint32_t)(j / W_STAGES) & 1, &patience);
+    for (int i = max(0, J - W_STAGES); i < J; ++i) mbar_wait(smem_u32(&q_full[i % W_STAGES]), (uint32_t)(i / W_STAGES) & 1, &patience);
     if (patience != 0) *abort_flag = 1;
   } else if (warp == W_ADDERS + 1) {
     const uint64_t k_desc = desc_k_major(sm), q_desc = desc_k_major(sm + W_OFF_Q);
-    int asked = 0;
-    for (int j = 0; j < tiles; ++j) {
-      const int st = j % W_STAGES, buf = j & 1;
-      bool ok = mbar_wait(smem_u32(&q_full[st]), (uint32_t)(j / W_STAGES) & 1, abort_flag);
-      if (ok && j >= 2) ok = mbar_wait(smem_u32(&s_empty[buf]), (uint32_t)(j / 2 - 1) & 1, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (elect_one()) {
-        const uint64_t qd = q_desc + (uint64_t)((st * Q_BYTES) >> 4);
+    int J = 0;
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&item_full[it % W_ITEMS]), (uint32_t)(it / W_ITEMS) & 1, abort_flag));
+      const int tiles = ok ? items[it % W_ITEMS].tiles : 0;
+      if (tiles == 0) break;
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full), (uint32_t)it & 1, abort_flag));
+      for (int j = 0; ok && j < tiles; ++j, ++J) {
+        const int st = J % W_STAGES, buf = J & 1;
+        ok = mbar_wait(smem_u32(&q_full[st]), (uint32_t)(J / W_STAGES) & 1, abort_flag);
+        if (ok && J >= 2) ok = mbar_wait(smem_u32(&s_empty[buf]), (uint32_t)(J / 2 - 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (elect_one()) {
+          const uint64_t qd = q_desc + (uint64_t)((st * Q_BYTES) >> 4);
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = ((ks >> 2) * (BM * 128) + (ks & 3) * 32) >> 4;
-          if (ks == 0) umma_bf16_first(tmem_base + buf * BM, k_desc + off, qd + off, idesc(BM, false));
-          else umma_bf16_more(tmem_base + buf * BM, k_desc + off, qd + off, idesc(BM, false));
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t off = ((ks >> 2) * (BM * 128) + (ks & 3) * 32) >> 4;
+            if (ks == 0) umma_bf16_first(tmem_base + buf * BM, k_desc + off, qd + off, idesc(BM, false));
+            else umma_bf16_more(tmem_base + buf * BM, k_desc + off, qd + off, idesc(BM, false));
+          }
+          umma_commit(smem_u32(&q_empty[st]));
+          umma_commit(smem_u32(&s_full[buf]));
         }
-        umma_commit(smem_u32(&q_empty[st]));
-        umma_commit(smem_u32(&s_full[buf]));
+        __syncwarp();
       }
-      __syncwarp();
-      asked = j + 1;
     }
     // and no product, nor the arrival that reports one
     int patience = 0;
-    for (int j = max(0, asked - W_STAGES); j < asked; ++j) mbar_wait(smem_u32(&q_empty[j % W_STAGES]), (uint32_t)(j / W_STAGES) & 1, &patience);
-    for (int j = max(0, asked - 2); j < asked; ++j) mbar_wait(smem_u32(&s_full[j & 1]), (uint32_t)(j / 2) & 1, &patience);
+    for (int i = max(0, J - W_STAGES); i < J; ++i) mbar_wait(smem_u32(&q_empty[i % W_STAGES]), (uint32_t)(i / W_STAGES) & 1, &patience);
+    for (int i = max(0, J - 2); i < J; ++i) mbar_wait(smem_u32(&s_full[i & 1]), (uint32_t)(i / 2) & 1, &patience);
     if (patience != 0) *abort_flag = 1;
   } else {
-    // ---- a thread per key and a slice of a tile's rows; group g takes the tiles g, g + 2, ...
-    const int quad = warp & 3, h = (warp >> 2) & 1, g = warp / W_GROUP, member = tid % (W_GROUP * 32), row = quad * 32 + lane, key = key0 + row;
+    // ---- a thread per key and a slice of a tile's rows; group g takes the tiles g, g + 2, ... counted over all items
+    const int quad = warp & 3, h = (warp >> 2) & 1, g = warp / W_GROUP, member = tid % (W_GROUP * 32), row = quad * 32 + lane;
     const uint32_t addr = tmem_base + ((uint32_t)(quad * 32) << 16) + g * BM + h * W_COLUMNS;
-    // A tile's rows: their logarithms and last visible keys; rows that are none give no weight.  Asked for a tile before they are told, so that nobody
-    // waits for them.
-    float told_lse = INFINITY;
-    int told_pos = -1;
-    auto ask = [&](int j) {
-      const int token = (tile0 + j) * per_tile + member / G;
-      const bool there = member < RT && token < q_len && j < tiles;
-      told_lse = there ? p.lse[(size_t)(q_begin + token) * p.nq + hk * G + member % G] : INFINITY;
-      told_pos = there ? before + token : -1;
-    };
-    auto tell = [&](int j) { lse_s[g][(j >> 1) & 1][member] = told_lse * 1.4426950408889634f, pos_s[g][(j >> 1) & 1][member] = told_pos; };
-    if (member < BM) {
-      ask(g);
-      tell(g);
-      ask(g + 2);
-    }
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    bool ok = true;
-    for (int j = g; j < tiles; j += 2) {
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(W_GROUP * 32) : "memory");  // tile j's rows are told, tile j - 2's have been read
-      if (member < BM) {
-        tell(j + 2);
-        ask(j + 4);
+    const int oldest = p.window > 0 ? p.window : 0x7fffffff;
+    // a thread's share of an item's keys: 16 bytes of the operand (8 channels) each
+    constexpr int kShare = BM * 16 / adders;
+    uint32_t code[kShare], scale[kShare];
+    auto load_codes = [&](const WeightItem& item) {
+#pragma unroll
+      for (int i = 0; i < kShare; ++i) {
+        const int r = (tid + adders * i) >> 4, c = tid & 15;
+        code[i] = scale[i] = 0u;  // a key that is none: zeros
+        if (item.key0 + r < item.ctx) {
+          const uint8_t* rec = p.pool + (size_t)item.rec[r / KV4_BLOCK] * Kv4Record<D>::kBytes;
+          code[i] = *reinterpret_cast<const uint32_t*>(rec + r % KV4_BLOCK * (D / 2) + c * 4);
+          scale[i] = rec[Kv4Record<D>::kKeyScales + r % KV4_BLOCK * (D / 16) + c / 2];
+        }
       }
-      const int turn = (j >> 1) & 1;
-      if (ok) ok = mbar_wait(smem_u32(&s_full[g]), (uint32_t)turn, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const int first = (tile0 + j) * per_tile, last = first + per_tile - 1;  // the tile's tokens
-        const bool all = last < q_len && before + first >= last_key && (p.window == 0 || before + last - p.window < key0);
-        const int oldest = p.window > 0 ? p.window : 0x7fffffff;
+    };
+    if (items[0].tiles != 0) load_codes(items[0]);
+    bool ok = true;
+    int J0 = 0;  // tiles of the items before
+    for (int it = 0;; ++it) {
+      const WeightItem& item = items[it % W_ITEMS];
+      const int tiles = item.tiles;
+      if (tiles == 0) break;
+      const int key = item.key0 + row, last_key = min(item.key0 + BM, item.ctx) - 1, first_j = (g - J0) & 1;
+      // A tile's rows: their logarithms and last visible keys; rows that are none give no weight.  Asked for a tile before they are told, so that nobody
+      // waits for them.
+      float told_lse = INFINITY;
+      int told_pos = -1;
+      auto ask = [&](int j) {
+        const int token = (item.tile0 + j) * per_tile + member / G;
+        const bool there = member < RT && token < item.q_len && j < tiles;
+        told_lse = there ? p.lse[(size_t)(item.q_begin + token) * p.nq + item.head * G + member % G] : INFINITY;
+        told_pos = there ? item.before + token : -1;
+      };
+      auto tell = [&](int j) {
+        const int turn = ((J0 + j) >> 1) & 1;
+        lse_s[g][turn][member] = told_lse * 1.4426950408889634f, pos_s[g][turn][member] = told_pos;
+      };
+      if (member < BM) ask(first_j);
+      // the keys to their places in the swizzled operand (nothing reads the ones before any more: the barrier at the end of an item)
 #pragma unroll
-        for (int part = 0; part < W_COLUMNS / 32; ++part) {
-          uint32_t v[32];
-          tmem_ld32(addr + part * 32, v);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          if (part == W_COLUMNS / 32 - 1) {  // the scores are in registers: the next but one product may begin
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&s_empty[g]));
-          }
-          const float4* lse = reinterpret_cast<const float4*>(&lse_s[g][turn][h * W_COLUMNS + part * 32]);
-          const int4* pos = reinterpret_cast<const int4*>(&pos_s[g][turn][h * W_COLUMNS + part * 32]);
-          if (all) {
+      for (int i = 0; i < kShare; ++i) {
+        const int r = (tid + adders * i) >> 4, c = tid & 15;
+        *reinterpret_cast<uint4*>(smem + (c >> 3) * (BM * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = kv4_unpack(code[i], scale[i]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&k_full));
+      if (member < BM) {
+        tell(first_j);
+        ask(first_j + 2);
+      }
+      // the next item's codes are on their way while this one's tiles are added up
+      const bool known = mbar_wait(smem_u32(&item_full[(it + 1) % W_ITEMS]), (uint32_t)((it + 1) / W_ITEMS) & 1, abort_flag);
+      if (known && items[(it + 1) % W_ITEMS].tiles != 0) load_codes(items[(it + 1) % W_ITEMS]);
+
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int j = first_j; j < tiles; j += 2) {
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(W_GROUP * 32) : "memory");  // tile j's rows are told, tile j - 2's have been read
+        if (member < BM) {
+          tell(j + 2);
+          ask(j + 4);
+        }
+        const int turn = ((J0 + j) >> 1) & 1;
+        if (ok) ok = mbar_wait(smem_u32(&s_full[g]), (uint32_t)turn, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const int first = (item.tile0 + j) * per_tile, last = first + per_tile - 1;  // the tile's tokens
+          const bool all = last < item.q_len && item.before + first >= last_key && (p.window == 0 || item.before + last - p.window < item.key0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 l = lse[i];
-              sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
-              sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
-              sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
-              sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
+          for (int part = 0; part < W_COLUMNS / 32; ++part) {
+            uint32_t v[32];
+            tmem_ld32(addr + part * 32, v);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (part == W_COLUMNS / 32 - 1) {  // the scores are in registers: the next but one product may begin
+              asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_u32(&s_empty[g]));
             }
-          } else {
+            const float4* lse = reinterpret_cast<const float4*>(&lse_s[g][turn][h * W_COLUMNS + part * 32]);
+            const int4* pos = reinterpret_cast<const int4*>(&pos_s[g][turn][h * W_COLUMNS + part * 32]);
+            if (all) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 l = lse[i];
-              const int4 q = pos[i];
-              if (key <= q.x && q.x - key < oldest) sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
-              if (key <= q.y && q.y - key < oldest) sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
-              if (key <= q.z && q.z - key < oldest) sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
-              if (key <= q.w && q.w - key < oldest) sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
+              for (int i = 0; i < 8; ++i) {
+                const float4 l = lse[i];
+                sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
+                sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
+                sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
+                sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 l = lse[i];
+                const int4 q = pos[i];
+                if (key <= q.x && q.x - key < oldest) sum[0] += fast_exp2(fmaf(__uint_as_float(v[4 * i]), p.scale_log2, -l.x));
+                if (key <= q.y && q.y - key < oldest) sum[1] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 1]), p.scale_log2, -l.y));
+                if (key <= q.z && q.z - key < oldest) sum[2] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 2]), p.scale_log2, -l.z));
+                if (key <= q.w && q.w - key < oldest) sum[3] += fast_exp2(fmaf(__uint_as_float(v[4 * i + 3]), p.scale_log2, -l.w));
+              }
             }
           }
         }
       }
-    }
-    slice_s[warp >> 2][row] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    asm volatile("bar.sync 3, %0;" ::"n"(adders) : "memory");
-    if (warp < 4 && key < ctx && abort_s == 0) {
-      const int page = min(max(table[key / page_size], 0), p.num_pages - 1);
-      p.sums[((size_t)page * p.nkv + hk) * page_size + key % page_size] += (slice_s[0][row] + slice_s[1][row]) + (slice_s[2][row] + slice_s[3][row]);
+      float (*slice)[BM] = slice_s[it & 1];  // (in turns: the next item's may be written while these are read)
+      slice[warp >> 2][row] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      // All adding warps go on, or none: a wait that gave up anywhere ends it for all.
+      uint32_t go_on = ok && known;
+      asm volatile(
+          "{\n .reg .pred a, b;\n setp.ne.u32 a, %0, 0;\n bar.red.and.pred b, 3, %1, a;\n selp.u32 %0, 1, 0, b;\n}"
+          : "+r"(go_on)
+          : "n"(adders)
+          : "memory");
+      if (go_on == 0) break;
+      if (warp < 4 && key < item.ctx)
+        p.sums[(size_t)item.rec[row / KV4_BLOCK] * KV4_BLOCK + row % KV4_BLOCK] += (slice[0][row] + slice[1][row]) + (slice[2][row] + slice[3][row]);
+      J0 += tiles;
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1853,8 +1926,9 @@ TS_EXPORT int ts_kv4_weights_tcgen05(const void* q, const void* pool, const floa
                                      int table_stride, int page_blocks, int num_pages, int T, int B, int max_context, int nq, int nkv, float scale, int window,
                                      int* error, void* stream) {
   if (T <= 0 || B <= 0 || max_context <= 0) return 0;
-  if (nq % nkv || nq / nkv > BM || (uintptr_t)q % 16 || B > 65535 || nkv > 65535) return TS_ERR_UNSUPPORTED_SIZE;
-  WeightParams p = {(const uint8_t*)pool, sums, lse, cu, context, table, error, table_stride, page_blocks, num_pages, T, nq, nkv, window,
+  const long long chunks = (max_context + BM - 1) / BM, items = chunks * nkv * B;
+  if (nq % nkv || nq / nkv > BM || (uintptr_t)q % 16 || items > 0x7fff0000LL) return TS_ERR_UNSUPPORTED_SIZE;
+  WeightParams p = {(const uint8_t*)pool, sums, lse, cu, context, table, error, table_stride, page_blocks, num_pages, T, B, nq, nkv, (int)chunks, window,
                     scale * 1.4426950408889634f};
   CUtensorMap mq;
   int st = query_map(q, T, nq, nkv, &mq);
@@ -1866,7 +1940,15 @@ TS_EXPORT int ts_kv4_weights_tcgen05(const void* q, const void* pool, const floa
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
-  return ts_launch(kv4_weights_kernel, dim3((max_context + BM - 1) / BM, nkv, B), dim3((W_ADDERS + 2) * 32), smem, (cudaStream_t)stream, mq, p);
+  static int sms = 0;
+  if (sms == 0) {
+    int device = 0, n = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess) return (int)e;
+    sms = n;
+  }
+  return ts_launch(kv4_weights_kernel, dim3((unsigned)(items < sms ? items : sms)), dim3((W_ADDERS + 2) * 32), smem, (cudaStream_t)stream, mq, p);
 }
 #endif
 #else

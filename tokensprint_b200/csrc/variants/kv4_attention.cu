@@ -818,9 +818,10 @@ __global__ void __launch_bounds__(kWeightThreads, 1) weights_rows_kernel(const P
 template <typename T, int kQ>
 int launch_weights(const Params& p, float* sums, int num_seqs, int max_context, int max_q, cudaStream_t stream) {
   // Streamed: a record is read, used and done with, by as many warps as run at once, for kPass rows at a time (their registers hold so many queries).
-  // Else keys are unpacked once, 128 of a head to a CTA, which pays where those CTAs are few or the rows many.  us streamed / unpacked once, bfloat16,
-  // 16 requests of 4,096 rows: 24 queries 42 / 136, 64 81 / 154, 128 158 / 205; 2 of 16,384: 24 30 / 72, 64 56 / 80, 128 108 / 104; 1 of 2,048: 24
-  // 10 / 10, 64 17 / 12, 128 33 / 14; float32, 16 of 4,096: 64 180 / 199, 96 266 / 260.  (ops.py has the same rule for where tcgen05 takes over.)
+  // Else keys are unpacked once, 128 of a head to a CTA, which pays where those CTAs are few or the rows many.  us streamed / unpacked once, 16 requests
+  // of 4,096 rows, 24 / 64 / 128 query rows: bfloat16 heads of 64 35 / 117, 64 / 130, 122 / 166, of 256 79 / 281, 174 / 315, 343 / 420; float32 of
+  // 128 79 / 156, 180 / 199, 355 / 299; one request of 2,048 rows, bfloat16 heads of 128: 10 / 10, 17 / 12, 33 / 14.  (Of bfloat16 heads of 128 only
+  // up to 48 rows come here: ops.py.)
   constexpr int kPass = kQ == 1 && D <= 128 ? 32 : 16, kStreamed = kQ == 1 ? 128 : 64;
   const int rows = max_q * p.group, passes = (rows + kPass - 1) / kPass;
   if (passes == 1 || (rows <= kStreamed && (long long)((max_context + 127) / 128) * p.nkv * num_seqs > 148 * passes)) {

@@ -2746,6 +2746,9 @@ _KV4_EXPAND_PAGE = 128
 # Least key blocks of a run (us with 1 / 3 / 6 and without runs, 32 query and 8 key heads: 64 tokens over 1,024 rows 28 / 30 / 34 / 34, over 4,096
 # 38 / 36 / 40 / 83; 512 over 2,048 44 / 44 / 44 / 52; 256 over 512 28 / 26 / 26 / 26).
 _KV4_MIN_RUN = 3
+# Most query rows whose weights are streamed (kv4_attention.cu), of bfloat16 heads of 128; with more they are added up on tcgen05 (us streamed / tcgen05: 32
+# rows, 16 requests of 4,096 44 / 98, one of 8,192 21 / 23; 48 rows 71 / 98, 30 / 23; 64 rows 83 / 98, 36 / 23; 96 rows 120 / 100, 52 / 23).
+_KV4_WEIGHTS_STREAMED_ROWS = 48
 
 
 def _kv4_tcgen05_library(scored: bool = False) -> ctypes.CDLL:
@@ -2826,9 +2829,7 @@ def attention_kv4_weights(
         raise KernelError(f"attention_kv4_weights: lse must have {T * nq} entries, got {lse.numel()}")
     _kv4_sums("attention_kv4_weights", sums, pool)
     rows = max_seqlen_q * (nq // nkv)
-    # up to 128 rows of many keys are streamed (the figures stand at the rule in kv4_attention.cu)
-    streamed = rows <= ATTENTION_KV4_DIRECT_ROWS or (rows <= 128 and -(-max_context // 128) * nkv * num_seqs > 148 * -(-rows // 32))
-    if not streamed and code == 1 and attention_tcgen05_supported(nq, nkv, d, _KV4_EXPAND_PAGE):
+    if rows > _KV4_WEIGHTS_STREAMED_ROWS and code == 1 and attention_tcgen05_supported(nq, nkv, d, _KV4_EXPAND_PAGE):
         global _weights_kv4_tcgen05
         if _weights_kv4_tcgen05 is None:
             run = _kv4_tcgen05_library().ts_kv4_weights_tcgen05

@@ -1428,11 +1428,11 @@ TS_EXPORT int ts_latent_rebuilt_attention(const void* q, long long ld_q, const v
 // tile; the products take half as long and run on the other buffer meanwhile, and two groups of eight warps take the tiles in turn, so that one's
 // exponentials run while the other waits (a portion of 512 tokens over 2,048 rows, 32 query and 8 key heads: 22 us; with all sixteen warps on a
 // tile 26).  Before a CTA's first tile 2.5 us pass (block table, codes, tensor memory, queries), so a CTA stays and takes an item of 128 keys after
-// the other: the copying warp works out what they are and asks for their queries ahead, the adding warps have an item's codes in registers when
-// they begin it (16 requests of 4,096 rows with 192 query rows: 119 us, a CTA per item 222).
+// the other: the copying warp works out what they are and asks for their queries ahead, the adding warps unpack the next item's keys while the last
+// tiles are added up (16 requests of 4,096 rows with 192 query rows: 115 us, a CTA per item 222).
 constexpr int W_STAGES = 4, W_GROUP = 8, W_ADDERS = 2 * W_GROUP;  // warps that add; two groups of them take the tiles in turn
 constexpr int W_COLUMNS = BM / (W_GROUP / 4);                      // a tile's rows that a warp adds up
-constexpr uint32_t W_OFF_Q = 2 * BM * 128, W_SMEM = W_OFF_Q + W_STAGES * Q_BYTES, W_TMEM_COLS = 256;
+constexpr uint32_t W_KEYS = 2 * BM * 128, W_OFF_Q = 2 * W_KEYS, W_SMEM = W_OFF_Q + W_STAGES * Q_BYTES, W_TMEM_COLS = 256;
 // Places of the ring of items: the copying warp is at most six items ahead of the adding ones (four tiles asked for, two being added up) and writes two further.
 constexpr int W_ITEMS = 16;
 struct WeightParams {
@@ -1453,7 +1453,7 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
   ts_pdl_wait();  // (tensor memory is never held while waiting for another kernel)
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t q_full[W_STAGES], q_empty[W_STAGES], s_full[2], s_empty[2], k_full, item_full[W_ITEMS];
+  __shared__ __align__(8) uint64_t q_full[W_STAGES], q_empty[W_STAGES], s_full[2], s_empty[2], k_full[2], item_full[W_ITEMS];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
   __shared__ WeightItem items[W_ITEMS];
@@ -1507,8 +1507,7 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
     if (lane == 0) {
       abort_s = 0;
       for (int i = 0; i < W_STAGES; ++i) mbar_init(smem_u32(&q_full[i]), 1), mbar_init(smem_u32(&q_empty[i]), 1);
-      for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_full[i]), 1), mbar_init(smem_u32(&s_empty[i]), W_GROUP);
-      mbar_init(smem_u32(&k_full), W_ADDERS);
+      for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_full[i]), 1), mbar_init(smem_u32(&s_empty[i]), W_GROUP), mbar_init(smem_u32(&k_full[i]), W_ADDERS);
       for (int i = 0; i < W_ITEMS; ++i) mbar_init(smem_u32(&item_full[i]), 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1558,7 +1557,8 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&item_full[it % W_ITEMS]), (uint32_t)(it / W_ITEMS) & 1, abort_flag));
       const int tiles = ok ? items[it % W_ITEMS].tiles : 0;
       if (tiles == 0) break;
-      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full), (uint32_t)it & 1, abort_flag));
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[it & 1]), (uint32_t)(it >> 1) & 1, abort_flag));
+      const uint64_t kd = k_desc + (uint64_t)((it & 1) * W_KEYS >> 4);
       for (int j = 0; ok && j < tiles; ++j, ++J) {
         const int st = J % W_STAGES, buf = J & 1;
         ok = mbar_wait(smem_u32(&q_full[st]), (uint32_t)(J / W_STAGES) & 1, abort_flag);
@@ -1571,8 +1571,8 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
             const uint32_t off = ((ks >> 2) * (BM * 128) + (ks & 3) * 32) >> 4;
-            if (ks == 0) umma_bf16_first(tmem_base + buf * BM, k_desc + off, qd + off, idesc(BM, false));
-            else umma_bf16_more(tmem_base + buf * BM, k_desc + off, qd + off, idesc(BM, false));
+            if (ks == 0) umma_bf16_first(tmem_base + buf * BM, kd + off, qd + off, idesc(BM, false));
+            else umma_bf16_more(tmem_base + buf * BM, kd + off, qd + off, idesc(BM, false));
           }
           umma_commit(smem_u32(&q_empty[st]));
           umma_commit(smem_u32(&s_full[buf]));
@@ -1605,52 +1605,58 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
         }
       }
     };
-    if (items[0].tiles != 0) load_codes(items[0]);
+    // and to their places in the swizzled operand (two of them in turns: nothing reads the item's before the last any more)
+    auto unpack = [&](int it) {
+#pragma unroll
+      for (int i = 0; i < kShare; ++i) {
+        const int r = (tid + adders * i) >> 4, c = tid & 15;
+        *reinterpret_cast<uint4*>(smem + (it & 1) * W_KEYS + (c >> 3) * (BM * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = kv4_unpack(code[i], scale[i]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&k_full[it & 1]));
+    };
+    // A tile's rows: their logarithms and last visible keys; rows that are none give no weight.  Asked for a tile before they are told, so that nobody
+    // waits for them.
+    float told_lse = INFINITY;
+    int told_pos = -1;
+    auto ask = [&](const WeightItem& item, int j) {
+      const int token = (item.tile0 + j) * per_tile + member / G;
+      const bool there = member < RT && token < item.q_len && j < item.tiles;
+      told_lse = there ? p.lse[(size_t)(item.q_begin + token) * p.nq + item.head * G + member % G] : INFINITY;
+      told_pos = there ? item.before + token : -1;
+    };
+    if (items[0].tiles != 0) {
+      load_codes(items[0]);
+      if (member < BM) ask(items[0], g);
+      unpack(0);
+    }
     bool ok = true;
     int J0 = 0;  // tiles of the items before
     for (int it = 0;; ++it) {
-      const WeightItem& item = items[it % W_ITEMS];
+      const WeightItem &item = items[it % W_ITEMS], &next = items[(it + 1) % W_ITEMS];
       const int tiles = item.tiles;
       if (tiles == 0) break;
       const int key = item.key0 + row, last_key = min(item.key0 + BM, item.ctx) - 1, first_j = (g - J0) & 1;
-      // A tile's rows: their logarithms and last visible keys; rows that are none give no weight.  Asked for a tile before they are told, so that nobody
-      // waits for them.
-      float told_lse = INFINITY;
-      int told_pos = -1;
-      auto ask = [&](int j) {
-        const int token = (item.tile0 + j) * per_tile + member / G;
-        const bool there = member < RT && token < item.q_len && j < tiles;
-        told_lse = there ? p.lse[(size_t)(item.q_begin + token) * p.nq + item.head * G + member % G] : INFINITY;
-        told_pos = there ? item.before + token : -1;
-      };
       auto tell = [&](int j) {
         const int turn = ((J0 + j) >> 1) & 1;
         lse_s[g][turn][member] = told_lse * 1.4426950408889634f, pos_s[g][turn][member] = told_pos;
       };
-      if (member < BM) ask(first_j);
-      // the keys to their places in the swizzled operand (nothing reads the ones before any more: the barrier at the end of an item)
-#pragma unroll
-      for (int i = 0; i < kShare; ++i) {
-        const int r = (tid + adders * i) >> 4, c = tid & 15;
-        *reinterpret_cast<uint4*>(smem + (c >> 3) * (BM * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = kv4_unpack(code[i], scale[i]);
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&k_full));
       if (member < BM) {
         tell(first_j);
-        ask(first_j + 2);
+        ask(item, first_j + 2);
       }
       // the next item's codes are on their way while this one's tiles are added up
       const bool known = mbar_wait(smem_u32(&item_full[(it + 1) % W_ITEMS]), (uint32_t)((it + 1) / W_ITEMS) & 1, abort_flag);
-      if (known && items[(it + 1) % W_ITEMS].tiles != 0) load_codes(items[(it + 1) % W_ITEMS]);
+      const bool more = __all_sync(0xffffffffu, known) && next.tiles != 0;
+      if (more) load_codes(next);
 
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
       for (int j = first_j; j < tiles; j += 2) {
         asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(W_GROUP * 32) : "memory");  // tile j's rows are told, tile j - 2's have been read
         if (member < BM) {
           tell(j + 2);
-          ask(j + 4);
+          ask(item, j + 4);
         }
         const int turn = ((J0 + j) >> 1) & 1;
         if (ok) ok = mbar_wait(smem_u32(&s_full[g]), (uint32_t)turn, abort_flag);
@@ -1693,6 +1699,10 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
             }
           }
         }
+      }
+      if (more) {
+        unpack(it + 1);
+        if (member < BM) ask(next, (g - J0 - tiles) & 1);
       }
       float (*slice)[BM] = slice_s[it & 1];  // (in turns: the next item's may be written while these are read)
       slice[warp >> 2][row] = (sum[0] + sum[1]) + (sum[2] + sum[3]);

@@ -1426,10 +1426,11 @@ TS_EXPORT int ts_latent_rebuilt_attention(const void* q, long long ld_q, const v
 // by TMA as the second, so that S^T[key][row] lies in tensor memory with a key per lane: a thread adds up its own key's weights in a
 // register, nothing is exchanged until the end.  What bounds it is the special-function unit, 16 exponentials a clock for 16,384 of a
 // tile; the products take half as long and run on the other buffer meanwhile, and two groups of eight warps take the tiles in turn, so that one's
-// exponentials run while the other waits (a portion of 512 tokens over 2,048 rows, 32 query and 8 key heads: 22 us; with all sixteen warps on a
-// tile 26).  Before a CTA's first tile 2.5 us pass (block table, codes, tensor memory, queries), so a CTA stays and takes an item of 128 keys after
+// exponentials run while the other waits (a portion of 512 tokens over 2,048 rows, 32 query and 8 key heads: 21 us; with all sixteen warps on a
+// tile 25).  Before a CTA's first tile 2.5 us pass (block table, codes, tensor memory, queries), so a CTA stays and takes an item of 128 keys after
 // the other: the copying warp works out what they are and asks for their queries ahead, the adding warps unpack the next item's keys while the last
-// tiles are added up (16 requests of 4,096 rows with 192 query rows: 115 us, a CTA per item 222).
+// tiles are added up (16 requests of 4,096 rows with 192 query rows: 110 us, a CTA per item 222; a prompt of 8,192 tokens 382, 0.42 of the bf16
+// peak, 450 before).  A prompt of 2,048 has 128 items, of which the first of a head has 64 tiles and the last 4: 62 us.
 constexpr int W_STAGES = 4, W_GROUP = 8, W_ADDERS = 2 * W_GROUP;  // warps that add; two groups of them take the tiles in turn
 constexpr int W_COLUMNS = BM / (W_GROUP / 4);                      // a tile's rows that a warp adds up
 constexpr uint32_t W_KEYS = 2 * BM * 128, W_OFF_Q = 2 * W_KEYS, W_SMEM = W_OFF_Q + W_STAGES * Q_BYTES, W_TMEM_COLS = 256;
@@ -1466,14 +1467,16 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
   constexpr int adders = W_ADDERS * 32;
 
   // ---- the copying warp works out this CTA's items, two ahead of the one whose queries it asks for
-  int next_index = blockIdx.x;
+  // (the first chunks of all heads first: in a prompt they have the most tiles.  Round after round of the CTAs goes there and back over the items.)
+  int round = 0;
   auto publish = [&](int it) {
     WeightItem* item = &items[it % W_ITEMS];
-    const int per_seq = p.chunks * p.nkv, all = per_seq * p.num_seqs;
+    const int per_chunk = p.nkv * p.num_seqs, all = p.chunks * per_chunk, ctas = (int)gridDim.x;
     int tiles = 0;
-    while (next_index < all) {
-      const int index = next_index, b = index / per_seq, rest = index - b * per_seq, head = rest / p.chunks, key0 = (rest - head * p.chunks) * BM;
-      next_index += gridDim.x;
+    for (; round * ctas < all; ++round) {
+      const int index = round * ctas + (round & 1 ? ctas - 1 - (int)blockIdx.x : (int)blockIdx.x);
+      if (index >= all) continue;
+      const int chunk = index / per_chunk, rest = index - chunk * per_chunk, b = rest / p.nkv, head = rest - b * p.nkv, key0 = chunk * BM;
       const int q_begin = min(max(p.cu[b], 0), p.tokens), q_len = min(max(p.cu[b + 1], q_begin), p.tokens) - q_begin;
       const int ctx = min(p.context[b], p.table_stride * page_size), before = ctx - q_len;
       if (key0 >= ctx) continue;
@@ -1488,6 +1491,7 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
       }
       if (lane == 0)
         item->tile0 = tile0, item->key0 = key0, item->ctx = ctx, item->before = before, item->q_begin = q_begin, item->q_len = q_len, item->head = head;
+      ++round;
       break;
     }
     if (lane == 0) item->tiles = tiles;
@@ -1620,15 +1624,25 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
     // waits for them.
     float told_lse = INFINITY;
     int told_pos = -1;
-    auto ask = [&](const WeightItem& item, int j) {
-      const int token = (item.tile0 + j) * per_tile + member / G;
-      const bool there = member < RT && token < item.q_len && j < item.tiles;
-      told_lse = there ? p.lse[(size_t)(item.q_begin + token) * p.nq + item.head * G + member % G] : INFINITY;
-      told_pos = there ? item.before + token : -1;
+    const int my_token = member < RT ? member / G : 0x40000000, my_head = member % G;
+    int lse_token = 0, lse_end = 0, lse_before = 0;  // the item's next tile asked for: this thread's token, the end of the tokens, the keys ahead of them
+    const float* lse_at = nullptr;
+    auto ask = [&]() {
+      const bool there = lse_token < lse_end;
+      told_lse = there ? *lse_at : INFINITY;
+      told_pos = there ? lse_before + lse_token : -1;
+      lse_token += 2 * per_tile;
+      lse_at += (size_t)(2 * per_tile) * p.nq;
+    };
+    auto ask_first = [&](const WeightItem& item, int j) {
+      lse_token = (item.tile0 + j) * per_tile + my_token;
+      lse_end = min(item.q_len, (item.tile0 + item.tiles) * per_tile), lse_before = item.before;
+      lse_at = p.lse + (ptrdiff_t)(item.q_begin + lse_token) * p.nq + item.head * G + my_head;
+      ask();
     };
     if (items[0].tiles != 0) {
       load_codes(items[0]);
-      if (member < BM) ask(items[0], g);
+      if (member < BM) ask_first(items[0], g);
       unpack(0);
     }
     bool ok = true;
@@ -1638,13 +1652,16 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
       const int tiles = item.tiles;
       if (tiles == 0) break;
       const int key = item.key0 + row, last_key = min(item.key0 + BM, item.ctx) - 1, first_j = (g - J0) & 1;
+      // the tiles whose rows all exist and see all keys: before + their first token >= the last key, their last token < q_len and within the window
+      const int all0 = (max(0, last_key - item.before) + per_tile - 1) / per_tile - item.tile0;
+      const int all1 = (p.window == 0 ? item.q_len : min(item.q_len, max(0, item.key0 + p.window - item.before))) / per_tile - item.tile0;
       auto tell = [&](int j) {
         const int turn = ((J0 + j) >> 1) & 1;
         lse_s[g][turn][member] = told_lse * 1.4426950408889634f, pos_s[g][turn][member] = told_pos;
       };
       if (member < BM) {
         tell(first_j);
-        ask(item, first_j + 2);
+        ask();
       }
       // the next item's codes are on their way while this one's tiles are added up
       const bool known = mbar_wait(smem_u32(&item_full[(it + 1) % W_ITEMS]), (uint32_t)((it + 1) / W_ITEMS) & 1, abort_flag);
@@ -1656,15 +1673,14 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
         asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(W_GROUP * 32) : "memory");  // tile j's rows are told, tile j - 2's have been read
         if (member < BM) {
           tell(j + 2);
-          ask(item, j + 4);
+          ask();
         }
         const int turn = ((J0 + j) >> 1) & 1;
         if (ok) ok = mbar_wait(smem_u32(&s_full[g]), (uint32_t)turn, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const int first = (item.tile0 + j) * per_tile, last = first + per_tile - 1;  // the tile's tokens
-          const bool all = last < item.q_len && item.before + first >= last_key && (p.window == 0 || item.before + last - p.window < item.key0);
+          const bool all = j >= all0 && j < all1;
 #pragma unroll
           for (int part = 0; part < W_COLUMNS / 32; ++part) {
             uint32_t v[32];
@@ -1702,7 +1718,7 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
       }
       if (more) {
         unpack(it + 1);
-        if (member < BM) ask(next, (g - J0 - tiles) & 1);
+        if (member < BM) ask_first(next, (g - J0 - tiles) & 1);
       }
       float (*slice)[BM] = slice_s[it & 1];  // (in turns: the next item's may be written while these are read)
       slice[warp >> 2][row] = (sum[0] + sum[1]) + (sum[2] + sum[3]);

@@ -1,0 +1,36 @@
+"""The 4-bit cache: what its operators' workspaces held before, and the ends of what their arguments may be."""
+
+import pytest
+import torch
+
+from tests.test_kv4_gpu import check_attention
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from tokensprint_b200 import ops
+
+
+def spoil_workspaces(monkeypatch):
+    """Every float tensor of torch.empty is NaN from its first entry to its last."""
+    empty = torch.empty
+
+    def spoiled(*args, **kw):
+        t = empty(*args, **kw)
+        return t.fill_(float("nan")) if t.is_floating_point() else t
+
+    monkeypatch.setattr(torch, "empty", spoiled)
+
+
+@pytest.mark.parametrize("runs", [True, False])
+@pytest.mark.parametrize("oldest", [384, 385, 384 + 63, 384 + 64, 384 + 67, 384 + 127, 512])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_windowed_portions_read_only_what_was_unpacked(monkeypatch, runs, oldest, sinks):
+    """`oldest`, the first key that a query sees, lies anywhere in a page of 128 unpacked rows; the rows ahead of it have no weight, and
+    nothing times what they hold may be anything but zero."""
+    monkeypatch.setattr(ops, "_KV4_DIRECT_PIECES", 0)
+    if not runs:
+        monkeypatch.setattr(ops, "_KV4_MIN_RUN", 1 << 20)
+    spoil_workspaces(monkeypatch)
+    check_attention([(900, 150)], 5, 1, 128, 16, torch.bfloat16, window=900 - 150 + 1 - oldest, sinks=sinks)
+    check_attention([(900, 150), (300, 17), (64, 64)], 4, 2, 128, 32, torch.bfloat16, window=900 - 150 + 1 - oldest, sinks=sinks)

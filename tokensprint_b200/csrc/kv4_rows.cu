@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(128) load_kernel(const uint8_t* pool, const in
 
 // The rows that a batch's queries can see, of heads of 128, as bfloat16 pages of 128 rows for the prompt attention, and the block table of those
 // pages: request b has the pages [b * blocks, (b + 1) * blocks); out_lens: its rows, as many as have a place.  A CTA unpacks 64 rows of one head.
+// Of a page that holds a visible key every row up to the request's last is written; the attention itself clears what lies behind that one.
 // 2,048 rows of 8 heads: 6 us (2.4 MB in, 8.4 MB out), most of it the start and two trips to memory; the attention that follows reads them from the L2.
 constexpr int kExpandRows = 64, kExpandPage = 128, kExpandDim = 128;
 __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* pool, const int* table, int table_stride, const int* cu, const int* context, uint4* k,
@@ -166,7 +167,10 @@ __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* pool, const 
     if (first == 0) out_lens[b] = n;
   }
   const int queries = cu[b + 1] - cu[b], oldest = window > 0 ? n - queries - window + 1 : 0;  // the first key that some query sees
-  if (first >= n || first + kExpandRows <= oldest || queries <= 0) return;
+  // (The attention walks whole pages, from the first that holds a visible key on: what it reads ahead of that key weighs nothing, but has to be
+  // numbers.  So only whole pages are left out.)
+  const int page_end = first / kExpandPage * kExpandPage + kExpandPage;
+  if (first >= n || page_end <= oldest || queries <= 0) return;
   uint32_t code[kUnits], scale[kUnits];
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {

@@ -34,3 +34,14 @@ def test_windowed_portions_read_only_what_was_unpacked(monkeypatch, runs, oldest
     spoil_workspaces(monkeypatch)
     check_attention([(900, 150)], 5, 1, 128, 16, torch.bfloat16, window=900 - 150 + 1 - oldest, sinks=sinks)
     check_attention([(900, 150), (300, 17), (64, 64)], 4, 2, 128, 32, torch.bfloat16, window=900 - 150 + 1 - oldest, sinks=sinks)
+
+
+@pytest.mark.parametrize("lens", [[(3, 400)], [(0, 300), (20, 100)], [(130, 700), (700, 200), (1, 1)], [(1700, 30), (40, 330), (0, 65), (129, 129)]])
+@pytest.mark.parametrize("nq,nkv", [(4, 1), (6, 2)])
+@pytest.mark.parametrize("window,sinks", [(0, False), (0, True), (70, True)])
+def test_portions_with_more_tokens_than_rows(monkeypatch, lens, nq, nkv, window, sinks):
+    """Queries ahead of the first cached row see nothing, whole tiles of them included: zeros, and the logarithm of nothing or of the sink."""
+    monkeypatch.setattr(ops, "_KV4_DIRECT_PIECES", 0)
+    spoil_workspaces(monkeypatch)
+    check_attention(lens, nq, nkv, 128, 16, torch.bfloat16, window=window, sinks=sinks)
+    ops.check_device_errors()

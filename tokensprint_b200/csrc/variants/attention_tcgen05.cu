@@ -795,6 +795,22 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
   const int kb0 = lo / PBN + run * p.run_blocks;
   const int nblocks = p.run_blocks > 0 ? min(hi / PBN - kb0 + 1, p.run_blocks) : hi / PBN - kb0 + 1;
   if (run > 0 && nblocks <= 0) return;
+  if (hi < 0) {  // (a request with more tokens than rows) no row of the pair sees a key: zeros, before anything is copied or waited for
+    const int rows = min(ntiles * RT, rows_total - r0);
+    for (int i = tid; i < rows * (D / 8); i += blockDim.x) {
+      const int r = r0 + i / (D / 8), piece = i % (D / 8);
+      const size_t at = (size_t)(q_begin + r / G) * p.nq + hk * G + r % G;
+      const float lse = p.has_sink ? row_lse(p, row_sink_raw(p, hk, G, r), 1.f) : -INFINITY;
+      if (p.run_blocks > 0) {  // (run 0's, the only one that the rows have)
+        reinterpret_cast<float4*>(p.run_out + at * D)[2 * piece] = reinterpret_cast<float4*>(p.run_out + at * D)[2 * piece + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (piece == 0) p.run_lse[at] = lse;
+      } else {
+        reinterpret_cast<uint4*>(p.out + at * D)[piece] = make_uint4(0u, 0u, 0u, 0u);
+        if (piece == 0 && p.lse != nullptr) p.lse[at] = lse;
+      }
+    }
+    return;
+  }
 #else
   const int kb0 = lo / PBN;
   const int nblocks = hi / PBN - kb0 + 1;

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from tests.test_kv4_gpu import check_attention
+from tests.test_kv4_gpu import DEV, check_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,20 @@ def test_portions_with_more_tokens_than_rows(monkeypatch, lens, nq, nkv, window,
     spoil_workspaces(monkeypatch)
     check_attention(lens, nq, nkv, 128, 16, torch.bfloat16, window=window, sinks=sinks)
     ops.check_device_errors()
+
+
+def test_eviction_refuses_lengths_that_overlap():
+    """The new lengths in the place of the old ones, or of the block table: refused before anything is launched."""
+    nkv, d, page = 2, 64, 16
+    pool = torch.zeros(ops.kv4_pool_shape(8, page, nkv, d), dtype=torch.uint8, device=DEV)
+    sums = torch.ones((8, nkv, page), device=DEV)
+    words = torch.arange(16, dtype=torch.int32, device=DEV)
+    table, lens = words[:8].view(2, 4), words[8:12]
+    before = words.clone()
+    for new in (lens, words[9:], words[7:9], words[:2], words[6:8]):
+        with pytest.raises(ops.KernelError, match="overlap"):
+            ops.kv4_evict(pool, sums, table, lens, new, 2, 9, 4, 1)
+    assert torch.equal(words, before) and bool((sums == 1).all())
+    new = words[10:12]  # next to the two lengths that the call reads
+    ops.kv4_evict(pool, sums, table, lens, new, 2, 9, 4, 1)
+    assert new.tolist() == [4, 4] and torch.equal(words[:10], before[:10])

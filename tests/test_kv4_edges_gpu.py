@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from tests.test_kv4_gpu import DEV, check_attention
+from tests.test_kv4_gpu import DEV, check_attention, filled
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,19 @@ def test_eviction_refuses_lengths_that_overlap():
     new = words[10:12]  # next to the two lengths that the call reads
     ops.kv4_evict(pool, sums, table, lens, new, 2, 9, 4, 1)
     assert new.tolist() == [4, 4] and torch.equal(words[:10], before[:10])
+
+
+@pytest.mark.parametrize("budget,recent,first", [(300, 20, 4), (1 << 20, 1 << 19, 5), (1 << 45, 0, 1 << 44)])
+def test_a_budget_beyond_the_longest_request_takes_no_memory(budget, recent, first):
+    gen = torch.Generator().manual_seed(6)
+    lens, nkv, d, page = [300, 0, 7, 256], 2, 64, 16
+    pool, table, _, _ = filled([(n, 0) for n in lens], nkv, d, page, gen)
+    sums = torch.rand((pool.shape[0], nkv, page), generator=gen).to(DEV)
+    context, new = torch.tensor(lens, dtype=torch.int32, device=DEV), torch.full((4,), -5, dtype=torch.int32, device=DEV)
+    old_pool, old_sums = pool.clone(), sums.clone()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    ops.kv4_evict(pool, sums, table, context, new, 4, 300, budget, recent, first)
+    assert torch.cuda.max_memory_allocated() - held < 1 << 16
+    assert new.tolist() == lens and torch.equal(pool, old_pool) and torch.equal(sums, old_sums)

@@ -249,7 +249,7 @@ __device__ __forceinline__ uint4 peer_words(const uint32_t* p, int rank) {
 template <int D>
 __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(uint8_t* pool, float* sums, const int* table, int table_stride, const int* context,
                                                                  int* new_lens, int* order, int nkv, int page_blocks, int num_pages, int budget, int recent,
-                                                                 int first, int cluster, int room) {
+                                                                 int first, int longest, int cluster, int room) {
   extern __shared__ uint32_t kept_keys[];
   __shared__ __align__(16) uint32_t hist[3][kDigits], totals[4];
   __shared__ uint32_t scratch[kEvictWarps], chosen[2], warp_counts[2 * kEvictWarps], source[kMoveRows], target[kMoveRows];
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(uint8_t* pool, 
   ts_pdl_prologue();
   const int rank = blockIdx.x % cluster, head = blockIdx.x / cluster, b = blockIdx.y, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int page_size = page_blocks * KV4_BLOCK;
-  const int n = min(context[b], table_stride * page_size);
+  const int n = min(context[b], longest);  // (within the block table, and no row that has no place in `order`, whatever the length says)
   if (blockIdx.x == 0 && tid == 0) new_lens[b] = min(n, budget);
   if (n <= budget) return;
   table += (size_t)b * table_stride;
@@ -425,8 +425,10 @@ int launch_evict(uint8_t* pool, float* sums, const int* table, int table_stride,
   int cluster = 1;
   while (cluster < (pairs <= 16 ? 8 : 4) && cluster * kMoveRows < budget && pairs * cluster < 2 * 148) cluster *= 2;
   const int run = ((max_context + cluster - 1) / cluster + 31) / 32 * 32, room = run < kKeptKeys ? run : kKeptKeys;  // weights in shared memory
+  const long long places = (long long)table_stride * page_blocks * KV4_BLOCK;
+  const int longest = places < max_context ? (int)places : max_context;
   return ts_launch_cluster(evict_kernel<D>, dim3(nkv * cluster, num_seqs), dim3(kEvictThreads), (size_t)room * 4, stream, cluster, pool, sums, table, table_stride,
-                           context, new_lens, order, nkv, page_blocks, num_pages, budget, recent, first, cluster, room);
+                           context, new_lens, order, nkv, page_blocks, num_pages, budget, recent, first, longest, cluster, room);
 }
 
 }  // namespace
@@ -489,7 +491,7 @@ TS_EXPORT int ts_kv4_expand(const void* pool, const int* table, int table_stride
                    table_stride, cu, context, (uint4*)k, (uint4*)v, out_table, out_lens, nkv, page_blocks, num_pages, blocks, window);
 }
 
-// order: num_seqs * nkv * budget ints of workspace; context[b] <= max_context.
+// order: num_seqs * nkv * budget ints of workspace, none where budget >= max_context; context[b] <= max_context (a longer one counts as that).
 struct Kv4EvictArgs {
   void* pool;
   float* sums;

@@ -2852,7 +2852,7 @@ def kv4_evict(pool: torch.Tensor, sums: torch.Tensor, block_table: torch.Tensor,
 
     A request with more rows than that keeps, per head, the `first` first ones, the `recent` last ones and of the rest those with
     the largest `sums` (of equals the earlier, NaN before all).  They move to the front of the request's pages in their order, their sums with
-    them; the sums behind become 0.  block_table [B,max_blocks], context_lens [B] i32 (at most max_context); new_lens [B] i32, which must be
+    them; the sums behind become 0.  block_table [B,max_blocks], context_lens [B] i32 (at most max_context; a longer one counts as that); new_lens [B] i32, which must be
     memory of its own, receives min(length, budget).  Pages behind the new length can be given back.  A request's rows must all have their
     pages, and a page must belong to one request only."""
     flush_gemm_chain()
@@ -2871,7 +2871,10 @@ def kv4_evict(pool: torch.Tensor, sums: torch.Tensor, block_table: torch.Tensor,
     for label, t, n in (("context_lens", context_lens, num_seqs), ("block_table", block_table, num_seqs * block_table.shape[1])):
         if at < t.data_ptr() + 4 * n and t.data_ptr() < at + 4 * num_seqs:
             raise KernelError(f"kv4_evict: new_lens must not overlap {label}, which is read while it is written")
-    order = torch.empty(num_seqs * nkv * budget, device=pool.device, dtype=torch.int32)  # where every kept row comes from
+    places = budget
+    if budget >= max_context:  # no request has more rows: nothing to rank, and nowhere to move
+        budget, recent, first, places = max(1, max_context), 0, 0, 0
+    order = torch.empty(num_seqs * nkv * places, device=pool.device, dtype=torch.int32)  # where every kept row comes from
     _check("kv4_evict", _fn("ts_kv4_evict")(_KV4_EVICT_ARGS(
         pool.data_ptr(), sums.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(), new_lens.data_ptr(), order.data_ptr(), _stream(),
         block_table.shape[1], num_seqs, nkv, d, blocks, pages, max_context, budget, recent, first)))

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from tests.test_kv4_gpu import DEV, check_attention, filled
+from tests.test_kv4_gpu import DEV, batch, check_attention, filled
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,58 @@ def test_a_budget_beyond_the_longest_request_takes_no_memory(budget, recent, fir
     ops.kv4_evict(pool, sums, table, context, new, 4, 300, budget, recent, first)
     assert torch.cuda.max_memory_allocated() - held < 1 << 16
     assert new.tolist() == lens and torch.equal(pool, old_pool) and torch.equal(sums, old_sums)
+
+
+FORMS = [  # tokens of a request, head size, type: streamed, streamed in passes, keys in registers (twice), keys in tensor memory
+    (1, 128, torch.bfloat16), (20, 64, torch.bfloat16), (200, 64, torch.bfloat16), (90, 128, torch.float32), (200, 128, torch.bfloat16)]
+
+
+@pytest.mark.parametrize("tokens,d,dtype", FORMS)
+def test_weights_leave_rows_that_nobody_sees_alone(tokens, d, dtype):
+    """Pages ahead of the window have been given back (-1 in the block table, page 0 to the kernels): whoever has page 0 now loses nothing.
+    Every request adds to every row of its own once, so the bits are those of a call in which the pages are still held."""
+    gen = torch.Generator().manual_seed(21)
+    nq, nkv, page, window = 16, 8, 16, 20
+    lens = [(tokens, tokens)] + [(400 + 16 * b, tokens) for b in range(12)]
+    pool, table, _, _ = filled(lens, nkv, d, page, gen, spoil=False)
+    swap = table.clone()  # the request whose keys are all seen has page 0
+    swap[table == 0], swap[table == table[0, 0]] = table[0, 0], 0
+    table = swap
+    given = table.clone()
+    for b, (n, t) in enumerate(lens):
+        given[b, : max(0, n - t - window + 1) // page] = -1
+    assert int((given < 0).sum()) > int((table < 0).sum())
+    T = sum(t for _, t in lens)
+    q = torch.randn((T, nq * d), generator=gen).to(dtype).to(DEV)
+    cu, context = batch(lens)
+    lse = torch.full((T, nq), 3.0, device=DEV)
+    sizes = (len(lens), tokens, max(n for n, _ in lens), nq, nkv, d, d**-0.5)
+    want = torch.ones((pool.shape[0], nkv, page), device=DEV)
+    ops.attention_kv4_weights(q, pool, lse, want, cu, context, table, *sizes, window=window)
+    assert bool((want[0] != 1).all()) or tokens < page
+    for _ in range(20):
+        sums = torch.ones_like(want)
+        ops.attention_kv4_weights(q, pool, lse, sums, cu, context, given, *sizes, window=window)
+        assert torch.equal(sums, want)
+
+
+@pytest.mark.parametrize("tokens,d,dtype", FORMS)
+def test_weights_of_pages_that_requests_share(tokens, d, dtype):
+    """Requests over the same pages: every one of them adds its weights.  The sums of 13 float32 numbers in any order are off by 13 * 2^-24; a request
+    by itself may take another of the kernels, whose weights are off by 4 * 2^-18 (reach + 1) as in check_attention, with a reach below 15: 2^-12."""
+    gen = torch.Generator().manual_seed(22)
+    nq, nkv, page, n, B = 16, 8, 16, 400, 12
+    pool, table, _, _ = filled([(n, tokens)], nkv, d, page, gen)
+    q = torch.randn((B, tokens, nq * d), generator=gen).to(dtype).to(DEV)
+    lse = torch.full((B * tokens, nq), 3.0, device=DEV)
+    want = torch.ones((pool.shape[0], nkv, page), device=DEV, dtype=torch.float64)
+    cu, context = batch([(n, tokens)])
+    for b in range(B):
+        one = torch.zeros(want.shape, device=DEV)
+        ops.attention_kv4_weights(q[b], pool, lse[:tokens], one, cu, context, table, 1, tokens, n, nq, nkv, d, d**-0.5)
+        want += one
+    cu, context = batch([(n, tokens)] * B)
+    for _ in range(20):
+        sums = torch.ones(want.shape, device=DEV)
+        ops.attention_kv4_weights(q.flatten(0, 1), pool, lse, sums, cu, context, table.expand(B, -1).contiguous(), B, tokens, n, nq, nkv, d, d**-0.5)
+        assert ((sums - want).abs() <= 13 * 2.0**-24 * want + 2.0**-12 * (want - 1)).all()

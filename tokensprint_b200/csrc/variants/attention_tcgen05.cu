@@ -1746,8 +1746,11 @@ __global__ void __launch_bounds__((W_ADDERS + 2) * 32, 1) kv4_weights_kernel(con
           : "n"(adders)
           : "memory");
       if (go_on == 0) break;
-      if (warp < 4 && key < item.ctx)
-        p.sums[(size_t)item.rec[row / KV4_BLOCK] * KV4_BLOCK + row % KV4_BLOCK] += (slice[0][row] + slice[1][row]) + (slice[2][row] + slice[3][row]);
+      if (warp < 4 && key < item.ctx) {
+        // (a key that nobody sees is left alone: its page may have been given back, and `rec` then names another's)
+        const float w = (slice[0][row] + slice[1][row]) + (slice[2][row] + slice[3][row]);
+        if (w != 0.f) atomicAdd(p.sums + (size_t)item.rec[row / KV4_BLOCK] * KV4_BLOCK + row % KV4_BLOCK, w);
+      }
       J0 += tiles;
     }
   }

@@ -567,8 +567,8 @@ __global__ void __launch_bounds__(kWarps * 32, D > 128 || sizeof(T) != 2 ? 1 : k
 // weights: w_j += sum over the rows r of exp(s_rj - lse_r).  A warp owns 16 keys of one head at a time.
 
 // Few rows (kTiles tiles of 8): the warp goes over records kWarps * gridDim.x apart, the next one's codes on their way while it works on
-// one; a key's sum is complete when its record is done, and is added without being read first (no other warp of the launch adds to it, so its
-// value does not depend on any order).  Only the keys' half of a record is read, in words straight to registers: no shared memory, no barrier.
+// one; a key's sum is complete when its record is done, and is added without being read first (no other warp of the launch adds to it, unless requests
+// share its page, so its value does not depend on any order).  Only the keys' half of a record is read, in words straight to registers: no shared memory, no barrier.
 // Bound like attention_kernel by unpacking; 16 requests of up to 4,096 rows, 4 query rows a key head: 14 us (45 MB with the sums).
 template <typename T, int kQ, int kTiles>
 __global__ void __launch_bounds__(kWarps * 32) weights_kernel(const Params p, float* sums, int first_row) {
@@ -811,7 +811,8 @@ __global__ void __launch_bounds__(kWeightThreads, 1) weights_rows_kernel(const P
 #pragma unroll
     for (int i = 0; i < kRowWarps; ++i) sum += meet[i][threadIdx.x];
     const int page_size = p.page_blocks * KV4_BLOCK, page = p.table[(size_t)tile.b * p.table_stride + at / page_size];
-    sums[((size_t)min(max(page, 0), p.num_pages - 1) * p.nkv + tile.head) * page_size + at % page_size] += sum;
+    // (A key that nobody sees is left alone: its page may have been given back.  One add to a key of a page that requests do not share, so in one order.)
+    if (sum != 0.f) atomicAdd(sums + ((size_t)min(max(page, 0), p.num_pages - 1) * p.nkv + tile.head) * page_size + at % page_size, sum);
   }
 }
 

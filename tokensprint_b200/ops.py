@@ -2819,7 +2819,8 @@ def attention_kv4_weights(
 ) -> None:
     """Adds to every cached row the weight that this step's queries gave it: sums[row] += sum over the queries and the
     query heads of the row's key head of exp(scale q.k - lse).  Arguments as in attention_kv4, `lse` as it wrote it (sinks are in it);
-    sums [pages, nkv, page size] f32.  Every row's sum is formed in one order: equal inputs give equal bits."""
+    sums [pages, nkv, page size] f32.  Every row's sum is formed in one order: equal inputs give equal bits.  (A page that several
+    requests share gets the weights of all of them, one after the other in no fixed order.)"""
     flush_gemm_chain()
     nq, nkv, d = num_heads, num_kv_heads, head_dim
     pages, blocks, code, T, width = _check_attention_kv4("attention_kv4_weights", q, pool, cu_seqlens_q, context_lens, block_table, num_seqs,

@@ -133,3 +133,11 @@ def test_weights_of_pages_that_requests_share(tokens, d, dtype):
         sums = torch.ones(want.shape, device=DEV)
         ops.attention_kv4_weights(q.flatten(0, 1), pool, lse, sums, cu, context, table.expand(B, -1).contiguous(), B, tokens, n, nq, nkv, d, d**-0.5)
         assert ((sums - want).abs() <= 13 * 2.0**-24 * want + 2.0**-12 * (want - 1)).all()
+
+
+@pytest.mark.parametrize("tokens,d,dtype", FORMS)
+@pytest.mark.parametrize("window", [449, 450, 1 << 20, (1 << 31) - 1])
+def test_windows_beyond_the_longest_request(tokens, d, dtype, window):
+    """A window that no key falls out of is none, however large the number is (449 still hides a key from the last token)."""
+    check_attention([(450, tokens), (tokens, tokens), (30, 1)], 8, 4, d, 16, dtype, window=window)
+    check_attention([(450, tokens), (3, 9)], 4, 1, d, 16, dtype, window=window)

@@ -2729,6 +2729,8 @@ def attention_kv4(
                 _cuda_contig(f"attention_kv4: {label}", t, torch.float32)
                 if t.numel() != n:
                     raise KernelError(f"attention_kv4: {label} must have {n} entries, got {t.numel()}")
+    if window >= max_context:  # no key is older than that (and the kernels add windows to key numbers in 32 bits)
+        window = 0
     rows = max_seqlen_q * (nq // nkv)
     if (rows > ATTENTION_KV4_DIRECT_ROWS and code == 1 and -(-rows // 16) * -(-max_context // KV4_BLOCK) * nkv * num_seqs > _KV4_DIRECT_PIECES
             and attention_tcgen05_supported(nq, nkv, d, _KV4_EXPAND_PAGE)):
@@ -2829,6 +2831,8 @@ def attention_kv4_weights(
     if lse.numel() != T * nq:
         raise KernelError(f"attention_kv4_weights: lse must have {T * nq} entries, got {lse.numel()}")
     _kv4_sums("attention_kv4_weights", sums, pool)
+    if window >= max_context:  # as in attention_kv4
+        window = 0
     rows = max_seqlen_q * (nq // nkv)
     if rows > _KV4_WEIGHTS_STREAMED_ROWS and code == 1 and attention_tcgen05_supported(nq, nkv, d, _KV4_EXPAND_PAGE):
         global _weights_kv4_tcgen05

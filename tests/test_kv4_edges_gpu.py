@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from tests.plain import kv4_plain as plain
 from tests.test_kv4_gpu import DEV, batch, check_attention, filled
 
 pytestmark = pytest.mark.gpu
@@ -141,3 +142,30 @@ def test_windows_beyond_the_longest_request(tokens, d, dtype, window):
     """A window that no key falls out of is none, however large the number is (449 still hides a key from the last token)."""
     check_attention([(450, tokens), (tokens, tokens), (30, 1)], 8, 4, d, 16, dtype, window=window)
     check_attention([(450, tokens), (3, 9)], 4, 1, d, 16, dtype, window=window)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens", [1, 3, 100])
+@pytest.mark.parametrize("pieces", [0, 600])
+def test_sinks_of_minus_infinity_are_none(monkeypatch, dtype, tokens, pieces):
+    """Heads without a sink beside heads with one; requests that see nothing: zeros, and the logarithm of nothing or of the sink."""
+    monkeypatch.setattr(ops, "_KV4_DIRECT_PIECES", pieces)
+    gen = torch.Generator().manual_seed(31)
+    nq, nkv, d, page = 8, 2, 128, 16
+    lens = [(0, tokens), (40, tokens), (tokens, tokens), (0, 1)]
+    pool, table, keys, values = filled(lens, nkv, d, page, gen)
+    T = sum(t for _, t in lens)
+    q = torch.randn((T, nq * d), generator=gen).to(dtype).to(DEV)
+    cu, context = batch(lens)
+    sizes = (cu, context, table, len(lens), tokens, max(n for n, _ in lens), nq, nkv, d, d**-0.5)
+    sink = torch.randn(nq, generator=gen).to(DEV)
+    sink[::2] = -torch.inf
+    out, lse = torch.empty_like(q), torch.empty((T, nq), device=DEV)
+    ops.attention_kv4(q, pool, out, *sizes, head_sinks=sink, lse=lse)
+    want, want_lse, _, spread, reach = plain.attention(q.double().view(T, nq, d), keys, values, lens, 0, sink.double(), d**-0.5)
+    exact, slack = dtype == torch.float32, 2.0**-18 * (reach + 1)  # the bounds of check_attention
+    bound = ((2.0**-20 if exact else 2.0**-8) + 2 * slack[..., None]) * spread + (2.0**-22 if exact else 2.0**-8) * want.abs() + 1e-30
+    assert ((out.double().view(T, nq, d) - want).abs() <= bound).all()
+    empty = torch.isinf(want_lse)
+    assert torch.equal(torch.isinf(lse), empty) and int(empty.sum()) >= tokens * nq // 2
+    assert ((lse.double() - want_lse).abs() <= slack + 2.0**-20 * (1 + want_lse.abs()))[~empty].all()

@@ -146,7 +146,7 @@ template <typename T>
 __device__ __forceinline__ void write_row(const Params& p, const Tile& tile, int row, int channel, float4 o, float m, float l) {
   const int head = tile.query_head(p, row);
   if (p.sinks != nullptr) {
-    const float sink = fmaxf(p.sinks[head] * kLog2e, kLowest), top = fmaxf(m, sink), f = kv4_exp2(m - top);
+    const float sink = p.sinks[head] * kLog2e, top = fmaxf(m, sink), f = kv4_exp2(m - top);  // (m is finite, so a sink of -inf is none)
     l = l * f + kv4_exp2(sink - top);
     o.x *= f, o.y *= f, o.z *= f, o.w *= f;
     m = top;

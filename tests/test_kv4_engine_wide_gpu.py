@@ -40,3 +40,50 @@ def test_portions_in_bfloat16(tmp_path, monkeypatch, cfg, cuts):
     yard = plain.forward_logits(rounded(weights), cfg, ids, rounding=plain.round_to_bfloat16)
     assert (got.cpu().double() - want).norm() < 1.5 * (yard - want).norm()
     assert runner.cache_manager.pages_in_use() == 0
+
+
+def checked_engine(monkeypatch, folder, config, **kw):
+    """An engine whose requests are looked at after every step: [rows that one was cut from], and no request may hold more than the
+    budget and its slack."""
+    from tokensprint_b200.cache.manager import CacheManager
+    from tokensprint_b200.config.engine_config import Config
+    from tokensprint_b200.engine.llm_engine import LLMEngine
+    from tokensprint_b200.engine.runner import ModelRunner
+    from tokensprint_b200.models.api import load_model
+
+    cuts, shrink, step = [], CacheManager.shrink, ModelRunner.step
+
+    def counting(self, rc, rows):
+        cuts.append((rc.request, rc.num_tokens))
+        shrink(self, rc, rows)
+
+    def looking(self, entries, *args, **kw):
+        logits = step(self, entries, *args, **kw)
+        assert all(e.cache.num_tokens <= config["cache_budget"] + config["cache_slack"] for e in entries)
+        self.cache_manager.check_invariants()
+        return logits
+
+    monkeypatch.setattr(CacheManager, "shrink", counting)
+    monkeypatch.setattr(ModelRunner, "step", looking)
+    model, _ = load_model(folder, device="cuda", dtype="bfloat16")
+    return LLMEngine(model, Config(model=str(folder), max_model_len=1024, max_num_seqs=4, chunked_prefill=True, enforce_eager=False, cache_format="kv4",
+                                   **config, **kw)), cuts
+
+
+@pytest.mark.parametrize("overlap", [True, False])
+def test_a_prompt_larger_than_the_pool_through_the_entry_point(tmp_path, monkeypatch, overlap):
+    """Six pages of 16 rows, prompts of up to 700 tokens: cut after every portion, they run."""
+    from tokensprint_b200.config.engine_config import SamplingParams
+
+    folder, _ = make_folder(tmp_path, WIDE, 7)
+    config = dict(cache_budget=48, cache_recent=16, cache_slack=16, num_kvcache_blocks=6, kvcache_block_size=16, max_num_batched_tokens=32)
+    engine, cuts = checked_engine(monkeypatch, folder, config, overlap_steps=overlap)
+    prompts = [random_tokens(WIDE, n, 60 + n) for n in (700, 20, 333)]
+    out = engine.generate(prompts, SamplingParams(temperature=0.0, max_tokens=60, ignore_eos=True), use_tqdm=False)
+    assert [len(o) for o in out] == [60] * 3
+    # of n + 59 tokens that were stored at most 64 have a row at the end
+    dropped = {}
+    for request, rows in cuts:
+        dropped[request] = dropped.get(request, 0) + rows - 48
+    assert len(dropped) == 3 and all(gone >= n + 59 - 64 for gone, n in zip(sorted(dropped.values()), (20, 333, 700)))
+    assert engine.model_runner.cache_manager.pages_in_use() == 0

@@ -5,7 +5,9 @@ import pytest
 from tokensprint_b200 import ops
 from tokensprint_b200.cache.manager import CacheError, CacheManager, GroupSpec
 from tokensprint_b200.cache.tensors import page_bytes
-from tokensprint_b200.config.engine_config import Config
+from tokensprint_b200.config.engine_config import Config, SamplingParams
+from tokensprint_b200.engine.scheduler import Scheduler
+from tokensprint_b200.engine.sequence import Sequence
 from tokensprint_b200.parts.base import CacheNeed
 
 
@@ -69,3 +71,46 @@ def test_options(tmp_path):
         Config(model=str(tmp_path), cache_budget=512)
     with pytest.raises(ValueError, match="cache_budget"):
         Config(model=str(tmp_path), cache_format="kv4", cache_budget=-1)
+
+
+def budgeted(tmp_path, budget, **kw):
+    options = dict(num_kvcache_blocks=6, kvcache_block_size=16, max_num_batched_tokens=32, max_num_seqs=4, max_model_len=4096, chunked_prefill=True,
+                   cache_format="kv4", cache_budget=budget, cache_recent=8, cache_slack=16)
+    options.update(kw)
+    config = Config(model=str(tmp_path), **options)
+    cm = CacheManager([GroupSpec("full")], 16, [options["num_kvcache_blocks"]], options["max_num_seqs"])
+    return Scheduler(config, cm), config
+
+
+def test_a_budget_admits_prompts_longer_than_the_pool(tmp_path):
+    """48 + 16 + 32 rows at most: six pages of 16 carry any prompt that comes in portions, alone and beside others."""
+    s, config = budgeted(tmp_path, 48)
+    seqs = [Sequence([1] * n, SamplingParams(max_tokens=40, ignore_eos=True)) for n in (700, 90, 333)]
+    for x in seqs:
+        s.add_sequence(x)
+    most = steps = 0
+    while not s.is_finished():
+        step = s.schedule()
+        need = [i for i, x in enumerate(step) if x.num_cached_tokens + x.num_new_tokens == len(x)]
+        for x in step:  # what the runner does behind a step
+            most = max(most, x.cache.num_tokens)
+            if x.cache.num_tokens > config.cache_budget + config.cache_slack:
+                s.cache_manager.shrink(x.cache, config.cache_budget)
+        s.postprocess(step, [1] * len(need), need)
+        s.cache_manager.check_invariants()
+        steps += 1
+        assert steps < 5000
+    assert [x.num_completion_tokens for x in seqs] == [40] * 3 and most <= 96
+    assert s.cache_manager.pages_in_use() == 0
+
+
+def test_what_a_budget_does_not_admit(tmp_path):
+    for kw in (dict(budget=0), dict(budget=49), dict(budget=48, num_kvcache_blocks=5), dict(budget=48, cache_slack=17)):
+        if not kw["budget"]:
+            kw["cache_format"] = "model"
+        s, _ = budgeted(tmp_path, **kw)
+        with pytest.raises(ValueError, match="never be scheduled"):
+            s.add_sequence(Sequence([1] * 700, SamplingParams()))
+    s, _ = budgeted(tmp_path, 48, chunked_prefill=False, max_num_batched_tokens=1024)  # the whole prompt at once needs all its pages
+    with pytest.raises(ValueError, match="never be scheduled"):
+        s.add_sequence(Sequence([1] * 700, SamplingParams()))

@@ -39,6 +39,7 @@ class Scheduler:
         self.max_model_len = config.max_model_len
         self.max_num_seqs = config.max_num_seqs
         self.max_num_batched_tokens = config.max_num_batched_tokens
+        self.row_limit = config.cache_budget + config.cache_slack if config.cache_budget else 0  # rows a request keeps between steps; 0: all
         self.eos = config.eos
         self.cache_manager = cache_manager
         self.waiting: deque[Sequence] = deque()
@@ -61,12 +62,16 @@ class Scheduler:
         # The most pages the request holds at once: all of them in a group that keeps every key;
         # in a window group all of them too when the prompt comes in one portion (pages are given
         # back between steps only), else the window plus the largest portion (a chunk group
-        # likewise: at most one block of positions before the portion's first token is held).
+        # likewise: at most one block of positions before the portion's first token is held).  With a
+        # budget of rows a request that comes in portions is cut after every one of them: between
+        # steps it holds the budget and its slack at most.
         for g, pool in enumerate(cm.pools):
             spec = cm.groups[g]
             tokens = len(seq) + 1
             if spec.kind in ("window", "chunk") and self.enable_chunked:
                 tokens = min(tokens, spec.window + self.max_num_batched_tokens + cm.page_size)
+            if self.row_limit and self.enable_chunked:
+                tokens = min(tokens, self.row_limit + self.max_num_batched_tokens)
             need = -(-tokens // cm.page_size)
             if need > pool.num_pages:
                 raise ValueError(

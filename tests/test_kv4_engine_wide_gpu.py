@@ -87,3 +87,43 @@ def test_a_prompt_larger_than_the_pool_through_the_entry_point(tmp_path, monkeyp
         dropped[request] = dropped.get(request, 0) + rows - 48
     assert len(dropped) == 3 and all(gone >= n + 59 - 64 for gone, n in zip(sorted(dropped.values()), (20, 333, 700)))
     assert engine.model_runner.cache_manager.pages_in_use() == 0
+
+
+def test_a_budget_with_portions_on_tensor_memory(tmp_path, monkeypatch):
+    """What a step's queries give to the rows adds up to one a query and head; a cut keeps the rows with the largest sums; and with other
+    contents of the workspaces every bit is the same.  (The weights' own bound, as in check_attention: 4 * 2^-18 (reach + 1), with rows
+    of norm 11.3 a reach below 15: 2^-12.)"""
+    from tests.plain import kv4_plain
+    from tokensprint_b200 import ops
+
+    folder, _ = make_folder(tmp_path, SLIDING | {"use_sliding_window": False, "layer_types": ["full_attention"] * 3}, 11)
+    ids = random_tokens(WIDE, 900, 12)
+    budget, recent, first, slack = 256, 32, 4, 64
+    runner = make_runner(folder, "bfloat16", num_pages=128, max_model_len=1024, cache_budget=budget, cache_recent=recent, cache_first=first, cache_slack=slack)
+    evict, seen = ops.kv4_evict, []
+
+    def checked(pool, sums, table, lens, new, num_seqs, longest, *rest):
+        rows = int(lens[0])
+        pages = table[0].long().clamp(min=0)
+        flat = sums[pages].transpose(0, 1).flatten(1)[:, :rows].cpu()
+        evict(pool, sums, table, lens, new, num_seqs, longest, *rest)
+        after = sums[pages].transpose(0, 1).flatten(1)[:, :rows].cpu()
+        for w, x in zip(flat, after):
+            kept = kv4_plain.kept_rows(w.tolist(), budget, recent, first)
+            assert torch.equal(x[:budget], w[kept]) and bool((x[budget:] == 0).all())
+        seen.append(rows)
+
+    monkeypatch.setattr(ops, "kv4_evict", checked)
+    cuts = [300, 250, 1, 63, 1, 100, 185]
+    got, rc = run_portions(runner, ids, cuts[:1])
+    for sums in runner.cache_tensors.sums:  # nothing is cut yet
+        total = sums[torch.tensor(rc.tables[0], device=sums.device)].double().sum((0, 2))
+        assert ((total - 300 * 4).abs() <= 2.0**-12 * 300 * 4).all() and seen == []
+    runner.free(rc)
+    got, rc = run_portions(runner, ids, cuts, "b")
+    assert seen == [550] * 3 + [321] * 3 + [356] * 3 + [441] * 3 and rc.num_tokens == 256
+    runner.free(rc)
+    with monkeypatch.context() as m:
+        spoil_workspaces(m)
+        again, rc = run_portions(runner, ids, cuts, "c")
+    assert torch.isfinite(got).all() and torch.equal(got, again)

@@ -156,8 +156,8 @@ __global__ void __launch_bounds__(128) load_kernel(const uint8_t* pool, const in
 // 2,048 rows of 8 heads: 6 us (2.4 MB in, 8.4 MB out), most of it the start and two trips to memory; the attention that follows reads them from the L2.
 constexpr int kExpandRows = 64, kExpandPage = 128, kExpandDim = 128;
 __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* pool, const int* table, int table_stride, const int* cu, const int* context, uint4* k,
-                                                     uint4* v, int* out_table, int* out_lens, int nkv, int page_blocks, int num_pages, int blocks,
-                                                     int window) {
+                                                     uint4* v, int* out_table, int* out_lens, uint4* out, float* lse, const float* sinks, int group, int nkv,
+                                                     int page_blocks, int num_pages, int blocks, int window) {
   ts_pdl_prologue();
   constexpr int kWords = kExpandDim / 8, kUnits = kExpandRows * kWords * 2 / 256;
   const int b = blockIdx.z, head = blockIdx.y, first = blockIdx.x * kExpandRows;
@@ -167,6 +167,14 @@ __global__ void __launch_bounds__(256) expand_kernel(const uint8_t* pool, const 
     if (first == 0) out_lens[b] = n;
   }
   const int queries = cu[b + 1] - cu[b], oldest = window > 0 ? n - queries - window + 1 : 0;  // the first key that some query sees
+  // Tokens ahead of the first row see nothing: zeros, and the logarithm of nothing or of the sink.  The attention leaves out tiles that have no others.
+  const int unseen = (queries - max(n, 0)) * group;
+  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < unseen * kWords; i += gridDim.x * blockDim.x) {
+    const int row = i / kWords, query_head = head * group + row % group;
+    const size_t at = (size_t)(cu[b] + row / group) * (nkv * group) + query_head;
+    out[at * kWords + i % kWords] = make_uint4(0u, 0u, 0u, 0u);
+    if (lse != nullptr && i % kWords == 0) lse[at] = sinks != nullptr ? sinks[query_head] : -INFINITY;
+  }
   // (The attention walks whole pages, from the first that holds a visible key on: what it reads ahead of that key weighs nothing, but has to be
   // numbers.  So only whole pages are left out.)
   const int page_end = first / kExpandPage * kExpandPage + kExpandPage;
@@ -482,13 +490,15 @@ TS_EXPORT int ts_kv4_load(const Kv4LoadArgs* args) {
                    log_groups, page_blocks, num_slots, width);
 }
 
-// k, v: [num_seqs * blocks][128][nkv][128] bfloat16, out_table [num_seqs][blocks]; blocks * 128 rows hold the longest request.
+// k, v: [num_seqs * blocks][128][nkv][128] bfloat16, out_table [num_seqs][blocks]; blocks * 128 rows hold the longest request.  out [tokens][nkv * group][128],
+// lse and sinks (or null) of as many heads: the attention's, of which the tokens that see nothing are written here.
 TS_EXPORT int ts_kv4_expand(const void* pool, const int* table, int table_stride, const int* cu, const int* context, void* k, void* v, int* out_table,
-                            int* out_lens, int num_seqs, int nkv, int page_blocks, int num_pages, int blocks, int window, void* stream) {
+                            int* out_lens, void* out, float* lse, const float* sinks, int num_seqs, int group, int nkv, int page_blocks, int num_pages,
+                            int blocks, int window, void* stream) {
   if (num_seqs < 1 || blocks < 1) return 0;
   if (num_seqs > 65535 || nkv > 65535) return TS_ERR_UNSUPPORTED_SIZE;
   return ts_launch(expand_kernel, dim3(blocks * (kExpandPage / kExpandRows), nkv, num_seqs), dim3(256), 0, (cudaStream_t)stream, (const uint8_t*)pool, table,
-                   table_stride, cu, context, (uint4*)k, (uint4*)v, out_table, out_lens, nkv, page_blocks, num_pages, blocks, window);
+                   table_stride, cu, context, (uint4*)k, (uint4*)v, out_table, out_lens, (uint4*)out, lse, sinks, group, nkv, page_blocks, num_pages, blocks, window);
 }
 
 // order: num_seqs * nkv * budget ints of workspace, none where budget >= max_context; context[b] <= max_context (a longer one counts as that).

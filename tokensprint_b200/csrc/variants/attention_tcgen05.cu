@@ -794,23 +794,7 @@ __global__ void __launch_bounds__(608, 1) attention_tcgen05_pair_kernel(const __
 #if TS_ATT_LSE
   const int kb0 = lo / PBN + run * p.run_blocks;
   const int nblocks = p.run_blocks > 0 ? min(hi / PBN - kb0 + 1, p.run_blocks) : hi / PBN - kb0 + 1;
-  if (run > 0 && nblocks <= 0) return;
-  if (hi < 0) {  // (a request with more tokens than rows) no row of the pair sees a key: zeros, before anything is copied or waited for
-    const int rows = min(ntiles * RT, rows_total - r0);
-    for (int i = tid; i < rows * (D / 8); i += blockDim.x) {
-      const int r = r0 + i / (D / 8), piece = i % (D / 8);
-      const size_t at = (size_t)(q_begin + r / G) * p.nq + hk * G + r % G;
-      const float lse = p.has_sink ? row_lse(p, row_sink_raw(p, hk, G, r), 1.f) : -INFINITY;
-      if (p.run_blocks > 0) {  // (run 0's, the only one that the rows have)
-        reinterpret_cast<float4*>(p.run_out + at * D)[2 * piece] = reinterpret_cast<float4*>(p.run_out + at * D)[2 * piece + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (piece == 0) p.run_lse[at] = lse;
-      } else {
-        reinterpret_cast<uint4*>(p.out + at * D)[piece] = make_uint4(0u, 0u, 0u, 0u);
-        if (piece == 0 && p.lse != nullptr) p.lse[at] = lse;
-      }
-    }
-    return;
-  }
+  if (nblocks <= 0 || hi < 0) return;  // (hi < 0: a request with more tokens than rows; kv4_expand has written these)
 #else
   const int kb0 = lo / PBN;
   const int nblocks = hi / PBN - kb0 + 1;
@@ -1778,6 +1762,7 @@ __global__ void __launch_bounds__(256) join_runs_kernel(const Params p) {
   const int start_pos = ctx - q_len, rows_total = q_len * G, RT = (BM / G) * G;
   const int r0 = (token * G + head % G) / (2 * RT) * (2 * RT);
   const int lo = first_visible_key(p, start_pos + r0 / G), hi = start_pos + (min(r0 + 2 * RT, rows_total) - 1) / G;
+  if (hi < 0) return;  // no row of the pair sees a key, and no CTA has left anything here (kv4_expand has written the row)
   const int runs = min(max(1, (hi / PBN - lo / PBN + p.run_blocks) / p.run_blocks), p.runs);
   const size_t at = (size_t)(q_begin + token) * p.nq + head, step = (size_t)p.tokens * p.nq;
   float top = -INFINITY, sum = 0.f, o[16];

@@ -2519,7 +2519,7 @@ _KV4_LOAD_ARGS = _struct.Struct("@PPPPP6i").pack
 _KV4_EVICT_ARGS = _struct.Struct("@PPPPPPP10i").pack
 _KV4_ATTENTION_ARGS = _struct.Struct("@11P11if").pack
 _KV4_WEIGHTS_ARGS = _struct.Struct("@8P11if").pack
-_SIGNATURES["ts_kv4_expand"] = [_c_void_p, _c_void_p, _c_int] + [_c_void_p] * 6 + [_c_int] * 6 + [_c_void_p]
+_SIGNATURES["ts_kv4_expand"] = [_c_void_p, _c_void_p, _c_int] + [_c_void_p] * 9 + [_c_int] * 7 + [_c_void_p]
 _attention_kv4: dict[int, tuple] = {}
 # Portions of prompts with more rows (tokens x query heads of a key head) than this are attended to on tcgen05 tensor cores, over rows unpacked for
 # the step; up to it by the kernel of decoded tokens, which unpacks every code once for 16 rows (us, 16 requests of 8,000 rows with 48 / 64 / 96 rows:
@@ -2795,7 +2795,8 @@ def _attention_kv4_expanded(q, pool, out, cu_seqlens_q, context_lens, block_tabl
         cu, lens = cu_seqlens_q[lo : lo + n + 1], context_lens[lo : lo + n]
         _check("kv4_expand", _fn("ts_kv4_expand")(
             pool.data_ptr(), block_table[lo:].data_ptr(), block_table.shape[1], cu.data_ptr(), lens.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(),
-            table.data_ptr(), kept_lens.data_ptr(), n, nkv, pool_blocks, pages, blocks, int(window), _stream()))
+            table.data_ptr(), kept_lens.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(head_sinks), n, G, nkv, pool_blocks, pages, blocks, int(window),
+            _stream()))
         _check("attention_kv4", run(
             q.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), out.data_ptr(), cu.data_ptr(), kept_lens.data_ptr(), table.data_ptr(), blocks, page,
             group * blocks * page, T, n, max_seqlen_q, nq, nkv, float(scale), int(window), 0, 0, 0.0, 0.0, _ptr(head_sinks), 0, error.data_ptr(),
@@ -2871,18 +2872,17 @@ def kv4_evict(pool: torch.Tensor, sums: torch.Tensor, block_table: torch.Tensor,
         raise KernelError(f"kv4_evict: a budget of {budget} rows cannot hold the first {first} and the last {recent}")
     if max_context < 0 or num_seqs < 0:
         raise KernelError("kv4_evict: negative sizes")
+    table_at, lens_at, new_at, width, n = block_table.data_ptr(), context_lens.data_ptr(), new_lens.data_ptr(), block_table.shape[1], 4 * num_seqs
     # (the first CTA of a request writes its new length while others may not have read the old one)
-    at = new_lens.data_ptr()
-    for label, t, n in (("context_lens", context_lens, num_seqs), ("block_table", block_table, num_seqs * block_table.shape[1])):
-        if at < t.data_ptr() + 4 * n and t.data_ptr() < at + 4 * num_seqs:
-            raise KernelError(f"kv4_evict: new_lens must not overlap {label}, which is read while it is written")
+    if new_at < lens_at + n and lens_at < new_at + n or new_at < table_at + n * width and table_at < new_at + n:
+        raise KernelError("kv4_evict: new_lens must not overlap context_lens or block_table, which are read while it is written")
     places = budget
     if budget >= max_context:  # no request has more rows: nothing to rank, and nowhere to move
         budget, recent, first, places = max(1, max_context), 0, 0, 0
     order = torch.empty(num_seqs * nkv * places, device=pool.device, dtype=torch.int32)  # where every kept row comes from
     _check("kv4_evict", _fn("ts_kv4_evict")(_KV4_EVICT_ARGS(
-        pool.data_ptr(), sums.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(), new_lens.data_ptr(), order.data_ptr(), _stream(),
-        block_table.shape[1], num_seqs, nkv, d, blocks, pages, max_context, budget, recent, first)))
+        pool.data_ptr(), sums.data_ptr(), table_at, lens_at, new_at, order.data_ptr(), _stream(), width, num_seqs, nkv, d, blocks, pages, max_context,
+        budget, recent, first)))
 
 
 # ---------------------------------------------------------------------------

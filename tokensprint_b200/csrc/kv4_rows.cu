@@ -46,8 +46,8 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[16], uint2& w) {
   uint32_t half[2] = {0u, 0u};
   const float t = amax / 7.f;
   if (t >= 6.103515625e-05f && t < 8192.f) {
-    // A normal scale: |x / s| stays below 7.5.  The quotient is rounded as a division would: with inv = 1/s rounded, q = x inv, then q + (x - q s) inv,
-    // whose remainder is exact.  Adding 1.5 * 2^23 + 8 rounds it to a whole number, ties to even, and leaves the code in the low bits.
+    // A normal scale: |x / s| stays below 7.5.  The quotient is rounded as a division would, by Markstein's correction: with inv = 1/s rounded, q = x inv, then
+    // q + (x - q s) inv, whose remainder is exact.  Adding 1.5 * 2^23 + 8 rounds it to a whole number, ties to even, and leaves the code in the low bits.
     const uint32_t byte = scale_byte(amax);
     const float s = scale_of(byte), inv = 1.f / s;
 #pragma unroll
@@ -441,8 +441,8 @@ int launch_evict(uint8_t* pool, float* sums, const int* table, int table_stride,
 
 }  // namespace
 
-// Threads per token of the row kernels: with few tokens all groups of a token at once, with many a warp per token.  us of 128 / 32 threads, rows of 8
-// heads of 128: store of 8 tokens 7 / 10, of 1,024 8 / 10, of 4,096 14 / 12; load of 8 6 / 8, of 1,024 8 / 8, of 4,096 14 / 10.
+// Threads per token of the row kernels: with few tokens all groups of a token at once, with many a warp per token.  us a call of 128 / 32 threads, the host's
+// part among them, rows of 8 heads of 128: store of 8 tokens 7 / 10, of 1,024 8 / 10, of 4,096 14 / 12; load of 8 6 / 8, of 1,024 8 / 8, of 4,096 14 / 10.
 static int threads_per_token(int tokens) { return tokens < 1024 ? 128 : 32; }
 
 // k, v: rows [tokens] of nkv * d entries, `stride` entries apart; slots [tokens], -1: not stored; sums: null or the pool's weights.

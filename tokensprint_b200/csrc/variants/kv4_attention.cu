@@ -15,7 +15,7 @@
 // run them (integer 54 % busy, multiply-add 37 %, tensor 20 %) share the issue slots: 3.5 TB/s of cache where the same kernel without the arithmetic
 // reads 5.8.  tcgen05 does not fit: its smallest tile is 128 keys by 8 rows whose operands must lie unpacked in shared memory or tensor memory, so
 // every value would be written and read once more, and unpacking is what the time goes into.  us with 32 query and 8 key heads of 128:
-// 4 requests of up to 60,000 rows 78 (276 MB), 32 of up to 4,096 36 (96 MB), 1 of 517 (16 query heads) 11.4.
+// 4 requests of up to 60,000 rows 78 (276 MB), 32 of up to 4,096 36 (96 MB), 1 of 517 (16 query heads) 10.4.
 #include "kv4.cuh"
 
 #ifndef TS_HEAD_DIM

@@ -2714,8 +2714,13 @@ def attention_kv4(
     block_table [B,max_blocks] i32.  The tokens of a sequence are consecutive and are its cache's last rows: query i of
     n sees the rows up to context_lens[b] - n + i.  (A row's number in the cache need not be its position: after kv4_evict it is
     not.)  `max_seqlen_q` and `max_context` bound the lengths.  window > 0: a query sees the last `window` rows only; head_sinks [nq] f32:
-    a score that joins a head's softmax without a value; lse [T,nq] f32: receives the logarithm of every softmax's denominator
-    (-inf for a query that sees nothing; its output is zero)."""
+    a score that joins a head's softmax without a value (-inf: none); lse [T,nq] f32: receives the logarithm of every softmax's
+    denominator.  A query that sees nothing (a request may bring more tokens than it has rows) gives zero, its logarithm is the sink's
+    score or -inf.
+
+    Scores, maxima and sums are float32.  For their product with the values, weights have 16 bits in bfloat16 calls of few rows
+    (max_seqlen_q times the query heads of a key head up to ATTENTION_KV4_DIRECT_ROWS, or short prompts) and in all of heads of 64
+    and 256, 8 bits in the others, which run on tcgen05, and 24 in float32 calls."""
     flush_gemm_chain()
     nq, nkv, d = num_heads, num_kv_heads, head_dim
     pages, blocks, code, T, width = _check_attention_kv4("attention_kv4", q, pool, cu_seqlens_q, context_lens, block_table, num_seqs, max_seqlen_q,

@@ -2891,6 +2891,276 @@ def kv4_evict(pool: torch.Tensor, sums: torch.Tensor, block_table: torch.Tensor,
 
 
 # ---------------------------------------------------------------------------
+# drafted tokens: attention of a tree of them, their verification, the accepted rows of the caches, drafts
+# from a request's own tokens
+
+TREE_MAX_NODES = 256
+TREE_MAX_HEAD_DIM = 256
+VERIFY_MAX_VOCAB = 1 << 20
+LOOKUP_MAX_BRANCHES, LOOKUP_MAX_DEPTH, LOOKUP_MAX_SUFFIX = 16, 64, 16
+_SIGNATURES["ts_verify_drafts"] = [_c_void_p, _c_int, _c_ll, _c_void_p, _c_ll] + [_c_void_p] * 9 + [_c_int] * 3 + [_c_void_p]
+_SIGNATURES["ts_keep_drafted_rows"] = [_c_void_p, _c_int, _c_int, _c_int, _c_ll, _c_int, _c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] * 2 + [_c_void_p]
+_SIGNATURES["ts_lookup_drafts"] = [_c_void_p, _c_ll] + [_c_void_p] * 4 + [_c_int] * 6 + [_c_void_p]
+_attention_trees: dict[int, tuple] = {}
+
+
+def _on_current_device(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise KernelError(f"{name}: a tensor lies on {t.device}, the current device is cuda:{here}")
+
+
+def attention_tree_supported(head_dim: int) -> bool:
+    return head_dim % 8 == 0 and 8 <= head_dim <= TREE_MAX_HEAD_DIM
+
+
+def _attention_tree_fns(head_dim: int) -> tuple:
+    fns = _attention_trees.get(head_dim)
+    if fns is None:
+        if not attention_tree_supported(head_dim):
+            raise KernelError(f"attention_tree: head_dim must be a multiple of 8 up to {TREE_MAX_HEAD_DIM}, got {head_dim}")
+        lib = _build.load_variant("attention_tree", {"TS_HEAD_DIM": head_dim})
+        run = lib.ts_attention_tree
+        run.argtypes = ([_c_void_p] * 4 + [_c_int, _c_void_p, _c_int] + [_c_void_p] * 3 + [_c_int] * 3 + [_c_void_p] * 2 + [_c_int] * 5
+                        + [_c_float, _c_int, _c_float, _c_int, _c_void_p, _c_void_p])
+        run.restype = _c_int
+        splits = lib.ts_attention_tree_splits
+        splits.argtypes = [_c_int] * 5
+        splits.restype = _c_int
+        fns = _attention_trees[head_dim] = (run, splits)
+    return fns
+
+
+def attention_tree(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    out: torch.Tensor,
+    tree_mask: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    page_size: int,
+    num_seqs: int,
+    max_seqlen_q: int,
+    max_context: int,
+    num_heads: int,
+    num_kv_heads: int,
+    head_dim: int,
+    scale: float,
+    window: int = 0,
+    positions: Optional[torch.Tensor] = None,
+    head_sinks: Optional[torch.Tensor] = None,
+    softcap: float = 0.0,
+) -> None:
+    """Attention of trees of drafted tokens over the paged cache, bfloat16 or float32.
+
+    q/out [T,nq*d]; caches [pages,page,nkv,d]; cu_seqlens_q [B+1], context_lens [B] i32; block_table [B,max_blocks] i32 (-1: a page given
+    back).  The tokens of a request are its tree's nodes, at most 256, and its last rows in the cache.  A node sees the rows before the
+    step and, of the step's rows, node k's where bit k % 64 of word k // 64 of its row of tree_mask [T,words] i64 is set (its own bit among them).
+    window > 0: and of these only those at positions greater than its own less the window; `positions` [T] i32 are then the nodes' (a row before
+    the step stands at its own number).  head_sinks [nq] f32: a score per query head that joins its softmax without a value;
+    softcap > 0: the scaled score passes through softcap * tanh(s / softcap).  max_seqlen_q and max_context: the most nodes and rows of any request.
+    A node that sees nothing gets zeros; rows of `out` behind the last request stay as they are.  Rows of the cache that a request holds are numbers
+    (a value of infinity counts for the nodes that do not see its row, too).
+    """
+    flush_gemm_chain()
+    run, plan = _attention_tree_fns(head_dim)
+    for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("out", out)):
+        _cuda_contig(f"attention_tree: {name}", t, q.dtype)
+    code = _act_code("attention_tree: q", q)
+    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("context_lens", context_lens), ("block_table", block_table)):
+        _cuda_contig(f"attention_tree: {name}", t, torch.int32)
+    _cuda_contig("attention_tree: tree_mask", tree_mask, torch.int64)
+    _on_current_device("attention_tree", q, k_cache, v_cache, out, tree_mask, cu_seqlens_q, context_lens, block_table, positions, head_sinks)
+    T, nq, nkv, d = q.shape[0], num_heads, num_kv_heads, head_dim
+    if nkv < 1 or nq < 1 or nq % nkv:
+        raise KernelError(f"attention_tree: {nq} query heads are no multiple of {nkv} key/value heads")
+    if q.numel() != T * nq * d or out.numel() != T * nq * d:
+        raise KernelError(f"attention_tree: q {tuple(q.shape)} and out {tuple(out.shape)} do not match [T, {nq} heads of {d}]")
+    if page_size < 1 or tuple(k_cache.shape[-3:]) != (page_size, nkv, d) or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise KernelError(f"attention_tree: caches must be [pages,{page_size},{nkv},{d}], got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    if not 1 <= max_seqlen_q <= TREE_MAX_NODES:
+        raise KernelError(f"attention_tree: a request brings 1 to {TREE_MAX_NODES} nodes, got {max_seqlen_q}")
+    if tree_mask.dim() != 2 or tree_mask.shape[0] < T or 64 * tree_mask.shape[1] < max_seqlen_q:
+        raise KernelError(f"attention_tree: tree_mask must be [T, a word per 64 nodes], got {tuple(tree_mask.shape)} for {T} tokens and {max_seqlen_q} nodes")
+    if block_table.dim() != 2 or block_table.shape[0] < num_seqs or block_table.shape[1] < 1:
+        raise KernelError("attention_tree: block_table must be [B,max_blocks]")
+    if cu_seqlens_q.numel() < num_seqs + 1 or context_lens.numel() < num_seqs:
+        raise KernelError("attention_tree: cu_seqlens_q/context_lens are shorter than the batch")
+    if num_seqs > 65535 or max_context < 0 or window < 0 or not softcap >= 0.0:
+        raise KernelError("attention_tree: at most 65535 requests, and max_context, window and softcap must not be negative")
+    if window > 0:
+        if positions is None:
+            raise KernelError("attention_tree: a window needs the nodes' positions")
+        _cuda_contig("attention_tree: positions", positions, torch.int32)
+        if positions.numel() < T:
+            raise KernelError("attention_tree: positions is shorter than the batch")
+    if head_sinks is not None:
+        _cuda_contig("attention_tree: head_sinks", head_sinks, torch.float32)
+        if head_sinks.numel() != nq:
+            raise KernelError(f"attention_tree: head_sinks must have one entry per query head ({nq}), got {head_sinks.numel()}")
+    if num_seqs < 1 or T < 1:
+        return
+    splits = plan(num_seqs, max_seqlen_q, nq, nkv, min(max_context, window + max_seqlen_q + 64) if window > 0 else max_context)
+    part = torch.empty(T * nq * splits * (d + 2), device=q.device, dtype=torch.float32) if splits > 1 else None
+    _check("attention_tree", run(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), code, tree_mask.data_ptr(), tree_mask.shape[1], cu_seqlens_q.data_ptr(),
+        context_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, k_cache.shape[0], _ptr(positions) if window > 0 else None,
+        _ptr(head_sinks), T, num_seqs, max_seqlen_q, nq, nkv, float(scale), int(window), float(softcap), splits, _ptr(part), _stream()))
+    if splits > 1:
+        global launch_count
+        launch_count += 1
+
+
+def verify_drafts(
+    logits: torch.Tensor,
+    tokens: torch.Tensor,
+    parents: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    temperatures: torch.Tensor,
+    uniforms: torch.Tensor,
+    keys: torch.Tensor,
+    path: torch.Tensor,
+    next_tokens: torch.Tensor,
+    counts: torch.Tensor,
+    num_seqs: int,
+    max_nodes: int,
+    draft_probs: Optional[torch.Tensor] = None,
+) -> None:
+    """Which drafted tokens the target's probabilities accept, and the token behind them, for every request.
+
+    logits [T,V] float32 or bfloat16 (rows may lie further apart): those behind every node; tokens, parents [T] i32: the nodes' (parents by their
+    number inside the request, smaller than the node's; the first node of a request is its root, certain already); cu_seqlens [B+1] i32;
+    temperatures [B] f32 (0: greedy); uniforms [T] f32 in [0, 1): the number that decides on a node; keys [B] i64: the key of the
+    draw behind the last accepted node (as `sample` takes them; the draw is not `sample`'s: its logarithms are the accurate ones).
+    From the root on, the children of the node where the walk stands are asked in the order of their numbers.  draft_probs [T,V] f32: row t holds the
+    probabilities from which the children of node t were drawn, independently of one another; a child with token x is accepted with
+    probability r(x) / q(x), r being the target's probabilities and, after a refusal, max(r - q, 0) over its sum.  Without draft_probs the drafts are
+    guesses that nobody drew: accepted with probability r(x), and a refused token leaves r.  If no child is accepted, the next token is drawn from r.
+    Into path [B,columns] i32 go the accepted nodes' numbers, 0 for the root first, into next_tokens [B,columns] i32 their tokens
+    and the drawn one, -1 behind both, into counts [B] i32 how many drafts were accepted; columns >= max_nodes, the most nodes of any request (at most 256).
+    NaN and -inf are logits of no probability; tokens outside the vocabulary are never accepted.
+    """
+    flush_gemm_chain()
+    if not logits.is_cuda or logits.dim() != 2 or logits.stride(1) != 1:
+        raise KernelError(f"verify_drafts: logits must be a CUDA matrix [T,V] with neighbouring entries in a row, got {tuple(logits.shape)}, strides {logits.stride()}")
+    code = _act_code("verify_drafts: logits", logits)
+    T, V = logits.shape
+    if not 1 <= V <= VERIFY_MAX_VOCAB:
+        raise KernelError(f"verify_drafts: a vocabulary of 1 to {VERIFY_MAX_VOCAB} entries, got {V}")
+    if T > 1 and logits.stride(0) < V:
+        raise KernelError("verify_drafts: rows of logits overlap")
+    for name, t, dtype, n in (("tokens", tokens, torch.int32, T), ("parents", parents, torch.int32, T), ("uniforms", uniforms, torch.float32, T),
+                              ("cu_seqlens", cu_seqlens, torch.int32, num_seqs + 1), ("temperatures", temperatures, torch.float32, num_seqs),
+                              ("keys", keys, torch.int64, num_seqs), ("counts", counts, torch.int32, num_seqs)):
+        _cuda_contig(f"verify_drafts: {name}", t, dtype)
+        if t.numel() < n:
+            raise KernelError(f"verify_drafts: {name} needs {n} entries, got {t.numel()}")
+    if not 1 <= max_nodes <= TREE_MAX_NODES:
+        raise KernelError(f"verify_drafts: a request brings 1 to {TREE_MAX_NODES} nodes, got {max_nodes}")
+    for name, t in (("path", path), ("next_tokens", next_tokens)):
+        _cuda_contig(f"verify_drafts: {name}", t, torch.int32)
+        if t.dim() != 2 or t.shape[0] < num_seqs or t.shape[1] < max_nodes or t.shape != path.shape:
+            raise KernelError(f"verify_drafts: path and next_tokens must be [B, {max_nodes} or more], got {tuple(path.shape)} and {tuple(next_tokens.shape)}")
+    if draft_probs is not None:
+        if not draft_probs.is_cuda or draft_probs.dtype != torch.float32 or draft_probs.shape != logits.shape or draft_probs.stride(1) != 1 or (
+                T > 1 and draft_probs.stride(0) < V):
+            raise KernelError(f"verify_drafts: draft_probs must be float32 of the logits' shape {tuple(logits.shape)}")
+    _on_current_device("verify_drafts", logits, tokens, parents, cu_seqlens, temperatures, uniforms, keys, path, next_tokens, counts, draft_probs)
+    if num_seqs < 1 or T < 1:
+        return
+    _check("verify_drafts", _fn("ts_verify_drafts")(
+        logits.data_ptr(), code, max(logits.stride(0), V), _ptr(draft_probs), 0 if draft_probs is None else max(draft_probs.stride(0), V), tokens.data_ptr(),
+        parents.data_ptr(), cu_seqlens.data_ptr(), temperatures.data_ptr(), uniforms.data_ptr(), keys.data_ptr(), path.data_ptr(), next_tokens.data_ptr(),
+        counts.data_ptr(), V, num_seqs, path.shape[1], _stream()))
+
+
+class RowPools:
+    """The paged pools [pages,page,...] of a model's layers, keys and values, as `keep_drafted_rows` takes them: all of one shape and
+    type, contiguous, on one device.  Made once for the life of the cache (it keeps the pools, and their addresses on the device)."""
+
+    def __init__(self, pools: "list[torch.Tensor]") -> None:
+        if not pools:
+            raise KernelError("RowPools: at least one pool")
+        first = pools[0]
+        for t in pools:
+            _cuda_contig("RowPools: a pool", t, first.dtype)
+            if t.dim() < 3 or t.shape != first.shape or t.device != first.device:
+                raise KernelError(f"RowPools: pools [pages,page,...] of one shape and device, got {tuple(first.shape)} and {tuple(t.shape)}")
+        self.pools = list(pools)
+        self.num_pages, self.page_size = int(first.shape[0]), int(first.shape[1])
+        self.row_bytes = first[0, 0].numel() * first.element_size() if first.numel() else 0
+        if self.row_bytes == 0 or self.row_bytes % 2:
+            raise KernelError("RowPools: rows of an even number of bytes")
+        every = [self.row_bytes] + [t.data_ptr() for t in pools]
+        self.align = next(a for a in (16, 4, 2) if all(x % a == 0 for x in every))
+        self.addresses = torch.tensor([t.data_ptr() for t in pools], dtype=torch.int64).to(first.device)
+
+
+def keep_drafted_rows(pools: RowPools, path: torch.Tensor, counts: torch.Tensor, cu_seqlens: torch.Tensor, context_lens: torch.Tensor,
+                      block_table: torch.Tensor, page_size: int, num_seqs: int) -> None:
+    """Moves the accepted nodes' rows of every pool to the front of the step's rows.
+
+    A request's last t rows (t from cu_seqlens [B+1] i32) of its context_lens[b] are its nodes'; row path[b, k] of them goes to place k, for k = 1 ..
+    counts[b]; path [B,columns] and counts [B] i32 as `verify_drafts` leaves them (numbers that grow).  The first of the t rows stays, and so do rows
+    behind the last accepted one (they hold what they held, or what has not been moved from them)."""
+    flush_gemm_chain()
+    for name, t, n in (("counts", counts, num_seqs), ("cu_seqlens", cu_seqlens, num_seqs + 1), ("context_lens", context_lens, num_seqs)):
+        _cuda_contig(f"keep_drafted_rows: {name}", t, torch.int32)
+        if t.numel() < n:
+            raise KernelError(f"keep_drafted_rows: {name} needs {n} entries, got {t.numel()}")
+    for name, t in (("path", path), ("block_table", block_table)):
+        _cuda_contig(f"keep_drafted_rows: {name}", t, torch.int32)
+        if t.dim() != 2 or t.shape[0] < num_seqs or t.shape[1] < 1:
+            raise KernelError(f"keep_drafted_rows: {name} must be a matrix with a row per request, got {tuple(t.shape)}")
+    if page_size != pools.page_size:
+        raise KernelError(f"keep_drafted_rows: pages of {page_size} rows, but the pools' have {pools.page_size}")
+    if num_seqs > 65535:
+        raise KernelError(f"keep_drafted_rows: at most 65535 requests, got {num_seqs}")
+    _on_current_device("keep_drafted_rows", pools.addresses, path, counts, cu_seqlens, context_lens, block_table)
+    if num_seqs < 1:
+        return
+    _check("keep_drafted_rows", _fn("ts_keep_drafted_rows")(
+        pools.addresses.data_ptr(), len(pools.pools), pools.row_bytes, pools.align, pools.num_pages, page_size, path.data_ptr(), path.shape[1], counts.data_ptr(),
+        cu_seqlens.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], num_seqs, _stream()))
+
+
+def lookup_drafts(history: torch.Tensor, lengths: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, counts: torch.Tensor, num_seqs: int,
+                  depth: int, branches: int, max_suffix: int = 4, min_suffix: int = 1) -> None:
+    """Drafts from what a request's tokens have said before.
+
+    history [B,L] i32 (rows may lie further apart), lengths [B] i32: a request's tokens.  A place matches with the number of tokens up to it, at most max_suffix,
+    that equal the request's last ones; those with min_suffix or more give chains of the up to `depth` tokens behind them: the longest match first, of
+    equals the latest, up to `branches` chains whose first tokens differ.  Into tokens and parents [B, 1 + depth * branches] i32 goes the tree: the request's
+    last token as the root (parent -1), then chain after chain, -1 behind; into counts [B] i32 its nodes (0 for a request without tokens)."""
+    flush_gemm_chain()
+    if not history.is_cuda or history.dtype != torch.int32 or history.dim() != 2 or history.stride(1) != 1 or history.shape[0] < num_seqs:
+        raise KernelError(f"lookup_drafts: history must be an int32 CUDA matrix with a row per request, got {tuple(history.shape)}")
+    if history.shape[1] < 1 or history.shape[0] > 1 and history.stride(0) < history.shape[1]:
+        raise KernelError("lookup_drafts: rows of history are empty or overlap")
+    if not (1 <= depth <= LOOKUP_MAX_DEPTH and 1 <= branches <= LOOKUP_MAX_BRANCHES and 1 <= min_suffix <= max_suffix <= LOOKUP_MAX_SUFFIX):
+        raise KernelError(f"lookup_drafts: depth 1..{LOOKUP_MAX_DEPTH}, branches 1..{LOOKUP_MAX_BRANCHES} and 1 <= min_suffix <= max_suffix <= {LOOKUP_MAX_SUFFIX}, "
+                          f"got {depth}, {branches}, {min_suffix}, {max_suffix}")
+    width = 1 + depth * branches
+    for name, t in (("tokens", tokens), ("parents", parents)):
+        _cuda_contig(f"lookup_drafts: {name}", t, torch.int32)
+        if t.dim() != 2 or t.shape[0] < num_seqs or t.shape[1] != width:
+            raise KernelError(f"lookup_drafts: {name} must be [B,{width}], got {tuple(t.shape)}")
+    for name, t in (("lengths", lengths), ("counts", counts)):
+        _cuda_contig(f"lookup_drafts: {name}", t, torch.int32)
+        if t.numel() < num_seqs:
+            raise KernelError(f"lookup_drafts: {name} needs {num_seqs} entries, got {t.numel()}")
+    _on_current_device("lookup_drafts", history, lengths, tokens, parents, counts)
+    if num_seqs < 1:
+        return
+    _check("lookup_drafts", _fn("ts_lookup_drafts")(
+        history.data_ptr(), max(history.stride(0), history.shape[1]), lengths.data_ptr(), tokens.data_ptr(), parents.data_ptr(), counts.data_ptr(),
+        history.shape[1], num_seqs, depth, branches, max_suffix, min_suffix, _stream()))
+
+
+# ---------------------------------------------------------------------------
 # skinny GEMM on tcgen05 tensor cores (decode steps)
 
 GEMM_SKINNY_MAX_ROWS = 128

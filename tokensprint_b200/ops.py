@@ -2901,7 +2901,9 @@ LOOKUP_MAX_BRANCHES, LOOKUP_MAX_DEPTH, LOOKUP_MAX_SUFFIX = 16, 64, 16
 _SIGNATURES["ts_verify_drafts"] = [_c_void_p, _c_int, _c_ll, _c_void_p, _c_ll] + [_c_void_p] * 9 + [_c_int] * 3 + [_c_void_p]
 _SIGNATURES["ts_keep_drafted_rows"] = [_c_void_p, _c_int, _c_int, _c_int, _c_ll, _c_int, _c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] * 2 + [_c_void_p]
 _SIGNATURES["ts_lookup_drafts"] = [_c_void_p, _c_ll] + [_c_void_p] * 4 + [_c_int] * 6 + [_c_void_p]
+TREE_TCGEN05_HEAD_DIMS = (64, 128)
 _attention_trees: dict[int, tuple] = {}
+_attention_trees_tcgen05: dict[int, tuple] = {}
 
 
 def _on_current_device(name: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -2929,6 +2931,24 @@ def _attention_tree_fns(head_dim: int) -> tuple:
         splits.argtypes = [_c_int] * 5
         splits.restype = _c_int
         fns = _attention_trees[head_dim] = (run, splits)
+    return fns
+
+
+def _attention_tree_tcgen05_fns(head_dim: int) -> tuple:
+    fns = _attention_trees_tcgen05.get(head_dim)
+    if fns is None:
+        lib = _build.load_variant("attention_tree_tcgen05", {"TS_HEAD_DIM": head_dim})
+        run = lib.ts_attention_tree_tcgen05
+        run.argtypes = ([_c_void_p] * 5 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 2 + [_c_ll] + [_c_void_p] * 2 + [_c_int] * 5
+                        + [_c_float, _c_int, _c_float, _c_int, _c_int] + [_c_void_p] * 3)
+        run.restype = _c_int
+        takes = lib.ts_attention_tree_tcgen05_takes
+        takes.argtypes = [_c_int] * 6 + [_c_ll, _c_float]
+        takes.restype = _c_int
+        scratch = lib.ts_attention_tree_tcgen05_scratch
+        scratch.argtypes = [_c_int] * 6 + [_c_void_p] * 2
+        scratch.restype = _c_ll
+        fns = _attention_trees_tcgen05[head_dim] = (run, takes, scratch)
     return fns
 
 
@@ -3003,6 +3023,22 @@ def attention_tree(
             raise KernelError(f"attention_tree: head_sinks must have one entry per query head ({nq}), got {head_sinks.numel()}")
     if num_seqs < 1 or T < 1:
         return
+    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise KernelError("attention_tree: the caches must begin at multiples of 16 bytes")
+    global launch_count
+    if code == 1 and d in TREE_TCGEN05_HEAD_DIMS and (q.data_ptr() | out.data_ptr()) % 16 == 0:
+        run_tcgen05, takes, scratch = _attention_tree_tcgen05_fns(d)
+        if takes(num_seqs, max_seqlen_q, max_context, nq, nkv, page_size, k_cache.shape[0], float(scale)):
+            ctas, part_rows = _c_int(), _c_int()
+            words = scratch(num_seqs, max_seqlen_q, max_context, nq, nkv, _sm_count(q.device), ctypes.byref(ctas), ctypes.byref(part_rows))
+            part, error = torch.empty(words, device=q.device, dtype=torch.float32), _gemm_workspace(q.device)[1]
+            _check("attention_tree", run_tcgen05(
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), tree_mask.data_ptr(), tree_mask.shape[1], cu_seqlens_q.data_ptr(),
+                context_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, k_cache.shape[0], _ptr(positions) if window > 0 else None,
+                _ptr(head_sinks), T, num_seqs, max_seqlen_q, nq, nkv, float(scale), int(window), float(softcap), ctas.value, part_rows.value,
+                part.data_ptr(), error.data_ptr(), _stream()))
+            launch_count += 1
+            return
     splits = plan(num_seqs, max_seqlen_q, nq, nkv, min(max_context, window + max_seqlen_q + 64) if window > 0 else max_context)
     part = torch.empty(T * nq * splits * (d + 2), device=q.device, dtype=torch.float32) if splits > 1 else None
     _check("attention_tree", run(
@@ -3010,7 +3046,6 @@ def attention_tree(
         context_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, k_cache.shape[0], _ptr(positions) if window > 0 else None,
         _ptr(head_sinks), T, num_seqs, max_seqlen_q, nq, nkv, float(scale), int(window), float(softcap), splits, _ptr(part), _stream()))
     if splits > 1:
-        global launch_count
         launch_count += 1
 
 

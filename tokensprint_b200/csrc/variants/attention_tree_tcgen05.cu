@@ -34,7 +34,7 @@ constexpr int CH = 16;                           // columns of the result that p
 constexpr uint32_t MERGE = 8 * 32 * CH * 4;
 constexpr int MAX_SEQS = 1024;
 constexpr int MAX_NODES = 256;
-constexpr int THREADS = 320;                     // eight warps of softmax, one that copies, one that issues products
+constexpr int THREADS = 352;                     // eight warps of softmax, one that copies Q and K, one that issues products, one that copies V
 constexpr uint32_t SPIN_LIMIT = 1u << 22;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LAG = 8.f;
@@ -486,62 +486,64 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
   Piece piece;
   walk.begin(p, before_s, RT, from, to);
 
-  if (warp == 8) {
-    // ---------------- copies ----------------
+  if (warp == 8 || warp == 10) {
+    // ---------------- copies: Q and K, and V ----------------
+    const bool keys = warp == 8;
     const int box_rows = min(p.page, BN), copies = BN / box_rows;
-    const int c = lane / HALVES, half = lane % HALVES;
-    int kc = 0, vc = 0, qc = 0;
+    const int c = lane / HALVES, half = lane % HALVES;  // this lane's box of a block (at most 16 a half: pages of 8)
+    const int stages = keys ? NK : NV;
+    uint64_t* full = keys ? k_full : v_full;
+    uint64_t* empty = keys ? k_empty : v_empty;
+    const uint32_t to_smem = sm + (keys ? L::K : L::V) + half * ATOM + c * box_rows * 128;
+    int count = 0, qc = 0;
     bool ok = true;
-    // K (or V) of block kb of a request's rows: lanes ask for a box each
-    auto load = [&](const Request& r, const int* table, int hk, int kb, bool keys) {
-      int& count = keys ? kc : vc;
-      const int stages = keys ? NK : NV, st = count % stages, use = count / stages;
-      const uint32_t full = smem_u32(keys ? &k_full[st] : &v_full[st]), empty = smem_u32(keys ? &k_empty[st] : &v_empty[st]);
-      if (use > 0) ok = mbar_wait(empty, (uint32_t)(use - 1) & 1, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return;
-      if (lane == 0) mbar_expect_tx(full, TILE);
-      __syncwarp();
-      const uint32_t to_smem = sm + (keys ? L::K : L::V) + st * TILE + half * ATOM;
-      for (int i = c; i < copies; i += 32 / HALVES) {
-        const int key = kb * BN + i * box_rows, e = key / p.page;
-        int slot = p.total_slots;  // beyond the end: zeros (a page that is not held)
-        if (key < r.n && e < p.max_blocks) {
-          const int page = table[e];
-          if (page >= 0) slot = (int)min((long long)page * p.page + (key - e * p.page), (long long)p.total_slots);
-        }
-        tma_load_3d(to_smem + i * box_rows * 128, keys ? &map_k : &map_v, full, half * 64, hk, slot);
+    // Where this lane's box of a block lies in the cache (asked for two blocks ahead).
+    auto find = [&](const Request& r, const int* table, int kb) -> int {
+      const int key = kb * BN + c * box_rows, e = key / p.page;
+      int slot = p.total_slots;  // beyond the end: zeros (a page that is not held)
+      if (c < copies && key < r.n && e < p.max_blocks) {
+        const int page = __ldg(table + e);
+        if (page >= 0) slot = (int)min((long long)page * p.page + (key - e * p.page), (long long)p.total_slots);
       }
-      ++count;
+      return slot;
     };
     while (ok && walk.next(p, RT, piece)) {
       const Request r = walk.last;
       const int* table = p.table + (size_t)piece.b * p.max_blocks;
-      const int r0 = piece.g * (WIDE ? 2 * RT : RT), rows = min(r.rows - r0, WIDE ? 2 * RT : RT), sets = sets_of(rows, RT);
-      if (qc > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_empty), (uint32_t)(qc - 1) & 1, abort_flag));
-      if (!ok) break;
-      if (lane == 0) {
-        // the queries: one or two tiles, or one tile's in two or four copies
-        const int boxes = sets == 8 ? 2 : 4 / sets, box = sets == 8 || sets == 4 ? BM / G : sets == 2 ? 64 / G : 32 / G;
-        mbar_expect_tx(smem_u32(&q_full), (uint32_t)(boxes * HALVES * box * G * 128));
-        for (int i = 0; i < boxes; ++i)
-          for (int h = 0; h < HALVES; ++h)
-            tma_load_4d(sm + L::Q + (sets == 8 ? i * TILE : i * sets * 32 * 128) + h * ATOM, sets >= 4 ? &map_q1 : sets == 2 ? &map_q2 : &map_q4, smem_u32(&q_full), h * 64, 0,
-                        piece.hk, r.q_begin + (r0 + (sets == 8 ? i * RT : 0)) / G);
+      const int nb = piece.blk1 - piece.blk0, kb = r.kb0 + piece.blk0;
+      int slot = find(r, table, kb), ahead = nb > 1 ? find(r, table, kb + 1) : 0;
+      if (keys) {
+        const int r0 = piece.g * (WIDE ? 2 * RT : RT), rows = min(r.rows - r0, WIDE ? 2 * RT : RT), sets = sets_of(rows, RT);
+        if (qc > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_empty), (uint32_t)(qc - 1) & 1, abort_flag));
+        if (!ok) break;
+        if (lane == 0) {
+          // the queries: one or two tiles, or one tile's in two or four copies
+          const int boxes = sets == 8 ? 2 : 4 / sets, box = sets == 8 || sets == 4 ? BM / G : sets == 2 ? 64 / G : 32 / G;
+          mbar_expect_tx(smem_u32(&q_full), (uint32_t)(boxes * HALVES * box * G * 128));
+          for (int i = 0; i < boxes; ++i)
+            for (int h = 0; h < HALVES; ++h)
+              tma_load_4d(sm + L::Q + (sets == 8 ? i * TILE : i * sets * 32 * 128) + h * ATOM, sets >= 4 ? &map_q1 : sets == 2 ? &map_q2 : &map_q4, smem_u32(&q_full), h * 64, 0,
+                          piece.hk, r.q_begin + (r0 + (sets == 8 ? i * RT : 0)) / G);
+        }
+        ++qc;
       }
-      ++qc;
-      const int nb = piece.blk1 - piece.blk0;
-      for (int s = 0; ok && s <= nb; ++s) {
-        if (s < nb) load(r, table, piece.hk, r.kb0 + piece.blk0 + s, true);
-        if (ok && s > 0) load(r, table, piece.hk, r.kb0 + piece.blk0 + s - 1, false);
+      for (int s = 0; s < nb; ++s) {
+        const int after = s + 2 < nb ? find(r, table, kb + s + 2) : 0;
+        const int st = count % stages, use = count / stages;
+        if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[st]), (uint32_t)(use - 1) & 1, abort_flag));
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(smem_u32(&full[st]), TILE);
+        __syncwarp();
+        if (c < copies) tma_load_3d(to_smem + st * TILE, keys ? &map_k : &map_v, smem_u32(&full[st]), half * 64, piece.hk, slot);
+        ++count;
+        slot = ahead, ahead = after;
       }
     }
     if (*abort_flag) {
       // leave nothing in flight: wait (bounded, on a count of its own) for the copies already asked for
       int patience = 0;
       volatile int* own = &patience;
-      for (int i = max(0, kc - NK); i < kc; ++i) mbar_wait(smem_u32(&k_full[i % NK]), (uint32_t)(i / NK) & 1, own);
-      for (int i = max(0, vc - NV); i < vc; ++i) mbar_wait(smem_u32(&v_full[i % NV]), (uint32_t)(i / NV) & 1, own);
+      for (int i = max(0, count - stages); i < count; ++i) mbar_wait(smem_u32(&full[i % stages]), (uint32_t)(i / stages) & 1, own);
       if (qc > 0) mbar_wait(smem_u32(&q_full), (uint32_t)(qc - 1) & 1, own);
     }
   } else if (warp == 9) {

@@ -31,10 +31,10 @@ constexpr int HALVES = D / 64;
 constexpr uint32_t ATOM = 128 * 128;             // [128 rows x 128 bytes]: 64 entries of every row, swizzled
 constexpr uint32_t TILE = HALVES * ATOM;         // Q of a tile, K or V of a block
 constexpr int CH = 16;                           // columns of the result that pass from the lanes that hold them to whole lines at a time
-constexpr uint32_t MERGE = 8 * 32 * CH * 4;
-constexpr int MAX_SEQS = 1024;
+constexpr uint32_t MERGE = 8 * 32 * CH * 4;       // a half of the columns each for two times four warps
 constexpr int MAX_NODES = 256;
-constexpr int THREADS = 352;                     // eight warps of softmax, one that copies Q and K, one that issues products, one that copies V
+constexpr int THREADS = 384;                     // eight warps of softmax; one that copies K, one that issues products, one that copies Q and V, one that plans
+constexpr int AHEAD = 4;                         // pieces of work that are planned ahead
 constexpr uint32_t SPIN_LIMIT = 1u << 22;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LAG = 8.f;
@@ -59,7 +59,7 @@ struct Params {
   const float* head_sinks;  // [nq] or null
   float* part_o;          // [CTA, 2, part_rows, D]
   float* part_ml;         // [CTA, 2, part_rows, 2]
-  int* plan;              // [B + 1] what stands before each request, [B + 1]: the share of a CTA, for the joining kernel
+  int* plan;              // [B] what stands before each request and, behind them, the share of a CTA: for the joining kernel
   int* error;
   int words, max_blocks, page, nq, nkv, window, num_seqs, total_slots, part_rows, ctas;
   float scale_log2, cap_log2, cap_inv;  // cap * log2(e) and scale / cap
@@ -72,6 +72,7 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+#pragma unroll 1  // (the waits are many: unrolled they alone overflow the instruction cache)
   for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
     uint32_t done;
     asm volatile(
@@ -101,20 +102,19 @@ __device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
 __device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)((ATOM >> 4) & 0x3FFF) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool more) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)more) : "memory");
+// D = A B and D += A B, A and B in shared memory
+__device__ __forceinline__ void umma_first(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
 }
-// A (P, [128 rows x 16 keys], two bfloat16 per column) from tensor memory
+__device__ __forceinline__ void umma_more(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
+}
+// the same with A (P, [128 rows x 16 keys], two bfloat16 per column) in tensor memory
 __device__ __forceinline__ void umma_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool more) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)more) : "memory");
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)more) : "memory");
+}
+__device__ __forceinline__ void umma_tmem_a_more(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc) : "memory");
 }
 __device__ __forceinline__ bool elect_one() {
   uint32_t chosen;
@@ -188,7 +188,7 @@ struct Request {
   int q_begin, t, n, kb0, blocks, rows, groups;
 };
 template <bool WIDE>
-__device__ __forceinline__ Request request_of(const Params& p, int b, int RT) {
+__device__ __noinline__ Request request_of(const Params& p, int b, int RT) {
   Request r;
   r.q_begin = p.cu[b];
   r.t = p.cu[b + 1] - r.q_begin;
@@ -198,6 +198,7 @@ __device__ __forceinline__ Request request_of(const Params& p, int b, int RT) {
   int lo = 0;
   if (p.window > 0 && r.t > 0) {  // the first row that any node sees
     int lowest = INT_MAX;
+#pragma unroll 1
     for (int i = 0; i < r.t; ++i) lowest = min(lowest, p.positions[r.q_begin + i]);
     const long long from = (long long)lowest - p.window + 1;
     lo = from < 0 ? 0 : from > r.n - r.t ? max(r.n - r.t, 0) : (int)from;
@@ -217,70 +218,129 @@ __device__ __forceinline__ int cost_of_head(const Request& r, int RT) {  // of a
   return r.groups == 0 ? 0 : r.blocks * ((r.groups - 1) * (WIDE ? COST_TWO : COST_ONE) + cost_of<WIDE>(r, r.groups - 1, RT));
 }
 
-// A piece of work: blocks blk0 .. blk1 - 1 (of all `blocks`) of a group of rows.
-struct Piece {
-  int b, hk, g, blk0, blk1, at;  // at: where the group begins
-};
-
-// Walks over the pieces of one CTA's share [from, to).
-template <bool WIDE>
-struct Walk {
-  int b, hk, g, from, to, at;  // at: where group (b, hk, g) begins
-  Request r;
-  __device__ __forceinline__ void begin(const Params& p, const int* before, int RT, int from_, int to_) {
-    from = from_, to = to_;
-    int lo = 0, hi = p.num_seqs;  // the last request that begins at or before `from`
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (before[mid] <= from) lo = mid; else hi = mid;
-    }
-    b = lo;
-    r = request_of<WIDE>(p, b, RT);
-    const int head = cost_of_head<WIDE>(r, RT);
-    hk = head > 0 ? min((from - before[b]) / head, p.nkv - 1) : p.nkv - 1;
-    const int group = r.blocks * (WIDE ? COST_TWO : COST_ONE);
-    const int rest = from - before[b] - hk * head;
-    g = group > 0 ? min(rest / group, max(r.groups - 1, 0)) : 0;
-    at = before[b] + hk * head + g * group;
-  }
-  __device__ __forceinline__ bool next(const Params& p, int RT, Piece& out) {
-    while (b < p.num_seqs && at < to) {
-      bool found = false;
-      if (r.groups > 0) {
-        const int cost = cost_of<WIDE>(r, g, RT);
-        // blocks whose beginning lies in [from, to)
-        const int blk0 = from > at ? (from - at + cost - 1) / cost : 0;
-        const int blk1 = min(r.blocks, (to - at + cost - 1) / cost);
-        found = blk0 < blk1;
-        out = Piece{b, hk, g, blk0, blk1, at};
-        at += r.blocks * cost;
-      }
-      if (found) {
-        last = r;
-        step(p, RT);
-        return true;
-      }
-      step(p, RT);
-    }
-    return false;
-  }
-  Request last;  // the request of the piece that `next` gave
-  __device__ __forceinline__ void step(const Params& p, int RT) {
-    if (++g < r.groups) return;
-    g = 0;
-    if (r.groups > 0 && ++hk < p.nkv) return;
-    hk = 0;
-    if (++b < p.num_seqs) r = request_of<WIDE>(p, b, RT);
-  }
+// A piece of work: nb key blocks from kb on for the rows r0 .. r0 + rows - 1 of a request and KV head.
+struct __align__(16) Piece {
+  int b, hk, q_begin, t;
+  int n, kb, nb, r0;  // nb 0: no more pieces
+  int rows, sets, whole, slot;
 };
 
 // How the rows of a piece lie in the tensor memory: `sets` sets of 32 rows in different warps (8: two tiles of rows; 4, 2, 1: one tile once, twice, four times, in
 // each of the two accumulators).  Warp w holds set w % sets.
 __device__ __forceinline__ int sets_of(int rows_of_group, int RT) { return rows_of_group > RT ? 8 : rows_of_group > 64 ? 4 : rows_of_group > 32 ? 2 : 1; }
 
+// Walks over the pieces of one CTA's share [from, to); the lanes of a warp walk together.
+template <bool WIDE>
+struct Walk {
+  int b, hk, g, from, to, at;  // at: where group (b, hk, g) begins
+  Request r;
+  // The batch is added up by every warp for itself, 32 requests at a time: no memory, no barrier between.
+  __device__ __forceinline__ void begin(const Params& p, int RT, bool leave_plan) {
+    const int lane = threadIdx.x & 31;
+    int total = 0;
+    Request mine;
+    int cost = 0, sum = 0;
+    auto scan = [&](int b0) {
+      cost = 0;
+      if (b0 + lane < p.num_seqs) {
+        mine = request_of<WIDE>(p, b0 + lane, RT);
+        cost = cost_of_head<WIDE>(mine, RT) * p.nkv;
+      }
+      sum = cost;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+      }
+    };
+#pragma unroll 1
+    for (int b0 = 0; b0 < p.num_seqs; b0 += 32) {
+      scan(b0);
+      if (leave_plan && b0 + lane < p.num_seqs) p.plan[b0 + lane] = total + sum - cost;
+      total += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    const int share = max(1, (total + p.ctas - 1) / p.ctas);
+    if (leave_plan && lane == 0) p.plan[p.num_seqs] = share;
+    from = (int)min((long long)blockIdx.x * share, (long long)total);
+    to = (int)min((long long)from + share, (long long)total);
+    b = p.num_seqs, hk = g = 0, at = total;
+    r.groups = 0;
+    if (from >= to) return;
+    int before = 0;
+#pragma unroll 1
+    for (int b0 = 0; b0 < p.num_seqs; b0 += 32) {
+      if (p.num_seqs > 32) scan(b0);  // (else it is there still)
+      const unsigned here = __ballot_sync(0xffffffffu, from >= before + sum - cost && from < before + sum);
+      if (here != 0) {
+        const int who = __ffs(here) - 1;
+        r.q_begin = __shfl_sync(0xffffffffu, mine.q_begin, who);
+        r.t = __shfl_sync(0xffffffffu, mine.t, who);
+        r.n = __shfl_sync(0xffffffffu, mine.n, who);
+        r.kb0 = __shfl_sync(0xffffffffu, mine.kb0, who);
+        r.blocks = __shfl_sync(0xffffffffu, mine.blocks, who);
+        r.rows = __shfl_sync(0xffffffffu, mine.rows, who);
+        r.groups = __shfl_sync(0xffffffffu, mine.groups, who);
+        before += __shfl_sync(0xffffffffu, sum - cost, who);
+        b = b0 + who;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (b >= p.num_seqs) return;
+    const int head = cost_of_head<WIDE>(r, RT), group = r.blocks * (WIDE ? COST_TWO : COST_ONE);
+    hk = (from - before) / head;
+    g = min((from - before - hk * head) / group, r.groups - 1);
+    at = before + hk * head + g * group;
+  }
+  __device__ __forceinline__ bool next(const Params& p, int RT, Piece& out) {
+#pragma unroll 1
+    while (b < p.num_seqs && at < to) {
+      if (r.groups == 0 || g >= r.groups) {
+        g = 0;
+        if (r.groups == 0 || ++hk >= p.nkv) {
+          hk = 0;
+          if (++b < p.num_seqs) r = request_of<WIDE>(p, b, RT);
+          continue;
+        }
+      }
+      const int cost = cost_of<WIDE>(r, g, RT);
+      // blocks whose beginning lies in [from, to)
+      const int blk0 = from > at ? (from - at + cost - 1) / cost : 0, blk1 = min(r.blocks, (to - at + cost - 1) / cost);
+      const int RG = WIDE ? 2 * RT : RT, r0 = g * RG, rows = min(r.rows - r0, RG);
+      // (a share has two groups in part at most, its first and its last: their places in scratch)
+      out = Piece{b, hk, r.q_begin, r.t, r.n, r.kb0 + blk0, blk1 - blk0, r0, rows, sets_of(rows, RT), blk0 == 0 && blk1 == r.blocks, at <= from ? 0 : 1};
+      at += r.blocks * cost;
+      ++g;
+      if (blk0 < blk1) return true;
+    }
+    out.nb = 0;
+    return false;
+  }
+};
+
+// The planning warp: pieces into a ring, in whose places the other warps find them.  (A function of its own: what it holds need not stay in registers elsewhere.)
+template <bool WIDE>
+__device__ __noinline__ void plan(const Params& p, int RT, Piece* ring, uint32_t full, uint32_t empty, volatile int* abort_flag) {
+  Walk<WIDE> walk;
+  Piece piece;
+  walk.begin(p, RT, blockIdx.x == 0);
+  bool more = true;
+#pragma unroll 1
+  for (int i = 0; more; ++i) {
+    more = walk.next(p, RT, piece);
+    const int at = i % AHEAD;
+    if (i >= AHEAD && !__all_sync(0xffffffffu, mbar_wait(empty + 8 * at, (uint32_t)(i / AHEAD - 1) & 1, abort_flag))) break;
+    if ((threadIdx.x & 31) == 0) {
+      ring[at] = piece;
+      mbar_arrive(full + 8 * at);
+    }
+    __syncwarp();
+  }
+}
+
 // Which of the 32 keys from `base` on a node sees, as bits.
-__device__ __forceinline__ uint32_t seen_bits(const Params& p, const Request& r, int token, int pos, int base) {
-  const int first = r.n - r.t;
+__device__ __noinline__ uint32_t seen_bits(const Params& p, int q_begin, int t, int n, int token, int pos, int base) {
+  const int first = n - t;
   uint32_t out = 0;
   const int ahead = first - base;  // keys of these 32 ahead of the step's rows
   if (ahead > 0) {
@@ -290,19 +350,19 @@ __device__ __forceinline__ uint32_t seen_bits(const Params& p, const Request& r,
       out = hidden >= 32 ? 0u : hidden > 0 ? out & ~((1u << (int)hidden) - 1) : out;
     }
   }
-  if (ahead < 32 && base < r.n) {
+  if (ahead < 32 && base < n) {
     const unsigned long long* words = p.mask + (size_t)token * p.words;
     const int from = max(-ahead, 0);  // the first node among these keys
     const int w = from >> 6, off = from & 63;
     unsigned long long x = w < p.words ? words[w] >> off : 0ull;
     if (off > 32 && w + 1 < p.words) x |= words[w + 1] << (64 - off);
     uint32_t bits = (uint32_t)x;
-    const int nodes = min(r.t - from, 32);
+    const int nodes = min(t - from, 32);
     bits = nodes >= 32 ? bits : nodes > 0 ? bits & ((1u << nodes) - 1) : 0u;
     if (p.window > 0) {
       for (uint32_t left = bits; left != 0; left &= left - 1) {
         const int i = __ffs(left) - 1;
-        if (p.positions[r.q_begin + from + i] <= pos - p.window) bits &= ~(1u << i);
+        if (p.positions[q_begin + from + i] <= pos - p.window) bits &= ~(1u << i);
       }
     }
     out |= ahead > 0 ? bits << ahead : bits;
@@ -310,64 +370,61 @@ __device__ __forceinline__ uint32_t seen_bits(const Params& p, const Request& r,
   return out;
 }
 
-// N scores of a row from column `col` of the block on, capped, and with -inf for keys that its node does not see.
-template <int N, bool CAP>
-__device__ __forceinline__ void scores(const Params& p, const Request& r, int token, int pos, int kbase, int col, bool open, uint32_t s_addr, uint32_t* v) {
+// 32 scores of a row: -inf for keys that its node does not see.
+__device__ __forceinline__ void hide(uint32_t bits, uint32_t (&v)[32]) {
 #pragma unroll
-  for (int c = 0; c < N; c += 32) tmem_ld32(s_addr + col + c, v + c);
-  tmem_ld_wait();
-  if (CAP) {
-    // cap * tanh(x), in units of log2: tanh(x) = 1 - 2 / (exp(2x) + 1), exact at both ends, absolute error of a few 1e-7 in between
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      v[i] = __float_as_uint(p.cap_log2 * (1.f - __fdividef(2.f, __expf(2.f * p.cap_inv * __uint_as_float(v[i])) + 1.f)));
-  }
-  if (!open) {
-#pragma unroll
-    for (int c = 0; c < N; c += 32) {
-      const uint32_t bits = token >= 0 ? seen_bits(p, r, token, pos, kbase + col + c) : 0u;
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (!((bits >> i) & 1)) v[c + i] = 0xff800000u;  // -inf
-    }
-  }
+  for (int i = 0; i < 32; ++i)
+    if (!((bits >> i) & 1)) v[i] = 0xff800000u;
 }
-template <int N>
-__device__ __forceinline__ float largest(const uint32_t* v) {
+__device__ __forceinline__ float largest(const uint32_t (&v)[32]) {
   float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int i = 0; i < N; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
+  for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
   return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
-// N scores to N / 2 pairs of weights (in v's first half); returns their sum.
-template <int N>
-__device__ __forceinline__ float weights(uint32_t* v, float scale, float off) {
+// 32 scores to 16 pairs of weights; returns their sum.
+__device__ __forceinline__ float weights(const uint32_t (&v)[32], uint32_t (&w)[16], float scale, float off) {
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
+  for (int i = 0; i < 32; i += 2) {
     const float a = fast_exp2(fmaf(__uint_as_float(v[i]), scale, -off)), b = fast_exp2(fmaf(__uint_as_float(v[i + 1]), scale, -off));
     sum[i >> 1 & 3] += a + b;
-    v[i >> 1] = pack_bf16(a, b);
+    w[i >> 1] = pack_bf16(a, b);
   }
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// One block's weights for one warp's 32 rows: KEYS keys from column `key0` of the block on.  Scores come from `s_addr` (the tile's columns at this warp's lanes); the
-// weights of all 128 keys go over them as bfloat16, zeros for keys that are other copies' part.
-template <int KEYS, bool CAP>
-__device__ __forceinline__ void weigh(const Params& p, const Request& r, int token, int pos, int kbase, int key0, bool open, uint32_t s_addr, uint32_t o_addr,
-                                      bool first_item, float& m_run, float& l_run) {
-  constexpr int HELD = KEYS < 64 ? KEYS : 64;  // (of 128 the second 64 are kept and the first read again: all would not fit the registers)
-  const float scale = CAP ? 1.f : p.scale_log2;
-  uint32_t v[HELD];
-  float m_blk = -INFINITY;
-  if (KEYS == 128) {
-    scores<64, CAP>(p, r, token, pos, kbase, 0, open, s_addr, v);
-    m_blk = largest<64>(v);
+// One block's weights for one warp's 32 rows: 32 N keys from column `key0` of the block on.  Scores come from `s_addr` (the tile's columns at this warp's lanes); the
+// weights of all 128 keys go over them as bfloat16, zeros for keys that are other copies' part.  Two walks over the scores, 32 at a time and the next 32 on their way:
+// for the largest, and for the weights (kept in registers in between they would spill what the loop around holds).
+template <int N, bool CAP>
+__device__ __forceinline__ void weigh(const Params& p, const Piece& r, int token, int pos, int kbase, int key0, bool open, uint32_t s_addr, uint32_t o_addr, bool first_item,
+                                      float scale, float& m_run, float& l_run) {
+  uint32_t v[2][32], w[16], bits[N];
+  if (!open) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) bits[c] = token >= 0 ? seen_bits(p, r.q_begin, r.t, r.n, token, pos, kbase + key0 + 32 * c) : 0u;
   }
-  scores<HELD, CAP>(p, r, token, pos, kbase, KEYS == 128 ? 64 : key0, open, s_addr, v);
-  m_blk = fmaxf(m_blk, largest<HELD>(v)) * scale;  // (scale > 0)
-  const bool raise = m_blk - m_run > LAG;          // also where m_run is -inf and m_blk is not
+  float m_blk = -INFINITY;
+  tmem_ld32(s_addr + key0, v[0]);
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    tmem_ld_wait();
+    if (c + 1 < N) tmem_ld32(s_addr + key0 + 32 * (c + 1), v[(c + 1) & 1]);
+    if (CAP) {
+      // cap * tanh(x), in units of log2: tanh(x) = 1 - 2 / (exp(2x) + 1), exact at both ends, absolute error of a few 1e-7 in between; the second walk finds it in place
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        v[c & 1][i] = __float_as_uint(p.cap_log2 * (1.f - __fdividef(2.f, __expf(2.f * p.cap_inv * __uint_as_float(v[c & 1][i])) + 1.f)));
+      if (c + 1 < N) tmem_st32(s_addr + key0 + 32 * c, v[c & 1]);
+    }
+    if (!open) hide(bits[c], v[c & 1]);
+    m_blk = fmaxf(m_blk, largest(v[c & 1]));
+  }
+  if (CAP && N > 1) tmem_st_wait();
+  if (N > 1) tmem_ld32(s_addr + key0, v[N & 1]);  // (the last 32 are kept, in v[(N - 1) & 1])
+  m_blk *= scale;                           // (scale > 0)
+  const bool raise = m_blk - m_run > LAG;   // also where m_run is -inf and m_blk is not
   if (__any_sync(0xffffffffu, raise)) {
     const float m_new = raise ? m_blk : m_run;
     const float corr = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
@@ -375,67 +432,154 @@ __device__ __forceinline__ void weigh(const Params& p, const Request& r, int tok
     l_run *= corr;
     if (!first_item) {
       // (the product before this one on the accumulator is complete: the scores, asked for behind it, are)
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < D; c += 16) {
-        uint32_t o[16];
-        tmem_ld16(o_addr + c, o);
+        tmem_ld16(o_addr + c, w);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-        tmem_st16(o_addr + c, o);
+        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * corr);
+        tmem_st16(o_addr + c, w);
       }
-      tmem_st_wait();
     }
   }
   const float off = m_run == -INFINITY ? 0.f : m_run;
-  l_run += weights<HELD>(v, scale, off);
-  if (KEYS == 128) {
-    uint32_t w[64];
-    scores<64, CAP>(p, r, token, pos, kbase, 0, open, s_addr, w);
-    l_run += weights<64>(w, scale, off);
-    tmem_st32(s_addr, w);
-    tmem_st32(s_addr + 32, v);
-  } else if (KEYS == 64) {
-    uint32_t zero[32];
+  uint32_t last[16];
+  l_run += weights(v[(N - 1) & 1], last, scale, off);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) zero[i] = 0u;
-    tmem_st32(s_addr + key0 / 2, v);
-    tmem_st32(s_addr + 32 - key0 / 2, zero);
-  } else {
-    uint32_t zero[16];
+  for (int c = 0; c + 1 < N; ++c) {
+    tmem_ld_wait();
+    if (c + 2 < N) tmem_ld32(s_addr + key0 + 32 * (c + 1), v[(N + c + 1) & 1]);
+    if (!open) hide(bits[c], v[(N + c) & 1]);
+    l_run += weights(v[(N + c) & 1], w, scale, off);
+    tmem_st16(s_addr + key0 / 2 + 16 * c, w);  // (over scores that have been read: those of keys below 32 c + 32)
+  }
+  tmem_st16(s_addr + key0 / 2 + 16 * (N - 1), last);
+  if (N < 4) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) zero[i] = 0u;
+    for (int i = 0; i < 16; ++i) w[i] = 0u;
 #pragma unroll
-    for (int c = 0; c < 64; c += 16) {
-      if (c == key0 / 2) tmem_st16(s_addr + c, v);
-      else tmem_st16(s_addr + c, zero);
-    }
+    for (int c = 16 * N; c < 64; c += 16) tmem_st16(s_addr + (key0 / 2 ^ c), w);  // (key0 is a multiple of 32 N: the other multiples of 16)
   }
   tmem_st_wait();
+}
+
+// A finished piece's rows leave: whole groups as results, others as parts.
+// Warp (half, quad) takes half of the columns of both accumulators at its 32 lanes.  Rows that stand there once leave from the registers; copies in
+// other lanes are added up through shared memory, CH columns at a time.  Parts stand as [4 columns][row][4], so that lanes write and read whole lines.
+template <int SETS>
+__device__ __noinline__ void leave(const Params& p, const Piece& w, bool good, int G, int RT, const float2 (*ml)[32], unsigned char* merge, uint32_t tmem, int warp, int lane) {
+  constexpr int TILES = SETS == 8 ? 2 : 1;  // of rows; else the two accumulators hold the same rows
+  const int half = warp >> 2, quad = warp & 3, c_begin = half * (D / 2);
+  const uint32_t o_lane = tmem + ((uint32_t)(quad * 32) << 16) + 256 + c_begin;
+  const size_t part = ((size_t)blockIdx.x * 2 + w.slot) * p.part_rows;
+  const bool both = w.nb > 1;  // the second accumulator holds something too
+#pragma unroll
+  for (int x = 0; x < TILES; ++x) {
+    const int in = (SETS == 8 ? quad : quad % SETS) * 32 + lane, place = x * BM + in, row = w.r0 + x * RT + in;
+    const bool real = in < RT && x * RT + in < w.rows, kept = good && place < p.part_rows;
+    // the row's maximum and sum over its copies, and what this lane's sums are multiplied by
+    float2 y[8 / SETS];
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8 / SETS; ++i) y[i] = ml[(place >> 5) + i * SETS][lane], top = fmaxf(top, y[i].x);
+#pragma unroll
+    for (int i = 0; i < 8 / SETS; ++i) sum += y[i].x == -INFINITY ? 0.f : y[i].y * fast_exp2(y[i].x - top);
+    const float m0 = ml[(SETS == 8 ? 4 * x : 0) + quad][lane].x, m1 = ml[4 + quad][lane].x;
+    float all = 1.f;
+    if (w.whole) {
+      float down = 1.f;
+      if (p.head_sinks != nullptr && real) {
+        const float sink = p.head_sinks[w.hk * G + row % G] * LOG2E, over = fmaxf(top, sink);
+        down = top == -INFINITY ? 0.f : fast_exp2(top - over);
+        sum = sum * down + (sink == -INFINITY ? 0.f : fast_exp2(sink - over));
+      }
+      all = sum > 0.f ? down / sum : 0.f;
+    } else if (half == 0 && quad < SETS && kept) {
+      *reinterpret_cast<float2*>(p.part_ml + (part + place) * 2) = make_float2(top, sum);
+    }
+    const float f0 = m0 == -INFINITY ? 0.f : all * fast_exp2(m0 - top), f1 = SETS == 8 || !both || m1 == -INFINITY ? 0.f : all * fast_exp2(m1 - top);
+    __nv_bfloat16* out = p.out + ((size_t)(w.q_begin + row / G) * p.nq + w.hk * G + row % G) * D + c_begin;
+    float* to_part = p.part_o + part * D + ((size_t)(c_begin / 4) * p.part_rows + place) * 4;
+    const int step = p.part_rows * 4;
+    unsigned char* mine = merge + half * (MERGE / 2) + (quad * 32 + lane) * (CH * 4);
+    const int swizzle = (lane >> 1 & 3) << 4;
+#pragma unroll 1
+    for (int c = 0; c < D / 2; c += CH) {
+      uint32_t o0[CH], o1[CH];
+      tmem_ld16(o_lane + x * D + c, o0);
+      if (SETS < 8 && both) tmem_ld16(o_lane + D + c, o1);
+      tmem_ld_wait();
+      float v[CH];
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        v[i] = f0 > 0.f ? __uint_as_float(o0[i]) * f0 : 0.f;
+        if (SETS < 8 && f1 > 0.f) v[i] = fmaf(__uint_as_float(o1[i]), f1, v[i]);
+      }
+      // of a row's four pieces of 4 columns: which this warp adds up and writes (its copies' warps share them)
+      constexpr int PIECES = SETS >= 4 ? 4 : SETS, COPIES = SETS >= 4 ? 1 : 4 / SETS;
+      const int first = SETS >= 4 ? 0 : SETS == 2 ? (quad >> 1) * 2 : quad;
+      if (SETS < 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(mine + ((i << 4) ^ swizzle)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
+        const unsigned char* row_at = merge + half * (MERGE / 2) + ((quad % SETS) * 32 + lane) * (CH * 4);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          float4 z[COPIES];
+#pragma unroll
+          for (int k = 0; k < COPIES; ++k) z[k] = *reinterpret_cast<const float4*>(row_at + k * (SETS * 32 * CH * 4) + (((first + i) << 4) ^ swizzle));
+#pragma unroll
+          for (int k = 1; k < COPIES; ++k) z[0].x += z[k].x, z[0].y += z[k].y, z[0].z += z[k].z, z[0].w += z[k].w;
+          v[4 * i] = z[0].x, v[4 * i + 1] = z[0].y, v[4 * i + 2] = z[0].z, v[4 * i + 3] = z[0].w;
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
+      }
+      if (w.whole) {
+        if (real && good) {
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i)
+            *reinterpret_cast<uint2*>(out + c + 4 * (first + i)) = make_uint2(pack_bf16(v[4 * i], v[4 * i + 1]), pack_bf16(v[4 * i + 2], v[4 * i + 3]));
+        }
+      } else if (kept) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+          *reinterpret_cast<float4*>(to_part + (size_t)(c / 4 + first + i) * step) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      }
+    }
+  }
 }
 
 template <bool WIDE, bool CAP>
 __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid_constant__ CUtensorMap map_q1, const __grid_constant__ CUtensorMap map_q2,
                                                                     const __grid_constant__ CUtensorMap map_q4, const __grid_constant__ CUtensorMap map_k,
-                                                                    const __grid_constant__ CUtensorMap map_v, const Params p) {
+                                                                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Params params) {
   using L = Layout<WIDE>;
   constexpr int NK = L::NK, NV = L::NV;
   ts_pdl_wait();  // tensor memory is never held while waiting for another kernel
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[NK], k_empty[NK], v_full[NV], v_empty[NV], s_full[2], p_full[2], o_full[2], all_done;
+  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[NK], k_empty[NK], v_full[NV], v_empty[NV], s_full[2], p_full[2], o_full[2], piece_full[AHEAD], piece_empty[AHEAD], all_done;
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
-  __shared__ int before_s[MAX_SEQS + 1], sum_s[THREADS / 32];
   __shared__ float2 ml_s[8][32];
+  __shared__ Piece piece_s[AHEAD];
+  __shared__ Params params_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // The arguments in shared memory: what is read once a piece is seldom in the constant cache.
+  static_assert(sizeof(Params) % 4 == 0 && sizeof(Params) / 4 <= THREADS, "a word per thread");
+  if (tid < (int)(sizeof(Params) / 4)) reinterpret_cast<uint32_t*>(&params_s)[tid] = reinterpret_cast<const uint32_t*>(&params)[tid];
+  __syncthreads();
+  const Params& p = params_s;
   const int G = p.nq / p.nkv, RT = BM / G * G;
 
+  if (warp == 9 && lane < 5)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &map_k : lane == 1 ? &map_v : lane == 2 ? &map_q1 : lane == 3 ? &map_q2 : &map_q4) : "memory");
   if (tid == 0) {
     abort_s = 0;
     mbar_init(smem_u32(&q_full), 1);
     mbar_init(smem_u32(&q_empty), 1);
     mbar_init(smem_u32(&all_done), 1);
+    for (int s = 0; s < AHEAD; ++s) mbar_init(smem_u32(&piece_full[s]), 1), mbar_init(smem_u32(&piece_empty[s]), 11);
     for (int s = 0; s < NK; ++s) mbar_init(smem_u32(&k_full[s]), 1), mbar_init(smem_u32(&k_empty[s]), 1);
     for (int s = 0; s < NV; ++s) mbar_init(smem_u32(&v_full[s]), 1), mbar_init(smem_u32(&v_empty[s]), 1);
     for (int t = 0; t < 2; ++t) mbar_init(smem_u32(&s_full[t]), 1), mbar_init(smem_u32(&p_full[t]), 4), mbar_init(smem_u32(&o_full[t]), 1);
@@ -446,48 +590,26 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // What stands before each request: a running sum over the batch, every CTA for itself.
-  int total = 0;
-  for (int b0 = 0; b0 < p.num_seqs; b0 += THREADS) {
-    const int b = b0 + tid;
-    int mine = 0;
-    if (b < p.num_seqs) mine = cost_of_head<WIDE>(request_of<WIDE>(p, b, RT), RT) * p.nkv;
-    int sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
-    }
-    if (lane == 31) sum_s[warp] = sum;
-    __syncthreads();
-    int ahead = total, all = total;
-    for (int w = 0; w < THREADS / 32; ++w) {
-      if (w < warp) ahead += sum_s[w];
-      all += sum_s[w];
-    }
-    if (b < p.num_seqs) before_s[b] = ahead + sum - mine;
-    total = all;
-    __syncthreads();
-  }
-  const int share = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
-  if (tid == 0) before_s[p.num_seqs] = total;
   fence_before();
   __syncthreads();
   fence_after();
   ts_pdl_launch_dependents();
-  if (blockIdx.x == 0) {
-    for (int b = tid; b <= p.num_seqs; b += THREADS) p.plan[b] = before_s[b];
-    if (tid == 0) p.plan[p.num_seqs + 1] = share;
-  }
   const uint32_t tmem = tmem_base_s, sm = smem_u32(smem);
   volatile int* abort_flag = &abort_s;
-  const int from = min((long long)blockIdx.x * share, (long long)total), to = min((long long)from + share, (long long)total);
-  Walk<WIDE> walk;
-  Piece piece;
-  walk.begin(p, before_s, RT, from, to);
+  // The next piece of work, for every warp but the one that plans, which reads it where it stands and gives the place back when it is done; false: a wait gave up.
+  int pieces = 0;
+  auto fetch = [&]() -> bool { return mbar_wait(smem_u32(&piece_full[pieces % AHEAD]), (uint32_t)(pieces / AHEAD) & 1, abort_flag); };
+  auto release = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&piece_empty[pieces % AHEAD]));
+    ++pieces;
+  };
 
-  if (warp == 8 || warp == 10) {
-    // ---------------- copies: Q and K, and V ----------------
+  if (warp == 11) {
+    // ---------------- plan ----------------
+    plan<WIDE>(p, RT, piece_s, smem_u32(piece_full), smem_u32(piece_empty), abort_flag);
+  } else if (warp == 8 || warp == 10) {
+    // ---------------- copies: K, and Q and V ----------------
     const bool keys = warp == 8;
     const int box_rows = min(p.page, BN), copies = BN / box_rows;
     const int c = lane / HALVES, half = lane % HALVES;  // this lane's box of a block (at most 16 a half: pages of 8)
@@ -497,46 +619,49 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
     const uint32_t to_smem = sm + (keys ? L::K : L::V) + half * ATOM + c * box_rows * 128;
     int count = 0, qc = 0;
     bool ok = true;
-    // Where this lane's box of a block lies in the cache (asked for two blocks ahead).
-    auto find = [&](const Request& r, const int* table, int kb) -> int {
+    // The page of this lane's box of a block, -1 where it has none: asked for two blocks ahead, looked at when its turn comes.
+    auto page_of = [&](const Piece& r, const int* table, int kb) -> int {
       const int key = kb * BN + c * box_rows, e = key / p.page;
-      int slot = p.total_slots;  // beyond the end: zeros (a page that is not held)
-      if (c < copies && key < r.n && e < p.max_blocks) {
-        const int page = __ldg(table + e);
-        if (page >= 0) slot = (int)min((long long)page * p.page + (key - e * p.page), (long long)p.total_slots);
-      }
-      return slot;
+      int page = -1;
+      if (c < copies && key < r.n && e < p.max_blocks) page = __ldg(table + e);
+      return page;
     };
-    while (ok && walk.next(p, RT, piece)) {
-      const Request r = walk.last;
-      const int* table = p.table + (size_t)piece.b * p.max_blocks;
-      const int nb = piece.blk1 - piece.blk0, kb = r.kb0 + piece.blk0;
-      int slot = find(r, table, kb), ahead = nb > 1 ? find(r, table, kb + 1) : 0;
-      if (keys) {
-        const int r0 = piece.g * (WIDE ? 2 * RT : RT), rows = min(r.rows - r0, WIDE ? 2 * RT : RT), sets = sets_of(rows, RT);
+    while (ok) {
+      ok = __all_sync(0xffffffffu, fetch());
+      const Piece r = piece_s[pieces % AHEAD];
+      release();
+      if (!ok || r.nb == 0) break;
+      const int* table = p.table + (size_t)r.b * p.max_blocks;
+      int page = page_of(r, table, r.kb), ahead = r.nb > 1 ? page_of(r, table, r.kb + 1) : -1;
+      if (!keys) {
         if (qc > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_empty), (uint32_t)(qc - 1) & 1, abort_flag));
         if (!ok) break;
         if (lane == 0) {
           // the queries: one or two tiles, or one tile's in two or four copies
-          const int boxes = sets == 8 ? 2 : 4 / sets, box = sets == 8 || sets == 4 ? BM / G : sets == 2 ? 64 / G : 32 / G;
+          const int boxes = r.sets == 8 ? 2 : 4 / r.sets, box = r.sets >= 4 ? BM / G : r.sets == 2 ? 64 / G : 32 / G;
           mbar_expect_tx(smem_u32(&q_full), (uint32_t)(boxes * HALVES * box * G * 128));
-          for (int i = 0; i < boxes; ++i)
-            for (int h = 0; h < HALVES; ++h)
-              tma_load_4d(sm + L::Q + (sets == 8 ? i * TILE : i * sets * 32 * 128) + h * ATOM, sets >= 4 ? &map_q1 : sets == 2 ? &map_q2 : &map_q4, smem_u32(&q_full), h * 64, 0,
-                          piece.hk, r.q_begin + (r0 + (sets == 8 ? i * RT : 0)) / G);
+#pragma unroll 1
+          for (int i = 0; i < boxes * HALVES; ++i) {
+            const int x = i / HALVES, h = i % HALVES;
+            tma_load_4d(sm + L::Q + (r.sets == 8 ? x * TILE : x * r.sets * 32 * 128) + h * ATOM, r.sets >= 4 ? &map_q1 : r.sets == 2 ? &map_q2 : &map_q4, smem_u32(&q_full), h * 64,
+                        0, r.hk, r.q_begin + (r.r0 + (r.sets == 8 ? x * RT : 0)) / G);
+          }
         }
         ++qc;
       }
-      for (int s = 0; s < nb; ++s) {
-        const int after = s + 2 < nb ? find(r, table, kb + s + 2) : 0;
+#pragma unroll 1
+      for (int s = 0; s < r.nb; ++s) {
+        const int after = s + 2 < r.nb ? page_of(r, table, r.kb + s + 2) : -1;
         const int st = count % stages, use = count / stages;
         if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[st]), (uint32_t)(use - 1) & 1, abort_flag));
         if (!ok) break;
         if (lane == 0) mbar_expect_tx(smem_u32(&full[st]), TILE);
         __syncwarp();
-        if (c < copies) tma_load_3d(to_smem + st * TILE, keys ? &map_k : &map_v, smem_u32(&full[st]), half * 64, piece.hk, slot);
+        // (beyond the end: the copy engine fills zeros)
+        const int slot = page < 0 ? p.total_slots : (int)min((long long)page * p.page + ((r.kb + s) * BN + c * box_rows) % p.page, (long long)p.total_slots);
+        if (c < copies) tma_load_3d(to_smem + st * TILE, keys ? &map_k : &map_v, smem_u32(&full[st]), half * 64, r.hk, slot);
         ++count;
-        slot = ahead, ahead = after;
+        page = ahead, ahead = after;
       }
     }
     if (*abort_flag) {
@@ -547,58 +672,65 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
       if (qc > 0) mbar_wait(smem_u32(&q_full), (uint32_t)(qc - 1) & 1, own);
     }
   } else if (warp == 9) {
-    // ---------------- products: the warp runs together, one elected lane issues ----------------
+    // ---------------- products: the warp runs together, one elected lane issues (a lane by itself takes 100 cycles for an instruction, not 57) ----------------
     // Items of a piece: tile i & 1, block i >> 1 for two tiles of rows, i where one tile's blocks alternate.  S of item i + 2 goes where S and P of item i lay: the
     // tensor core runs what one thread issues in order, so P V of item i has read P before.
     int kc = 0, vc = 0, qc = 0, pc[2] = {0, 0};
     bool ok = true;
     const uint64_t q_desc = desc_k_major(sm + L::Q), k_desc = desc_k_major(sm + L::K), v_desc = desc_mn_major(sm + L::V);
-    while (ok && walk.next(p, RT, piece)) {
-      const Request r = walk.last;
-      const int rows = min(r.rows - piece.g * (WIDE ? 2 * RT : RT), WIDE ? 2 * RT : RT);
-      const bool two = WIDE && rows > RT;
-      const int nb = piece.blk1 - piece.blk0, items = two ? 2 * nb : nb;
+    while (ok) {
+      ok = __all_sync(0xffffffffu, fetch());
+      const Piece r = piece_s[pieces % AHEAD];
+      release();
+      if (!ok || r.nb == 0) break;
+      const bool two = WIDE && r.sets == 8;
+      const int nb = r.nb, items = two ? 2 * nb : nb;
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_full), (uint32_t)qc & 1, abort_flag));
       if (!ok) break;
-      auto issue_s = [&](int i) {
-        const int blk = two ? i >> 1 : i, st = (kc + blk) % NK;
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[st]), (uint32_t)((kc + blk) / NK) & 1, abort_flag));
-        if (!ok) return;
-        fence_after();
-        if (elect_one()) {
-          const uint64_t kd = k_desc + (uint64_t)((st * TILE) >> 4), qd = q_desc + (uint64_t)(two && (i & 1) ? TILE >> 4 : 0);
+#pragma unroll 1
+      for (int i = 0; i < items + 2; ++i) {
+        if (i >= 2) {  // P V of item i - 2, once its weights and (for the first of two tiles) V are there
+          const int j = i - 2, blk = two ? j >> 1 : j, st = (vc + blk) % NV, t = j & 1;
+          bool there = true;
+          if (!two || t == 0) there = mbar_wait(smem_u32(&v_full[st]), (uint32_t)((vc + blk) / NV) & 1, abort_flag);
+          there = there && mbar_wait(smem_u32(&p_full[t]), (uint32_t)pc[t] & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, there);
+          if (!ok) break;
+          ++pc[t];
+          fence_after();
+          if (elect_one()) {
+            const uint64_t vd = v_desc + (uint64_t)((st * TILE) >> 4);
+            const uint32_t to = tmem + 256 + t * D, from_p = tmem + t * 128;
+            umma_tmem_a(to, from_p, vd, idesc(D, true), j >= 2);
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) {
-            const uint32_t off = ((ks >> 2) * ATOM + (ks & 3) * 32) >> 4;
-            umma(tmem + (i & 1) * 128, qd + off, kd + off, idesc(BN, false), ks > 0);
+            for (int kk = 1; kk < BN / 16; ++kk) umma_tmem_a_more(to, from_p + kk * 8, vd + ((kk * 2048) >> 4), idesc(D, true));
+            if (!two || t == 1) umma_commit(smem_u32(&v_empty[st]));
+            if (j >= items - 2) umma_commit(smem_u32(&o_full[t]));
+            if (items == 1) umma_commit(smem_u32(&o_full[1]));  // (a tile without items: its accumulator is not read)
           }
-          umma_commit(smem_u32(&s_full[i & 1]));
-          if (!two || (i & 1)) umma_commit(smem_u32(&k_empty[st]));
-          if (i == items - 1) umma_commit(smem_u32(&q_empty));
+          __syncwarp();
         }
-        __syncwarp();
-      };
-      issue_s(0);
-      if (ok && items > 1) issue_s(1);
-      for (int i = 0; ok && i < items; ++i) {
-        const int blk = two ? i >> 1 : i, st = (vc + blk) % NV, t = i & 1;
-        ok = mbar_wait(smem_u32(&v_full[st]), (uint32_t)((vc + blk) / NV) & 1, abort_flag);
-        if (ok) ok = mbar_wait(smem_u32(&p_full[t]), (uint32_t)pc[t] & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        ++pc[t];
-        fence_after();
-        if (elect_one()) {
-          const uint64_t vd = v_desc + (uint64_t)((st * TILE) >> 4);
+        if (i < items) {  // S of item i, once its K is there (of two tiles the second finds it there)
+          const int blk = two ? i >> 1 : i, st = (kc + blk) % NK, t = i & 1;
+          if (!two || t == 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[st]), (uint32_t)((kc + blk) / NK) & 1, abort_flag));
+            if (!ok) break;
+          }
+          if (elect_one()) {
+            const uint64_t kd = k_desc + (uint64_t)((st * TILE) >> 4), qd = q_desc + (uint64_t)(two && t ? TILE >> 4 : 0);
+            const uint32_t to = tmem + t * 128;
+            umma_first(to, qd, kd, idesc(BN, false));
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            umma_tmem_a(tmem + 256 + t * D, tmem + t * 128 + kk * 8, vd + ((kk * 2048) >> 4), idesc(D, true), kk > 0 || i >= 2);
-          if (!two || (i & 1)) umma_commit(smem_u32(&v_empty[st]));
-          if (i >= items - 2) umma_commit(smem_u32(&o_full[t]));
-          if (items == 1) umma_commit(smem_u32(&o_full[1]));  // (a tile without items: its warps do not read it)
+            for (int ks = 1; ks < D / 16; ++ks) {
+              const uint32_t off = ((ks >> 2) * ATOM + (ks & 3) * 32) >> 4;
+              umma_more(to, qd + off, kd + off, idesc(BN, false));
+            }
+            umma_commit(smem_u32(&s_full[t]));
+            if (!two || t == 1) umma_commit(smem_u32(&k_empty[st]));
+            if (i == items - 1) umma_commit(smem_u32(&q_empty));
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        if (i + 2 < items) issue_s(i + 2);
       }
       kc += nb, vc += nb, ++qc;
     }
@@ -610,39 +742,43 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
     if (patience != 0) *abort_flag = 1;
   } else {
     // ---------------- softmax ----------------
-    // (A wait that gives up raises the flag at which all later ones return at once; these warps then run to the end of their pieces, barriers included, and store nothing.)
+    // (A wait that gives up raises the flag at which all later ones return at once; these warps then run to the end of the piece, barriers included, and store nothing.)
     const int t = warp >> 2, quad = warp & 3;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t s_addr = tmem + lanes + t * 128, o_addr = tmem + lanes + 256 + t * D;
-    unsigned char* merge = smem + L::MERGE_AT;
-    int sc = 0, pieces = 0, vc = 0;
-    while (walk.next(p, RT, piece)) {
-      const Request r = walk.last;
-      const int r0 = piece.g * (WIDE ? 2 * RT : RT), rows = min(r.rows - r0, WIDE ? 2 * RT : RT), sets = sets_of(rows, RT);
-      const bool two = sets == 8;
-      const int nb = piece.blk1 - piece.blk0, first = r.n - r.t;
+    const float scale = CAP ? 1.f : p.scale_log2;
+    int sc = 0, vc = 0, done = 0;
+    for (;;) {
+      uint32_t there = fetch();
+      const Piece& r = piece_s[pieces % AHEAD];
+      asm volatile(  // (all eight warps go on, or none)
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %0, 0;\n\tbarrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "+r"(there)::"memory");
+      if (!there || r.nb == 0) break;
+      const int sets = r.sets, nb = r.nb, first = r.n - r.t;
+      const bool two = WIDE && sets == 8;
       // this thread's row of the group
-      const int in_group = (warp % sets) * 32 + lane;
-      const bool mine = two ? (t == 0 ? in_group < RT : in_group - BM < RT && RT + in_group - BM < rows) : in_group < rows;
-      const int row = r0 + (two && t == 1 ? in_group - BM + RT : in_group);
+      const int in_group = (warp & (sets - 1)) * 32 + lane;
+      const bool mine = two ? (t == 0 ? in_group < RT : in_group - BM < RT && RT + in_group - BM < r.rows) : in_group < r.rows;
+      const int row = r.r0 + (two && t == 1 ? in_group - BM + RT : in_group);
       const int token = mine ? r.q_begin + row / G : -1;
       const int pos = mine && p.window > 0 ? p.positions[token] : 0;
-      const int keys = sets >= 4 ? 128 : sets * 32, key0 = sets >= 4 ? 0 : sets == 2 ? (quad >> 1) * 64 : quad * 32;
+      const int key0 = sets >= 4 ? 0 : sets == 2 ? (quad >> 1) * 64 : quad * 32;
       float m = -INFINITY, l = 0.f;
       const int items = two ? nb : (nb + 1 - t) / 2;
+#pragma unroll 1
       for (int it = 0; it < items; ++it) {
-        const int blk = two ? it : 2 * it + t, kbase = (r.kb0 + piece.blk0 + blk) * BN;
+        const int blk = two ? it : 2 * it + t, kbase = (r.kb + blk) * BN;
         mbar_wait(smem_u32(&s_full[t]), (uint32_t)sc & 1, abort_flag);
         ++sc;
         __syncwarp();
         fence_after();
         const bool open = p.window == 0 && kbase + BN <= first;
-        if (keys == 128)
-          weigh<128, CAP>(p, r, token, pos, kbase, 0, open, s_addr, o_addr, it == 0, m, l);
-        else if (keys == 64)
-          weigh<64, CAP>(p, r, token, pos, kbase, key0, open, s_addr, o_addr, it == 0, m, l);
+        if (sets >= 4)
+          weigh<4, CAP>(p, r, token, pos, kbase, 0, open, s_addr, o_addr, it == 0, scale, m, l);
+        else if (sets == 2)
+          weigh<2, CAP>(p, r, token, pos, kbase, key0, open, s_addr, o_addr, it == 0, scale, m, l);
         else
-          weigh<32, CAP>(p, r, token, pos, kbase, key0, open, s_addr, o_addr, it == 0, m, l);
+          weigh<1, CAP>(p, r, token, pos, kbase, key0, open, s_addr, o_addr, it == 0, scale, m, l);
         if (kbase + BN > r.n) {
           // rows of V that no request has written: zeros (a masked key's weight is zero, but zero times garbage must stay zero)
           const int st = (vc + blk) % NV, bad = max(r.n - kbase, 0);
@@ -659,71 +795,28 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
         if (lane == 0) mbar_arrive(smem_u32(&p_full[t]));
       }
       vc += nb;
-      // ---- the group's rows: sums over a row's copies, through shared memory, as whole lines ----
-      mbar_wait(smem_u32(&o_full[t]), (uint32_t)pieces & 1, abort_flag);
-      ++pieces;
+      // ---- the group's rows ----
+      mbar_wait(smem_u32(&o_full[0]), (uint32_t)done & 1, abort_flag);
+      mbar_wait(smem_u32(&o_full[1]), (uint32_t)done & 1, abort_flag);
+      ++done;
+      ml_s[warp][lane] = make_float2(m, l);
       __syncwarp();
       fence_after();
-      ml_s[warp][lane] = make_float2(m, l);
       asm volatile("bar.sync 1, 256;" ::: "memory");
       const bool good = *abort_flag == 0;
-      const bool whole = piece.blk0 == 0 && piece.blk1 == r.blocks;
-      float top = -INFINITY, sum = 0.f;
-      for (int w = warp % sets; w < 8; w += sets) top = fmaxf(top, ml_s[w][lane].x);
-      for (int w = warp % sets; w < 8; w += sets) {
-        const float2 x = ml_s[w][lane];
-        if (x.x > -INFINITY) sum += x.y * fast_exp2(x.x - top);
-      }
-      float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
-      const int slot = piece.at <= from ? 0 : 1;  // a share has two groups in part at most: its first and its last
-      float* part_o = p.part_o + ((size_t)blockIdx.x * 2 + slot) * p.part_rows * D;
-      if (whole) {
-        if (p.head_sinks != nullptr && mine) {
-          const float sink = p.head_sinks[piece.hk * G + row % G] * LOG2E, over = fmaxf(top, sink);
-          const float down = top == -INFINITY ? 0.f : fast_exp2(top - over);
-          sum = sum * down + (sink == -INFINITY ? 0.f : fast_exp2(sink - over));
-          f *= down;
-        }
-        f = sum > 0.f ? f / sum : 0.f;
-      } else if (warp < sets && good && in_group < p.part_rows) {
-        float* ml = p.part_ml + (((size_t)blockIdx.x * 2 + slot) * p.part_rows + in_group) * 2;
-        ml[0] = top, ml[1] = sum;
-      }
-      for (int c0 = 0; c0 < D; c0 += CH) {
-        uint32_t o[CH];
-        if (items > 0) {
-          tmem_ld16(o_addr + c0, o);
-          tmem_ld_wait();
-        }
-#pragma unroll
-        for (int i = 0; i < CH / 4; ++i) {
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (f > 0.f) x = make_float4(__uint_as_float(o[4 * i]) * f, __uint_as_float(o[4 * i + 1]) * f, __uint_as_float(o[4 * i + 2]) * f, __uint_as_float(o[4 * i + 3]) * f);
-          *reinterpret_cast<float4*>(merge + (warp * 32 + lane) * (CH * 4) + ((i ^ (lane >> 1 & 3)) << 4)) = x;
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        for (int i = warp * 32 + lane; i < sets * 32 * (CH / 4); i += 256) {
-          const int at = i / (CH / 4), c = i % (CH / 4), ln = at & 31;  // row `at` of the group's lanes, 16-byte piece c
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int w = at >> 5; w < 8; w += sets) {
-            const float4 y = *reinterpret_cast<const float4*>(merge + (w * 32 + ln) * (CH * 4) + ((c ^ (ln >> 1 & 3)) << 4));
-            x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-          }
-          if (!good) continue;
-          if (whole) {
-            const bool tile1 = two && at >= BM;
-            const int in = tile1 ? at - BM : at, rr = r0 + (tile1 ? RT : 0) + in;
-            if (in < RT && rr < r0 + rows) {
-              uint2 y;
-              y.x = pack_bf16(x.x, x.y), y.y = pack_bf16(x.z, x.w);
-              *reinterpret_cast<uint2*>(p.out + ((size_t)(r.q_begin + rr / G) * p.nq + piece.hk * G + rr % G) * D + c0 + c * 4) = y;
-            }
-          } else if (at < p.part_rows) {
-            *reinterpret_cast<float4*>(part_o + (size_t)at * D + c0 + c * 4) = x;
-          }
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-      }
+      unsigned char* merge = smem + L::MERGE_AT;
+      if (WIDE && sets == 8)
+        leave<8>(p, r, good, G, RT, ml_s, merge, tmem, warp, lane);
+      else if (sets == 4)
+        leave<4>(p, r, good, G, RT, ml_s, merge, tmem, warp, lane);
+      else if (sets == 2)
+        leave<2>(p, r, good, G, RT, ml_s, merge, tmem, warp, lane);
+      else
+        leave<1>(p, r, good, G, RT, ml_s, merge, tmem, warp, lane);
+      release();
+      fence_before();
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // (nobody reads an accumulator when the next piece's products go there)
+      fence_after();
     }
   }
 
@@ -736,52 +829,57 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
   }
 }
 
-// The parts of a group that fell to several CTAs: o = sum 2^(m - M) o_part / (sum 2^(m - M) l + 2^(sink - M)), the CTAs in their order.  A warp per row.
+// The parts of a group that fell to several CTAs: o = sum 2^(m - M) o_part / (sum 2^(m - M) l + 2^(sink - M)), the CTAs in their order.  A CTA for 32
+// places of a group, a lane per place, a warp per 4 columns in turn.
 template <bool WIDE>
 __global__ void __launch_bounds__(256) join_tree_parts_kernel(const Params p) {
   ts_pdl_prologue();
-  constexpr int VEC = D / 32;
-  const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5), hk = blockIdx.y, b = blockIdx.z;
+  constexpr int VEC = D / 32;  // pieces of 4 columns per warp
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hk = blockIdx.y, b = blockIdx.z;
   const int G = p.nq / p.nkv, RT = BM / G * G, RG = WIDE ? 2 * RT : RT;
-  if (row >= (p.cu[b + 1] - p.cu[b]) * G) return;
+  const int per_group = p.part_rows / 32, g = blockIdx.x / per_group, place = blockIdx.x % per_group * 32 + lane;
+  if (p.cu[b + 1] - p.cu[b] <= 0) return;
   const Request r = request_of<WIDE>(p, b, RT);
-  const int g = row / RG, cost = cost_of<WIDE>(r, g, RT), share = p.plan[p.num_seqs + 1];
+  if (g >= r.groups) return;
+  const int cost = cost_of<WIDE>(r, g, RT), share = p.plan[p.num_seqs];
   const int at = p.plan[b] + hk * cost_of_head<WIDE>(r, RT) + g * r.blocks * (WIDE ? COST_TWO : COST_ONE);
   const int c0 = at / share, c1 = (at + (r.blocks - 1) * cost) / share;
   if (c0 == c1) return;  // (its CTA has written it)
-  const int in = row - g * RG, place = in < RT ? in : BM + in - RT;
-  if (place >= p.part_rows) return;
+  const int in_tile = place % BM, in = place / BM * RT + in_tile, row = g * RG + in;
+  if (in_tile >= RT || in >= RG || row >= r.rows) return;
   const int head = hk * G + row % G;
   float top = p.head_sinks ? p.head_sinks[head] * LOG2E : -INFINITY;
   const float sink = top;
-  auto part = [&](int c) -> size_t {  // where CTA c left its part of the row; it has one: share >= cost, or a block of it begins there
-    return ((size_t)c * 2 + (at <= c * share ? 0 : 1)) * p.part_rows + place;
-  };
-  auto has = [&](int c) {
+  auto part = [&](int c) -> size_t { return ((size_t)c * 2 + (at <= c * share ? 0 : 1)) * p.part_rows; };  // where CTA c left its part
+  auto has = [&](int c) {  // (a share smaller than a block's cost may hold no block's beginning)
     const int from = c * share;
     return (from > at ? (from - at + cost - 1) / cost : 0) < min(r.blocks, (from + share - at + cost - 1) / cost);
   };
-  for (int c = c0 + lane; c <= c1; c += 32)
-    if (has(c)) top = fmaxf(top, p.part_ml[2 * part(c)]);
-  top = ts_warp_max(top);
-  float total = sink == -INFINITY ? 0.f : fast_exp2(sink - top), o[VEC];
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c)
+    if (has(c)) top = fmaxf(top, p.part_ml[2 * (part(c) + place)]);
+  float total = sink == -INFINITY ? 0.f : fast_exp2(sink - top);
+  float4 o[VEC];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) o[i] = 0.f;
+  for (int i = 0; i < VEC; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
   for (int c = c0; c <= c1; ++c) {
     if (!has(c)) continue;
     const size_t x = part(c);
-    const float m = p.part_ml[2 * x];
-    if (m == -INFINITY) continue;
-    const float f = fast_exp2(m - top);
-    total += f * p.part_ml[2 * x + 1];
-    const float* from = p.part_o + x * D + lane * VEC;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (x + place));
+    const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+    total += f * ml.y;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i] = fmaf(f, from[i], o[i]);
+    for (int i = 0; i < VEC; ++i) {
+      const float4 y = *reinterpret_cast<const float4*>(p.part_o + x * D + ((size_t)(warp + 8 * i) * p.part_rows + place) * 4);
+      o[i].x = fmaf(f, y.x, o[i].x), o[i].y = fmaf(f, y.y, o[i].y), o[i].z = fmaf(f, y.z, o[i].z), o[i].w = fmaf(f, y.w, o[i].w);
+    }
   }
   const float inv = total > 0.f ? 1.f / total : 0.f;
-  __nv_bfloat16* out = p.out + ((size_t)(r.q_begin + row / G) * p.nq + head) * D + lane * VEC;
+  __nv_bfloat16* out = p.out + ((size_t)(r.q_begin + row / G) * p.nq + head) * D;
 #pragma unroll
-  for (int i = 0; i < VEC; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack_bf16(o[i] * inv, o[i + 1] * inv);
+  for (int i = 0; i < VEC; ++i)
+    *reinterpret_cast<uint2*>(out + (warp + 8 * i) * 4) = make_uint2(pack_bf16(o[i].x * inv, o[i].y * inv), pack_bf16(o[i].z * inv, o[i].w * inv));
 }
 
 // q [T, nq, D] as a 4-d tensor {D, G, nkv, T}; boxes of {64, G, 1, tokens}: the rows of a box come out ordered (token, head of the group).
@@ -818,14 +916,15 @@ int launch(const CUtensorMap* maps, const Params& p, int max_t, cudaStream_t str
   if (e != cudaSuccess) return (int)e;
   const int status = ts_launch(attention_tree_kernel<WIDE, CAP>, dim3(p.ctas), dim3(THREADS), smem, stream, maps[0], maps[1], maps[2], maps[3], maps[4], p);
   if (status != 0) return status;
-  return ts_launch(join_tree_parts_kernel<WIDE>, dim3((max_t * (p.nq / p.nkv) + 7) / 8, p.nkv, p.num_seqs), dim3(256), 0, stream, p);
+  const int G = p.nq / p.nkv, RG = BM / G * G * (WIDE ? 2 : 1), groups = (max_t * G + RG - 1) / RG;
+  return ts_launch(join_tree_parts_kernel<WIDE>, dim3(groups * (p.part_rows / 32), p.nkv, p.num_seqs), dim3(256), 0, stream, p);
 }
 
 }  // namespace
 
 // Whether these kernels take the sizes (the CUDA-core kernel takes all).
 TS_EXPORT int ts_attention_tree_tcgen05_takes(int B, int max_t, int max_context, int nq, int nkv, int page, long long num_pages, float scale) {
-  if (nkv <= 0 || nq % nkv || nq / nkv > BM || B > MAX_SEQS || max_t > MAX_NODES || nkv > 65535 || !(scale > 0.f)) return 0;
+  if (nkv <= 0 || nq % nkv || nq / nkv > BM || B > 65535 || max_t > MAX_NODES || nkv > 65535 || !(scale > 0.f)) return 0;
   if (page < 8 || !(BN % page == 0 || page % BN == 0) || num_pages * page > 0x7fffffffLL - page) return 0;
   const long long rows = (long long)max_t * (nq / nkv), groups = rows / (BM / (nq / nkv) * (nq / nkv)) + 1;
   return (long long)B * nkv * groups * COST_TWO * ((max_context + BN - 1) / BN + 1) < (1ll << 30) ? 1 : 0;  // places of the plan fit 32 bits

@@ -33,7 +33,7 @@ constexpr uint32_t TILE = HALVES * ATOM;         // Q of a tile, K or V of a blo
 constexpr int CH = 16;                           // columns of the result that pass from the lanes that hold them to whole lines at a time
 constexpr uint32_t MERGE = 8 * 32 * CH * 4;       // a half of the columns each for two times four warps
 constexpr int MAX_NODES = 256;
-constexpr int THREADS = 384;                     // eight warps of softmax; one that copies K, one that issues products, one that copies Q and V, one that plans
+constexpr int THREADS = 384;                     // eight warps of softmax, three that copy (the last also plans), one that issues products
 constexpr int AHEAD = 4;                         // pieces of work that are planned ahead
 constexpr uint32_t SPIN_LIMIT = 1u << 22;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -318,26 +318,6 @@ struct Walk {
   }
 };
 
-// The planning warp: pieces into a ring, in whose places the other warps find them.  (A function of its own: what it holds need not stay in registers elsewhere.)
-template <bool WIDE>
-__device__ __noinline__ void plan(const Params& p, int RT, Piece* ring, uint32_t full, uint32_t empty, volatile int* abort_flag) {
-  Walk<WIDE> walk;
-  Piece piece;
-  walk.begin(p, RT, blockIdx.x == 0);
-  bool more = true;
-#pragma unroll 1
-  for (int i = 0; more; ++i) {
-    more = walk.next(p, RT, piece);
-    const int at = i % AHEAD;
-    if (i >= AHEAD && !__all_sync(0xffffffffu, mbar_wait(empty + 8 * at, (uint32_t)(i / AHEAD - 1) & 1, abort_flag))) break;
-    if ((threadIdx.x & 31) == 0) {
-      ring[at] = piece;
-      mbar_arrive(full + 8 * at);
-    }
-    __syncwarp();
-  }
-}
-
 // Which of the 32 keys from `base` on a node sees, as bits.
 __device__ __noinline__ uint32_t seen_bits(const Params& p, int q_begin, int t, int n, int token, int pos, int base) {
   const int first = n - t;
@@ -549,6 +529,11 @@ __device__ __noinline__ void leave(const Params& p, const Piece& w, bool good, i
   }
 }
 
+template <int X>
+struct Const {
+  static constexpr int value = X;
+};
+
 template <bool WIDE, bool CAP>
 __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid_constant__ CUtensorMap map_q1, const __grid_constant__ CUtensorMap map_q2,
                                                                     const __grid_constant__ CUtensorMap map_q4, const __grid_constant__ CUtensorMap map_k,
@@ -579,7 +564,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
     mbar_init(smem_u32(&q_full), 1);
     mbar_init(smem_u32(&q_empty), 1);
     mbar_init(smem_u32(&all_done), 1);
-    for (int s = 0; s < AHEAD; ++s) mbar_init(smem_u32(&piece_full[s]), 1), mbar_init(smem_u32(&piece_empty[s]), 11);
+    for (int s = 0; s < AHEAD; ++s) mbar_init(smem_u32(&piece_full[s]), 1), mbar_init(smem_u32(&piece_empty[s]), THREADS / 32);
     for (int s = 0; s < NK; ++s) mbar_init(smem_u32(&k_full[s]), 1), mbar_init(smem_u32(&k_empty[s]), 1);
     for (int s = 0; s < NV; ++s) mbar_init(smem_u32(&v_full[s]), 1), mbar_init(smem_u32(&v_empty[s]), 1);
     for (int t = 0; t < 2; ++t) mbar_init(smem_u32(&s_full[t]), 1), mbar_init(smem_u32(&p_full[t]), 4), mbar_init(smem_u32(&o_full[t]), 1);
@@ -596,7 +581,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
   ts_pdl_launch_dependents();
   const uint32_t tmem = tmem_base_s, sm = smem_u32(smem);
   volatile int* abort_flag = &abort_s;
-  // The next piece of work, for every warp but the one that plans, which reads it where it stands and gives the place back when it is done; false: a wait gave up.
+  // The next piece of work, read where it stands; a warp gives the place back when it is done with it.  false: a wait gave up.
   int pieces = 0;
   auto fetch = [&]() -> bool { return mbar_wait(smem_u32(&piece_full[pieces % AHEAD]), (uint32_t)(pieces / AHEAD) & 1, abort_flag); };
   auto release = [&]() {
@@ -605,134 +590,176 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
     ++pieces;
   };
 
-  if (warp == 11) {
-    // ---------------- plan ----------------
-    plan<WIDE>(p, RT, piece_s, smem_u32(piece_full), smem_u32(piece_empty), abort_flag);
-  } else if (warp == 8 || warp == 10) {
-    // ---------------- copies: K, and Q and V ----------------
-    const bool keys = warp == 8;
-    const int box_rows = min(p.page, BN), copies = BN / box_rows;
-    const int c = lane / HALVES, half = lane % HALVES;  // this lane's box of a block (at most 16 a half: pages of 8)
-    const int stages = keys ? NK : NV;
-    uint64_t* full = keys ? k_full : v_full;
-    uint64_t* empty = keys ? k_empty : v_empty;
-    const uint32_t to_smem = sm + (keys ? L::K : L::V) + half * ATOM + c * box_rows * 128;
-    int count = 0, qc = 0;
+  if (warp == 8 || warp >= 10) {
+    // ---------------- copies ----------------
+    // Asking for a box of 2 KB (half a head's rows of a page of 16) takes a warp 75 cycles and the copy engine under 50: three warps share every block's boxes.
+    const int copier = warp == 8 ? 0 : warp - 9;
+    const int box_rows = min(p.page, BN), boxes = BN / box_rows * HALVES;
+    const int mine = copier + 3 * lane;  // this lane's box of a block, if it has one (11 lanes a warp at most: 32 boxes)
+    const bool copies = mine < boxes;
+    const int c = mine / HALVES, half = mine % HALVES;
+    const uint32_t in_tile = half * ATOM + c * box_rows * 128;
+    int kc = 0, vc = 0, qc = 0;
     bool ok = true;
+    // The last of them plans: pieces into a ring, some ahead of the one it copies for.
+    Walk<WIDE> walk;
+    int planned = 0;
+    bool more = copier == 2;
+    if (copier == 2) walk.begin(p, RT, blockIdx.x == 0);
+    auto plan = [&](int until) {
+#pragma unroll 1
+      while (more && planned < until) {
+        Piece piece;
+        more = walk.next(p, RT, piece);
+        const int at = planned % AHEAD;
+        if (planned >= AHEAD && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&piece_empty[at]), (uint32_t)(planned / AHEAD - 1) & 1, abort_flag))) more = false;
+        else if (lane == 0) {
+          piece_s[at] = piece;
+          mbar_arrive(smem_u32(&piece_full[at]));
+        }
+        __syncwarp();
+        ++planned;
+      }
+    };
     // The page of this lane's box of a block, -1 where it has none: asked for two blocks ahead, looked at when its turn comes.
     auto page_of = [&](const Piece& r, const int* table, int kb) -> int {
       const int key = kb * BN + c * box_rows, e = key / p.page;
       int page = -1;
-      if (c < copies && key < r.n && e < p.max_blocks) page = __ldg(table + e);
+      if (copies && key < r.n && e < p.max_blocks) page = __ldg(table + e);
       return page;
     };
+    // beyond the end: the copy engine fills zeros
+    auto slot_of = [&](int page, int kb) -> int {
+      return page < 0 ? p.total_slots : (int)min((long long)page * p.page + (kb * BN + c * box_rows) % p.page, (long long)p.total_slots);
+    };
+    auto load = [&](bool keys, int slot, int hk) {
+      int& count = keys ? kc : vc;
+      const int stages = keys ? NK : NV, st = count % stages, use = count / stages;
+      const uint32_t full = smem_u32(keys ? &k_full[st] : &v_full[st]), empty = smem_u32(keys ? &k_empty[st] : &v_empty[st]);
+      if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty, (uint32_t)(use - 1) & 1, abort_flag));
+      if (!ok) return;
+      if (copier == 0 && lane == 0) mbar_expect_tx(full, TILE);  // (bytes that land before count too: the phase waits for this arrival)
+      __syncwarp();
+      if (copies) tma_load_3d(sm + (keys ? L::K : L::V) + st * TILE + in_tile, keys ? &map_k : &map_v, full, half * 64, hk, slot);
+      ++count;
+    };
+    plan(1);
     while (ok) {
       ok = __all_sync(0xffffffffu, fetch());
       const Piece r = piece_s[pieces % AHEAD];
       release();
       if (!ok || r.nb == 0) break;
       const int* table = p.table + (size_t)r.b * p.max_blocks;
-      int page = page_of(r, table, r.kb), ahead = r.nb > 1 ? page_of(r, table, r.kb + 1) : -1;
-      if (!keys) {
+      int page = page_of(r, table, r.kb), ahead = r.nb > 1 ? page_of(r, table, r.kb + 1) : -1, behind = 0;
+      if (copier == 1) {
         if (qc > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_empty), (uint32_t)(qc - 1) & 1, abort_flag));
-        if (!ok) break;
-        if (lane == 0) {
+        if (ok && lane == 0) {
           // the queries: one or two tiles, or one tile's in two or four copies
-          const int boxes = r.sets == 8 ? 2 : 4 / r.sets, box = r.sets >= 4 ? BM / G : r.sets == 2 ? 64 / G : 32 / G;
-          mbar_expect_tx(smem_u32(&q_full), (uint32_t)(boxes * HALVES * box * G * 128));
+          const int tiles = r.sets == 8 ? 2 : 4 / r.sets, box = r.sets >= 4 ? BM / G : r.sets == 2 ? 64 / G : 32 / G;
+          mbar_expect_tx(smem_u32(&q_full), (uint32_t)(tiles * HALVES * box * G * 128));
 #pragma unroll 1
-          for (int i = 0; i < boxes * HALVES; ++i) {
+          for (int i = 0; i < tiles * HALVES; ++i) {
             const int x = i / HALVES, h = i % HALVES;
             tma_load_4d(sm + L::Q + (r.sets == 8 ? x * TILE : x * r.sets * 32 * 128) + h * ATOM, r.sets >= 4 ? &map_q1 : r.sets == 2 ? &map_q2 : &map_q4, smem_u32(&q_full), h * 64,
                         0, r.hk, r.q_begin + (r.r0 + (r.sets == 8 ? x * RT : 0)) / G);
           }
         }
+        __syncwarp();
         ++qc;
       }
 #pragma unroll 1
-      for (int s = 0; s < r.nb; ++s) {
-        const int after = s + 2 < r.nb ? page_of(r, table, r.kb + s + 2) : -1;
-        const int st = count % stages, use = count / stages;
-        if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[st]), (uint32_t)(use - 1) & 1, abort_flag));
-        if (!ok) break;
-        if (lane == 0) mbar_expect_tx(smem_u32(&full[st]), TILE);
-        __syncwarp();
-        // (beyond the end: the copy engine fills zeros)
-        const int slot = page < 0 ? p.total_slots : (int)min((long long)page * p.page + ((r.kb + s) * BN + c * box_rows) % p.page, (long long)p.total_slots);
-        if (c < copies) tma_load_3d(to_smem + st * TILE, keys ? &map_k : &map_v, smem_u32(&full[st]), half * 64, r.hk, slot);
-        ++count;
-        page = ahead, ahead = after;
+      for (int s = 0; ok && s <= r.nb; ++s) {  // K of block s, V of the one before: the order in which the products need them
+        const int after = s + 2 < r.nb ? page_of(r, table, r.kb + s + 2) : -1, slot = slot_of(page, r.kb + s);
+        if (s < r.nb) load(true, slot, r.hk);
+        if (ok && s > 0) load(false, behind, r.hk);
+        if (s == 0) plan(pieces + AHEAD - 2);  // (places that the rows of the piece before the last have left: nobody waits for a copy that this warp has not asked for)
+        behind = slot, page = ahead, ahead = after;
       }
     }
     if (*abort_flag) {
       // leave nothing in flight: wait (bounded, on a count of its own) for the copies already asked for
       int patience = 0;
       volatile int* own = &patience;
-      for (int i = max(0, count - stages); i < count; ++i) mbar_wait(smem_u32(&full[i % stages]), (uint32_t)(i / stages) & 1, own);
+#pragma unroll 1
+      for (int i = max(0, kc - NK); i < kc; ++i) mbar_wait(smem_u32(&k_full[i % NK]), (uint32_t)(i / NK) & 1, own);
+#pragma unroll 1
+      for (int i = max(0, vc - NV); i < vc; ++i) mbar_wait(smem_u32(&v_full[i % NV]), (uint32_t)(i / NV) & 1, own);
       if (qc > 0) mbar_wait(smem_u32(&q_full), (uint32_t)(qc - 1) & 1, own);
     }
   } else if (warp == 9) {
-    // ---------------- products: the warp runs together, one elected lane issues (a lane by itself takes 100 cycles for an instruction, not 57) ----------------
+    // ---------------- products: the warp runs together, one elected lane issues ----------------
     // Items of a piece: tile i & 1, block i >> 1 for two tiles of rows, i where one tile's blocks alternate.  S of item i + 2 goes where S and P of item i lay: the
     // tensor core runs what one thread issues in order, so P V of item i has read P before.
-    int kc = 0, vc = 0, qc = 0, pc[2] = {0, 0};
+    // An instruction's operands stand in uniform registers: with stages and tiles known when compiling (a switch over them) it takes a fraction of the 75 cycles that
+    // operands from ordinary registers cost.  (The whole tensor memory is this CTA's, so it begins at 0.)
+    int ks = 0, vs = 0, qc = 0;               // stages of K and V that come next
+    uint32_t kp = 0, vp = 0, pp0 = 0, pp1 = 0;  // and the phases that are waited for
     bool ok = true;
-    const uint64_t q_desc = desc_k_major(sm + L::Q), k_desc = desc_k_major(sm + L::K), v_desc = desc_mn_major(sm + L::V);
+    auto issue_pv = [&](auto stage, auto tile, bool more) {
+      constexpr int ST = decltype(stage)::value, T = decltype(tile)::value;
+      const uint64_t vd = desc_mn_major(sm + L::V + ST * TILE);
+      constexpr uint32_t to = 256 + T * D, from_p = T * 128;
+      umma_tmem_a(to, from_p, vd, idesc(D, true), more);
+#pragma unroll
+      for (int kk = 1; kk < BN / 16; ++kk) umma_tmem_a_more(to, from_p + kk * 8, vd + ((kk * 2048) >> 4), idesc(D, true));
+    };
+    auto issue_s = [&](auto stage, auto tile, bool second_q) {
+      constexpr int ST = decltype(stage)::value, T = decltype(tile)::value;
+      const uint64_t kd = desc_k_major(sm + L::K + ST * TILE), qd = desc_k_major(sm + L::Q) + (uint64_t)(WIDE && T && second_q ? TILE >> 4 : 0);
+      umma_first(T * 128, qd, kd, idesc(BN, false));
+#pragma unroll
+      for (int x = 1; x < D / 16; ++x) {
+        const uint32_t off = ((x >> 2) * ATOM + (x & 3) * 32) >> 4;
+        umma_more(T * 128, qd + off, kd + off, idesc(BN, false));
+      }
+    };
     while (ok) {
       ok = __all_sync(0xffffffffu, fetch());
-      const Piece r = piece_s[pieces % AHEAD];
+      const bool two = WIDE && piece_s[pieces % AHEAD].sets == 8;
+      const int nb = piece_s[pieces % AHEAD].nb, items = two ? 2 * nb : nb;
       release();
-      if (!ok || r.nb == 0) break;
-      const bool two = WIDE && r.sets == 8;
-      const int nb = r.nb, items = two ? 2 * nb : nb;
+      if (!ok || nb == 0) break;
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_full), (uint32_t)qc & 1, abort_flag));
-      if (!ok) break;
 #pragma unroll 1
-      for (int i = 0; i < items + 2; ++i) {
+      for (int i = 0; ok && i < items + 2; ++i) {
+        const int t = i & 1;
         if (i >= 2) {  // P V of item i - 2, once its weights and (for the first of two tiles) V are there
-          const int j = i - 2, blk = two ? j >> 1 : j, st = (vc + blk) % NV, t = j & 1;
           bool there = true;
-          if (!two || t == 0) there = mbar_wait(smem_u32(&v_full[st]), (uint32_t)((vc + blk) / NV) & 1, abort_flag);
-          there = there && mbar_wait(smem_u32(&p_full[t]), (uint32_t)pc[t] & 1, abort_flag);
+          if (!two || t == 0) there = mbar_wait(smem_u32(&v_full[vs]), vp, abort_flag);
+          there = there && mbar_wait(smem_u32(&p_full[t]), t ? pp1 : pp0, abort_flag);
           ok = __all_sync(0xffffffffu, there);
           if (!ok) break;
-          ++pc[t];
           fence_after();
           if (elect_one()) {
-            const uint64_t vd = v_desc + (uint64_t)((st * TILE) >> 4);
-            const uint32_t to = tmem + 256 + t * D, from_p = tmem + t * 128;
-            umma_tmem_a(to, from_p, vd, idesc(D, true), j >= 2);
-#pragma unroll
-            for (int kk = 1; kk < BN / 16; ++kk) umma_tmem_a_more(to, from_p + kk * 8, vd + ((kk * 2048) >> 4), idesc(D, true));
-            if (!two || t == 1) umma_commit(smem_u32(&v_empty[st]));
-            if (j >= items - 2) umma_commit(smem_u32(&o_full[t]));
+            switch (vs * 2 + t) {
+#define PV_CASE(x) case x: if constexpr (x / 2 < NV) issue_pv(Const<x / 2>(), Const<x % 2>(), i >= 4); break;
+              PV_CASE(0) PV_CASE(1) PV_CASE(2) PV_CASE(3) PV_CASE(4) PV_CASE(5) PV_CASE(6) PV_CASE(7)
+            }
+            if (!two || t == 1) umma_commit(smem_u32(&v_empty[vs]));
+            if (i >= items) umma_commit(smem_u32(&o_full[t]));
             if (items == 1) umma_commit(smem_u32(&o_full[1]));  // (a tile without items: its accumulator is not read)
           }
           __syncwarp();
+          if (t) pp1 ^= 1; else pp0 ^= 1;
+          if ((!two || t == 1) && ++vs == NV) vs = 0, vp ^= 1;
         }
         if (i < items) {  // S of item i, once its K is there (of two tiles the second finds it there)
-          const int blk = two ? i >> 1 : i, st = (kc + blk) % NK, t = i & 1;
-          if (!two || t == 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[st]), (uint32_t)((kc + blk) / NK) & 1, abort_flag));
-            if (!ok) break;
-          }
+          if (!two || t == 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[ks]), kp, abort_flag));
+          if (!ok) break;
           if (elect_one()) {
-            const uint64_t kd = k_desc + (uint64_t)((st * TILE) >> 4), qd = q_desc + (uint64_t)(two && t ? TILE >> 4 : 0);
-            const uint32_t to = tmem + t * 128;
-            umma_first(to, qd, kd, idesc(BN, false));
-#pragma unroll
-            for (int ks = 1; ks < D / 16; ++ks) {
-              const uint32_t off = ((ks >> 2) * ATOM + (ks & 3) * 32) >> 4;
-              umma_more(to, qd + off, kd + off, idesc(BN, false));
+            switch (ks * 2 + t) {
+#define S_CASE(x) case x: if constexpr (x / 2 < NK) issue_s(Const<x / 2>(), Const<x % 2>(), two); break;
+              S_CASE(0) S_CASE(1) S_CASE(2) S_CASE(3) S_CASE(4) S_CASE(5) S_CASE(6) S_CASE(7)
             }
             umma_commit(smem_u32(&s_full[t]));
-            if (!two || t == 1) umma_commit(smem_u32(&k_empty[st]));
+            if (!two || t == 1) umma_commit(smem_u32(&k_empty[ks]));
             if (i == items - 1) umma_commit(smem_u32(&q_empty));
           }
           __syncwarp();
+          if ((!two || t == 1) && ++ks == NK) ks = 0, kp ^= 1;
         }
       }
-      kc += nb, vc += nb, ++qc;
+      ++qc;
     }
     // Everything this CTA asked of the tensor core is done when this arrives, the arrivals of the commits above included: nobody leaves before.
     if (elect_one()) umma_commit(smem_u32(&all_done));

@@ -33,7 +33,7 @@ constexpr uint32_t TILE = HALVES * ATOM;         // Q of a tile, K or V of a blo
 constexpr int CH = 16;                           // columns of the result that pass from the lanes that hold them to whole lines at a time
 constexpr uint32_t MERGE = 8 * 32 * CH * 4;       // a half of the columns each for two times four warps
 constexpr int MAX_NODES = 256;
-constexpr int THREADS = 384;                     // eight warps of softmax, three that copy (the last also plans), one that issues products
+constexpr int THREADS = 384;                     // eight warps of softmax, two that copy (the second also plans), two that issue products
 constexpr int AHEAD = 4;                         // pieces of work that are planned ahead
 constexpr uint32_t SPIN_LIMIT = 1u << 22;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -144,16 +144,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
@@ -374,37 +364,39 @@ __device__ __forceinline__ float weights(const uint32_t (&v)[32], uint32_t (&w)[
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
+// cap * tanh(x), in units of log2: tanh(x) = 1 - 2 / (exp(2x) + 1), exact at both ends, absolute error of a few 1e-7 in between.
+__device__ __forceinline__ void bend(const Params& p, uint32_t (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(p.cap_log2 * (1.f - __fdividef(2.f, __expf(2.f * p.cap_inv * __uint_as_float(v[i])) + 1.f)));
+}
+
 // One block's weights for one warp's 32 rows: 32 N keys from column `key0` of the block on.  Scores come from `s_addr` (the tile's columns at this warp's lanes); the
-// weights of all 128 keys go over them as bfloat16, zeros for keys that are other copies' part.  Two walks over the scores, 32 at a time and the next 32 on their way:
-// for the largest, and for the weights (kept in registers in between they would spill what the loop around holds).
+// weights of all 128 keys go over them as bfloat16, zeros for keys that are other copies' part.  Of 128 keys the second 64 are kept between the look for the
+// largest and the weights, and the first are read again: all would not fit the registers.
 template <int N, bool CAP>
 __device__ __forceinline__ void weigh(const Params& p, const Piece& r, int token, int pos, int kbase, int key0, bool open, uint32_t s_addr, uint32_t o_addr, bool first_item,
                                       float scale, float& m_run, float& l_run) {
-  uint32_t v[2][32], w[16], bits[N];
+  constexpr int H = N < 2 ? N : 2;  // 32s of keys that are held
+  uint32_t v[H][32], bits[N];
   if (!open) {
 #pragma unroll
     for (int c = 0; c < N; ++c) bits[c] = token >= 0 ? seen_bits(p, r.q_begin, r.t, r.n, token, pos, kbase + key0 + 32 * c) : 0u;
   }
   float m_blk = -INFINITY;
-  tmem_ld32(s_addr + key0, v[0]);
 #pragma unroll
-  for (int c = 0; c < N; ++c) {
+  for (int c0 = 0; c0 < N; c0 += H) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) tmem_ld32(s_addr + key0 + 32 * (c0 + h), v[h]);
     tmem_ld_wait();
-    if (c + 1 < N) tmem_ld32(s_addr + key0 + 32 * (c + 1), v[(c + 1) & 1]);
-    if (CAP) {
-      // cap * tanh(x), in units of log2: tanh(x) = 1 - 2 / (exp(2x) + 1), exact at both ends, absolute error of a few 1e-7 in between; the second walk finds it in place
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        v[c & 1][i] = __float_as_uint(p.cap_log2 * (1.f - __fdividef(2.f, __expf(2.f * p.cap_inv * __uint_as_float(v[c & 1][i])) + 1.f)));
-      if (c + 1 < N) tmem_st32(s_addr + key0 + 32 * c, v[c & 1]);
+    for (int h = 0; h < H; ++h) {
+      if (CAP) bend(p, v[h]);
+      if (!open) hide(bits[c0 + h], v[h]);
+      m_blk = fmaxf(m_blk, largest(v[h]));
     }
-    if (!open) hide(bits[c], v[c & 1]);
-    m_blk = fmaxf(m_blk, largest(v[c & 1]));
   }
-  if (CAP && N > 1) tmem_st_wait();
-  if (N > 1) tmem_ld32(s_addr + key0, v[N & 1]);  // (the last 32 are kept, in v[(N - 1) & 1])
-  m_blk *= scale;                           // (scale > 0)
-  const bool raise = m_blk - m_run > LAG;   // also where m_run is -inf and m_blk is not
+  m_blk *= scale;                          // (scale > 0)
+  const bool raise = m_blk - m_run > LAG;  // also where m_run is -inf and m_blk is not
   if (__any_sync(0xffffffffu, raise)) {
     const float m_new = raise ? m_blk : m_run;
     const float corr = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
@@ -414,31 +406,41 @@ __device__ __forceinline__ void weigh(const Params& p, const Piece& r, int token
       // (the product before this one on the accumulator is complete: the scores, asked for behind it, are)
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {
-        tmem_ld16(o_addr + c, w);
+        uint32_t o[16];
+        tmem_ld16(o_addr + c, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * corr);
-        tmem_st16(o_addr + c, w);
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+        tmem_st16(o_addr + c, o);
       }
     }
   }
   const float off = m_run == -INFINITY ? 0.f : m_run;
-  uint32_t last[16];
-  l_run += weights(v[(N - 1) & 1], last, scale, off);
+  uint32_t w[H][16];
 #pragma unroll
-  for (int c = 0; c + 1 < N; ++c) {
+  for (int h = 0; h < H; ++h) l_run += weights(v[h], w[h], scale, off);
+  if (N == 4) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) tmem_ld32(s_addr + 32 * h, v[h]);
     tmem_ld_wait();
-    if (c + 2 < N) tmem_ld32(s_addr + key0 + 32 * (c + 1), v[(N + c + 1) & 1]);
-    if (!open) hide(bits[c], v[(N + c) & 1]);
-    l_run += weights(v[(N + c) & 1], w, scale, off);
-    tmem_st16(s_addr + key0 / 2 + 16 * c, w);  // (over scores that have been read: those of keys below 32 c + 32)
-  }
-  tmem_st16(s_addr + key0 / 2 + 16 * (N - 1), last);
-  if (N < 4) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = 0u;
+    for (int h = 0; h < 2; ++h) {  // (the kept ones' place is over scores that have been read by now)
+      tmem_st16(s_addr + 32 + 16 * h, w[h]);
+      if (CAP) bend(p, v[h]);
+      if (!open) hide(bits[h], v[h]);
+    }
 #pragma unroll
-    for (int c = 16 * N; c < 64; c += 16) tmem_st16(s_addr + (key0 / 2 ^ c), w);  // (key0 is a multiple of 32 N: the other multiples of 16)
+    for (int h = 0; h < 2; ++h) {
+      l_run += weights(v[h], w[h], scale, off);
+      tmem_st16(s_addr + 16 * h, w[h]);
+    }
+  } else {
+#pragma unroll
+    for (int h = 0; h < H; ++h) tmem_st16(s_addr + key0 / 2 + 16 * h, w[h]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[0][i] = 0u;
+#pragma unroll
+    for (int c = 16 * N; c < 64; c += 16) tmem_st16(s_addr + (key0 / 2 ^ c), w[0]);  // (key0 is a multiple of 32 N: the other multiples of 16)
   }
   tmem_st_wait();
 }
@@ -529,11 +531,6 @@ __device__ __noinline__ void leave(const Params& p, const Piece& w, bool good, i
   }
 }
 
-template <int X>
-struct Const {
-  static constexpr int value = X;
-};
-
 template <bool WIDE, bool CAP>
 __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid_constant__ CUtensorMap map_q1, const __grid_constant__ CUtensorMap map_q2,
                                                                     const __grid_constant__ CUtensorMap map_q4, const __grid_constant__ CUtensorMap map_k,
@@ -543,7 +540,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
   ts_pdl_wait();  // tensor memory is never held while waiting for another kernel
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[NK], k_empty[NK], v_full[NV], v_empty[NV], s_full[2], p_full[2], o_full[2], piece_full[AHEAD], piece_empty[AHEAD], all_done;
+  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[NK], k_empty[NK], v_full[NV], v_empty[NV], s_full[2], p_full[2], o_full[2], piece_full[AHEAD], piece_empty[AHEAD], all_done[2];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
   __shared__ float2 ml_s[8][32];
@@ -562,12 +559,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
   if (tid == 0) {
     abort_s = 0;
     mbar_init(smem_u32(&q_full), 1);
-    mbar_init(smem_u32(&q_empty), 1);
-    mbar_init(smem_u32(&all_done), 1);
+    mbar_init(smem_u32(&q_empty), 2);
     for (int s = 0; s < AHEAD; ++s) mbar_init(smem_u32(&piece_full[s]), 1), mbar_init(smem_u32(&piece_empty[s]), THREADS / 32);
-    for (int s = 0; s < NK; ++s) mbar_init(smem_u32(&k_full[s]), 1), mbar_init(smem_u32(&k_empty[s]), 1);
-    for (int s = 0; s < NV; ++s) mbar_init(smem_u32(&v_full[s]), 1), mbar_init(smem_u32(&v_empty[s]), 1);
-    for (int t = 0; t < 2; ++t) mbar_init(smem_u32(&s_full[t]), 1), mbar_init(smem_u32(&p_full[t]), 4), mbar_init(smem_u32(&o_full[t]), 1);
+    for (int s = 0; s < NK; ++s) mbar_init(smem_u32(&k_full[s]), 1), mbar_init(smem_u32(&k_empty[s]), 2);
+    for (int s = 0; s < NV; ++s) mbar_init(smem_u32(&v_full[s]), 1), mbar_init(smem_u32(&v_empty[s]), 2);
+    for (int t = 0; t < 2; ++t) mbar_init(smem_u32(&s_full[t]), 1), mbar_init(smem_u32(&p_full[t]), 4), mbar_init(smem_u32(&o_full[t]), 1), mbar_init(smem_u32(&all_done[t]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -590,12 +586,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
     ++pieces;
   };
 
-  if (warp == 8 || warp >= 10) {
+  if (warp == 8 || warp == 10) {
     // ---------------- copies ----------------
-    // Asking for a box of 2 KB (half a head's rows of a page of 16) takes a warp 75 cycles and the copy engine under 50: three warps share every block's boxes.
-    const int copier = warp == 8 ? 0 : warp - 9;
+    // Asking for a box of 2 KB (half a head's rows of a page of 16) takes a warp 75 cycles and the copy engine under 50: two warps share every block's boxes.
+    const int copier = warp == 8 ? 0 : 1;
     const int box_rows = min(p.page, BN), boxes = BN / box_rows * HALVES;
-    const int mine = copier + 3 * lane;  // this lane's box of a block, if it has one (11 lanes a warp at most: 32 boxes)
+    const int mine = copier + 2 * lane;  // this lane's box of a block, if it has one (16 lanes a warp at most: 32 boxes)
     const bool copies = mine < boxes;
     const int c = mine / HALVES, half = mine % HALVES;
     const uint32_t in_tile = half * ATOM + c * box_rows * 128;
@@ -604,8 +600,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
     // The last of them plans: pieces into a ring, some ahead of the one it copies for.
     Walk<WIDE> walk;
     int planned = 0;
-    bool more = copier == 2;
-    if (copier == 2) walk.begin(p, RT, blockIdx.x == 0);
+    bool more = copier == 1;
+    if (copier == 1) walk.begin(p, RT, blockIdx.x == 0);
     auto plan = [&](int until) {
 #pragma unroll 1
       while (more && planned < until) {
@@ -651,7 +647,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
       if (!ok || r.nb == 0) break;
       const int* table = p.table + (size_t)r.b * p.max_blocks;
       int page = page_of(r, table, r.kb), ahead = r.nb > 1 ? page_of(r, table, r.kb + 1) : -1, behind = 0;
-      if (copier == 1) {
+      if (copier == 0) {
         if (qc > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_empty), (uint32_t)(qc - 1) & 1, abort_flag));
         if (ok && lane == 0) {
           // the queries: one or two tiles, or one tile's in two or four copies
@@ -686,86 +682,78 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
       for (int i = max(0, vc - NV); i < vc; ++i) mbar_wait(smem_u32(&v_full[i % NV]), (uint32_t)(i / NV) & 1, own);
       if (qc > 0) mbar_wait(smem_u32(&q_full), (uint32_t)(qc - 1) & 1, own);
     }
-  } else if (warp == 9) {
-    // ---------------- products: the warp runs together, one elected lane issues ----------------
-    // Items of a piece: tile i & 1, block i >> 1 for two tiles of rows, i where one tile's blocks alternate.  S of item i + 2 goes where S and P of item i lay: the
-    // tensor core runs what one thread issues in order, so P V of item i has read P before.
-    // An instruction's operands stand in uniform registers: with stages and tiles known when compiling (a switch over them) it takes a fraction of the 75 cycles that
-    // operands from ordinary registers cost.  (The whole tensor memory is this CTA's, so it begins at 0.)
-    int ks = 0, vs = 0, qc = 0;               // stages of K and V that come next
-    uint32_t kp = 0, vp = 0, pp0 = 0, pp1 = 0;  // and the phases that are waited for
+  } else if (warp >= 8) {
+    // ---------------- products: a warp per tile, which runs together; one elected lane issues ----------------
+    // Items of a piece: tile t takes every block for its rows (two tiles of rows), or blocks t, t + 2, .. (one).  S of an item goes where S and P of the one before lay: the
+    // tensor core runs what one thread issues in order, so P V has read P before.  A warp's waits take it some 200 cycles each even where nothing is waited for, and
+    // an instruction as long as the tensor core needs for it: the two warps fill each other's gaps.
+    const int t = warp == 9 ? 0 : 1;
+    int kc = 0, qc = 0;        // blocks, pieces
+    uint32_t pp = 0;           // the phase of the weights that are waited for
     bool ok = true;
-    auto issue_pv = [&](auto stage, auto tile, bool more) {
-      constexpr int ST = decltype(stage)::value, T = decltype(tile)::value;
-      const uint64_t vd = desc_mn_major(sm + L::V + ST * TILE);
-      constexpr uint32_t to = 256 + T * D, from_p = T * 128;
-      umma_tmem_a(to, from_p, vd, idesc(D, true), more);
-#pragma unroll
-      for (int kk = 1; kk < BN / 16; ++kk) umma_tmem_a_more(to, from_p + kk * 8, vd + ((kk * 2048) >> 4), idesc(D, true));
-    };
-    auto issue_s = [&](auto stage, auto tile, bool second_q) {
-      constexpr int ST = decltype(stage)::value, T = decltype(tile)::value;
-      const uint64_t kd = desc_k_major(sm + L::K + ST * TILE), qd = desc_k_major(sm + L::Q) + (uint64_t)(WIDE && T && second_q ? TILE >> 4 : 0);
-      umma_first(T * 128, qd, kd, idesc(BN, false));
-#pragma unroll
-      for (int x = 1; x < D / 16; ++x) {
-        const uint32_t off = ((x >> 2) * ATOM + (x & 3) * 32) >> 4;
-        umma_more(T * 128, qd + off, kd + off, idesc(BN, false));
-      }
-    };
+    const uint64_t q_desc = desc_k_major(sm + L::Q), k_desc = desc_k_major(sm + L::K), v_desc = desc_mn_major(sm + L::V);
+    const uint32_t s_col = tmem + t * 128, o_col = tmem + 256 + t * D;
     while (ok) {
       ok = __all_sync(0xffffffffu, fetch());
-      const bool two = WIDE && piece_s[pieces % AHEAD].sets == 8;
-      const int nb = piece_s[pieces % AHEAD].nb, items = two ? 2 * nb : nb;
+      // (a reduction's result stands in a uniform register, and what is worked out from it: the operands of the products then need not be moved there one by one)
+      const bool two = WIDE && __reduce_or_sync(0xffffffffu, (unsigned)piece_s[pieces % AHEAD].sets) == 8;
+      const int nb = (int)__reduce_or_sync(0xffffffffu, (unsigned)piece_s[pieces % AHEAD].nb);
       release();
       if (!ok || nb == 0) break;
+      const int first = two ? 0 : t, step = two ? 1 : 2;
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_full), (uint32_t)qc & 1, abort_flag));
+      if (first >= nb) {  // nothing for this tile (and nobody waits for its accumulator: an arrival there could be the second before the first is looked at)
+        if (ok && elect_one()) mbar_arrive(smem_u32(&q_empty));
+        __syncwarp();
+      }
 #pragma unroll 1
-      for (int i = 0; ok && i < items + 2; ++i) {
-        const int t = i & 1;
-        if (i >= 2) {  // P V of item i - 2, once its weights and (for the first of two tiles) V are there
-          bool there = true;
-          if (!two || t == 0) there = mbar_wait(smem_u32(&v_full[vs]), vp, abort_flag);
-          there = there && mbar_wait(smem_u32(&p_full[t]), t ? pp1 : pp0, abort_flag);
+      for (int blk = first - step; ok && blk < nb; blk += step) {
+        if (blk >= 0) {  // P V of this block
+          const int st = (kc + blk) % NV;
+          const bool there = mbar_wait(smem_u32(&v_full[st]), (uint32_t)((kc + blk) / NV) & 1, abort_flag) && mbar_wait(smem_u32(&p_full[t]), pp, abort_flag);
           ok = __all_sync(0xffffffffu, there);
           if (!ok) break;
+          pp ^= 1;
           fence_after();
           if (elect_one()) {
-            switch (vs * 2 + t) {
-#define PV_CASE(x) case x: if constexpr (x / 2 < NV) issue_pv(Const<x / 2>(), Const<x % 2>(), i >= 4); break;
-              PV_CASE(0) PV_CASE(1) PV_CASE(2) PV_CASE(3) PV_CASE(4) PV_CASE(5) PV_CASE(6) PV_CASE(7)
-            }
-            if (!two || t == 1) umma_commit(smem_u32(&v_empty[vs]));
-            if (i >= items) umma_commit(smem_u32(&o_full[t]));
-            if (items == 1) umma_commit(smem_u32(&o_full[1]));  // (a tile without items: its accumulator is not read)
+            const uint64_t vd = v_desc + (uint64_t)((st * TILE) >> 4);
+            umma_tmem_a(o_col, s_col, vd, idesc(D, true), blk != first);
+#pragma unroll
+            for (int kk = 1; kk < BN / 16; ++kk) umma_tmem_a_more(o_col, s_col + kk * 8, vd + ((kk * 2048) >> 4), idesc(D, true));
+            umma_commit(smem_u32(&v_empty[st]));
+            if (!two) umma_commit(smem_u32(&v_empty[st]));  // (two arrivals give a stage back: of both tiles, or of the one that read it)
+            if (blk + step >= nb) umma_commit(smem_u32(&o_full[t]));
           }
           __syncwarp();
-          if (t) pp1 ^= 1; else pp0 ^= 1;
-          if ((!two || t == 1) && ++vs == NV) vs = 0, vp ^= 1;
         }
-        if (i < items) {  // S of item i, once its K is there (of two tiles the second finds it there)
-          if (!two || t == 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[ks]), kp, abort_flag));
+        const int next = blk + step;
+        if (next < nb) {  // S of the next
+          const int st = (kc + next) % NK;
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[st]), (uint32_t)((kc + next) / NK) & 1, abort_flag));
           if (!ok) break;
           if (elect_one()) {
-            switch (ks * 2 + t) {
-#define S_CASE(x) case x: if constexpr (x / 2 < NK) issue_s(Const<x / 2>(), Const<x % 2>(), two); break;
-              S_CASE(0) S_CASE(1) S_CASE(2) S_CASE(3) S_CASE(4) S_CASE(5) S_CASE(6) S_CASE(7)
+            const uint64_t kd = k_desc + (uint64_t)((st * TILE) >> 4), qd = q_desc + (uint64_t)(two && t ? TILE >> 4 : 0);
+            umma_first(s_col, qd, kd, idesc(BN, false));
+#pragma unroll
+            for (int x = 1; x < D / 16; ++x) {
+              const uint32_t off = ((x >> 2) * ATOM + (x & 3) * 32) >> 4;
+              umma_more(s_col, qd + off, kd + off, idesc(BN, false));
             }
             umma_commit(smem_u32(&s_full[t]));
-            if (!two || t == 1) umma_commit(smem_u32(&k_empty[ks]));
-            if (i == items - 1) umma_commit(smem_u32(&q_empty));
+            umma_commit(smem_u32(&k_empty[st]));
+            if (!two) umma_commit(smem_u32(&k_empty[st]));
+            if (next + step >= nb) umma_commit(smem_u32(&q_empty));
           }
           __syncwarp();
-          if ((!two || t == 1) && ++ks == NK) ks = 0, kp ^= 1;
         }
       }
-      ++qc;
+      kc += nb, ++qc;
     }
-    // Everything this CTA asked of the tensor core is done when this arrives, the arrivals of the commits above included: nobody leaves before.
-    if (elect_one()) umma_commit(smem_u32(&all_done));
+    // Everything this warp asked of the tensor core is done when this arrives, the arrivals of the commits above included: nobody leaves before.
+    if (elect_one()) umma_commit(smem_u32(&all_done[t]));
     __syncwarp();
     int patience = 0;
-    mbar_wait(smem_u32(&all_done), 0, &patience);
+    mbar_wait(smem_u32(&all_done[t]), 0, &patience);
     if (patience != 0) *abort_flag = 1;
   } else {
     // ---------------- softmax ----------------
@@ -774,7 +762,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t s_addr = tmem + lanes + t * 128, o_addr = tmem + lanes + 256 + t * D;
     const float scale = CAP ? 1.f : p.scale_log2;
-    int sc = 0, vc = 0, done = 0;
+    int sc = 0, vc = 0, done = 0, done1 = 0;
     for (;;) {
       uint32_t there = fetch();
       const Piece& r = piece_s[pieces % AHEAD];
@@ -824,7 +812,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
       vc += nb;
       // ---- the group's rows ----
       mbar_wait(smem_u32(&o_full[0]), (uint32_t)done & 1, abort_flag);
-      mbar_wait(smem_u32(&o_full[1]), (uint32_t)done & 1, abort_flag);
+      if (two || nb > 1) mbar_wait(smem_u32(&o_full[1]), (uint32_t)done1++ & 1, abort_flag);
       ++done;
       ml_s[warp][lane] = make_float2(m, l);
       __syncwarp();

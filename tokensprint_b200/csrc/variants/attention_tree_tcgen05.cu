@@ -33,13 +33,13 @@ constexpr uint32_t TILE = HALVES * ATOM;         // Q of a tile, K or V of a blo
 constexpr int CH = 16;                           // columns of the result that pass from the lanes that hold them to whole lines at a time
 constexpr uint32_t MERGE = 8 * 32 * CH * 4;       // a half of the columns each for two times four warps
 constexpr int MAX_NODES = 256;
-constexpr int THREADS = 384;                     // eight warps of softmax, two that copy (the second also plans), two that issue products
+constexpr int THREADS = 384;                     // eight warps of softmax, three that copy (the last also plans), one that issues products
 constexpr int AHEAD = 4;                         // pieces of work that are planned ahead
 constexpr uint32_t SPIN_LIMIT = 1u << 22;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LAG = 8.f;
 // What a block costs, in parts of a group of one tile's: shares are even in this measure.
-constexpr int COST_ONE = 2, COST_TWO = 3;
+constexpr int COST_ONE = 1, COST_TWO = 2;
 
 // Builds of the kernel: WIDE, for groups of up to two tiles of rows, else of one (K has a third stage where the second tile's Q would lie).
 template <bool WIDE>
@@ -59,7 +59,7 @@ struct Params {
   const float* head_sinks;  // [nq] or null
   float* part_o;          // [CTA, 2, part_rows, D]
   float* part_ml;         // [CTA, 2, part_rows, 2]
-  int* plan;              // [B] what stands before each request and, behind them, the share of a CTA: for the joining kernel
+  int4* plan;             // [CTA, 2] the group of rows whose first part is this CTA's, for the joining kernel: (first token, row, rows, KV head), (last CTA or 0, slot, -, -)
   int* error;
   int words, max_blocks, page, nq, nkv, window, num_seqs, total_slots, part_rows, ctas;
   float scale_log2, cap_log2, cap_inv;  // cap * log2(e) and scale / cap
@@ -213,6 +213,7 @@ struct __align__(16) Piece {
   int b, hk, q_begin, t;
   int n, kb, nb, r0;  // nb 0: no more pieces
   int rows, sets, whole, slot;
+  int last_cta, pad[3];   // where the group's last blocks fall
 };
 
 // How the rows of a piece lie in the tensor memory: `sets` sets of 32 rows in different warps (8: two tiles of rows; 4, 2, 1: one tile once, twice, four times, in
@@ -222,10 +223,10 @@ __device__ __forceinline__ int sets_of(int rows_of_group, int RT) { return rows_
 // Walks over the pieces of one CTA's share [from, to); the lanes of a warp walk together.
 template <bool WIDE>
 struct Walk {
-  int b, hk, g, from, to, at;  // at: where group (b, hk, g) begins
+  int b, hk, g, from, to, at, share;  // at: where group (b, hk, g) begins
   Request r;
   // The batch is added up by every warp for itself, 32 requests at a time: no memory, no barrier between.
-  __device__ __forceinline__ void begin(const Params& p, int RT, bool leave_plan) {
+  __device__ __forceinline__ void begin(const Params& p, int RT) {
     const int lane = threadIdx.x & 31;
     int total = 0;
     Request mine;
@@ -246,11 +247,9 @@ struct Walk {
 #pragma unroll 1
     for (int b0 = 0; b0 < p.num_seqs; b0 += 32) {
       scan(b0);
-      if (leave_plan && b0 + lane < p.num_seqs) p.plan[b0 + lane] = total + sum - cost;
       total += __shfl_sync(0xffffffffu, sum, 31);
     }
-    const int share = max(1, (total + p.ctas - 1) / p.ctas);
-    if (leave_plan && lane == 0) p.plan[p.num_seqs] = share;
+    share = max(COST_TWO, (total + p.ctas - 1) / p.ctas);  // (at least a block: every CTA between a group's first and last has a part of it)
     from = (int)min((long long)blockIdx.x * share, (long long)total);
     to = (int)min((long long)from + share, (long long)total);
     b = p.num_seqs, hk = g = 0, at = total;
@@ -298,7 +297,7 @@ struct Walk {
       const int blk0 = from > at ? (from - at + cost - 1) / cost : 0, blk1 = min(r.blocks, (to - at + cost - 1) / cost);
       const int RG = WIDE ? 2 * RT : RT, r0 = g * RG, rows = min(r.rows - r0, RG);
       // (a share has two groups in part at most, its first and its last: their places in scratch)
-      out = Piece{b, hk, r.q_begin, r.t, r.n, r.kb0 + blk0, blk1 - blk0, r0, rows, sets_of(rows, RT), blk0 == 0 && blk1 == r.blocks, at <= from ? 0 : 1};
+      out = Piece{b, hk, r.q_begin, r.t, r.n, r.kb0 + blk0, blk1 - blk0, r0, rows, sets_of(rows, RT), blk0 == 0 && blk1 == r.blocks, at <= from ? 0 : 1, (at + (r.blocks - 1) * cost) / share, {blk0, 0, 0}};
       at += r.blocks * cost;
       ++g;
       if (blk0 < blk1) return true;
@@ -352,16 +351,40 @@ __device__ __forceinline__ float largest(const uint32_t (&v)[32]) {
   for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
   return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
-// 32 scores to 16 pairs of weights; returns their sum.
+// two float32 in one 64-bit register, and the packed arithmetic on them
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 32 scores to 16 pairs of weights; returns their sum.  (With every fourth or second pair's exponentials on the FMA units instead of the special-function one:
+// 4 trees of 61 at 30,000 rows 222 -> 231, 258 us; what the weights wait for is tensor memory.)
 __device__ __forceinline__ float weights(const uint32_t (&v)[32], uint32_t (&w)[16], float scale, float off) {
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  const uint64_t scale2 = pack2(scale, scale), off2 = pack2(-off, -off);
+  uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-  for (int i = 0; i < 32; i += 2) {
-    const float a = fast_exp2(fmaf(__uint_as_float(v[i]), scale, -off)), b = fast_exp2(fmaf(__uint_as_float(v[i + 1]), scale, -off));
-    sum[i >> 1 & 3] += a + b;
-    w[i >> 1] = pack_bf16(a, b);
+  for (int i = 0; i < 16; ++i) {
+    const uint64_t x = fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, off2);
+    float a, b;
+    unpack2(x, a, b);
+    a = fast_exp2(a), b = fast_exp2(b);
+    sum[i & 3] = add2(sum[i & 3], pack2(a, b));
+    w[i] = pack_bf16(a, b);
   }
-  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  float a, b;
+  unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b);
+  return a + b;
 }
 
 // cap * tanh(x), in units of log2: tanh(x) = 1 - 2 / (exp(2x) + 1), exact at both ends, absolute error of a few 1e-7 in between.
@@ -540,7 +563,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
   ts_pdl_wait();  // tensor memory is never held while waiting for another kernel
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[NK], k_empty[NK], v_full[NV], v_empty[NV], s_full[2], p_full[2], o_full[2], piece_full[AHEAD], piece_empty[AHEAD], all_done[2];
+  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[NK], k_empty[NK], v_full[NV], v_empty[NV], s_full[2], p_full[2], o_full[2], piece_full[AHEAD], piece_empty[AHEAD], all_done;
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
   __shared__ float2 ml_s[8][32];
@@ -559,11 +582,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
   if (tid == 0) {
     abort_s = 0;
     mbar_init(smem_u32(&q_full), 1);
-    mbar_init(smem_u32(&q_empty), 2);
+    mbar_init(smem_u32(&q_empty), 1);
+    mbar_init(smem_u32(&all_done), 1);
     for (int s = 0; s < AHEAD; ++s) mbar_init(smem_u32(&piece_full[s]), 1), mbar_init(smem_u32(&piece_empty[s]), THREADS / 32);
-    for (int s = 0; s < NK; ++s) mbar_init(smem_u32(&k_full[s]), 1), mbar_init(smem_u32(&k_empty[s]), 2);
-    for (int s = 0; s < NV; ++s) mbar_init(smem_u32(&v_full[s]), 1), mbar_init(smem_u32(&v_empty[s]), 2);
-    for (int t = 0; t < 2; ++t) mbar_init(smem_u32(&s_full[t]), 1), mbar_init(smem_u32(&p_full[t]), 4), mbar_init(smem_u32(&o_full[t]), 1), mbar_init(smem_u32(&all_done[t]), 1);
+    for (int s = 0; s < NK; ++s) mbar_init(smem_u32(&k_full[s]), 1), mbar_init(smem_u32(&k_empty[s]), 1);
+    for (int s = 0; s < NV; ++s) mbar_init(smem_u32(&v_full[s]), 1), mbar_init(smem_u32(&v_empty[s]), 1);
+    for (int t = 0; t < 2; ++t) mbar_init(smem_u32(&s_full[t]), 1), mbar_init(smem_u32(&p_full[t]), 4), mbar_init(smem_u32(&o_full[t]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -586,12 +610,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
     ++pieces;
   };
 
-  if (warp == 8 || warp == 10) {
+  if (warp == 8 || warp >= 10) {
     // ---------------- copies ----------------
-    // Asking for a box of 2 KB (half a head's rows of a page of 16) takes a warp 75 cycles and the copy engine under 50: two warps share every block's boxes.
-    const int copier = warp == 8 ? 0 : 1;
+    // Asking for a box of 2 KB (half a head's rows of a page of 16) takes a warp 75 cycles and the copy engine under 50: three warps share every block's boxes.
+    const int copier = warp == 8 ? 0 : warp - 9;
     const int box_rows = min(p.page, BN), boxes = BN / box_rows * HALVES;
-    const int mine = copier + 2 * lane;  // this lane's box of a block, if it has one (16 lanes a warp at most: 32 boxes)
+    const int mine = copier + 3 * lane;  // this lane's box of a block, if it has one (11 lanes a warp at most: 32 boxes)
     const bool copies = mine < boxes;
     const int c = mine / HALVES, half = mine % HALVES;
     const uint32_t in_tile = half * ATOM + c * box_rows * 128;
@@ -600,8 +624,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
     // The last of them plans: pieces into a ring, some ahead of the one it copies for.
     Walk<WIDE> walk;
     int planned = 0;
-    bool more = copier == 1;
-    if (copier == 1) walk.begin(p, RT, blockIdx.x == 0);
+    bool more = copier == 2;
+    if (copier == 2) {
+      if (lane == 0) p.plan[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
+      walk.begin(p, RT);
+    }
     auto plan = [&](int until) {
 #pragma unroll 1
       while (more && planned < until) {
@@ -612,6 +639,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
         else if (lane == 0) {
           piece_s[at] = piece;
           mbar_arrive(smem_u32(&piece_full[at]));
+          if (piece.nb > 0 && !piece.whole && piece.pad[0] == 0) {
+            p.plan[2 * blockIdx.x] = make_int4(piece.q_begin, piece.r0, piece.rows, piece.hk);
+            p.plan[2 * blockIdx.x + 1] = make_int4(piece.last_cta, piece.slot, 0, 0);
+          }
         }
         __syncwarp();
         ++planned;
@@ -647,7 +678,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
       if (!ok || r.nb == 0) break;
       const int* table = p.table + (size_t)r.b * p.max_blocks;
       int page = page_of(r, table, r.kb), ahead = r.nb > 1 ? page_of(r, table, r.kb + 1) : -1, behind = 0;
-      if (copier == 0) {
+      if (copier == 1) {
         if (qc > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_empty), (uint32_t)(qc - 1) & 1, abort_flag));
         if (ok && lane == 0) {
           // the queries: one or two tiles, or one tile's in two or four copies
@@ -682,78 +713,75 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
       for (int i = max(0, vc - NV); i < vc; ++i) mbar_wait(smem_u32(&v_full[i % NV]), (uint32_t)(i / NV) & 1, own);
       if (qc > 0) mbar_wait(smem_u32(&q_full), (uint32_t)(qc - 1) & 1, own);
     }
-  } else if (warp >= 8) {
-    // ---------------- products: a warp per tile, which runs together; one elected lane issues ----------------
-    // Items of a piece: tile t takes every block for its rows (two tiles of rows), or blocks t, t + 2, .. (one).  S of an item goes where S and P of the one before lay: the
-    // tensor core runs what one thread issues in order, so P V has read P before.  A warp's waits take it some 200 cycles each even where nothing is waited for, and
-    // an instruction as long as the tensor core needs for it: the two warps fill each other's gaps.
-    const int t = warp == 9 ? 0 : 1;
-    int kc = 0, qc = 0;        // blocks, pieces
-    uint32_t pp = 0;           // the phase of the weights that are waited for
+  } else if (warp == 9) {
+    // ---------------- products: the warp runs together, one elected lane issues ----------------
+    // Items of a piece: tile i & 1, block i >> 1 for two tiles of rows, i where one tile's blocks alternate.  S of item i + 2 goes where S and P of item i lay: the
+    // tensor core runs what one thread issues in order, so P V of item i has read P before.  (Two warps, one a tile, end up in step: exponentials of both tiles at
+    // once and then products of both: 4 trees of 61 at 30,000 rows 330 us instead of the turns that one warp takes.)
+    int ks = 0, vs = 0, qc = 0;      // stages of K and V that come next
+    uint32_t kp = 0, vp = 0, pp = 0;   // and the phases that are waited for (of weights a bit per tile)
     bool ok = true;
     const uint64_t q_desc = desc_k_major(sm + L::Q), k_desc = desc_k_major(sm + L::K), v_desc = desc_mn_major(sm + L::V);
-    const uint32_t s_col = tmem + t * 128, o_col = tmem + 256 + t * D;
     while (ok) {
       ok = __all_sync(0xffffffffu, fetch());
       // (a reduction's result stands in a uniform register, and what is worked out from it: the operands of the products then need not be moved there one by one)
       const bool two = WIDE && __reduce_or_sync(0xffffffffu, (unsigned)piece_s[pieces % AHEAD].sets) == 8;
-      const int nb = (int)__reduce_or_sync(0xffffffffu, (unsigned)piece_s[pieces % AHEAD].nb);
+      const int nb = (int)__reduce_or_sync(0xffffffffu, (unsigned)piece_s[pieces % AHEAD].nb), items = two ? 2 * nb : nb;
       release();
       if (!ok || nb == 0) break;
-      const int first = two ? 0 : t, step = two ? 1 : 2;
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_full), (uint32_t)qc & 1, abort_flag));
-      if (first >= nb) {  // nothing for this tile (and nobody waits for its accumulator: an arrival there could be the second before the first is looked at)
-        if (ok && elect_one()) mbar_arrive(smem_u32(&q_empty));
-        __syncwarp();
-      }
 #pragma unroll 1
-      for (int blk = first - step; ok && blk < nb; blk += step) {
-        if (blk >= 0) {  // P V of this block
-          const int st = (kc + blk) % NV;
-          const bool there = mbar_wait(smem_u32(&v_full[st]), (uint32_t)((kc + blk) / NV) & 1, abort_flag) && mbar_wait(smem_u32(&p_full[t]), pp, abort_flag);
+      for (int i = 0; ok && i < items + 2; ++i) {
+        const int t = i & 1;
+        const bool begins = !two || t == 0, ends = !two || t == 1;  // the first and the last item that reads a block
+        if (i >= 2) {  // P V of item i - 2, once its weights and V are there
+          bool there = true;
+          if (begins) there = mbar_wait(smem_u32(&v_full[vs]), vp, abort_flag);
+          there = there && mbar_wait(smem_u32(&p_full[t]), pp >> t & 1, abort_flag);
           ok = __all_sync(0xffffffffu, there);
           if (!ok) break;
-          pp ^= 1;
+          pp ^= 1u << t;
           fence_after();
           if (elect_one()) {
-            const uint64_t vd = v_desc + (uint64_t)((st * TILE) >> 4);
-            umma_tmem_a(o_col, s_col, vd, idesc(D, true), blk != first);
+            const uint32_t to = 256 + t * D, from_p = t * 128;  // (the whole tensor memory is this CTA's: it begins at 0)
+            const uint64_t vd = v_desc + (uint64_t)((vs * TILE) >> 4);
+            umma_tmem_a(to, from_p, vd, idesc(D, true), i >= 4);
 #pragma unroll
-            for (int kk = 1; kk < BN / 16; ++kk) umma_tmem_a_more(o_col, s_col + kk * 8, vd + ((kk * 2048) >> 4), idesc(D, true));
-            umma_commit(smem_u32(&v_empty[st]));
-            if (!two) umma_commit(smem_u32(&v_empty[st]));  // (two arrivals give a stage back: of both tiles, or of the one that read it)
-            if (blk + step >= nb) umma_commit(smem_u32(&o_full[t]));
+            for (int kk = 1; kk < BN / 16; ++kk) umma_tmem_a_more(to, from_p + kk * 8, vd + ((kk * 2048) >> 4), idesc(D, true));
+            if (ends) umma_commit(smem_u32(&v_empty[vs]));
+            if (i >= items) umma_commit(smem_u32(&o_full[t]));
+            if (items == 1) umma_commit(smem_u32(&o_full[1]));  // (a tile without items: its accumulator is not read)
           }
           __syncwarp();
+          if (ends && ++vs == NV) vs = 0, vp ^= 1;
         }
-        const int next = blk + step;
-        if (next < nb) {  // S of the next
-          const int st = (kc + next) % NK;
-          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[st]), (uint32_t)((kc + next) / NK) & 1, abort_flag));
+        if (i < items) {  // S of item i, once its K is there
+          if (begins) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[ks]), kp, abort_flag));
           if (!ok) break;
           if (elect_one()) {
-            const uint64_t kd = k_desc + (uint64_t)((st * TILE) >> 4), qd = q_desc + (uint64_t)(two && t ? TILE >> 4 : 0);
-            umma_first(s_col, qd, kd, idesc(BN, false));
+            const uint32_t to = t * 128;
+            const uint64_t kd = k_desc + (uint64_t)((ks * TILE) >> 4), qd = q_desc + (uint64_t)(two && t ? TILE >> 4 : 0);
+            umma_first(to, qd, kd, idesc(BN, false));
 #pragma unroll
             for (int x = 1; x < D / 16; ++x) {
               const uint32_t off = ((x >> 2) * ATOM + (x & 3) * 32) >> 4;
-              umma_more(s_col, qd + off, kd + off, idesc(BN, false));
+              umma_more(to, qd + off, kd + off, idesc(BN, false));
             }
             umma_commit(smem_u32(&s_full[t]));
-            umma_commit(smem_u32(&k_empty[st]));
-            if (!two) umma_commit(smem_u32(&k_empty[st]));
-            if (next + step >= nb) umma_commit(smem_u32(&q_empty));
+            if (ends) umma_commit(smem_u32(&k_empty[ks]));
+            if (i == items - 1) umma_commit(smem_u32(&q_empty));
           }
           __syncwarp();
+          if (ends && ++ks == NK) ks = 0, kp ^= 1;
         }
       }
-      kc += nb, ++qc;
+      ++qc;
     }
-    // Everything this warp asked of the tensor core is done when this arrives, the arrivals of the commits above included: nobody leaves before.
-    if (elect_one()) umma_commit(smem_u32(&all_done[t]));
+    // Everything this CTA asked of the tensor core is done when this arrives, the arrivals of the commits above included: nobody leaves before.
+    if (elect_one()) umma_commit(smem_u32(&all_done));
     __syncwarp();
     int patience = 0;
-    mbar_wait(smem_u32(&all_done[t]), 0, &patience);
+    mbar_wait(smem_u32(&all_done), 0, &patience);
     if (patience != 0) *abort_flag = 1;
   } else {
     // ---------------- softmax ----------------
@@ -762,7 +790,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t s_addr = tmem + lanes + t * 128, o_addr = tmem + lanes + 256 + t * D;
     const float scale = CAP ? 1.f : p.scale_log2;
-    int sc = 0, vc = 0, done = 0, done1 = 0;
+    int sc = 0, vc = 0, done = 0;
     for (;;) {
       uint32_t there = fetch();
       const Piece& r = piece_s[pieces % AHEAD];
@@ -812,7 +840,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
       vc += nb;
       // ---- the group's rows ----
       mbar_wait(smem_u32(&o_full[0]), (uint32_t)done & 1, abort_flag);
-      if (two || nb > 1) mbar_wait(smem_u32(&o_full[1]), (uint32_t)done1++ & 1, abort_flag);
+      mbar_wait(smem_u32(&o_full[1]), (uint32_t)done & 1, abort_flag);
       ++done;
       ml_s[warp][lane] = make_float2(m, l);
       __syncwarp();
@@ -844,42 +872,30 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
   }
 }
 
-// The parts of a group that fell to several CTAs: o = sum 2^(m - M) o_part / (sum 2^(m - M) l + 2^(sink - M)), the CTAs in their order.  A CTA for 32
-// places of a group, a lane per place, a warp per 4 columns in turn.
-template <bool WIDE>
+// The parts of a group that fell to several CTAs: o = sum 2^(m - M) o_part / (sum 2^(m - M) l + 2^(sink - M)), the CTAs in their order.  A CTA for 32 places of
+// the group whose first part is main CTA blockIdx.x's, a lane per place, a warp per 4 columns in turn.
 __global__ void __launch_bounds__(256) join_tree_parts_kernel(const Params p) {
   ts_pdl_prologue();
   constexpr int VEC = D / 32;  // pieces of 4 columns per warp
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hk = blockIdx.y, b = blockIdx.z;
-  const int G = p.nq / p.nkv, RT = BM / G * G, RG = WIDE ? 2 * RT : RT;
-  const int per_group = p.part_rows / 32, g = blockIdx.x / per_group, place = blockIdx.x % per_group * 32 + lane;
-  if (p.cu[b + 1] - p.cu[b] <= 0) return;
-  const Request r = request_of<WIDE>(p, b, RT);
-  if (g >= r.groups) return;
-  const int cost = cost_of<WIDE>(r, g, RT), share = p.plan[p.num_seqs];
-  const int at = p.plan[b] + hk * cost_of_head<WIDE>(r, RT) + g * r.blocks * (WIDE ? COST_TWO : COST_ONE);
-  const int c0 = at / share, c1 = (at + (r.blocks - 1) * cost) / share;
-  if (c0 == c1) return;  // (its CTA has written it)
-  const int in_tile = place % BM, in = place / BM * RT + in_tile, row = g * RG + in;
-  if (in_tile >= RT || in >= RG || row >= r.rows) return;
-  const int head = hk * G + row % G;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x, place = blockIdx.y * 32 + lane;
+  const int4 ends = p.plan[2 * c0 + 1], group = p.plan[2 * c0];
+  const int c1 = ends.x;
+  if (c1 <= c0) return;  // its last group was whole, or another's
+  const int G = p.nq / p.nkv, RT = BM / G * G;
+  const int in_tile = place % BM, in = place / BM * RT + in_tile, row = group.y + in;
+  if (in_tile >= RT || in >= group.z) return;
+  const int head = group.w * G + row % G;
   float top = p.head_sinks ? p.head_sinks[head] * LOG2E : -INFINITY;
   const float sink = top;
-  auto part = [&](int c) -> size_t { return ((size_t)c * 2 + (at <= c * share ? 0 : 1)) * p.part_rows; };  // where CTA c left its part
-  auto has = [&](int c) {  // (a share smaller than a block's cost may hold no block's beginning)
-    const int from = c * share;
-    return (from > at ? (from - at + cost - 1) / cost : 0) < min(r.blocks, (from + share - at + cost - 1) / cost);
-  };
+  auto part = [&](int c) -> size_t { return ((size_t)c * 2 + (c == c0 ? ends.y : 0)) * p.part_rows; };
 #pragma unroll 4
-  for (int c = c0; c <= c1; ++c)
-    if (has(c)) top = fmaxf(top, p.part_ml[2 * (part(c) + place)]);
+  for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.part_ml[2 * (part(c) + place)]);
   float total = sink == -INFINITY ? 0.f : fast_exp2(sink - top);
   float4 o[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
+#pragma unroll 4
   for (int c = c0; c <= c1; ++c) {
-    if (!has(c)) continue;
     const size_t x = part(c);
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (x + place));
     const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
@@ -891,7 +907,7 @@ __global__ void __launch_bounds__(256) join_tree_parts_kernel(const Params p) {
     }
   }
   const float inv = total > 0.f ? 1.f / total : 0.f;
-  __nv_bfloat16* out = p.out + ((size_t)(r.q_begin + row / G) * p.nq + head) * D;
+  __nv_bfloat16* out = p.out + ((size_t)(group.x + row / G) * p.nq + head) * D;
 #pragma unroll
   for (int i = 0; i < VEC; ++i)
     *reinterpret_cast<uint2*>(out + (warp + 8 * i) * 4) = make_uint2(pack_bf16(o[i].x * inv, o[i].y * inv), pack_bf16(o[i].z * inv, o[i].w * inv));
@@ -931,8 +947,7 @@ int launch(const CUtensorMap* maps, const Params& p, int max_t, cudaStream_t str
   if (e != cudaSuccess) return (int)e;
   const int status = ts_launch(attention_tree_kernel<WIDE, CAP>, dim3(p.ctas), dim3(THREADS), smem, stream, maps[0], maps[1], maps[2], maps[3], maps[4], p);
   if (status != 0) return status;
-  const int G = p.nq / p.nkv, RG = BM / G * G * (WIDE ? 2 : 1), groups = (max_t * G + RG - 1) / RG;
-  return ts_launch(join_tree_parts_kernel<WIDE>, dim3(groups * (p.part_rows / 32), p.nkv, p.num_seqs), dim3(256), 0, stream, p);
+  return ts_launch(join_tree_parts_kernel, dim3(p.ctas, p.part_rows / 32), dim3(256), 0, stream, p);
 }
 
 }  // namespace
@@ -952,7 +967,7 @@ TS_EXPORT long long ts_attention_tree_tcgen05_scratch(int B, int max_t, int max_
   const long long blocks = (long long)B * nkv * groups * ((max_context + BN - 1) / BN);
   *ctas = (int)(blocks < 1 ? 1 : blocks < sms ? blocks : sms);
   *part_rows = wide ? 2 * BM : rows <= 32 ? 32 : rows <= 64 ? 64 : BM;
-  return 2ll * *ctas * *part_rows * (D + 2) + B + 2;
+  return 2ll * *ctas * *part_rows * (D + 2) + 8ll * *ctas;
 }
 
 TS_EXPORT int ts_attention_tree_tcgen05(const void* q, const void* k, const void* v, void* out, const unsigned long long* mask, int words, const int* cu,
@@ -968,7 +983,7 @@ TS_EXPORT int ts_attention_tree_tcgen05(const void* q, const void* k, const void
   p.mask = mask, p.cu = cu, p.context = context, p.table = table, p.positions = positions, p.head_sinks = head_sinks;
   p.part_o = scratch;
   p.part_ml = scratch + 2ll * ctas * part_rows * D;
-  p.plan = (int*)(p.part_ml + 4ll * ctas * part_rows);
+  p.plan = (int4*)(p.part_ml + 4ll * ctas * part_rows);
   p.error = error;
   p.words = words, p.max_blocks = max_blocks, p.page = page, p.nq = nq, p.nkv = nkv, p.window = window, p.num_seqs = B;
   p.total_slots = (int)(num_pages * page), p.part_rows = part_rows, p.ctas = ctas;

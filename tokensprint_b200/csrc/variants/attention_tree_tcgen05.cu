@@ -970,10 +970,23 @@ TS_EXPORT long long ts_attention_tree_tcgen05_scratch(int B, int max_t, int max_
   return 2ll * *ctas * *part_rows * (D + 2) + 8ll * *ctas;
 }
 
-TS_EXPORT int ts_attention_tree_tcgen05(const void* q, const void* k, const void* v, void* out, const unsigned long long* mask, int words, const int* cu,
-                                        const int* context, const int* table, int max_blocks, int page, long long num_pages, const int* positions,
-                                        const float* head_sinks, int T, int B, int max_t, int nq, int nkv, float scale, int window, float cap, int ctas,
-                                        int part_rows, float* scratch, int* error, void* stream) {
+struct TreeArgs {
+  const void *q, *k, *v;
+  void* out;
+  const unsigned long long* mask;
+  const int *cu, *context, *table, *positions;
+  const float* head_sinks;
+  float* scratch;
+  int* error;
+  void* stream;
+  long long num_pages;
+  int words, max_blocks, page, T, B, max_t, nq, nkv, window, ctas, part_rows;
+  float scale, cap;
+};
+
+TS_EXPORT int ts_attention_tree_tcgen05(const TreeArgs* args) {
+  const auto [q, k, v, out, mask, cu, context, table, positions, head_sinks, scratch, error, stream, num_pages, words, max_blocks, page, T, B, max_t, nq, nkv, window, ctas, part_rows,
+              scale, cap] = *args;
   if (B <= 0 || T <= 0) return 0;
   if (scratch == nullptr || error == nullptr || max_blocks <= 0 || ctas <= 0 || max_t <= 0 || (window > 0 && positions == nullptr)) return TS_ERR_BAD_ARGUMENT;
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)scratch) % 16) return TS_ERR_BAD_ARGUMENT;

@@ -2898,16 +2898,25 @@ TREE_MAX_NODES = 256
 TREE_MAX_HEAD_DIM = 256
 VERIFY_MAX_VOCAB = 1 << 20
 LOOKUP_MAX_BRANCHES, LOOKUP_MAX_DEPTH, LOOKUP_MAX_SUFFIX = 16, 64, 16
-_SIGNATURES["ts_verify_drafts"] = [_c_void_p, _c_int, _c_ll, _c_void_p, _c_ll] + [_c_void_p] * 9 + [_c_int] * 3 + [_c_void_p]
-_SIGNATURES["ts_keep_drafted_rows"] = [_c_void_p, _c_int, _c_int, _c_int, _c_ll, _c_int, _c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] * 2 + [_c_void_p]
-_SIGNATURES["ts_lookup_drafts"] = [_c_void_p, _c_ll] + [_c_void_p] * 4 + [_c_int] * 6 + [_c_void_p]
+# Entry points that take one block of arguments, laid out as the C structs beside them.
+for _name in ("ts_verify_drafts", "ts_keep_drafted_rows", "ts_lookup_drafts"):
+    _SIGNATURES[_name] = [ctypes.c_char_p]
+_VERIFY_ARGS = _struct.Struct("@12P2q5i4x").pack
+_KEEP_ARGS = _struct.Struct("@7Pq7i4x").pack
+_LOOKUP_ARGS = _struct.Struct("@6Pq6i").pack
 TREE_TCGEN05_HEAD_DIMS = (64, 128)
 _attention_trees: dict[int, tuple] = {}
 _attention_trees_tcgen05: dict[int, tuple] = {}
+_attention_tree_plans: dict[tuple, Optional[tuple]] = {}
+_TREE_ARGS = _struct.Struct("@13Pq11i2f").pack
+
+
+def _current_device() -> int:
+    return _raw_device() if _raw_device is not None else torch.cuda.current_device()
 
 
 def _on_current_device(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    here = _current_device()
     for t in tensors:
         if t is not None and t.device.index != here:
             raise KernelError(f"{name}: a tensor lies on {t.device}, the current device is cuda:{here}")
@@ -2939,8 +2948,7 @@ def _attention_tree_tcgen05_fns(head_dim: int) -> tuple:
     if fns is None:
         lib = _build.load_variant("attention_tree_tcgen05", {"TS_HEAD_DIM": head_dim})
         run = lib.ts_attention_tree_tcgen05
-        run.argtypes = ([_c_void_p] * 5 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 2 + [_c_ll] + [_c_void_p] * 2 + [_c_int] * 5
-                        + [_c_float, _c_int, _c_float, _c_int, _c_int] + [_c_void_p] * 3)
+        run.argtypes = [ctypes.c_char_p]
         run.restype = _c_int
         takes = lib.ts_attention_tree_tcgen05_takes
         takes.argtypes = [_c_int] * 6 + [_c_ll, _c_float]
@@ -2950,6 +2958,65 @@ def _attention_tree_tcgen05_fns(head_dim: int) -> tuple:
         scratch.restype = _c_ll
         fns = _attention_trees_tcgen05[head_dim] = (run, takes, scratch)
     return fns
+
+
+def _attention_tree_plan(d: int, num_seqs: int, max_t: int, max_context: int, nq: int, nkv: int, page: int, pages: int, scale: float, sms: int) -> Optional[tuple]:
+    """(CTAs, rows of a part, floats of scratch) of the tcgen05 kernels, None where they do not take the sizes."""
+    key = (d, num_seqs, max_t, max_context, nq, nkv, page, pages, scale, sms)
+    plan = _attention_tree_plans.get(key, 0)
+    if plan == 0:
+        _, takes, scratch = _attention_tree_tcgen05_fns(d)
+        plan = None
+        if takes(num_seqs, max_t, max_context, nq, nkv, page, pages, scale):
+            ctas, rows = _c_int(), _c_int()
+            words = scratch(num_seqs, max_t, max_context, nq, nkv, sms, ctypes.byref(ctas), ctypes.byref(rows))
+            plan = (ctas.value, rows.value, words)
+        if len(_attention_tree_plans) >= 4096:
+            _attention_tree_plans.clear()
+        _attention_tree_plans[key] = plan
+    return plan
+
+
+def _refuse_attention_tree(q, k_cache, v_cache, out, tree_mask, cu_seqlens_q, context_lens, block_table, page_size, num_seqs, max_seqlen_q, max_context, nq, nkv, d,
+                           window, positions, head_sinks, softcap) -> None:
+    """Raises for the argument that attention_tree does not take."""
+    if not attention_tree_supported(d):
+        raise KernelError(f"attention_tree: head_dim must be a multiple of 8 up to {TREE_MAX_HEAD_DIM}, got {d}")
+    for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("out", out)):
+        _cuda_contig(f"attention_tree: {name}", t, q.dtype)
+    _act_code("attention_tree: q", q)
+    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("context_lens", context_lens), ("block_table", block_table)):
+        _cuda_contig(f"attention_tree: {name}", t, torch.int32)
+    _cuda_contig("attention_tree: tree_mask", tree_mask, torch.int64)
+    _on_current_device("attention_tree", q, k_cache, v_cache, out, tree_mask, cu_seqlens_q, context_lens, block_table, positions, head_sinks)
+    T = q.shape[0]
+    if nkv < 1 or nq < 1 or nq % nkv:
+        raise KernelError(f"attention_tree: {nq} query heads are no multiple of {nkv} key/value heads")
+    if q.numel() != T * nq * d or out.numel() != T * nq * d:
+        raise KernelError(f"attention_tree: q {tuple(q.shape)} and out {tuple(out.shape)} do not match [T, {nq} heads of {d}]")
+    if page_size < 1 or k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (page_size, nkv, d) or k_cache.shape != v_cache.shape:
+        raise KernelError(f"attention_tree: caches must be [pages,{page_size},{nkv},{d}], got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    if not 1 <= max_seqlen_q <= TREE_MAX_NODES:
+        raise KernelError(f"attention_tree: a request brings 1 to {TREE_MAX_NODES} nodes, got {max_seqlen_q}")
+    if tree_mask.dim() != 2 or tree_mask.shape[0] < T or 64 * tree_mask.shape[1] < max_seqlen_q:
+        raise KernelError(f"attention_tree: tree_mask must be [T, a word per 64 nodes], got {tuple(tree_mask.shape)} for {T} tokens and {max_seqlen_q} nodes")
+    if block_table.dim() != 2 or block_table.shape[0] < num_seqs or block_table.shape[1] < 1:
+        raise KernelError("attention_tree: block_table must be [B,max_blocks]")
+    if cu_seqlens_q.numel() < num_seqs + 1 or context_lens.numel() < num_seqs:
+        raise KernelError("attention_tree: cu_seqlens_q/context_lens are shorter than the batch")
+    if num_seqs > 65535 or max_context < 0 or window < 0 or not softcap >= 0.0:
+        raise KernelError("attention_tree: at most 65535 requests, and max_context, window and softcap must not be negative")
+    if window > 0:
+        if positions is None:
+            raise KernelError("attention_tree: a window needs the nodes' positions")
+        _cuda_contig("attention_tree: positions", positions, torch.int32)
+        if positions.numel() < T:
+            raise KernelError("attention_tree: positions is shorter than the batch")
+    if head_sinks is not None:
+        _cuda_contig("attention_tree: head_sinks", head_sinks, torch.float32)
+        if head_sinks.numel() != nq:
+            raise KernelError(f"attention_tree: head_sinks must have one entry per query head ({nq}), got {head_sinks.numel()}")
+    raise KernelError("attention_tree: the caches must begin at multiples of 16 bytes")
 
 
 def attention_tree(
@@ -2986,67 +3053,89 @@ def attention_tree(
     (a value of infinity counts for the nodes that do not see its row, too).
     """
     flush_gemm_chain()
-    run, plan = _attention_tree_fns(head_dim)
-    for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("out", out)):
-        _cuda_contig(f"attention_tree: {name}", t, q.dtype)
-    code = _act_code("attention_tree: q", q)
-    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("context_lens", context_lens), ("block_table", block_table)):
-        _cuda_contig(f"attention_tree: {name}", t, torch.int32)
-    _cuda_contig("attention_tree: tree_mask", tree_mask, torch.int64)
-    _on_current_device("attention_tree", q, k_cache, v_cache, out, tree_mask, cu_seqlens_q, context_lens, block_table, positions, head_sinks)
-    T, nq, nkv, d = q.shape[0], num_heads, num_kv_heads, head_dim
-    if nkv < 1 or nq < 1 or nq % nkv:
-        raise KernelError(f"attention_tree: {nq} query heads are no multiple of {nkv} key/value heads")
-    if q.numel() != T * nq * d or out.numel() != T * nq * d:
-        raise KernelError(f"attention_tree: q {tuple(q.shape)} and out {tuple(out.shape)} do not match [T, {nq} heads of {d}]")
-    if page_size < 1 or tuple(k_cache.shape[-3:]) != (page_size, nkv, d) or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
-        raise KernelError(f"attention_tree: caches must be [pages,{page_size},{nkv},{d}], got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    if not 1 <= max_seqlen_q <= TREE_MAX_NODES:
-        raise KernelError(f"attention_tree: a request brings 1 to {TREE_MAX_NODES} nodes, got {max_seqlen_q}")
-    if tree_mask.dim() != 2 or tree_mask.shape[0] < T or 64 * tree_mask.shape[1] < max_seqlen_q:
-        raise KernelError(f"attention_tree: tree_mask must be [T, a word per 64 nodes], got {tuple(tree_mask.shape)} for {T} tokens and {max_seqlen_q} nodes")
-    if block_table.dim() != 2 or block_table.shape[0] < num_seqs or block_table.shape[1] < 1:
-        raise KernelError("attention_tree: block_table must be [B,max_blocks]")
-    if cu_seqlens_q.numel() < num_seqs + 1 or context_lens.numel() < num_seqs:
-        raise KernelError("attention_tree: cu_seqlens_q/context_lens are shorter than the batch")
-    if num_seqs > 65535 or max_context < 0 or window < 0 or not softcap >= 0.0:
-        raise KernelError("attention_tree: at most 65535 requests, and max_context, window and softcap must not be negative")
-    if window > 0:
-        if positions is None:
-            raise KernelError("attention_tree: a window needs the nodes' positions")
-        _cuda_contig("attention_tree: positions", positions, torch.int32)
-        if positions.numel() < T:
-            raise KernelError("attention_tree: positions is shorter than the batch")
-    if head_sinks is not None:
-        _cuda_contig("attention_tree: head_sinks", head_sinks, torch.float32)
-        if head_sinks.numel() != nq:
-            raise KernelError(f"attention_tree: head_sinks must have one entry per query head ({nq}), got {head_sinks.numel()}")
+    nq, nkv, d = num_heads, num_kv_heads, head_dim
+    dtype, qs, ks, ms, ts, here = q.dtype, q.shape, k_cache.shape, tree_mask.shape, block_table.shape, _current_device()
+    T = qs[0]
+    # every check in one expression (by name and with its words they take as long as the kernels of a small step)
+    if not (
+        attention_tree_supported(d) and (dtype is torch.bfloat16 or dtype is torch.float32) and q.is_cuda and q.is_contiguous() and q.get_device() == here
+        and k_cache.is_contiguous() and k_cache.dtype is dtype and k_cache.get_device() == here and v_cache.is_contiguous() and v_cache.dtype is dtype
+        and v_cache.get_device() == here and out.is_contiguous() and out.dtype is dtype and out.get_device() == here
+        and cu_seqlens_q.dtype is torch.int32 and cu_seqlens_q.is_contiguous() and cu_seqlens_q.get_device() == here
+        and context_lens.dtype is torch.int32 and context_lens.is_contiguous() and context_lens.get_device() == here
+        and block_table.dtype is torch.int32 and block_table.is_contiguous() and block_table.get_device() == here
+        and tree_mask.dtype is torch.int64 and tree_mask.is_contiguous() and tree_mask.get_device() == here
+        and nkv >= 1 and nq >= 1 and nq % nkv == 0 and q.numel() == T * nq * d == out.numel()
+        and len(ks) == 4 and ks == v_cache.shape and ks[1] == page_size and ks[2] == nkv and ks[3] == d and page_size >= 1
+        and 1 <= max_seqlen_q <= TREE_MAX_NODES and len(ms) == 2 and ms[0] >= T and 64 * ms[1] >= max_seqlen_q
+        and len(ts) == 2 and ts[0] >= num_seqs and ts[1] >= 1 and cu_seqlens_q.numel() > num_seqs and context_lens.numel() >= num_seqs
+        and num_seqs <= 65535 and max_context >= 0 and window >= 0 and softcap >= 0.0
+        and (window == 0 or positions is not None and positions.dtype is torch.int32 and positions.is_contiguous() and positions.get_device() == here
+             and positions.numel() >= T)
+        and (head_sinks is None or head_sinks.dtype is torch.float32 and head_sinks.is_contiguous() and head_sinks.get_device() == here
+             and head_sinks.numel() == nq)
+        and (num_seqs < 1 or T < 1 or (k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0)
+    ):
+        _refuse_attention_tree(q, k_cache, v_cache, out, tree_mask, cu_seqlens_q, context_lens, block_table, page_size, num_seqs, max_seqlen_q, max_context, nq, nkv, d,
+                               window, positions, head_sinks, softcap)
     if num_seqs < 1 or T < 1:
         return
-    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
-        raise KernelError("attention_tree: the caches must begin at multiples of 16 bytes")
     global launch_count
-    if code == 1 and d in TREE_TCGEN05_HEAD_DIMS and (q.data_ptr() | out.data_ptr()) % 16 == 0:
-        run_tcgen05, takes, scratch = _attention_tree_tcgen05_fns(d)
-        if takes(num_seqs, max_seqlen_q, max_context, nq, nkv, page_size, k_cache.shape[0], float(scale)):
-            ctas, part_rows = _c_int(), _c_int()
-            words = scratch(num_seqs, max_seqlen_q, max_context, nq, nkv, _sm_count(q.device), ctypes.byref(ctas), ctypes.byref(part_rows))
-            part, error = torch.empty(words, device=q.device, dtype=torch.float32), _gemm_workspace(q.device)[1]
-            _check("attention_tree", run_tcgen05(
-                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), tree_mask.data_ptr(), tree_mask.shape[1], cu_seqlens_q.data_ptr(),
-                context_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, k_cache.shape[0], _ptr(positions) if window > 0 else None,
-                _ptr(head_sinks), T, num_seqs, max_seqlen_q, nq, nkv, float(scale), int(window), float(softcap), ctas.value, part_rows.value,
-                part.data_ptr(), error.data_ptr(), _stream()))
+    seen = positions.data_ptr() if window > 0 else 0
+    if dtype is torch.bfloat16 and d in TREE_TCGEN05_HEAD_DIMS and (q.data_ptr() | out.data_ptr()) % 16 == 0:
+        plan = _attention_tree_plan(d, num_seqs, max_seqlen_q, max_context, nq, nkv, page_size, ks[0], scale, _sm_count(q.device))
+        if plan is not None:
+            ctas, part_rows, words = plan
+            part = torch.empty(words, device=q.device, dtype=torch.float32)
+            _check("attention_tree", _attention_tree_tcgen05_fns(d)[0](_TREE_ARGS(
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), tree_mask.data_ptr(), cu_seqlens_q.data_ptr(), context_lens.data_ptr(),
+                block_table.data_ptr(), seen, 0 if head_sinks is None else head_sinks.data_ptr(), part.data_ptr(), _gemm_workspace(q.device)[1].data_ptr(), _stream(),
+                ks[0], ms[1], ts[1], page_size, T, num_seqs, max_seqlen_q, nq, nkv, window, ctas, part_rows, scale, softcap)))
             launch_count += 1
             return
-    splits = plan(num_seqs, max_seqlen_q, nq, nkv, min(max_context, window + max_seqlen_q + 64) if window > 0 else max_context)
+    run, split = _attention_tree_fns(d)
+    splits = split(num_seqs, max_seqlen_q, nq, nkv, min(max_context, window + max_seqlen_q + 64) if window > 0 else max_context)
     part = torch.empty(T * nq * splits * (d + 2), device=q.device, dtype=torch.float32) if splits > 1 else None
     _check("attention_tree", run(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), code, tree_mask.data_ptr(), tree_mask.shape[1], cu_seqlens_q.data_ptr(),
-        context_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, k_cache.shape[0], _ptr(positions) if window > 0 else None,
-        _ptr(head_sinks), T, num_seqs, max_seqlen_q, nq, nkv, float(scale), int(window), float(softcap), splits, _ptr(part), _stream()))
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), int(dtype is torch.bfloat16), tree_mask.data_ptr(), ms[1], cu_seqlens_q.data_ptr(),
+        context_lens.data_ptr(), block_table.data_ptr(), ts[1], page_size, ks[0], seen or None, _ptr(head_sinks), T, num_seqs, max_seqlen_q, nq, nkv, float(scale),
+        int(window), float(softcap), splits, _ptr(part), _stream()))
     if splits > 1:
         launch_count += 1
+
+
+def _takes_vector(t: torch.Tensor, dtype: torch.dtype, n: int, here: int) -> bool:
+    return t.dtype is dtype and t.is_cuda and t.is_contiguous() and t.get_device() == here and t.numel() >= n
+
+
+def _refuse_verify_drafts(logits, tokens, parents, cu_seqlens, temperatures, uniforms, keys, path, next_tokens, counts, num_seqs, max_nodes, draft_probs) -> None:
+    """Raises for the argument that verify_drafts does not take."""
+    if not logits.is_cuda or logits.dim() != 2 or logits.stride(1) != 1:
+        raise KernelError(f"verify_drafts: logits must be a CUDA matrix [T,V] with neighbouring entries in a row, got {tuple(logits.shape)}, strides {logits.stride()}")
+    _act_code("verify_drafts: logits", logits)
+    T, V = logits.shape
+    if not 1 <= V <= VERIFY_MAX_VOCAB:
+        raise KernelError(f"verify_drafts: a vocabulary of 1 to {VERIFY_MAX_VOCAB} entries, got {V}")
+    if T > 1 and logits.stride(0) < V:
+        raise KernelError("verify_drafts: rows of logits overlap")
+    for name, t, dtype, n in (("tokens", tokens, torch.int32, T), ("parents", parents, torch.int32, T), ("uniforms", uniforms, torch.float32, T),
+                              ("cu_seqlens", cu_seqlens, torch.int32, num_seqs + 1), ("temperatures", temperatures, torch.float32, num_seqs),
+                              ("keys", keys, torch.int64, num_seqs), ("counts", counts, torch.int32, num_seqs)):
+        _cuda_contig(f"verify_drafts: {name}", t, dtype)
+        if t.numel() < n:
+            raise KernelError(f"verify_drafts: {name} needs {n} entries, got {t.numel()}")
+    if not 1 <= max_nodes <= TREE_MAX_NODES:
+        raise KernelError(f"verify_drafts: a request brings 1 to {TREE_MAX_NODES} nodes, got {max_nodes}")
+    for name, t in (("path", path), ("next_tokens", next_tokens)):
+        _cuda_contig(f"verify_drafts: {name}", t, torch.int32)
+        if t.dim() != 2 or t.shape[0] < num_seqs or t.shape[1] < max_nodes or t.shape != path.shape:
+            raise KernelError(f"verify_drafts: path and next_tokens must be [B, {max_nodes} or more], got {tuple(path.shape)} and {tuple(next_tokens.shape)}")
+    if draft_probs is not None:
+        if not draft_probs.is_cuda or draft_probs.dtype != torch.float32 or draft_probs.shape != logits.shape or draft_probs.stride(1) != 1 or (
+                T > 1 and draft_probs.stride(0) < V):
+            raise KernelError(f"verify_drafts: draft_probs must be float32 of the logits' shape {tuple(logits.shape)}")
+    _on_current_device("verify_drafts", logits, tokens, parents, cu_seqlens, temperatures, uniforms, keys, path, next_tokens, counts, draft_probs)
+    raise KernelError("verify_drafts: arguments that are not taken")
 
 
 def verify_drafts(
@@ -3079,37 +3168,26 @@ def verify_drafts(
     NaN and -inf are logits of no probability; tokens outside the vocabulary are never accepted.
     """
     flush_gemm_chain()
-    if not logits.is_cuda or logits.dim() != 2 or logits.stride(1) != 1:
-        raise KernelError(f"verify_drafts: logits must be a CUDA matrix [T,V] with neighbouring entries in a row, got {tuple(logits.shape)}, strides {logits.stride()}")
-    code = _act_code("verify_drafts: logits", logits)
-    T, V = logits.shape
-    if not 1 <= V <= VERIFY_MAX_VOCAB:
-        raise KernelError(f"verify_drafts: a vocabulary of 1 to {VERIFY_MAX_VOCAB} entries, got {V}")
-    if T > 1 and logits.stride(0) < V:
-        raise KernelError("verify_drafts: rows of logits overlap")
-    for name, t, dtype, n in (("tokens", tokens, torch.int32, T), ("parents", parents, torch.int32, T), ("uniforms", uniforms, torch.float32, T),
-                              ("cu_seqlens", cu_seqlens, torch.int32, num_seqs + 1), ("temperatures", temperatures, torch.float32, num_seqs),
-                              ("keys", keys, torch.int64, num_seqs), ("counts", counts, torch.int32, num_seqs)):
-        _cuda_contig(f"verify_drafts: {name}", t, dtype)
-        if t.numel() < n:
-            raise KernelError(f"verify_drafts: {name} needs {n} entries, got {t.numel()}")
-    if not 1 <= max_nodes <= TREE_MAX_NODES:
-        raise KernelError(f"verify_drafts: a request brings 1 to {TREE_MAX_NODES} nodes, got {max_nodes}")
-    for name, t in (("path", path), ("next_tokens", next_tokens)):
-        _cuda_contig(f"verify_drafts: {name}", t, torch.int32)
-        if t.dim() != 2 or t.shape[0] < num_seqs or t.shape[1] < max_nodes or t.shape != path.shape:
-            raise KernelError(f"verify_drafts: path and next_tokens must be [B, {max_nodes} or more], got {tuple(path.shape)} and {tuple(next_tokens.shape)}")
-    if draft_probs is not None:
-        if not draft_probs.is_cuda or draft_probs.dtype != torch.float32 or draft_probs.shape != logits.shape or draft_probs.stride(1) != 1 or (
-                T > 1 and draft_probs.stride(0) < V):
-            raise KernelError(f"verify_drafts: draft_probs must be float32 of the logits' shape {tuple(logits.shape)}")
-    _on_current_device("verify_drafts", logits, tokens, parents, cu_seqlens, temperatures, uniforms, keys, path, next_tokens, counts, draft_probs)
+    shape, here = logits.shape, _current_device()
+    if len(shape) != 2 or not (
+        logits.is_cuda and logits.get_device() == here and (logits.dtype is torch.float32 or logits.dtype is torch.bfloat16) and logits.stride(1) == 1
+        and 1 <= shape[1] <= VERIFY_MAX_VOCAB and (shape[0] <= 1 or logits.stride(0) >= shape[1]) and 1 <= max_nodes <= TREE_MAX_NODES
+        and _takes_vector(tokens, torch.int32, shape[0], here) and _takes_vector(parents, torch.int32, shape[0], here)
+        and _takes_vector(uniforms, torch.float32, shape[0], here) and _takes_vector(cu_seqlens, torch.int32, num_seqs + 1, here)
+        and _takes_vector(temperatures, torch.float32, num_seqs, here) and _takes_vector(keys, torch.int64, num_seqs, here)
+        and _takes_vector(counts, torch.int32, num_seqs, here) and _takes_vector(path, torch.int32, 0, here) and _takes_vector(next_tokens, torch.int32, 0, here)
+        and path.dim() == 2 and path.shape == next_tokens.shape and path.shape[0] >= num_seqs and path.shape[1] >= max_nodes
+        and (draft_probs is None or draft_probs.is_cuda and draft_probs.get_device() == here and draft_probs.dtype is torch.float32
+             and draft_probs.shape == shape and draft_probs.stride(1) == 1 and (shape[0] <= 1 or draft_probs.stride(0) >= shape[1]))
+    ):
+        _refuse_verify_drafts(logits, tokens, parents, cu_seqlens, temperatures, uniforms, keys, path, next_tokens, counts, num_seqs, max_nodes, draft_probs)
+    T, V = shape
     if num_seqs < 1 or T < 1:
         return
-    _check("verify_drafts", _fn("ts_verify_drafts")(
-        logits.data_ptr(), code, max(logits.stride(0), V), _ptr(draft_probs), 0 if draft_probs is None else max(draft_probs.stride(0), V), tokens.data_ptr(),
-        parents.data_ptr(), cu_seqlens.data_ptr(), temperatures.data_ptr(), uniforms.data_ptr(), keys.data_ptr(), path.data_ptr(), next_tokens.data_ptr(),
-        counts.data_ptr(), V, num_seqs, path.shape[1], _stream()))
+    _check("verify_drafts", _fn("ts_verify_drafts")(_VERIFY_ARGS(
+        logits.data_ptr(), 0 if draft_probs is None else draft_probs.data_ptr(), tokens.data_ptr(), parents.data_ptr(), cu_seqlens.data_ptr(), temperatures.data_ptr(),
+        uniforms.data_ptr(), keys.data_ptr(), path.data_ptr(), next_tokens.data_ptr(), counts.data_ptr(), _stream(), max(logits.stride(0), V),
+        0 if draft_probs is None else max(draft_probs.stride(0), V), V, num_seqs, path.shape[1], int(logits.dtype is torch.bfloat16), 0)))
 
 
 class RowPools:
@@ -3143,11 +3221,11 @@ def keep_drafted_rows(pools: RowPools, path: torch.Tensor, counts: torch.Tensor,
     behind the last accepted one (they hold what they held, or what has not been moved from them)."""
     flush_gemm_chain()
     for name, t, n in (("counts", counts, num_seqs), ("cu_seqlens", cu_seqlens, num_seqs + 1), ("context_lens", context_lens, num_seqs)):
-        _cuda_contig(f"keep_drafted_rows: {name}", t, torch.int32)
+        _cuda_contig(name, t, torch.int32)
         if t.numel() < n:
             raise KernelError(f"keep_drafted_rows: {name} needs {n} entries, got {t.numel()}")
     for name, t in (("path", path), ("block_table", block_table)):
-        _cuda_contig(f"keep_drafted_rows: {name}", t, torch.int32)
+        _cuda_contig(name, t, torch.int32)
         if t.dim() != 2 or t.shape[0] < num_seqs or t.shape[1] < 1:
             raise KernelError(f"keep_drafted_rows: {name} must be a matrix with a row per request, got {tuple(t.shape)}")
     if page_size != pools.page_size:
@@ -3157,9 +3235,9 @@ def keep_drafted_rows(pools: RowPools, path: torch.Tensor, counts: torch.Tensor,
     _on_current_device("keep_drafted_rows", pools.addresses, path, counts, cu_seqlens, context_lens, block_table)
     if num_seqs < 1:
         return
-    _check("keep_drafted_rows", _fn("ts_keep_drafted_rows")(
-        pools.addresses.data_ptr(), len(pools.pools), pools.row_bytes, pools.align, pools.num_pages, page_size, path.data_ptr(), path.shape[1], counts.data_ptr(),
-        cu_seqlens.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], num_seqs, _stream()))
+    _check("keep_drafted_rows", _fn("ts_keep_drafted_rows")(_KEEP_ARGS(
+        pools.addresses.data_ptr(), path.data_ptr(), counts.data_ptr(), cu_seqlens.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(), _stream(),
+        pools.num_pages, len(pools.pools), path.shape[1], block_table.shape[1], page_size, pools.row_bytes, pools.align, num_seqs)))
 
 
 def lookup_drafts(history: torch.Tensor, lengths: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, counts: torch.Tensor, num_seqs: int,
@@ -3180,19 +3258,19 @@ def lookup_drafts(history: torch.Tensor, lengths: torch.Tensor, tokens: torch.Te
                           f"got {depth}, {branches}, {min_suffix}, {max_suffix}")
     width = 1 + depth * branches
     for name, t in (("tokens", tokens), ("parents", parents)):
-        _cuda_contig(f"lookup_drafts: {name}", t, torch.int32)
+        _cuda_contig(name, t, torch.int32)
         if t.dim() != 2 or t.shape[0] < num_seqs or t.shape[1] != width:
             raise KernelError(f"lookup_drafts: {name} must be [B,{width}], got {tuple(t.shape)}")
     for name, t in (("lengths", lengths), ("counts", counts)):
-        _cuda_contig(f"lookup_drafts: {name}", t, torch.int32)
+        _cuda_contig(name, t, torch.int32)
         if t.numel() < num_seqs:
             raise KernelError(f"lookup_drafts: {name} needs {num_seqs} entries, got {t.numel()}")
     _on_current_device("lookup_drafts", history, lengths, tokens, parents, counts)
     if num_seqs < 1:
         return
-    _check("lookup_drafts", _fn("ts_lookup_drafts")(
-        history.data_ptr(), max(history.stride(0), history.shape[1]), lengths.data_ptr(), tokens.data_ptr(), parents.data_ptr(), counts.data_ptr(),
-        history.shape[1], num_seqs, depth, branches, max_suffix, min_suffix, _stream()))
+    _check("lookup_drafts", _fn("ts_lookup_drafts")(_LOOKUP_ARGS(
+        history.data_ptr(), lengths.data_ptr(), tokens.data_ptr(), parents.data_ptr(), counts.data_ptr(), _stream(), max(history.stride(0), history.shape[1]),
+        history.shape[1], num_seqs, depth, branches, max_suffix, min_suffix)))
 
 
 # ---------------------------------------------------------------------------

@@ -28,7 +28,7 @@ namespace {
 // asked for ahead, and the first child's row is brought to the L2 meanwhile.  The race takes its logarithm only where it may win: E >= the uniform number v that it is
 // made from, so an entry with r <= best v is behind.
 
-constexpr int VT = 512;              // threads that scan
+constexpr int VT = 384;                // threads that scan
 constexpr int VERIFY_THREADS = VT + 32;  // and a warp that looks the children up
 constexpr int MAX_CLUSTER = 16;
 constexpr int VERIFY_MAX_NODES = 256;
@@ -94,53 +94,81 @@ __device__ __forceinline__ void load4(const void* row, bool vector, int at, int 
     }
   }
 }
-// Four quadruples a thread, VT * 4 entries from one to the next, the next four on their way while `use(entry, values)` works on these.
+// Four quadruples a thread at a time, VT * 4 entries from one to the next, all asked for before `use(entry, values)` works on them.  (Two CTAs of 56 registers on an SM hide
+// more than one of 96 that asks for the next four meanwhile: 32 chains 92 us so.)
 template <bool BF16, typename F>
 __device__ __forceinline__ void scan(const void* row, int begin, int end, F use) {
   constexpr int U = 4, STEP = VT * 4;
   const bool vector = ((uintptr_t)row & (BF16 ? 7 : 15)) == 0;
-  float v[U][4];
-#pragma unroll
-  for (int u = 0; u < U; ++u) load4<BF16>(row, vector, begin + u * STEP, end, v[u]);
 #pragma unroll 1
   for (int at = begin; at < end; at += U * STEP) {
     float x[U][4];
 #pragma unroll
+    for (int u = 0; u < U; ++u) load4<BF16>(row, vector, at + u * STEP, end, x[u]);
+#pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[u][j] = usable(v[u][j]);
-    if (at + U * STEP < end) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) load4<BF16>(row, vector, at + (U + u) * STEP, end, v[u]);
-    }
+      for (int j = 0; j < 4; ++j) x[u][j] = usable(x[u][j]);
     use(at, x);
   }
 }
 
 // what is left of an entry with probability p and guess q after `n` refusals with the sums `total`
 __device__ __forceinline__ float left_of(float p, float q, const float* total, int n) {
+#pragma unroll 1
   for (int j = 0; j < n; ++j)
     if (total[j] > 0.f) p = __fdividef(fmaxf(p - q, 0.f), total[j]);
   return p;
 }
 
+// The lanes' (m, s, i), joined: m the largest with its lowest index, s the sum of s exp((m_lane - m) / T), or with `plain_sum` the plain sum.
+__device__ __forceinline__ Stat join(Stat x, bool plain_sum, float inv_t) {
+  const float top = ts_warp_max(x.m);
+  // (an index of -1 is none: the largest unsigned number)
+  const unsigned i = __reduce_min_sync(0xffffffffu, x.m == top ? (unsigned)x.i : 0xffffffffu);
+  const float s = plain_sum ? x.s : x.m == -INFINITY ? 0.f : x.s * __expf((x.m - top) * inv_t);
+  return Stat{top, ts_warp_sum(s), (int)i, 0};
+}
+// The same over all threads of the cluster that scan: every warp leaves what it found with every CTA, and every warp joins them all.  (A function of its own: what a
+// launch runs once comes to the SM instruction by instruction from far away, so the kernel is kept short.)
+__device__ __noinline__ Stat meet_all(Stat x, bool scans, bool plain_sum, float inv_t, Stat* met) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (scans) {
+    const Stat w = join(x, plain_sum, inv_t);
+    if (lane < C) *cluster.map_shared_rank(&met[(int)cluster.block_rank() * (VT / 32) + warp], lane) = w;
+  }
+  cluster.sync();  // (the places of the next round are others: nobody writes what somebody still reads)
+  Stat out{-INFINITY, 0.f, -1, 0};
+#pragma unroll 1
+  for (int k = lane; k < C * (VT / 32); k += 32) {
+    const Stat w = met[k];
+    const float top = fmaxf(out.m, w.m);
+    out.i = w.m > out.m || (w.m == out.m && (unsigned)w.i < (unsigned)out.i) ? w.i : out.i;
+    out.s = plain_sum ? out.s + w.s : top == -INFINITY ? 0.f : out.s * __expf((out.m - top) * inv_t) + w.s * __expf((w.m - top) * inv_t);
+    out.m = top;
+  }
+  return join(out, plain_sum, inv_t);
+}
+
 template <bool BF16>
-__global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const VerifyArgs a) {
   ts_pdl_prologue();
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool scans = warp < VT / 32;
   extern __shared__ uint32_t refused_s[];  // a bit per entry of this CTA's piece: tokens that were refused at the node
-  __shared__ Stat met[2][MAX_CLUSTER];
-  __shared__ Stat of_warp[VT / 32];
+  __shared__ Stat met[2][MAX_CLUSTER * (VT / 32)];  // what every warp of the cluster found
   __shared__ int parent_s[VERIFY_MAX_NODES], token_s[VERIFY_MAX_NODES];
   __shared__ float child_x[VERIFY_MAX_NODES], child_q[VERIFY_MAX_NODES], uniform_s[VERIFY_MAX_NODES];
   __shared__ float total_s[VERIFY_MAX_NODES];
-  __shared__ int child_s[VERIFY_MAX_NODES], children_s, next_s;
+  __shared__ int child_s[VERIFY_MAX_NODES], children_s, next_s, asked_s, whole_s, pass_s;
+  __shared__ float mass_s;
 
   const int first = a.cu[b], nodes = min(min(a.cu[b + 1] - first, VERIFY_MAX_NODES), a.columns);
   if (rank == 0) {
+#pragma unroll 1
     for (int k = tid; k < a.columns; k += VERIFY_THREADS) a.path[(size_t)b * a.columns + k] = k == 0 && nodes > 0 ? 0 : -1, a.fresh[(size_t)b * a.columns + k] = -1;
   }
   if (nodes <= 0) {  // (all CTAs of the cluster alike)
@@ -150,41 +178,14 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const VerifyArgs
   const float T = a.temperatures[b];
   const bool greedy = !(T > 1e-10f);
   const float inv_t = greedy ? 1.f : 1.f / T;
+#pragma unroll 1
   for (int i = tid; i < nodes; i += VERIFY_THREADS) parent_s[i] = a.parents[first + i], token_s[i] = a.tokens[first + i], uniform_s[i] = a.uniforms[first + i];
   const int lo = rank * a.piece, hi = min(a.V, lo + a.piece), begin = lo + tid * 4;
   constexpr int ITEM = BF16 ? 2 : 4, STEP = VT * 4;
   int round = 0;
   cluster.sync();  // every CTA of the cluster has begun: its places may be written to
 
-  // Every CTA's (m, s, i), joined: m the largest with its lowest index, s the sum of s exp((m_piece - m) / T), or with `plain_sum` the plain sum.
-  auto add = [&](Stat& x, const Stat& y, bool plain_sum) {
-    const float top = fmaxf(x.m, y.m);
-    x.s = plain_sum ? x.s + y.s : top == -INFINITY ? 0.f : x.s * __expf((x.m - top) * inv_t) + y.s * __expf((y.m - top) * inv_t);
-    take_better(x.m, x.i, y.m, y.i);
-  };
-  auto meet = [&](float m, float s, int i, bool plain_sum) -> Stat {
-    Stat w{m, s, i, 0};
-    if (scans) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-        add(w, Stat{__shfl_xor_sync(0xffffffffu, w.m, o), __shfl_xor_sync(0xffffffffu, w.s, o), __shfl_xor_sync(0xffffffffu, w.i, o), 0}, plain_sum);
-      if (lane == 0) of_warp[warp] = w;
-    }
-    __syncthreads();
-    if (warp == 0) {
-      w = lane < VT / 32 ? of_warp[lane] : Stat{-INFINITY, 0.f, -1, 0};
-#pragma unroll
-      for (int o = VT / 64; o > 0; o >>= 1)
-        add(w, Stat{__shfl_xor_sync(0xffffffffu, w.m, o), __shfl_xor_sync(0xffffffffu, w.s, o), __shfl_xor_sync(0xffffffffu, w.i, o), 0}, plain_sum);
-      w = Stat{__shfl_sync(0xffffffffu, w.m, 0), __shfl_sync(0xffffffffu, w.s, 0), __shfl_sync(0xffffffffu, w.i, 0), 0};
-      if (lane < C) *cluster.map_shared_rank(&met[round & 1][rank], lane) = w;
-    }
-    cluster.sync();  // (the places of the next round are others: nobody writes what somebody still reads)
-    Stat out = met[round & 1][0];
-    for (int c = 1; c < C; ++c) add(out, met[round & 1][c], plain_sum);
-    ++round;
-    return out;
-  };
+  auto meet = [&](float m, float s, int i, bool plain_sum) -> Stat { return meet_all(Stat{m, s, i, 0}, scans, plain_sum, inv_t, &met[round++ & 1][0]); };
 
   int here = 0, accepted = 0, token = 0;
   for (;;) {
@@ -192,6 +193,8 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const VerifyArgs
     const float* guess = a.probs ? a.probs + (size_t)(first + here) * a.probs_stride : nullptr;
     float m = -INFINITY, s = 0.f;
     int mi = -1;
+#pragma unroll 1
+    for (int x = tid * 128; x < (hi - lo) * ITEM; x += VERIFY_THREADS * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + (size_t)lo * ITEM + x));
     if (scans) {
       // maximum, sum and argmax of the row: a thread's own running pair
       scan<BF16>(row, begin, hi, [&](int at, const float (&x)[4][4]) {
@@ -215,6 +218,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const VerifyArgs
     } else {
       // the children, in their order, and their logits
       int n = 0, oldest = -1;
+#pragma unroll 1
       for (int i0 = here + 1; i0 < nodes; i0 += 32) {
         const int i = i0 + lane;
         const bool mine = i < nodes && parent_s[i] == here && token_s[i] >= 0 && token_s[i] < a.V;
@@ -232,62 +236,122 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const VerifyArgs
       if (lane == 0) children_s = n;
       if (oldest >= 0) {  // the likeliest next row, this CTA's piece of it
         const unsigned char* ahead = reinterpret_cast<const unsigned char*>(a.logits) + ((size_t)(first + oldest) * a.row_stride + lo) * ITEM;
+#pragma unroll 1
         for (int x = lane * 128; x < (hi - lo) * ITEM; x += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(ahead + x));
       }
     }
     const Stat all = meet(m, s, mi, false);
     const float inv_s = all.s > 0.f ? 1.f / all.s : 0.f;
     const int children = children_s;  // (written before the barriers of `meet`)
-    // Which child, decided alike in every CTA.
-    int next = -1;
-    if (greedy || guess == nullptr) {
+    // Which child, decided alike in every CTA; with the drafter's probabilities a refusal needs the sum of what is left.
+    const bool summed = guess != nullptr && !greedy;
+    if (tid == 0) asked_s = 0, whole_s = 0, mass_s = 1.f;
+    float best = -1.f, bound = -1.f;  // this thread's best of the race, and the warp's
+    int best_i = -1, next = -1;
+    for (;;) {
+      __syncthreads();
       if (tid == 0) {
-        float mass = 1.f;
-        for (int k = 0; k < children && next < 0; ++k) {
-          const int x = token_s[child_s[k]];
+        int found = -1, k = asked_s;
+        float mass = mass_s;
+#pragma unroll 1
+        for (; k < children; ++k) {
+          const int i = child_s[k], x = token_s[i];
+          const float p = all.m == -INFINITY ? 0.f : expf((child_x[k] - all.m) * inv_t) * inv_s;
+          bool yes;
           if (greedy) {
-            if (x == all.i) next = child_s[k];
-            continue;
+            yes = x == all.i;
+          } else if (summed) {
+            yes = uniform_s[i] * child_q[k] < left_of(p, child_q[k], total_s, k);
+          } else {
+            float r = p;
+#pragma unroll 1
+            for (int l = 0; l < k; ++l)
+              if (token_s[child_s[l]] == x) r = 0.f;  // the same token twice: nothing is left of it
+            yes = uniform_s[i] * mass < r;
+            if (!yes && mass - r > 0.f) mass -= r;
           }
-          bool again = false;  // the same token twice: nothing is left of it
-          for (int l = 0; l < k; ++l) again |= token_s[child_s[l]] == x;
-          const float r = again || all.m == -INFINITY ? 0.f : expf((child_x[k] - all.m) * inv_t) * inv_s;
-          if (uniform_s[child_s[k]] * mass < r)
-            next = child_s[k];
-          else if (mass - r > 0.f)
-            mass -= r;
+          if (yes) {
+            found = i;
+            break;
+          }
+          if (summed && children > 1) break;  // (the sum scales all entries of the race alike: a lone child's is not needed)
         }
-        next_s = next;
+        next_s = found;
+        asked_s = k;
+        mass_s = mass;
+        // What follows: 0 the sum of what is left, 1 the race over it; 2: over r = max(p - q, 0) of one refused child, whose sum does not matter.
+        pass_s = k < children ? 0 : summed && children == 1 && whole_s == 0 ? 2 : 1;
       }
       __syncthreads();
       next = next_s;
-    } else {
-      // with the drafter's probabilities: a refusal needs the sum of what is left
-      for (int k = 0; k < children && next < 0; ++k) {
-        const float p = all.m == -INFINITY ? 0.f : expf((child_x[k] - all.m) * inv_t) * inv_s;
-        const float r = left_of(p, child_q[k], total_s, k);
-        if (uniform_s[child_s[k]] * child_q[k] < r) {
-          next = child_s[k];
-          break;
-        }
-        if (k + 1 == children && children == 1) break;  // (the sum scales all entries of the race alike: a lone child's is not needed)
-        float sum = 0.f;
-        if (scans && all.m > -INFINITY) {
-          const bool vector = ((uintptr_t)guess & 15) == 0;
-          scan<BF16>(row, begin, hi, [&](int at, const float (&x)[4][4]) {
-            float q[4][4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) load4<false>(guess, vector, at + u * STEP, hi, q[u]);
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (at + u * STEP + j < hi) sum += fmaxf(left_of(__expf((x[u][j] - all.m) * inv_t) * inv_s, q[u][j], total_s, k) - q[u][j], 0.f);
-          });
-        }
-        const float total = meet(0.f, sum, -1, true).s;
-        if (tid == 0) total_s[k] = total;
+      const int asked = asked_s, pass = pass_s;
+      if (next >= 0 || greedy) break;
+      const bool race = pass != 0;
+      if (race && !summed && children > 0) {
+#pragma unroll 1
+        for (int i = tid; i < a.piece / 32; i += VERIFY_THREADS) refused_s[i] = 0;
         __syncthreads();
+#pragma unroll 1
+        for (int k = tid; k < children; k += VERIFY_THREADS) {
+          const int x = token_s[child_s[k]] - lo;
+          if (x >= 0 && x < a.piece) atomicOr(&refused_s[x >> 5], 1u << (x & 31));
+        }
+        __syncthreads();
+      }
+      best = bound = -1.f, best_i = -1;
+      float sum = 0.f;
+      if (scans) {
+        // A pair of entries a time, two on their way; whole warps walk, those whose entries are behind the end too.
+        const uint64_t key = a.keys[b];
+        const bool mask = race && !summed && children > 0;
+        const int refusals = summed && whole_s == 0 ? asked : 0;
+        float x[3][2], q[3][2];
+        auto load2 = [&](int at, float (&x)[2], float (&q)[2]) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const bool in = at + j < hi;
+            x[j] = !in ? -INFINITY : BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[at + j]) : reinterpret_cast<const float*>(row)[at + j];
+            q[j] = in && summed ? guess[at + j] : 0.f;
+          }
+        };
+        const int from = lo + tid * 2;
+        load2(from, x[0], q[0]);
+        load2(from + VT * 2, x[1], q[1]);
+#pragma unroll 1
+        for (int at = from; at - lane * 2 < hi; at += VT * 2) {
+          load2(at + 2 * VT * 2, x[2], q[2]);
+          const uint32_t out = mask && at < hi ? refused_s[(at - lo) >> 5] >> ((at - lo) & 31) : 0u;
+          float r[2], v[2];
+          bool may_win[2];
+          const uint64_t z = pair_hash(key, (uint32_t)at >> 1);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            r[j] = all.m == -INFINITY || ((out >> j) & 1) ? 0.f : __expf((usable(x[0][j]) - all.m) * inv_t) * inv_s;
+            if (pass == 2) r[j] = fmaxf(r[j] - q[0][j], 0.f);
+            else if (refusals > 0) r[j] = left_of(r[j], q[0][j], total_s, refusals);
+            sum += fmaxf(r[j] - q[0][j], 0.f);
+            v[j] = ((float)((uint32_t)(z >> (j ? 16 : 40)) & 0xFFFFFFu) + 0.5f) * (1.f / 16777216.f);
+            may_win[j] = race && at + j < hi && (best_i < 0 || r[j] > bound * v[j]);
+            x[0][j] = x[1][j], x[1][j] = x[2][j], q[0][j] = q[1][j], q[1][j] = q[2][j];
+          }
+          if (__any_sync(0xffffffffu, may_win[0] || may_win[1])) {
+#pragma unroll 1
+            for (int j = 0; j < 2; ++j) {
+              const float rj = j ? r[1] : r[0], vj = j ? v[1] : v[0];
+              if (j ? may_win[1] : may_win[0]) take_better(best, best_i, __fdividef(rj, -log1pf(-vj)), at + j);
+            }
+            bound = fmaxf(bound, __uint_as_float(__reduce_max_sync(0xffffffffu, best < 0.f ? 0u : __float_as_uint(best))));
+          }
+        }
+      }
+      const Stat found = meet(best, race ? 0.f : sum, best_i, true);
+      if (race) {
+        token = found.i;
+        if (pass == 1 || found.m > 0.f) break;
+        if (tid == 0) whole_s = 1;  // nothing was left behind the lone refusal: as if nothing had been refused
+      } else if (tid == 0) {
+        total_s[asked] = found.s;
+        asked_s = asked + 1;
       }
     }
     if (next >= 0) {
@@ -300,64 +364,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS) verify_kernel(const VerifyArgs
       __syncthreads();  // (the children's places are written again)
       continue;
     }
-    if (greedy) {
-      token = max(all.i, 0);
-      break;
-    }
-    // the race over what is left
-    const bool mask = guess == nullptr && children > 0;
-    if (mask) {
-      for (int i = tid; i < a.piece / 32; i += VERIFY_THREADS) refused_s[i] = 0;
-      __syncthreads();
-      for (int k = tid; k < children; k += VERIFY_THREADS) {
-        const int x = token_s[child_s[k]] - lo;
-        if (x >= 0 && x < a.piece) atomicOr(&refused_s[x >> 5], 1u << (x & 31));
-      }
-      __syncthreads();
-    }
-    const uint64_t key = a.keys[b];
-    float best = -1.f;
-    int best_i = -1;
-    auto race = [&](bool lone) {
-      // lone: a refused child by itself: r = max(p - q, 0), whose sum does not matter (and where it is 0, r is p)
-      const bool vector = ((uintptr_t)guess & 15) == 0;
-      scan<BF16>(row, begin, hi, [&](int at, const float (&x)[4][4]) {
-        float q[4][4];
-        if (guess != nullptr) {
-#pragma unroll
-          for (int u = 0; u < 4; ++u) load4<false>(guess, vector, at + u * STEP, hi, q[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int i = at + u * STEP;
-          if (i >= hi) continue;
-          const uint32_t out = mask ? refused_s[(i - lo) >> 5] >> ((i - lo) & 31) : 0u;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint64_t z = pair_hash(key, (uint32_t)(i >> 1) + h);
-#pragma unroll
-            for (int j = 2 * h; j < 2 * h + 2; ++j) {
-              if (i + j >= hi) continue;
-              float r = all.m == -INFINITY || ((out >> j) & 1) ? 0.f : __expf((x[u][j] - all.m) * inv_t) * inv_s;
-              if (guess != nullptr) r = lone ? fmaxf(r - q[u][j], 0.f) : left_of(r, q[u][j], total_s, children);
-              const float v = ((float)((uint32_t)(z >> (j & 1 ? 16 : 40)) & 0xFFFFFFu) + 0.5f) * (1.f / 16777216.f);
-              if (best_i < 0 || r > best * v) take_better(best, best_i, __fdividef(r, -log1pf(-v)), i + j);
-            }
-          }
-        }
-      });
-    };
-    const bool lone = guess != nullptr && children == 1;
-    if (scans) race(lone);
-    Stat won = meet(best, 0.f, best_i, true);
-    if (lone && !(won.m > 0.f)) {  // nothing was left: as if nothing had been refused
-      if (tid == 0) total_s[0] = 0.f;
-      __syncthreads();
-      best = -1.f, best_i = -1;
-      if (scans) race(false);
-      won = meet(best, 0.f, best_i, true);
-    }
-    token = won.i;
+    if (greedy) token = max(all.i, 0);
     break;
   }
   if (rank == 0 && tid == 0) {
@@ -400,6 +407,7 @@ __global__ void __launch_bounds__(128) keep_rows_kernel(const KeepArgs a) {
     const long long page = table[row / a.page];
     return page < 0 || page >= a.num_pages ? -1 : (page * a.page + row % a.page) * a.row_bytes;
   };
+#pragma unroll 1
   for (int k0 = 1; k0 <= count; k0 += 4) {
     long long src[4], dst[4];
 #pragma unroll
@@ -409,6 +417,7 @@ __global__ void __launch_bounds__(128) keep_rows_kernel(const KeepArgs a) {
       src[i] = moves ? place(from) : -1;
       dst[i] = moves ? place(k) : -1;
     }
+#pragma unroll 1
     for (int c = threadIdx.x * (int)sizeof(W); c < a.row_bytes; c += 128 * (int)sizeof(W)) {
       W w[4];
 #pragma unroll
@@ -453,6 +462,7 @@ __global__ void __launch_bounds__(LT) lookup_kernel(const LookupArgs a) {
   int* tokens = a.tokens + (size_t)b * width;
   int* parents = a.parents + (size_t)b * width;
   if (n <= 0) {
+#pragma unroll 1
     for (int i = tid; i < width; i += LT) tokens[i] = parents[i] = -1;
     if (tid == 0) a.counts[b] = 0;
     return;
@@ -464,11 +474,13 @@ __global__ void __launch_bounds__(LT) lookup_kernel(const LookupArgs a) {
   // (m, j + 1) of a place whose token is the last one, 0 where too little matches
   auto match = [&](int j) -> unsigned long long {
     int m = 1;
+#pragma unroll 1
     while (m < a.longest && m <= j && h[j - m] == suffix_s[m]) ++m;
     return m < a.shortest ? 0ull : ((unsigned long long)m << 32) | (unsigned)(j + 1);
   };
   {
     const bool vector = ((uintptr_t)h & 15) == 0;
+#pragma unroll 1
     for (int at = tid * 4; at < n - 1; at += 4 * LT * 4) {
       int x[4][4];
 #pragma unroll
@@ -504,6 +516,7 @@ __global__ void __launch_bounds__(LT) lookup_kernel(const LookupArgs a) {
       if (tid + i * LT < listed) mine[i] = list_s[tid + i * LT], following[i] = h[(unsigned)mine[i]];
   }
   int chains = 0;
+#pragma unroll 1
   for (; chains < a.branches; ++chains) {
     unsigned long long best = 0;
     if (listed <= LISTED) {
@@ -513,12 +526,14 @@ __global__ void __launch_bounds__(LT) lookup_kernel(const LookupArgs a) {
         best = mine[i] > best ? mine[i] : best;
       }
     } else {
+#pragma unroll 1
       for (int j = tid; j < n - 1; j += LT) {
         if (h[j] != last) continue;
         const unsigned long long key = match(j);
         if (key <= best) continue;
         const int next = h[j + 1];
         bool taken = false;
+#pragma unroll 1
         for (int c = 0; c < chains; ++c) taken |= used_s[c] == next;
         if (!taken) best = key;
       }
@@ -547,11 +562,13 @@ __global__ void __launch_bounds__(LT) lookup_kernel(const LookupArgs a) {
   }
   __syncthreads();
   int total = 1;
+#pragma unroll 1
   for (int c = 0; c < chains; ++c) {
     const int begin = begin_s[c], len = min(a.depth, n - begin);
     if (tid < len) tokens[total + tid] = h[begin + tid], parents[total + tid] = tid == 0 ? 0 : total + tid - 1;
     total += len;
   }
+#pragma unroll 1
   for (int i = tid; i < width; i += LT)
     if (i == 0 || i >= total) tokens[i] = i == 0 ? last : -1, parents[i] = -1;
   if (tid == 0) a.counts[b] = total;

@@ -55,6 +55,8 @@ def parse_args(argv=None) -> argparse.Namespace:
     p.add_argument("--cache-format", choices=("model", "kv4"), default="model")
     p.add_argument("--cache-budget", type=int, default=0)
     p.add_argument("--cache-recent", type=int, default=64)
+    p.add_argument("--speculate", type=int, default=0, metavar="N", help="check up to N guessed tokens (and their alternatives) with every decoded one")
+    p.add_argument("--speculate-branches", type=int, default=1)
     return p.parse_args(argv)
 
 
@@ -105,6 +107,8 @@ def main(args: argparse.Namespace) -> None:
         cache_format=args.cache_format,
         cache_budget=args.cache_budget,
         cache_recent=args.cache_recent,
+        speculate=args.speculate,
+        speculate_branches=args.speculate_branches,
     )
     engine = LLMEngine(model=model, config=config, tokenizer=tokenizer)
     sampling_params = SamplingParams(temperature=args.temperature, max_tokens=args.max_tokens, seed=args.seed)

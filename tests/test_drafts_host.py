@@ -181,3 +181,55 @@ def look(**change):
 def test_lookup_refuses(change, why):
     with pytest.raises(KernelError, match=why):
         look(**change)
+
+
+# ---------------------------------------------------------------------------
+# the engine's side
+
+
+def test_a_tree_is_cut_to_a_depth():
+    from tokensprint_b200.engine.speculation import Tree
+
+    tree = Tree([9, 1, 2, 3, 4, 5, 6], [-1, 0, 1, 2, 0, 4, 1])
+    assert tree.cut(9) == tree
+    assert tree.cut(1) == Tree([9, 1, 4], [-1, 0, 0])
+    assert tree.cut(2) == Tree([9, 1, 2, 4, 5, 6], [-1, 0, 1, 0, 3, 1])
+    assert tree.cut(0) == tree.root() == Tree([9], [-1])
+
+
+def test_places_of_drafts_that_were_not_accepted_go_back():
+    from tokensprint_b200.cache.manager import CacheError, CacheManager, GroupSpec
+
+    cm = CacheManager([GroupSpec("full"), GroupSpec("window", 32)], 16, [10, 10], 4)
+    rc = cm.admit("a")
+    cm.extend(rc, 0, 100)
+    cm.extend(rc, 100, 130)
+    kept = [t[:7] for t in rc.tables]
+    cm.retract(rc, 103)
+    assert rc.num_tokens == 103 and [len(t) for t in rc.tables] == [7, 7] and rc.tables == kept
+    cm.check_invariants()
+    cm.extend(rc, 103, 125)
+    cm.check_invariants()
+    for tokens in (126, -1):
+        with pytest.raises(CacheError, match="cannot retract"):
+            cm.retract(rc, tokens)
+    cm.retract(rc, 125)
+    cm.free(rc)
+    cm.check_invariants()
+    with pytest.raises(CacheError, match="freed"):
+        cm.retract(rc, 5)
+
+
+def test_options_that_do_not_go_together(tmp_path):
+    from tokensprint_b200.config.engine_config import Config
+
+    Config(model=str(tmp_path), speculate=4, speculate_branches=2)
+    for bad in ({"speculate": -1}, {"speculate": 2, "speculate_branches": 0}, {"speculate": 2, "speculate_suffix": 0}, {"speculate": 2, "cache_format": "kv4"}):
+        with pytest.raises(ValueError, match="speculate"):
+            Config(model=str(tmp_path), **bad)
+
+
+def test_layers_that_take_tokens_one_behind_the_other_say_so():
+    from tokensprint_b200.parts.base import Mixer
+
+    assert "one behind the other" in Mixer.tree_refusal(object.__new__(Mixer))

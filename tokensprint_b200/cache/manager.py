@@ -242,6 +242,22 @@ class CacheManager:
         rc.dropped += rc.num_tokens - rows
         rc.num_tokens = rows
 
+    def retract(self, rc: RequestCache, tokens: int) -> None:
+        """Positions from `tokens` on were given a place for drafted tokens that were not accepted: their pages are given back."""
+        if rc.released:
+            raise CacheError(f"request {rc.request!r} was freed")
+        rows = tokens - rc.dropped
+        if not 0 <= rows <= rc.num_tokens:
+            raise CacheError(f"cannot retract request {rc.request!r} from {rc.num_tokens} rows to {rows}")
+        pages = -(-rows // self.page_size)
+        for g, pool in enumerate(self.pools):
+            gone = [p for p in rc.tables[g][pages:] if p >= 0]
+            if gone:
+                pool.give(list(reversed(gone)), rc.request)
+            del rc.tables[g][pages:]
+            rc.first_held[g] = min(rc.first_held[g], len(rc.tables[g]))
+        rc.num_tokens = rows
+
     # -- what a step needs ---------------------------------------------------------
 
     def slots_for(self, rc: RequestCache, g: int, start: int, count: int) -> "np.ndarray":

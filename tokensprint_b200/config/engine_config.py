@@ -73,6 +73,12 @@ class Config:
     cache_recent: int = 64
     cache_first: int = 4
     cache_slack: int = 64
+    # speculate > 0: every decoded token is followed by guesses, up to `speculate_branches` chains of up to `speculate` tokens that followed earlier
+    # occurrences of the request's last 1 to `speculate_suffix` tokens; a step checks them all and keeps those that the model's probabilities
+    # accept, so that the tokens are distributed as without (greedy ones: are the same).  For models whose layers are all plain attention; steps do not overlap.
+    speculate: int = 0
+    speculate_branches: int = 1
+    speculate_suffix: int = 4
 
     def __post_init__(self) -> None:
         if not os.path.isdir(self.model):
@@ -91,5 +97,9 @@ class Config:
         self.dtype = canonical_dtype(self.dtype)
         if self.cache_format not in ("model", "kv4"):
             raise ValueError(f"cache_format must be 'model' or 'kv4', got {self.cache_format!r}")
+        if self.speculate < 0 or self.speculate_branches < 1 or self.speculate_suffix < 1:
+            raise ValueError("speculate must not be negative, speculate_branches and speculate_suffix must be positive")
+        if self.speculate and self.cache_format != "model":
+            raise ValueError("speculate needs cache_format 'model'")
         if self.cache_budget < 0 or (self.cache_budget and self.cache_format != "kv4"):
             raise ValueError("cache_budget must not be negative, and needs cache_format 'kv4'")

@@ -19,6 +19,7 @@ from tokensprint_b200 import ops
 from tokensprint_b200.config.engine_config import Config, SamplingParams
 from tokensprint_b200.engine.runner import ModelRunner, StepEntry
 from tokensprint_b200.engine.scheduler import Scheduler
+from tokensprint_b200.engine.speculation import Speculator
 from tokensprint_b200.engine.sequence import UNKNOWN_TOKEN, Sequence
 from tokensprint_b200.models.model import Model
 from tokensprint_b200.sampling.sampler import Sampler, sample_key
@@ -108,6 +109,10 @@ class LLMEngine:
         # (sequences, which of them are sampled for, the positions of their tokens, the ids' ticket).
         self.overlap = bool(getattr(config, "overlap_steps", True))
         self._inflight = None
+        self.speculator: Optional[Speculator] = None
+        if getattr(config, "speculate", 0):
+            self.speculator = Speculator(self.model_runner, config.speculate, config.speculate_branches, config.speculate_suffix)
+            self.overlap = False  # what a step drafts from is what the step before has accepted
         self.stats: Optional[StepStats] = None
 
     def collect_stats(self, kernels: bool = False) -> StepStats:
@@ -176,11 +181,46 @@ class LLMEngine:
             self.stats.end(begun, kind, tokens)
             self._step_begun = None
 
+    def _step_speculative(self) -> list[Sequence]:
+        """One step in which every decoding request brings a tree of drafted tokens; returns the requests that finished."""
+        begun = self.stats.begin() if self.stats is not None else None
+        self.speculator.propose(self.scheduler.running)
+        seqs = sorted(self.scheduler.schedule(), key=lambda s: s.tree is None)  # (stable: trees first)
+        trees = [s for s in seqs if s.tree is not None]
+        portions = seqs[len(trees) :]
+        entries = [StepEntry(s.cache, s.tree.tokens, s.num_cached_tokens, range(len(s.tree)), parents=s.tree.parents) for s in trees]
+        need = []
+        for i, s in enumerate(portions):
+            start, n = s.num_cached_tokens, s.num_new_tokens
+            ends = start + n == len(s)
+            entries.append(StepEntry(s.cache, s.token_ids[start : start + n], start, [n - 1] if ends else [], parents=[-1] if n == 1 and trees else None))
+            if ends:
+                need.append(i)
+        if trees and portions:  # (a portion of one token goes with the trees, behind those that are checked)
+            order = sorted(range(len(entries)), key=lambda i: entries[i].parents is None)
+            entries = [entries[i] for i in order]
+            portions = [portions[i - len(trees)] for i in order[len(trees) :]]
+            need = [i for i, s in enumerate(portions) if s.num_cached_tokens + s.num_new_tokens == len(s)]
+        logits = self.model_runner.step(entries)
+        checked = sum(len(s.tree) for s in trees)
+        ticket = self.sampler.sample_async(logits[checked:], [portions[i].temperature for i in need],
+                                           [sample_key(portions[i].seed, portions[i].sample_stream, len(portions[i])) for i in need])
+        tokens = self.speculator.verify(logits[:checked], trees) if trees else []
+        if begun is not None:
+            self.stats.end(begun, "prefill" if not trees else "mixed" if portions else "decode", sum(s.num_new_tokens for s in seqs))
+        sampled = ticket.result()
+        ops.check_device_errors()
+        self.scheduler.postprocess_trees(trees, tokens)
+        self.scheduler.postprocess(portions, sampled, need)
+        return [s for s in seqs if s.is_finished]
+
     def step(self) -> tuple[list[tuple[int, list[int]]], int]:
         """One step.  Returns the requests that finished, as (id, completion token ids), and the
         number of their tokens.  With overlapping steps a call launches the next step and then
         reads the ids of the step before, so a request's end is reported one call later."""
-        if not self.overlap:
+        if self.speculator is not None:
+            finished = self._step_speculative()
+        elif not self.overlap:
             seqs, need, logits, temps, keys = self._launch()
             ticket = self.sampler.sample_async(logits, temps, keys)
             self._step_launched()

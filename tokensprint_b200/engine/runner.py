@@ -39,6 +39,9 @@ class StepEntry:
     # A single token that the host does not know yet: row `feed` of the ids that the step's
     # caller names (what an earlier step sampled, still on the device) takes the place of tokens[0].
     feed: int = -1
+    # `tokens` are the nodes of a tree of drafted tokens (the first is certain, at position `start`; a node stands one position behind its
+    # parent, its row in the cache is the next one all the same): every node's parent, by its place among `tokens` (-1: none).
+    parents: Optional[Sequence[int]] = None
 
 
 @dataclass
@@ -168,6 +171,8 @@ class ModelRunner:
         self._capture_stream: Optional[torch.cuda.Stream] = None
         self.graph_launches = 0  # kernels of this library replayed inside graphs so far
         self._sizing_step = False
+        self._last_trees: Optional[StepContext] = None  # the last step that brought trees of drafted tokens
+        self._row_pools: Optional[tuple] = None
         self.sizing: Optional[dict] = None  # how the page count was derived, when it came from free memory
 
         if num_pages is None:
@@ -290,7 +295,7 @@ class ModelRunner:
         # the logits keep the order of the entries as they were given.
         row_base = None
         singles = sum(1 for n in lens if n == 1)
-        if 0 < singles < B:
+        if 0 < singles < B and all(e.parents is None for e in entries):
             order = sorted(range(B), key=lambda i: lens[i] != 1)  # stable: each kind keeps its order
             if order != list(range(B)):
                 base, acc = [0] * B, 0
@@ -302,6 +307,11 @@ class ModelRunner:
                 lens = [lens[i] for i in order]
         else:
             singles = B if singles == B else 0
+        trees = sum(1 for e in entries if e.parents is not None)
+        if trees:
+            singles = 0
+            if any(e.parents is None for e in entries[:trees]) or row_base is not None and any(len(e.tokens) == 1 and e.parents is None for e in entries):
+                raise ValueError("entries with trees of drafted tokens come first in a step, and tokens that are decoded without drafts are trees of one node")
         widths = []
         for g in range(len(self.groups)):
             widths.append(max(1, max(-(-(e.start + n - e.cache.dropped) // P) for e, n in zip(entries, lens))))
@@ -324,7 +334,42 @@ class ModelRunner:
         step.rows_all = row_base is None and all(list(e.want) == list(range(n)) for e, n in zip(entries, lens))
         step.decode_seqs = singles
         step.sizing = self._sizing_step
+        if trees:
+            self._describe_trees(step, entries[:trees])
         return step, layout.view(dev, "rows"), R
+
+    def _describe_trees(self, step: StepContext, entries: Sequence[StepEntry]) -> None:
+        most = max(len(e.tokens) for e in entries)
+        words = -(-most // 64)
+        rows = []
+        for e in entries:
+            seen: list[int] = []
+            for i, p in enumerate(e.parents):
+                seen.append((seen[p] if p >= 0 else 0) | 1 << i)
+            rows += [[x >> 64 * w & (1 << 64) - 1 for w in range(words)] for x in seen]
+        mask = torch.from_numpy(np.array(rows, dtype=np.uint64).view(np.int64).reshape(len(rows), words)).pin_memory()
+        step.tree_seqs, step.tree_tokens, step.tree_most = len(entries), len(rows), most
+        step.tree_mask = mask.to(self.device, non_blocking=True)
+        self.h2d_bytes += mask.numel() * 8
+        self._last_trees = step
+
+    def keep_drafted(self, path: torch.Tensor, counts: torch.Tensor) -> None:
+        """After a step with trees: the rows of the nodes that were accepted (ops.verify_drafts' path and counts, for the first entries of the step) to the
+        front of the step's rows, in every layer."""
+        step, self._last_trees = self._last_trees, None
+        if step is None:
+            return
+        from tokensprint_b200 import ops
+
+        if self._row_pools is None or self._row_pools[0] is not self.cache_tensors:
+            by_shape: dict[tuple, list[torch.Tensor]] = {}
+            for g, *pools in zip(self.cache_tensors.group_index, self.cache_tensors.k, self.cache_tensors.v):
+                for t in pools:
+                    if t is not None:
+                        by_shape.setdefault((g, tuple(t.shape)), []).append(t)
+            self._row_pools = (self.cache_tensors, [(g, ops.RowPools(pools)) for (g, _), pools in by_shape.items()])
+        for g, pools in self._row_pools[1]:
+            ops.keep_drafted_rows(pools, path, counts, step.cu_seqlens_q, step.context_lens, step.groups[g].block_table, self.page_size, path.shape[0])
 
     def _fill(self, host, layout: _Layout, entries: Sequence[StepEntry], lens: Sequence[int], row_marks=None, row_base=None) -> int:
         """Writes the step's index arrays into `host` (a numpy view of pinned memory).  A
@@ -383,7 +428,13 @@ class ModelRunner:
                 if ids.min() < 0 or ids.max() >= self.vocab_size:
                     raise ValueError(f"request {rc.request!r}: token id outside 0..{self.vocab_size - 1}")
                 tok[t0 : t0 + n] = ids
-                pos[t0 : t0 + n] = np.arange(e.start, e.start + n)
+                if e.parents is None:
+                    pos[t0 : t0 + n] = np.arange(e.start, e.start + n)
+                else:
+                    if len(e.parents) != n or any(not -1 <= p < i for i, p in enumerate(e.parents)):
+                        raise ValueError(f"request {rc.request!r}: a tree's nodes hang on nodes before them")
+                    for i, p in enumerate(e.parents):
+                        pos[t0 + i] = e.start if p < 0 else pos[t0 + p] + 1
                 sidx[t0 : t0 + n] = b
             cu[b + 1] = t0 + n
             ctx_lens[b] = row + n

@@ -85,6 +85,10 @@ class Scheduler:
         """How many of the tokens it has not cached yet `seq` runs in a step with `budget` left:
         all of them, cut to the budget where portions are allowed, and never past the model's length."""
         share = len(seq) - seq.num_cached_tokens
+        if seq.tree is not None:
+            if len(seq.tree) > budget:
+                seq.tree = seq.tree.root()
+            return len(seq.tree)
         if self.enable_chunked:
             share = min(share, budget)
         return min(share, self.max_model_len - 1 - seq.num_cached_tokens)
@@ -92,6 +96,8 @@ class Scheduler:
     def _reserve(self, seq: Sequence, share: int) -> bool:
         """Pages for the next `share` tokens of a sequence that has a cache; False: not now."""
         first = seq.num_cached_tokens
+        if share > 1 and seq.tree is not None and not self.cache_manager.can_extend(seq.cache, first, first + share):
+            seq.tree, share = seq.tree.root(), 1  # the drafts find no pages
         if not self.cache_manager.can_extend(seq.cache, first, first + share):
             return False
         self.cache_manager.extend(seq.cache, first, first + share)
@@ -115,7 +121,7 @@ class Scheduler:
             if seq.status != SequenceStatus.RUNNING:
                 break  # it gave up its own place; it was the last one
             step.append(seq)
-            budget -= share
+            budget -= seq.num_new_tokens
             place += 1
         return budget, evicted
 
@@ -174,6 +180,7 @@ class Scheduler:
             seq.cache = None
         seq.num_cached_tokens = 0
         seq.num_new_tokens = 0
+        seq.tree = None
 
     def _ends_by_count(self, seq: Sequence) -> bool:
         """Ends that depend on lengths alone: the request's max_tokens, the model's length."""
@@ -206,6 +213,19 @@ class Scheduler:
             if (token == self.eos and not seq.ignore_eos) or self._ends_by_count(seq):
                 self._finish(seq)
         self._commit(seqs)
+
+    def postprocess_trees(self, seqs: list[Sequence], tokens: list[list[int]]) -> None:
+        """After a step that checked trees: `tokens[i]` are the accepted drafts of `seqs[i]` and the token behind them."""
+        for seq, fresh in zip(seqs, tokens):
+            seq.num_cached_tokens += len(fresh)  # the tree's first node and the accepted ones
+            seq.num_new_tokens = 0
+            seq.tree = None
+            self.cache_manager.retract(seq.cache, seq.num_cached_tokens)
+            for token in fresh:
+                seq.append_token(token)
+                if (token == self.eos and not seq.ignore_eos) or self._ends_by_count(seq):
+                    self._finish(seq)
+                    break
 
     # -- steps that overlap ------------------------------------------------------------------
     #

@@ -52,6 +52,8 @@ class Sequence:
         # Steps that overlap: tokens appended as UNKNOWN_TOKEN and not yet filled in; the row that
         # holds this sequence's newest id among the ids the last step sampled; the position of an
         # end-of-sequence token once one was seen (what later steps sampled for it is dropped).
+        # Speculation: the tree of drafted tokens that the next step checks, its first node the newest token; None: none.
+        self.tree = None
         self.unresolved = 0
         self.sample_row = -1
         self.ended_at = -1

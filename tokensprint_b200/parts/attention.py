@@ -208,6 +208,13 @@ class AttentionMixer(Mixer):
             return f"a 4-bit cache takes heads of {ops.KV4_HEAD_DIMS}, got {self.head_dim}"
         return None
 
+    def tree_refusal(self) -> Optional[str]:
+        if self.general or self.joint_norm or self.chunk or self.sink is not None:
+            return "attention over trees of drafted tokens takes a norm per head, a rotation and a window, and none of the further options"
+        if not ops.attention_tree_supported(self.head_dim):
+            return f"attention over trees of drafted tokens takes heads of a multiple of 8 up to {ops.TREE_MAX_HEAD_DIM}, got {self.head_dim}"
+        return None
+
     def tensor_specs(self) -> list[TensorSpec]:
         H, nq, nkv, d, e = self.hidden_size, self.num_heads, self.num_kv_heads, self.head_dim, self.value_dim
         n = self.names
@@ -397,7 +404,32 @@ class AttentionMixer(Mixer):
 
     # -- attention proper ---------------------------------------------------
 
+    def _attend_trees(self, q, out, step: StepContext, cache: LayerCache, tables) -> None:
+        """Trees of drafted tokens at the front of the batch, portions of prompts behind them."""
+        nq, nkv, d, n, T, B = self.num_heads, self.num_kv_heads, self.head_dim, step.tree_seqs, step.tree_tokens, step.num_seqs
+        ops.attention_tree(
+            q[:T], cache.k_pages, cache.v_pages, out[:T], step.tree_mask, step.cu_seqlens_q[: n + 1], step.context_lens[:n], tables.block_table[:n],
+            step.page_size, n, step.tree_most, step.max_context_len, nq, nkv, d, self.scale, window=self.window, positions=step.positions)
+        if n == B:
+            return
+        cu, lens, table = step.cu_seqlens_q[n:], step.context_lens[n:], tables.block_table[n:]
+        if q.dtype == torch.bfloat16 and ops.attention_tcgen05_supported(nq, nkv, d, step.page_size):
+            ops.attention_prefill_tcgen05(q, cache.k_pages, cache.v_pages, out, cu, lens, table, step.page_size, B - n, step.max_seqlen_q, nq, nkv, self.scale,
+                                          self.window)
+        elif q.dtype == torch.bfloat16 and ops.attention_mma_supported(d):
+            ops.attention_paged_mma(q, cache.k_pages, cache.v_pages, out, cu, lens, table, step.seq_index - n, step.page_size, B - n, step.max_seqlen_q, nq, nkv, d,
+                                    self.scale, self.window)
+        elif ops.attention_float32_supported(d, q, cache.k_pages, cache.v_pages, out):
+            ops.attention_paged_float32(q, cache.k_pages, cache.v_pages, out, cu, lens, table, step.page_size, B - n, step.max_seqlen_q, nq, nkv, d, self.scale,
+                                        self.window)
+        else:
+            ops.attention_paged_simple(q[T:], cache.k_pages, cache.v_pages, out[T:], step.positions[T:], step.seq_index[T:], tables.block_table, step.page_size,
+                                       nq, nkv, d, self.scale, self.window)
+
     def _attend(self, q, out, step: StepContext, cache: LayerCache, tables) -> None:
+        if step.tree_seqs:
+            self._attend_trees(q, out, step, cache, tables)
+            return
         nq, nkv, d = self.num_heads, self.num_kv_heads, self.kernel_dim
         scored = {"softcap": self.softcap, "head_sinks": self.head_sinks}
         if self.distance is not None:

@@ -153,6 +153,12 @@ class StepContext:
     # first in a step that also carries portions of prompts, so that a mixer may treat the two kinds apart)
     decode_seqs: int = 0
     rows_all: bool = False  # the logits of every token are wanted, in the tokens' order
+    # Trees of drafted tokens: how many sequences at the front of the batch bring one, their tokens together, the most of any, and which
+    # of its request's nodes each of them sees ([tree_tokens, words] i64, see ops.attention_tree).
+    tree_seqs: int = 0
+    tree_tokens: int = 0
+    tree_most: int = 0
+    tree_mask: Optional[torch.Tensor] = None
     # The step measures how much memory a step takes: a part that has several ways to work, which others
     # of the same size may take, goes the one with the most scratch.
     sizing: bool = False
@@ -328,6 +334,10 @@ class Mixer(Part):
     def kv4_refusal(self) -> Optional[str]:
         """Why this mixer cannot keep its cache in 4 bits; None: it can."""
         return f"{type(self).__name__} has no 4-bit form"
+
+    def tree_refusal(self) -> Optional[str]:
+        """Why this mixer cannot run the nodes of a tree of drafted tokens in one step; None: it can."""
+        return f"{type(self).__name__} takes a request's tokens one behind the other"
 
     def forward(self, x: torch.Tensor, step: StepContext, cache: LayerCache) -> torch.Tensor:
         raise NotImplementedError

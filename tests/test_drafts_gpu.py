@@ -244,6 +244,44 @@ def test_attention_captured_and_replayed_on_other_lengths(d, dtype):
         check(cut, out)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_many_requests(dtype):
+    rng = random.Random(7)
+    s = step([(n := rng.randrange(1, 300), rng.randrange(0, min(n, 9) + 1)) for _ in range(150)], 4, 2, 64, 16, dtype, seed=13)
+    check(s, attend(s))
+
+
+def test_attention_on_two_streams_at_once():
+    steps = [step([(900, 20), (1400, 7)], 16, 4, 128, 16, BF16, seed=14), step([(2000, 33), (64, 3), (500, 1)], 16, 4, 128, 16, BF16, seed=15)]
+    want = [attend(s) for s in steps]
+    sides = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[i].append(attend(steps[i]))
+    torch.cuda.synchronize()
+    for i, s in enumerate(steps):
+        check(s, want[i])
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_caches_that_begin_beside_16_bytes_are_refused():
+    s = step([(40, 3)], 4, 2, 64, 16, BF16)
+    s["k"] = torch.empty(s["k"].numel() + 1, dtype=BF16, device=DEV)[1:].view(s["k"].shape)
+    with pytest.raises(ops.KernelError, match="16 bytes"):
+        attend(s)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_queries_that_begin_beside_16_bytes(d):
+    s = step([(400, 9), (70, 2)], 8, 2, d, 16, BF16, seed=16)
+    q = torch.empty(s["q"].numel() + 1, dtype=BF16, device=DEV)[1:].view(s["q"].shape)
+    s["q"] = q.copy_(s["q"])
+    check(s, attend(s))
+
+
 # ---------------------------------------------------------------------------
 # verification
 
@@ -330,6 +368,47 @@ def test_verification_of_rows_that_lie_apart(stride, dtype):
 def test_verification_of_large_vocabularies(V):
     s = verification([5, 9, 1], V, seed=1, temps=(0.8, 0.0, 1.0))
     check_verify(s, run_verify(s))
+
+
+def test_verification_on_two_streams_at_once():
+    cases = [verification([9, 4, 1], 20011, seed=2, shape="chain", probs=True), verification([6] * 12, 5003, seed=3)]
+    want = [run_verify(s) for s in cases]
+    sides = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for s, side in zip(cases, sides):
+            with torch.cuda.stream(side):
+                got.append(run_verify(s))
+        assert got == want
+
+
+def test_verification_without_rows():
+    """Requests without nodes accept nothing and draw nothing, and nodes behind the rows of logits are none."""
+    path, fresh = (torch.full((2, 3), 77, dtype=torch.int32, device=DEV) for _ in range(2))
+    counts = torch.full((2,), 77, dtype=torch.int32, device=DEV)
+    for T, cu, nodes in ((0, [0, 0, 0], [0, 0]), (0, [0, 2, 3], [0, 0]), (2, [0, 0, 3], [0, 2]), (2, [5, 7, 9], [0, 0])):
+        ops.verify_drafts(torch.zeros((T, 9), device=DEV), ints([0] * T), ints([-1] + [0] * (T - 1))[:T], ints(cu), torch.zeros(2, device=DEV), torch.zeros(T, device=DEV),
+                          torch.zeros(2, dtype=torch.int64, device=DEV), path, fresh, counts, 2, 3)
+        # (equal logits: the first entry is the largest, and the child's)
+        assert counts.tolist() == [1 if n == 2 else 0 for n in nodes]
+        assert path.tolist() == [[0, 1, -1] if n == 2 else [-1] * 3 for n in nodes] and fresh.tolist() == [[0, 0, -1] if n == 2 else [-1] * 3 for n in nodes]
+
+
+@pytest.mark.parametrize("T", [1e-9, 1e30, 3e38, math.inf])
+def test_temperatures_at_the_ends(T):
+    """The smallest leave the largest entry, the largest every entry that is a number, alike (five sigma)."""
+    B, V = 4000, 8
+    logits = torch.tensor([1.0, -math.inf, 3.0, math.nan, -2.0, 2.0, -math.inf, 0.0], device=DEV).repeat(B, 1)
+    path, fresh = (torch.empty((B, 1), dtype=torch.int32, device=DEV) for _ in range(2))
+    counts = torch.empty(B, dtype=torch.int32, device=DEV)
+    ops.verify_drafts(logits, ints([0] * B), ints([-1] * B), torch.arange(B + 1, device=DEV).int(), torch.full((B,), T, device=DEV), torch.zeros(B, device=DEV),
+                      torch.arange(B, device=DEV) * 0x9E3779B97F4A7C1, path, fresh, counts, B, 1)
+    seen = torch.bincount(fresh[:, 0].long(), minlength=V).tolist()
+    if T < 1:
+        assert seen[2] == B
+    else:
+        assert sum(seen[i] for i in (0, 2, 4, 5, 7)) == B and all(abs(seen[i] - B / 5) < 5 * (B * 0.16) ** 0.5 for i in (0, 2, 4, 5, 7))
 
 
 def test_logits_that_are_no_numbers():
@@ -469,6 +548,15 @@ def test_paths_and_pages_that_do_not_exist_move_nothing():
     assert torch.equal(pools[0], want)
     ops.keep_drafted_rows(rows, ints([[0, 3]]), ints([1]), ints([0, 6]), ints([2]), ints([[0]]), 16, 1)
     assert torch.equal(pools[0], want)
+
+
+def test_pools_that_stand_twice_are_refused():
+    """Two blocks would move the same rows."""
+    whole = torch.zeros((6, 16, 2, 8), device=DEV)
+    for pools in ([whole, whole], [whole[:4], whole[2:]], [whole[:2], whole[4:], whole[1:3]]):
+        with pytest.raises(ops.KernelError, match="twice"):
+            ops.RowPools(pools)
+    ops.RowPools([whole[4:], whole[:2], whole[2:4]])
 
 
 # ---------------------------------------------------------------------------

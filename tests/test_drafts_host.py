@@ -62,6 +62,7 @@ def attend(**change):
     ({"window": -1}, "negative"),
     ({"softcap": -1.0}, "negative"),
     ({"softcap": float("nan")}, "negative"),
+    ({"softcap": float("inf")}, "finite"),
     ({"head_sinks": lambda: fake(5, dtype=F32)}, "one entry per query head"),
     ({"head_sinks": lambda: fake(4, dtype=BF16)}, "float32"),
 ])
@@ -165,6 +166,7 @@ def look(**change):
     ({"history": lambda: fake(2, 90, dtype=I64)}, "int32 CUDA matrix"),
     ({"history": lambda: fake(1, 90)}, "row per request"),
     ({"history": lambda: fake(2, 0)}, "empty"),
+    ({"history": lambda: fake(2, (1 << 30) + 1)}, "at most 1073741824 tokens"),
     ({"history": lambda: fake(1, 90).expand(2, 90)}, "overlap"),
     ({"depth": 0}, "depth 1"),
     ({"depth": 65}, "depth 1"),

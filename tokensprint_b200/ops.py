@@ -8,6 +8,7 @@ the limit in words; nothing falls back to another implementation.
 from __future__ import annotations
 
 import ctypes
+import math
 import os as _os
 import struct as _struct
 from typing import Optional
@@ -2897,11 +2898,11 @@ def kv4_evict(pool: torch.Tensor, sums: torch.Tensor, block_table: torch.Tensor,
 TREE_MAX_NODES = 256
 TREE_MAX_HEAD_DIM = 256
 VERIFY_MAX_VOCAB = 1 << 20
-LOOKUP_MAX_BRANCHES, LOOKUP_MAX_DEPTH, LOOKUP_MAX_SUFFIX = 16, 64, 16
+LOOKUP_MAX_BRANCHES, LOOKUP_MAX_DEPTH, LOOKUP_MAX_SUFFIX, LOOKUP_MAX_LENGTH = 16, 64, 16, 1 << 30
 # Entry points that take one block of arguments, laid out as the C structs beside them.
 for _name in ("ts_verify_drafts", "ts_keep_drafted_rows", "ts_lookup_drafts"):
     _SIGNATURES[_name] = [ctypes.c_char_p]
-_VERIFY_ARGS = _struct.Struct("@12P2q5i4x").pack
+_VERIFY_ARGS = _struct.Struct("@12P2q6i").pack
 _KEEP_ARGS = _struct.Struct("@7Pq7i4x").pack
 _LOOKUP_ARGS = _struct.Struct("@6Pq6i").pack
 TREE_TCGEN05_HEAD_DIMS = (64, 128)
@@ -3004,8 +3005,8 @@ def _refuse_attention_tree(q, k_cache, v_cache, out, tree_mask, cu_seqlens_q, co
         raise KernelError("attention_tree: block_table must be [B,max_blocks]")
     if cu_seqlens_q.numel() < num_seqs + 1 or context_lens.numel() < num_seqs:
         raise KernelError("attention_tree: cu_seqlens_q/context_lens are shorter than the batch")
-    if num_seqs > 65535 or max_context < 0 or window < 0 or not softcap >= 0.0:
-        raise KernelError("attention_tree: at most 65535 requests, and max_context, window and softcap must not be negative")
+    if num_seqs > 65535 or max_context < 0 or window < 0 or not 0.0 <= softcap < math.inf:
+        raise KernelError("attention_tree: at most 65535 requests, max_context and window not negative, softcap 0 or positive and finite")
     if window > 0:
         if positions is None:
             raise KernelError("attention_tree: a window needs the nodes' positions")
@@ -3069,7 +3070,7 @@ def attention_tree(
         and len(ks) == 4 and ks == v_cache.shape and ks[1] == page_size and ks[2] == nkv and ks[3] == d and page_size >= 1
         and 1 <= max_seqlen_q <= TREE_MAX_NODES and len(ms) == 2 and ms[0] >= T and 64 * ms[1] >= max_seqlen_q
         and len(ts) == 2 and ts[0] >= num_seqs and ts[1] >= 1 and cu_seqlens_q.numel() > num_seqs and context_lens.numel() >= num_seqs
-        and num_seqs <= 65535 and max_context >= 0 and window >= 0 and softcap >= 0.0
+        and num_seqs <= 65535 and max_context >= 0 and window >= 0 and 0.0 <= softcap < math.inf
         and (window == 0 or positions is not None and positions.dtype is torch.int32 and positions.is_contiguous() and positions.get_device() == here
              and positions.numel() >= T)
         and (head_sinks is None or head_sinks.dtype is torch.float32 and head_sinks.is_contiguous() and head_sinks.get_device() == here
@@ -3182,17 +3183,17 @@ def verify_drafts(
     ):
         _refuse_verify_drafts(logits, tokens, parents, cu_seqlens, temperatures, uniforms, keys, path, next_tokens, counts, num_seqs, max_nodes, draft_probs)
     T, V = shape
-    if num_seqs < 1 or T < 1:
+    if num_seqs < 1:
         return
     _check("verify_drafts", _fn("ts_verify_drafts")(_VERIFY_ARGS(
         logits.data_ptr(), 0 if draft_probs is None else draft_probs.data_ptr(), tokens.data_ptr(), parents.data_ptr(), cu_seqlens.data_ptr(), temperatures.data_ptr(),
         uniforms.data_ptr(), keys.data_ptr(), path.data_ptr(), next_tokens.data_ptr(), counts.data_ptr(), _stream(), max(logits.stride(0), V),
-        0 if draft_probs is None else max(draft_probs.stride(0), V), V, num_seqs, path.shape[1], int(logits.dtype is torch.bfloat16), 0)))
+        0 if draft_probs is None else max(draft_probs.stride(0), V), V, num_seqs, path.shape[1], int(logits.dtype is torch.bfloat16), 0, T)))
 
 
 class RowPools:
     """The paged pools [pages,page,...] of a model's layers, keys and values, as `keep_drafted_rows` takes them: all of one shape and
-    type, contiguous, on one device.  Made once for the life of the cache (it keeps the pools, and their addresses on the device)."""
+    type, contiguous, on one device, none twice.  Made once for the life of the cache (it keeps the pools, and their addresses on the device)."""
 
     def __init__(self, pools: "list[torch.Tensor]") -> None:
         if not pools:
@@ -3202,6 +3203,9 @@ class RowPools:
             _cuda_contig("RowPools: a pool", t, first.dtype)
             if t.dim() < 3 or t.shape != first.shape or t.device != first.device:
                 raise KernelError(f"RowPools: pools [pages,page,...] of one shape and device, got {tuple(first.shape)} and {tuple(t.shape)}")
+        starts = sorted(t.data_ptr() for t in pools)
+        if any(b - a < first.numel() * first.element_size() for a, b in zip(starts, starts[1:])):
+            raise KernelError("RowPools: a pool that stands twice, or overlaps another (its rows would move twice)")
         self.pools = list(pools)
         self.num_pages, self.page_size = int(first.shape[0]), int(first.shape[1])
         self.row_bytes = first[0, 0].numel() * first.element_size() if first.numel() else 0
@@ -3253,6 +3257,8 @@ def lookup_drafts(history: torch.Tensor, lengths: torch.Tensor, tokens: torch.Te
         raise KernelError(f"lookup_drafts: history must be an int32 CUDA matrix with a row per request, got {tuple(history.shape)}")
     if history.shape[1] < 1 or history.shape[0] > 1 and history.stride(0) < history.shape[1]:
         raise KernelError("lookup_drafts: rows of history are empty or overlap")
+    if history.shape[1] > LOOKUP_MAX_LENGTH:
+        raise KernelError(f"lookup_drafts: at most {LOOKUP_MAX_LENGTH} tokens a request, got {history.shape[1]}")
     if not (1 <= depth <= LOOKUP_MAX_DEPTH and 1 <= branches <= LOOKUP_MAX_BRANCHES and 1 <= min_suffix <= max_suffix <= LOOKUP_MAX_SUFFIX):
         raise KernelError(f"lookup_drafts: depth 1..{LOOKUP_MAX_DEPTH}, branches 1..{LOOKUP_MAX_BRANCHES} and 1 <= min_suffix <= max_suffix <= {LOOKUP_MAX_SUFFIX}, "
                           f"got {depth}, {branches}, {min_suffix}, {max_suffix}")

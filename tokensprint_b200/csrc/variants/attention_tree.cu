@@ -60,107 +60,119 @@ __device__ __forceinline__ bool sees(const Params& p, int token, int pos, int j,
 }
 
 // ---------------------------------------------------------------------------
-// CUDA cores, both types: 16 RPT rows against blocks of 64 keys, RPT x 4 scores and RPT x D/16 outputs a thread.  Arithmetic in float32.
+// mma.sync: 16 WM rows, of which every warp holds 16, against blocks of keys, cut among 8 / WM warps; a warp walks its keys with maxima and sums of its own, and the
+// CTA joins its warps at the end.  bfloat16: products as they are, weights rounded to bfloat16 (their values' type).  float32: every operand is the sum of
+// two tf32 (11 bits each, rounded to nearest), a product three: h h' + h l' + l h'; what is left out is below 2^-21 of it, where a float32 sum is off by 2^-24 a
+// term.
+//
+// The order of the entries inside a product does not matter, and the order of columns of the result is put right at the end: a lane takes 16 neighbouring bytes of
+// a row of queries or keys as its share of two products (for float32 values: four neighbouring columns of a row as its share of four), one load without conflicts.
+//
+// What bounds it: float32 the tensor cores' old path (a product of 16 x 8 x 8 takes 8 cycles, three a term: 65 TFLOP/s of whole terms a GPU) and the
+// instructions that cut operands in two.
 
-constexpr int BN = 64, TH = 256;
-constexpr int KS = D + 4;  // row of keys in shared memory: 16-byte pieces of 8 neighbouring rows lie in different banks
-constexpr int PS = BN + 4;
-constexpr int DC = (D + 63) / 64;  // 16-byte pieces of an output row per thread
+constexpr int TH = 256;
 
-template <int RPT>
-constexpr int rows_smem() { return (16 * RPT * KS + BN * KS + BN * D + 16 * RPT * PS) * 4 + 2 * BN * 8; }
+template <typename T, int WM>
+struct Tile {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int WN = 8 / WM;                                 // warps that share a block's keys
+  static constexpr int BN = !F32 && WN == 8 ? 128 : 64;             // keys of a block (a warp's at least a product's: 8 in float32, 16 in bfloat16)
+  static constexpr int RM = 16 * WM;
+  static constexpr int NT = BN / WN / 8;                            // 8s of keys per warp
+  static constexpr int CHUNK = 64 / sizeof(T);                      // columns that four lanes take at a time
+  static constexpr int DK = (D + CHUNK - 1) / CHUNK * CHUNK;        // columns of queries and keys, zeros behind D
+  static constexpr int KB = DK * sizeof(T) + (DK * sizeof(T) % 128 == 0 ? 64 : 0);  // bytes of such a row: two rows of 64 bytes lie in different banks
+  static constexpr int DV = F32 ? (D + 31) / 32 * 32 : (D + 15) / 16 * 16;  // columns of values (what stands behind D goes to columns that nobody reads)
+  static constexpr int VB = DV * sizeof(T) + 16;
+  static constexpr int OT = DV / 8;
+  static constexpr int K_AT = RM * KB, V_AT = K_AT + BN * KB, END = V_AT + BN * VB;
+  static constexpr int OUT = 8 * 16 * DV * 4;                       // the warps' results, when all else has been read
+  static constexpr int SMEM = END > OUT ? END : OUT;
+  static constexpr int CTAS = SMEM <= 110 * 1024 && (D <= 64 || (D <= 128 && WM <= 4)) ? 2 : 1;
+};
 
-__device__ __forceinline__ void copy16(float* dst, const void* src, bool there) {
+__device__ __forceinline__ void copy16(unsigned char* dst, const void* src, bool there) {
   const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
   const int bytes = there ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(bytes) : "memory");
 }
-
-// A block's rows into shared memory; `slots`: where each begins in the pool, in entries, or -1.
-template <typename T>
-__device__ __forceinline__ void load_rows(float* dst, int stride, const T* pool, const long long* slots) {
-  if constexpr (sizeof(T) == 4) {
-    for (int i = threadIdx.x; i < BN * (D / 4); i += TH) {
-      const int r = i / (D / 4), c = i % (D / 4) * 4;
-      const long long at = slots[r];
-      copy16(dst + r * stride + c, pool + (at < 0 ? 0 : at + c), at >= 0);
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  } else {
-    for (int i = threadIdx.x; i < BN * (D / 8); i += TH) {
-      const int r = i / (D / 8), c = i % (D / 8) * 8;
-      const long long at = slots[r];
-      const uint4 w = at < 0 ? make_uint4(0u, 0u, 0u, 0u) : *reinterpret_cast<const uint4*>(pool + at + c);
-      float4* to = reinterpret_cast<float4*>(dst + r * stride + c);
-      to[0] = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-      to[1] = make_float4(__uint_as_float(w.z << 16), __uint_as_float(w.z & 0xffff0000u), __uint_as_float(w.w << 16), __uint_as_float(w.w & 0xffff0000u));
-    }
+// A block's rows into shared memory; `slots`: where each begins in the pool, in entries, or -1 (zeros).
+template <typename T, int BN>
+__device__ __forceinline__ void load_rows(unsigned char* dst, int stride, const T* pool, const long long* slots) {
+  constexpr int PER = D * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T);
+  for (int i = threadIdx.x; i < BN * PER; i += TH) {
+    const int r = i / PER, c = i % PER;
+    const long long at = slots[r];
+    copy16(dst + r * stride + c * 16, pool + (at < 0 ? 0 : at + c * E), at >= 0);
   }
+  asm volatile("cp.async.commit_group;" ::: "memory");
 }
-template <typename T, int LEFT>
+template <int LEFT>
 __device__ __forceinline__ void rows_landed() {
-  if constexpr (sizeof(T) == 4) asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
   __syncthreads();
 }
 
-// two float32 in one 64-bit register, and their packed product and sum: twice the work of a scalar instruction, whose three operands the registers deliver 2.6
-// times a cycle and SM, the packed one's 1.9 times
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
+__device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
+// x as the sum of two tf32, each rounded to nearest (bits of an infinity stay; a NaN stays in the lower part at the least)
+__device__ __forceinline__ void cut(uint32_t x, uint32_t& high, uint32_t& low) {
+  high = (x + 0x1000u) & 0xffffe000u;
+  low = (__float_as_uint(__uint_as_float(x) - __uint_as_float(high)) + 0x1000u) & 0xffffe000u;
 }
-__device__ __forceinline__ ulonglong2 load_pairs(const float* x) { return *reinterpret_cast<const ulonglong2*>(x); }
-
-// The first row of the cache that any token of the request sees (0 without a window), worked out by one warp.
-__device__ __forceinline__ int first_row(const Params& p, int q_begin, int t, int first) {
-  if (p.window == 0) return 0;
-  int lowest = INT_MAX;
-  for (int i = threadIdx.x & 31; i < t; i += 32) lowest = min(lowest, p.positions[q_begin + i]);
-  for (int o = 16; o > 0; o >>= 1) lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, o));
-  const long long lo = (long long)lowest - p.window + 1;
-  return (int)(lo < 0 ? 0 : lo > first ? max(first, 0) : lo);
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float power2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-template <typename T, int RPT>
-__global__ void __launch_bounds__(TH) tree_rows_kernel(const Params p) {
+// The lowest and the highest position of a request's nodes (with a window), by every warp for itself.
+__device__ __forceinline__ int2 position_range(const Params& p, int q_begin, int t) {
+  int lowest = INT_MAX, highest = INT_MIN;
+  for (int i = threadIdx.x & 31; i < t; i += 32) {
+    const int x = p.positions[q_begin + i];
+    lowest = min(lowest, x), highest = max(highest, x);
+  }
+  return make_int2(__reduce_min_sync(0xffffffffu, lowest), __reduce_max_sync(0xffffffffu, highest));
+}
+
+template <typename T, int WM>
+__global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const Params p) {
   ts_pdl_prologue();
-  extern __shared__ __align__(16) float smem[];
-  constexpr int RM = 16 * RPT;
-  float* Qs = smem;
-  float* Ks = Qs + RM * KS;
-  float* Vs = Ks + BN * KS;
-  float* Ps = Vs + BN * D;
-  long long* slots_s = reinterpret_cast<long long*>(Ps + RM * PS);  // [2][BN]
-  __shared__ int lo_s;
+  using L = Tile<T, WM>;
+  constexpr bool F32 = L::F32;
+  constexpr int BN = L::BN, RM = L::RM, NT = L::NT, WN = L::WN, E = 16 / (int)sizeof(T);
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ long long slots_s[2][BN];
+  __shared__ float2 ml_s[8][16];
+  unsigned char *Qs = smem, *Ks = smem + L::K_AT, *Vs = smem + L::V_AT;
   const int split = blockIdx.x, hk = blockIdx.y % p.nkv, tile = blockIdx.y / p.nkv, b = blockIdx.z;
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  const int wm = warp / WN, wn = warp % WN;
   const int q_begin = p.cu[b], t = p.cu[b + 1] - q_begin, n = p.context[b], first = n - t;
   const int G = p.nq / p.nkv, rows = t * G, r0 = tile * RM;
   if (t <= 0 || r0 >= rows) return;
-  if (tid < 32) {
-    const int lo = first_row(p, q_begin, t, first);
-    if (tid == 0) lo_s = lo;
+  // the first row that any node sees, and the row from which on a window hides nothing of what is before the step
+  int lo = 0, whole_from = 0;
+  if (p.window > 0) {
+    const int2 range = position_range(p, q_begin, t);
+    const long long from = (long long)range.x - p.window + 1;
+    lo = (int)(from < 0 ? 0 : from > first ? max(first, 0) : from);
+    whole_from = max(range.y - p.window + 1, 0);
   }
-  // queries: row r of the tile is token r / G, head r % G
-  const T* q = reinterpret_cast<const T*>(p.q);
-  for (int i = tid; i < RM * D; i += TH) {
-    const int r = r0 + i / D, c = i % D;
-    Qs[i / D * KS + c] = r < rows ? ts_to_float(q[((size_t)(q_begin + r / G) * p.nq + hk * G + r % G) * D + c]) : 0.f;
-  }
-  __syncthreads();
   // this CTA's blocks of keys: an even share of the request's
-  const int kb0 = lo_s / BN, blocks = n > 0 ? (n - 1) / BN - kb0 + 1 : 0;
+  const int kb0 = lo / BN, blocks = n > 0 ? (n - 1) / BN - kb0 + 1 : 0;
   const int per = (blocks + p.splits - 1) / p.splits, begin = kb0 + split * per, end = min(kb0 + blocks, begin + per);
   const int* table = p.table + (size_t)b * p.max_blocks;
   auto find_slots = [&](int blk) {
@@ -171,146 +183,217 @@ __global__ void __launch_bounds__(TH) tree_rows_kernel(const Params p) {
         const int page = table[e];
         if (page >= 0 && page < p.num_pages) at = (((long long)page * p.page + j % p.page) * p.nkv + hk) * D;
       }
-      slots_s[(blk & 1) * BN + tid] = at;
+      slots_s[blk & 1][tid] = at;
     }
   };
-  int token[RPT], pos[RPT];
-  float m[RPT], l[RPT];
-  uint64_t o[RPT][DC * 2];  // pairs of columns
-#pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    const int r = r0 + ty * RPT + i;
-    token[i] = r < rows ? q_begin + r / G : -1;
-    pos[i] = token[i] >= 0 && p.window > 0 ? p.positions[token[i]] : 0;
-    m[i] = -INFINITY, l[i] = 0.f;
-#pragma unroll
-    for (int c = 0; c < DC * 2; ++c) o[i][c] = 0ull;
-  }
   const T* K = reinterpret_cast<const T*>(p.k);
   const T* V = reinterpret_cast<const T*>(p.v);
   if (begin < end) {
     find_slots(begin);
     __syncthreads();
-    load_rows<T>(Ks, KS, K, slots_s + (begin & 1) * BN);
-    load_rows<T>(Vs, D, V, slots_s + (begin & 1) * BN);
+    load_rows<T, BN>(Ks, L::KB, K, slots_s[begin & 1]);
+    load_rows<T, BN>(Vs, L::VB, V, slots_s[begin & 1]);
   }
+  // queries: row r of the tile is token r / G, head r % G
+  const T* q = reinterpret_cast<const T*>(p.q);
+  for (int i = tid; i < RM * L::DK; i += TH) {
+    const int x = i / L::DK, r = r0 + x, c = i % L::DK;
+    *reinterpret_cast<T*>(Qs + x * L::KB + c * sizeof(T)) = r < rows && c < D ? q[((size_t)(q_begin + r / G) * p.nq + hk * G + r % G) * D + c] : ts_from_float<T>(0.f);
+  }
+  if (L::DK > D)  // (a product with zeros needs numbers beside them)
+    for (int i = tid; i < BN * (L::DK - D); i += TH)
+      *reinterpret_cast<T*>(Ks + i / (L::DK > D ? L::DK - D : 1) * L::KB + (D + i % (L::DK > D ? L::DK - D : 1)) * sizeof(T)) = ts_from_float<T>(0.f);
+  const bool works = r0 + wm * 16 < rows;
+  int token[2], pos[2];
+  float m[2], l[2], o[L::OT][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = r0 + wm * 16 + g + 8 * h;
+    token[h] = r < rows ? q_begin + r / G : -1;
+    pos[h] = token[h] >= 0 && p.window > 0 ? p.positions[token[h]] : 0;
+    m[h] = -INFINITY, l[h] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < L::OT; ++i)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) o[i][x] = 0.f;
+  const unsigned char *q_row = Qs + (wm * 16 + g) * L::KB + t4 * 16, *k_row = Ks + (wn * NT * 8 + g) * L::KB + t4 * 16;
+#pragma unroll 1
   for (int blk = begin; blk < end; ++blk) {
     const bool more = blk + 1 < end;
     if (more) find_slots(blk + 1);
-    rows_landed<T, 1>();
-    uint64_t sum2[RPT][4];  // of even and of odd entries
+    rows_landed<1>();
+    float s[NT][4];
 #pragma unroll
-    for (int i = 0; i < RPT; ++i)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum2[i][j] = 0ull;
-#pragma unroll 4
-    for (int c = 0; c < D; c += 4) {
-      ulonglong2 a[RPT], k4[4];
-#pragma unroll
-      for (int i = 0; i < RPT; ++i) a[i] = load_pairs(Qs + (ty * RPT + i) * KS + c);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) k4[j] = load_pairs(Ks + (tx + 16 * j) * KS + c);
-#pragma unroll
-      for (int i = 0; i < RPT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum2[i][j] = fma2(a[i].y, k4[j].y, fma2(a[i].x, k4[j].x, sum2[i][j]));
-    }
-    float s[RPT][4];
-#pragma unroll
-    for (int i = 0; i < RPT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = unpack2(sum2[i][j]).x + unpack2(sum2[i][j]).y;
-    __syncthreads();  // the keys have been read
-    if (more) load_rows<T>(Ks, KS, K, slots_s + ((blk + 1) & 1) * BN);
-    // seen by every token: rows before the step, and none that a window may hide
-    const bool open = blk * BN + BN <= first && p.window == 0;
-#pragma unroll
-    for (int i = 0; i < RPT; ++i) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = blk * BN + tx + 16 * j;
-        const bool seen = token[i] >= 0 && (open || sees(p, token[i], pos[i], key, n, first, q_begin));
-        s[i][j] = seen ? score_log2(p, s[i][j]) : -INFINITY;
-        top = fmaxf(top, s[i][j]);
-      }
-#pragma unroll
-      for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const float m_new = fmaxf(m[i], top);
-      const float corr = m_new == -INFINITY ? 1.f : exp2f(m[i] - m_new);
-      m[i] = m_new;
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float w = s[i][j] == -INFINITY ? 0.f : exp2f(s[i][j] - m_new);
-        Ps[(ty * RPT + i) * PS + tx + 16 * j] = w;
-        sum += w;
-      }
-#pragma unroll
-      for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      l[i] = l[i] * corr + sum;
-#pragma unroll
-      for (int c = 0; c < DC * 2; ++c) {
-        const float2 x = unpack2(o[i][c]);
-        o[i][c] = pack2(x.x * corr, x.y * corr);
-      }
-    }
-    if (more)
-      rows_landed<T, 1>();
-    else
-      rows_landed<T, 0>();
+      for (int x = 0; x < 4; ++x) s[j][x] = 0.f;
+    if (works) {
 #pragma unroll 2
-    for (int k = 0; k < BN; k += 4) {
-      float4 w[RPT];
+      for (int c = 0; c < L::DK / L::CHUNK; ++c) {
+        const uint4 a = *reinterpret_cast<const uint4*>(q_row + c * 64), a8 = *reinterpret_cast<const uint4*>(q_row + 8 * L::KB + c * 64);
+        if constexpr (F32) {
+          uint32_t ah[8], al[8];
+          cut(a.x, ah[0], al[0]), cut(a8.x, ah[1], al[1]), cut(a.y, ah[2], al[2]), cut(a8.y, ah[3], al[3]);
+          cut(a.z, ah[4], al[4]), cut(a8.z, ah[5], al[5]), cut(a.w, ah[6], al[6]), cut(a8.w, ah[7], al[7]);
 #pragma unroll
-      for (int i = 0; i < RPT; ++i) w[i] = *reinterpret_cast<const float4*>(Ps + (ty * RPT + i) * PS + k);
+          for (int j = 0; j < NT; ++j) {
+            const uint4 k = *reinterpret_cast<const uint4*>(k_row + j * 8 * L::KB + c * 64);
+            uint32_t kh[4], kl[4];
+            cut(k.x, kh[0], kl[0]), cut(k.y, kh[1], kl[1]), cut(k.z, kh[2], kl[2]), cut(k.w, kh[3], kl[3]);
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
+            for (int u = 0; u < 2; ++u) {
+              mma_tf32(s[j], al[4 * u], al[4 * u + 1], al[4 * u + 2], al[4 * u + 3], kh[2 * u], kh[2 * u + 1]);
+              mma_tf32(s[j], ah[4 * u], ah[4 * u + 1], ah[4 * u + 2], ah[4 * u + 3], kl[2 * u], kl[2 * u + 1]);
+              mma_tf32(s[j], ah[4 * u], ah[4 * u + 1], ah[4 * u + 2], ah[4 * u + 3], kh[2 * u], kh[2 * u + 1]);
+            }
+          }
+        } else {
 #pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          const int col = tx * 4 + 64 * c;
-          if (D % 64 != 0 && col >= D) continue;
-          const ulonglong2 v4 = load_pairs(Vs + (k + kk) * D + col);
-#pragma unroll
-          for (int i = 0; i < RPT; ++i) {
-            const float x = kk == 0 ? w[i].x : kk == 1 ? w[i].y : kk == 2 ? w[i].z : w[i].w;
-            const uint64_t x2 = pack2(x, x);
-            o[i][2 * c] = fma2(x2, v4.x, o[i][2 * c]);
-            o[i][2 * c + 1] = fma2(x2, v4.y, o[i][2 * c + 1]);
+          for (int j = 0; j < NT; ++j) {
+            const uint4 k = *reinterpret_cast<const uint4*>(k_row + j * 8 * L::KB + c * 64);
+            mma_bf16(s[j], a.x, a8.x, a.y, a8.y, k.x, k.y);
+            mma_bf16(s[j], a.z, a8.z, a.w, a8.w, k.z, k.w);
           }
         }
       }
     }
-    __syncthreads();  // the values and the weights have been read
-    if (more) load_rows<T>(Vs, D, V, slots_s + ((blk + 1) & 1) * BN);
+    __syncthreads();  // the keys have been read
+    if (more) load_rows<T, BN>(Ks, L::KB, K, slots_s[(blk + 1) & 1]);
+    if (works) {
+      // seen by every token: rows before the step that no window hides
+      const bool open = blk * BN + BN <= first && blk * BN >= whole_from;
+      const int key0 = blk * BN + wn * NT * 8 + 2 * t4;
+      float corr[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float& v = s[j][2 * h + x];
+            const bool seen = token[h] >= 0 && (open || sees(p, token[h], pos[h], key0 + 8 * j + x, n, first, q_begin));
+            v = seen ? score_log2(p, v) : -INFINITY;
+            top = fmaxf(top, v);
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float m_new = fmaxf(m[h], top), off = m_new == -INFINITY ? 0.f : m_new;
+        corr[h] = power2(m[h] - off);
+        m[h] = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float& v = s[j][2 * h + x];
+            v = power2(v - off);
+            sum += v;
+          }
+        l[h] = l[h] * corr[h] + sum;  // (of this lane's keys)
+      }
+      if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < L::OT; ++i) o[i][0] *= corr[0], o[i][1] *= corr[0], o[i][2] *= corr[1], o[i][3] *= corr[1];
+      }
+    }
+    if (more)
+      rows_landed<1>();
+    else
+      rows_landed<0>();
+    if (works) {
+      if constexpr (F32) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          uint32_t ph[4], pl[4];  // (the product's key t is this lane's first, t + 4 its second)
+          cut(__float_as_uint(s[j][0]), ph[0], pl[0]), cut(__float_as_uint(s[j][2]), ph[1], pl[1]);
+          cut(__float_as_uint(s[j][1]), ph[2], pl[2]), cut(__float_as_uint(s[j][3]), ph[3], pl[3]);
+          const unsigned char* row = Vs + (wn * NT * 8 + 8 * j + 2 * t4) * L::VB + g * 16;
+#pragma unroll
+          for (int c = 0; c < L::DV / 32; ++c) {
+            const uint4 v0 = *reinterpret_cast<const uint4*>(row + c * 128), v1 = *reinterpret_cast<const uint4*>(row + L::VB + c * 128);
+            const uint32_t x0[4] = {v0.x, v0.y, v0.z, v0.w}, x1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t h0, l0, h1, l1;
+              cut(x0[i], h0, l0), cut(x1[i], h1, l1);
+              mma_tf32(o[4 * c + i], pl[0], pl[1], pl[2], pl[3], h0, h1);
+              mma_tf32(o[4 * c + i], ph[0], ph[1], ph[2], ph[3], l0, l1);
+              mma_tf32(o[4 * c + i], ph[0], ph[1], ph[2], ph[3], h0, h1);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j + 1 < NT; j += 2) {
+          const uint32_t p0 = pack_bf16(s[j][0], s[j][1]), p1 = pack_bf16(s[j][2], s[j][3]), p2 = pack_bf16(s[j + 1][0], s[j + 1][1]), p3 = pack_bf16(s[j + 1][2], s[j + 1][3]);
+          const uint32_t row = (uint32_t)__cvta_generic_to_shared(Vs + (wn * NT * 8 + 8 * j + (lane & 15)) * L::VB + (lane >> 4) * 16);
+#pragma unroll
+          for (int c = 0; c < L::DV / 16; ++c) {
+            uint32_t x[4];
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(row + c * 32) : "memory");
+            mma_bf16(o[2 * c], p0, p1, p2, p3, x[0], x[1]);
+            mma_bf16(o[2 * c + 1], p0, p1, p2, p3, x[2], x[3]);
+          }
+        }
+      }
+    }
+    __syncthreads();  // the values have been read
+    if (more) load_rows<T, BN>(Vs, L::VB, V, slots_s[(blk + 1) & 1]);
   }
+  __syncthreads();  // (queries, too: the results go over all of them)
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    if (token[i] < 0) continue;
-    const int head = hk * G + (r0 + ty * RPT + i) % G;
-    const size_t row = (size_t)token[i] * p.nq + head;
-    if (p.splits > 1) {
-      const size_t at = row * p.splits + split;
-      if (tx == 0) p.part_ml[2 * at] = m[i], p.part_ml[2 * at + 1] = l[i];
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    if (t4 == 0) ml_s[warp][g + 8 * h] = make_float2(m[h], l[h]);
+    float* mine = reinterpret_cast<float*>(smem) + (warp * 16 + g + 8 * h) * L::DV;
+    if constexpr (F32) {
 #pragma unroll
-      for (int c = 0; c < DC; ++c) {
-        const int col = tx * 4 + 64 * c;
-        if (D % 64 == 0 || col < D) *reinterpret_cast<ulonglong2*>(p.part_o + at * D + col) = make_ulonglong2(o[i][2 * c], o[i][2 * c + 1]);
+      for (int c = 0; c < L::DV / 32; ++c) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          *reinterpret_cast<float4*>(mine + 32 * c + 8 * t4 + 4 * x) = make_float4(o[4 * c][2 * h + x], o[4 * c + 1][2 * h + x], o[4 * c + 2][2 * h + x], o[4 * c + 3][2 * h + x]);
       }
     } else {
-      float total = l[i], f = 1.f;
-      if (p.head_sinks != nullptr) {
-        const float sink = p.head_sinks[head] * LOG2E, top = fmaxf(m[i], sink);
-        f = m[i] == -INFINITY ? 0.f : exp2f(m[i] - top);
-        total = total * f + (sink == -INFINITY ? 0.f : exp2f(sink - top));
-      }
-      const float inv = total > 0.f ? f / total : 0.f;
-      T* out = reinterpret_cast<T*>(p.out) + row * D;
 #pragma unroll
-      for (int c = 0; c < DC * 4; ++c) {
-        const int col = tx * 4 + 64 * (c / 4) + c % 4;
-        if (D % 64 == 0 || col < D) out[col] = ts_from_float<T>((c % 2 ? unpack2(o[i][c / 2]).y : unpack2(o[i][c / 2]).x) * inv);
+      for (int i = 0; i < L::OT; ++i) *reinterpret_cast<float2*>(mine + 8 * i + 2 * t4) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+    }
+  }
+  __syncthreads();
+  // the warps of a row, joined in one order, four columns a thread
+  for (int i = tid; i < RM * (D / 4); i += TH) {
+    const int x = i / (D / 4), c = i % (D / 4) * 4, r = r0 + x;
+    if (r >= rows) break;
+    const int w0 = x / 16 * WN, head = hk * G + r % G;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < WN; ++w) top = fmaxf(top, ml_s[w0 + w][x % 16].x);
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WN; ++w) {
+      const float2 ml = ml_s[w0 + w][x % 16];
+      const float f = ml.x == -INFINITY ? 0.f : power2(ml.x - top);
+      const float4 z = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) + ((w0 + w) * 16 + x % 16) * L::DV + c);
+      sum += f * ml.y;
+      if (f > 0.f) y.x = fmaf(f, z.x, y.x), y.y = fmaf(f, z.y, y.y), y.z = fmaf(f, z.z, y.z), y.w = fmaf(f, z.w, y.w);
+    }
+    const size_t row = (size_t)(q_begin + r / G) * p.nq + head;
+    if (p.splits > 1) {
+      const size_t at = row * p.splits + split;
+      if (c == 0) p.part_ml[2 * at] = top, p.part_ml[2 * at + 1] = sum;
+      *reinterpret_cast<float4*>(p.part_o + at * D + c) = y;
+    } else {
+      float f = 1.f;
+      if (p.head_sinks != nullptr) {
+        const float sink = p.head_sinks[head] * LOG2E, over = fmaxf(top, sink);
+        f = top == -INFINITY ? 0.f : exp2f(top - over);
+        sum = sum * f + (sink == -INFINITY ? 0.f : exp2f(sink - over));
       }
+      const float inv = sum > 0.f ? f / sum : 0.f;
+      T* out = reinterpret_cast<T*>(p.out) + row * D + c;
+      out[0] = ts_from_float<T>(y.x * inv), out[1] = ts_from_float<T>(y.y * inv), out[2] = ts_from_float<T>(y.z * inv), out[3] = ts_from_float<T>(y.w * inv);
     }
   }
 }
@@ -349,41 +432,42 @@ __global__ void __launch_bounds__(128) join_parts_kernel(const Params p) {
     if (D % 32 == 0 || c * 32 + lane < D) out[c * 32 + lane] = ts_from_float<T>(o[c] * inv);
 }
 
-template <typename T, int RPT>
-int launch_rows(const Params& p, int B, int tiles, cudaStream_t stream) {
-  constexpr int smem = rows_smem<RPT>();
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(tree_rows_kernel<T, RPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return (int)e;
-  }
-  return ts_launch(tree_rows_kernel<T, RPT>, dim3(p.splits, tiles * p.nkv, B), dim3(TH), smem, stream, p);
+template <typename T, int WM>
+int launch_rows(const Params& p, int B, int rows, cudaStream_t stream) {
+  using L = Tile<T, WM>;
+  static_assert(L::SMEM <= 223 * 1024, "shared memory of an SM");
+  const int tiles = (rows + L::RM - 1) / L::RM;
+  if ((long long)tiles * p.nkv > 65535 || B > 65535) return TS_ERR_UNSUPPORTED_SIZE;
+  const cudaError_t e = cudaFuncSetAttribute(tree_rows_kernel<T, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  if (e != cudaSuccess) return (int)e;
+  return ts_launch(tree_rows_kernel<T, WM>, dim3(p.splits, tiles * p.nkv, B), dim3(TH), L::SMEM, stream, p);
 }
+
+// Warps beside one another by the rows of the largest request: the fewest that hold them all.  (Eight of them in float32 and heads above 128 find no room beside the keys.)
+template <typename T>
+constexpr int most_warps() { return sizeof(T) == 4 && D > 128 ? 4 : 8; }
+template <typename T>
+int warps_beside(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : most_warps<T>(); }
 
 template <typename T>
 int run_rows(const Params& p, int B, int max_t, cudaStream_t stream) {
-  const int rows = max_t * (p.nq / p.nkv);
-  const int rpt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int tiles = (rows + 16 * rpt - 1) / (16 * rpt);
-  if ((long long)tiles * p.nkv > 65535 || B > 65535) return TS_ERR_UNSUPPORTED_SIZE;
-  int status = rpt == 1 ? launch_rows<T, 1>(p, B, tiles, stream) : rpt == 2 ? launch_rows<T, 2>(p, B, tiles, stream) : launch_rows<T, 4>(p, B, tiles, stream);
+  const int rows = max_t * (p.nq / p.nkv), wm = warps_beside<T>(rows);
+  const int status = wm == 1 ? launch_rows<T, 1>(p, B, rows, stream) : wm == 2 ? launch_rows<T, 2>(p, B, rows, stream)
+                     : wm == 4 ? launch_rows<T, 4>(p, B, rows, stream) : launch_rows<T, most_warps<T>()>(p, B, rows, stream);
   if (status != 0 || p.splits == 1) return status;
   return ts_launch(join_parts_kernel<T>, dim3(((size_t)p.tokens * p.nq + 3) / 4), dim3(128), 0, stream, p);
 }
 
-}  // namespace
+template <typename T, int WM>
+void sizes_of(int& rm, int& bn, int& ctas) { rm = Tile<T, WM>::RM, bn = Tile<T, WM>::BN, ctas = Tile<T, WM>::CTAS; }
 
-TS_EXPORT int ts_attention_tree_head_dim() { return D; }
-
-// In how many parts the CUDA-core kernel cuts the keys of a request of `max_context` rows: the fewest blocks in a row, counting every wave of CTAs (as many as
-// registers and shared memory let run at once) and one and a half blocks for a CTA's start and the joining of its part.  (4 requests of 12,000 rows, 16 nodes, float32:
-// 4 parts 567 us, one wave; 5 to 6 parts 770, two; the same work in 10 parts 692.)
-TS_EXPORT int ts_attention_tree_splits(int B, int max_t, int nq, int nkv, int max_context) {
-  const int rows = max_t * (nq / nkv), rpt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const long long units = (long long)B * nkv * ((rows + 16 * rpt - 1) / (16 * rpt));
-  const int blocks = (max_context + BN - 1) / BN;
-  const int smem = rpt == 1 ? rows_smem<1>() : rpt == 2 ? rows_smem<2>() : rows_smem<4>();
-  const int by_smem = 227 * 1024 / (smem + 1024), by_registers = rpt == 1 ? 4 : D > 128 ? (rpt == 2 ? 2 : 1) : rpt == 2 ? 3 : 2;
-  const long long slots = 148ll * (by_smem < by_registers ? by_smem : by_registers);
+template <typename T>
+int splits_of(int B, int rows, int nkv, int max_context) {
+  const int wm = warps_beside<T>(rows);
+  int rm, bn, ctas;
+  wm == 1 ? sizes_of<T, 1>(rm, bn, ctas) : wm == 2 ? sizes_of<T, 2>(rm, bn, ctas) : wm == 4 ? sizes_of<T, 4>(rm, bn, ctas) : sizes_of<T, most_warps<T>()>(rm, bn, ctas);
+  const long long units = (long long)B * nkv * ((rows + rm - 1) / rm), slots = 148ll * ctas;
+  const int blocks = (max_context + bn - 1) / bn;
   int best = 1;
   double least = 0;
   for (int s = 1; s <= 64 && s <= (blocks < 1 ? 1 : blocks); ++s) {
@@ -391,6 +475,15 @@ TS_EXPORT int ts_attention_tree_splits(int B, int max_t, int nq, int nkv, int ma
     if (s == 1 || cost < 0.98 * least) best = s, least = cost;
   }
   return best;
+}
+
+}  // namespace
+
+// In how many parts the keys of a request of `max_context` rows are cut: the fewest blocks in a row, counting every wave of CTAs (as many as
+// registers and shared memory let run at once) and one and a half blocks for a CTA's start and the joining of its part.
+TS_EXPORT int ts_attention_tree_splits(int bf16, int B, int max_t, int nq, int nkv, int max_context) {
+  const int rows = max_t * (nq / nkv);
+  return bf16 ? splits_of<__nv_bfloat16>(B, rows, nkv, max_context) : splits_of<float>(B, rows, nkv, max_context);
 }
 
 // `tokens`: rows of q.  part: floats of scratch, tokens * nq * splits * (D + 2), where splits > 1.

@@ -2938,7 +2938,7 @@ def _attention_tree_fns(head_dim: int) -> tuple:
                         + [_c_float, _c_int, _c_float, _c_int, _c_void_p, _c_void_p])
         run.restype = _c_int
         splits = lib.ts_attention_tree_splits
-        splits.argtypes = [_c_int] * 5
+        splits.argtypes = [_c_int] * 6
         splits.restype = _c_int
         fns = _attention_trees[head_dim] = (run, splits)
     return fns
@@ -3095,7 +3095,7 @@ def attention_tree(
             launch_count += 1
             return
     run, split = _attention_tree_fns(d)
-    splits = split(num_seqs, max_seqlen_q, nq, nkv, min(max_context, window + max_seqlen_q + 64) if window > 0 else max_context)
+    splits = split(int(dtype is torch.bfloat16), num_seqs, max_seqlen_q, nq, nkv, min(max_context, window + max_seqlen_q + 64) if window > 0 else max_context)
     part = torch.empty(T * nq * splits * (d + 2), device=q.device, dtype=torch.float32) if splits > 1 else None
     _check("attention_tree", run(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), int(dtype is torch.bfloat16), tree_mask.data_ptr(), ms[1], cu_seqlens_q.data_ptr(),

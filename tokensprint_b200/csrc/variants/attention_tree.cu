@@ -44,12 +44,6 @@ struct Params {
   float scale, cap;      // cap 0: none
 };
 
-// A score in units of log2: what enters 2^x.
-__device__ __forceinline__ float score_log2(const Params& p, float dot) {
-  if (p.cap > 0.f) return p.cap * LOG2E * tanhf(dot * (p.scale / p.cap));
-  return dot * (p.scale * LOG2E);
-}
-
 // Whether the token (global number `token`, position `pos`) of a request whose nodes begin at token q_begin and at row `first` sees row j of n.
 __device__ __forceinline__ bool sees(const Params& p, int token, int pos, int j, int n, int first, int q_begin) {
   if (j >= n) return false;
@@ -101,6 +95,7 @@ __device__ __forceinline__ void copy16(unsigned char* dst, const void* src, bool
 template <typename T, int BN>
 __device__ __forceinline__ void load_rows(unsigned char* dst, int stride, const T* pool, const long long* slots) {
   constexpr int PER = D * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T);
+#pragma unroll 4
   for (int i = threadIdx.x; i < BN * PER; i += TH) {
     const int r = i / PER, c = i % PER;
     const long long at = slots[r];
@@ -115,17 +110,21 @@ __device__ __forceinline__ void rows_landed() {
 }
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// x as the sum of two tf32, each rounded to nearest (bits of an infinity stay; a NaN stays in the lower part at the least)
+__device__ __forceinline__ void ldmatrix4(uint32_t (&x)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+}
+// x as the sum of two tf32: the upper rounded to nearest, the lower the rest, of which a product reads the upper 19 bits (11 significant ones; with it rounded, too, two
+// more instructions an operand).  Bits of an infinity stay; a NaN stays in the lower part at the least.
 __device__ __forceinline__ void cut(uint32_t x, uint32_t& high, uint32_t& low) {
   high = (x + 0x1000u) & 0xffffe000u;
-  low = (__float_as_uint(__uint_as_float(x) - __uint_as_float(high)) + 0x1000u) & 0xffffe000u;
+  low = __float_as_uint(__uint_as_float(x) - __uint_as_float(high));
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -175,21 +174,22 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
   const int kb0 = lo / BN, blocks = n > 0 ? (n - 1) / BN - kb0 + 1 : 0;
   const int per = (blocks + p.splits - 1) / p.splits, begin = kb0 + split * per, end = min(kb0 + blocks, begin + per);
   const int* table = p.table + (size_t)b * p.max_blocks;
+  // where a block's rows begin; the page is asked for a block ahead
+  int page = -1, in_page = 0;
+  auto ask_page = [&](int blk) {
+    const int j = blk * BN + tid, e = j / p.page;
+    page = -1, in_page = j - e * p.page;
+    if (tid < BN && blk < end && j < n && e < p.max_blocks) page = table[e];
+  };
   auto find_slots = [&](int blk) {
-    if (tid < BN) {
-      const int j = blk * BN + tid, e = j / p.page;
-      long long at = -1;
-      if (j < n && e < p.max_blocks) {
-        const int page = table[e];
-        if (page >= 0 && page < p.num_pages) at = (((long long)page * p.page + j % p.page) * p.nkv + hk) * D;
-      }
-      slots_s[blk & 1][tid] = at;
-    }
+    if (tid < BN) slots_s[blk & 1][tid] = page >= 0 && page < p.num_pages ? (((long long)page * p.page + in_page) * p.nkv + hk) * D : -1;
   };
   const T* K = reinterpret_cast<const T*>(p.k);
   const T* V = reinterpret_cast<const T*>(p.v);
   if (begin < end) {
+    ask_page(begin);
     find_slots(begin);
+    ask_page(begin + 1);
     __syncthreads();
     load_rows<T, BN>(Ks, L::KB, K, slots_s[begin & 1]);
     load_rows<T, BN>(Vs, L::VB, V, slots_s[begin & 1]);
@@ -217,11 +217,13 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
   for (int i = 0; i < L::OT; ++i)
 #pragma unroll
     for (int x = 0; x < 4; ++x) o[i][x] = 0.f;
+  // scores in units of log2, what enters 2^x: a product times `scale`, or cap_log2 times the tanh of that
+  const float scale = p.cap > 0.f ? p.scale / p.cap : p.scale * LOG2E, cap_log2 = p.cap * LOG2E;
   const unsigned char *q_row = Qs + (wm * 16 + g) * L::KB + t4 * 16, *k_row = Ks + (wn * NT * 8 + g) * L::KB + t4 * 16;
 #pragma unroll 1
   for (int blk = begin; blk < end; ++blk) {
     const bool more = blk + 1 < end;
-    if (more) find_slots(blk + 1);
+    if (more) find_slots(blk + 1), ask_page(blk + 2);
     rows_landed<1>();
     float s[NT][4];
 #pragma unroll
@@ -236,25 +238,34 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
           uint32_t ah[8], al[8];
           cut(a.x, ah[0], al[0]), cut(a8.x, ah[1], al[1]), cut(a.y, ah[2], al[2]), cut(a8.y, ah[3], al[3]);
           cut(a.z, ah[4], al[4]), cut(a8.z, ah[5], al[5]), cut(a.w, ah[6], al[6]), cut(a8.w, ah[7], al[7]);
+          // (a product waits for the one before it on the same scores: those of several keys take turns)
+          constexpr int J = NT < 4 ? NT : 4;
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const uint4 k = *reinterpret_cast<const uint4*>(k_row + j * 8 * L::KB + c * 64);
-            uint32_t kh[4], kl[4];
-            cut(k.x, kh[0], kl[0]), cut(k.y, kh[1], kl[1]), cut(k.z, kh[2], kl[2]), cut(k.w, kh[3], kl[3]);
+          for (int j0 = 0; j0 < NT; j0 += J) {
+            uint32_t kh[J][4], kl[J][4];
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+              const uint4 k = *reinterpret_cast<const uint4*>(k_row + (j0 + j) * 8 * L::KB + c * 64);
+              cut(k.x, kh[j][0], kl[j][0]), cut(k.y, kh[j][1], kl[j][1]), cut(k.z, kh[j][2], kl[j][2]), cut(k.w, kh[j][3], kl[j][3]);
+            }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              mma_tf32(s[j], al[4 * u], al[4 * u + 1], al[4 * u + 2], al[4 * u + 3], kh[2 * u], kh[2 * u + 1]);
-              mma_tf32(s[j], ah[4 * u], ah[4 * u + 1], ah[4 * u + 2], ah[4 * u + 3], kl[2 * u], kl[2 * u + 1]);
-              mma_tf32(s[j], ah[4 * u], ah[4 * u + 1], ah[4 * u + 2], ah[4 * u + 3], kh[2 * u], kh[2 * u + 1]);
+#pragma unroll
+              for (int j = 0; j < J; ++j) mma_tf32(s[j0 + j], al[4 * u], al[4 * u + 1], al[4 * u + 2], al[4 * u + 3], kh[j][2 * u], kh[j][2 * u + 1]);
+#pragma unroll
+              for (int j = 0; j < J; ++j) mma_tf32(s[j0 + j], ah[4 * u], ah[4 * u + 1], ah[4 * u + 2], ah[4 * u + 3], kl[j][2 * u], kl[j][2 * u + 1]);
+#pragma unroll
+              for (int j = 0; j < J; ++j) mma_tf32(s[j0 + j], ah[4 * u], ah[4 * u + 1], ah[4 * u + 2], ah[4 * u + 3], kh[j][2 * u], kh[j][2 * u + 1]);
             }
           }
         } else {
+          uint4 k[NT];
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const uint4 k = *reinterpret_cast<const uint4*>(k_row + j * 8 * L::KB + c * 64);
-            mma_bf16(s[j], a.x, a8.x, a.y, a8.y, k.x, k.y);
-            mma_bf16(s[j], a.z, a8.z, a.w, a8.w, k.z, k.w);
-          }
+          for (int j = 0; j < NT; ++j) k[j] = *reinterpret_cast<const uint4*>(k_row + j * 8 * L::KB + c * 64);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) mma_bf16(s[j], a.x, a8.x, a.y, a8.y, k[j].x, k[j].y);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) mma_bf16(s[j], a.z, a8.z, a.w, a8.w, k[j].z, k[j].w);
         }
       }
     }
@@ -264,19 +275,30 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
       // seen by every token: rows before the step that no window hides
       const bool open = blk * BN + BN <= first && blk * BN >= whole_from;
       const int key0 = blk * BN + wn * NT * 8 + 2 * t4;
+      if (p.cap > 0.f) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[j][x] = cap_log2 * tanhf(s[j][x] * scale);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[j][x] *= scale;
+      }
+      if (!open) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (token[x >> 1] < 0 || !sees(p, token[x >> 1], pos[x >> 1], key0 + 8 * j + (x & 1), n, first, q_begin)) s[j][x] = -INFINITY;
+      }
       float corr[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            float& v = s[j][2 * h + x];
-            const bool seen = token[h] >= 0 && (open || sees(p, token[h], pos[h], key0 + 8 * j + x, n, first, q_begin));
-            v = seen ? score_log2(p, v) : -INFINITY;
-            top = fmaxf(top, v);
-          }
+        for (int j = 0; j < NT; ++j) top = fmaxf(top, fmaxf(s[j][2 * h], s[j][2 * h + 1]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const float m_new = fmaxf(m[h], top), off = m_new == -INFINITY ? 0.f : m_new;
@@ -314,14 +336,15 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
           for (int c = 0; c < L::DV / 32; ++c) {
             const uint4 v0 = *reinterpret_cast<const uint4*>(row + c * 128), v1 = *reinterpret_cast<const uint4*>(row + L::VB + c * 128);
             const uint32_t x0[4] = {v0.x, v0.y, v0.z, v0.w}, x1[4] = {v1.x, v1.y, v1.z, v1.w};
+            uint32_t h0[4], l0[4], h1[4], l1[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t h0, l0, h1, l1;
-              cut(x0[i], h0, l0), cut(x1[i], h1, l1);
-              mma_tf32(o[4 * c + i], pl[0], pl[1], pl[2], pl[3], h0, h1);
-              mma_tf32(o[4 * c + i], ph[0], ph[1], ph[2], ph[3], l0, l1);
-              mma_tf32(o[4 * c + i], ph[0], ph[1], ph[2], ph[3], h0, h1);
-            }
+            for (int i = 0; i < 4; ++i) cut(x0[i], h0[i], l0[i]), cut(x1[i], h1[i], l1[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mma_tf32(o[4 * c + i], pl[0], pl[1], pl[2], pl[3], h0[i], h1[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mma_tf32(o[4 * c + i], ph[0], ph[1], ph[2], ph[3], l0[i], l1[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mma_tf32(o[4 * c + i], ph[0], ph[1], ph[2], ph[3], h0[i], h1[i]);
           }
         }
       } else {
@@ -329,12 +352,14 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
         for (int j = 0; j + 1 < NT; j += 2) {
           const uint32_t p0 = pack_bf16(s[j][0], s[j][1]), p1 = pack_bf16(s[j][2], s[j][3]), p2 = pack_bf16(s[j + 1][0], s[j + 1][1]), p3 = pack_bf16(s[j + 1][2], s[j + 1][3]);
           const uint32_t row = (uint32_t)__cvta_generic_to_shared(Vs + (wn * NT * 8 + 8 * j + (lane & 15)) * L::VB + (lane >> 4) * 16);
+          // (asked for two products ahead)
+          uint32_t x[2][4];
+          ldmatrix4(x[0], row);
 #pragma unroll
           for (int c = 0; c < L::DV / 16; ++c) {
-            uint32_t x[4];
-            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(row + c * 32) : "memory");
-            mma_bf16(o[2 * c], p0, p1, p2, p3, x[0], x[1]);
-            mma_bf16(o[2 * c + 1], p0, p1, p2, p3, x[2], x[3]);
+            if (c + 1 < L::DV / 16) ldmatrix4(x[(c + 1) & 1], row + (c + 1) * 32);
+            mma_bf16(o[2 * c], p0, p1, p2, p3, x[c & 1][0], x[c & 1][1]);
+            mma_bf16(o[2 * c + 1], p0, p1, p2, p3, x[c & 1][2], x[c & 1][3]);
           }
         }
       }

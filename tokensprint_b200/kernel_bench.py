@@ -1,7 +1,7 @@
 """Times the engine's kernels one at a time, at the layer sizes of a named preset and over a
 range of batch sizes and context lengths, and prints each one's share of its roofline.
 
-    python -m tokensprint_b200.kernel_bench [--preset qwen3-8b] [--only decode,prompt,gemm,small,layer,latent,experts,kv4]
+    python -m tokensprint_b200.kernel_bench [--preset qwen3-8b] [--only decode,prompt,gemm,small,layer,latent,experts,kv4,drafts]
 
 Every kernel runs after a read of a buffer larger than the L2 cache, so it reads its operands
 from device memory as it does inside a model step, and is timed on the device inside a CUDA graph,
@@ -431,8 +431,52 @@ def kv4_cache(cfg, timer, pk, rows, device):
     ops.check_device_errors()
 
 
+def drafted_tokens(cfg, timer, pk, rows, device):
+    """Steps that check drafted tokens: attention of chains and trees, their verification, the accepted rows, lookup."""
+    nq, nkv, d, V, page = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.vocab_size, 16
+
+    def ints(x):
+        return torch.tensor(x, dtype=torch.int32, device=device)
+
+    def add(name, case, us, gb):
+        rows.append((name, case, us, gb / (us * 1e-6), "GB/s", gb / (us * 1e-6) / pk["hbm_gbs"]))
+
+    for B, ctx, nodes in ((1, 512, 6), (32, 4096, 5), (16, 4096, 32), (4, 30000, 61)):
+        sees = []
+        for i in range(nodes):  # a chain, or two children a node
+            sees.append((sees[i - 1 if nodes <= 6 else (i - 1) // 2] if i else 0) | 1 << i)
+        mask = torch.tensor([[x] for x in sees], dtype=torch.int64, device=device).repeat(B, 1)
+        cu, lens = ints([b * nodes for b in range(B + 1)]), ints([ctx] * B)
+        for dtype in (torch.bfloat16, torch.float32):
+            k, v, table = _paged(B, ctx, nkv, d, page, device)
+            k, v, q = k.to(dtype), v.to(dtype), torch.randn(B * nodes, nq * d, device=device).to(dtype)
+            out = torch.empty_like(q)
+            us = timer(lambda: ops.attention_tree(q, k, v, out, mask, cu, lens, table, page, B, nodes, ctx, nq, nkv, d, d**-0.5))
+            add(f"attention of trees, {str(dtype)[6:]}", f"B={B} ctx={ctx} nodes={nodes}", us, B * 2 * ctx * nkv * d * k.element_size() / 1e9)
+    for B, nodes in ((1, 5), (32, 5), (16, 9)):
+        # chains whose drafts are the largest entries: greedy requests read every row
+        logits = torch.randn(B * nodes, V, device=device)
+        tokens = torch.cat([ints([[0]] * B), logits.argmax(1).int().view(B, nodes)[:, :-1]], 1).flatten().contiguous()
+        path, fresh = (torch.empty(B, nodes, dtype=torch.int32, device=device) for _ in range(2))
+        counts, cu = torch.empty(B, dtype=torch.int32, device=device), ints([b * nodes for b in range(B + 1)])
+        parents, zeros, keys = ints(list(range(-1, nodes - 1)) * B), torch.zeros(B * nodes, device=device), torch.arange(B, device=device)
+        add("verification", f"B={B}, {nodes} rows each",
+            timer(lambda: ops.verify_drafts(logits, tokens, parents, cu, zeros, zeros, keys, path, fresh, counts, B, nodes)), B * nodes * V * 4 / 1e9)
+    for B, layers in ((1, 28), (16, 36)):
+        pools = ops.RowPools([torch.zeros(B * 8, page, nkv, d, device=device, dtype=torch.bfloat16) for _ in range(2 * layers)])
+        args = ints([[0, 2, 4, 5]] * B), ints([3] * B), ints([b * 6 for b in range(B + 1)]), ints([90] * B), torch.arange(B * 8, device=device).int().view(B, 8)
+        add("accepted rows", f"B={B}, {layers} layers", timer(lambda: ops.keep_drafted_rows(pools, *args, page, B)), B * 3 * 2 * layers * 2 * nkv * d * 2 / 1e9)
+    for B, n in ((1, 700), (64, 30000)):
+        history = torch.randint(0, 1000, (B, n), device=device).int()
+        tokens, parents = (torch.empty(B, 33, dtype=torch.int32, device=device) for _ in range(2))
+        lens, counts = ints([n] * B), torch.empty(B, dtype=torch.int32, device=device)
+        add("lookup", f"B={B} n={n}", timer(lambda: ops.lookup_drafts(history, lens, tokens, parents, counts, B, 8, 4, 6)), B * n * 4 / 1e9)
+    ops.check_device_errors()
+
+
 GROUPS = {"decode": decode_attention, "prompt": prompt_attention, "gemm": skinny_gemm, "small": small_kernels, "layer": layer_products,
-          "latent": latent_attention, "experts": routed_experts, "kv4": kv4_cache}
+          "latent": latent_attention, "experts": routed_experts, "kv4": kv4_cache,
+          "drafts": drafted_tokens}
 
 
 def main(argv=None) -> int:

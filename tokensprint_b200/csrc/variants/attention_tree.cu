@@ -7,7 +7,7 @@
 //   o_i = sum_j p_ij v_j,  p_i = softmax over the rows it sees (and its head's sink) of s_ij = scale q_i k_j, or cap tanh(scale q_i k_j / cap).
 // A node that sees nothing gets zeros.  Scores, maxima, sums and outputs are float32 until the end.
 //
-// The (node, query head of a group) pairs of a request are the rows of a tile for each KV head, so that what is read of the cache is read once for them all;
+// This file takes float32 and the heads that attention_tree_tcgen05.cu does not.  The (node, query head of a group) pairs of a request are the rows of a tile for each KV head, so that what is read of the cache is read once for them all;
 // the keys are cut into parts, a CTA each, whose results (maximum, sum, unnormalised output) a second kernel joins, always in the same order.
 #include <math.h>
 
@@ -62,8 +62,10 @@ __device__ __forceinline__ bool sees(const Params& p, int token, int pos, int j,
 // The order of the entries inside a product does not matter, and the order of columns of the result is put right at the end: a lane takes 16 neighbouring bytes of
 // a row of queries or keys as its share of two products (for float32 values: four neighbouring columns of a row as its share of four), one load without conflicts.
 //
-// What bounds it: float32 the tensor cores' old path (a product of 16 x 8 x 8 takes 8 cycles, three a term: 65 TFLOP/s of whole terms a GPU) and the
-// instructions that cut operands in two.
+// What bounds it: the old path of the tensor cores, where any such product takes 8 cycles (three of 16 x 8 x 8 a term in float32: 90 TFLOP/s of whole terms a GPU),
+// half of whose time is spent: 16 requests of 2,000 rows, 32 nodes, float32 362 us (46 TFLOP/s), 8 of 4,000, 64 nodes, bfloat16 heads of 256 363 (182 TFLOP/s); in
+// float32 the rest is the instructions that cut operands in two, in bfloat16 the loads from shared memory (as many cycles as the products), and the weights between
+// them.  Few rows are bound by the copies: chains of 4 over 4,000 rows, heads of 256, 67 us (3.9 TB/s).
 
 constexpr int TH = 256;
 
@@ -76,14 +78,21 @@ struct Tile {
   static constexpr int NT = BN / WN / 8;                            // 8s of keys per warp
   static constexpr int CHUNK = 64 / sizeof(T);                      // columns that four lanes take at a time
   static constexpr int DK = (D + CHUNK - 1) / CHUNK * CHUNK;        // columns of queries and keys, zeros behind D
-  static constexpr int KB = DK * sizeof(T) + (DK * sizeof(T) % 128 == 0 ? 64 : 0);  // bytes of such a row: two rows of 64 bytes lie in different banks
+  static constexpr int KB = DK * sizeof(T);                         // bytes of such a row
+  static constexpr int FLIP = KB % 128 == 0 ? 64 : 0;               // its halves of 128 bytes change places in odd rows: 64 bytes of two rows lie in different banks
   static constexpr int DV = F32 ? (D + 31) / 32 * 32 : (D + 15) / 16 * 16;  // columns of values (what stands behind D goes to columns that nobody reads)
   static constexpr int VB = DV * sizeof(T) + 16;
   static constexpr int OT = DV / 8;
-  static constexpr int K_AT = RM * KB, V_AT = K_AT + BN * KB, END = V_AT + BN * VB;
   static constexpr int OUT = 8 * 16 * DV * 4;                       // the warps' results, when all else has been read
+  static constexpr int STAGE = BN * (KB + VB);
+  // Heads up to 64: two CTAs on an SM, a block each in shared memory (12 requests with a window of 1,024, 13 nodes, float32: 83 us; two blocks each: 86).  Larger
+  // ones: one CTA, and two blocks where they find room, the next one's copies asked for between the products of this one (8 of 4,000 rows, 16 nodes, bfloat16 heads
+  // of 256: 98 us, with one block 115).
+  static constexpr int CTAS = D <= 64 ? 2 : 1, ROOM = CTAS == 2 ? 112 * 1024 : 226 * 1024;
+  static constexpr int STAGES = CTAS == 1 && RM * KB + 2 * STAGE <= ROOM ? 2 : 1;
+  static constexpr int K_AT = RM * KB, V_AT = K_AT + BN * KB, END = K_AT + STAGES * STAGE;
   static constexpr int SMEM = END > OUT ? END : OUT;
-  static constexpr int CTAS = SMEM <= 110 * 1024 && (D <= 64 || (D <= 128 && WM <= 4)) ? 2 : 1;
+  static_assert(SMEM <= ROOM, "shared memory of an SM");
 };
 
 __device__ __forceinline__ void copy16(unsigned char* dst, const void* src, bool there) {
@@ -91,18 +100,7 @@ __device__ __forceinline__ void copy16(unsigned char* dst, const void* src, bool
   const int bytes = there ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(bytes) : "memory");
 }
-// A block's rows into shared memory; `slots`: where each begins in the pool, in entries, or -1 (zeros).
-template <typename T, int BN>
-__device__ __forceinline__ void load_rows(unsigned char* dst, int stride, const T* pool, const long long* slots) {
-  constexpr int PER = D * (int)sizeof(T) / 16, E = 16 / (int)sizeof(T);
-#pragma unroll 4
-  for (int i = threadIdx.x; i < BN * PER; i += TH) {
-    const int r = i / PER, c = i % PER;
-    const long long at = slots[r];
-    copy16(dst + r * stride + c * 16, pool + (at < 0 ? 0 : at + c * E), at >= 0);
-  }
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
 __device__ __forceinline__ void rows_landed() {
   asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
@@ -151,9 +149,8 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
   ts_pdl_prologue();
   using L = Tile<T, WM>;
   constexpr bool F32 = L::F32;
-  constexpr int BN = L::BN, RM = L::RM, NT = L::NT, WN = L::WN, E = 16 / (int)sizeof(T);
-  extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ long long slots_s[2][BN];
+  constexpr int BN = L::BN, RM = L::RM, NT = L::NT, WN = L::WN, CHUNKS = L::KB / 64, LINES = (D * (int)sizeof(T) + 127) / 128, COPIES = BN / 32;
+  extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float2 ml_s[8][16];
   unsigned char *Qs = smem, *Ks = smem + L::K_AT, *Vs = smem + L::V_AT;
   const int split = blockIdx.x, hk = blockIdx.y % p.nkv, tile = blockIdx.y / p.nkv, b = blockIdx.z;
@@ -174,35 +171,62 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
   const int kb0 = lo / BN, blocks = n > 0 ? (n - 1) / BN - kb0 + 1 : 0;
   const int per = (blocks + p.splits - 1) / p.splits, begin = kb0 + split * per, end = min(kb0 + blocks, begin + per);
   const int* table = p.table + (size_t)b * p.max_blocks;
-  // where a block's rows begin; the page is asked for a block ahead
-  int page = -1, in_page = 0;
+  // A thread copies an eighth of every 128 bytes of the rows tid / 8, tid / 8 + 32, ...  Where they begin in the pool: their pages are asked for a block ahead.
+  int page[COPIES], in_page[COPIES];
+  long long at[COPIES];
   auto ask_page = [&](int blk) {
-    const int j = blk * BN + tid, e = j / p.page;
-    page = -1, in_page = j - e * p.page;
-    if (tid < BN && blk < end && j < n && e < p.max_blocks) page = table[e];
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int j = blk * BN + tid / 8 + 32 * i, e = j / p.page;
+      page[i] = -1, in_page[i] = j - e * p.page;
+      if (blk < end && j < n && e < p.max_blocks) page[i] = table[e];
+    }
   };
-  auto find_slots = [&](int blk) {
-    if (tid < BN) slots_s[blk & 1][tid] = page >= 0 && page < p.num_pages ? (((long long)page * p.page + in_page) * p.nkv + hk) * D : -1;
+  auto find_rows = [&]() {
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) at[i] = page[i] >= 0 && page[i] < p.num_pages ? ((((long long)page[i] * p.page + in_page[i]) * p.nkv + hk) * D) * (long long)sizeof(T) : -1;
   };
-  const T* K = reinterpret_cast<const T*>(p.k);
-  const T* V = reinterpret_cast<const T*>(p.v);
+  auto copy_keys = [&](int c, int stage) {
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int row = tid / 8 + 32 * i, from = c * 128 + (tid & 7) * 16;
+      if (D * sizeof(T) % 128 == 0 || from < D * (int)sizeof(T))
+        copy16(Ks + stage * L::STAGE + row * L::KB + (from ^ (row & 1) * L::FLIP), static_cast<const unsigned char*>(p.k) + (at[i] < 0 ? 0 : at[i] + from), at[i] >= 0);
+    }
+  };
+  auto copy_values = [&](int c, int stage) {
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int row = tid / 8 + 32 * i, from = c * 128 + (tid & 7) * 16;
+      if (D * sizeof(T) % 128 == 0 || from < D * (int)sizeof(T))
+        copy16(Vs + stage * L::STAGE + row * L::VB + from, static_cast<const unsigned char*>(p.v) + (at[i] < 0 ? 0 : at[i] + from), at[i] >= 0);
+    }
+  };
   if (begin < end) {
     ask_page(begin);
-    find_slots(begin);
+    find_rows();
     ask_page(begin + 1);
-    __syncthreads();
-    load_rows<T, BN>(Ks, L::KB, K, slots_s[begin & 1]);
-    load_rows<T, BN>(Vs, L::VB, V, slots_s[begin & 1]);
+#pragma unroll 4
+    for (int c = 0; c < LINES; ++c) copy_keys(c, 0);
+    if (L::STAGES == 1) copies_end();
+#pragma unroll 4
+    for (int c = 0; c < LINES; ++c) copy_values(c, 0);
+    copies_end();
   }
   // queries: row r of the tile is token r / G, head r % G
   const T* q = reinterpret_cast<const T*>(p.q);
   for (int i = tid; i < RM * L::DK; i += TH) {
     const int x = i / L::DK, r = r0 + x, c = i % L::DK;
-    *reinterpret_cast<T*>(Qs + x * L::KB + c * sizeof(T)) = r < rows && c < D ? q[((size_t)(q_begin + r / G) * p.nq + hk * G + r % G) * D + c] : ts_from_float<T>(0.f);
+    *reinterpret_cast<T*>(Qs + x * L::KB + ((c * (int)sizeof(T)) ^ (x & 1) * L::FLIP)) =
+        r < rows && c < D ? q[((size_t)(q_begin + r / G) * p.nq + hk * G + r % G) * D + c] : ts_from_float<T>(0.f);
   }
-  if (L::DK > D)  // (a product with zeros needs numbers beside them)
-    for (int i = tid; i < BN * (L::DK - D); i += TH)
-      *reinterpret_cast<T*>(Ks + i / (L::DK > D ? L::DK - D : 1) * L::KB + (D + i % (L::DK > D ? L::DK - D : 1)) * sizeof(T)) = ts_from_float<T>(0.f);
+  if constexpr (L::DK > D) {  // (a product with zeros needs numbers beside them)
+    constexpr int PAD = L::DK - D;
+    for (int i = tid; i < L::STAGES * BN * PAD; i += TH) {
+      const int x = i / PAD % BN, c = (D + i % PAD) * (int)sizeof(T);
+      *reinterpret_cast<T*>(Ks + i / (BN * PAD) * L::STAGE + x * L::KB + (c ^ (x & 1) * L::FLIP)) = ts_from_float<T>(0.f);
+    }
+  }
   const bool works = r0 + wm * 16 < rows;
   int token[2], pos[2];
   float m[2], l[2], o[L::OT][4];
@@ -220,11 +244,13 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
   // scores in units of log2, what enters 2^x: a product times `scale`, or cap_log2 times the tanh of that
   const float scale = p.cap > 0.f ? p.scale / p.cap : p.scale * LOG2E, cap_log2 = p.cap * LOG2E;
   const unsigned char *q_row = Qs + (wm * 16 + g) * L::KB + t4 * 16, *k_row = Ks + (wn * NT * 8 + g) * L::KB + t4 * 16;
+  const int flip = (g & 1) * L::FLIP;
 #pragma unroll 1
   for (int blk = begin; blk < end; ++blk) {
     const bool more = blk + 1 < end;
-    if (more) find_slots(blk + 1), ask_page(blk + 2);
-    rows_landed<1>();
+    const int stage = L::STAGES == 2 ? (blk - begin) & 1 : 0;
+    if (more) find_rows(), ask_page(blk + 2);
+    rows_landed<L::STAGES == 2 ? 0 : 1>();
     float s[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -232,8 +258,11 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
       for (int x = 0; x < 4; ++x) s[j][x] = 0.f;
     if (works) {
 #pragma unroll 2
-      for (int c = 0; c < L::DK / L::CHUNK; ++c) {
-        const uint4 a = *reinterpret_cast<const uint4*>(q_row + c * 64), a8 = *reinterpret_cast<const uint4*>(q_row + 8 * L::KB + c * 64);
+      for (int c = 0; c < CHUNKS; ++c) {
+        if (L::STAGES == 2 && more && c % 2 == 0) copy_keys(c / 2, stage ^ 1), copy_values(c / 2, stage ^ 1);
+        const int here = (c * 64) ^ flip;
+        const uint4 a = *reinterpret_cast<const uint4*>(q_row + here), a8 = *reinterpret_cast<const uint4*>(q_row + 8 * L::KB + here);
+        const unsigned char* keys = k_row + stage * L::STAGE + here;
         if constexpr (F32) {
           uint32_t ah[8], al[8];
           cut(a.x, ah[0], al[0]), cut(a8.x, ah[1], al[1]), cut(a.y, ah[2], al[2]), cut(a8.y, ah[3], al[3]);
@@ -245,7 +274,7 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
             uint32_t kh[J][4], kl[J][4];
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-              const uint4 k = *reinterpret_cast<const uint4*>(k_row + (j0 + j) * 8 * L::KB + c * 64);
+              const uint4 k = *reinterpret_cast<const uint4*>(keys + (j0 + j) * 8 * L::KB);
               cut(k.x, kh[j][0], kl[j][0]), cut(k.y, kh[j][1], kl[j][1]), cut(k.z, kh[j][2], kl[j][2]), cut(k.w, kh[j][3], kl[j][3]);
             }
 #pragma unroll
@@ -261,7 +290,7 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
         } else {
           uint4 k[NT];
 #pragma unroll
-          for (int j = 0; j < NT; ++j) k[j] = *reinterpret_cast<const uint4*>(k_row + j * 8 * L::KB + c * 64);
+          for (int j = 0; j < NT; ++j) k[j] = *reinterpret_cast<const uint4*>(keys + j * 8 * L::KB);
 #pragma unroll
           for (int j = 0; j < NT; ++j) mma_bf16(s[j], a.x, a8.x, a.y, a8.y, k[j].x, k[j].y);
 #pragma unroll
@@ -269,8 +298,16 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
         }
       }
     }
-    __syncthreads();  // the keys have been read
-    if (more) load_rows<T, BN>(Ks, L::KB, K, slots_s[(blk + 1) & 1]);
+    if (L::STAGES == 2) {
+      if (!works && more)
+        for (int c = 0; c < LINES; ++c) copy_keys(c, stage ^ 1), copy_values(c, stage ^ 1);
+      copies_end();
+    } else {
+      __syncthreads();  // the keys have been read
+#pragma unroll 4
+      for (int c = 0; c < LINES && more; ++c) copy_keys(c, 0);
+      copies_end();
+    }
     if (works) {
       // seen by every token: rows before the step that no window hides
       const bool open = blk * BN + BN <= first && blk * BN >= whole_from;
@@ -320,10 +357,7 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
         for (int i = 0; i < L::OT; ++i) o[i][0] *= corr[0], o[i][1] *= corr[0], o[i][2] *= corr[1], o[i][3] *= corr[1];
       }
     }
-    if (more)
-      rows_landed<1>();
-    else
-      rows_landed<0>();
+    if (L::STAGES == 1) rows_landed<1>();
     if (works) {
       if constexpr (F32) {
 #pragma unroll
@@ -331,7 +365,7 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
           uint32_t ph[4], pl[4];  // (the product's key t is this lane's first, t + 4 its second)
           cut(__float_as_uint(s[j][0]), ph[0], pl[0]), cut(__float_as_uint(s[j][2]), ph[1], pl[1]);
           cut(__float_as_uint(s[j][1]), ph[2], pl[2]), cut(__float_as_uint(s[j][3]), ph[3], pl[3]);
-          const unsigned char* row = Vs + (wn * NT * 8 + 8 * j + 2 * t4) * L::VB + g * 16;
+          const unsigned char* row = Vs + stage * L::STAGE + (wn * NT * 8 + 8 * j + 2 * t4) * L::VB + g * 16;
 #pragma unroll
           for (int c = 0; c < L::DV / 32; ++c) {
             const uint4 v0 = *reinterpret_cast<const uint4*>(row + c * 128), v1 = *reinterpret_cast<const uint4*>(row + L::VB + c * 128);
@@ -351,7 +385,7 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
 #pragma unroll
         for (int j = 0; j + 1 < NT; j += 2) {
           const uint32_t p0 = pack_bf16(s[j][0], s[j][1]), p1 = pack_bf16(s[j][2], s[j][3]), p2 = pack_bf16(s[j + 1][0], s[j + 1][1]), p3 = pack_bf16(s[j + 1][2], s[j + 1][3]);
-          const uint32_t row = (uint32_t)__cvta_generic_to_shared(Vs + (wn * NT * 8 + 8 * j + (lane & 15)) * L::VB + (lane >> 4) * 16);
+          const uint32_t row = (uint32_t)__cvta_generic_to_shared(Vs + stage * L::STAGE + (wn * NT * 8 + 8 * j + (lane & 15)) * L::VB + (lane >> 4) * 16);
           // (asked for two products ahead)
           uint32_t x[2][4];
           ldmatrix4(x[0], row);
@@ -364,8 +398,12 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
         }
       }
     }
-    __syncthreads();  // the values have been read
-    if (more) load_rows<T, BN>(Vs, L::VB, V, slots_s[(blk + 1) & 1]);
+    if (L::STAGES == 1) {
+      __syncthreads();  // the values have been read
+#pragma unroll 4
+      for (int c = 0; c < LINES && more; ++c) copy_values(c, 0);
+      copies_end();
+    }
   }
   __syncthreads();  // (queries, too: the results go over all of them)
 #pragma unroll
@@ -460,7 +498,6 @@ __global__ void __launch_bounds__(128) join_parts_kernel(const Params p) {
 template <typename T, int WM>
 int launch_rows(const Params& p, int B, int rows, cudaStream_t stream) {
   using L = Tile<T, WM>;
-  static_assert(L::SMEM <= 223 * 1024, "shared memory of an SM");
   const int tiles = (rows + L::RM - 1) / L::RM;
   if ((long long)tiles * p.nkv > 65535 || B > 65535) return TS_ERR_UNSUPPORTED_SIZE;
   const cudaError_t e = cudaFuncSetAttribute(tree_rows_kernel<T, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);

@@ -7,8 +7,9 @@
 //   o_i = sum_j p_ij v_j,  p_i = softmax over the rows it sees (and its head's sink) of s_ij = scale q_i k_j, or cap tanh(scale q_i k_j / cap).
 // A node that sees nothing gets zeros.  Scores, maxima, sums and outputs are float32 until the end.
 //
-// This file takes float32 and the heads that attention_tree_tcgen05.cu does not.  The (node, query head of a group) pairs of a request are the rows of a tile for each KV head, so that what is read of the cache is read once for them all;
-// the keys are cut into parts, a CTA each, whose results (maximum, sum, unnormalised output) a second kernel joins, always in the same order.
+// This file takes float32 and the heads that attention_tree_tcgen05.cu does not.  The (node, query head of a group) pairs of a request are the rows of a tile for
+// each KV head, so that what is read of the cache is read once for them all; the keys are cut into parts, a CTA each, whose results (maximum, sum, unnormalised
+// output) a second kernel joins, always in the same order.
 #include <math.h>
 
 #include "../common.cuh"
@@ -56,14 +57,14 @@ __device__ __forceinline__ bool sees(const Params& p, int token, int pos, int j,
 // ---------------------------------------------------------------------------
 // mma.sync: 16 WM rows, of which every warp holds 16, against blocks of keys, cut among 8 / WM warps; a warp walks its keys with maxima and sums of its own, and the
 // CTA joins its warps at the end.  bfloat16: products as they are, weights rounded to bfloat16 (their values' type).  float32: every operand is the sum of
-// two tf32 (11 bits each, rounded to nearest), a product three: h h' + h l' + l h'; what is left out is below 2^-21 of it, where a float32 sum is off by 2^-24 a
+// two tf32 (11 bits each), a product three: h h' + h l' + l h'; what is left out is below 2^-21 of it, where a float32 sum is off by 2^-24 a
 // term.
 //
 // The order of the entries inside a product does not matter, and the order of columns of the result is put right at the end: a lane takes 16 neighbouring bytes of
 // a row of queries or keys as its share of two products (for float32 values: four neighbouring columns of a row as its share of four), one load without conflicts.
 //
 // What bounds it: the old path of the tensor cores, where any such product takes 8 cycles (three of 16 x 8 x 8 a term in float32: 90 TFLOP/s of whole terms a GPU),
-// half of whose time is spent: 16 requests of 2,000 rows, 32 nodes, float32 362 us (46 TFLOP/s), 8 of 4,000, 64 nodes, bfloat16 heads of 256 363 (182 TFLOP/s); in
+// half of whose time is spent: 16 requests of 2,000 rows, 32 nodes, float32 394 us (42 TFLOP/s), 8 of 4,000, 64 nodes, bfloat16 heads of 256 365 (181 TFLOP/s); in
 // float32 the rest is the instructions that cut operands in two, in bfloat16 the loads from shared memory (as many cycles as the products), and the weights between
 // them.  Few rows are bound by the copies: chains of 4 over 4,000 rows, heads of 256, 67 us (3.9 TB/s).
 
@@ -85,7 +86,7 @@ struct Tile {
   static constexpr int OT = DV / 8;
   static constexpr int OUT = 8 * 16 * DV * 4;                       // the warps' results, when all else has been read
   static constexpr int STAGE = BN * (KB + VB);
-  // Heads up to 64: two CTAs on an SM, a block each in shared memory (12 requests with a window of 1,024, 13 nodes, float32: 83 us; two blocks each: 86).  Larger
+  // Heads up to 64: two CTAs on an SM, a block each in shared memory (12 requests with a window of 1,024, 13 nodes, float32: two blocks each 3 % slower).  Larger
   // ones: one CTA, and two blocks where they find room, the next one's copies asked for between the products of this one (8 of 4,000 rows, 16 nodes, bfloat16 heads
   // of 256: 98 us, with one block 115).
   static constexpr int CTAS = D <= 64 ? 2 : 1, ROOM = CTAS == 2 ? 112 * 1024 : 226 * 1024;
@@ -257,44 +258,50 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
 #pragma unroll
       for (int x = 0; x < 4; ++x) s[j][x] = 0.f;
     if (works) {
+      // Keys in groups, a chunk of columns a time; the next block's copies go out during the first group.  In float32 a chunk's products are summed from zero and
+      // then added: a tensor core cuts its sums off instead of rounding them, and along whole rows and blocks that was ten times the error of a float32 sum (12 requests
+      // with a window of 1,024: 3.1e-6 relative to 64 bits, 2.4e-7 so, plain float32 6.7e-7; 85 us, 92 so).
+      constexpr int J = F32 && NT > 4 ? 4 : NT;
+#pragma unroll
+      for (int j0 = 0; j0 < NT; j0 += J) {
 #pragma unroll 2
-      for (int c = 0; c < CHUNKS; ++c) {
-        if (L::STAGES == 2 && more && c % 2 == 0) copy_keys(c / 2, stage ^ 1), copy_values(c / 2, stage ^ 1);
-        const int here = (c * 64) ^ flip;
-        const uint4 a = *reinterpret_cast<const uint4*>(q_row + here), a8 = *reinterpret_cast<const uint4*>(q_row + 8 * L::KB + here);
-        const unsigned char* keys = k_row + stage * L::STAGE + here;
-        if constexpr (F32) {
-          uint32_t ah[8], al[8];
-          cut(a.x, ah[0], al[0]), cut(a8.x, ah[1], al[1]), cut(a.y, ah[2], al[2]), cut(a8.y, ah[3], al[3]);
-          cut(a.z, ah[4], al[4]), cut(a8.z, ah[5], al[5]), cut(a.w, ah[6], al[6]), cut(a8.w, ah[7], al[7]);
+        for (int c = 0; c < CHUNKS; ++c) {
+          if (L::STAGES == 2 && j0 == 0 && more && c % 2 == 0) copy_keys(c / 2, stage ^ 1), copy_values(c / 2, stage ^ 1);
+          const int here = (c * 64) ^ flip;
+          const uint4 a = *reinterpret_cast<const uint4*>(q_row + here), a8 = *reinterpret_cast<const uint4*>(q_row + 8 * L::KB + here);
+          const unsigned char* keys = k_row + stage * L::STAGE + here + j0 * 8 * L::KB;
+          uint4 k[J];
+#pragma unroll
+          for (int j = 0; j < J; ++j) k[j] = *reinterpret_cast<const uint4*>(keys + j * 8 * L::KB);
           // (a product waits for the one before it on the same scores: those of several keys take turns)
-          constexpr int J = NT < 4 ? NT : 4;
+          if constexpr (F32) {
+            uint32_t ah[8], al[8], kh[J][4], kl[J][4];
+            cut(a.x, ah[0], al[0]), cut(a8.x, ah[1], al[1]), cut(a.y, ah[2], al[2]), cut(a8.y, ah[3], al[3]);
+            cut(a.z, ah[4], al[4]), cut(a8.z, ah[5], al[5]), cut(a.w, ah[6], al[6]), cut(a8.w, ah[7], al[7]);
 #pragma unroll
-          for (int j0 = 0; j0 < NT; j0 += J) {
-            uint32_t kh[J][4], kl[J][4];
+            for (int j = 0; j < J; ++j) cut(k[j].x, kh[j][0], kl[j][0]), cut(k[j].y, kh[j][1], kl[j][1]), cut(k[j].z, kh[j][2], kl[j][2]), cut(k[j].w, kh[j][3], kl[j][3]);
+            float x[J][4];
 #pragma unroll
-            for (int j = 0; j < J; ++j) {
-              const uint4 k = *reinterpret_cast<const uint4*>(keys + (j0 + j) * 8 * L::KB);
-              cut(k.x, kh[j][0], kl[j][0]), cut(k.y, kh[j][1], kl[j][1]), cut(k.z, kh[j][2], kl[j][2]), cut(k.w, kh[j][3], kl[j][3]);
-            }
+            for (int j = 0; j < J; ++j) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
 #pragma unroll
-              for (int j = 0; j < J; ++j) mma_tf32(s[j0 + j], al[4 * u], al[4 * u + 1], al[4 * u + 2], al[4 * u + 3], kh[j][2 * u], kh[j][2 * u + 1]);
+              for (int j = 0; j < J; ++j) mma_tf32(x[j], al[4 * u], al[4 * u + 1], al[4 * u + 2], al[4 * u + 3], kh[j][2 * u], kh[j][2 * u + 1]);
 #pragma unroll
-              for (int j = 0; j < J; ++j) mma_tf32(s[j0 + j], ah[4 * u], ah[4 * u + 1], ah[4 * u + 2], ah[4 * u + 3], kl[j][2 * u], kl[j][2 * u + 1]);
-#pragma unroll
-              for (int j = 0; j < J; ++j) mma_tf32(s[j0 + j], ah[4 * u], ah[4 * u + 1], ah[4 * u + 2], ah[4 * u + 3], kh[j][2 * u], kh[j][2 * u + 1]);
+              for (int j = 0; j < J; ++j) mma_tf32(x[j], ah[4 * u], ah[4 * u + 1], ah[4 * u + 2], ah[4 * u + 3], kl[j][2 * u], kl[j][2 * u + 1]);
             }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int j = 0; j < J; ++j) mma_tf32(x[j], ah[4 * u], ah[4 * u + 1], ah[4 * u + 2], ah[4 * u + 3], kh[j][2 * u], kh[j][2 * u + 1]);
+#pragma unroll
+            for (int j = 0; j < J; ++j) s[j0 + j][0] += x[j][0], s[j0 + j][1] += x[j][1], s[j0 + j][2] += x[j][2], s[j0 + j][3] += x[j][3];
+          } else {
+#pragma unroll
+            for (int j = 0; j < J; ++j) mma_bf16(s[j], a.x, a8.x, a.y, a8.y, k[j].x, k[j].y);
+#pragma unroll
+            for (int j = 0; j < J; ++j) mma_bf16(s[j], a.z, a8.z, a.w, a8.w, k[j].z, k[j].w);
           }
-        } else {
-          uint4 k[NT];
-#pragma unroll
-          for (int j = 0; j < NT; ++j) k[j] = *reinterpret_cast<const uint4*>(keys + j * 8 * L::KB);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) mma_bf16(s[j], a.x, a8.x, a.y, a8.y, k[j].x, k[j].y);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) mma_bf16(s[j], a.z, a8.z, a.w, a8.w, k[j].z, k[j].w);
         }
       }
     }
@@ -360,25 +367,43 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
     if (L::STAGES == 1) rows_landed<1>();
     if (works) {
       if constexpr (F32) {
+        constexpr int J = NT > 1 && D <= 128 ? 2 : 1;  // 8s of keys whose products are summed from zero and then added
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          uint32_t ph[4], pl[4];  // (the product's key t is this lane's first, t + 4 its second)
-          cut(__float_as_uint(s[j][0]), ph[0], pl[0]), cut(__float_as_uint(s[j][2]), ph[1], pl[1]);
-          cut(__float_as_uint(s[j][1]), ph[2], pl[2]), cut(__float_as_uint(s[j][3]), ph[3], pl[3]);
-          const unsigned char* row = Vs + stage * L::STAGE + (wn * NT * 8 + 8 * j + 2 * t4) * L::VB + g * 16;
+        for (int j0 = 0; j0 < NT; j0 += J) {
+          uint32_t ph[J][4], pl[J][4];  // (the product's key t is this lane's first, t + 4 its second)
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            const float* w = s[j0 + j];
+            cut(__float_as_uint(w[0]), ph[j][0], pl[j][0]), cut(__float_as_uint(w[2]), ph[j][1], pl[j][1]);
+            cut(__float_as_uint(w[1]), ph[j][2], pl[j][2]), cut(__float_as_uint(w[3]), ph[j][3], pl[j][3]);
+          }
+          const unsigned char* row = Vs + stage * L::STAGE + (wn * NT * 8 + 8 * j0 + 2 * t4) * L::VB + g * 16;
 #pragma unroll
           for (int c = 0; c < L::DV / 32; ++c) {
-            const uint4 v0 = *reinterpret_cast<const uint4*>(row + c * 128), v1 = *reinterpret_cast<const uint4*>(row + L::VB + c * 128);
-            const uint32_t x0[4] = {v0.x, v0.y, v0.z, v0.w}, x1[4] = {v1.x, v1.y, v1.z, v1.w};
-            uint32_t h0[4], l0[4], h1[4], l1[4];
+            uint32_t h[J][4][2], l[J][4][2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) cut(x0[i], h0[i], l0[i]), cut(x1[i], h1[i], l1[i]);
+            for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mma_tf32(o[4 * c + i], pl[0], pl[1], pl[2], pl[3], h0[i], h1[i]);
+              for (int i = 0; i < 2; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4*>(row + (8 * j + i) * L::VB + c * 128);
+                cut(v.x, h[j][0][i], l[j][0][i]), cut(v.y, h[j][1][i], l[j][1][i]), cut(v.z, h[j][2][i], l[j][2][i]), cut(v.w, h[j][3][i], l[j][3][i]);
+              }
+            float x[4][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mma_tf32(o[4 * c + i], ph[0], ph[1], ph[2], ph[3], l0[i], l1[i]);
+            for (int i = 0; i < 4; ++i) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mma_tf32(o[4 * c + i], ph[0], ph[1], ph[2], ph[3], h0[i], h1[i]);
+            for (int j = 0; j < J; ++j) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) mma_tf32(x[i], pl[j][0], pl[j][1], pl[j][2], pl[j][3], h[j][i][0], h[j][i][1]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) mma_tf32(x[i], ph[j][0], ph[j][1], ph[j][2], ph[j][3], l[j][i][0], l[j][i][1]);
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) mma_tf32(x[i], ph[j][0], ph[j][1], ph[j][2], ph[j][3], h[j][i][0], h[j][i][1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[4 * c + i][0] += x[i][0], o[4 * c + i][1] += x[i][1], o[4 * c + i][2] += x[i][2], o[4 * c + i][3] += x[i][3];
           }
         }
       } else {

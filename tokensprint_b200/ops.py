@@ -3216,14 +3216,8 @@ class RowPools:
         self.addresses = torch.tensor([t.data_ptr() for t in pools], dtype=torch.int64).to(first.device)
 
 
-def keep_drafted_rows(pools: RowPools, path: torch.Tensor, counts: torch.Tensor, cu_seqlens: torch.Tensor, context_lens: torch.Tensor,
-                      block_table: torch.Tensor, page_size: int, num_seqs: int) -> None:
-    """Moves the accepted nodes' rows of every pool to the front of the step's rows.
-
-    A request's last t rows (t from cu_seqlens [B+1] i32) of its context_lens[b] are its nodes'; row path[b, k] of them goes to place k, for k = 1 ..
-    counts[b]; path [B,columns] and counts [B] i32 as `verify_drafts` leaves them (numbers that grow).  The first of the t rows stays, and so do rows
-    behind the last accepted one (they hold what they held, or what has not been moved from them)."""
-    flush_gemm_chain()
+def _refuse_keep_drafted_rows(pools, path, counts, cu_seqlens, context_lens, block_table, page_size, num_seqs) -> None:
+    """Raises for the argument that keep_drafted_rows does not take."""
     for name, t, n in (("counts", counts, num_seqs), ("cu_seqlens", cu_seqlens, num_seqs + 1), ("context_lens", context_lens, num_seqs)):
         _cuda_contig(name, t, torch.int32)
         if t.numel() < n:
@@ -3237,6 +3231,25 @@ def keep_drafted_rows(pools: RowPools, path: torch.Tensor, counts: torch.Tensor,
     if num_seqs > 65535:
         raise KernelError(f"keep_drafted_rows: at most 65535 requests, got {num_seqs}")
     _on_current_device("keep_drafted_rows", pools.addresses, path, counts, cu_seqlens, context_lens, block_table)
+    raise KernelError("keep_drafted_rows: arguments that are not taken")
+
+
+def keep_drafted_rows(pools: RowPools, path: torch.Tensor, counts: torch.Tensor, cu_seqlens: torch.Tensor, context_lens: torch.Tensor,
+                      block_table: torch.Tensor, page_size: int, num_seqs: int) -> None:
+    """Moves the accepted nodes' rows of every pool to the front of the step's rows.
+
+    A request's last t rows (t from cu_seqlens [B+1] i32) of its context_lens[b] are its nodes'; row path[b, k] of them goes to place k, for k = 1 ..
+    counts[b]; path [B,columns] and counts [B] i32 as `verify_drafts` leaves them (numbers that grow).  The first of the t rows stays, and so do rows
+    behind the last accepted one (they hold what they held, or what has not been moved from them)."""
+    flush_gemm_chain()
+    here = _current_device()
+    if not (
+        _takes_vector(counts, torch.int32, num_seqs, here) and _takes_vector(cu_seqlens, torch.int32, num_seqs + 1, here)
+        and _takes_vector(context_lens, torch.int32, num_seqs, here) and _takes_vector(path, torch.int32, 0, here) and _takes_vector(block_table, torch.int32, 0, here)
+        and path.dim() == 2 and path.shape[0] >= num_seqs and path.shape[1] >= 1 and block_table.dim() == 2 and block_table.shape[0] >= num_seqs
+        and block_table.shape[1] >= 1 and page_size == pools.page_size and num_seqs <= 65535 and pools.addresses.get_device() == here
+    ):
+        _refuse_keep_drafted_rows(pools, path, counts, cu_seqlens, context_lens, block_table, page_size, num_seqs)
     if num_seqs < 1:
         return
     _check("keep_drafted_rows", _fn("ts_keep_drafted_rows")(_KEEP_ARGS(
@@ -3244,15 +3257,8 @@ def keep_drafted_rows(pools: RowPools, path: torch.Tensor, counts: torch.Tensor,
         pools.num_pages, len(pools.pools), path.shape[1], block_table.shape[1], page_size, pools.row_bytes, pools.align, num_seqs)))
 
 
-def lookup_drafts(history: torch.Tensor, lengths: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, counts: torch.Tensor, num_seqs: int,
-                  depth: int, branches: int, max_suffix: int = 4, min_suffix: int = 1) -> None:
-    """Drafts from what a request's tokens have said before.
-
-    history [B,L] i32 (rows may lie further apart), lengths [B] i32: a request's tokens.  A place matches with the number of tokens up to it, at most max_suffix,
-    that equal the request's last ones; those with min_suffix or more give chains of the up to `depth` tokens behind them: the longest match first, of
-    equals the latest, up to `branches` chains whose first tokens differ.  Into tokens and parents [B, 1 + depth * branches] i32 goes the tree: the request's
-    last token as the root (parent -1), then chain after chain, -1 behind; into counts [B] i32 its nodes (0 for a request without tokens)."""
-    flush_gemm_chain()
+def _refuse_lookup_drafts(history, lengths, tokens, parents, counts, num_seqs, depth, branches, max_suffix, min_suffix) -> None:
+    """Raises for the argument that lookup_drafts does not take."""
     if not history.is_cuda or history.dtype != torch.int32 or history.dim() != 2 or history.stride(1) != 1 or history.shape[0] < num_seqs:
         raise KernelError(f"lookup_drafts: history must be an int32 CUDA matrix with a row per request, got {tuple(history.shape)}")
     if history.shape[1] < 1 or history.shape[0] > 1 and history.stride(0) < history.shape[1]:
@@ -3272,11 +3278,33 @@ def lookup_drafts(history: torch.Tensor, lengths: torch.Tensor, tokens: torch.Te
         if t.numel() < num_seqs:
             raise KernelError(f"lookup_drafts: {name} needs {num_seqs} entries, got {t.numel()}")
     _on_current_device("lookup_drafts", history, lengths, tokens, parents, counts)
+    raise KernelError("lookup_drafts: arguments that are not taken")
+
+
+def lookup_drafts(history: torch.Tensor, lengths: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, counts: torch.Tensor, num_seqs: int,
+                  depth: int, branches: int, max_suffix: int = 4, min_suffix: int = 1) -> None:
+    """Drafts from what a request's tokens have said before.
+
+    history [B,L] i32 (rows may lie further apart), lengths [B] i32: a request's tokens.  A place matches with the number of tokens up to it, at most max_suffix,
+    that equal the request's last ones; those with min_suffix or more give chains of the up to `depth` tokens behind them: the longest match first, of
+    equals the latest, up to `branches` chains whose first tokens differ.  Into tokens and parents [B, 1 + depth * branches] i32 goes the tree: the request's
+    last token as the root (parent -1), then chain after chain, -1 behind; into counts [B] i32 its nodes (0 for a request without tokens)."""
+    flush_gemm_chain()
+    shape, here, width = history.shape, _current_device(), 1 + depth * branches
+    if len(shape) != 2 or not (
+        history.is_cuda and history.get_device() == here and history.dtype is torch.int32 and history.stride(1) == 1 and shape[0] >= num_seqs
+        and 1 <= shape[1] <= LOOKUP_MAX_LENGTH and (shape[0] <= 1 or history.stride(0) >= shape[1])
+        and 1 <= depth <= LOOKUP_MAX_DEPTH and 1 <= branches <= LOOKUP_MAX_BRANCHES and 1 <= min_suffix <= max_suffix <= LOOKUP_MAX_SUFFIX
+        and _takes_vector(tokens, torch.int32, 0, here) and _takes_vector(parents, torch.int32, 0, here) and tokens.dim() == 2 and parents.dim() == 2
+        and tokens.shape[0] >= num_seqs and parents.shape[0] >= num_seqs and tokens.shape[1] == width == parents.shape[1]
+        and _takes_vector(lengths, torch.int32, num_seqs, here) and _takes_vector(counts, torch.int32, num_seqs, here)
+    ):
+        _refuse_lookup_drafts(history, lengths, tokens, parents, counts, num_seqs, depth, branches, max_suffix, min_suffix)
     if num_seqs < 1:
         return
     _check("lookup_drafts", _fn("ts_lookup_drafts")(_LOOKUP_ARGS(
-        history.data_ptr(), lengths.data_ptr(), tokens.data_ptr(), parents.data_ptr(), counts.data_ptr(), _stream(), max(history.stride(0), history.shape[1]),
-        history.shape[1], num_seqs, depth, branches, max_suffix, min_suffix)))
+        history.data_ptr(), lengths.data_ptr(), tokens.data_ptr(), parents.data_ptr(), counts.data_ptr(), _stream(), max(history.stride(0), shape[1]),
+        shape[1], num_seqs, depth, branches, max_suffix, min_suffix)))
 
 
 # ---------------------------------------------------------------------------

@@ -12,7 +12,8 @@ instead of text; without tokenizer files in the folder this is the only way),
 --dtype, --kvcache-block-size, --num-kvcache-blocks, --max-num-batched-tokens,
 --chunked-prefill, --seed, --overlap-steps (launch a step before the host has read the ids
 of the step before; default True), --cache-format kv4 (keys and values in 4 bits), --cache-budget ROWS (with it: about
-how many rows a request keeps, by the attention they get) and --cache-recent ROWS (how many of the last ones always stay).
+how many rows a request keeps, by the attention they get) and --cache-recent ROWS (how many of the last ones always stay), --speculate N (every
+decoded token is followed by guesses of up to N tokens from the request's own, which a step checks) and --speculate-branches (chains of them).
 """
 
 from __future__ import annotations

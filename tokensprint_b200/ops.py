@@ -3051,7 +3051,7 @@ def attention_tree(
     the step stands at its own number).  head_sinks [nq] f32: a score per query head that joins its softmax without a value;
     softcap > 0: the scaled score passes through softcap * tanh(s / softcap).  max_seqlen_q and max_context: the most nodes and rows of any request.
     A node that sees nothing gets zeros; rows of `out` behind the last request stay as they are.  Rows of the cache that a request holds are numbers
-    (a value of infinity counts for the nodes that do not see its row, too).
+    (an infinite value, or a float32 one above 3.4e38, counts for the nodes that do not see its row, too).
     """
     flush_gemm_chain()
     nq, nkv, d = num_heads, num_kv_heads, head_dim

@@ -32,6 +32,7 @@ namespace {
 
 constexpr int VT = 384;                // threads that scan
 constexpr int VERIFY_THREADS = VT + 32;  // and a warp that looks the children up
+constexpr int QUADS = 4;                 // four entries each that a thread asks for at once
 constexpr int MAX_CLUSTER = 16;
 constexpr int VERIFY_MAX_NODES = 256;
 
@@ -101,21 +102,23 @@ __device__ __forceinline__ void load4(const void* row, bool vector, int at, int 
 // registers on an SM hide more than one of 96 that asks for the next four meanwhile.)
 template <bool BF16, typename F>
 __device__ __forceinline__ void scan(const void* row, int begin, int end, F use) {
-  constexpr int U = 4, STEP = VT * 4;
+  constexpr int U = QUADS, STEP = VT * 4;
   const bool vector = ((uintptr_t)row & (BF16 ? 7 : 15)) == 0;
 #pragma unroll 1
   for (int at = begin; at < end; at += U * STEP) {
     float x[U][4];
 #pragma unroll
     for (int u = 0; u < U; ++u) load4<BF16>(row, vector, at + u * STEP, end, x[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[u][j] = usable(x[u][j]);
     use(at, x);
   }
 }
 
+// e^((x - m) / T) with `rate` = log2(e) / T and x <= m, but for infinity (m is the largest number then): 1.  NaN: 0.
+__device__ __forceinline__ float weight(float x, float m, float rate) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x - m) * rate));
+  return __saturatef(y);
+}
 // what is left of an entry with probability p and guess q after `n` refusals with the sums `total`
 __device__ __forceinline__ float left_of(float p, float q, const float* total, int n) {
 #pragma unroll 1
@@ -126,7 +129,8 @@ __device__ __forceinline__ float left_of(float p, float q, const float* total, i
 
 // The lanes' (m, s, i), joined: m the largest with its lowest index, s the sum of s exp((m_lane - m) / T), or with `plain_sum` the plain sum.
 __device__ __forceinline__ Stat join(Stat x, bool plain_sum, float inv_t) {
-  const float top = ts_warp_max(x.m);
+  float top;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(x.m));
   // (an index of -1 is none: the largest unsigned number)
   const unsigned i = __reduce_min_sync(0xffffffffu, x.m == top ? (unsigned)x.i : 0xffffffffu);
   const float s = plain_sum ? x.s : x.m == -INFINITY ? 0.f : x.s * __expf((x.m - top) * inv_t);
@@ -180,9 +184,11 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const VerifyA
   }
   const float T = a.temperatures[b];
   const bool greedy = !(T > 1e-10f);
+  // (a row's weights are worked out on their own, everything else about T from inv_t)
   const float inv_t = greedy ? 1.f : fmaxf(1.f / T, FLT_MIN);  // (not 0: an entry of -inf has no probability at any temperature)
 #pragma unroll 1
   for (int i = tid; i < nodes; i += VERIFY_THREADS) parent_s[i] = a.parents[first + i], token_s[i] = a.tokens[first + i], uniform_s[i] = a.uniforms[first + i];
+  const float rate = inv_t * 1.4426950408889634f;
   const int lo = rank * a.piece, hi = min(a.V, lo + a.piece), begin = lo + tid * 4;
   constexpr int ITEM = BF16 ? 2 : 4, STEP = VT * 4;
   int round = 0;
@@ -200,22 +206,23 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const VerifyA
     for (int x = tid * 128; x < (hi - lo) * ITEM; x += VERIFY_THREADS * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + (size_t)lo * ITEM + x));
     if (scans) {
       // maximum, sum and argmax of the row: a thread's own running pair
-      scan<BF16>(row, begin, hi, [&](int at, const float (&x)[4][4]) {
-        float top = -INFINITY;
+      scan<BF16>(row, begin, hi, [&](int at, const float (&x)[QUADS][4]) {
+        float most = -INFINITY;  // (NaN is never the larger one)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) top = fmaxf(top, fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])));
+        for (int u = 0; u < QUADS; ++u) most = fmaxf(most, fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])));
+        const float top = fminf(most, FLT_MAX);
         if (mi < 0 || top > m) {
           s = m == -INFINITY ? 0.f : s * __expf((m - top) * inv_t);
           m = top;
 #pragma unroll
-          for (int u = 3; u >= 0; --u)
+          for (int u = QUADS - 1; u >= 0; --u)
 #pragma unroll
             for (int j = 3; j >= 0; --j)
-              if (x[u][j] == top && at + u * STEP + j < hi) mi = at + u * STEP + j;  // (the first of equals is looked at last)
+              if (x[u][j] == most && at + u * STEP + j < hi) mi = at + u * STEP + j;  // (the first of equals is looked at last)
         }
         if (m > -INFINITY) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) s += (__expf((x[u][0] - m) * inv_t) + __expf((x[u][1] - m) * inv_t)) + (__expf((x[u][2] - m) * inv_t) + __expf((x[u][3] - m) * inv_t));
+          for (int u = 0; u < QUADS; ++u) s += (weight(x[u][0], m, rate) + weight(x[u][1], m, rate)) + (weight(x[u][2], m, rate) + weight(x[u][3], m, rate));
         }
       });
     } else {
@@ -243,7 +250,8 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const VerifyA
         for (int x = lane * 128; x < (hi - lo) * ITEM; x += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(ahead + x));
       }
     }
-    const Stat all = meet(m, s, mi, false);
+    Stat all = meet(m, s, mi, false);
+    if (all.m == -INFINITY) all.i = 0;  // (nothing but NaN and -inf)
     const float inv_s = all.s > 0.f ? 1.f / all.s : 0.f;
     const int children = children_s;  // (written before the barriers of `meet`)
     // Which child, decided alike in every CTA; with the drafter's probabilities a refusal needs the sum of what is left.
@@ -252,8 +260,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const VerifyA
     float best = -1.f, bound = -1.f;  // this thread's best of the race, and the warp's
     int best_i = -1, next = -1;
     for (;;) {
-      __syncthreads();
-      if (tid == 0) {
+      if (tid == 0) {  // (all have passed a meeting since they read what this writes, and what this reads was written ahead of one)
         int found = -1, k = asked_s;
         float mass = mass_s;
 #pragma unroll 1
@@ -304,44 +311,49 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const VerifyA
       best = bound = -1.f, best_i = -1;
       float sum = 0.f;
       if (scans) {
-        // A pair of entries a time, two on their way; whole warps walk, those whose entries are behind the end too.
+        // Four entries a time, the next ones on their way; whole warps walk, those whose entries are behind the end too.
         const uint64_t key = a.keys[b];
         const bool mask = race && !summed && children > 0;
         const int refusals = summed && whole_s == 0 ? asked : 0;
-        float x[3][2], q[3][2];
-        auto load2 = [&](int at, float (&x)[2], float (&q)[2]) {
+        const bool row_vector = ((uintptr_t)row & (BF16 ? 7 : 15)) == 0, guess_vector = summed && ((uintptr_t)guess & 15) == 0;
+        float x[2][4], q[2][4];
+        auto load = [&](int at, float (&x)[4], float (&q)[4]) {
+          load4<BF16>(row, row_vector, at, hi, x);
+          if (guess_vector && at + 4 <= hi) {
+            const float4 w = __ldg(reinterpret_cast<const float4*>(guess + at));
+            q[0] = w.x, q[1] = w.y, q[2] = w.z, q[3] = w.w;
+          } else {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const bool in = at + j < hi;
-            x[j] = !in ? -INFINITY : BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[at + j]) : reinterpret_cast<const float*>(row)[at + j];
-            q[j] = in && summed ? guess[at + j] : 0.f;
+            for (int j = 0; j < 4; ++j) q[j] = summed && at + j < hi ? guess[at + j] : 0.f;
           }
         };
-        const int from = lo + tid * 2;
-        load2(from, x[0], q[0]);
-        load2(from + VT * 2, x[1], q[1]);
+        load(begin, x[0], q[0]);
 #pragma unroll 1
-        for (int at = from; at - lane * 2 < hi; at += VT * 2) {
-          load2(at + 2 * VT * 2, x[2], q[2]);
+        for (int at = begin; at - lane * 4 < hi; at += STEP) {
+          load(at + STEP, x[1], q[1]);
           const uint32_t out = mask && at < hi ? refused_s[(at - lo) >> 5] >> ((at - lo) & 31) : 0u;
-          float r[2], v[2];
-          bool may_win[2];
-          const uint64_t z = pair_hash(key, (uint32_t)at >> 1);
+          float r[4];
+          uint32_t c[4];
+          bool may_win[4], any = false;
+          const uint64_t z0 = pair_hash(key, (uint32_t)at >> 1), z1 = pair_hash(key, ((uint32_t)at >> 1) + 1);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            r[j] = all.m == -INFINITY || ((out >> j) & 1) ? 0.f : __expf((usable(x[0][j]) - all.m) * inv_t) * inv_s;
+          for (int j = 0; j < 4; ++j) {
+            r[j] = all.m == -INFINITY || ((out >> j) & 1) ? 0.f : weight(x[0][j], all.m, rate) * inv_s;
             if (pass == 2) r[j] = fmaxf(r[j] - q[0][j], 0.f);
             else if (refusals > 0) r[j] = left_of(r[j], q[0][j], total_s, refusals);
             sum += fmaxf(r[j] - q[0][j], 0.f);
-            v[j] = ((float)((uint32_t)(z >> (j ? 16 : 40)) & 0xFFFFFFu) + 0.5f) * (1.f / 16777216.f);
-            may_win[j] = race && at + j < hi && (best_i < 0 || r[j] > bound * v[j]);
-            x[0][j] = x[1][j], x[1][j] = x[2][j], q[0][j] = q[1][j], q[1][j] = q[2][j];
+            c[j] = (uint32_t)((j < 2 ? z0 : z1) >> (j & 1 ? 16 : 40)) & 0xFFFFFFu;
+            // (from below by the upper 23 of its bits, as those of a number in [1, 2): a conversion takes longer)
+            may_win[j] = race && at + j < hi && (best_i < 0 || r[j] > fmaf(bound, __uint_as_float(0x3f800000u | (c[j] >> 1)), -bound) * 0.999999f);
+            any |= may_win[j];
+            x[0][j] = x[1][j], q[0][j] = q[1][j];
           }
-          if (__any_sync(0xffffffffu, may_win[0] || may_win[1])) {
+          if (__any_sync(0xffffffffu, any)) {
 #pragma unroll 1
-            for (int j = 0; j < 2; ++j) {
-              const float rj = j ? r[1] : r[0], vj = j ? v[1] : v[0];
-              if (j ? may_win[1] : may_win[0]) take_better(best, best_i, __fdividef(rj, -log1pf(-vj)), at + j);
+            for (int j = 0; j < 4; ++j) {
+              const float rj = j < 2 ? (j ? r[1] : r[0]) : j == 2 ? r[2] : r[3];
+              const float vj = ((float)(j < 2 ? (j ? c[1] : c[0]) : j == 2 ? c[2] : c[3]) + 0.5f) * (1.f / 16777216.f);
+              if (j < 2 ? (j ? may_win[1] : may_win[0]) : j == 2 ? may_win[2] : may_win[3]) take_better(best, best_i, __fdividef(rj, -log1pf(-vj)), at + j);
             }
             bound = fmaxf(bound, __uint_as_float(__reduce_max_sync(0xffffffffu, best < 0.f ? 0u : __float_as_uint(best))));
           }
@@ -363,8 +375,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const VerifyA
         a.path[(size_t)b * a.columns + accepted + 1] = next;
       }
       ++accepted;
-      here = next;
-      __syncthreads();  // (the children's places are written again)
+      here = next;  // (nobody but thread 0, ahead of the barrier, has read the children's places that are written again)
       continue;
     }
     if (greedy) token = max(all.i, 0);

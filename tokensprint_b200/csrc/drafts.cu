@@ -27,11 +27,10 @@ namespace {
 // entries a thread, joined in one order.  What bounds it is the chain of nodes: a trip to memory and a meeting each, so a thread asks for 16 entries at
 // once, and the first child's row is brought to the L2 meanwhile.  The race takes its logarithm only where it may win: E >= the uniform number v that it is
 // made from, so an entry with r <= best v is behind.
-// Vocabulary of 151,936, float32, us: one chain of 5 nodes 20; 32 chains of up to 6 with the drafter's probabilities 61 (59 MB, 1.0 TB/s); 16 trees of 61 nodes 35.
-// Of that a node costs some 4,000 cycles of scanning and as many of meeting and deciding, the race 11,000 to 23,000 once.
+// Vocabulary of 151,936, float32, us: one chain of 5 nodes 15.5; 32 chains of up to 6 with the drafter's probabilities 53 (59 MB, 1.1 TB/s); 16 trees of 61 nodes 36.
+// Of that a node costs 3,500 to 7,000 cycles of scanning and 5,000 of meeting and deciding, the race 10,000 to 17,000 once (1,000 for every four entries of a thread:
+// hash, exponential and comparisons; as much again where a logarithm is taken).
 
-constexpr int VT = 384;                // threads that scan
-constexpr int VERIFY_THREADS = VT + 32;  // and a warp that looks the children up
 constexpr int QUADS = 4;                 // four entries each that a thread asks for at once
 constexpr int MAX_CLUSTER = 16;
 constexpr int VERIFY_MAX_NODES = 256;
@@ -100,7 +99,7 @@ __device__ __forceinline__ void load4(const void* row, bool vector, int at, int 
 }
 // Four quadruples a thread at a time, VT * 4 entries from one to the next, all asked for before `use(entry, values)` works on them.  (Two CTAs of 72
 // registers on an SM hide more than one of 96 that asks for the next four meanwhile.)
-template <bool BF16, typename F>
+template <bool BF16, int VT, typename F>
 __device__ __forceinline__ void scan(const void* row, int begin, int end, F use) {
   constexpr int U = QUADS, STEP = VT * 4;
   const bool vector = ((uintptr_t)row & (BF16 ? 7 : 15)) == 0;
@@ -136,37 +135,36 @@ __device__ __forceinline__ Stat join(Stat x, bool plain_sum, float inv_t) {
   const float s = plain_sum ? x.s : x.m == -INFINITY ? 0.f : x.s * __expf((x.m - top) * inv_t);
   return Stat{top, ts_warp_sum(s), (int)i, 0};
 }
-// The same over all threads of the cluster that scan: every warp leaves what it found with every CTA, and every warp joins them all.  (A function of its own: what a
+// The same over all threads of the cluster that scan: the warps of a CTA, then the CTAs, each of which leaves what it found with every other.  (A function of its own: what a
 // launch runs once comes to the SM instruction by instruction from far away, so the kernel is kept short.)
-__device__ __noinline__ Stat meet_all(Stat x, bool scans, bool plain_sum, float inv_t, Stat* met) {
+template <int VT>
+__device__ __noinline__ Stat meet_all(Stat x, bool scans, bool plain_sum, float inv_t, Stat* warps, Stat* met) {
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (scans) {
     const Stat w = join(x, plain_sum, inv_t);
-    if (lane < C) *cluster.map_shared_rank(&met[(int)cluster.block_rank() * (VT / 32) + warp], lane) = w;
+    if (lane == 0) warps[warp] = w;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const Stat w = join(lane < VT / 32 ? warps[lane] : Stat{-INFINITY, 0.f, -1, 0}, plain_sum, inv_t);
+    if (lane < C) *cluster.map_shared_rank(&met[(int)cluster.block_rank()], lane) = w;
   }
   cluster.sync();  // (the places of the next round are others: nobody writes what somebody still reads)
-  Stat out{-INFINITY, 0.f, -1, 0};
-#pragma unroll 1
-  for (int k = lane; k < C * (VT / 32); k += 32) {
-    const Stat w = met[k];
-    const float top = fmaxf(out.m, w.m);
-    out.i = w.m > out.m || (w.m == out.m && (unsigned)w.i < (unsigned)out.i) ? w.i : out.i;
-    out.s = plain_sum ? out.s + w.s : top == -INFINITY ? 0.f : out.s * __expf((out.m - top) * inv_t) + w.s * __expf((w.m - top) * inv_t);
-    out.m = top;
-  }
-  return join(out, plain_sum, inv_t);
+  return join(lane < C ? met[lane] : Stat{-INFINITY, 0.f, -1, 0}, plain_sum, inv_t);
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const VerifyArgs a) {
+// VT threads scan, and a warp looks the children up.
+template <bool BF16, int VT>
+__global__ void __launch_bounds__(VT + 32, VT > 512 ? 1 : 2) verify_kernel(const VerifyArgs a) {
+  constexpr int VERIFY_THREADS = VT + 32;
   ts_pdl_prologue();
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool scans = warp < VT / 32;
   extern __shared__ uint32_t refused_s[];  // a bit per entry of this CTA's piece: tokens that were refused at the node
-  __shared__ Stat met[2][MAX_CLUSTER * (VT / 32)];  // what every warp of the cluster found
+  __shared__ Stat warps_s[VT / 32], met[2][MAX_CLUSTER];  // what the warps and the CTAs of the cluster found
   __shared__ int parent_s[VERIFY_MAX_NODES], token_s[VERIFY_MAX_NODES];
   __shared__ float child_x[VERIFY_MAX_NODES], child_q[VERIFY_MAX_NODES], uniform_s[VERIFY_MAX_NODES];
   __shared__ float total_s[VERIFY_MAX_NODES];
@@ -194,7 +192,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const VerifyA
   int round = 0;
   cluster.sync();  // every CTA of the cluster has begun: its places may be written to
 
-  auto meet = [&](float m, float s, int i, bool plain_sum) -> Stat { return meet_all(Stat{m, s, i, 0}, scans, plain_sum, inv_t, &met[round++ & 1][0]); };
+  auto meet = [&](float m, float s, int i, bool plain_sum) -> Stat { return meet_all<VT>(Stat{m, s, i, 0}, scans, plain_sum, inv_t, warps_s, met[round++ & 1]); };
 
   int here = 0, accepted = 0, token = 0;
   for (;;) {
@@ -206,7 +204,7 @@ __global__ void __launch_bounds__(VERIFY_THREADS, 2) verify_kernel(const VerifyA
     for (int x = tid * 128; x < (hi - lo) * ITEM; x += VERIFY_THREADS * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + (size_t)lo * ITEM + x));
     if (scans) {
       // maximum, sum and argmax of the row: a thread's own running pair
-      scan<BF16>(row, begin, hi, [&](int at, const float (&x)[QUADS][4]) {
+      scan<BF16, VT>(row, begin, hi, [&](int at, const float (&x)[QUADS][4]) {
         float most = -INFINITY;  // (NaN is never the larger one)
 #pragma unroll
         for (int u = 0; u < QUADS; ++u) most = fmaxf(most, fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])));
@@ -595,15 +593,18 @@ TS_EXPORT int ts_verify_drafts(const VerifyArgs* args) {
   VerifyArgs a = *args;
   if (a.B <= 0) return 0;
   if (a.V <= 0 || a.columns <= 0 || a.row_stride < a.V) return TS_ERR_BAD_ARGUMENT;
-  // Few requests: sixteen CTAs each, more than clusters need to run everywhere (the GPU may then be asked for it); else eight.
+  // Few requests: sixteen CTAs each, more than clusters need to run everywhere (the GPU may then be asked for it), with an SM each and as many threads as it
+  // has use for (one chain of 5: 384 threads 16.3 us, 768 15.5, 992 17.0); else eight, of which two share an SM.
   const int C = a.B <= 8 ? 16 : 8;
   a.piece = ((a.V + C - 1) / C + 31) / 32 * 32;
   const size_t smem = (size_t)a.piece / 8;
   if (smem > 32 * 1024 || (long long)a.B * C > (1ll << 30)) return TS_ERR_UNSUPPORTED_SIZE;
-  auto kernel = a.bf16 ? verify_kernel<true> : verify_kernel<false>;
+  constexpr int FEW = 768, MANY = 384;
+  const int threads = C == 16 ? FEW : MANY;
+  auto kernel = C == 16 ? (a.bf16 ? verify_kernel<true, FEW> : verify_kernel<false, FEW>) : a.bf16 ? verify_kernel<true, MANY> : verify_kernel<false, MANY>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return (int)e;
-  return ts_launch_cluster(kernel, dim3(a.B * C), dim3(VERIFY_THREADS), smem, (cudaStream_t)a.stream, C, a);
+  return ts_launch_cluster(kernel, dim3(a.B * C), dim3(threads + 32), smem, (cudaStream_t)a.stream, C, a);
 }
 
 TS_EXPORT int ts_keep_drafted_rows(const KeepArgs* args) {

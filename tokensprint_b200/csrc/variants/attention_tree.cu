@@ -63,10 +63,10 @@ __device__ __forceinline__ bool sees(const Params& p, int token, int pos, int j,
 // The order of the entries inside a product does not matter, and the order of columns of the result is put right at the end: a lane takes 16 neighbouring bytes of
 // a row of queries or keys as its share of two products (for float32 values: four neighbouring columns of a row as its share of four), one load without conflicts.
 //
-// What bounds it: the old path of the tensor cores, where any such product takes 8 cycles (three of 16 x 8 x 8 a term in float32: 90 TFLOP/s of whole terms a GPU),
-// half of whose time is spent: 16 requests of 2,000 rows, 32 nodes, float32 394 us (42 TFLOP/s), 8 of 4,000, 64 nodes, bfloat16 heads of 256 365 (181 TFLOP/s); in
-// float32 the rest is the instructions that cut operands in two, in bfloat16 the loads from shared memory (as many cycles as the products), and the weights between
-// them.  Few rows are bound by the copies: chains of 4 over 4,000 rows, heads of 256, 67 us (3.9 TB/s).
+// What bounds it: the old path of the tensor cores, where any such product takes 8 cycles (three of 16 x 8 x 8 a term in float32: 90 TFLOP/s of whole terms a GPU) and
+// other arithmetic hardly runs beside it.  16 requests of 2,000 rows, 32 nodes, float32: 366 us (45 TFLOP/s), the rest cuts operands in two; 8 of 4,000, 64 nodes, bfloat16 heads of
+// 256: 293 (226 TFLOP/s), the rest are loads from shared memory (as many cycles as the products) and weights.  Few rows are bound by the copies: chains of 4 over
+// 4,000 rows, heads of 256, 63 us (4.2 TB/s).
 
 constexpr int TH = 256;
 
@@ -88,7 +88,7 @@ struct Tile {
   static constexpr int STAGE = BN * (KB + VB);
   // Heads up to 64: two CTAs on an SM, a block each in shared memory (12 requests with a window of 1,024, 13 nodes, float32: two blocks each 3 % slower).  Larger
   // ones: one CTA, and two blocks where they find room, the next one's copies asked for between the products of this one (8 of 4,000 rows, 16 nodes, bfloat16 heads
-  // of 256: 98 us, with one block 115).
+  // of 256: with one block 17 % slower).
   static constexpr int CTAS = D <= 64 ? 2 : 1, ROOM = CTAS == 2 ? 112 * 1024 : 226 * 1024;
   static constexpr int STAGES = CTAS == 1 && RM * KB + 2 * STAGE <= ROOM ? 2 : 1;
   static constexpr int K_AT = RM * KB, V_AT = K_AT + BN * KB, END = K_AT + STAGES * STAGE;
@@ -205,6 +205,24 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
   };
   if (begin < end) {
     ask_page(begin);
+    // queries: row r of the tile is token r / G, head r % G; zeros behind the rows and the columns.  (Entry by entry they took as long as two blocks: 8 requests of
+    // 4,000 rows, 64 nodes, heads of 256 362 us, with copies of 16 bytes 293.)
+    if (((uintptr_t)p.q & 15) == 0) {
+#pragma unroll 4
+      for (int i = tid; i < RM * (L::KB / 16); i += TH) {
+        const int x = i / (L::KB / 16), r = r0 + x, from = i % (L::KB / 16) * 16;
+        const bool there = r < rows && from < D * (int)sizeof(T);
+        copy16(Qs + x * L::KB + (from ^ (x & 1) * L::FLIP),
+               static_cast<const unsigned char*>(p.q) + (there ? ((size_t)(q_begin + r / G) * p.nq + hk * G + r % G) * D * sizeof(T) + from : 0), there);
+      }
+    } else {
+      const T* q = reinterpret_cast<const T*>(p.q);
+      for (int i = tid; i < RM * L::DK; i += TH) {
+        const int x = i / L::DK, r = r0 + x, c = i % L::DK;
+        *reinterpret_cast<T*>(Qs + x * L::KB + ((c * (int)sizeof(T)) ^ (x & 1) * L::FLIP)) =
+            r < rows && c < D ? q[((size_t)(q_begin + r / G) * p.nq + hk * G + r % G) * D + c] : ts_from_float<T>(0.f);
+      }
+    }
     find_rows();
     ask_page(begin + 1);
 #pragma unroll 4
@@ -213,13 +231,6 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
 #pragma unroll 4
     for (int c = 0; c < LINES; ++c) copy_values(c, 0);
     copies_end();
-  }
-  // queries: row r of the tile is token r / G, head r % G
-  const T* q = reinterpret_cast<const T*>(p.q);
-  for (int i = tid; i < RM * L::DK; i += TH) {
-    const int x = i / L::DK, r = r0 + x, c = i % L::DK;
-    *reinterpret_cast<T*>(Qs + x * L::KB + ((c * (int)sizeof(T)) ^ (x & 1) * L::FLIP)) =
-        r < rows && c < D ? q[((size_t)(q_begin + r / G) * p.nq + hk * G + r % G) * D + c] : ts_from_float<T>(0.f);
   }
   if constexpr (L::DK > D) {  // (a product with zeros needs numbers beside them)
     constexpr int PAD = L::DK - D;

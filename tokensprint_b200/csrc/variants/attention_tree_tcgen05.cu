@@ -176,6 +176,7 @@ __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn_major) {
 // A request as the plan sees it: its key blocks kb0 .. kb0 + blocks - 1, its rows for a KV head and their groups.
 struct Request {
   int q_begin, t, n, kb0, blocks, rows, groups;
+  int whole_from;  // the row from which on a window hides nothing of what is before the step
 };
 template <bool WIDE>
 __device__ __noinline__ Request request_of(const Params& p, int b, int RT) {
@@ -186,10 +187,18 @@ __device__ __noinline__ Request request_of(const Params& p, int b, int RT) {
   r.rows = r.t > 0 ? r.t * (p.nq / p.nkv) : 0;
   r.groups = (r.rows + (WIDE ? 2 * RT : RT) - 1) / (WIDE ? 2 * RT : RT);
   int lo = 0;
+  r.whole_from = 0;
   if (p.window > 0 && r.t > 0) {  // the first row that any node sees
-    int lowest = INT_MAX;
+    int lowest = INT_MAX, highest = 0;
 #pragma unroll 1
-    for (int i = 0; i < r.t; ++i) lowest = min(lowest, p.positions[r.q_begin + i]);
+    for (int i = 0; i < r.t; i += 8) {  // (eight loads on their way: one behind the other they take 600 cycles each)
+      int x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = p.positions[r.q_begin + min(i + j, r.t - 1)];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) lowest = min(lowest, x[j]), highest = max(highest, x[j]);
+    }
+    r.whole_from = max(highest - p.window + 1, 0);
     const long long from = (long long)lowest - p.window + 1;
     lo = from < 0 ? 0 : from > r.n - r.t ? max(r.n - r.t, 0) : (int)from;
   }
@@ -213,7 +222,7 @@ struct __align__(16) Piece {
   int b, hk, q_begin, t;
   int n, kb, nb, r0;  // nb 0: no more pieces
   int rows, sets, whole, slot;
-  int last_cta, pad[3];   // where the group's last blocks fall
+  int last_cta, first_blk, whole_from, pad;   // where the group's last blocks fall; the group's block kb; see Request
 };
 
 // How the rows of a piece lie in the tensor memory: `sets` sets of 32 rows in different warps (8: two tiles of rows; 4, 2, 1: one tile once, twice, four times, in
@@ -269,6 +278,7 @@ struct Walk {
         r.blocks = __shfl_sync(0xffffffffu, mine.blocks, who);
         r.rows = __shfl_sync(0xffffffffu, mine.rows, who);
         r.groups = __shfl_sync(0xffffffffu, mine.groups, who);
+        r.whole_from = __shfl_sync(0xffffffffu, mine.whole_from, who);
         before += __shfl_sync(0xffffffffu, sum - cost, who);
         b = b0 + who;
         break;
@@ -297,7 +307,7 @@ struct Walk {
       const int blk0 = from > at ? (from - at + cost - 1) / cost : 0, blk1 = min(r.blocks, (to - at + cost - 1) / cost);
       const int RG = WIDE ? 2 * RT : RT, r0 = g * RG, rows = min(r.rows - r0, RG);
       // (a share has two groups in part at most, its first and its last: their places in scratch)
-      out = Piece{b, hk, r.q_begin, r.t, r.n, r.kb0 + blk0, blk1 - blk0, r0, rows, sets_of(rows, RT), blk0 == 0 && blk1 == r.blocks, at <= from ? 0 : 1, (at + (r.blocks - 1) * cost) / share, {blk0, 0, 0}};
+      out = Piece{b, hk, r.q_begin, r.t, r.n, r.kb0 + blk0, blk1 - blk0, r0, rows, sets_of(rows, RT), blk0 == 0 && blk1 == r.blocks, at <= from ? 0 : 1, (at + (r.blocks - 1) * cost) / share, blk0, r.whole_from, 0};
       at += r.blocks * cost;
       ++g;
       if (blk0 < blk1) return true;
@@ -639,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
         else if (lane == 0) {
           piece_s[at] = piece;
           mbar_arrive(smem_u32(&piece_full[at]));
-          if (piece.nb > 0 && !piece.whole && piece.pad[0] == 0) {
+          if (piece.nb > 0 && !piece.whole && piece.first_blk == 0) {
             p.plan[2 * blockIdx.x] = make_int4(piece.q_begin, piece.r0, piece.rows, piece.hk);
             p.plan[2 * blockIdx.x + 1] = make_int4(piece.last_cta, piece.slot, 0, 0);
           }
@@ -797,7 +807,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
       asm volatile(  // (all eight warps go on, or none)
           "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %0, 0;\n\tbarrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "+r"(there)::"memory");
       if (!there || r.nb == 0) break;
-      const int sets = r.sets, nb = r.nb, first = r.n - r.t;
+      const int sets = r.sets, nb = r.nb, first = r.n - r.t, whole_from = r.whole_from;
       const bool two = WIDE && sets == 8;
       // this thread's row of the group
       const int in_group = (warp & (sets - 1)) * 32 + lane;
@@ -815,7 +825,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_kernel(const __grid
         ++sc;
         __syncwarp();
         fence_after();
-        const bool open = p.window == 0 && kbase + BN <= first;
+        const bool open = kbase >= whole_from && kbase + BN <= first;
         if (sets >= 4)
           weigh<4, CAP>(p, r, token, pos, kbase, 0, open, s_addr, o_addr, it == 0, scale, m, l);
         else if (sets == 2)

@@ -331,20 +331,24 @@ __global__ void __launch_bounds__(VT + 32, VT > 512 ? 1 : 2) verify_kernel(const
           load(at + STEP, x[1], q[1]);
           const uint32_t out = mask && at < hi ? refused_s[(at - lo) >> 5] >> ((at - lo) & 31) : 0u;
           float r[4];
-          uint32_t c[4];
-          bool may_win[4], any = false;
-          const uint64_t z0 = pair_hash(key, (uint32_t)at >> 1), z1 = pair_hash(key, ((uint32_t)at >> 1) + 1);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             r[j] = all.m == -INFINITY || ((out >> j) & 1) ? 0.f : weight(x[0][j], all.m, rate) * inv_s;
             if (pass == 2) r[j] = fmaxf(r[j] - q[0][j], 0.f);
             else if (refusals > 0) r[j] = left_of(r[j], q[0][j], total_s, refusals);
             sum += fmaxf(r[j] - q[0][j], 0.f);
+            x[0][j] = x[1][j], q[0][j] = q[1][j];
+          }
+          if (!race) continue;
+          uint32_t c[4];
+          bool may_win[4], any = false;
+          const uint64_t z0 = pair_hash(key, (uint32_t)at >> 1), z1 = pair_hash(key, ((uint32_t)at >> 1) + 1);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
             c[j] = (uint32_t)((j < 2 ? z0 : z1) >> (j & 1 ? 16 : 40)) & 0xFFFFFFu;
             // (from below by the upper 23 of its bits, as those of a number in [1, 2): a conversion takes longer)
-            may_win[j] = race && at + j < hi && (best_i < 0 || r[j] > fmaf(bound, __uint_as_float(0x3f800000u | (c[j] >> 1)), -bound) * 0.999999f);
+            may_win[j] = at + j < hi && (best_i < 0 || r[j] > fmaf(bound, __uint_as_float(0x3f800000u | (c[j] >> 1)), -bound) * 0.999999f);
             any |= may_win[j];
-            x[0][j] = x[1][j], q[0][j] = q[1][j];
           }
           if (__any_sync(0xffffffffu, any)) {
 #pragma unroll 1
@@ -593,15 +597,17 @@ TS_EXPORT int ts_verify_drafts(const VerifyArgs* args) {
   VerifyArgs a = *args;
   if (a.B <= 0) return 0;
   if (a.V <= 0 || a.columns <= 0 || a.row_stride < a.V) return TS_ERR_BAD_ARGUMENT;
-  // Few requests: sixteen CTAs each, more than clusters need to run everywhere (the GPU may then be asked for it), with an SM each and as many threads as it
-  // has use for (one chain of 5: 384 threads 16.3 us, 768 15.5, 992 17.0); else eight, of which two share an SM.
+  // Few requests: sixteen CTAs each, more than clusters need to run everywhere (the GPU may then be asked for it); else eight.  With an SM for every CTA (two
+  // clusters of eight to each of the GPU's eight groups of SMs) as many threads as it has use for (one chain of 5: 384 threads 16.3 us, 768 15.5, 992 17.0; 16 trees of 61
+  // 29.5 and 25.2), else half, and two CTAs an SM (18 trees of 9: 32.4, with 768 threads 37.5).
   const int C = a.B <= 8 ? 16 : 8;
   a.piece = ((a.V + C - 1) / C + 31) / 32 * 32;
   const size_t smem = (size_t)a.piece / 8;
   if (smem > 32 * 1024 || (long long)a.B * C > (1ll << 30)) return TS_ERR_UNSUPPORTED_SIZE;
   constexpr int FEW = 768, MANY = 384;
-  const int threads = C == 16 ? FEW : MANY;
-  auto kernel = C == 16 ? (a.bf16 ? verify_kernel<true, FEW> : verify_kernel<false, FEW>) : a.bf16 ? verify_kernel<true, MANY> : verify_kernel<false, MANY>;
+  const bool few = (long long)a.B * C <= 128;
+  const int threads = few ? FEW : MANY;
+  auto kernel = few ? (a.bf16 ? verify_kernel<true, FEW> : verify_kernel<false, FEW>) : a.bf16 ? verify_kernel<true, MANY> : verify_kernel<false, MANY>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return (int)e;
   return ts_launch_cluster(kernel, dim3(a.B * C), dim3(threads + 32), smem, (cudaStream_t)a.stream, C, a);

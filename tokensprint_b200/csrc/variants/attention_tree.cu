@@ -135,6 +135,11 @@ __device__ __forceinline__ float power2(float x) {
   return y;
 }
 
+// tanh; on bfloat16 as 1 - 2 / (e^2x + 1), exact at both ends, off by a few 1e-7 in between (the weights' own rounding is 2^-9).
+template <bool ACCURATE>
+__device__ __forceinline__ float bent(float x) {
+  return ACCURATE ? tanhf(x) : 1.f - __fdividef(2.f, __expf(2.f * x) + 1.f);
+}
 // The lowest and the highest position of a request's nodes (with a window), by every warp for itself.
 __device__ __forceinline__ int2 position_range(const Params& p, int q_begin, int t) {
   int lowest = INT_MAX, highest = INT_MIN;
@@ -334,7 +339,7 @@ __global__ void __launch_bounds__(TH, Tile<T, WM>::CTAS) tree_rows_kernel(const 
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[j][x] = cap_log2 * tanhf(s[j][x] * scale);
+          for (int x = 0; x < 4; ++x) s[j][x] = cap_log2 * bent<F32>(s[j][x] * scale);
       } else {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -541,11 +546,16 @@ int launch_rows(const Params& p, int B, int rows, cudaStream_t stream) {
   return ts_launch(tree_rows_kernel<T, WM>, dim3(p.splits, tiles * p.nkv, B), dim3(TH), L::SMEM, stream, p);
 }
 
-// Warps beside one another by the rows of the largest request: the fewest that hold them all.  (Eight of them in float32 and heads above 128 find no room beside the keys.)
+// Warps beside one another by the rows of the largest request: the fewest that hold them all.  Many rows take eight (four in float32 and heads above 128, which
+// leave no room beside the keys for more), unless that would leave half of the last tile empty (16 requests of 2,000 rows, 33 nodes of four heads, float32: eight
+// 723 us, four 516; 48 nodes 724 and 589; bfloat16 heads of 256, 33 nodes 291 and 271).
 template <typename T>
 constexpr int most_warps() { return sizeof(T) == 4 && D > 128 ? 4 : 8; }
 template <typename T>
-int warps_beside(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : most_warps<T>(); }
+int warps_beside(int rows) {
+  if (rows <= 64) return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  return rows > 128 && rows % 128 > 0 && rows % 128 <= 64 ? 4 : most_warps<T>();
+}
 
 template <typename T>
 int run_rows(const Params& p, int B, int max_t, cudaStream_t stream) {

@@ -27,7 +27,7 @@ namespace {
 // entries a thread, joined in one order.  What bounds it is the chain of nodes: a trip to memory and a meeting each, so a thread asks for 16 entries at
 // once, and the first child's row is brought to the L2 meanwhile.  The race takes its logarithm only where it may win: E >= the uniform number v that it is
 // made from, so an entry with r <= best v is behind.
-// Vocabulary of 151,936, float32, us: one chain of 5 nodes 15.5; 32 chains of up to 6 with the drafter's probabilities 53 (59 MB, 1.1 TB/s); 16 trees of 61 nodes 36.
+// Vocabulary of 151,936, float32, us: one chain of 5 nodes 15.5; 32 chains of up to 6 with the drafter's probabilities 50 (59 MB, 1.2 TB/s); 16 trees of 61 nodes 34.
 // Of that a node costs 3,500 to 7,000 cycles of scanning and 5,000 of meeting and deciding, the race 10,000 to 17,000 once (1,000 for every four entries of a thread:
 // hash, exponential and comparisons; as much again where a logarithm is taken).
 

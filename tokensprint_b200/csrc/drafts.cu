@@ -118,6 +118,10 @@ __device__ __forceinline__ float weight(float x, float m, float rate) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x - m) * rate));
   return __saturatef(y);
 }
+// -ln(1 - (c + 1/2) / 2^24) of 24 bits c.  In float32 c + 1/2 is exact below 2^23 only; above, what is taken from 1 is (and the longest time is 17.3, not infinite).
+__device__ __forceinline__ float waiting(uint32_t c) {
+  return c < 1u << 23 ? -log1pf(((float)c + 0.5f) * (-1.f / 16777216.f)) : -logf(((float)((1u << 24) - c) - 0.5f) * (1.f / 16777216.f));
+}
 // what is left of an entry with probability p and guess q after `n` refusals with the sums `total`
 __device__ __forceinline__ float left_of(float p, float q, const float* total, int n) {
 #pragma unroll 1
@@ -354,8 +358,8 @@ __global__ void __launch_bounds__(VT + 32, VT > 512 ? 1 : 2) verify_kernel(const
 #pragma unroll 1
             for (int j = 0; j < 4; ++j) {
               const float rj = j < 2 ? (j ? r[1] : r[0]) : j == 2 ? r[2] : r[3];
-              const float vj = ((float)(j < 2 ? (j ? c[1] : c[0]) : j == 2 ? c[2] : c[3]) + 0.5f) * (1.f / 16777216.f);
-              if (j < 2 ? (j ? may_win[1] : may_win[0]) : j == 2 ? may_win[2] : may_win[3]) take_better(best, best_i, __fdividef(rj, -log1pf(-vj)), at + j);
+              const uint32_t cj = j < 2 ? (j ? c[1] : c[0]) : j == 2 ? c[2] : c[3];
+              if (j < 2 ? (j ? may_win[1] : may_win[0]) : j == 2 ? may_win[2] : may_win[3]) take_better(best, best_i, __fdividef(rj, waiting(cj)), at + j);
             }
             bound = fmaxf(bound, __uint_as_float(__reduce_max_sync(0xffffffffu, best < 0.f ? 0u : __float_as_uint(best))));
           }

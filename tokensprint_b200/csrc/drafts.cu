@@ -18,7 +18,8 @@ namespace {
 //
 // p = softmax(logits / T) of the node the walk stands at.  Its children in the order of their numbers: child c with token x is accepted when
 // u_c q(x) < r(x), r = p at first; a refused one takes its guess out of r: r <- max(r - q, 0) / sum.  q are the drafter's
-// probabilities there, or, without them, 1 for x alone (then r(x) = 0 and the sum is what is left of the mass).  Where no child is accepted, a token is
+// probabilities there, or, without them, 1 for x alone (then r(x) = 0 and the sum is what is left of the mass: taken off it while an eighth is left at the
+// least, else added up anew over what is left, since a difference of float32 keeps no more bits than it has).  Where no child is accepted, a token is
 // drawn from r by a race: the largest r_i / E_i, E_i = -ln(1 - (c_i + 1/2) / 2^24), c_i 24 bits of a hash of (key, i / 2).  With that the tokens that come out
 // are distributed as if the target had been asked one by one.  Temperature 0: the argmax decides.
 //
@@ -118,9 +119,13 @@ __device__ __forceinline__ float weight(float x, float m, float rate) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x - m) * rate));
   return __saturatef(y);
 }
-// -ln(1 - (c + 1/2) / 2^24) of 24 bits c.  In float32 c + 1/2 is exact below 2^23 only; above, what is taken from 1 is (and the longest time is 17.3, not infinite).
+// -ln(1 - (c + 1/2) / 2^24) of 24 bits c.  In float32 c + 1/2 is exact below 2^23 only; above, 2^24 - c - 1/2 = 2^e f with 1 <= f < 2 is: (24 - e) ln 2 - ln f, 17.3 for
+// the largest c.  One logarithm, of 1 + z, for both (one each: a chain of five 14.9 us, of which 0.7).
 __device__ __forceinline__ float waiting(uint32_t c) {
-  return c < 1u << 23 ? -log1pf(((float)c + 0.5f) * (-1.f / 16777216.f)) : -logf(((float)((1u << 24) - c) - 0.5f) * (1.f / 16777216.f));
+  const bool upper = c >= 1u << 23;
+  const uint32_t left = __float_as_uint((float)((1u << 24) - c) - 0.5f);
+  const float z = upper ? __uint_as_float((left & 0x7fffffu) | 0x3f800000u) - 1.f : ((float)c + 0.5f) * (-1.f / 16777216.f);
+  return fmaf(upper ? (float)(24 + 127 - (int)(left >> 23)) : 0.f, 0.6931471805599453f, -log1pf(z));
 }
 // what is left of an entry with probability p and guess q after `n` refusals with the sums `total`
 __device__ __forceinline__ float left_of(float p, float q, const float* total, int n) {
@@ -133,16 +138,16 @@ __device__ __forceinline__ float left_of(float p, float q, const float* total, i
 // The lanes' (m, s, i), joined: m the largest with its lowest index, s the sum of s exp((m_lane - m) / T), or with `plain_sum` the plain sum.
 __device__ __forceinline__ Stat join(Stat x, bool plain_sum, float inv_t) {
   float top;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(x.m));
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(x.m));
   // (an index of -1 is none: the largest unsigned number)
   const unsigned i = __reduce_min_sync(0xffffffffu, x.m == top ? (unsigned)x.i : 0xffffffffu);
   const float s = plain_sum ? x.s : x.m == -INFINITY ? 0.f : x.s * __expf((x.m - top) * inv_t);
   return Stat{top, ts_warp_sum(s), (int)i, 0};
 }
-// The same over all threads of the cluster that scan: the warps of a CTA, then the CTAs, each of which leaves what it found with every other.  (A function of its own: what a
-// launch runs once comes to the SM instruction by instruction from far away, so the kernel is kept short.)
+// The same over all threads of the cluster that scan: the warps of a CTA, then the CTAs, each of which leaves what it found with every other.  (As a function that is
+// called a chain of five takes 13.5 us, in place 13.1.)
 template <int VT>
-__device__ __noinline__ Stat meet_all(Stat x, bool scans, bool plain_sum, float inv_t, Stat* warps, Stat* met) {
+__device__ __forceinline__ Stat meet_all(Stat x, bool scans, bool plain_sum, float inv_t, Stat* warps, Stat* met) {
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (scans) {
@@ -158,8 +163,60 @@ __device__ __noinline__ Stat meet_all(Stat x, bool scans, bool plain_sum, float 
   return join(lane < C ? met[lane] : Stat{-INFINITY, 0.f, -1, 0}, plain_sum, inv_t);
 }
 
-// VT threads scan, and a warp looks the children up.
-template <bool BF16, int VT>
+// A request's nodes and where the walk stands among the children of one.
+struct Nodes {
+  int parent[VERIFY_MAX_NODES], token[VERIFY_MAX_NODES];
+  float uniform[VERIFY_MAX_NODES];
+  int child[VERIFY_MAX_NODES], children;                 // the children in their order,
+  float x[VERIFY_MAX_NODES], q[VERIFY_MAX_NODES];        // their logits and the drafter's probabilities,
+  float total[VERIFY_MAX_NODES];                         // and the sums of what was left behind each (with the drafter's probabilities)
+  int asked, found;      // the child that is asked next, and the one that is accepted (-1: none)
+  int last, whole;       // the last child that lost its mass (-1: none); a lone refusal left nothing
+  float mass, added;     // without the drafter's probabilities: what is left, and the sum that it was taken off
+};
+
+// Asks the children from `asked` on, until one is accepted or what is left behind a refusal has to be added up.  One thread decides, alike in every CTA.
+template <bool PROBS>
+__device__ __forceinline__ void ask(Nodes& t, float most, float inv_s, int best, float inv_t, float rate, bool greedy) {
+  const float added = t.added;
+  const int children = t.children;
+  int k = t.asked, found = -1;
+  float mass = t.mass;
+#pragma unroll 1
+  for (; k < children; ++k) {
+    const int i = t.child[k], x = t.token[i];
+    bool yes;
+    if (greedy) {
+      yes = x == best;
+    } else {
+      const float p = most == -INFINITY ? 0.f : expf((t.x[k] - most) * inv_t) * inv_s;
+      if (PROBS) {
+        yes = t.uniform[i] * t.q[k] < left_of(p, t.q[k], t.total, k);
+      } else {
+        float r = added < 1.f ? weight(t.x[k], most, rate) * inv_s : p;  // (beside a sum as the sum has it: a child with all of it is accepted)
+#pragma unroll 1
+        for (int l = 0; l < k; ++l)
+          if (t.token[t.child[l]] == x) r = 0.f;  // the same token twice: nothing is left of it
+        yes = t.uniform[i] * mass < r;
+        if (!yes && r > 0.f) {
+          t.last = i;
+          if (mass - r >= 0.125f * added) mass -= r;
+          else if (k + 1 < children) break;  // (behind the last child only the race follows, which the mass does not matter to)
+        }
+      }
+    }
+    if (yes) {
+      found = i;
+      break;
+    }
+    if (PROBS && !greedy && children > 1) break;  // (the sum scales all entries of the race alike: a lone child's is not needed)
+  }
+  t.found = found, t.asked = k, t.mass = mass;
+}
+
+// VT threads scan, and a warp looks the children up.  With the drafter's probabilities and without them are builds apart: each is shorter (16 chains without 35.1 us in a build for
+// both, 31.2), and in a build for both nvcc 12.9 took the one condition on them for true here and for false there (not with -Xcicc -O1).
+template <bool BF16, bool PROBS, int VT>
 __global__ void __launch_bounds__(VT + 32, VT > 512 ? 1 : 2) verify_kernel(const VerifyArgs a) {
   constexpr int VERIFY_THREADS = VT + 32;
   ts_pdl_prologue();
@@ -169,11 +226,7 @@ __global__ void __launch_bounds__(VT + 32, VT > 512 ? 1 : 2) verify_kernel(const
   const bool scans = warp < VT / 32;
   extern __shared__ uint32_t refused_s[];  // a bit per entry of this CTA's piece: tokens that were refused at the node
   __shared__ Stat warps_s[VT / 32], met[2][MAX_CLUSTER];  // what the warps and the CTAs of the cluster found
-  __shared__ int parent_s[VERIFY_MAX_NODES], token_s[VERIFY_MAX_NODES];
-  __shared__ float child_x[VERIFY_MAX_NODES], child_q[VERIFY_MAX_NODES], uniform_s[VERIFY_MAX_NODES];
-  __shared__ float total_s[VERIFY_MAX_NODES];
-  __shared__ int child_s[VERIFY_MAX_NODES], children_s, next_s, asked_s, whole_s, pass_s;
-  __shared__ float mass_s;
+  __shared__ Nodes tree;
 
   const int first = a.cu[b], nodes = first < 0 ? 0 : min(min(a.cu[b + 1], a.T) - first, min(VERIFY_MAX_NODES, a.columns));
   if (rank == 0) {
@@ -189,7 +242,7 @@ __global__ void __launch_bounds__(VT + 32, VT > 512 ? 1 : 2) verify_kernel(const
   // (a row's weights are worked out on their own, everything else about T from inv_t)
   const float inv_t = greedy ? 1.f : fmaxf(1.f / T, FLT_MIN);  // (not 0: an entry of -inf has no probability at any temperature)
 #pragma unroll 1
-  for (int i = tid; i < nodes; i += VERIFY_THREADS) parent_s[i] = a.parents[first + i], token_s[i] = a.tokens[first + i], uniform_s[i] = a.uniforms[first + i];
+  for (int i = tid; i < nodes; i += VERIFY_THREADS) tree.parent[i] = a.parents[first + i], tree.token[i] = a.tokens[first + i], tree.uniform[i] = a.uniforms[first + i];
   const float rate = inv_t * 1.4426950408889634f;
   const int lo = rank * a.piece, hi = min(a.V, lo + a.piece), begin = lo + tid * 4;
   constexpr int ITEM = BF16 ? 2 : 4, STEP = VT * 4;
@@ -201,7 +254,7 @@ __global__ void __launch_bounds__(VT + 32, VT > 512 ? 1 : 2) verify_kernel(const
   int here = 0, accepted = 0, token = 0;
   for (;;) {
     const unsigned char* row = reinterpret_cast<const unsigned char*>(a.logits) + (size_t)(first + here) * a.row_stride * ITEM;
-    const float* guess = a.probs ? a.probs + (size_t)(first + here) * a.probs_stride : nullptr;
+    const float* guess = PROBS ? a.probs + (size_t)(first + here) * a.probs_stride : nullptr;
     float m = -INFINITY, s = 0.f;
     int mi = -1;
 #pragma unroll 1
@@ -233,19 +286,19 @@ __global__ void __launch_bounds__(VT + 32, VT > 512 ? 1 : 2) verify_kernel(const
 #pragma unroll 1
       for (int i0 = here + 1; i0 < nodes; i0 += 32) {
         const int i = i0 + lane;
-        const bool mine = i < nodes && parent_s[i] == here && token_s[i] >= 0 && token_s[i] < a.V;
+        const bool mine = i < nodes && tree.parent[i] == here && tree.token[i] >= 0 && tree.token[i] < a.V;
         const unsigned all = __ballot_sync(0xffffffffu, mine);
         if (oldest < 0 && all != 0) oldest = i0 + __ffs(all) - 1;
         if (mine) {
           const int k = n + __popc(all & ((1u << lane) - 1));
-          child_s[k] = i;
-          const int x = token_s[i];
-          child_x[k] = usable(BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[x]) : reinterpret_cast<const float*>(row)[x]);
-          child_q[k] = guess ? guess[x] : 1.f;
+          tree.child[k] = i;
+          const int x = tree.token[i];
+          tree.x[k] = usable(BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[x]) : reinterpret_cast<const float*>(row)[x]);
+          if (PROBS) tree.q[k] = guess[x];
         }
         n += __popc(all);
       }
-      if (lane == 0) children_s = n;
+      if (lane == 0) tree.children = n;
       if (oldest >= 0) {  // the likeliest next row, this CTA's piece of it
         const unsigned char* ahead = reinterpret_cast<const unsigned char*>(a.logits) + ((size_t)(first + oldest) * a.row_stride + lo) * ITEM;
 #pragma unroll 1
@@ -255,57 +308,28 @@ __global__ void __launch_bounds__(VT + 32, VT > 512 ? 1 : 2) verify_kernel(const
     Stat all = meet(m, s, mi, false);
     if (all.m == -INFINITY) all.i = 0;  // (nothing but NaN and -inf)
     const float inv_s = all.s > 0.f ? 1.f / all.s : 0.f;
-    const int children = children_s;  // (written before the barriers of `meet`)
-    // Which child, decided alike in every CTA; with the drafter's probabilities a refusal needs the sum of what is left.
-    const bool summed = guess != nullptr && !greedy;
-    if (tid == 0) asked_s = 0, whole_s = 0, mass_s = 1.f;
+    const int children = tree.children;  // (written before the barriers of `meet`)
+    // Which child, decided alike in every CTA; with the drafter's probabilities a refusal needs the sum of what is left, without them where little is.
+    if (tid == 0) tree.asked = 0, tree.whole = 0, tree.mass = tree.added = 1.f, tree.last = -1;
     float best = -1.f, bound = -1.f;  // this thread's best of the race, and the warp's
     int best_i = -1, next = -1;
     for (;;) {
-      if (tid == 0) {  // (all have passed a meeting since they read what this writes, and what this reads was written ahead of one)
-        int found = -1, k = asked_s;
-        float mass = mass_s;
-#pragma unroll 1
-        for (; k < children; ++k) {
-          const int i = child_s[k], x = token_s[i];
-          const float p = all.m == -INFINITY ? 0.f : expf((child_x[k] - all.m) * inv_t) * inv_s;
-          bool yes;
-          if (greedy) {
-            yes = x == all.i;
-          } else if (summed) {
-            yes = uniform_s[i] * child_q[k] < left_of(p, child_q[k], total_s, k);
-          } else {
-            float r = p;
-#pragma unroll 1
-            for (int l = 0; l < k; ++l)
-              if (token_s[child_s[l]] == x) r = 0.f;  // the same token twice: nothing is left of it
-            yes = uniform_s[i] * mass < r;
-            if (!yes && mass - r > 0.f) mass -= r;
-          }
-          if (yes) {
-            found = i;
-            break;
-          }
-          if (summed && children > 1) break;  // (the sum scales all entries of the race alike: a lone child's is not needed)
-        }
-        next_s = found;
-        asked_s = k;
-        mass_s = mass;
-        // What follows: 0 the sum of what is left, 1 the race over it; 2: over r = max(p - q, 0) of one refused child, whose sum does not matter.
-        pass_s = k < children ? 0 : summed && children == 1 && whole_s == 0 ? 2 : 1;
-      }
+      if (tid == 0) ask<PROBS>(tree, all.m, inv_s, all.i, inv_t, rate, greedy);  // (all have passed a meeting since they read what this writes)
       __syncthreads();
-      next = next_s;
-      const int asked = asked_s, pass = pass_s;
+      next = tree.found;
       if (next >= 0 || greedy) break;
-      const bool race = pass != 0;
-      if (race && !summed && children > 0) {
+      // What follows: 0 the sum of what is left, 1 the race over it; 2: over r = max(p - q, 0) of one refused child, whose sum does not matter.
+      const int asked = tree.asked, last = tree.last;
+      const bool whole = tree.whole != 0;
+      const int pass = asked < children ? 0 : PROBS && children == 1 && !whole ? 2 : 1;
+      const bool race = pass != 0, mask = !PROBS && children > 0;
+      if (mask) {
 #pragma unroll 1
         for (int i = tid; i < a.piece / 32; i += VERIFY_THREADS) refused_s[i] = 0;
         __syncthreads();
 #pragma unroll 1
-        for (int k = tid; k < children; k += VERIFY_THREADS) {
-          const int x = token_s[child_s[k]] - lo;
+        for (int k = tid; k < (race ? children : asked + 1); k += VERIFY_THREADS) {
+          const int x = tree.token[tree.child[k]] - lo;
           if (x >= 0 && x < a.piece) atomicOr(&refused_s[x >> 5], 1u << (x & 31));
         }
         __syncthreads();
@@ -315,18 +339,18 @@ __global__ void __launch_bounds__(VT + 32, VT > 512 ? 1 : 2) verify_kernel(const
       if (scans) {
         // Four entries a time, the next ones on their way; whole warps walk, those whose entries are behind the end too.
         const uint64_t key = a.keys[b];
-        const bool mask = race && !summed && children > 0;
-        const int refusals = summed && whole_s == 0 ? asked : 0;
-        const bool row_vector = ((uintptr_t)row & (BF16 ? 7 : 15)) == 0, guess_vector = summed && ((uintptr_t)guess & 15) == 0;
-        float x[2][4], q[2][4];
+        const int refusals = PROBS && !whole ? asked : 0;
+        const bool row_vector = ((uintptr_t)row & (BF16 ? 7 : 15)) == 0, guess_vector = PROBS && ((uintptr_t)guess & 15) == 0;
+        float x[2][4], q[2][4] = {};  // (without the drafter's probabilities zeros throughout)
         auto load = [&](int at, float (&x)[4], float (&q)[4]) {
           load4<BF16>(row, row_vector, at, hi, x);
+          if (!PROBS) return;
           if (guess_vector && at + 4 <= hi) {
             const float4 w = __ldg(reinterpret_cast<const float4*>(guess + at));
             q[0] = w.x, q[1] = w.y, q[2] = w.z, q[3] = w.w;
           } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) q[j] = summed && at + j < hi ? guess[at + j] : 0.f;
+            for (int j = 0; j < 4; ++j) q[j] = at + j < hi ? guess[at + j] : 0.f;
           }
         };
         load(begin, x[0], q[0]);
@@ -339,7 +363,7 @@ __global__ void __launch_bounds__(VT + 32, VT > 512 ? 1 : 2) verify_kernel(const
           for (int j = 0; j < 4; ++j) {
             r[j] = all.m == -INFINITY || ((out >> j) & 1) ? 0.f : weight(x[0][j], all.m, rate) * inv_s;
             if (pass == 2) r[j] = fmaxf(r[j] - q[0][j], 0.f);
-            else if (refusals > 0) r[j] = left_of(r[j], q[0][j], total_s, refusals);
+            else if (refusals > 0) r[j] = left_of(r[j], q[0][j], tree.total, refusals);
             sum += fmaxf(r[j] - q[0][j], 0.f);
             x[0][j] = x[1][j], q[0][j] = q[1][j];
           }
@@ -367,17 +391,20 @@ __global__ void __launch_bounds__(VT + 32, VT > 512 ? 1 : 2) verify_kernel(const
       }
       const Stat found = meet(best, race ? 0.f : sum, best_i, true);
       if (race) {
-        token = found.i;
+        token = mask && last >= 0 && !(found.m > 0.f) ? tree.token[last] : found.i;  // (nothing is left: what was refused last had it all)
         if (pass == 1 || found.m > 0.f) break;
-        if (tid == 0) whole_s = 1;  // nothing was left behind the lone refusal: as if nothing had been refused
-      } else if (tid == 0) {
-        total_s[asked] = found.s;
-        asked_s = asked + 1;
+        if (tid == 0) tree.whole = 1;  // nothing was left behind the lone refusal: as if nothing had been refused
+      } else {
+        if (tid == 0) tree.total[asked] = tree.mass = tree.added = found.s, tree.asked = asked + 1;
+        if (mask && !(found.s > 0.f)) {
+          token = tree.token[last];
+          break;
+        }
       }
     }
     if (next >= 0) {
       if (rank == 0 && tid == 0) {
-        a.fresh[(size_t)b * a.columns + accepted] = token_s[next];
+        a.fresh[(size_t)b * a.columns + accepted] = tree.token[next];
         a.path[(size_t)b * a.columns + accepted + 1] = next;
       }
       ++accepted;
@@ -611,7 +638,8 @@ TS_EXPORT int ts_verify_drafts(const VerifyArgs* args) {
   constexpr int FEW = 768, MANY = 384;
   const bool few = (long long)a.B * C <= 128;
   const int threads = few ? FEW : MANY;
-  auto kernel = few ? (a.bf16 ? verify_kernel<true, FEW> : verify_kernel<false, FEW>) : a.bf16 ? verify_kernel<true, MANY> : verify_kernel<false, MANY>;
+  auto kernel = a.probs != nullptr ? (few ? (a.bf16 ? verify_kernel<true, true, FEW> : verify_kernel<false, true, FEW>) : a.bf16 ? verify_kernel<true, true, MANY> : verify_kernel<false, true, MANY>)
+                : few ? (a.bf16 ? verify_kernel<true, false, FEW> : verify_kernel<false, false, FEW>) : a.bf16 ? verify_kernel<true, false, MANY> : verify_kernel<false, false, MANY>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return (int)e;
   return ts_launch_cluster(kernel, dim3(a.B * C), dim3(threads + 32), smem, (cudaStream_t)a.stream, C, a);

@@ -96,10 +96,10 @@ class Scheduler:
     def _reserve(self, seq: Sequence, share: int) -> bool:
         """Pages for the next `share` tokens of a sequence that has a cache; False: not now."""
         first = seq.num_cached_tokens
-        if share > 1 and seq.tree is not None and not self.cache_manager.can_extend(seq.cache, first, first + share):
-            seq.tree, share = seq.tree.root(), 1  # the drafts find no pages
         if not self.cache_manager.can_extend(seq.cache, first, first + share):
-            return False
+            if seq.tree is None or share == 1 or not self.cache_manager.can_extend(seq.cache, first, first + 1):
+                return False
+            seq.tree, share = seq.tree.root(), 1  # the drafts find no pages
         self.cache_manager.extend(seq.cache, first, first + share)
         seq.num_new_tokens = share
         return True

@@ -81,12 +81,13 @@ class Scheduler:
 
     # -- one step ---------------------------------------------------------------------
 
-    def _share(self, seq: Sequence, budget: int) -> int:
+    def _share(self, seq: Sequence, budget: int, behind: int = 0) -> int:
         """How many of the tokens it has not cached yet `seq` runs in a step with `budget` left:
-        all of them, cut to the budget where portions are allowed, and never past the model's length."""
+        all of them, cut to the budget where portions are allowed, and never past the model's length.
+        Drafts leave a token of the budget to each of the `behind` requests that come after."""
         share = len(seq) - seq.num_cached_tokens
         if seq.tree is not None:
-            if len(seq.tree) > budget:
+            if len(seq.tree) > budget - behind:
                 seq.tree = seq.tree.root()
             return len(seq.tree)
         if self.enable_chunked:
@@ -104,18 +105,35 @@ class Scheduler:
         seq.num_new_tokens = share
         return True
 
+    def _give_up_drafts(self, step: list[Sequence]) -> int:
+        """The last request of the step whose drafts hold pages of their own goes on with its root alone; how many
+        tokens that leaves, 0: there is none."""
+        cm = self.cache_manager
+        for seq in reversed(step):
+            root = seq.num_cached_tokens + 1
+            if seq.tree is not None and any(len(t) > -(-root // cm.page_size) for t in seq.cache.tables):
+                cm.retract(seq.cache, root)
+                left = seq.num_new_tokens - 1
+                seq.tree, seq.num_new_tokens = seq.tree.root(), 1
+                return left
+        return 0
+
     def _continue_running(self, budget: int, step: list[Sequence]) -> tuple[int, bool]:
-        """Running requests in their order while the budget lasts.  One that finds no pages takes
-        them from the tail of the running list, request by request, itself last.  Returns the
+        """Running requests in their order while the budget lasts.  One that finds no pages takes those that
+        drafts hold, then, from the tail of the running list, request by request, itself last, those of others.  Returns the
         budget left and whether anybody lost its place."""
         evicted = False
         place = 0
         while place < len(self.running) and budget > 0:
             seq = self.running[place]
-            share = self._share(seq, budget)
+            share = self._share(seq, budget, len(self.running) - place - 1)
             if share < 1:
                 raise RuntimeError(f"Running sequence {seq.seq_id} has nothing to compute (share {share}).")
             while seq.status == SequenceStatus.RUNNING and not self._reserve(seq, share):
+                left = self._give_up_drafts(step)
+                if left:
+                    budget += left
+                    continue
                 self.preempt(self.running[-1])
                 evicted = True
             if seq.status != SequenceStatus.RUNNING:

@@ -82,6 +82,7 @@ class StepStats:
 class LLMEngine:
     def __init__(self, model: Model, config: Config, tokenizer: Optional[Any] = None) -> None:
         self.config = config
+        drafts = getattr(config, "speculate", 0)
         self.model_runner = ModelRunner(
             model,
             page_size=config.kvcache_block_size,
@@ -96,6 +97,8 @@ class LLMEngine:
             cache_recent=config.cache_recent,
             cache_first=config.cache_first,
             cache_slack=config.cache_slack,
+            rows_per_request=1 + drafts * config.speculate_branches if drafts else 1,
+            reserved_bytes=Speculator.history_bytes(config.max_num_seqs, config.max_model_len) if drafts else 0,
         )
         # (a model whose mixers keep fixed-size state only has no page pool at all)
         config.num_kvcache_blocks = self.model_runner.num_pages[0] if self.model_runner.num_pages else 0
@@ -110,7 +113,7 @@ class LLMEngine:
         self.overlap = bool(getattr(config, "overlap_steps", True))
         self._inflight = None
         self.speculator: Optional[Speculator] = None
-        if getattr(config, "speculate", 0):
+        if drafts:
             self.speculator = Speculator(self.model_runner, config.speculate, config.speculate_branches, config.speculate_suffix)
             self.overlap = False  # what a step drafts from is what the step before has accepted
         self.stats: Optional[StepStats] = None

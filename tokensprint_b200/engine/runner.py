@@ -113,6 +113,8 @@ class ModelRunner:
         cache_recent: int = 64,
         cache_first: int = 4,
         cache_slack: int = 64,
+        rows_per_request: int = 1,
+        reserved_bytes: int = 0,
     ) -> None:
         if model.device.type != "cuda":
             raise RuntimeError("ModelRunner needs a CUDA device: the engine has no CPU path")
@@ -171,6 +173,9 @@ class ModelRunner:
         self._capture_stream: Optional[torch.cuda.Stream] = None
         self.graph_launches = 0  # kernels of this library replayed inside graphs so far
         self._sizing_step = False
+        # How many rows of logits a step may want of every request (a row a node, where steps check drafts), and bytes that the engine
+        # will take beside pages and steps: what sizing from free memory leaves room for.
+        self.rows_per_request, self.reserved_bytes = max(1, rows_per_request), reserved_bytes
         self._last_trees: Optional[StepContext] = None  # the last step that brought trees of drafted tokens
         self._row_pools: Optional[tuple] = None
         self.sizing: Optional[dict] = None  # how the page count was derived, when it came from free memory
@@ -207,8 +212,8 @@ class ModelRunner:
         (engine/generation/model_runner.py:392-411).  Here the peak is measured the same way: a
         step of `max_num_batched_tokens` tokens runs once against a throw-away pool just large
         enough for it, torch's peak statistics give what its activations need, and the pool gets
-        `utilization` of what is free afterwards less that peak and less what the decode graphs
-        will hold (their static logits).  All groups get the same number of pages."""
+        `utilization` of what is free afterwards less that peak, less what the decode graphs
+        will hold (their static logits) and less `reserved_bytes`.  All groups get the same number of pages."""
         P = self.page_size
         tokens = max(1, self.max_num_batched_tokens)
         per_request = max(1, min(tokens, self.max_model_len - 1))
@@ -220,10 +225,14 @@ class ModelRunner:
         torch.cuda.reset_peak_memory_stats(self.device)
         before = torch.cuda.memory_allocated(self.device)
         entries = []
+        # A row of logits a request; where requests want several, as many as all of them together may want of a step.
+        rows = 0 if self.rows_per_request == 1 else min(self.num_slots * self.rows_per_request, tokens)
         for i, n in enumerate(lengths):
             rc = self.cache_manager.admit(("sizing", i))
             self.cache_manager.extend(rc, 0, n)
-            entries.append(StepEntry(rc, [0] * n, 0, [n - 1]))
+            want = min(n, max(1, rows - (len(lengths) - 1 - i)))
+            rows -= want
+            entries.append(StepEntry(rc, [0] * n, 0, range(n - want, n)))
         graphs, self.use_graphs = self.use_graphs, False
         self._sizing_step = True
         self.step(entries)
@@ -240,16 +249,16 @@ class ModelRunner:
         if self.use_graphs:  # every bucket keeps its logits [bucket, vocab] float32, and a little beside
             graph_reserve = int(sum(self.graph_buckets) * self.vocab_size * 4 * 1.25)
         margin = 256 << 20
-        budget = int(free * utilization) - peak - graph_reserve - margin
+        budget = int(free * utilization) - peak - graph_reserve - self.reserved_bytes - margin
         per_page = sum(self.page_bytes)
         n = budget // max(per_page, 1)
         self.sizing = {"free_bytes": int(free), "total_bytes": int(total), "utilization": utilization,
                        "step_tokens": sum(lengths), "step_peak_bytes": int(peak), "graph_reserve_bytes": graph_reserve,
-                       "margin_bytes": margin, "bytes_per_page": int(per_page), "pages": int(n)}
+                       "reserved_bytes": self.reserved_bytes, "margin_bytes": margin, "bytes_per_page": int(per_page), "pages": int(n)}
         if n < 1:
             raise RuntimeError(
                 f"Insufficient GPU memory for the cache: {budget} bytes are left after a step of {sum(lengths)} tokens "
-                f"({peak} bytes) and the graphs' reserve ({graph_reserve}); one page costs {per_page} bytes")
+                f"({peak} bytes), the graphs' reserve ({graph_reserve}) and {self.reserved_bytes} kept for the engine; one page costs {per_page} bytes")
         return [int(n)] * len(self.groups)
 
     # -- the step ----------------------------------------------------------------------

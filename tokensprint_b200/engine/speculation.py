@@ -56,6 +56,11 @@ def _uniforms(key: int, count: int) -> np.ndarray:
 
 
 class Speculator:
+    @staticmethod
+    def history_bytes(num_slots: int, max_model_len: int) -> int:
+        """What it keeps on the device: every request's tokens."""
+        return 4 * num_slots * max_model_len
+
     def __init__(self, runner: ModelRunner, depth: int, branches: int, suffix: int) -> None:
         for run in runner.model.spec.run_order:
             why = runner.model.blocks[run.layer].mixer.tree_refusal()

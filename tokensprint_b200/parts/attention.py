@@ -417,8 +417,10 @@ class AttentionMixer(Mixer):
             ops.attention_prefill_tcgen05(q, cache.k_pages, cache.v_pages, out, cu, lens, table, step.page_size, B - n, step.max_seqlen_q, nq, nkv, self.scale,
                                           self.window)
         elif q.dtype == torch.bfloat16 and ops.attention_mma_supported(d):
+            # The keys of a portion are not split among CTAs: the kernels that join such parts go over every row of `out` (and write zeros where
+            # the sequence's number is negative, which here are the trees' results).
             ops.attention_paged_mma(q, cache.k_pages, cache.v_pages, out, cu, lens, table, step.seq_index - n, step.page_size, B - n, step.max_seqlen_q, nq, nkv, d,
-                                    self.scale, self.window)
+                                    self.scale, self.window, splits=1)
         elif ops.attention_float32_supported(d, q, cache.k_pages, cache.v_pages, out):
             ops.attention_paged_float32(q, cache.k_pages, cache.v_pages, out, cu, lens, table, step.page_size, B - n, step.max_seqlen_q, nq, nkv, d, self.scale,
                                         self.window)

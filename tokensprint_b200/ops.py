@@ -3005,8 +3005,8 @@ def _refuse_attention_tree(q, k_cache, v_cache, out, tree_mask, cu_seqlens_q, co
         raise KernelError("attention_tree: block_table must be [B,max_blocks]")
     if cu_seqlens_q.numel() < num_seqs + 1 or context_lens.numel() < num_seqs:
         raise KernelError("attention_tree: cu_seqlens_q/context_lens are shorter than the batch")
-    if num_seqs > 65535 or max_context < 0 or window < 0 or not 0.0 <= softcap < math.inf:
-        raise KernelError("attention_tree: at most 65535 requests, max_context and window not negative, softcap 0 or positive and finite")
+    if num_seqs > 65535 or not 0 <= max_context < 1 << 31 or not 0 <= window < 1 << 31 or not 0.0 <= softcap < math.inf:
+        raise KernelError("attention_tree: at most 65535 requests, max_context and window not negative and below 2^31, softcap 0 or positive and finite")
     if window > 0:
         if positions is None:
             raise KernelError("attention_tree: a window needs the nodes' positions")
@@ -3017,7 +3017,9 @@ def _refuse_attention_tree(q, k_cache, v_cache, out, tree_mask, cu_seqlens_q, co
         _cuda_contig("attention_tree: head_sinks", head_sinks, torch.float32)
         if head_sinks.numel() != nq:
             raise KernelError(f"attention_tree: head_sinks must have one entry per query head ({nq}), got {head_sinks.numel()}")
-    raise KernelError("attention_tree: the caches must begin at multiples of 16 bytes")
+    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise KernelError("attention_tree: the caches must begin at multiples of 16 bytes")
+    raise KernelError("attention_tree: arguments that are not taken")
 
 
 def attention_tree(
@@ -3070,7 +3072,7 @@ def attention_tree(
         and len(ks) == 4 and ks == v_cache.shape and ks[1] == page_size and ks[2] == nkv and ks[3] == d and page_size >= 1
         and 1 <= max_seqlen_q <= TREE_MAX_NODES and len(ms) == 2 and ms[0] >= T and 64 * ms[1] >= max_seqlen_q
         and len(ts) == 2 and ts[0] >= num_seqs and ts[1] >= 1 and cu_seqlens_q.numel() > num_seqs and context_lens.numel() >= num_seqs
-        and num_seqs <= 65535 and max_context >= 0 and window >= 0 and 0.0 <= softcap < math.inf
+        and num_seqs <= 65535 and 0 <= max_context < 1 << 31 and 0 <= window < 1 << 31 and 0.0 <= softcap < math.inf
         and (window == 0 or positions is not None and positions.dtype is torch.int32 and positions.is_contiguous() and positions.get_device() == here
              and positions.numel() >= T)
         and (head_sinks is None or head_sinks.dtype is torch.float32 and head_sinks.is_contiguous() and head_sinks.get_device() == here

@@ -75,7 +75,8 @@ class Config:
     cache_slack: int = 64
     # speculate > 0: every decoded token is followed by guesses, up to `speculate_branches` chains of up to `speculate` tokens that followed earlier
     # occurrences of the request's last 1 to `speculate_suffix` tokens; a step checks them all and keeps those that the model's probabilities
-    # accept, so that the tokens are distributed as without (greedy ones: are the same).  For models whose layers are all plain attention; steps do not overlap.
+    # accept, so that the tokens are distributed as without (greedy ones: are the same; sampled ones may be others of the same distribution, from run to run too where
+    # portions, budget or pages make steps fall elsewhere).  For models whose layers are all plain attention; steps do not overlap.
     speculate: int = 0
     speculate_branches: int = 1
     speculate_suffix: int = 4

@@ -28,7 +28,8 @@ namespace {
 // entries a thread, joined in one order.  What bounds it is the chain of nodes: a trip to memory and a meeting each, so a thread asks for 16 entries at
 // once, and the first child's row is brought to the L2 meanwhile.  The race takes its logarithm only where it may win: E >= the uniform number v that it is
 // made from, so an entry with r <= best v is behind.
-// Vocabulary of 151,936, float32, us: one chain of 5 nodes 15.5; 32 chains of up to 6 with the drafter's probabilities 50 (59 MB, 1.2 TB/s); 16 trees of 61 nodes 34.
+// Vocabulary of 151,936, float32, us on the device: one chain of 5 nodes 13.1; 32 chains of up to 6 with the drafter's probabilities 50 (59 MB, 1.2 TB/s); 16 greedy trees of 61
+// nodes 27.7.
 // Of that a node costs 3,500 to 7,000 cycles of scanning and 5,000 of meeting and deciding, the race 10,000 to 17,000 once (1,000 for every four entries of a thread:
 // hash, exponential and comparisons; as much again where a logarithm is taken).
 
@@ -629,8 +630,8 @@ TS_EXPORT int ts_verify_drafts(const VerifyArgs* args) {
   if (a.B <= 0) return 0;
   if (a.V <= 0 || a.columns <= 0 || a.row_stride < a.V) return TS_ERR_BAD_ARGUMENT;
   // Few requests: sixteen CTAs each, more than clusters need to run everywhere (the GPU may then be asked for it); else eight.  With an SM for every CTA (two
-  // clusters of eight to each of the GPU's eight groups of SMs) as many threads as it has use for (one chain of 5: 384 threads 16.3 us, 768 15.5, 992 17.0; 16 trees of 61
-  // 29.5 and 25.2), else half, and two CTAs an SM (18 trees of 9: 32.4, with 768 threads 37.5).
+  // clusters of eight to each of the GPU's eight groups of SMs) as many threads as it has use for (one chain of 5: 384 threads 13.4 us, 768 13.1, 992 14.0; 16 greedy
+  // trees of 61 32.2, 27.7, 30.0), else half, and two CTAs an SM (32 chains with the drafter's probabilities 49.9, with 768 threads 66).
   const int C = a.B <= 8 ? 16 : 8;
   a.piece = ((a.V + C - 1) / C + 31) / 32 * 32;
   const size_t smem = (size_t)a.piece / 8;

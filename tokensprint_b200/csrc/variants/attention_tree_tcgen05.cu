@@ -6,7 +6,7 @@
 // What bounds a step is reading the cache: 64 KB a block at 44 GB/s an SM are 1.5 us, the products of one tile 0.55.  The rest follows from that:
 // * Persistent CTAs, each with an even share of all (request, KV head, group, block)s, worked out on the device: lengths and trees differ, and a
 //   captured step serves them all.  A group whose blocks fall to several CTAs leaves parts, joined by a second kernel in a fixed order.
-// * The copying warp runs ahead over the ends of groups, so that the rings stay full while a group's results leave.
+// * The copying warps run ahead over the ends of groups, so that the rings stay full while a group's results leave.
 // * Groups of one tile take turns on two accumulators: tile 0 the even blocks, tile 1 the odd ones, so that one block's exponentials run beside the next one's products.
 // * Few rows would leave the exponentials of a block to one warp: up to 64 rows stand in the tile twice, up to 32 four times, and every copy weighs its own
 //   half or quarter of the block's keys (the others' weights are zero).  The copies' sums are added when the group is done.
@@ -14,6 +14,9 @@
 // A row's maximum is raised only when it lags more than 2^8 behind (the weights stay far inside bfloat16's range, and the division by the sum, taken with
 // the same maximum, cancels it).  Weights are rounded to bfloat16 for the product with the values, their own type; sums take them unrounded.
 // Every wait is bounded: one that gives up raises the error word, and the CTA ends in order.
+//
+// Times below of 4 trees of 61 at 30,000 rows are of short bursts at 1.95 GHz, where the present kernel takes 218 us; in a loop of seconds the power cap holds 1.5 GHz, and it
+// takes 260.
 #include <math.h>
 
 #include "../common.cuh"
@@ -962,7 +965,7 @@ int launch(const CUtensorMap* maps, const Params& p, int max_t, cudaStream_t str
 
 }  // namespace
 
-// Whether these kernels take the sizes (the CUDA-core kernel takes all).
+// Whether these kernels take the sizes (those of attention_tree.cu take all).
 TS_EXPORT int ts_attention_tree_tcgen05_takes(int B, int max_t, int max_context, int nq, int nkv, int page, long long num_pages, float scale) {
   if (nkv <= 0 || nq % nkv || nq / nkv > BM || B > 65535 || max_t > MAX_NODES || nkv > 65535 || !(scale > 0.f)) return 0;
   if (page < 8 || !(BN % page == 0 || page % BN == 0) || num_pages * page > 0x7fffffffLL - page) return 0;

@@ -3,7 +3,9 @@
 A decoding request brings a small tree to a step: its newest token and, hanging on it, chains of guesses (ops.lookup_drafts: what
 followed the earlier occurrences of its last few tokens).  The step runs all nodes at once; ops.verify_drafts walks down the guesses that the model's
 probabilities accept and draws the token behind them, and the accepted nodes' rows of the cache move to where their positions are.  The tokens
-that come out are distributed as those of plain decoding.
+that come out are distributed as those of plain decoding.  Which ones they are is, unlike there, no function of (seed, stream, position) alone: the numbers that decide
+belong to the position where a step's tree begins, the token behind a prompt is drawn by the sampler, and where a tree begins and what it holds depends on portions, on
+the budget and pages that drafts find, and on preemption.  With room for all of them, the batch does not matter.
 """
 
 from __future__ import annotations

@@ -5,7 +5,7 @@ sampler.py:11-16) from torch's global random stream; greedy is refused there
 (engine/generation/config.py:13-15).  Here temperature 0 is greedy, and the race's noise
 is a pure function of (seed, request's stream, position of the new token, vocabulary
 index), so a request draws the same tokens whatever it is batched with and however often
-it is preempted and recomputed.
+it is preempted and recomputed (with drafted tokens, engine/speculation.py, only their distribution is the same).
 """
 
 from __future__ import annotations
